@@ -249,6 +249,74 @@ int oz_cross_gemm_arrivals(const void *a_slices, const void *b_slices, const flo
                            uint32_t flags, void *stream);
 
 /*
+ * Ragged products of an expert layer (no counterpart in the reference):
+ *   y[r] = x[r] @ w[e]  for offsets[e] <= r < offsets[e + 1]; other rows are 0.
+ *
+ *   x         : (rows, k) fp16 or bf16, element (r, i) at r*x_sr + i*x_sk
+ *   w         : (groups, k, n) of x's type, element (e, i, j) at
+ *               e*w_se + i*w_sk + j*w_sn (element strides; with k and n swapped
+ *               it is the gradient dx = dy @ w^T)
+ *   offsets   : device int32 (or int64, offsets_64 != 0) [groups + 1], read on
+ *               the device only and clamped to [0, rows]
+ *   y         : (rows, n), row pitch ldy, of x's type or fp32 (out_dtype)
+ * Sums are held in fp32 and rounded once.
+ */
+int oz_grouped_matmul(const void *x, const void *w, const void *offsets, int offsets_64, int dtype,
+                      int out_dtype, int32_t groups, int64_t rows, int64_t k, int64_t n,
+                      int64_t x_sr, int64_t x_sk, int64_t w_se, int64_t w_sk, int64_t w_sn,
+                      void *y, int64_t ldy, void *stream);
+
+/*
+ * Weight gradient of oz_grouped_matmul:
+ *   dw[e] = sum over the rows r of group e of x[r]^T dy[r]   (0 for an empty group)
+ * dw: contiguous (groups, k, n) of the operands' type or fp32 (out_dtype).
+ */
+int oz_grouped_wgrad(const void *x, const void *dy, const void *offsets, int offsets_64, int dtype,
+                     int out_dtype, int32_t groups, int64_t rows, int64_t k, int64_t n,
+                     int64_t x_sr, int64_t x_sk, int64_t dy_sr, int64_t dy_sn, void *dw,
+                     void *stream);
+
+/*
+ * Product of a few rows with 4-bit weights (no counterpart in the reference):
+ *   y[r, j] = sum_i x[r, i] (q[j, i] - z[j, i / group]) s[j, i / group]
+ *
+ *   x         : (rows, k) fp16 or bf16, unit stride along k, row pitch x_sr
+ *   packed    : (experts, n, k / 2) bytes, two q a byte (even i in the low
+ *               half); byte strides p_se, p_sn, unit stride along k
+ *   scales    : (experts, n, k / group) fp16, bf16 or fp32 (scale_dtype);
+ *               element strides s_se, s_sn
+ *   zeros     : uint8 with the scales' strides, or NULL: z = 8
+ *   offsets   : row groups of the experts as in oz_grouped_matmul, or NULL
+ *               for one expert with every row
+ * group is a multiple of 32 that divides k.  y: (rows, n), row pitch ldy, of
+ * x's type or fp32.
+ */
+int oz_matmul_w4(const void *x, const void *packed, const void *scales, const void *zeros,
+                 const void *offsets, int offsets_64, int dtype, int scale_dtype, int out_dtype,
+                 int32_t experts, int64_t rows, int64_t k, int64_t n, int32_t group, int64_t x_sr,
+                 int64_t p_se, int64_t p_sn, int64_t s_se, int64_t s_sn, void *y, int64_t ldy,
+                 void *stream);
+
+/*
+ * Newton-Schulz orthogonalisation (no counterpart in the reference) of a
+ * batch of m x n matrices:
+ *   X = g / (|g|_F + eps);  `steps` times with A = X X^T:
+ *   X <- a X + (b A + c A^2) X
+ *
+ *   g            : fp32, fp16 or bf16, element (z, i, j) at z*g_sb + i*g_sr + j*g_sc
+ *   coefficients : host array of `steps` triples (a, b, c)
+ *   num_splits   : fp16 slices of a matrix in the products, 1 or 2
+ *   out          : contiguous (batch, m, n) of g's type
+ *   workspace    : oz_orthogonalize_workspace_bytes() bytes, 256-byte aligned
+ */
+int64_t oz_orthogonalize_workspace_bytes(int dtype, int64_t batch, int64_t m, int64_t n,
+                                         int32_t num_splits);
+int oz_orthogonalize(const void *g, int dtype, int64_t batch, int64_t m, int64_t n, int64_t g_sb,
+                     int64_t g_sr, int64_t g_sc, int32_t steps, const double *coefficients,
+                     double eps, int32_t num_splits, void *out, void *workspace,
+                     int64_t workspace_bytes, void *stream);
+
+/*
  * Peer mappings for the multi-GPU gather (no counterpart in the reference,
  * which has no multi-GPU path).  One process per GPU: a rank exports the
  * allocation holding its slice buffer, each peer imports it once and pulls
