@@ -252,29 +252,30 @@ int oz_cross_gemm_arrivals(const void *a_slices, const void *b_slices, const flo
  * Ragged products of an expert layer (no counterpart in the reference):
  *   y[r] = x[r] @ w[e]  for offsets[e] <= r < offsets[e + 1]; other rows are 0.
  *
- *   x         : (rows, k) fp16 or bf16, element (r, i) at r*x_sr + i*x_sk
+ *   x         : (rows, k) fp16 or bf16, unit stride along k, row pitch x_sr
  *   w         : (groups, k, n) of x's type, element (e, i, j) at
- *               e*w_se + i*w_sk + j*w_sn (element strides; with k and n swapped
- *               it is the gradient dx = dy @ w^T)
+ *               e*w_se + i*w_sk + j*w_sn with a unit stride along k or n (with k
+ *               and n swapped it is the gradient dx = dy @ w^T)
  *   offsets   : device int32 (or int64, offsets_64 != 0) [groups + 1], read on
  *               the device only and clamped to [0, rows]
  *   y         : (rows, n), row pitch ldy, of x's type or fp32 (out_dtype)
- * Sums are held in fp32 and rounded once.
+ * Operands start on 16-byte boundaries and their other strides are multiples
+ * of 8 elements.  Sums are held in fp32 and rounded once.
  */
 int oz_grouped_matmul(const void *x, const void *w, const void *offsets, int offsets_64, int dtype,
                       int out_dtype, int32_t groups, int64_t rows, int64_t k, int64_t n,
-                      int64_t x_sr, int64_t x_sk, int64_t w_se, int64_t w_sk, int64_t w_sn,
-                      void *y, int64_t ldy, void *stream);
+                      int64_t x_sr, int64_t w_se, int64_t w_sk, int64_t w_sn, void *y, int64_t ldy,
+                      void *stream);
 
 /*
  * Weight gradient of oz_grouped_matmul:
  *   dw[e] = sum over the rows r of group e of x[r]^T dy[r]   (0 for an empty group)
- * dw: contiguous (groups, k, n) of the operands' type or fp32 (out_dtype).
+ * x (rows, k) and dy (rows, n) as x there, row pitches x_sr and dy_sr; dw:
+ * contiguous (groups, k, n) of the operands' type or fp32 (out_dtype).
  */
 int oz_grouped_wgrad(const void *x, const void *dy, const void *offsets, int offsets_64, int dtype,
                      int out_dtype, int32_t groups, int64_t rows, int64_t k, int64_t n,
-                     int64_t x_sr, int64_t x_sk, int64_t dy_sr, int64_t dy_sn, void *dw,
-                     void *stream);
+                     int64_t x_sr, int64_t dy_sr, void *dw, void *stream);
 
 /*
  * Product of a few rows with 4-bit weights (no counterpart in the reference):

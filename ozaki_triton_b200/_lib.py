@@ -49,9 +49,9 @@ SIGNATURES = {
                          _i64, _i64, _i64, _i64, _i64, _i32, _int, _int, _vp, _i64, _u32, _vp,
                          _i64, _vp]),
     "oz_grouped_matmul": (_int, [_vp, _vp, _vp, _int, _int, _int, _i32, _i64, _i64, _i64, _i64,
-                                 _i64, _i64, _i64, _i64, _vp, _i64, _vp]),
+                                 _i64, _i64, _i64, _vp, _i64, _vp]),
     "oz_grouped_wgrad": (_int, [_vp, _vp, _vp, _int, _int, _int, _i32, _i64, _i64, _i64, _i64,
-                                _i64, _i64, _i64, _vp, _vp]),
+                                _i64, _vp, _vp]),
     "oz_matmul_w4": (_int, [_vp, _vp, _vp, _vp, _vp, _int, _int, _int, _int, _i32, _i64, _i64,
                             _i64, _i32, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _vp]),
     "oz_orthogonalize_workspace_bytes": (_i64, [_int, _i64, _i64, _i64, _i32]),

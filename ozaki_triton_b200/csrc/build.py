@@ -20,7 +20,7 @@ ROOT = os.path.dirname(PKG)
 LIB = os.path.join(PKG, "liboz_b200.so")
 UNITS = ["oz_api.cu", "oz_split.cu", "oz_gemm.cu", "oz_peer.cu",
          "oz_experts.cu", "oz_w4.cu", "oz_newton.cu"]
-SOURCES = UNITS + ["oz_common.cuh", "oz_log2_table.h", "oz_tile_table.h"]
+SOURCES = UNITS + ["oz_common.cuh", "oz_tile.cuh", "oz_log2_table.h", "oz_tile_table.h"]
 BUILD_DIR = os.path.join(PKG, "_build")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 

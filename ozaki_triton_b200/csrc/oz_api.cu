@@ -63,10 +63,12 @@ extern "C" int oz_device_status(void *stream, int32_t *code) {
   using namespace oz;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (int rc = check_cuda(cudaStreamSynchronize(st), "cudaStreamSynchronize")) return rc;
-  int v1 = 0, v2 = 0;
-  if (int rc = status_split(&v1, true)) return rc;
-  if (int rc = status_gemm(&v2, true)) return rc;
-  const int v = v1 ? v1 : v2;
+  int v = 0;
+  for (auto unit : {status_split, status_gemm, status_experts}) {
+    int u = 0;
+    if (int rc = unit(&u, true)) return rc;
+    if (!v) v = u;
+  }
   if (code) *code = v;
   if (v != 0) return set_error(OZ_ERR_TIMEOUT, "device-side wait timed out (code %d)", v);
   return OZ_OK;

@@ -1,21 +1,23 @@
-// oz_experts.cu -- ragged products of an expert layer and their gradients.
+// oz_experts.cu -- ragged products of an expert layer and their gradients on
+// the tile engine (oz_tile.cuh).
 //
 //   y[r]  = x[r] @ w[e]                     offsets[e] <= r < offsets[e + 1]
 //   dx[r] = dy[r] @ w[e]^T                  (the same product with w transposed)
 //   dw[e] = sum_r x[r]^T dy[r]              r over the group's rows
 //
-// The groups are runs of rows given by device offsets, so no size of a group
-// is known on the host: every block finds its group itself.  Offsets are
-// clamped to [0, rows] before they are used as row numbers.  Products of
-// fp16 / bf16 values are exact in fp32; sums are held in fp32 and rounded once.
+// The groups are runs of rows given by device offsets, so the number of tiles
+// is not known on the host: the grid is sized for the most there can be and
+// every role of every CTA walks the groups itself.  Offsets are clamped to
+// [0, rows] before they are used as row numbers.  Products of fp16 / bf16
+// values are exact in fp32; sums are held in fp32 and rounded once.
 
-#include "oz_common.cuh"
+#include "oz_tile.cuh"
 
 namespace oz {
-namespace {
+int status_experts(int *value, bool clear) { return read_status_word(value, clear); }
 
-constexpr int kTile = 64;       // rows and columns of a block's tile
-constexpr int kStep = 16;       // contraction steps staged at a time
+namespace {
+using namespace tile;
 
 __device__ __forceinline__ int64_t load_offset(const void *offsets, int wide, int64_t i) {
   return wide ? __ldg(static_cast<const long long *>(offsets) + i)
@@ -23,113 +25,191 @@ __device__ __forceinline__ int64_t load_offset(const void *offsets, int wide, in
 }
 
 // Row range of group e, clamped so that a bad offset never leaves the tensor.
-__device__ __forceinline__ void group_rows(const void *offsets, int wide, int e, int64_t rows,
-                                           int64_t &begin, int64_t &end) {
-  begin = min(max(load_offset(offsets, wide, e), (int64_t)0), rows);
-  end = min(max(load_offset(offsets, wide, e + 1), begin), rows);
-}
-
-template <typename T> __device__ __forceinline__ void store_out(void *p, int64_t i, float v);
-template <> __device__ __forceinline__ void store_out<float>(void *p, int64_t i, float v) {
-  static_cast<float *>(p)[i] = v;
-}
-template <> __device__ __forceinline__ void store_out<__half>(void *p, int64_t i, float v) {
-  static_cast<__half *>(p)[i] = __float2half_rn(v);
-}
-template <> __device__ __forceinline__ void store_out<__nv_bfloat16>(void *p, int64_t i, float v) {
-  static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(v);
-}
-
-// One 64 x 64 tile of sum_q a(i, q) b(q, j): 256 threads, 4 x 4 values each.
-template <typename T>
-__device__ __forceinline__ void tile_product(const T *a, int64_t a_i, int64_t a_q, int64_t ni,
-                                             const T *b, int64_t b_q, int64_t b_j, int64_t nj,
-                                             int64_t nq, float (&acc)[4][4]) {
-  __shared__ float sa[kStep][kTile + 1], sb[kStep][kTile + 1];
-  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  for (int64_t q0 = 0; q0 < nq; q0 += kStep) {
-    for (int v = threadIdx.x; v < kStep * kTile; v += 256) {
-      const int q = v / kTile, i = v % kTile;
-      const bool in_q = q0 + q < nq;
-      sa[q][i] = in_q && i < ni ? InTraits<T>::to_float(a[i * a_i + (q0 + q) * a_q]) : 0.f;
-      sb[q][i] = in_q && i < nj ? InTraits<T>::to_float(b[(q0 + q) * b_q + i * b_j]) : 0.f;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int q = 0; q < kStep; ++q)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] += sa[q][ty * 4 + i] * sb[q][tx * 4 + j];
-    __syncthreads();
-  }
+__device__ __forceinline__ void group_rows(const void *offsets, int wide, int e, int rows,
+                                           int &begin, int &end) {
+  begin = (int)min(max(load_offset(offsets, wide, e), (int64_t)0), (int64_t)rows);
+  end = (int)min(max(load_offset(offsets, wide, e + 1), (int64_t)begin), (int64_t)rows);
 }
 
 struct GroupedParams {
-  const void *a, *b, *offsets;
-  void *c;
-  int wide, groups;
-  int64_t rows, k, n;
-  int64_t a_sr, a_sk;          // x: row and inner strides
-  int64_t b_se, b_sk, b_sn;    // w: expert, k and n strides (wgrad: dy's row and column ones)
-  int64_t ldc;
+  const void *offsets;
+  void *out;
+  int64_t ld;                  // output row pitch
+  int wide, groups, rows, k, n;
+  int column_tiles;
+  int vectors;                 // output rows may be written 16 bytes at a time
+  uint32_t idesc;
 };
 
-// Block (row block, column tile): row blocks count the groups' 64-row tiles in
-// order; the blocks after the last one zero the rows that no group holds.
-template <typename T, typename O>
-__global__ void __launch_bounds__(256) grouped_kernel(const GroupedParams p) {
-  int64_t block = blockIdx.x, begin = 0, end = 0;
-  int e = 0;
-  for (; e < p.groups; ++e) {
-    group_rows(p.offsets, p.wide, e, p.rows, begin, end);
-    const int64_t tiles = (end - begin + kTile - 1) / kTile;
-    if (block < tiles) break;
-    block -= tiles;
-  }
-  const int64_t n0 = (int64_t)blockIdx.y * kTile, nj = min((int64_t)kTile, p.n - n0);
-  if (e == p.groups) {
-    int64_t first, last;
-    group_rows(p.offsets, p.wide, 0, p.rows, first, last);
-    group_rows(p.offsets, p.wide, p.groups - 1, p.rows, begin, last);
-    const int64_t outside = first + p.rows - last;
-    for (int64_t v = block * kTile * nj + threadIdx.x; v < min((block + 1) * kTile, outside) * nj;
-         v += 256) {
-      const int64_t r = v / nj, row = r < first ? r : last + r - first;
-      store_out<O>(p.c, row * p.ldc + n0 + v % nj, 0.f);
+// Tiles of row blocks: group by group, `per_rows` rows a block, every column
+// tile of a block.  A warp holds the ranges of 32 groups, one a lane.
+struct GroupWalk {
+  int first, before, begin, end, tiles, upto;   // first group of the 32; tiles before it
+  __device__ GroupWalk(const GroupedParams &) : first(-32), before(0), tiles(0), upto(0) {}
+
+  // The group, block and column tile of tile i; false past the last one.  Calls
+  // have increasing i.  Blocks of `span` consecutive rows of tiles sweep all columns
+  // together (their operands stay in L2).
+  __device__ bool find(const GroupedParams &p, int per_rows, int span, int i, int &e, int &lo, int &hi,
+                       int &block, int &column) {
+    const int lane = threadIdx.x % 32;
+    int total = __shfl_sync(0xffffffffu, upto, 31);
+    while (first < 0 || i >= before + total) {
+      before += total;
+      first += 32;
+      if (first >= p.groups) return false;
+      begin = end = 0;
+      if (first + lane < p.groups) group_rows(p.offsets, p.wide, first + lane, p.rows, begin, end);
+      tiles = (end - begin + per_rows - 1) / per_rows * p.column_tiles;
+      upto = tiles;
+#pragma unroll
+      for (int o = 1; o < 32; o *= 2) {
+        const int v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+      }
+      total = __shfl_sync(0xffffffffu, upto, 31);
     }
-    return;
+    const int src = __ffs(__ballot_sync(0xffffffffu, i < before + upto)) - 1;
+    e = first + src;
+    lo = __shfl_sync(0xffffffffu, begin, src);
+    hi = __shfl_sync(0xffffffffu, end, src);
+    const int local = i - before - __shfl_sync(0xffffffffu, upto - tiles, src);
+    const int blocks = (hi - lo + per_rows - 1) / per_rows;
+    const int sweep = local / (span * p.column_tiles);
+    const int in = local - sweep * span * p.column_tiles;
+    const int size = min(blocks - sweep * span, span);
+    block = sweep * span + in % size;
+    column = in / size;
+    return true;
   }
-  const int64_t row = begin + block * kTile, ni = min((int64_t)kTile, end - row);
-  float acc[4][4] = {};
-  tile_product<T>(static_cast<const T *>(p.a) + row * p.a_sr, p.a_sr, p.a_sk, ni,
-                  static_cast<const T *>(p.b) + e * p.b_se + n0 * p.b_sn, p.b_sk, p.b_sn, nj, p.k,
-                  acc);
-  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j)
-      if (ty * 4 + i < ni && tx * 4 + j < nj)
-        store_out<O>(p.c, (row + ty * 4 + i) * p.ldc + n0 + tx * 4 + j, acc[i][j]);
+};
+
+// Zeros in the rows that no group holds, warp `me` of `warps`.
+template <typename O>
+__device__ __forceinline__ void clear_outside(const GroupedParams &p, int me, int warps) {
+  int first, last, a, b;
+  group_rows(p.offsets, p.wide, 0, p.rows, first, a);
+  group_rows(p.offsets, p.wide, p.groups - 1, p.rows, b, last);
+  for (int v = me; v < first + p.rows - last; v += warps) {
+    O *row = static_cast<O *>(p.out) + (int64_t)(v < first ? v : last + v - first) * p.ld;
+    for (int c = threadIdx.x % 32; c < p.n; c += 32) row[c] = O(0.f);
+  }
 }
 
-// Block (n tile, k tile, group): dw[e] tile over the rows of the group.
-template <typename T, typename O>
-__global__ void __launch_bounds__(256) grouped_wgrad_kernel(const GroupedParams p) {
-  int64_t begin, end;
-  const int e = blockIdx.z;
-  group_rows(p.offsets, p.wide, e, p.rows, begin, end);
-  const int64_t n0 = (int64_t)blockIdx.x * kTile, nj = min((int64_t)kTile, p.n - n0);
-  const int64_t k0 = (int64_t)blockIdx.y * kTile, ni = min((int64_t)kTile, p.k - k0);
-  float acc[4][4] = {};
-  tile_product<T>(static_cast<const T *>(p.a) + begin * p.a_sr + k0 * p.a_sk, p.a_sk, p.a_sr, ni,
-                  static_cast<const T *>(p.b) + begin * p.b_sk + n0 * p.b_sn, p.b_sk, p.b_sn, nj,
-                  end - begin, acc);
-  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j)
-      if (ty * 4 + i < ni && tx * 4 + j < nj)
-        store_out<O>(p.c, ((int64_t)e * p.k + k0 + ty * 4 + i) * p.n + n0 + tx * 4 + j, acc[i][j]);
-}
+struct RowTile { int row, rows, column; };   // first row, rows from there to the group's end
+
+// y = x w: A is the rows of x, B the columns of w[e].
+template <typename O, int PAIR_, int NT_, bool BMN_> struct RowsJob {
+  static constexpr int PAIR = PAIR_, NT = NT_, PLANES = 1;
+  static constexpr bool AMN = false, BMN = BMN_, RAGGED = false;
+  using Params = GroupedParams;
+  using Extra = RowTile;
+  static __device__ int plane_stride(const Params &) { return 0; }
+  struct Walk : GroupWalk {
+    using GroupWalk::GroupWalk;
+    __device__ bool find(const Params &p, int i, TileOf<Extra> &t) {
+      int e, lo, hi, block, column;
+      if (!GroupWalk::find(p, kRows * PAIR, 8, i, e, lo, hi, block, column)) return false;
+      t.a_row = lo + block * kRows * PAIR;
+      t.a_mat = 0;
+      t.b_row = column * NT;
+      t.b_mat = e;
+      t.k_begin = 0;
+      t.k_len = p.k;
+      t.extra = RowTile{t.a_row, hi - t.a_row, t.b_row};
+      return true;
+    }
+  };
+  static __device__ void epilogue(const Params &p, const TileOf<Extra> &t, bool some, uint32_t columns,
+                                  int row, int column, unsigned char *mine) {
+    const int64_t c0 = t.extra.column + column;
+    write_rows<O, NT / 2>(some, columns, mine,
+                          static_cast<O *>(p.out) + (int64_t)(t.extra.row + row) * p.ld + c0, p.ld,
+                          t.extra.rows - row, p.n - c0, p.vectors);
+  }
+  static __device__ void finish(const Params &p, int me, int warps) { clear_outside<O>(p, me, warps); }
+};
+
+// The same product with the roles exchanged, for groups of a few rows: A is
+// 128 columns of w[e], B up to NT rows of x, so a tile's weights are read
+// once and hardly any of the staged bytes belong to rows that are not there.
+template <typename O, int NT_, bool AMN_> struct ColumnsJob {
+  static constexpr int PAIR = 1, NT = NT_, PLANES = 1;
+  static constexpr bool AMN = AMN_, BMN = false, RAGGED = false;
+  using Params = GroupedParams;
+  using Extra = RowTile;
+  static __device__ int plane_stride(const Params &) { return 0; }
+  struct Walk : GroupWalk {
+    using GroupWalk::GroupWalk;
+    __device__ bool find(const Params &p, int i, TileOf<Extra> &t) {
+      int e, lo, hi, block, column;
+      if (!GroupWalk::find(p, NT, 1 << 16, i, e, lo, hi, block, column)) return false;
+      t.a_row = column * kRows;
+      t.a_mat = e;
+      t.b_row = lo + block * NT;
+      t.b_mat = 0;
+      t.k_begin = 0;
+      t.k_len = p.k;
+      t.extra = RowTile{t.b_row, hi - t.b_row, t.a_row};
+      return true;
+    }
+  };
+  static __device__ void epilogue(const Params &p, const TileOf<Extra> &t, bool some, uint32_t columns,
+                                  int row, int column, unsigned char *) {
+    const int64_t c = t.extra.column + row + threadIdx.x % 32;
+    O *out = static_cast<O *>(p.out) + (int64_t)(t.extra.row + column) * p.ld + c;
+    const int rows = t.extra.rows - column;
+#pragma unroll
+    for (int r0 = 0; r0 < NT / 2; r0 += 16) {
+      if (r0 >= rows) break;
+      float v[16];
+      read16(some, columns + (uint32_t)r0, v);
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (r0 + r < rows && c < p.n) out[(r0 + r) * p.ld] = O(v[r]);
+    }
+  }
+  static __device__ void finish(const Params &p, int me, int warps) { clear_outside<O>(p, me, warps); }
+};
+
+struct WeightTile { int row, column, group; };
+
+// dw[e] = x^T dy over the group's rows: both operands are stored across the
+// contraction, whose range is the group.
+template <typename O, int PAIR_, int NT_> struct WeightsJob {
+  static constexpr int PAIR = PAIR_, NT = NT_, PLANES = 1;
+  static constexpr bool AMN = true, BMN = true, RAGGED = true;
+  using Params = GroupedParams;
+  using Extra = WeightTile;
+  static __device__ int plane_stride(const Params &) { return 0; }
+  struct Walk {
+    int group, begin, end;
+    __device__ Walk(const Params &) : group(-1) {}
+    __device__ bool find(const Params &p, int i, TileOf<Extra> &t) {
+      const int row_tiles = (p.k + kRows * PAIR - 1) / (kRows * PAIR);
+      const int per = row_tiles * p.column_tiles;
+      const int e = i / per;
+      if (e >= p.groups) return false;
+      if (e != group) group_rows(p.offsets, p.wide, group = e, p.rows, begin, end);
+      const int local = i - e * per;
+      t.a_row = local % row_tiles * kRows * PAIR;
+      t.b_row = local / row_tiles * NT;
+      t.a_mat = t.b_mat = 0;
+      t.k_begin = begin;
+      t.k_len = end - begin;
+      t.extra = WeightTile{t.a_row, t.b_row, e};
+      return true;
+    }
+  };
+  static __device__ void epilogue(const Params &p, const TileOf<Extra> &t, bool some, uint32_t columns,
+                                  int row, int column, unsigned char *mine) {
+    const int64_t r0 = t.extra.row + row, c0 = t.extra.column + column;
+    write_rows<O, NT / 2>(some, columns, mine,
+                          static_cast<O *>(p.out) + ((int64_t)t.extra.group * p.k + r0) * p.ld + c0,
+                          p.ld, (int)(p.k - r0), p.n - c0, p.vectors);
+  }
+  static __device__ void finish(const Params &, int, int) {}
+};
 
 int check_grouped(int dtype, int out_dtype, int32_t groups, int64_t rows, int64_t k, int64_t n) {
   if (dtype != OZ_F16 && dtype != OZ_BF16)
@@ -138,9 +218,78 @@ int check_grouped(int dtype, int out_dtype, int32_t groups, int64_t rows, int64_
     return set_error(OZ_ERR_UNSUPPORTED, "unsupported output dtype %d", out_dtype);
   if (groups < 1) return set_error(OZ_ERR_INVALID, "at least one group is needed, got %d", groups);
   if (rows < 0 || k < 0 || n < 0) return set_error(OZ_ERR_INVALID, "negative size");
-  if (rows > (1 << 30) || k > (1 << 30) || n > (1 << 30))
+  if (rows > (1 << 30) || k > (1 << 30) || n > (1 << 30) || groups > (1 << 24))
     return set_error(OZ_ERR_INVALID, "size out of range");
   return OZ_OK;
+}
+
+// Whether the copy unit can read rows (and matrices) that far apart.
+bool pitch_ok(int64_t stride, int64_t count) {
+  return count <= 1 || (stride > 0 && stride % 8 == 0 && stride < ((int64_t)1 << 38));
+}
+int64_t pitch_bytes(int64_t stride, int64_t count, int64_t inner) {
+  return 2 * (count <= 1 ? (inner + 7) / 8 * 8 : stride);
+}
+
+int check_operand(const char *name, const void *p, int64_t rows, int64_t row_stride, int64_t mats,
+                  int64_t mat_stride) {
+  if ((uintptr_t)p % 16 != 0 || !pitch_ok(row_stride, rows) || !pitch_ok(mat_stride, mats))
+    return set_error(OZ_ERR_INVALID,
+                     "%s must start on a 16-byte boundary, its strides must be multiples of 16 bytes "
+                     "(row %lld, matrix %lld elements)",
+                     name, (long long)row_stride, (long long)mat_stride);
+  return OZ_OK;
+}
+
+template <class J>
+int run(const CUtensorMap &a, const CUtensorMap &b, GroupedParams p, int64_t row_tiles, int64_t n_side,
+        int n_per_tile, cudaStream_t st, const char *what) {
+  const int64_t columns = (n_side + n_per_tile - 1) / n_per_tile;
+  if (row_tiles * columns > INT32_MAX / 2) return set_error(OZ_ERR_INVALID, "too many tiles");
+  p.column_tiles = (int)columns;
+  return launch<J>(a, b, p, row_tiles * columns, st, what);
+}
+
+template <typename O>
+int grouped(const void *x, const void *w, int64_t x_sr, int64_t w_se, bool across, int64_t w_row,
+            const GroupedParams &p, cudaStream_t st) {
+  // Columns as A (at most 32 rows of a group a tile) while the mean group has no
+  // more than 32 rows; pairs of CTAs (256-row tiles) from 192 rows on.
+  const int64_t mean = p.rows / p.groups;
+  const int pair = mean >= 192 ? 2 : 1;
+  const bool few = mean <= 32;
+  CUtensorMap tx, tw;
+  const int64_t wr = across ? p.k : p.n, wi = across ? p.n : p.k;
+  const int nt = pair == 2 ? 256 : 128;
+  const int64_t xb = pitch_bytes(x_sr, p.rows, p.k), wb = pitch_bytes(w_row, wr, wi);
+  if (int rc = make_map(&tx, x, p.k, p.rows, 1, xb, xb, few ? 32 : kRows))
+    return rc;
+  if (int rc = make_map(&tw, w, wi, wr, p.groups, wb, p.groups > 1 ? 2 * w_se : wb, across ? kBlock : few ? kRows : nt / pair))
+    return rc;
+  const char *what = "grouped product launch";
+  const int64_t per = few ? 32 : kRows * pair;
+  const int64_t blocks = p.rows / per + min((int64_t)p.groups, (int64_t)p.rows);
+  if (few)
+    return across ? run<ColumnsJob<O, 32, true>>(tw, tx, p, blocks, p.n, kRows, st, what)
+                  : run<ColumnsJob<O, 32, false>>(tw, tx, p, blocks, p.n, kRows, st, what);
+  if (pair == 1)
+    return across ? run<RowsJob<O, 1, 128, true>>(tx, tw, p, blocks, p.n, 128, st, what)
+                  : run<RowsJob<O, 1, 128, false>>(tx, tw, p, blocks, p.n, 128, st, what);
+  return across ? run<RowsJob<O, 2, 256, true>>(tx, tw, p, blocks, p.n, 256, st, what)
+                : run<RowsJob<O, 2, 256, false>>(tx, tw, p, blocks, p.n, 256, st, what);
+}
+
+template <typename O>
+int wgrad(const void *x, const void *dy, int64_t x_sr, int64_t dy_sr, const GroupedParams &p,
+          cudaStream_t st) {
+  CUtensorMap tx, ty;
+  const int64_t xb = pitch_bytes(x_sr, p.rows, p.k), yb = pitch_bytes(dy_sr, p.rows, p.n);
+  if (int rc = make_map(&tx, x, p.k, p.rows, 1, xb, xb, kBlock)) return rc;
+  if (int rc = make_map(&ty, dy, p.n, p.rows, 1, yb, yb, kBlock)) return rc;
+  const char *what = "grouped weight gradient launch";
+  if (p.k > kRows && p.n > 128)
+    return run<WeightsJob<O, 2, 256>>(tx, ty, p, (int64_t)p.groups * ((p.k + 255) / 256), p.n, 256, st, what);
+  return run<WeightsJob<O, 1, 128>>(tx, ty, p, (int64_t)p.groups * ((p.k + 127) / 128), p.n, 128, st, what);
 }
 
 }  // namespace
@@ -148,51 +297,51 @@ int check_grouped(int dtype, int out_dtype, int32_t groups, int64_t rows, int64_
 
 extern "C" int oz_grouped_matmul(const void *x, const void *w, const void *offsets,
                                  int offsets_64, int dtype, int out_dtype, int32_t groups,
-                                 int64_t rows, int64_t k, int64_t n, int64_t x_sr, int64_t x_sk,
-                                 int64_t w_se, int64_t w_sk, int64_t w_sn, void *y, int64_t ldy,
-                                 void *stream) {
+                                 int64_t rows, int64_t k, int64_t n, int64_t x_sr, int64_t w_se,
+                                 int64_t w_sk, int64_t w_sn, void *y, int64_t ldy, void *stream) {
   using namespace oz;
   if (int rc = check_grouped(dtype, out_dtype, groups, rows, k, n)) return rc;
   if (rows == 0 || n == 0) return OZ_OK;
   if (!y || ldy < n) return set_error(OZ_ERR_INVALID, "bad output (ldy=%lld n=%lld)",
                                       (long long)ldy, (long long)n);
-  if (!offsets || (k > 0 && (!x || !w))) return set_error(OZ_ERR_INVALID, "null pointer");
-  GroupedParams p{x, w, offsets, y, offsets_64, groups, rows, k, n, x_sr, x_sk, w_se, w_sk, w_sn,
-                  ldy};
-  const int64_t blocks = (rows + kTile - 1) / kTile + groups + 1;
-  const dim3 grid((unsigned)blocks, (unsigned)((n + kTile - 1) / kTile));
-  if (grid.y > 65535) return set_error(OZ_ERR_INVALID, "size out of range");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  count_launch();
-  if (dtype == OZ_F16 && out_dtype == OZ_F32) grouped_kernel<__half, float><<<grid, 256, 0, st>>>(p);
-  else if (dtype == OZ_F16) grouped_kernel<__half, __half><<<grid, 256, 0, st>>>(p);
-  else if (out_dtype == OZ_F32) grouped_kernel<__nv_bfloat16, float><<<grid, 256, 0, st>>>(p);
-  else grouped_kernel<__nv_bfloat16, __nv_bfloat16><<<grid, 256, 0, st>>>(p);
-  return check_cuda(cudaGetLastError(), "grouped_kernel launch");
+  const int es = dtype_size(out_dtype);
+  if (k == 0)
+    return check_cuda(cudaMemset2DAsync(y, (size_t)(ldy * es), 0, (size_t)(n * es), (size_t)rows, st),
+                      "cudaMemset2DAsync");
+  if (!offsets || !x || !w) return set_error(OZ_ERR_INVALID, "null pointer");
+  // stored across the contraction (unit stride along n) or along it
+  const bool across = w_sn == 1 || (n == 1 && w_sk != 1);
+  if (!across && w_sk != 1 && k != 1)
+    return set_error(OZ_ERR_INVALID, "w must have a unit stride along k or n");
+  const int64_t w_row = across ? w_sk : w_sn;
+  if (int rc = check_operand("x", x, rows, x_sr, 1, 0)) return rc;
+  if (int rc = check_operand("w", w, across ? k : n, w_row, groups, w_se)) return rc;
+  GroupedParams p{offsets, y, ldy, offsets_64, groups, (int)rows, (int)k, (int)n, 0,
+                  (uintptr_t)y % 16 == 0 && ldy * es % 16 == 0, tile::instruction(dtype)};
+  if (out_dtype == OZ_F32) return grouped<float>(x, w, x_sr, w_se, across, w_row, p, st);
+  if (dtype == OZ_F16) return grouped<__half>(x, w, x_sr, w_se, across, w_row, p, st);
+  return grouped<__nv_bfloat16>(x, w, x_sr, w_se, across, w_row, p, st);
 }
 
 extern "C" int oz_grouped_wgrad(const void *x, const void *dy, const void *offsets,
                                 int offsets_64, int dtype, int out_dtype, int32_t groups,
-                                int64_t rows, int64_t k, int64_t n, int64_t x_sr, int64_t x_sk,
-                                int64_t dy_sr, int64_t dy_sn, void *dw, void *stream) {
+                                int64_t rows, int64_t k, int64_t n, int64_t x_sr, int64_t dy_sr,
+                                void *dw, void *stream) {
   using namespace oz;
   if (int rc = check_grouped(dtype, out_dtype, groups, rows, k, n)) return rc;
   if (k == 0 || n == 0) return OZ_OK;
-  if (!dw || !offsets || (rows > 0 && (!x || !dy)))
-    return set_error(OZ_ERR_INVALID, "null pointer");
-  if (groups > 65535) return set_error(OZ_ERR_INVALID, "too many groups");
-  GroupedParams p{x, dy, offsets, dw, offsets_64, groups, rows, k, n, x_sr, x_sk, 0, dy_sr, dy_sn,
-                  n};
-  const dim3 grid((unsigned)((n + kTile - 1) / kTile), (unsigned)((k + kTile - 1) / kTile),
-                  (unsigned)groups);
-  if (grid.y > 65535) return set_error(OZ_ERR_INVALID, "size out of range");
+  if (!dw) return set_error(OZ_ERR_INVALID, "null pointer");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  count_launch();
-  if (dtype == OZ_F16 && out_dtype == OZ_F32)
-    grouped_wgrad_kernel<__half, float><<<grid, 256, 0, st>>>(p);
-  else if (dtype == OZ_F16) grouped_wgrad_kernel<__half, __half><<<grid, 256, 0, st>>>(p);
-  else if (out_dtype == OZ_F32)
-    grouped_wgrad_kernel<__nv_bfloat16, float><<<grid, 256, 0, st>>>(p);
-  else grouped_wgrad_kernel<__nv_bfloat16, __nv_bfloat16><<<grid, 256, 0, st>>>(p);
-  return check_cuda(cudaGetLastError(), "grouped_wgrad_kernel launch");
+  const int es = dtype_size(out_dtype);
+  if (rows == 0)
+    return check_cuda(cudaMemsetAsync(dw, 0, (size_t)(groups * k * n * es), st), "cudaMemsetAsync");
+  if (!offsets || !x || !dy) return set_error(OZ_ERR_INVALID, "null pointer");
+  if (int rc = check_operand("x", x, rows, x_sr, 1, 0)) return rc;
+  if (int rc = check_operand("dy", dy, rows, dy_sr, 1, 0)) return rc;
+  GroupedParams p{offsets, dw, n, offsets_64, groups, (int)rows, (int)k, (int)n, 0,
+                  (uintptr_t)dw % 16 == 0 && n * es % 16 == 0, tile::instruction(dtype)};
+  if (out_dtype == OZ_F32) return wgrad<float>(x, dy, x_sr, dy_sr, p, st);
+  if (dtype == OZ_F16) return wgrad<__half>(x, dy, x_sr, dy_sr, p, st);
+  return wgrad<__nv_bfloat16>(x, dy, x_sr, dy_sr, p, st);
 }

@@ -1,0 +1,504 @@
+// oz_tile.cuh -- a persistent tcgen05 tile engine for products of fp16 / bf16
+// operands whose tiles, extents and epilogues differ from job to job.
+//
+// A job (a class with the members used below) says which tiles there are,
+// where their operands lie and what becomes of an accumulator; the engine
+// moves the data and issues the matrix instructions:
+//   warp 0     TMA producer: 64-deep blocks of A and B into a ring of stages;
+//   warp 1     TMEM allocator and the one thread that issues tcgen05.mma;
+//   warps 2-9  epilogue: the job's, from TMEM (fp32 accumulators, two buffers,
+//              so the epilogue of one tile runs under the products of the next).
+// A tile is 128 * PAIR rows by NT columns; with PAIR = 2 two CTAs of a
+// cluster hold half of A's rows and half of B's columns each and one
+// cta_group::2 instruction multiplies both halves: each CTA then feeds 256
+// rows or columns of products with 128 of its own loads.
+//
+// An operand is stored either along the contraction ("K-major") or across it
+// ("MN-major": AMN / BMN).  Both are staged with the 128-byte swizzle; an
+// MN-major tile is a row of chunks of 64 elements, each chunk 64 contraction
+// rows of 128 bytes.  Elements outside a tensor's extents arrive as zeros.
+// With RAGGED the contraction runs over a tile's own range of rows
+// [k_begin, k_begin + k_len) of longer operands: the rows of the last block
+// past the range are overwritten with zeros in shared memory before they are
+// multiplied (in both operands: a zero times a stray NaN is a NaN).
+//
+// With PLANES = 2 each operand is a sum of two fp16 slices and a block adds
+// high*high, high*low and low*high to the accumulator (low*low is below the
+// last bit of the others).
+//
+// Every wait is bounded (oz_common.cuh).
+#pragma once
+
+#include <cudaTypedefs.h>
+
+#include "oz_common.cuh"
+
+namespace oz {
+namespace tile {
+
+constexpr int kRows = 128;              // rows of one CTA's part of a tile
+constexpr int kBlock = 64;              // contraction elements of a stage
+constexpr int kLine = 128;              // bytes of a swizzled row
+constexpr int kMaxStages = 10;
+constexpr int kEpilogueWarps = 8;
+constexpr int kThreads = 64 + 32 * kEpilogueWarps;
+constexpr int kStagingBytes = 4096;     // of each epilogue warp: 32 rows of 128 bytes
+constexpr int kBarrierBytes = 512;
+constexpr int kSmemLimit = 227 * 1024;
+
+template <class J> __host__ __device__ constexpr int a_bytes() { return kRows * kLine; }
+template <class J> __host__ __device__ constexpr int b_bytes() { return J::NT / J::PAIR * kLine; }
+template <class J> __host__ __device__ constexpr int stage_bytes() { return J::PLANES * (a_bytes<J>() + b_bytes<J>()); }
+template <class J> __host__ __device__ constexpr int stages() {
+  constexpr int room = kSmemLimit - 1024 - kBarrierBytes - kEpilogueWarps * kStagingBytes;
+  constexpr int n = room / stage_bytes<J>();
+  return n < kMaxStages ? n : kMaxStages;
+}
+template <class J> __host__ __device__ constexpr int smem_bytes() {
+  return 1024 + stages<J>() * stage_bytes<J>() + kEpilogueWarps * kStagingBytes + kBarrierBytes;
+}
+
+// Where a tile's operands lie: first row (or column) and matrix of A and B in
+// their tensor maps, the contraction range, and what the job's epilogue wants.
+template <class Extra> struct TileOf {
+  int a_row, a_mat, b_row, b_mat;
+  int64_t k_begin, k_len;
+  Extra extra;
+};
+
+// 3-D operand map: `inner` contiguous elements, `rows` of them `row_bytes`
+// apart, `mats` of those `mat_bytes` apart; boxes of 64 x box_rows.
+inline int make_map(CUtensorMap *map, const void *base, int64_t inner, int64_t rows, int64_t mats,
+                    int64_t row_bytes, int64_t mat_bytes, int box_rows) {
+  static PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
+  if (!encode) {
+    void *ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &ptr, 12000, cudaEnableDefault,
+                                         &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      return set_error(OZ_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+    encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+  }
+  cuuint64_t dims[3] = {(cuuint64_t)inner, (cuuint64_t)rows, (cuuint64_t)mats};
+  cuuint64_t strides[2] = {(cuuint64_t)row_bytes, (cuuint64_t)mat_bytes};
+  cuuint32_t box[3] = {kBlock, (cuuint32_t)box_rows, 1};
+  cuuint32_t steps[3] = {1, 1, 1};
+  const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void *>(base), dims,
+                            strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(OZ_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return OZ_OK;
+}
+
+inline int sm_count() {
+  static int n = 0;
+  if (!n) {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    if (n <= 0) n = 148;
+  }
+  return n;
+}
+
+// Shared-memory descriptors (128-byte swizzle).  K-major: rows of 128 bytes,
+// 1024 bytes from one group of 8 rows to the next.  MN-major: chunks of 64
+// elements 64 * 128 bytes apart, 1024 bytes from 8 contraction rows to the next.
+template <bool MN> __device__ __forceinline__ uint64_t operand_desc(uint32_t addr) {
+  if constexpr (!MN) return smem_desc_sw128(addr);
+  uint64_t d = (uint64_t)((addr & 0x3FFFF) >> 4);
+  d |= (uint64_t)((kBlock * kLine) >> 4) << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+
+// Wait for arrivals of the other CTA of a pair too (acquire over the cluster).
+__device__ __forceinline__ bool wait_cluster(uint64_t *bar, uint32_t parity, volatile int *abort,
+                                             int code) {
+  const uint32_t a = smem_u32(bar);
+  const long long t0 = clock64();
+  for (uint32_t it = 0;; ++it) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(a), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if ((it & 63u) == 63u) {
+      if (*abort) return false;
+      if (clock64() - t0 > kWaitBoundCycles) {
+        *abort = code;
+        atomicCAS(&g_device_status, 0, code);
+        return false;
+      }
+    }
+  }
+}
+
+template <class J>
+__global__ void __launch_bounds__(kThreads, 1)
+    tile_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
+                const typename J::Params p) {
+  using Tile = TileOf<typename J::Extra>;
+  constexpr int PAIR = J::PAIR, NT = J::NT, S = stages<J>(), SB = stage_bytes<J>();
+  constexpr int BR = NT / PAIR;                       // B rows (columns of the tile) of one CTA
+  constexpr int kTmemColumns = 2 * NT < 32 ? 32 : 2 * NT;
+  static_assert((NT & (NT - 1)) == 0 && NT >= 32 && NT <= 256 && 2 * NT <= 512, "tile columns");
+  static_assert(!J::BMN || BR % 64 == 0, "an MN-major B comes in chunks of 64");
+  static_assert(S >= 3, "too few stages");
+
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  unsigned char *staging = smem + S * SB;
+  uint64_t *full = reinterpret_cast<uint64_t *>(staging + kEpilogueWarps * kStagingBytes);
+  uint64_t *empty = full + kMaxStages;
+  uint64_t *acc_full = empty + kMaxStages;            // [2]
+  uint64_t *acc_empty = acc_full + 2;                 // [2]
+  uint64_t *drain = acc_empty + 2;
+  uint64_t *tail = drain + 1;                         // RAGGED: this CTA's last block has landed
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tail + 1);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const uint32_t rank = PAIR == 2 ? cluster_ctarank() : 0;
+  const bool leader = rank == 0;
+  const int unit = blockIdx.x / PAIR, units = gridDim.x / PAIR;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S; ++i) {
+      mbar_init(&full[i], J::RAGGED ? PAIR : 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], PAIR * kEpilogueWarps);
+    }
+    mbar_init(drain, 1);
+    mbar_init(tail, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    prefetch_tmap(&tm_a);
+    prefetch_tmap(&tm_b);
+  }
+  if (warp == 1) {
+    if constexpr (PAIR == 2) {
+      tmem_alloc_pair(tmem_slot, kTmemColumns);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(tmem_slot, kTmemColumns);
+      tmem_relinquish();
+    }
+  }
+  tc_fence_before();
+  if constexpr (PAIR == 2) cluster_sync();
+  else __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  auto leader_addr = [&](uint64_t *bar) -> uint32_t {
+    if constexpr (PAIR == 2) return map_to_cta(smem_u32(bar), 0);
+    else return smem_u32(bar);
+  };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    typename J::Walk walk(p);
+    Tile t;
+    uint32_t it = 0, tails = 0;
+    bool ok = true;
+    for (int i = unit; ok && walk.find(p, i, t); i += units) {
+      const int blocks = (int)((t.k_len + kBlock - 1) / kBlock);
+      const int rest = J::RAGGED ? (int)(t.k_len % kBlock) : 0;
+      for (int kb = 0; kb < blocks; ++kb, ++it) {
+        const int slot = it % S;
+        unsigned char *st = smem + slot * SB;
+        const bool last = J::RAGGED && rest && kb == blocks - 1;
+        if (lane == 0) {
+          ok = mbar_wait_bounded(&empty[slot], ((it / S) & 1) ^ 1, abort_flag, DEV_TIMEOUT_PRODUCER);
+          if (ok) {
+            // every box lands in this CTA; its bytes count on the leader's
+            // barrier, or on the CTA's own before a ragged end is cleared
+            uint32_t bar;
+            if (last) {
+              mbar_arrive_expect_tx(tail, SB);
+              bar = smem_u32(tail);
+            } else {
+              bar = leader_addr(&full[slot]);
+              if (leader) mbar_arrive_expect_tx(&full[slot], PAIR * SB);
+              else if constexpr (J::RAGGED) mbar_arrive_remote(bar);
+            }
+            auto load = [&](void *dst, const CUtensorMap *map, int c0, int c1, int c2) {
+              if constexpr (PAIR == 2) {
+                if (!last) {
+                  tma_load_3d_pair(dst, map, bar, c0, c1, c2);
+                  return;
+                }
+              }
+              tma_load_3d(dst, map, last ? tail : &full[slot], c0, c1, c2);
+            };
+            const int k = (int)(t.k_begin + (int64_t)kb * kBlock);
+            const int ar = t.a_row + (int)rank * kRows, br = t.b_row + (int)rank * BR;
+#pragma unroll
+            for (int pl = 0; pl < J::PLANES; ++pl) {
+              unsigned char *sa = st + pl * a_bytes<J>();
+              unsigned char *sb = st + J::PLANES * a_bytes<J>() + pl * b_bytes<J>();
+              const int am = t.a_mat + pl * J::plane_stride(p), bm = t.b_mat + pl * J::plane_stride(p);
+              if constexpr (J::AMN)
+                for (int c = 0; c < kRows / 64; ++c)
+                  load(sa + c * kBlock * kLine, &tm_a, ar + c * 64, k, am);
+              else load(sa, &tm_a, k, ar, am);
+              if constexpr (J::BMN)
+                for (int c = 0; c < BR / 64; ++c)
+                  load(sb + c * kBlock * kLine, &tm_b, br + c * 64, k, bm);
+              else load(sb, &tm_b, k, br, bm);
+            }
+            if (last) ok = mbar_wait_bounded(tail, tails & 1, abort_flag, DEV_TIMEOUT_PRODUCER);
+          }
+        }
+        if constexpr (J::RAGGED) {
+          if (last) {
+            ++tails;
+            ok = __shfl_sync(0xffffffffu, (int)ok, 0);
+            if (ok) {
+              // rows [rest, 64) of every chunk: whole 128-byte lines, so the swizzle does not matter
+              constexpr int chunks = SB / (kBlock * kLine);
+              const int lines = (kBlock - rest) * 8;           // 16-byte pieces of a chunk's lines
+              for (int v = lane; v < chunks * lines; v += 32)
+                *reinterpret_cast<uint4 *>(st + v / lines * (kBlock * kLine) + rest * kLine +
+                                           v % lines * 16) = make_uint4(0, 0, 0, 0);
+              fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0) {
+                if (leader) mbar_arrive(&full[slot]);
+                else mbar_arrive_remote(leader_addr(&full[slot]));
+              }
+            }
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, (int)ok, 0);
+        if (!ok) break;
+      }
+    }
+    // every load that counts on the leader's barriers must have landed before
+    // shared memory goes away
+    if (lane == 0 && leader)
+      for (uint32_t k = (it > (uint32_t)S ? it - S : 0); k < it; ++k)
+        mbar_wait_bounded(&full[k % S], (k / S) & 1, abort_flag, DEV_TIMEOUT_PRODUCER);
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    typename J::Walk walk(p);
+    Tile t;
+    uint32_t it = 0, done = 0;
+    bool ok = true;
+    const uint32_t base = smem_u32(smem);
+    const uint32_t idesc = p.idesc | ((uint32_t)(NT >> 3) << 17) |
+                           ((uint32_t)((kRows * PAIR) >> 4) << 24) | (J::AMN ? 1u << 15 : 0u) |
+                           (J::BMN ? 1u << 16 : 0u);
+    constexpr uint64_t a_step = J::AMN ? (16 * kLine) >> 4 : 2, b_step = J::BMN ? (16 * kLine) >> 4 : 2;
+    auto release = [&](uint64_t *bar) {
+      if constexpr (PAIR == 2) {
+        tc_commit_pair(smem_u32(bar));
+        tc_commit_pair(map_to_cta(smem_u32(bar), 1));
+      } else {
+        tc_commit(bar);
+      }
+    };
+    auto wait = [&](uint64_t *bar, uint32_t parity) {
+      if constexpr (PAIR == 2) return wait_cluster(bar, parity, abort_flag, DEV_TIMEOUT_MMA);
+      else return mbar_wait_bounded(bar, parity, abort_flag, DEV_TIMEOUT_MMA);
+    };
+    for (int i = unit; ok && walk.find(p, i, t); i += units) {
+      const int blocks = (int)((t.k_len + kBlock - 1) / kBlock);
+      if (blocks == 0) continue;                      // the epilogue writes zeros by itself
+      if (lane == 0 && leader) {
+        const int buf = done & 1;
+        ok = wait(&acc_empty[buf], ((done >> 1) & 1) ^ 1);
+        tc_fence_after();
+        const uint32_t d = tmem + (uint32_t)(buf * NT);
+        for (int kb = 0; ok && kb < blocks; ++kb, ++it) {
+          const int slot = it % S;
+          if (!(ok = wait(&full[slot], (it / S) & 1))) break;
+          const uint32_t sa = base + slot * SB, sb = sa + J::PLANES * a_bytes<J>();
+#pragma unroll
+          for (int q = 0; q < (J::PLANES == 2 ? 3 : 1); ++q) {
+            const uint64_t ad = operand_desc<J::AMN>(sa + (q == 2 ? a_bytes<J>() : 0));
+            const uint64_t bd = operand_desc<J::BMN>(sb + (q == 1 ? b_bytes<J>() : 0));
+#pragma unroll
+            for (int kk = 0; kk < kBlock / 16; ++kk) {
+              const uint32_t add = (uint32_t)((kb | kk | q) != 0);
+              if constexpr (PAIR == 2) tc_mma_pair<1>(d, ad + kk * a_step, bd + kk * b_step, idesc, add);
+              else tc_mma<1>(d, ad + kk * a_step, bd + kk * b_step, idesc, add);
+            }
+          }
+          release(&empty[slot]);
+        }
+        if (ok) release(&acc_full[buf]);
+      }
+      ++done;
+      ok = __shfl_sync(0xffffffffu, (int)ok, 0);
+    }
+    if (lane == 0 && leader) {
+      if constexpr (PAIR == 2) tc_commit_pair(smem_u32(drain));
+      else tc_commit(drain);
+      mbar_wait_bounded(drain, 0, abort_flag, DEV_TIMEOUT_MMA);
+    }
+  } else {
+    // ------------------------------------------------------------ epilogue
+    const int sub = warp & 3, half = (warp - 2) >> 2;
+    unsigned char *mine = staging + (warp - 2) * kStagingBytes;
+    const uint32_t columns = tmem + ((uint32_t)(sub * 32) << 16) + (uint32_t)(half * (NT / 2));
+    typename J::Walk walk(p);
+    Tile t;
+    uint32_t done = 0;
+    for (int i = unit; walk.find(p, i, t); i += units) {
+      const bool some = t.k_len > 0;
+      const int buf = done & 1;
+      if (some) {
+        bool ok = mbar_wait_bounded(&acc_full[buf], (done >> 1) & 1, abort_flag, DEV_TIMEOUT_EPILOGUE);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        tc_fence_after();
+      }
+      J::epilogue(p, t, some, columns + (uint32_t)(buf * NT), (int)rank * kRows + sub * 32,
+                  half * (NT / 2), mine);
+      if (some) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (leader) mbar_arrive(&acc_empty[buf]);
+          else mbar_arrive_remote(leader_addr(&acc_empty[buf]));
+        }
+        ++done;
+      }
+    }
+    J::finish(p, (blockIdx.x * kEpilogueWarps + warp - 2), gridDim.x * kEpilogueWarps);
+  }
+
+  tc_fence_before();
+  if constexpr (PAIR == 2) cluster_sync();
+  else __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    if constexpr (PAIR == 2) tmem_dealloc_pair(tmem, kTmemColumns);
+    else tmem_dealloc(tmem, kTmemColumns);
+  }
+}
+
+template <class J>
+int launch(const CUtensorMap &a, const CUtensorMap &b, const typename J::Params &p, int64_t tiles,
+           cudaStream_t st, const char *what) {
+  auto kernel = tile_kernel<J>;
+  constexpr int smem = smem_bytes<J>();
+  static_assert(smem <= kSmemLimit, "shared memory");
+  if (int rc = set_smem_once((const void *)kernel, smem, what)) return rc;
+  const int64_t most = sm_count() / J::PAIR;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((tiles < most ? tiles : most) * J::PAIR));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = J::PAIR;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  count_launch();
+  return check_cuda(cudaLaunchKernelEx(&cfg, kernel, a, b, p), what);
+}
+
+// ---------------------------------------------------------------------------
+// epilogue pieces
+// ---------------------------------------------------------------------------
+template <typename O> __device__ __forceinline__ uint32_t pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
+
+// 16 accumulator columns of the warp's 32 rows (zeros where there are none).
+__device__ __forceinline__ void read16(bool some, uint32_t addr, float (&v)[16]) {
+  if (some) {
+    uint32_t r[16];
+    tmem_ld16_at(addr, r);
+    tmem_ld_wait16(r);
+#pragma unroll
+    for (int x = 0; x < 16; ++x) v[x] = __uint_as_float(r[x]);
+  } else {
+#pragma unroll
+    for (int x = 0; x < 16; ++x) v[x] = 0.f;
+  }
+}
+
+// The 16-byte piece u of row r in a warp's staging (32 rows of 128 bytes,
+// pieces swizzled so that neither row-wise nor piece-wise access conflicts).
+__device__ __forceinline__ uint4 *staged(unsigned char *mine, int r, int u) {
+  return reinterpret_cast<uint4 *>(mine + r * 128 + ((u ^ (r & 7)) << 4));
+}
+
+// Rounds the warp's 32 x COLS accumulators to O and writes the first `rows`
+// rows and `cols` columns of them to out (row pitch ld): every lane rounds
+// its row into the staging, then 8 lanes write 128 consecutive bytes of a row.
+template <typename O, int COLS>
+__device__ __forceinline__ void write_rows(bool some, uint32_t columns, unsigned char *mine, O *out,
+                                           int64_t ld, int rows, int64_t cols, bool vectors) {
+  constexpr int ES = (int)sizeof(O);
+  constexpr int CH = 128 / ES < COLS ? 128 / ES : COLS;   // columns staged at a time
+  constexpr int PIECES = CH * ES / 16;
+  const int lane = threadIdx.x % 32;
+#pragma unroll
+  for (int c0 = 0; c0 < COLS; c0 += CH) {
+    if (c0 >= cols || rows <= 0) break;
+#pragma unroll
+    for (int c = 0; c < CH; c += 16) {
+      float v[16];
+      read16(some, columns + (uint32_t)(c0 + c), v);
+      if constexpr (ES == 4) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          *staged(mine, lane, c / 4 + u) = *reinterpret_cast<uint4 *>(&v[u * 4]);
+      } else {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          *staged(mine, lane, c / 8 + u) =
+              make_uint4(pack2<O>(v[u * 8], v[u * 8 + 1]), pack2<O>(v[u * 8 + 2], v[u * 8 + 3]),
+                         pack2<O>(v[u * 8 + 4], v[u * 8 + 5]), pack2<O>(v[u * 8 + 6], v[u * 8 + 7]));
+      }
+    }
+    __syncwarp();
+    if (vectors && c0 + CH <= cols) {
+#pragma unroll
+      for (int v = lane; v < 32 * PIECES; v += 32) {
+        const int r = v / PIECES, u = v % PIECES;
+        if (r < rows)
+          *reinterpret_cast<uint4 *>(out + r * ld + c0 + u * (16 / ES)) = *staged(mine, r, u);
+      }
+    } else {
+      for (int r = 0; r < rows && r < 32; ++r)
+        for (int c = lane; c < CH && c0 + c < cols; c += 32)
+          out[r * ld + c0 + c] =
+              reinterpret_cast<const O *>(staged(mine, r, c * ES / 16))[c % (16 / ES)];
+    }
+    __syncwarp();
+  }
+}
+
+// fp16 operands (0) or bf16 (1), fp32 accumulator.
+inline uint32_t instruction(int dtype) {
+  const uint32_t f = dtype == OZ_BF16 ? 1 : 0;
+  return 1u << 4 | f << 7 | f << 10;
+}
+
+}  // namespace tile
+}  // namespace oz

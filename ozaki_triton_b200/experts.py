@@ -57,18 +57,41 @@ def _out_dtype(dtype: Optional[torch.dtype], operand: torch.dtype) -> torch.dtyp
     return dtype
 
 
+def _copied(t: torch.Tensor) -> torch.Tensor:
+    """A copy of t whose rows start on 16-byte boundaries."""
+    inner = t.shape[-1]
+    laid = torch.empty((*t.shape[:-1], (inner + 7) // 8 * 8), dtype=t.dtype, device=t.device)
+    return laid[..., :inner].copy_(t)
+
+
+def _as_operand(t: torch.Tensor) -> torch.Tensor:
+    """t, or a copy where the copy unit cannot read its layout: it wants a unit
+    stride along the last dimension, 16-byte boundaries and no repeated rows."""
+    if (t.stride(-1) == 1 or t.shape[-1] == 1) and t.data_ptr() % 16 == 0 and all(
+            n <= 1 or (s > 0 and s % 8 == 0) for n, s in zip(t.shape[:-1], t.stride()[:-1])):
+        return t
+    return _copied(t)
+
+
+def _as_weights(w: torch.Tensor) -> torch.Tensor:
+    """The same for (E, K, N) weights, which may be stored along K or along N."""
+    if w.stride(1) == 1 and w.stride(2) != 1:
+        return _as_operand(w.transpose(1, 2)).transpose(1, 2)
+    return _as_operand(w)
+
+
 def _product(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor,
              out_dtype: torch.dtype) -> torch.Tensor:
     rows, k = x.shape
     groups, _, n = w.shape
     y = torch.empty((rows, n), dtype=out_dtype, device=x.device)
-    x_sr, x_sk = x.stride()
-    w_se, w_sk, w_sn = w.stride()
+    if k > 0 and y.numel() > 0:
+        x, w = _as_operand(x), _as_weights(w)
     with torch.cuda.device(x.device):
         _lib.check(_lib.load().oz_grouped_matmul(
             x.data_ptr(), w.data_ptr(), offsets.data_ptr(), offsets.dtype == torch.int64,
-            _OZ_DTYPE[x.dtype], _OZ_DTYPE[out_dtype], groups, rows, k, n, x_sr, x_sk,
-            w_se, w_sk, w_sn, y.data_ptr(), n, _stream_ptr(x.device)))
+            _OZ_DTYPE[x.dtype], _OZ_DTYPE[out_dtype], groups, rows, k, n, x.stride(0),
+            *w.stride(), y.data_ptr(), n, _stream_ptr(x.device)))
     return y
 
 
@@ -77,11 +100,13 @@ def _weight_gradient(x: torch.Tensor, dy: torch.Tensor, offsets: torch.Tensor, g
     rows, k = x.shape
     n = dy.shape[1]
     dw = torch.empty((groups, k, n), dtype=out_dtype, device=x.device)
+    if rows > 0 and dw.numel() > 0:
+        x, dy = _as_operand(x), _as_operand(dy)
     with torch.cuda.device(x.device):
         _lib.check(_lib.load().oz_grouped_wgrad(
             x.data_ptr(), dy.data_ptr(), offsets.data_ptr(), offsets.dtype == torch.int64,
-            _OZ_DTYPE[x.dtype], _OZ_DTYPE[out_dtype], groups, rows, k, n, *x.stride(),
-            *dy.stride(), dw.data_ptr(), _stream_ptr(x.device)))
+            _OZ_DTYPE[x.dtype], _OZ_DTYPE[out_dtype], groups, rows, k, n, x.stride(0),
+            dy.stride(0), dw.data_ptr(), _stream_ptr(x.device)))
     return dw
 
 
@@ -114,7 +139,9 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, *,
                    out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """y[r] = x[r] @ w[e] for the rows r of each group e; zero rows outside the groups.
 
-    x (T, K) and w (E, K, N) of the same dtype (bf16 or fp16), any strides;
+    x (T, K) and w (E, K, N) of the same dtype (bf16 or fp16), w stored along K
+    or along N (other layouts, and rows that do not start on 16-byte
+    boundaries, are copied first);
     offsets (E + 1,) int32 or int64.  Returns (T, N) in the operands' dtype, or
     fp32 with ``out_dtype=torch.float32``.  Sums are held in fp32 and rounded
     once.  Differentiable in x and w.

@@ -99,7 +99,7 @@ def test_library_entries_validate_without_a_launch():
     n0 = lib.oz_launch_count()
 
     def grouped(dtype=_lib.OZ_F16, out=_lib.OZ_F16, groups=2, rows=4, k=8, n=8, x=p, y=p, ldy=8):
-        return lib.oz_grouped_matmul(x, p, p, 0, dtype, out, groups, rows, k, n, k, 1, k * n, n, 1, y, ldy, None)
+        return lib.oz_grouped_matmul(x, p, p, 0, dtype, out, groups, rows, k, n, k, k * n, n, 1, y, ldy, None)
     assert grouped(dtype=_lib.OZ_F32) == _lib.OZ_ERR_UNSUPPORTED
     assert grouped(out=_lib.OZ_BF16) == _lib.OZ_ERR_UNSUPPORTED
     assert grouped(groups=0) == _lib.OZ_ERR_INVALID
@@ -109,9 +109,11 @@ def test_library_entries_validate_without_a_launch():
     assert grouped(x=None) == _lib.OZ_ERR_INVALID
     assert grouped(y=None) == _lib.OZ_ERR_INVALID
     assert grouped(rows=0, y=None) == _lib.OZ_OK
+    assert grouped(x=ctypes.c_void_p(264)) == _lib.OZ_ERR_INVALID
+    assert grouped(k=12) == _lib.OZ_ERR_INVALID          # rows 24 bytes apart
 
     def wgrad(dtype=_lib.OZ_F16, groups=2, dw=p, k=8):
-        return lib.oz_grouped_wgrad(p, p, p, 0, dtype, dtype, groups, 4, k, 8, 8, 1, 8, 1, dw, None)
+        return lib.oz_grouped_wgrad(p, p, p, 0, dtype, dtype, groups, 4, k, 8, 8, 8, dw, None)
     assert wgrad(dtype=_lib.OZ_I8) == _lib.OZ_ERR_UNSUPPORTED
     assert wgrad(groups=-1) == _lib.OZ_ERR_INVALID
     assert wgrad(dw=None) == _lib.OZ_ERR_INVALID
