@@ -318,6 +318,14 @@ __device__ __forceinline__ void tc_commit_pair(uint32_t bar_cluster_addr) {
           bar_cluster_addr)
       : "memory");
 }
+// The same on the barrier at this offset of both CTAs of the pair (bar: this CTA's).
+__device__ __forceinline__ void tc_commit_both(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+      "[%0], %1;" ::"r"(bar),
+      "h"((uint16_t)3)
+      : "memory");
+}
 // Arrive on an mbarrier of another CTA of the cluster.
 __device__ __forceinline__ void mbar_arrive_remote(uint32_t bar_cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(

@@ -100,7 +100,7 @@ struct RowTile { int row, rows, column; };   // first row, rows from there to th
 
 // y = x w: A is the rows of x, B the columns of w[e].
 template <typename O, int PAIR_, int NT_, bool BMN_> struct RowsJob {
-  static constexpr int PAIR = PAIR_, NT = NT_, PLANES = 1;
+  static constexpr int PAIR = PAIR_, NT = NT_, PLANES = 1, PASS = sizeof(O) == 4 ? 8 : 0;
   static constexpr bool AMN = false, BMN = BMN_, RAGGED = false;
   using Params = GroupedParams;
   using Extra = RowTile;
@@ -120,10 +120,11 @@ template <typename O, int PAIR_, int NT_, bool BMN_> struct RowsJob {
       return true;
     }
   };
-  static __device__ void epilogue(const Params &p, const TileOf<Extra> &t, bool some, uint32_t columns,
-                                  int row, int column, unsigned char *mine) {
+  template <class Source>
+  static __device__ void epilogue(const Params &p, const TileOf<Extra> &t, const Source &source, int row,
+                                  int column, unsigned char *mine) {
     const int64_t c0 = t.extra.column + column;
-    write_rows<O, NT / 2>(some, columns, mine,
+    write_rows<O, NT / 2>(source, mine,
                           static_cast<O *>(p.out) + (int64_t)(t.extra.row + row) * p.ld + c0, p.ld,
                           t.extra.rows - row, p.n - c0, p.vectors);
   }
@@ -134,7 +135,7 @@ template <typename O, int PAIR_, int NT_, bool BMN_> struct RowsJob {
 // 128 columns of w[e], B up to NT rows of x, so a tile's weights are read
 // once and hardly any of the staged bytes belong to rows that are not there.
 template <typename O, int NT_, bool AMN_> struct ColumnsJob {
-  static constexpr int PAIR = 1, NT = NT_, PLANES = 1;
+  static constexpr int PAIR = 1, NT = NT_, PLANES = 1, PASS = sizeof(O) == 4 ? 8 : 0;
   static constexpr bool AMN = AMN_, BMN = false, RAGGED = false;
   using Params = GroupedParams;
   using Extra = RowTile;
@@ -154,16 +155,17 @@ template <typename O, int NT_, bool AMN_> struct ColumnsJob {
       return true;
     }
   };
-  static __device__ void epilogue(const Params &p, const TileOf<Extra> &t, bool some, uint32_t columns,
-                                  int row, int column, unsigned char *) {
+  template <class Source>
+  static __device__ void epilogue(const Params &p, const TileOf<Extra> &t, const Source &source, int row,
+                                  int column, unsigned char *) {
     const int64_t c = t.extra.column + row + threadIdx.x % 32;
     O *out = static_cast<O *>(p.out) + (int64_t)(t.extra.row + column) * p.ld + c;
     const int rows = t.extra.rows - column;
 #pragma unroll
     for (int r0 = 0; r0 < NT / 2; r0 += 16) {
-      if (r0 >= rows) break;
+      if (r0 >= rows) continue;
       float v[16];
-      read16(some, columns + (uint32_t)r0, v);
+      source.read(r0, v);
 #pragma unroll
       for (int r = 0; r < 16; ++r)
         if (r0 + r < rows && c < p.n) out[(r0 + r) * p.ld] = O(v[r]);
@@ -177,7 +179,7 @@ struct WeightTile { int row, column, group; };
 // dw[e] = x^T dy over the group's rows: both operands are stored across the
 // contraction, whose range is the group.
 template <typename O, int PAIR_, int NT_> struct WeightsJob {
-  static constexpr int PAIR = PAIR_, NT = NT_, PLANES = 1;
+  static constexpr int PAIR = PAIR_, NT = NT_, PLANES = 1, PASS = sizeof(O) == 4 ? 8 : 0;
   static constexpr bool AMN = true, BMN = true, RAGGED = true;
   using Params = GroupedParams;
   using Extra = WeightTile;
@@ -191,9 +193,12 @@ template <typename O, int PAIR_, int NT_> struct WeightsJob {
       const int e = i / per;
       if (e >= p.groups) return false;
       if (e != group) group_rows(p.offsets, p.wide, group = e, p.rows, begin, end);
-      const int local = i - e * per;
-      t.a_row = local % row_tiles * kRows * PAIR;
-      t.b_row = local / row_tiles * NT;
+      // 8 row tiles at a time sweep the columns, so that the tiles of a wave
+      // share their operands in L2
+      const int local = i - e * per, sweep = local / (8 * p.column_tiles);
+      const int in = local - sweep * 8 * p.column_tiles, size = min(row_tiles - sweep * 8, 8);
+      t.a_row = (sweep * 8 + in % size) * kRows * PAIR;
+      t.b_row = in / size * NT;
       t.a_mat = t.b_mat = 0;
       t.k_begin = begin;
       t.k_len = end - begin;
@@ -201,10 +206,11 @@ template <typename O, int PAIR_, int NT_> struct WeightsJob {
       return true;
     }
   };
-  static __device__ void epilogue(const Params &p, const TileOf<Extra> &t, bool some, uint32_t columns,
-                                  int row, int column, unsigned char *mine) {
+  template <class Source>
+  static __device__ void epilogue(const Params &p, const TileOf<Extra> &t, const Source &source, int row,
+                                  int column, unsigned char *mine) {
     const int64_t r0 = t.extra.row + row, c0 = t.extra.column + column;
-    write_rows<O, NT / 2>(some, columns, mine,
+    write_rows<O, NT / 2>(source, mine,
                           static_cast<O *>(p.out) + ((int64_t)t.extra.group * p.k + r0) * p.ld + c0,
                           p.ld, (int)(p.k - r0), p.n - c0, p.vectors);
   }

@@ -20,7 +20,13 @@
 // With RAGGED the contraction runs over a tile's own range of rows
 // [k_begin, k_begin + k_len) of longer operands: the rows of the last block
 // past the range are overwritten with zeros in shared memory before they are
-// multiplied (in both operands: a zero times a stray NaN is a NaN).
+// multiplied (in both operands: a zero times a stray NaN is a NaN), by each
+// CTA's MMA warp, so that the producer runs on to the next tile's blocks.
+//
+// With PASS > 0 an accumulator takes at most PASS blocks and the epilogue adds
+// the passes in registers: the tensor core cuts each sum off instead of
+// rounding it, an error that grows with the number of blocks (relative 1.1e-6
+// at 2048 terms of one sign), and that an fp32 result would show.
 //
 // With PLANES = 2 each operand is a sum of two fp16 slices and a block adds
 // high*high, high*low and low*high to the accumulator (low*low is below the
@@ -142,6 +148,33 @@ __device__ __forceinline__ bool wait_cluster(uint64_t *bar, uint32_t parity, vol
   }
 }
 
+// Where an epilogue finds its warp's accumulators, 32 rows (one a lane) by
+// NT / 2 columns, 16 columns at a time: in TMEM (zeros for an empty
+// contraction), or summed over the passes in registers.
+struct Columns {
+  bool some;
+  uint32_t addr;
+  __device__ __forceinline__ void read(int c, float (&v)[16]) const {
+    if (some) {
+      uint32_t r[16];
+      tmem_ld16_at(addr + (uint32_t)c, r);
+      tmem_ld_wait16(r);
+#pragma unroll
+      for (int x = 0; x < 16; ++x) v[x] = __uint_as_float(r[x]);
+    } else {
+#pragma unroll
+      for (int x = 0; x < 16; ++x) v[x] = 0.f;
+    }
+  }
+};
+template <int N> struct Registers {
+  const float (&sum)[N];
+  __device__ __forceinline__ void read(int c, float (&v)[16]) const {
+#pragma unroll
+    for (int x = 0; x < 16; ++x) v[x] = sum[c + x];
+  }
+};
+
 template <class J>
 __global__ void __launch_bounds__(kThreads, 1)
     tile_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
@@ -163,7 +196,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t *acc_empty = acc_full + 2;                 // [2]
   uint64_t *drain = acc_empty + 2;
   uint64_t *tail = drain + 1;                         // RAGGED: this CTA's last block has landed
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tail + 1);
+  uint64_t *peer_tail = tail + kMaxStages;            // RAGGED: the other CTA's has been cleared
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(peer_tail + kMaxStages);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -173,15 +207,16 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < S; ++i) {
-      mbar_init(&full[i], J::RAGGED ? PAIR : 1);
+      mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
+      mbar_init(&tail[i], 1);
+      mbar_init(&peer_tail[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&acc_full[i], 1);
       mbar_init(&acc_empty[i], PAIR * kEpilogueWarps);
     }
     mbar_init(drain, 1);
-    mbar_init(tail, 1);
     *abort_flag = 0;
     fence_mbar_init();
     prefetch_tmap(&tm_a);
@@ -211,83 +246,70 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ------------------------------------------------------------ producer
     typename J::Walk walk(p);
     Tile t;
-    uint32_t it = 0, tails = 0;
+    uint32_t it = 0, ended = 0, turn = 0;             // slots whose tail was used; parity of the last use
     bool ok = true;
     for (int i = unit; ok && walk.find(p, i, t); i += units) {
       const int blocks = (int)((t.k_len + kBlock - 1) / kBlock);
-      const int rest = J::RAGGED ? (int)(t.k_len % kBlock) : 0;
-      for (int kb = 0; kb < blocks; ++kb, ++it) {
-        const int slot = it % S;
-        unsigned char *st = smem + slot * SB;
-        const bool last = J::RAGGED && rest && kb == blocks - 1;
-        if (lane == 0) {
-          ok = mbar_wait_bounded(&empty[slot], ((it / S) & 1) ^ 1, abort_flag, DEV_TIMEOUT_PRODUCER);
-          if (ok) {
-            // every box lands in this CTA; its bytes count on the leader's
-            // barrier, or on the CTA's own before a ragged end is cleared
-            uint32_t bar;
-            if (last) {
-              mbar_arrive_expect_tx(tail, SB);
-              bar = smem_u32(tail);
-            } else {
-              bar = leader_addr(&full[slot]);
-              if (leader) mbar_arrive_expect_tx(&full[slot], PAIR * SB);
-              else if constexpr (J::RAGGED) mbar_arrive_remote(bar);
-            }
-            auto load = [&](void *dst, const CUtensorMap *map, int c0, int c1, int c2) {
-              if constexpr (PAIR == 2) {
-                if (!last) {
-                  tma_load_3d_pair(dst, map, bar, c0, c1, c2);
-                  return;
-                }
-              }
-              tma_load_3d(dst, map, last ? tail : &full[slot], c0, c1, c2);
-            };
-            const int k = (int)(t.k_begin + (int64_t)kb * kBlock);
-            const int ar = t.a_row + (int)rank * kRows, br = t.b_row + (int)rank * BR;
-#pragma unroll
-            for (int pl = 0; pl < J::PLANES; ++pl) {
-              unsigned char *sa = st + pl * a_bytes<J>();
-              unsigned char *sb = st + J::PLANES * a_bytes<J>() + pl * b_bytes<J>();
-              const int am = t.a_mat + pl * J::plane_stride(p), bm = t.b_mat + pl * J::plane_stride(p);
-              if constexpr (J::AMN)
-                for (int c = 0; c < kRows / 64; ++c)
-                  load(sa + c * kBlock * kLine, &tm_a, ar + c * 64, k, am);
-              else load(sa, &tm_a, k, ar, am);
-              if constexpr (J::BMN)
-                for (int c = 0; c < BR / 64; ++c)
-                  load(sb + c * kBlock * kLine, &tm_b, br + c * 64, k, bm);
-              else load(sb, &tm_b, k, br, bm);
-            }
-            if (last) ok = mbar_wait_bounded(tail, tails & 1, abort_flag, DEV_TIMEOUT_PRODUCER);
-          }
-        }
-        if constexpr (J::RAGGED) {
+      const bool ragged = J::RAGGED && t.k_len % kBlock;
+      if (lane == 0) {
+        const int ar = t.a_row + (int)rank * kRows, br = t.b_row + (int)rank * BR;
+        for (int kb = 0; kb < blocks; ++kb, ++it) {
+          const int slot = it % S;
+          unsigned char *st = smem + slot * SB;
+          if (!(ok = mbar_wait_bounded(&empty[slot], ((it / S) & 1) ^ 1, abort_flag,
+                                       DEV_TIMEOUT_PRODUCER)))
+            break;
+          // a block's bytes count on the leader's barrier; those of a block
+          // that ends the range count on each CTA's own, for its MMA warp
+          const bool last = ragged && kb == blocks - 1;
+          const uint32_t bar = leader_addr(&full[slot]);
           if (last) {
-            ++tails;
-            ok = __shfl_sync(0xffffffffu, (int)ok, 0);
-            if (ok) {
-              // rows [rest, 64) of every chunk: whole 128-byte lines, so the swizzle does not matter
-              constexpr int chunks = SB / (kBlock * kLine);
-              const int lines = (kBlock - rest) * 8;           // 16-byte pieces of a chunk's lines
-              for (int v = lane; v < chunks * lines; v += 32)
-                *reinterpret_cast<uint4 *>(st + v / lines * (kBlock * kLine) + rest * kLine +
-                                           v % lines * 16) = make_uint4(0, 0, 0, 0);
-              fence_proxy_async_smem();
-              __syncwarp();
-              if (lane == 0) {
-                if (leader) mbar_arrive(&full[slot]);
-                else mbar_arrive_remote(leader_addr(&full[slot]));
+            mbar_arrive_expect_tx(&tail[slot], SB);
+            turn ^= ((ended >> slot) & 1) << slot;
+            ended |= 1u << slot;
+            if (leader) mbar_arrive(&full[slot]);
+          } else if (leader) {
+            mbar_arrive_expect_tx(&full[slot], PAIR * SB);
+          }
+          auto load = [&](void *dst, const CUtensorMap *map, int c0, int c1, int c2) {
+            if constexpr (PAIR == 2) {
+              if (!last) {
+                tma_load_3d_pair(dst, map, bar, c0, c1, c2);
+                return;
               }
+            }
+            tma_load_3d(dst, map, last ? &tail[slot] : &full[slot], c0, c1, c2);
+          };
+          const int k = (int)(t.k_begin + (int64_t)kb * kBlock);
+#pragma unroll
+          for (int pl = 0; pl < J::PLANES; ++pl) {
+            unsigned char *sa = st + pl * a_bytes<J>();
+            unsigned char *sb = st + J::PLANES * a_bytes<J>() + pl * b_bytes<J>();
+            const int am = t.a_mat + pl * J::plane_stride(p), bm = t.b_mat + pl * J::plane_stride(p);
+            if constexpr (J::AMN) {
+#pragma unroll
+              for (int c = 0; c < kRows / 64; ++c)
+                load(sa + c * kBlock * kLine, &tm_a, ar + c * 64, k, am);
+            } else {
+              load(sa, &tm_a, k, ar, am);
+            }
+            if constexpr (J::BMN) {
+#pragma unroll
+              for (int c = 0; c < BR / 64; ++c)
+                load(sb + c * kBlock * kLine, &tm_b, br + c * 64, k, bm);
+            } else {
+              load(sb, &tm_b, k, br, bm);
             }
           }
         }
-        ok = __shfl_sync(0xffffffffu, (int)ok, 0);
-        if (!ok) break;
       }
+      ok = __shfl_sync(0xffffffffu, (int)ok, 0);
     }
-    // every load that counts on the leader's barriers must have landed before
-    // shared memory goes away
+    // every load must have landed before shared memory goes away
+    if (lane == 0)
+      for (int slot = 0; J::RAGGED && slot < S; ++slot)
+        if ((ended >> slot) & 1)
+          mbar_wait_bounded(&tail[slot], (turn >> slot) & 1, abort_flag, DEV_TIMEOUT_PRODUCER);
     if (lane == 0 && leader)
       for (uint32_t k = (it > (uint32_t)S ? it - S : 0); k < it; ++k)
         mbar_wait_bounded(&full[k % S], (k / S) & 1, abort_flag, DEV_TIMEOUT_PRODUCER);
@@ -295,7 +317,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ------------------------------------------------------------ MMA issuer
     typename J::Walk walk(p);
     Tile t;
-    uint32_t it = 0, done = 0;
+    uint32_t done = 0;
     bool ok = true;
     const uint32_t base = smem_u32(smem);
     const uint32_t idesc = p.idesc | ((uint32_t)(NT >> 3) << 17) |
@@ -303,45 +325,114 @@ __global__ void __launch_bounds__(kThreads, 1)
                            (J::BMN ? 1u << 16 : 0u);
     constexpr uint64_t a_step = J::AMN ? (16 * kLine) >> 4 : 2, b_step = J::BMN ? (16 * kLine) >> 4 : 2;
     auto release = [&](uint64_t *bar) {
-      if constexpr (PAIR == 2) {
-        tc_commit_pair(smem_u32(bar));
-        tc_commit_pair(map_to_cta(smem_u32(bar), 1));
-      } else {
-        tc_commit(bar);
-      }
+      if constexpr (PAIR == 2) tc_commit_both(smem_u32(bar));
+      else tc_commit(bar);
     };
     auto wait = [&](uint64_t *bar, uint32_t parity) {
       if constexpr (PAIR == 2) return wait_cluster(bar, parity, abort_flag, DEV_TIMEOUT_MMA);
       else return mbar_wait_bounded(bar, parity, abort_flag, DEV_TIMEOUT_MMA);
     };
+    // the issuing thread must not fall behind the tensor core, which holds only
+    // a few instructions: descriptors are one base plus the slot's offset
+    const uint64_t a_desc = operand_desc<J::AMN>(base);
+    const uint64_t b_desc = operand_desc<J::BMN>(base + J::PLANES * a_bytes<J>());
+    uint32_t slot = 0, phase = 0;
+    auto multiply = [&](uint32_t d, bool first) {
+      const uint64_t ad = a_desc + slot * (SB >> 4), bd = b_desc + slot * (SB >> 4);
+#pragma unroll
+      for (int q = 0; q < (J::PLANES == 2 ? 3 : 1); ++q) {
+        const uint64_t aq = ad + (q == 2 ? a_bytes<J>() >> 4 : 0);
+        const uint64_t bq = bd + (q == 1 ? b_bytes<J>() >> 4 : 0);
+#pragma unroll
+        for (int kk = 0; kk < kBlock / 16; ++kk) {
+          const uint32_t add = (kk | q) ? 1u : (first ? 0u : 1u);
+          if constexpr (PAIR == 2) tc_mma_pair<1>(d, aq + kk * a_step, bq + kk * b_step, idesc, add);
+          else tc_mma<1>(d, aq + kk * a_step, bq + kk * b_step, idesc, add);
+        }
+      }
+      release(&empty[slot]);
+    };
+    auto advance = [&]() {
+      if (++slot == S) {
+        slot = 0;
+        phase ^= 1;
+      }
+    };
+    uint32_t tails = 0;                               // parity of each slot's tail barriers
     for (int i = unit; ok && walk.find(p, i, t); i += units) {
-      const int blocks = (int)((t.k_len + kBlock - 1) / kBlock);
-      if (blocks == 0) continue;                      // the epilogue writes zeros by itself
-      if (lane == 0 && leader) {
+      const int blocks = (int)((t.k_len + kBlock - 1) / kBlock);   // none: the epilogue writes zeros
+      const int rest = J::RAGGED ? (int)(t.k_len % kBlock) : 0;
+      const int whole = blocks - (rest ? 1 : 0);
+      const uint32_t slot0 = slot, phase0 = phase;
+      uint32_t d = 0;
+      auto start = [&]() {
         const int buf = done & 1;
-        ok = wait(&acc_empty[buf], ((done >> 1) & 1) ^ 1);
+        if (!wait(&acc_empty[buf], ((done >> 1) & 1) ^ 1)) return false;
         tc_fence_after();
-        const uint32_t d = tmem + (uint32_t)(buf * NT);
-        for (int kb = 0; ok && kb < blocks; ++kb, ++it) {
-          const int slot = it % S;
-          if (!(ok = wait(&full[slot], (it / S) & 1))) break;
-          const uint32_t sa = base + slot * SB, sb = sa + J::PLANES * a_bytes<J>();
-#pragma unroll
-          for (int q = 0; q < (J::PLANES == 2 ? 3 : 1); ++q) {
-            const uint64_t ad = operand_desc<J::AMN>(sa + (q == 2 ? a_bytes<J>() : 0));
-            const uint64_t bd = operand_desc<J::BMN>(sb + (q == 1 ? b_bytes<J>() : 0));
-#pragma unroll
-            for (int kk = 0; kk < kBlock / 16; ++kk) {
-              const uint32_t add = (uint32_t)((kb | kk | q) != 0);
-              if constexpr (PAIR == 2) tc_mma_pair<1>(d, ad + kk * a_step, bd + kk * b_step, idesc, add);
-              else tc_mma<1>(d, ad + kk * a_step, bd + kk * b_step, idesc, add);
+        d = tmem + (uint32_t)(buf * NT);
+        return true;
+      };
+      auto end = [&]() {
+        release(&acc_full[done & 1]);
+        ++done;
+      };
+      if (lane == 0 && leader) {
+        // accumulator by accumulator: all blocks, or PASS at a time
+        int kb = 0;
+        while (kb < whole) {
+          const int stop = J::PASS ? min(whole, kb + J::PASS) : whole;
+          if (!(ok = start())) break;
+          bool first = true;
+          for (; kb < stop; ++kb) {
+            if (!(ok = wait(&full[slot], phase))) break;
+            multiply(d, first);
+            first = false;
+            advance();
+          }
+          if (!ok) break;
+          if (kb < whole || !rest || (J::PASS && kb % (J::PASS + !J::PASS) == 0)) end();
+        }
+      }
+      if (whole > 0) {                                // the other lanes, and where this one stopped
+        const uint32_t n = slot0 + (uint32_t)whole;
+        slot = n % S;
+        phase = phase0 ^ (n / S & 1);
+      }
+      if constexpr (J::RAGGED) {
+        if (rest) {
+          unsigned char *st = smem + slot * SB;
+          const uint32_t parity = (tails >> slot) & 1;
+          ok = __shfl_sync(0xffffffffu, (int)ok, 0);
+          ok = ok && mbar_wait_bounded(&tail[slot], parity, abort_flag, DEV_TIMEOUT_MMA);
+          ok = __all_sync(0xffffffffu, ok);
+          if (ok) {
+            // rows [rest, 64) of every chunk: whole 128-byte lines, so the swizzle does not matter
+            constexpr int chunks = SB / (kBlock * kLine);
+            const int pieces = (kBlock - rest) * 8;          // 16-byte pieces of a chunk's lines
+            for (int c = 0; c < chunks; ++c)
+              for (int v = lane; v < pieces; v += 32)
+                *reinterpret_cast<uint4 *>(st + c * (kBlock * kLine) + rest * kLine + v * 16) =
+                    make_uint4(0, 0, 0, 0);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              if (leader) {
+                const bool first = whole == 0 || (J::PASS && whole % (J::PASS + !J::PASS) == 0);
+                ok = (!first || start()) && wait(&full[slot], phase);
+                if constexpr (PAIR == 2) ok = ok && wait(&peer_tail[slot], parity);
+                if (ok) {
+                  multiply(d, first);
+                  end();
+                }
+              } else {
+                mbar_arrive_remote(leader_addr(&peer_tail[slot]));
+              }
             }
           }
-          release(&empty[slot]);
+          tails ^= 1u << slot;
+          advance();
         }
-        if (ok) release(&acc_full[buf]);
       }
-      ++done;
       ok = __shfl_sync(0xffffffffu, (int)ok, 0);
     }
     if (lane == 0 && leader) {
@@ -357,24 +448,51 @@ __global__ void __launch_bounds__(kThreads, 1)
     typename J::Walk walk(p);
     Tile t;
     uint32_t done = 0;
-    for (int i = unit; walk.find(p, i, t); i += units) {
-      const bool some = t.k_len > 0;
-      const int buf = done & 1;
-      if (some) {
-        bool ok = mbar_wait_bounded(&acc_full[buf], (done >> 1) & 1, abort_flag, DEV_TIMEOUT_EPILOGUE);
-        if (!__all_sync(0xffffffffu, ok)) break;
-        tc_fence_after();
+    auto acquire = [&]() {
+      const bool ok = mbar_wait_bounded(&acc_full[done & 1], (done >> 1) & 1, abort_flag,
+                                        DEV_TIMEOUT_EPILOGUE);
+      if (!__all_sync(0xffffffffu, ok)) return false;
+      tc_fence_after();
+      return true;
+    };
+    auto hand_back = [&]() {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (leader) mbar_arrive(&acc_empty[done & 1]);
+        else mbar_arrive_remote(leader_addr(&acc_empty[done & 1]));
       }
-      J::epilogue(p, t, some, columns + (uint32_t)(buf * NT), (int)rank * kRows + sub * 32,
-                  half * (NT / 2), mine);
-      if (some) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          if (leader) mbar_arrive(&acc_empty[buf]);
-          else mbar_arrive_remote(leader_addr(&acc_empty[buf]));
+      ++done;
+    };
+    for (int i = unit; walk.find(p, i, t); i += units) {
+      const int row = (int)rank * kRows + sub * 32, column = half * (NT / 2);
+      if constexpr (J::PASS > 0) {
+        float sum[NT / 2];
+#pragma unroll
+        for (int c = 0; c < NT / 2; ++c) sum[c] = 0.f;
+        const int blocks = (int)((t.k_len + kBlock - 1) / kBlock);
+        bool ok = true;
+        for (int kb = 0; ok && kb < blocks; kb += J::PASS) {
+          if (!(ok = acquire())) break;
+#pragma unroll
+          for (int c = 0; c < NT / 2; c += 32) {
+            uint32_t r[32];
+            tmem_ld16_at(columns + (uint32_t)((done & 1) * NT + c), r);
+            tmem_ld16_at(columns + (uint32_t)((done & 1) * NT + c + 16), r + 16);
+            tmem_ld_wait16(*reinterpret_cast<uint32_t(*)[16]>(r));
+            tmem_ld_wait16(*reinterpret_cast<uint32_t(*)[16]>(r + 16));
+#pragma unroll
+            for (int x = 0; x < 32; ++x) sum[c + x] += __uint_as_float(r[x]);
+          }
+          hand_back();
         }
-        ++done;
+        if (!ok) break;
+        J::epilogue(p, t, Registers<NT / 2>{sum}, row, column, mine);
+      } else {
+        const bool some = t.k_len > 0;
+        if (some && !acquire()) break;
+        J::epilogue(p, t, Columns{some, columns + (uint32_t)((done & 1) * NT)}, row, column, mine);
+        if (some) hand_back();
       }
     }
     J::finish(p, (blockIdx.x * kEpilogueWarps + warp - 2), gridDim.x * kEpilogueWarps);
@@ -427,20 +545,6 @@ template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, fl
   return *reinterpret_cast<const uint32_t *>(&v);
 }
 
-// 16 accumulator columns of the warp's 32 rows (zeros where there are none).
-__device__ __forceinline__ void read16(bool some, uint32_t addr, float (&v)[16]) {
-  if (some) {
-    uint32_t r[16];
-    tmem_ld16_at(addr, r);
-    tmem_ld_wait16(r);
-#pragma unroll
-    for (int x = 0; x < 16; ++x) v[x] = __uint_as_float(r[x]);
-  } else {
-#pragma unroll
-    for (int x = 0; x < 16; ++x) v[x] = 0.f;
-  }
-}
-
 // The 16-byte piece u of row r in a warp's staging (32 rows of 128 bytes,
 // pieces swizzled so that neither row-wise nor piece-wise access conflicts).
 __device__ __forceinline__ uint4 *staged(unsigned char *mine, int r, int u) {
@@ -450,20 +554,19 @@ __device__ __forceinline__ uint4 *staged(unsigned char *mine, int r, int u) {
 // Rounds the warp's 32 x COLS accumulators to O and writes the first `rows`
 // rows and `cols` columns of them to out (row pitch ld): every lane rounds
 // its row into the staging, then 8 lanes write 128 consecutive bytes of a row.
-template <typename O, int COLS>
-__device__ __forceinline__ void write_rows(bool some, uint32_t columns, unsigned char *mine, O *out,
-                                           int64_t ld, int rows, int64_t cols, bool vectors) {
+template <typename O, int COLS, class Source>
+__device__ __forceinline__ void write_rows(const Source &source, unsigned char *mine, O *out, int64_t ld, int rows, int64_t cols, bool vectors) {
   constexpr int ES = (int)sizeof(O);
   constexpr int CH = 128 / ES < COLS ? 128 / ES : COLS;   // columns staged at a time
   constexpr int PIECES = CH * ES / 16;
   const int lane = threadIdx.x % 32;
 #pragma unroll
   for (int c0 = 0; c0 < COLS; c0 += CH) {
-    if (c0 >= cols || rows <= 0) break;
+    if (c0 >= cols || rows <= 0) continue;
 #pragma unroll
     for (int c = 0; c < CH; c += 16) {
       float v[16];
-      read16(some, columns + (uint32_t)(c0 + c), v);
+      source.read(c0 + c, v);
       if constexpr (ES == 4) {
 #pragma unroll
         for (int u = 0; u < 4; ++u)
