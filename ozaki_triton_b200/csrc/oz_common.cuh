@@ -59,6 +59,7 @@ static __device__ int g_device_status = 0;
 int status_split(int *value, bool clear);
 int status_gemm(int *value, bool clear);
 int status_experts(int *value, bool clear);
+int status_newton(int *value, bool clear);
 
 // Split of both operands of a product in one launch (oz_split.cu): A's rows
 // (a_sm, a_sk: line and k strides) and B's columns (b_sn, b_sk), each into

@@ -1,41 +1,91 @@
 // oz_newton.cu -- orthogonalisation of a batch of matrices by quintic
-// Newton-Schulz steps.
+// Newton-Schulz steps on the tile engine (oz_tile.cuh).
 //
 //   X_0 = G / (|G|_F + eps)
-//   A = X X^T,  X <- a X + (b A + c A^2) X        `steps` times
+//   S = X X^T,  P = b S + c S S,  X <- a X + P X          `steps` times
 //
 // for G with at most as many rows as columns; a tall G is worked on through
 // its transpose (the polynomial is odd, so it commutes with transposing).
-// Everything is held in fp32; the sum of squares in fp64.
+//
+// Every matrix is held as fp16 slices at a power-of-two scale of its own:
+// high = fp16(v 2^e), low = fp16(v 2^e - high).  The host bounds the norms
+// step by step (the singular values start in [0, 1] and a step's polynomial
+// is known), so e puts the bound at 2^15 and nothing can overflow; no data
+// is looked at.  With one slice the products use `high` alone (11 bits) and
+// only the term a X keeps X's 22: that term carries the directions that the
+// products hardly touch, and rounding it as well as P X makes both sides of
+// the sum consistent only for full-rank G (measured on a low-rank gradient:
+// 2.2e-2 with 11 bits there, 4.5e-4 with 22).  With two slices the products add
+// high*high + high*low + low*high.  S and P are symmetric: only the tiles on
+// and below the diagonal are multiplied, each written twice.
 
-#include "oz_common.cuh"
+#include <algorithm>
+#include <cmath>
+
+#include "oz_tile.cuh"
 
 namespace oz {
+int status_newton(int *value, bool clear) { return read_status_word(value, clear); }
+
 namespace {
+using namespace tile;
 
-constexpr int kTile = 64;
-constexpr int kStep = 16;
-constexpr int kNormBlocks = 64;
+constexpr int kMostPartials = 256;     // blocks that add the squares of a matrix
 
-template <typename T> __device__ __forceinline__ float get(const void *p, int64_t i) {
-  return InTraits<T>::to_float(static_cast<const T *>(p)[i]);
+__device__ __forceinline__ float load_value(const void *p, int dtype, int64_t i) {
+  if (dtype == OZ_F32) return static_cast<const float *>(p)[i];
+  if (dtype == OZ_F16) return __half2float(static_cast<const __half *>(p)[i]);
+  return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
 }
+
+// v as slices: high, and what is left of it.
+__device__ __forceinline__ void slice(float v, __half &high, __half &low) {
+  high = __float2half_rn(v);
+  low = __float2half_rn(v - __half2float(high));
+}
+
+// A matrix in slices: plane q of member z at base + (q * batch + z) * mat.
+struct Planes {
+  __half *base;
+  int64_t ld, mat, plane;
+  __device__ __half *at(int q, int z, int64_t row, int64_t column) const {
+    return base + q * plane + z * mat + row * ld + column;
+  }
+};
 
 struct InitParams {
   const void *g;
-  int64_t rows, cols;               // rows <= cols, after the transposition of a tall G
-  int64_t g_sb, g_sr, g_sc;
-  double *partial;                  // (batch, kNormBlocks) sums of squares
-  float *x;                         // (batch, rows, cols)
-  double eps;
+  int dtype, partials;
+  int rows, cols;                   // rows <= cols, after the transposition of a tall G
+  int64_t g_sb, g_sr, g_sc;         // strides of G's member, and of X's rows and columns in G
+  double *partial;                  // (batch, partials) sums of squares
+  Planes x;
+  double eps, scale;
 };
 
-template <typename T> __global__ void __launch_bounds__(256) squares_kernel(const InitParams p) {
+// Sums of squares in fp64 (fp32 would overflow from 1.8e19 on), each block a
+// fixed part: the order of the sum does not depend on the launch.
+__global__ void __launch_bounds__(256) squares_kernel(const InitParams p) {
   __shared__ double part[8];
-  const int64_t total = p.rows * p.cols;
+  // consecutive threads along the smaller stride
+  const bool across = p.g_sr < p.g_sc;
+  const int64_t inner = across ? p.rows : p.cols, total = (int64_t)p.rows * p.cols;
+  const int64_t s_in = across ? p.g_sr : p.g_sc, s_out = across ? p.g_sc : p.g_sr;
+  const int64_t base = blockIdx.y * p.g_sb, stride = (int64_t)gridDim.x * 256;
   double sum = 0;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += kNormBlocks * 256) {
-    const double v = get<T>(p.g, blockIdx.y * p.g_sb + i / p.cols * p.g_sr + i % p.cols * p.g_sc);
+  int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  for (; i + 3 * stride < total; i += 4 * stride) {
+    float v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int64_t q = i + u * stride;
+      v[u] = load_value(p.g, p.dtype, base + q / inner * s_out + q % inner * s_in);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) sum += (double)v[u] * v[u];
+  }
+  for (; i < total; i += stride) {
+    const double v = load_value(p.g, p.dtype, base + i / inner * s_out + i % inner * s_in);
     sum += v * v;
   }
   for (int o = 16; o; o /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -43,110 +93,451 @@ template <typename T> __global__ void __launch_bounds__(256) squares_kernel(cons
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int w = 1; w < 8; ++w) part[0] += part[w];
-    p.partial[(int64_t)blockIdx.y * kNormBlocks + blockIdx.x] = part[0];
+    p.partial[(int64_t)blockIdx.y * p.partials + blockIdx.x] = part[0];
   }
 }
 
-template <typename T> __global__ void __launch_bounds__(256) normalise_kernel(const InitParams p) {
+// X_0 in slices, 32 x 32 tiles through shared memory: G is read along its
+// smaller stride and X written along its rows.
+__global__ void __launch_bounds__(256) normalise_kernel(const InitParams p) {
+  __shared__ double part[8];
+  __shared__ float v[32][33];
   double sum = 0;
-  for (int i = 0; i < kNormBlocks; ++i) sum += p.partial[(int64_t)blockIdx.y * kNormBlocks + i];
-  const double scale = 1.0 / (sqrt(sum) + p.eps);
-  const int64_t total = p.rows * p.cols;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256)
-    p.x[blockIdx.y * total + i] = (float)(
-        get<T>(p.g, blockIdx.y * p.g_sb + i / p.cols * p.g_sr + i % p.cols * p.g_sc) * scale);
+  for (int i = threadIdx.x; i < p.partials; i += 256) sum += p.partial[(int64_t)blockIdx.z * p.partials + i];
+  for (int o = 16; o; o /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = sum;
+  __syncthreads();
+  sum = 0;
+  for (int w = 0; w < 8; ++w) sum += part[w];
+  const double scale = p.scale / (sqrt(sum) + p.eps);
+  const bool zero = sum == 0 && p.eps == 0;             // 0 / 0: a zero matrix stays zero
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const bool across = p.g_sr < p.g_sc;
+  const int r0 = blockIdx.y * 32, c0 = blockIdx.x * 32;
+  for (int i = warp; i < 32; i += 8) {
+    const int r = r0 + (across ? lane : i), c = c0 + (across ? i : lane);
+    if (r < p.rows && c < p.cols)
+      v[r - r0][c - c0] =
+          zero ? 0.f : (float)(load_value(p.g, p.dtype, blockIdx.z * p.g_sb + r * p.g_sr + c * p.g_sc) * scale);
+  }
+  __syncthreads();
+  for (int i = warp; i < 32; i += 8)
+    if (r0 + i < p.rows && c0 + lane < p.cols) {
+      __half high, low;
+      slice(v[i][lane], high, low);
+      *p.x.at(0, blockIdx.z, r0 + i, c0 + lane) = high;
+      *p.x.at(1, blockIdx.z, r0 + i, c0 + lane) = low;
+    }
 }
 
-// out = alpha * D + beta * (a b), a (ni, nq) and b (nq, nj) by their strides.
-struct ProductParams {
-  const float *a, *b, *d;
-  void *out;
-  float alpha, beta;
-  int64_t ni, nj, nq;
-  int64_t a_sb, a_i, a_q, b_sb, b_q, b_j, d_sb, o_sb, o_i, o_j;
+struct StepParams {
+  uint32_t idesc;
+  int batch, rows, cols, k;         // of the result; terms of the contraction
+  int row_tiles, column_tiles, tiles;   // tiles of one member
+  int in_planes, out_planes;
+  float alpha, beta;                // result = alpha * in + beta * accumulator
+  Planes in, out;
+  // the last step's result instead of `out`: element (z, r, c) of the type
+  void *last;
+  int last_dtype;
+  int64_t last_sb, last_sr, last_sc;
 };
 
-template <typename O> __device__ __forceinline__ void put(void *p, int64_t i, float v) {
-  if constexpr (sizeof(O) == 4) static_cast<float *>(p)[i] = v;
-  else if constexpr (__is_same(O, __half)) static_cast<__half *>(p)[i] = __float2half_rn(v);
-  else static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(v);
-}
-
-template <typename O> __global__ void __launch_bounds__(256) product_kernel(const ProductParams p) {
-  __shared__ float sa[kStep][kTile + 1], sb[kStep][kTile + 1];
-  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  const int64_t i0 = (int64_t)blockIdx.y * kTile, j0 = (int64_t)blockIdx.x * kTile;
-  const float *a = p.a + blockIdx.z * p.a_sb, *b = p.b + blockIdx.z * p.b_sb;
-  float acc[4][4] = {};
-  for (int64_t q0 = 0; q0 < p.nq; q0 += kStep) {
-    for (int v = threadIdx.x; v < kStep * kTile; v += 256) {
-      const int q = v / kTile, i = v % kTile;
-      const bool in = q0 + q < p.nq;
-      sa[q][i] = in && i0 + i < p.ni ? a[(i0 + i) * p.a_i + (q0 + q) * p.a_q] : 0.f;
-      sb[q][i] = in && j0 + i < p.nj ? b[(q0 + q) * p.b_q + (j0 + i) * p.b_j] : 0.f;
-    }
-    __syncthreads();
+// 32 rows x 32 fp16 columns at src, each lane its own row (4 pieces of 8
+// columns), read 64 bytes of a row at a time through the warp's staging.
+__device__ __forceinline__ void load_chunk(unsigned char *mine, const __half *src, int64_t ld, int rows,
+                                           int cols, uint4 (&v)[4]) {
+  const int lane = threadIdx.x % 32;
+  uint4 got[4];
 #pragma unroll
-    for (int q = 0; q < kStep; ++q)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] += sa[q][ty * 4 + i] * sb[q][tx * 4 + j];
-    __syncthreads();
+  for (int i = 0; i < 4; ++i) {
+    const int r = i * 8 + lane / 4, u = lane % 4;
+    got[i] = r < rows && u * 8 < cols ? *reinterpret_cast<const uint4 *>(src + r * ld + u * 8)
+                                      : make_uint4(0, 0, 0, 0);
   }
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int64_t r = i0 + ty * 4 + i, c = j0 + tx * 4 + j;
-      if (r >= p.ni || c >= p.nj) continue;
-      float v = p.beta * acc[i][j];
-      if (p.d) v += p.alpha * p.d[blockIdx.z * p.d_sb + r * p.nj + c];
-      put<O>(p.out, blockIdx.z * p.o_sb + r * p.o_i + c * p.o_j, v);
+  auto slot = [&](int r, int u) {
+    return reinterpret_cast<uint4 *>(mine + r * 64 + ((u ^ ((r >> 1) & 3)) << 4));
+  };
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) *slot(i * 8 + lane / 4, lane % 4) = got[i];
+  __syncwarp();
+#pragma unroll
+  for (int u = 0; u < 4; ++u) v[u] = *slot(lane, u);
+}
+
+// The way back, from each lane's row.
+__device__ __forceinline__ void store_chunk(unsigned char *mine, __half *dst, int64_t ld, int rows, int cols,
+                                            const uint4 (&v)[4]) {
+  const int lane = threadIdx.x % 32;
+  auto slot = [&](int r, int u) {
+    return reinterpret_cast<uint4 *>(mine + r * 64 + ((u ^ ((r >> 1) & 3)) << 4));
+  };
+  __syncwarp();
+#pragma unroll
+  for (int u = 0; u < 4; ++u) *slot(lane, u) = v[u];
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = i * 8 + lane / 4, u = lane % 4;
+    if (r < rows && u * 8 < cols) *reinterpret_cast<uint4 *>(dst + r * ld + u * 8) = *slot(r, u);
+  }
+}
+
+__device__ __forceinline__ const __half *halves(const uint4 (&v)[4]) {
+  return reinterpret_cast<const __half *>(&v[0]);
+}
+
+// alpha * in + beta * accumulator for 32 columns of the lane's row.
+template <class Source>
+__device__ __forceinline__ void combine(const StepParams &p, const Source &source, int c, unsigned char *mine,
+                                        int z, int row, int column, int rows, int cols, float (&v)[32]) {
+  float acc[16];
+#pragma unroll
+  for (int h = 0; h < 32; h += 16) {
+    source.read(c + h, acc);
+#pragma unroll
+    for (int x = 0; x < 16; ++x) v[h + x] = p.beta * acc[x];
+  }
+  for (int q = 0; q < p.in_planes; ++q) {
+    uint4 in[4];
+    load_chunk(mine, p.in.at(q, z, row, column), p.in.ld, rows, cols, in);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const __half2 *h = reinterpret_cast<const __half2 *>(&in[u]);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const float2 f = __half22float2(h[x]);
+        v[u * 8 + x * 2] += p.alpha * f.x;
+        v[u * 8 + x * 2 + 1] += p.alpha * f.y;
+      }
     }
+  }
 }
 
-template <typename O> int product(const ProductParams &p, int64_t batch, cudaStream_t st) {
-  const dim3 grid((unsigned)((p.nj + kTile - 1) / kTile), (unsigned)((p.ni + kTile - 1) / kTile),
-                  (unsigned)batch);
-  count_launch();
-  product_kernel<O><<<grid, 256, 0, st>>>(p);
-  return check_cuda(cudaGetLastError(), "product_kernel launch");
+__device__ __forceinline__ void slices_of(const float (&v)[32], uint4 (&high)[4], uint4 (&low)[4]) {
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const float a = v[u * 8 + x * 2], b = v[u * 8 + x * 2 + 1];
+      const __half2 hh = __floats2half2_rn(a, b);
+      const float2 f = __half22float2(hh);
+      h[x] = *reinterpret_cast<const uint32_t *>(&hh);
+      l[x] = pack2<__half>(a - f.x, b - f.y);
+    }
+    high[u] = make_uint4(h[0], h[1], h[2], h[3]);
+    low[u] = make_uint4(l[0], l[1], l[2], l[3]);
+  }
 }
 
-template <typename T>
-int run(const void *g, int64_t batch, int64_t m, int64_t n, int64_t g_sb, int64_t g_sr,
-        int64_t g_sc, int steps, const double *coefficients, double eps, void *out, void *workspace,
-        cudaStream_t st) {
-  const bool tall = m > n;
-  const int64_t rows = tall ? n : m, cols = tall ? m : n;
-  double *partial = static_cast<double *>(workspace);
-  float *x0 = reinterpret_cast<float *>(partial + batch * kNormBlocks);
-  float *x1 = x0 + batch * rows * cols, *s = x1 + batch * rows * cols, *q = s + batch * rows * rows;
-  const InitParams ip{g, rows, cols, g_sb, tall ? g_sc : g_sr, tall ? g_sr : g_sc, partial, x0, eps};
+struct StepTile { int z, row, column; bool mirror; };
+
+// S = X X^T (in_planes 0) and P = b S + c S S: tiles (i, j) on and below the
+// diagonal, the others their mirror images.
+template <int PAIR_, int NT_, int PLANES_> struct SymmetricJob {
+  static constexpr int PAIR = PAIR_, NT = NT_, PLANES = PLANES_, PASS = 0;
+  static constexpr bool AMN = false, BMN = false, RAGGED = false;
+  static constexpr int R = kRows * PAIR / NT;           // column tiles as wide as a tile is high
+  using Params = StepParams;
+  using Extra = StepTile;
+  static __device__ int plane_stride(const Params &p) { return p.batch; }
+  struct Walk {
+    __device__ Walk(const Params &) {}
+    __device__ bool find(const Params &p, int t, TileOf<Extra> &tile) {
+      const int z = t / p.tiles, local = t - z * p.tiles;
+      if (z >= p.batch) return false;
+      // rows of tiles 0 .. i-1 hold R i (i + 1) / 2 tiles
+      int i = (int)((sqrtf(8.f * (float)(local / R) + 1.f) - 1.f) * 0.5f);
+      while (R * (i + 1) * (i + 2) / 2 <= local) ++i;
+      while (R * i * (i + 1) / 2 > local) --i;
+      const int j = local - R * i * (i + 1) / 2;
+      tile.a_row = i * kRows * PAIR;
+      tile.b_row = j * NT;
+      tile.a_mat = tile.b_mat = z;
+      tile.k_begin = 0;
+      tile.k_len = p.k;
+      tile.extra = StepTile{z, tile.a_row, tile.b_row, j < R * i};
+      return true;
+    }
+  };
+  template <class Source>
+  static __device__ void epilogue(const Params &p, const TileOf<Extra> &t, const Source &source, int row,
+                                  int column, unsigned char *mine) {
+    const int r0 = t.extra.row + row, rows = p.rows - r0, lane = threadIdx.x % 32;
+    if (rows <= 0) return;
+#pragma unroll
+    for (int c = 0; c < NT / 2; c += 32) {
+      const int c0 = t.extra.column + column + c, cols = p.cols - c0;
+      if (cols <= 0) continue;
+      float v[32];
+      combine(p, source, c, mine, t.extra.z, r0, c0, rows, cols, v);
+      uint4 high[4], low[4];
+      slices_of(v, high, low);
+      store_chunk(mine, p.out.at(0, t.extra.z, r0, c0), p.out.ld, rows, cols, high);
+      if constexpr (PLANES == 2)
+        store_chunk(mine, p.out.at(1, t.extra.z, r0, c0), p.out.ld, rows, cols, low);
+      if (t.extra.mirror && lane < rows) {
+        __half *h = p.out.at(0, t.extra.z, c0, r0 + lane), *l = h + p.out.plane;
+#pragma unroll
+        for (int x = 0; x < 32; ++x)
+          if (x < cols) {
+            h[x * p.out.ld] = halves(high)[x];
+            if constexpr (PLANES == 2) l[x * p.out.ld] = halves(low)[x];
+          }
+      }
+    }
+  }
+  static __device__ void finish(const Params &, int, int) {}
+};
+
+// X <- a X + P X: A is the rows of P, B the columns of X.
+template <int PAIR_, int NT_, int PLANES_> struct UpdateJob {
+  static constexpr int PAIR = PAIR_, NT = NT_, PLANES = PLANES_, PASS = 0;
+  static constexpr bool AMN = false, BMN = true, RAGGED = false;
+  using Params = StepParams;
+  using Extra = StepTile;
+  static __device__ int plane_stride(const Params &p) { return p.batch; }
+  struct Walk {
+    __device__ Walk(const Params &) {}
+    __device__ bool find(const Params &p, int t, TileOf<Extra> &tile) {
+      const int z = t / p.tiles, local = t - z * p.tiles;
+      if (z >= p.batch) return false;
+      const int sweep = local / (8 * p.column_tiles), in = local - sweep * 8 * p.column_tiles;
+      const int size = min(p.row_tiles - sweep * 8, 8);
+      tile.a_row = (sweep * 8 + in % size) * kRows * PAIR;
+      tile.b_row = in / size * NT;
+      tile.a_mat = tile.b_mat = z;
+      tile.k_begin = 0;
+      tile.k_len = p.k;
+      tile.extra = StepTile{z, tile.a_row, tile.b_row, false};
+      return true;
+    }
+  };
+  template <class Source>
+  static __device__ void epilogue(const Params &p, const TileOf<Extra> &t, const Source &source, int row,
+                                  int column, unsigned char *mine) {
+    const int r0 = t.extra.row + row, rows = p.rows - r0, lane = threadIdx.x % 32;
+    if (rows <= 0) return;
+#pragma unroll
+    for (int c = 0; c < NT / 2; c += 32) {
+      const int c0 = t.extra.column + column + c, cols = p.cols - c0;
+      if (cols <= 0) continue;
+      float v[32];
+      combine(p, source, c, mine, t.extra.z, r0, c0, rows, cols, v);
+      if (!p.last) {
+        uint4 high[4], low[4];
+        slices_of(v, high, low);
+        store_chunk(mine, p.out.at(0, t.extra.z, r0, c0), p.out.ld, rows, cols, high);
+        store_chunk(mine, p.out.at(1, t.extra.z, r0, c0), p.out.ld, rows, cols, low);
+      } else {
+        // the result: through the staging where it is stored along the rows,
+        // from the lanes where it is stored across them
+        const int64_t at = t.extra.z * p.last_sb + r0 * p.last_sr + c0 * p.last_sc;
+        float *out32 = static_cast<float *>(p.last) + at;
+        __half *out16 = static_cast<__half *>(p.last) + at;   // or bf16: 2 bytes either way
+        const bool wide = p.last_dtype == OZ_F32;
+        auto bits = [&](float f) {
+          return p.last_dtype == OZ_F16 ? __float2half_rn(f)
+                                        : __ushort_as_half(__bfloat16_as_ushort(__float2bfloat16_rn(f)));
+        };
+        if (p.last_sr == 1) {
+          if (lane < rows) {
+#pragma unroll
+            for (int x = 0; x < 32; ++x)
+              if (x < cols) {
+                if (wide) out32[lane + x * p.last_sc] = v[x];
+                else out16[lane + x * p.last_sc] = bits(v[x]);
+              }
+          }
+        } else {
+          __syncwarp();
+#pragma unroll
+          for (int u = 0; u < 8; ++u)
+            *staged(mine, lane, u) = *reinterpret_cast<const uint4 *>(&v[u * 4]);
+          __syncwarp();
+#pragma unroll 4
+          for (int r = 0; r < 32; ++r)
+            if (r < rows && lane < cols) {
+              const float f = reinterpret_cast<const float *>(staged(mine, r, lane / 4))[lane % 4];
+              if (wide) out32[r * p.last_sr + lane] = f;
+              else out16[r * p.last_sr + lane] = bits(f);
+            }
+        }
+      }
+    }
+  }
+  static __device__ void finish(const Params &, int, int) {}
+};
+
+int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
+int64_t pitch(int64_t n) { return (n + 7) / 8 * 8; }
+
+// Workspace of a call: sums of squares, two X's, S and P in slices.
+struct Layout {
+  int64_t rows, cols, x_mat, s_mat, x0, x1, s, p, total;
+};
+Layout layout(int64_t batch, int64_t m, int64_t n, int splits) {
+  Layout l{};
+  l.rows = m < n ? m : n;
+  l.cols = m < n ? n : m;
+  l.x_mat = l.rows * pitch(l.cols);
+  l.s_mat = l.rows * pitch(l.rows);
+  int64_t at = align256(batch * kMostPartials * 8);
+  const int64_t x = align256(2 * batch * l.x_mat * 2), s = align256(splits * batch * l.s_mat * 2);
+  l.x0 = at;
+  l.x1 = l.x0 + x;
+  l.s = l.x1 + x;
+  l.p = l.s + s;
+  l.total = l.p + s;
+  return l;
+}
+
+// The exponent that puts a bound on a matrix's entries at 2^15.
+int exponent(double bound) {
+  if (!(bound > 0)) return 15;
+  int e;
+  frexp(bound, &e);                                    // bound <= 2^e
+  return std::min(std::max(15 - e, -40), 40);
+}
+
+// Largest |a s + b s^3 + c s^5| for s in [0, most], and |b u + c u^2| for u = s^2.
+double largest_value(double a, double b, double c, double most) {
+  auto f = [&](double s) { return std::fabs(s * (a + s * s * (b + s * s * c))); };
+  double v = f(most);
+  const double disc = 9 * b * b - 20 * a * c;          // a + 3 b u + 5 c u^2 = 0
+  if (c != 0 && disc >= 0)
+    for (int sign = -1; sign <= 1; sign += 2) {
+      const double u = (-3 * b + sign * std::sqrt(disc)) / (10 * c);
+      if (u > 0 && u < most * most) v = std::max(v, f(std::sqrt(u)));
+    }
+  if (c == 0 && b != 0 && -a / (3 * b) > 0 && -a / (3 * b) < most * most)
+    v = std::max(v, f(std::sqrt(-a / (3 * b))));
+  return v;
+}
+double largest_poly(double b, double c, double most) {
+  auto f = [&](double u) { return std::fabs(u * (b + u * c)); };
+  const double end = most * most;
+  double v = f(end);
+  if (c != 0 && -b / (2 * c) > 0 && -b / (2 * c) < end) v = std::max(v, f(-b / (2 * c)));
+  return v;
+}
+
+// Tile counts of a member, and the estimated time of all tiles: waves over the
+// GPU times the bytes a CTA loads for each block, which is what bounds both
+// shapes (pairs of CTAs load 32 KB for 256 x 256, one CTA 24 KB for 128 x 64).
+int64_t member_tiles(bool symmetric, int64_t rows, int64_t cols, int high, int wide) {
+  const int64_t tm = (rows + high - 1) / high, tn = (cols + wide - 1) / wide, r = high / wide;
+  return symmetric ? r * tm * (tm + 1) / 2 - (r * tm - tn) : tm * tn;
+}
+bool use_pairs(bool symmetric, int64_t batch, int64_t rows, int64_t cols) {
+  const int64_t pairs = sm_count() / 2, singles = sm_count();
+  const int64_t two = batch * member_tiles(symmetric, rows, cols, 256, 256);
+  const int64_t one = batch * member_tiles(symmetric, rows, cols, 128, 64);
+  return 4 * ((two + pairs - 1) / pairs) <= 3 * ((one + singles - 1) / singles);
+}
+
+template <class J>
+int step_product(const CUtensorMap &a, const CUtensorMap &b, StepParams p, bool symmetric, cudaStream_t st) {
+  const int64_t tiles = member_tiles(symmetric, p.rows, p.cols, kRows * J::PAIR, J::NT);
+  if (tiles * p.batch > INT32_MAX / 2) return set_error(OZ_ERR_INVALID, "too many tiles");
+  p.row_tiles = (p.rows + kRows * J::PAIR - 1) / (kRows * J::PAIR);
+  p.column_tiles = (p.cols + J::NT - 1) / J::NT;
+  p.tiles = (int)tiles;
+  return launch<J>(a, b, p, tiles * p.batch, st, "newton step launch");
+}
+
+template <int SPLITS>
+int run(const InitParams &init, const Layout &l, int batch, int steps, const double *coefficients,
+        unsigned char *ws, StepParams last, cudaStream_t st) {
+  const int rows = (int)l.rows, cols = (int)l.cols;
+  const int64_t ldx = pitch(cols), lds = pitch(rows);
+  auto planes = [&](int64_t offset, int64_t ld, int64_t mat) {
+    return Planes{reinterpret_cast<__half *>(ws + offset), ld, mat, mat * batch};
+  };
+  Planes x[2] = {planes(l.x0, ldx, l.x_mat), planes(l.x1, ldx, l.x_mat)};
+  const Planes s = planes(l.s, lds, l.s_mat), q = planes(l.p, lds, l.s_mat);
+
   count_launch();
-  squares_kernel<T><<<dim3(kNormBlocks, (unsigned)batch), 256, 0, st>>>(ip);
+  squares_kernel<<<dim3((unsigned)init.partials, (unsigned)batch), 256, 0, st>>>(init);
   if (int rc = check_cuda(cudaGetLastError(), "squares_kernel launch")) return rc;
-  const int64_t blocks = (rows * cols + 255) / 256;
   count_launch();
-  normalise_kernel<T><<<dim3((unsigned)(blocks < 4096 ? blocks : 4096), (unsigned)batch), 256, 0, st>>>(ip);
+  normalise_kernel<<<dim3((unsigned)((cols + 31) / 32), (unsigned)((rows + 31) / 32), (unsigned)batch), 256, 0,
+                     st>>>(init);
   if (int rc = check_cuda(cudaGetLastError(), "normalise_kernel launch")) return rc;
-  const int64_t xs = rows * cols, ss = rows * rows;
+
+  const bool pair_s = use_pairs(true, batch, rows, rows), pair_x = use_pairs(false, batch, rows, cols);
+  // each matrix in the boxes its products read: 128 rows (A), the columns of a
+  // tile as rows (B of a symmetric product) or 64 rows across (B of the update)
+  auto map = [&](CUtensorMap *m, const Planes &v, int64_t inner, int count, int box) {
+    return make_map(m, v.base, inner, rows, (int64_t)batch * count, v.ld * 2, v.mat * 2, box);
+  };
+  CUtensorMap xa[2], xb[2], xu[2], sa, sb, pa;
+  for (int i = 0; i < 2; ++i) {
+    if (int rc = map(&xa[i], x[i], cols, 2, kRows)) return rc;
+    if (int rc = map(&xb[i], x[i], cols, 2, pair_s ? 128 : 64)) return rc;
+    if (int rc = map(&xu[i], x[i], cols, 2, kBlock)) return rc;
+  }
+  if (int rc = map(&sa, s, rows, SPLITS, kRows)) return rc;
+  if (int rc = map(&sb, s, rows, SPLITS, pair_s ? 128 : 64)) return rc;
+  if (int rc = map(&pa, q, rows, SPLITS, kRows)) return rc;
+
+  StepParams sym{};
+  sym.idesc = instruction(OZ_F16);
+  sym.batch = batch;
+  sym.rows = sym.cols = rows;
+  double most = 1 + 1e-6;                              // largest singular value of X
+  int ex = exponent(most), cur = 0;
   for (int i = 0; i < steps; ++i) {
-    const float a = (float)coefficients[3 * i], b = (float)coefficients[3 * i + 1],
-                c = (float)coefficients[3 * i + 2];
-    if (int rc = product<float>({x0, x0, nullptr, s, 0.f, 1.f, rows, rows, cols, xs, cols, 1, xs, 1,
-                                 cols, 0, ss, rows, 1}, batch, st)) return rc;
-    if (int rc = product<float>({s, s, s, q, b, c, rows, rows, rows, ss, rows, 1, ss, rows, 1, ss,
-                                 ss, rows, 1}, batch, st)) return rc;
-    const ProductParams last{q, x0, x0, i + 1 < steps ? (void *)x1 : out, a, 1.f, rows, cols, rows,
-                             ss, rows, 1, xs, cols, 1, xs, xs,
-                             i + 1 < steps || !tall ? cols : 1, i + 1 < steps || !tall ? 1 : rows};
-    if (int rc = i + 1 < steps ? product<float>(last, batch, st) : product<T>(last, batch, st))
-      return rc;
-    float *t = x0;
-    x0 = x1;
-    x1 = t;
+    const double a = coefficients[3 * i], b = coefficients[3 * i + 1], c = coefficients[3 * i + 2];
+    // rounded operands give a little more than the exact bounds
+    const double slack = 1 + 1.0 / 64;
+    const int es = exponent(most * most * slack), ep = exponent(largest_poly(b, c, most) * slack);
+    sym.k = cols;
+    sym.in_planes = 0;
+    sym.alpha = 0;
+    sym.beta = (float)std::ldexp(1.0, es - 2 * ex);
+    sym.out = s;
+    int rc = pair_s ? step_product<SymmetricJob<2, 256, SPLITS>>(xa[cur], xb[cur], sym, true, st)
+                    : step_product<SymmetricJob<1, 64, SPLITS>>(xa[cur], xb[cur], sym, true, st);
+    if (rc) return rc;
+    sym.k = rows;
+    sym.in_planes = SPLITS;
+    sym.in = s;
+    sym.alpha = (float)std::ldexp(b, ep - es);
+    sym.beta = (float)std::ldexp(c, ep - 2 * es);
+    sym.out = q;
+    rc = pair_s ? step_product<SymmetricJob<2, 256, SPLITS>>(sa, sb, sym, true, st)
+                : step_product<SymmetricJob<1, 64, SPLITS>>(sa, sb, sym, true, st);
+    if (rc) return rc;
+    most = std::min(largest_value(a, b, c, most) * slack, 1e15);
+    const bool end = i + 1 == steps;
+    const int en = end ? 0 : exponent(most);
+    StepParams up = last;
+    if (!end) up.last = nullptr;
+    up.idesc = sym.idesc;
+    up.batch = batch;
+    up.rows = rows;
+    up.cols = cols;
+    up.k = rows;
+    up.in_planes = 2;
+    up.in = x[cur];
+    up.out = x[cur ^ 1];
+    up.alpha = (float)std::ldexp(a, en - ex);
+    up.beta = (float)std::ldexp(1.0, en - ep - ex);
+    rc = pair_x ? step_product<UpdateJob<2, 256, SPLITS>>(pa, xu[cur], up, false, st)
+                : step_product<UpdateJob<1, 64, SPLITS>>(pa, xu[cur], up, false, st);
+    if (rc) return rc;
+    cur ^= 1;
+    ex = en;
   }
   return OZ_OK;
+}
+
+bool valid(int dtype, int64_t batch, int64_t m, int64_t n, int splits) {
+  return (dtype == OZ_F32 || dtype == OZ_F16 || dtype == OZ_BF16) && batch >= 0 && m >= 0 && n >= 0 &&
+         splits >= 1 && splits <= 2;
 }
 
 }  // namespace
@@ -154,12 +545,8 @@ int run(const void *g, int64_t batch, int64_t m, int64_t n, int64_t g_sb, int64_
 
 extern "C" int64_t oz_orthogonalize_workspace_bytes(int dtype, int64_t batch, int64_t m, int64_t n,
                                                     int32_t num_splits) {
-  using namespace oz;
-  if ((dtype != OZ_F32 && dtype != OZ_F16 && dtype != OZ_BF16) || batch < 0 || m < 0 || n < 0 ||
-      num_splits < 1 || num_splits > 2)
-    return OZ_ERR_INVALID;
-  const int64_t rows = m < n ? m : n, cols = m < n ? n : m;
-  return batch * (kNormBlocks * 8 + (2 * rows * cols + 2 * rows * rows) * 4);
+  if (!oz::valid(dtype, batch, m, n, num_splits)) return OZ_ERR_INVALID;
+  return oz::layout(batch, m, n, num_splits).total;
 }
 
 extern "C" int oz_orthogonalize(const void *g, int dtype, int64_t batch, int64_t m, int64_t n,
@@ -171,21 +558,35 @@ extern "C" int oz_orthogonalize(const void *g, int dtype, int64_t batch, int64_t
   if (dtype != OZ_F32 && dtype != OZ_F16 && dtype != OZ_BF16)
     return set_error(OZ_ERR_UNSUPPORTED, "unsupported dtype %d (fp32, fp16 or bf16)", dtype);
   if (batch < 0 || m < 0 || n < 0) return set_error(OZ_ERR_INVALID, "negative size");
-  if (m > (1 << 30) || n > (1 << 30) || batch > 65535)
+  if (m > (1 << 20) || n > (1 << 20) || batch > 65535)
     return set_error(OZ_ERR_INVALID, "size out of range");
   if (steps < 1 || !coefficients) return set_error(OZ_ERR_INVALID, "at least one step is needed");
   if (!(eps >= 0)) return set_error(OZ_ERR_INVALID, "eps must not be negative");
   if (num_splits < 1 || num_splits > 2)
     return set_error(OZ_ERR_INVALID, "num_splits must be 1 or 2, got %d", num_splits);
+  for (int i = 0; i < 3 * steps; ++i)
+    if (!std::isfinite(coefficients[i])) return set_error(OZ_ERR_INVALID, "coefficients must be finite");
   if (batch == 0 || m == 0 || n == 0) return OZ_OK;
   if (!g || !out) return set_error(OZ_ERR_INVALID, "null pointer");
-  const int64_t need = oz_orthogonalize_workspace_bytes(dtype, batch, m, n, num_splits);
-  if (!workspace || workspace_bytes < need || (uintptr_t)workspace % 256 != 0)
+  const Layout l = layout(batch, m, n, num_splits);
+  if (!workspace || workspace_bytes < l.total || (uintptr_t)workspace % 256 != 0)
     return set_error(OZ_ERR_INVALID,
                      "workspace of %lld bytes (256-byte aligned) needed, got %lld at %p",
-                     (long long)need, (long long)workspace_bytes, workspace);
+                     (long long)l.total, (long long)workspace_bytes, workspace);
+  unsigned char *ws = static_cast<unsigned char *>(workspace);
+  const bool tall = m > n;
+  const int64_t blocks = (l.rows * l.cols + 4095) / 4096;
+  InitParams init{g, dtype, (int)std::min<int64_t>(blocks, kMostPartials), (int)l.rows, (int)l.cols, g_sb,
+                  tall ? g_sc : g_sr, tall ? g_sr : g_sc, reinterpret_cast<double *>(ws),
+                  Planes{reinterpret_cast<__half *>(ws + l.x0), pitch(l.cols), l.x_mat, l.x_mat * batch}, eps,
+                  std::ldexp(1.0, exponent(1 + 1e-6))};
+  StepParams last{};
+  last.last = out;
+  last.last_dtype = dtype;
+  last.last_sb = m * n;
+  last.last_sr = tall ? 1 : n;
+  last.last_sc = tall ? n : 1;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (dtype == OZ_F32) return run<float>(g, batch, m, n, g_sb, g_sr, g_sc, steps, coefficients, eps, out, workspace, st);
-  if (dtype == OZ_F16) return run<__half>(g, batch, m, n, g_sb, g_sr, g_sc, steps, coefficients, eps, out, workspace, st);
-  return run<__nv_bfloat16>(g, batch, m, n, g_sb, g_sr, g_sc, steps, coefficients, eps, out, workspace, st);
+  return num_splits == 1 ? run<1>(init, l, (int)batch, steps, coefficients, ws, last, st)
+                         : run<2>(init, l, (int)batch, steps, coefficients, ws, last, st);
 }
