@@ -237,7 +237,7 @@ struct StepTile { int z, row, column; bool mirror; };
 // S = X X^T (in_planes 0) and P = b S + c S S: tiles (i, j) on and below the
 // diagonal, the others their mirror images.
 template <int PAIR_, int NT_, int PLANES_> struct SymmetricJob {
-  static constexpr int PAIR = PAIR_, NT = NT_, PLANES = PLANES_, PASS = 0;
+  static constexpr int PAIR = PAIR_, NT = NT_, PLANES = PLANES_, PASS = (PLANES_ - 1) * 4;
   static constexpr bool AMN = false, BMN = false, RAGGED = false;
   static constexpr int R = kRows * PAIR / NT;           // column tiles as wide as a tile is high
   using Params = StepParams;
@@ -294,7 +294,7 @@ template <int PAIR_, int NT_, int PLANES_> struct SymmetricJob {
 
 // X <- a X + P X: A is the rows of P, B the columns of X.
 template <int PAIR_, int NT_, int PLANES_> struct UpdateJob {
-  static constexpr int PAIR = PAIR_, NT = NT_, PLANES = PLANES_, PASS = 0;
+  static constexpr int PAIR = PAIR_, NT = NT_, PLANES = PLANES_, PASS = (PLANES_ - 1) * 4;
   static constexpr bool AMN = false, BMN = true, RAGGED = false;
   using Params = StepParams;
   using Extra = StepTile;

@@ -236,6 +236,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   else __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  // up to here nothing depends on earlier kernels: the next launch may do as
+  // much while this one runs, and this one waits here for what came before
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 
   auto leader_addr = [&](uint64_t *bar) -> uint32_t {
     if constexpr (PAIR == 2) return map_to_cta(smem_u32(bar), 0);
@@ -341,7 +345,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint64_t ad = a_desc + slot * (SB >> 4), bd = b_desc + slot * (SB >> 4);
 #pragma unroll
       for (int q = 0; q < (J::PLANES == 2 ? 3 : 1); ++q) {
-        const uint64_t aq = ad + (q == 2 ? a_bytes<J>() >> 4 : 0);
+        // the small products first: what the sum cuts off is relative to its size
+        const uint64_t aq = ad + (J::PLANES == 2 && q == 0 ? a_bytes<J>() >> 4 : 0);
         const uint64_t bq = bd + (q == 1 ? b_bytes<J>() >> 4 : 0);
 #pragma unroll
         for (int kk = 0; kk < kBlock / 16; ++kk) {
@@ -521,13 +526,15 @@ int launch(const CUtensorMap &a, const CUtensorMap &b, const typename J::Params 
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = J::PAIR;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   count_launch();
   return check_cuda(cudaLaunchKernelEx(&cfg, kernel, a, b, p), what);
 }
