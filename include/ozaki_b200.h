@@ -289,8 +289,9 @@ int oz_grouped_wgrad(const void *x, const void *dy, const void *offsets, int off
  *   zeros     : uint8 with the scales' strides, or NULL: z = 8
  *   offsets   : row groups of the experts as in oz_grouped_matmul, or NULL
  *               for one expert with every row
- * group is a multiple of 32 that divides k.  y: (rows, n), row pitch ldy, of
- * x's type or fp32.
+ * group is a multiple of 32 that divides k.  x and packed start on 16-byte
+ * boundaries and their row pitches are multiples of 16 bytes.  y: (rows, n),
+ * row pitch ldy, of x's type or fp32.
  */
 int oz_matmul_w4(const void *x, const void *packed, const void *scales, const void *zeros,
                  const void *offsets, int offsets_64, int dtype, int scale_dtype, int out_dtype,

@@ -64,7 +64,7 @@ extern "C" int oz_device_status(void *stream, int32_t *code) {
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (int rc = check_cuda(cudaStreamSynchronize(st), "cudaStreamSynchronize")) return rc;
   int v = 0;
-  for (auto unit : {status_split, status_gemm, status_experts, status_newton}) {
+  for (auto unit : {status_split, status_gemm, status_experts, status_newton, status_w4}) {
     int u = 0;
     if (int rc = unit(&u, true)) return rc;
     if (!v) v = u;

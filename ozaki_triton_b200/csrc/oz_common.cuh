@@ -60,6 +60,7 @@ int status_split(int *value, bool clear);
 int status_gemm(int *value, bool clear);
 int status_experts(int *value, bool clear);
 int status_newton(int *value, bool clear);
+int status_w4(int *value, bool clear);
 
 // Split of both operands of a product in one launch (oz_split.cu): A's rows
 // (a_sm, a_sk: line and k strides) and B's columns (b_sn, b_sk), each into

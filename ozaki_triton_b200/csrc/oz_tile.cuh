@@ -72,30 +72,37 @@ template <class Extra> struct TileOf {
   Extra extra;
 };
 
-// 3-D operand map: `inner` contiguous elements, `rows` of them `row_bytes`
-// apart, `mats` of those `mat_bytes` apart; boxes of 64 x box_rows.
-inline int make_map(CUtensorMap *map, const void *base, int64_t inner, int64_t rows, int64_t mats,
-                    int64_t row_bytes, int64_t mat_bytes, int box_rows) {
-  static PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
-  if (!encode) {
+// 3-D tensor map: `inner` contiguous elements, `rows` of them `row_bytes`
+// apart, `mats` of those `mat_bytes` apart, and the box of a copy.
+inline int encode(CUtensorMap *map, CUtensorMapDataType type, const void *base, int64_t inner, int64_t rows,
+                  int64_t mats, int64_t row_bytes, int64_t mat_bytes, int box_inner, int box_rows, int box_mats,
+                  CUtensorMapSwizzle swizzle) {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  if (!fn) {
     void *ptr = nullptr;
     cudaDriverEntryPointQueryResult q;
     if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &ptr, 12000, cudaEnableDefault,
                                          &q) != cudaSuccess ||
         q != cudaDriverEntryPointSuccess)
       return set_error(OZ_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
-    encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+    fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
   }
   cuuint64_t dims[3] = {(cuuint64_t)inner, (cuuint64_t)rows, (cuuint64_t)mats};
   cuuint64_t strides[2] = {(cuuint64_t)row_bytes, (cuuint64_t)mat_bytes};
-  cuuint32_t box[3] = {kBlock, (cuuint32_t)box_rows, 1};
+  cuuint32_t box[3] = {(cuuint32_t)box_inner, (cuuint32_t)box_rows, (cuuint32_t)box_mats};
   cuuint32_t steps[3] = {1, 1, 1};
-  const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void *>(base), dims,
-                            strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const CUresult r = fn(map, type, 3, const_cast<void *>(base), dims, strides, box, steps,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return set_error(OZ_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
   return OZ_OK;
+}
+
+// A 16-bit operand of the engine: boxes of 64 elements x box_rows, swizzled.
+inline int make_map(CUtensorMap *map, const void *base, int64_t inner, int64_t rows, int64_t mats,
+                    int64_t row_bytes, int64_t mat_bytes, int box_rows) {
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, base, inner, rows, mats, row_bytes, mat_bytes, kBlock,
+                box_rows, 1, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 inline int sm_count() {

@@ -242,8 +242,10 @@ def matmul_w4(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor,
     if offsets is not None:
         _check_offsets(offsets, experts)
     _check_places(x, packed, scales, zeros, offsets)
-    x = x if x.stride(1) == 1 else x.contiguous()
+    x = _as_operand(x)
     packed, scales = packed.contiguous(), scales.contiguous()
+    if packed.data_ptr() % 16:
+        packed = packed.clone()
     zeros = zeros.contiguous() if zeros is not None else None
     y = torch.empty((rows, n), dtype=out_dtype, device=x.device)
     with torch.cuda.device(x.device):
