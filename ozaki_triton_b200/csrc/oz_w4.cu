@@ -41,12 +41,6 @@ struct W4Params {
   int column_tiles;
 };
 
-__device__ __forceinline__ float load_scale(const void *s, int dtype, int64_t i) {
-  if (dtype == OZ_F32) return __ldg(static_cast<const float *>(s) + i);
-  if (dtype == OZ_F16) return __half2float(__ldg(static_cast<const __half *>(s) + i));
-  return __bfloat162float(__ldg(static_cast<const __nv_bfloat16 *>(s) + i));
-}
-
 // Rows of expert e, clamped to the tensor; without offsets every row.
 __device__ __forceinline__ void expert_rows(const W4Params &p, int e, int &begin, int &end) {
   if (!p.offsets) {
@@ -97,39 +91,57 @@ struct W4Walk {
   }
 };
 
-// Two 16-bit values q - z from bits [SHIFT, SHIFT + 4) of both halves of a
-// word: as 1024 + q (fp16) or 128 + q (bf16), less the same with z.
+// Four pairs of 16-bit values q - z from a word's eight fields (bits 0-3 and
+// 16-19 first), exactly: a field becomes the low mantissa bits of a constant
+// that is a power of two, and the same constant plus z is subtracted.  fp16
+// has room for a field in bits 4-7 too (64 + q beside 1024 + q), bf16 has not.
 template <typename T> struct Unpack;
 template <> struct Unpack<__half> {
-  static __device__ __forceinline__ uint32_t zero(int z) { return 0x64006400u | (uint32_t)(z * 0x10001); }
-  static __device__ __forceinline__ uint32_t value(uint32_t w, uint32_t z) {
-    const uint32_t v = (w & 0x000f000fu) | 0x64006400u;
+  static __device__ __forceinline__ uint2 zero(uint32_t z) {
+    z *= 0x10001u;
+    return make_uint2(0x64006400u | z, 0x54005400u | z << 4);
+  }
+  static __device__ __forceinline__ uint32_t less(uint32_t v, uint32_t z) {
     const __half2 d = __hsub2(*reinterpret_cast<const __half2 *>(&v), *reinterpret_cast<const __half2 *>(&z));
     return *reinterpret_cast<const uint32_t *>(&d);
   }
+  static __device__ __forceinline__ void values(uint32_t w, uint2 z, uint32_t (&v)[4]) {
+    v[0] = less((w & 0x000f000fu) | 0x64006400u, z.x);
+    v[1] = less((w & 0x00f000f0u) | 0x54005400u, z.y);
+    w >>= 8;
+    v[2] = less((w & 0x000f000fu) | 0x64006400u, z.x);
+    v[3] = less((w & 0x00f000f0u) | 0x54005400u, z.y);
+  }
 };
 template <> struct Unpack<__nv_bfloat16> {
-  static __device__ __forceinline__ uint32_t zero(int z) { return 0x43004300u | (uint32_t)(z * 0x10001); }
-  static __device__ __forceinline__ uint32_t value(uint32_t w, uint32_t z) {
-    const uint32_t v = (w & 0x000f000fu) | 0x43004300u;
-    const __nv_bfloat162 d =
-        __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&v), *reinterpret_cast<const __nv_bfloat162 *>(&z));
-    return *reinterpret_cast<const uint32_t *>(&d);
+  static __device__ __forceinline__ uint2 zero(uint32_t z) {
+    return make_uint2(0x43004300u | z * 0x10001u, 0);
+  }
+  static __device__ __forceinline__ void values(uint32_t w, uint2 z, uint32_t (&v)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t u = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+      const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&u),
+                                       *reinterpret_cast<const __nv_bfloat162 *>(&z.x));
+      v[i] = *reinterpret_cast<const uint32_t *>(&d);
+    }
   }
 };
 
+// d = c + a b, 16 weight rows x 16 k by 8 rows of x
 template <typename T>
-__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                    uint32_t b1, float c0, float c1, float c2, float c3) {
   if constexpr (__is_same(T, __half))
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
-                 "{%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+                 "{%8, %9}, {%10, %11, %12, %13};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
   else
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
-                 "{%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+                 "{%8, %9}, {%10, %11, %12, %13};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
 
 __device__ __forceinline__ void put(const W4Params &p, int64_t i, float v) {
@@ -138,31 +150,36 @@ __device__ __forceinline__ void put(const W4Params &p, int64_t i, float v) {
   else static_cast<__nv_bfloat16 *>(p.y)[i] = __float2bfloat16_rn(v);
 }
 
-template <int RT, int NB> struct W4Shape {
+template <int RT, int NB, bool WHOLE> struct W4Shape {
   static constexpr int kRows = 16 * RT;                    // weight rows of a tile
   static constexpr int kWeights = kRows * kChunk / 2;      // bytes of a chunk
   static constexpr int kX = 8 * NB * kChunk * 2;
   static constexpr int kStage = kWeights + kX;
   static constexpr int kSums = kRows * 8 * NB * 4;         // of a warp
-  static constexpr int kBytes = 512 + kWarps * (kDepth * kStage + kSums) + kWarps * kDepth * 8 + 16;
+  static constexpr int kEntries = kRows * (WHOLE ? 1 : 4); // scales of a chunk
+  static constexpr int kWarpBytes = kDepth * kStage + kEntries * 16 + kSums;
+  static constexpr int kBytes = 512 + kWarps * kWarpBytes + kWarps * kDepth * 8 + 16;
+  static constexpr int kCtas = 2 * (kBytes + 1024) <= 228 * 1024 ? 2 : 1;
 };
 
 // RT: 16-row blocks of weights of a tile; NB: 8-row blocks of x.
-// WHOLE: a group covers whole chunks (g a multiple of 128), one scale a chunk.
+// WHOLE: a group covers whole chunks (g a multiple of 128), one scale a chunk
+// and row; otherwise one for every 32 k.
 template <typename T, int RT, int NB, bool WHOLE>
-__global__ void __launch_bounds__(kWarps * 32, RT * NB >= 8 ? 1 : 2)
+__global__ void __launch_bounds__(kWarps * 32, (W4Shape<RT, NB, WHOLE>::kCtas))
     w4_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
               const W4Params p) {
-  using Shape = W4Shape<RT, NB>;
+  using Shape = W4Shape<RT, NB, WHOLE>;
+  static_assert(kDepth == 2, "the scales of a chunk are loaded two chunks ahead");
   extern __shared__ unsigned char raw[];
   unsigned char *smem = raw + ((512 - (smem_u32(raw) & 511)) & 511);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
   unsigned char *ring = smem + warp * kDepth * Shape::kStage;
-  float *sums = reinterpret_cast<float *>(smem + kWarps * kDepth * Shape::kStage);
-  uint64_t *full = reinterpret_cast<uint64_t *>(sums + kWarps * Shape::kSums / 4) + warp * kDepth;
-  volatile int *abort_flag =
-      reinterpret_cast<volatile int *>(reinterpret_cast<uint64_t *>(sums + kWarps * Shape::kSums / 4) +
-                                       kWarps * kDepth);
+  uint4 *entries = reinterpret_cast<uint4 *>(smem + kWarps * kDepth * Shape::kStage) + warp * Shape::kEntries;
+  float *sums = reinterpret_cast<float *>(smem + kWarps * (kDepth * Shape::kStage + Shape::kEntries * 16));
+  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + kWarps * Shape::kWarpBytes);
+  uint64_t *full = bars + warp * kDepth;
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(bars + kWarps * kDepth);
   if (threadIdx.x == 0) *abort_flag = 0;
   if (lane == 0)
     for (int i = 0; i < kDepth; ++i) mbar_init(&full[i], 1);
@@ -179,31 +196,62 @@ __global__ void __launch_bounds__(kWarps * 32, RT * NB >= 8 ? 1 : 2)
   const int unit = blockIdx.x * teams + team, units = gridDim.x * teams;
   const int chunks = (p.k + kChunk - 1) / kChunk;
 
-  // this warp's chunks of this team's tiles, in order: what is copied (ahead)
-  // and what is multiplied walk the same sequence
+  // This warp's chunks of this team's tiles, in order; what is copied runs two
+  // chunks ahead of what is multiplied.  A chunk's scales and zeros are loaded
+  // into registers with its copy and put into shared memory, ready for use, a
+  // chunk later (when the chunk before it has been multiplied).
+  constexpr int kMine = (Shape::kEntries + 31) / 32;
   W4Walk ahead;
   int a_tile = unit, a_chunk = member, a_e = 0, a_row = 0, a_rows = 0, a_column = 0;
   bool a_more = ahead.find(p, 8 * NB, a_tile, a_e, a_row, a_rows, a_column);
   uint32_t issued = 0;
+  uint32_t scale_bits[kMine], zero_bits[kMine];
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) scale_bits[i] = zero_bits[i] = 0;
   auto issue = [&]() {
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const uint32_t bits = scale_bits[i];
+      const float f = p.scale_dtype == OZ_F32 ? __uint_as_float(bits)
+                      : p.scale_dtype == OZ_BF16 ? __uint_as_float(bits << 16)
+                                                 : __half2float(__ushort_as_half((unsigned short)bits));
+      const uint2 z = Unpack<T>::zero(zero_bits[i]);
+      if (Shape::kEntries >= 32 || lane < Shape::kEntries)
+        entries[i * 32 + lane] = make_uint4(__float_as_uint(f), z.x, z.y, 0);
+    }
     while (a_more && a_chunk >= chunks) {
       a_tile += units;
       a_chunk = member;
       a_more = ahead.find(p, 8 * NB, a_tile, a_e, a_row, a_rows, a_column);
     }
-    if (!a_more) return;
-    if (lane == 0) {
-      unsigned char *st = ring + issued % kDepth * Shape::kStage;
-      uint64_t *bar = &full[issued % kDepth];
-      mbar_arrive_expect_tx(bar, Shape::kStage);
-      tma_load_3d(st, &tm_w, bar, a_chunk * (kChunk / 2), a_column * Shape::kRows, a_e);
-      tma_load_3d(st + Shape::kWeights, &tm_x, bar, 0, a_row, a_chunk * (kChunk / 32));
+    if (a_more) {
+      if (lane == 0) {
+        unsigned char *st = ring + (issued & 1) * Shape::kStage;
+        uint64_t *bar = &full[issued & 1];
+        mbar_arrive_expect_tx(bar, Shape::kStage);
+        tma_load_3d(st, &tm_w, bar, a_chunk * (kChunk / 2), a_column * Shape::kRows, a_e);
+        tma_load_3d(st + Shape::kWeights, &tm_x, bar, 0, a_row, a_chunk * (kChunk / 32));
+      }
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        const int entry = i * 32 + lane, n = a_column * Shape::kRows + entry % Shape::kRows;
+        const int group = (a_chunk * kChunk + entry / Shape::kRows * 32) / p.group;
+        scale_bits[i] = 0;
+        zero_bits[i] = 8;
+        if (n < p.n && group < p.groups && (Shape::kEntries >= 32 || lane < Shape::kEntries)) {
+          const int64_t at = a_e * p.s_se + n * p.s_sn + group;
+          if (p.scale_dtype == OZ_F32) scale_bits[i] = __ldg(static_cast<const uint32_t *>(p.scales) + at);
+          else scale_bits[i] = __ldg(static_cast<const unsigned short *>(p.scales) + at);
+          if (p.zeros) zero_bits[i] = __ldg(p.zeros + at);
+        }
+      }
+      a_chunk += p.along;
+      ++issued;
     }
-    a_chunk += p.along;
-    ++issued;
+    __syncwarp();
   };
-  if (member < chunks)
-    for (int i = 0; i < kDepth; ++i) issue();
+  issue();
+  issue();
 
   W4Walk walk;
   uint32_t used = 0;
@@ -219,41 +267,27 @@ __global__ void __launch_bounds__(kWarps * 32, RT * NB >= 8 ? 1 : 2)
       for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int c = 0; c < 4; ++c) acc[r][b][c] = 0.f;
-    const int64_t s0 = e * p.s_se;
     for (int chunk = member; chunk < chunks; chunk += p.along) {
-      float scale[RT][2];
-      uint32_t zero[RT][2];
-      auto load_group = [&](int k) {
-        const int group = k / p.group;
-#pragma unroll
-        for (int r = 0; r < RT; ++r)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int n = n0 + r * 16 + h * 8 + g;
-            const bool in = n < p.n && group < p.groups;
-            const int64_t at = s0 + n * p.s_sn + group;
-            scale[r][h] = in ? load_scale(p.scales, p.scale_dtype, at) : 0.f;
-            zero[r][h] = Unpack<T>::zero(in && p.zeros ? __ldg(p.zeros + at) : 8);
-          }
-      };
-      if constexpr (WHOLE) load_group(chunk * kChunk);
-      const unsigned char *st = ring + used % kDepth * Shape::kStage;
-      ok = mbar_wait_bounded(&full[used % kDepth], used / kDepth & 1, abort_flag, DEV_TIMEOUT_PRODUCER);
+      const unsigned char *st = ring + (used & 1) * Shape::kStage;
+      ok = mbar_wait_bounded(&full[used & 1], used >> 1 & 1, abort_flag, DEV_TIMEOUT_PRODUCER);
       if (!__all_sync(0xffffffffu, ok)) {
         ok = false;
         break;
       }
       float part[RT][NB][4];
+      uint2 zero[RT][2];
+      float scale[RT][2];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {                       // 32 k at a time
-        if constexpr (!WHOLE) load_group(chunk * kChunk + i * 32);
         if (!WHOLE || i == 0) {
 #pragma unroll
           for (int r = 0; r < RT; ++r)
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-              for (int c = 0; c < 4; ++c) part[r][b][c] = 0.f;
+            for (int h = 0; h < 2; ++h) {
+              const uint4 v = entries[(WHOLE ? 0 : i * Shape::kRows) + r * 16 + h * 8 + g];
+              scale[r][h] = __uint_as_float(v.x);
+              zero[r][h] = make_uint2(v.y, v.z);
+            }
         }
         // x: row g of each block of 8, the lane's 8 k, as the pairs (0 4) (1 5) (2 6) (3 7)
         uint32_t x[NB][4];
@@ -268,22 +302,22 @@ __global__ void __launch_bounds__(kWarps * 32, RT * NB >= 8 ? 1 : 2)
         }
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
-          uint32_t w[2];
+          uint32_t w[2][4];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int rr = r * 16 + h * 8 + g;
-            w[h] = *reinterpret_cast<const uint32_t *>(st + rr * 64 + ((i ^ ((rr >> 1) & 3)) << 4) + t * 4);
+            Unpack<T>::values(
+                *reinterpret_cast<const uint32_t *>(st + rr * 64 + ((i ^ ((rr >> 1) & 3)) << 4) + t * 4),
+                zero[r][h], w[h]);
           }
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            uint32_t a[4];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              a[h] = Unpack<T>::value(w[h] >> (8 * half), zero[r][h]);
-              a[2 + h] = Unpack<T>::value(w[h] >> (8 * half + 4), zero[r][h]);
-            }
-#pragma unroll
-            for (int b = 0; b < NB; ++b) mma<T>(part[r][b], a, x[b][2 * half], x[b][2 * half + 1]);
+          for (int b = 0; b < NB; ++b) {
+            float(&d)[4] = part[r][b];
+            if (!WHOLE || i == 0)
+              mma<T>(d, w[0][0], w[1][0], w[0][1], w[1][1], x[b][0], x[b][1], 0.f, 0.f, 0.f, 0.f);
+            else
+              mma<T>(d, w[0][0], w[1][0], w[0][1], w[1][1], x[b][0], x[b][1], d[0], d[1], d[2], d[3]);
+            mma<T>(d, w[0][2], w[1][2], w[0][3], w[1][3], x[b][2], x[b][3], d[0], d[1], d[2], d[3]);
           }
         }
         if (!WHOLE || i == 3) {
@@ -322,7 +356,7 @@ __global__ void __launch_bounds__(kWarps * 32, RT * NB >= 8 ? 1 : 2)
   // copies still in flight after a wait gave up
   if (lane == 0)
     for (; used < issued; ++used)
-      mbar_wait_bounded(&full[used % kDepth], used / kDepth & 1, abort_flag, DEV_TIMEOUT_PRODUCER);
+      mbar_wait_bounded(&full[used & 1], used >> 1 & 1, abort_flag, DEV_TIMEOUT_PRODUCER);
 
   if (p.offsets) {                                        // rows that no group holds are zero
     int first, last, a, b;
@@ -343,10 +377,10 @@ int make_maps(CUtensorMap *w, CUtensorMap *x, const void *packed, const void *xp
                       kChunk / 32, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
-template <typename T, int RT, int NB>
-int run(const void *packed, const void *x, W4Params p, int dtype, int64_t x_sr, int64_t p_se, int64_t p_sn,
-        cudaStream_t st) {
-  using Shape = W4Shape<RT, NB>;
+template <typename T, int RT, int NB, bool WHOLE>
+int run_shape(const void *packed, const void *x, W4Params p, int dtype, int64_t x_sr, int64_t p_se, int64_t p_sn,
+              cudaStream_t st) {
+  using Shape = W4Shape<RT, NB, WHOLE>;
   CUtensorMap tw, tx;
   if (int rc = make_maps(&tw, &tx, packed, x, p, dtype, x_sr, p_se, p_sn, Shape::kRows, 8 * NB)) return rc;
   p.column_tiles = (p.n + Shape::kRows - 1) / Shape::kRows;
@@ -354,9 +388,10 @@ int run(const void *packed, const void *x, W4Params p, int dtype, int64_t x_sr, 
   const int64_t tiles = blocks * p.column_tiles;
   if (tiles > INT32_MAX / 2) return set_error(OZ_ERR_INVALID, "too many tiles");
   const int teams = kWarps / p.along;
-  const int64_t most = (RT * NB >= 8 ? 1 : 2) * (int64_t)tile::sm_count();
+  const int64_t most = Shape::kCtas * (int64_t)tile::sm_count();
   const int64_t need = (tiles + teams - 1) / teams;
-  auto kernel = p.group % kChunk == 0 ? w4_kernel<T, RT, NB, true> : w4_kernel<T, RT, NB, false>;
+  auto kernel = w4_kernel<T, RT, NB, WHOLE>;
+  static_assert(Shape::kBytes <= 227 * 1024, "shared memory");
   if (int rc = set_smem_once((const void *)kernel, Shape::kBytes, "w4_kernel shared memory")) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(need < most ? need : most));
@@ -370,6 +405,13 @@ int run(const void *packed, const void *x, W4Params p, int dtype, int64_t x_sr, 
   cfg.numAttrs = 1;
   count_launch();
   return check_cuda(cudaLaunchKernelEx(&cfg, kernel, tw, tx, p), "w4_kernel launch");
+}
+
+template <typename T, int RT, int NB>
+int run(const void *packed, const void *x, const W4Params &p, int dtype, int64_t x_sr, int64_t p_se, int64_t p_sn,
+        cudaStream_t st) {
+  return p.group % kChunk == 0 ? run_shape<T, RT, NB, true>(packed, x, p, dtype, x_sr, p_se, p_sn, st)
+                               : run_shape<T, RT, NB, false>(packed, x, p, dtype, x_sr, p_se, p_sn, st);
 }
 
 template <typename T>
