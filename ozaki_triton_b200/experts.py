@@ -22,23 +22,49 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .api import _OZ_DTYPE, _check_cuda, _stream_ptr
+from .api import _OZ_DTYPE, _RAW_STREAM, _check_cuda
 
 # operand types: products are exact in fp32, sums are held in fp32
 GROUPED_DTYPES = (torch.bfloat16, torch.float16)
 
+_OFFSET_DTYPES = (torch.int32, torch.int64)
+_SCALE_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
 
-def _check_places(x: torch.Tensor, *ts: Optional[torch.Tensor]) -> None:
-    given = [t for t in ts if t is not None]
-    _check_cuda(x, *given)
-    for t in given:
-        if t.device != x.device:
+
+def _check_places(x: torch.Tensor, *ts: Optional[torch.Tensor]) -> int:
+    """The index of the device that holds every tensor."""
+    _check_cuda(x)
+    index = x.get_device()
+    for t in ts:
+        if t is not None and (not t.is_cuda or t.get_device() != index):
             raise ValueError(f"tensors on different devices: {x.device} and {t.device}")
+    return index
+
+
+class _OnDevice:
+    """Makes a device current for a call, at no cost where it is already."""
+
+    __slots__ = ("index", "other")
+
+    def __init__(self, index: int):
+        self.index = index
+
+    def __enter__(self):
+        self.other = torch.cuda.current_device()
+        if self.other != self.index:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *_):
+        if self.other != self.index:
+            torch.cuda.set_device(self.other)
+
+
+def _stream_of(device: int) -> int:
+    return _RAW_STREAM(device) if _RAW_STREAM is not None else torch.cuda.current_stream(device).cuda_stream
 
 
 def _check_offsets(offsets: torch.Tensor, groups: int) -> None:
-    assert offsets.dtype in (torch.int32, torch.int64), \
-        f"offsets must be int32 or int64, got {offsets.dtype}"
+    assert offsets.dtype in _OFFSET_DTYPES, f"offsets must be int32 or int64, got {offsets.dtype}"
     assert offsets.dim() == 1 and offsets.shape[0] == groups + 1, \
         f"offsets must have {groups + 1} entries, got shape {tuple(offsets.shape)}"
     assert offsets.is_contiguous(), "offsets must be contiguous"
@@ -52,7 +78,7 @@ def _check_rows(x: torch.Tensor, what: str) -> None:
 def _out_dtype(dtype: Optional[torch.dtype], operand: torch.dtype) -> torch.dtype:
     if dtype is None:
         return operand
-    assert dtype in (operand, torch.float32), \
+    assert dtype is operand or dtype is torch.float32, \
         f"results are {operand} or torch.float32, not {dtype}"
     return dtype
 
@@ -67,9 +93,13 @@ def _copied(t: torch.Tensor) -> torch.Tensor:
 def _as_operand(t: torch.Tensor) -> torch.Tensor:
     """t, or a copy where the copy unit cannot read its layout: it wants a unit
     stride along the last dimension, 16-byte boundaries and no repeated rows."""
-    if (t.stride(-1) == 1 or t.shape[-1] == 1) and t.data_ptr() % 16 == 0 and all(
-            n <= 1 or (s > 0 and s % 8 == 0) for n, s in zip(t.shape[:-1], t.stride()[:-1])):
-        return t
+    shape, strides = t.shape, t.stride()
+    if (strides[-1] == 1 or shape[-1] == 1) and t.data_ptr() % 16 == 0:
+        for n, s in zip(shape[:-1], strides):
+            if n > 1 and (s <= 0 or s % 8):
+                break
+        else:
+            return t
     return _copied(t)
 
 
@@ -80,33 +110,38 @@ def _as_weights(w: torch.Tensor) -> torch.Tensor:
     return _as_operand(w)
 
 
-def _product(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor,
-             out_dtype: torch.dtype) -> torch.Tensor:
+def _product(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, out_dtype: torch.dtype,
+             device: int) -> torch.Tensor:
     rows, k = x.shape
     groups, _, n = w.shape
-    y = torch.empty((rows, n), dtype=out_dtype, device=x.device)
-    if k > 0 and y.numel() > 0:
+    y = x.new_empty((rows, n), dtype=out_dtype)
+    if rows == 0 or n == 0:
+        return y
+    if k > 0:
         x, w = _as_operand(x), _as_weights(w)
-    with torch.cuda.device(x.device):
+    w_se, w_sk, w_sn = w.stride()
+    with _OnDevice(device):
         _lib.check(_lib.load().oz_grouped_matmul(
-            x.data_ptr(), w.data_ptr(), offsets.data_ptr(), offsets.dtype == torch.int64,
+            x.data_ptr(), w.data_ptr(), offsets.data_ptr(), offsets.dtype is torch.int64,
             _OZ_DTYPE[x.dtype], _OZ_DTYPE[out_dtype], groups, rows, k, n, x.stride(0),
-            *w.stride(), y.data_ptr(), n, _stream_ptr(x.device)))
+            w_se, w_sk, w_sn, y.data_ptr(), n, _stream_of(device)))
     return y
 
 
 def _weight_gradient(x: torch.Tensor, dy: torch.Tensor, offsets: torch.Tensor, groups: int,
-                     out_dtype: torch.dtype) -> torch.Tensor:
+                     out_dtype: torch.dtype, device: int) -> torch.Tensor:
     rows, k = x.shape
     n = dy.shape[1]
-    dw = torch.empty((groups, k, n), dtype=out_dtype, device=x.device)
-    if rows > 0 and dw.numel() > 0:
+    dw = x.new_empty((groups, k, n), dtype=out_dtype)
+    if k == 0 or n == 0:
+        return dw
+    if rows > 0:
         x, dy = _as_operand(x), _as_operand(dy)
-    with torch.cuda.device(x.device):
+    with _OnDevice(device):
         _lib.check(_lib.load().oz_grouped_wgrad(
-            x.data_ptr(), dy.data_ptr(), offsets.data_ptr(), offsets.dtype == torch.int64,
+            x.data_ptr(), dy.data_ptr(), offsets.data_ptr(), offsets.dtype is torch.int64,
             _OZ_DTYPE[x.dtype], _OZ_DTYPE[out_dtype], groups, rows, k, n, x.stride(0),
-            dy.stride(0), dw.data_ptr(), _stream_ptr(x.device)))
+            dy.stride(0), dw.data_ptr(), _stream_of(device)))
     return dw
 
 
@@ -123,15 +158,15 @@ class _GroupedMatmul(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, offsets, out_dtype):
         ctx.save_for_backward(x, w, offsets)
-        return _product(x, w, offsets, out_dtype)
+        return _product(x, w, offsets, out_dtype, x.get_device())
 
     @staticmethod
     def backward(ctx, dy):
         x, w, offsets = ctx.saved_tensors
-        dy = dy.to(x.dtype)
+        dy, device = dy.to(x.dtype), x.get_device()
         need_x, need_w = ctx.needs_input_grad[:2]
-        dx = _product(dy, w.transpose(1, 2), offsets, x.dtype) if need_x else None
-        dw = _weight_gradient(x, dy, offsets, w.shape[0], w.dtype) if need_w else None
+        dx = _product(dy, w.transpose(1, 2), offsets, x.dtype, device) if need_x else None
+        dw = _weight_gradient(x, dy, offsets, w.shape[0], w.dtype, device) if need_w else None
         return dx, dw, None, None
 
 
@@ -148,10 +183,10 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, *,
     """
     _check_grouped(x, w, offsets)
     out_dtype = _out_dtype(out_dtype, x.dtype)
-    _check_places(x, w, offsets)
+    device = _check_places(x, w, offsets)
     if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
         return _GroupedMatmul.apply(x, w, offsets, out_dtype)
-    return _product(x, w, offsets, out_dtype)
+    return _product(x, w, offsets, out_dtype, device)
 
 
 def grouped_matmul_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor,
@@ -169,9 +204,10 @@ def grouped_matmul_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor,
     assert tuple(dy.shape) == (x.shape[0], w.shape[2]), \
         f"dy must be {(x.shape[0], w.shape[2])}, got {tuple(dy.shape)}"
     dw_dtype = _out_dtype(dw_dtype, x.dtype)
-    _check_places(x, w, offsets, dy)
-    return (_product(dy, w.transpose(1, 2), offsets, x.dtype),
-            _weight_gradient(x, dy, offsets, w.shape[0], dw_dtype))
+    device = _check_places(x, w, offsets, dy)
+    x, dy = _as_operand(x), _as_operand(dy)               # once for both products
+    return (_product(dy, w.transpose(1, 2), offsets, x.dtype, device),
+            _weight_gradient(x, dy, offsets, w.shape[0], dw_dtype, device))
 
 
 def quantize_w4(w: torch.Tensor, group_size: int = 128, *, symmetric: bool = True,
@@ -220,41 +256,44 @@ def matmul_w4(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor,
     """
     _check_rows(x, "x")
     lead = 2 if offsets is None else 3
-    assert packed.dim() == lead, f"packed must have {lead} dimensions, got shape {tuple(packed.shape)}"
-    assert packed.dtype == torch.uint8, f"packed must be uint8, got {packed.dtype}"
+    p_shape, s_shape = packed.shape, scales.shape
     rows, k = x.shape
-    n = packed.shape[-2]
-    assert packed.shape[-1] * 2 == k, f"contraction dim mismatch: x K={k}, packed K={packed.shape[-1] * 2}"
-    assert scales.dim() == lead and scales.shape[:-1] == packed.shape[:-1], \
-        f"scales of shape {tuple(scales.shape)} do not fit packed {tuple(packed.shape)}"
-    assert scales.dtype in (torch.float16, torch.bfloat16, torch.float32), \
-        f"unsupported scale dtype: {scales.dtype}"
-    groups = scales.shape[-1]
-    assert groups > 0 and k % groups == 0 and (k // groups) % 32 == 0 and k > 0, \
+    assert len(p_shape) == lead, f"packed must have {lead} dimensions, got shape {tuple(p_shape)}"
+    assert packed.dtype is torch.uint8, f"packed must be uint8, got {packed.dtype}"
+    n = p_shape[-2]
+    assert p_shape[-1] * 2 == k, f"contraction dim mismatch: x K={k}, packed K={p_shape[-1] * 2}"
+    assert len(s_shape) == lead and s_shape[:-1] == p_shape[:-1], \
+        f"scales of shape {tuple(s_shape)} do not fit packed {tuple(p_shape)}"
+    assert scales.dtype in _SCALE_DTYPES, f"unsupported scale dtype: {scales.dtype}"
+    groups = s_shape[-1]
+    assert groups > 0 and k > 0 and k % groups == 0 and (k // groups) % 32 == 0, \
         f"the group size must be a multiple of 32 that divides K ({groups} scales, K={k})"
     if zeros is not None:
-        assert zeros.dtype == torch.uint8, f"zeros must be uint8, got {zeros.dtype}"
-        assert zeros.shape == scales.shape, \
-            f"zeros of shape {tuple(zeros.shape)} do not fit scales {tuple(scales.shape)}"
-    experts = 1 if offsets is None else packed.shape[0]
+        assert zeros.dtype is torch.uint8, f"zeros must be uint8, got {zeros.dtype}"
+        assert zeros.shape == s_shape, \
+            f"zeros of shape {tuple(zeros.shape)} do not fit scales {tuple(s_shape)}"
+    experts = 1 if offsets is None else p_shape[0]
     assert experts >= 1, "packed must hold at least one expert"
     out_dtype = _out_dtype(out_dtype, x.dtype)
     if offsets is not None:
         _check_offsets(offsets, experts)
-    _check_places(x, packed, scales, zeros, offsets)
+    device = _check_places(x, packed, scales, zeros, offsets)
+    y = x.new_empty((rows, n), dtype=out_dtype)
+    if rows == 0 or n == 0:
+        return y
     x = _as_operand(x)
     packed, scales = packed.contiguous(), scales.contiguous()
     if packed.data_ptr() % 16:
         packed = packed.clone()
-    zeros = zeros.contiguous() if zeros is not None else None
-    y = torch.empty((rows, n), dtype=out_dtype, device=x.device)
-    with torch.cuda.device(x.device):
+    if zeros is not None:
+        zeros = zeros.contiguous()
+    with _OnDevice(device):
         _lib.check(_lib.load().oz_matmul_w4(
             x.data_ptr(), packed.data_ptr(), scales.data_ptr(),
             zeros.data_ptr() if zeros is not None else None,
             offsets.data_ptr() if offsets is not None else None,
-            offsets is not None and offsets.dtype == torch.int64, _OZ_DTYPE[x.dtype],
+            offsets is not None and offsets.dtype is torch.int64, _OZ_DTYPE[x.dtype],
             _OZ_DTYPE[scales.dtype], _OZ_DTYPE[out_dtype], experts, rows, k, n, k // groups,
             x.stride(0), n * (k // 2), k // 2, n * groups, groups, y.data_ptr(), n,
-            _stream_ptr(x.device)))
+            _stream_of(device)))
     return y

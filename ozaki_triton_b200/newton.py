@@ -8,7 +8,8 @@ from typing import Optional, Sequence, Union
 import torch
 
 from . import _lib
-from .api import _OZ_DTYPE, _check_cuda, _stream_ptr
+from .api import _OZ_DTYPE, _check_cuda
+from .experts import _OnDevice, _stream_of
 
 ORTHOGONALIZE_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 
@@ -55,8 +56,9 @@ def orthogonalize(g: torch.Tensor, steps: int = 5,
     code = _OZ_DTYPE[g.dtype]
     ws_bytes = lib.oz_orthogonalize_workspace_bytes(code, g3.shape[0], m, n, num_splits)
     ws = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=g.device)
-    with torch.cuda.device(g.device):
+    device = g.get_device()
+    with _OnDevice(device):
         _lib.check(lib.oz_orthogonalize(
             g3.data_ptr(), code, g3.shape[0], m, n, *g3.stride(), steps, coeffs, float(eps),
-            num_splits, out.data_ptr(), ws.data_ptr(), ws_bytes, _stream_ptr(g.device)))
+            num_splits, out.data_ptr(), ws.data_ptr(), ws_bytes, _stream_of(device)))
     return out
