@@ -99,7 +99,7 @@ __device__ __forceinline__ void clear_outside(const GroupedParams &p, int me, in
 struct RowTile { int row, rows, column; };   // first row, rows from there to the group's end
 
 // y = x w: A is the rows of x, B the columns of w[e].
-template <typename O, int PAIR_, int NT_, bool BMN_> struct RowsJob {
+template <typename O, int PAIR_, int NT_, bool BMN_> struct RowsJob : NoLookAhead {
   static constexpr int PAIR = PAIR_, NT = NT_, PLANES = 1, PASS = sizeof(O) == 4 ? 8 : 0;
   static constexpr bool AMN = false, BMN = BMN_, RAGGED = false;
   using Params = GroupedParams;
@@ -122,7 +122,7 @@ template <typename O, int PAIR_, int NT_, bool BMN_> struct RowsJob {
   };
   template <class Source>
   static __device__ void epilogue(const Params &p, const TileOf<Extra> &t, const Source &source, int row,
-                                  int column, unsigned char *mine) {
+                                  int column, unsigned char *mine, Ahead &) {
     const int64_t c0 = t.extra.column + column;
     write_rows<O, NT / 2>(source, mine,
                           static_cast<O *>(p.out) + (int64_t)(t.extra.row + row) * p.ld + c0, p.ld,
@@ -134,7 +134,7 @@ template <typename O, int PAIR_, int NT_, bool BMN_> struct RowsJob {
 // The same product with the roles exchanged, for groups of a few rows: A is
 // 128 columns of w[e], B up to NT rows of x, so a tile's weights are read
 // once and hardly any of the staged bytes belong to rows that are not there.
-template <typename O, int NT_, bool AMN_> struct ColumnsJob {
+template <typename O, int NT_, bool AMN_> struct ColumnsJob : NoLookAhead {
   static constexpr int PAIR = 1, NT = NT_, PLANES = 1, PASS = sizeof(O) == 4 ? 8 : 0;
   static constexpr bool AMN = AMN_, BMN = false, RAGGED = false;
   using Params = GroupedParams;
@@ -157,7 +157,7 @@ template <typename O, int NT_, bool AMN_> struct ColumnsJob {
   };
   template <class Source>
   static __device__ void epilogue(const Params &p, const TileOf<Extra> &t, const Source &source, int row,
-                                  int column, unsigned char *) {
+                                  int column, unsigned char *, Ahead &) {
     const int64_t c = t.extra.column + row + threadIdx.x % 32;
     O *out = static_cast<O *>(p.out) + (int64_t)(t.extra.row + column) * p.ld + c;
     const int rows = t.extra.rows - column;
@@ -178,7 +178,7 @@ struct WeightTile { int row, column, group; };
 
 // dw[e] = x^T dy over the group's rows: both operands are stored across the
 // contraction, whose range is the group.
-template <typename O, int PAIR_, int NT_> struct WeightsJob {
+template <typename O, int PAIR_, int NT_> struct WeightsJob : NoLookAhead {
   static constexpr int PAIR = PAIR_, NT = NT_, PLANES = 1, PASS = sizeof(O) == 4 ? 8 : 0;
   static constexpr bool AMN = true, BMN = true, RAGGED = true;
   using Params = GroupedParams;
@@ -208,7 +208,7 @@ template <typename O, int PAIR_, int NT_> struct WeightsJob {
   };
   template <class Source>
   static __device__ void epilogue(const Params &p, const TileOf<Extra> &t, const Source &source, int row,
-                                  int column, unsigned char *mine) {
+                                  int column, unsigned char *mine, Ahead &) {
     const int64_t r0 = t.extra.row + row, c0 = t.extra.column + column;
     write_rows<O, NT / 2>(source, mine,
                           static_cast<O *>(p.out) + ((int64_t)t.extra.group * p.k + r0) * p.ld + c0,

@@ -38,12 +38,6 @@ __device__ __forceinline__ float load_value(const void *p, int dtype, int64_t i)
   return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
 }
 
-// v as slices: high, and what is left of it.
-__device__ __forceinline__ void slice(float v, __half &high, __half &low) {
-  high = __float2half_rn(v);
-  low = __float2half_rn(v - __half2float(high));
-}
-
 // A matrix in slices: plane q of member z at base + (q * batch + z) * mat.
 struct Planes {
   __half *base;
@@ -56,6 +50,7 @@ struct Planes {
 struct InitParams {
   const void *g;
   int dtype, partials;
+  bool flat, vectors;               // G's member is one run of elements; its lines start on 16-byte boundaries
   int rows, cols;                   // rows <= cols, after the transposition of a tall G
   int64_t g_sb, g_sr, g_sc;         // strides of G's member, and of X's rows and columns in G
   double *partial;                  // (batch, partials) sums of squares
@@ -63,78 +58,128 @@ struct InitParams {
   double eps, scale;
 };
 
-// Sums of squares in fp64 (fp32 would overflow from 1.8e19 on), each block a
-// fixed part: the order of the sum does not depend on the launch.
-__global__ void __launch_bounds__(256) squares_kernel(const InitParams p) {
-  __shared__ double part[8];
-  // consecutive threads along the smaller stride
-  const bool across = p.g_sr < p.g_sc;
-  const int64_t inner = across ? p.rows : p.cols, total = (int64_t)p.rows * p.cols;
-  const int64_t s_in = across ? p.g_sr : p.g_sc, s_out = across ? p.g_sc : p.g_sr;
-  const int64_t base = blockIdx.y * p.g_sb, stride = (int64_t)gridDim.x * 256;
-  double sum = 0;
-  int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  for (; i + 3 * stride < total; i += 4 * stride) {
-    float v[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int64_t q = i + u * stride;
-      v[u] = load_value(p.g, p.dtype, base + q / inner * s_out + q % inner * s_in);
-    }
-#pragma unroll
-    for (int u = 0; u < 4; ++u) sum += (double)v[u] * v[u];
+// 8 consecutive elements from a 16-byte boundary.
+__device__ __forceinline__ void load8(const void *p, int dtype, int64_t i, float (&v)[8]) {
+  if (dtype == OZ_F32) {
+    const float4 *q = reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i);
+    const float4 a = __ldg(q), b = __ldg(q + 1);
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    return;
   }
-  for (; i < total; i += stride) {
-    const double v = load_value(p.g, p.dtype, base + i / inner * s_out + i % inner * s_in);
-    sum += v * v;
-  }
-  for (int o = 16; o; o /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = sum;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < 8; ++w) part[0] += part[w];
-    p.partial[(int64_t)blockIdx.y * p.partials + blockIdx.x] = part[0];
+  const uint4 a = __ldg(reinterpret_cast<const uint4 *>(static_cast<const __half *>(p) + i));
+  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    const float2 f = dtype == OZ_F16 ? __half22float2(*reinterpret_cast<const __half2 *>(&w[x]))
+                                     : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&w[x]));
+    v[2 * x] = f.x;
+    v[2 * x + 1] = f.y;
   }
 }
 
-// X_0 in slices, 32 x 32 tiles through shared memory: G is read along its
-// smaller stride and X written along its rows.
-__global__ void __launch_bounds__(256) normalise_kernel(const InitParams p) {
-  __shared__ double part[8];
-  __shared__ float v[32][33];
-  double sum = 0;
-  for (int i = threadIdx.x; i < p.partials; i += 256) sum += p.partial[(int64_t)blockIdx.z * p.partials + i];
+__device__ double block_sum(double sum, double *part) {
   for (int o = 16; o; o /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = sum;
   __syncthreads();
   sum = 0;
   for (int w = 0; w < 8; ++w) sum += part[w];
+  return sum;
+}
+
+// Sums of squares in fp64 (fp32 would overflow from 1.8e19 on), each block a
+// fixed part: the order of the sum does not depend on the launch.
+__global__ void __launch_bounds__(256) squares_kernel(const InitParams p) {
+  __shared__ double part[8];
+  const int64_t base = blockIdx.y * p.g_sb, stride = (int64_t)gridDim.x * 256;
+  double sum = 0;
+  if (p.flat) {
+    const int64_t pieces = (int64_t)p.rows * p.cols / 8;
+    int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    for (; i < pieces; i += 2 * stride) {
+      float v[2][8];
+      load8(p.g, p.dtype, base + i * 8, v[0]);
+      const bool two = i + stride < pieces;
+      if (two) load8(p.g, p.dtype, base + (i + stride) * 8, v[1]);
+#pragma unroll
+      for (int x = 0; x < 8; ++x) sum += (double)v[0][x] * v[0][x];
+      if (two)
+#pragma unroll
+        for (int x = 0; x < 8; ++x) sum += (double)v[1][x] * v[1][x];
+    }
+  } else {
+    // a line at a time, consecutive threads along the smaller stride
+    const bool across = p.g_sr < p.g_sc;
+    const int inner = across ? p.rows : p.cols, outer = across ? p.cols : p.rows;
+    const int64_t s_in = across ? p.g_sr : p.g_sc, s_out = across ? p.g_sc : p.g_sr;
+    const int wide = inner >= 256 ? 256 : 32;                // threads of a line
+    for (int o = blockIdx.x * (256 / wide) + threadIdx.x / wide; o < outer; o += gridDim.x * (256 / wide))
+      for (int i = threadIdx.x % wide; i < inner; i += wide) {
+        const double v = load_value(p.g, p.dtype, base + o * s_out + i * s_in);
+        sum += v * v;
+      }
+  }
+  sum = block_sum(sum, part);
+  if (threadIdx.x == 0) p.partial[(int64_t)blockIdx.y * p.partials + blockIdx.x] = sum;
+}
+
+// X_0 in slices, 64 x 64 tiles: 8 elements at a time from G along its smaller
+// stride, through shared memory where that is across X's rows, and 8 at a
+// time to X along its rows (whose pitch is a multiple of 8).
+__global__ void __launch_bounds__(256) normalise_kernel(const InitParams p) {
+  __shared__ double part[8];
+  __shared__ float tile[64][65];
+  double sum = 0;
+  for (int i = threadIdx.x; i < p.partials; i += 256) sum += p.partial[(int64_t)blockIdx.z * p.partials + i];
+  sum = block_sum(sum, part);
   const double scale = p.scale / (sqrt(sum) + p.eps);
   const bool zero = sum == 0 && p.eps == 0;             // 0 / 0: a zero matrix stays zero
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const bool across = p.g_sr < p.g_sc;
-  const int r0 = blockIdx.y * 32, c0 = blockIdx.x * 32;
-  for (int i = warp; i < 32; i += 8) {
-    const int r = r0 + (across ? lane : i), c = c0 + (across ? i : lane);
-    if (r < p.rows && c < p.cols)
-      v[r - r0][c - c0] =
-          zero ? 0.f : (float)(load_value(p.g, p.dtype, blockIdx.z * p.g_sb + r * p.g_sr + c * p.g_sc) * scale);
+  const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
+#pragma unroll
+  for (int i = threadIdx.x; i < 512; i += 256) {
+    // line and piece of G's tile
+    const int line = i / 8, u = i % 8 * 8;
+    const int r = r0 + (across ? u : line), c = c0 + (across ? line : u);
+    if (r >= p.rows || c >= p.cols) continue;
+    const int left = across ? p.rows - r : p.cols - c;
+    const int64_t at = blockIdx.z * p.g_sb + r * p.g_sr + c * p.g_sc, step = across ? p.g_sr : p.g_sc;
+    float v[8];
+    if (p.vectors && left >= 8) {
+      load8(p.g, p.dtype, at, v);
+    } else {
+#pragma unroll
+      for (int x = 0; x < 8; ++x) v[x] = x < left ? load_value(p.g, p.dtype, at + x * step) : 0.f;
+    }
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const float f = zero ? 0.f : (float)(v[x] * scale);
+      if (across) tile[u + x][line] = f;
+      else tile[line][u + x] = f;
+    }
   }
   __syncthreads();
-  for (int i = warp; i < 32; i += 8)
-    if (r0 + i < p.rows && c0 + lane < p.cols) {
-      __half high, low;
-      slice(v[i][lane], high, low);
-      *p.x.at(0, blockIdx.z, r0 + i, c0 + lane) = high;
-      *p.x.at(1, blockIdx.z, r0 + i, c0 + lane) = low;
+#pragma unroll
+  for (int i = threadIdx.x; i < 512; i += 256) {
+    const int r = i / 8, u = i % 8 * 8;
+    if (r0 + r >= p.rows || c0 + u >= p.cols) continue;
+    uint32_t high[4], low[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const float a = tile[r][u + 2 * x], b = tile[r][u + 2 * x + 1];
+      const __half2 h = __floats2half2_rn(a, b);
+      const float2 f = __half22float2(h);
+      high[x] = *reinterpret_cast<const uint32_t *>(&h);
+      low[x] = pack2<__half>(a - f.x, b - f.y);
     }
+    *reinterpret_cast<uint4 *>(p.x.at(0, blockIdx.z, r0 + r, c0 + u)) = make_uint4(high[0], high[1], high[2], high[3]);
+    *reinterpret_cast<uint4 *>(p.x.at(1, blockIdx.z, r0 + r, c0 + u)) = make_uint4(low[0], low[1], low[2], low[3]);
+  }
 }
 
 struct StepParams {
   uint32_t idesc;
   int batch, rows, cols, k;         // of the result; terms of the contraction
   int row_tiles, column_tiles, tiles;   // tiles of one member
-  int in_planes, out_planes;
   float alpha, beta;                // result = alpha * in + beta * accumulator
   Planes in, out;
   // the last step's result instead of `out`: element (z, r, c) of the type
@@ -143,68 +188,85 @@ struct StepParams {
   int64_t last_sb, last_sr, last_sc;
 };
 
-// 32 rows x 32 fp16 columns at src, each lane its own row (4 pieces of 8
-// columns), read 64 bytes of a row at a time through the warp's staging.
-__device__ __forceinline__ void load_chunk(unsigned char *mine, const __half *src, int64_t ld, int rows,
-                                           int cols, uint4 (&v)[4]) {
+// 32 rows x 32 fp16 columns: each lane 4 pieces of 8 columns, 64 bytes of a
+// row by 4 lanes; the warp's staging turns them into each lane's own row.
+struct Chunk { uint4 piece[4]; };
+
+__device__ __forceinline__ uint4 *chunk_slot(unsigned char *mine, int r, int u) {
+  return reinterpret_cast<uint4 *>(mine + r * 64 + ((u ^ ((r >> 1) & 3)) << 4));
+}
+__device__ __forceinline__ void fetch(const __half *src, int64_t ld, int rows, int cols, Chunk &v) {
   const int lane = threadIdx.x % 32;
-  uint4 got[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int r = i * 8 + lane / 4, u = lane % 4;
-    got[i] = r < rows && u * 8 < cols ? *reinterpret_cast<const uint4 *>(src + r * ld + u * 8)
-                                      : make_uint4(0, 0, 0, 0);
+    v.piece[i] = r < rows && u * 8 < cols ? *reinterpret_cast<const uint4 *>(src + r * ld + u * 8)
+                                          : make_uint4(0, 0, 0, 0);
   }
-  auto slot = [&](int r, int u) {
-    return reinterpret_cast<uint4 *>(mine + r * 64 + ((u ^ ((r >> 1) & 3)) << 4));
-  };
+}
+__device__ __forceinline__ void to_rows(unsigned char *mine, Chunk &v) {
+  const int lane = threadIdx.x % 32;
   __syncwarp();
 #pragma unroll
-  for (int i = 0; i < 4; ++i) *slot(i * 8 + lane / 4, lane % 4) = got[i];
+  for (int i = 0; i < 4; ++i) *chunk_slot(mine, i * 8 + lane / 4, lane % 4) = v.piece[i];
   __syncwarp();
 #pragma unroll
-  for (int u = 0; u < 4; ++u) v[u] = *slot(lane, u);
+  for (int u = 0; u < 4; ++u) v.piece[u] = *chunk_slot(mine, lane, u);
 }
 
-// The way back, from each lane's row.
-__device__ __forceinline__ void store_chunk(unsigned char *mine, __half *dst, int64_t ld, int rows, int cols,
-                                            const uint4 (&v)[4]) {
+// The way back: the chunk in the staging to memory.
+__device__ __forceinline__ void flush(unsigned char *mine, __half *dst, int64_t ld, int rows, int cols) {
   const int lane = threadIdx.x % 32;
-  auto slot = [&](int r, int u) {
-    return reinterpret_cast<uint4 *>(mine + r * 64 + ((u ^ ((r >> 1) & 3)) << 4));
-  };
-  __syncwarp();
-#pragma unroll
-  for (int u = 0; u < 4; ++u) *slot(lane, u) = v[u];
   __syncwarp();
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int r = i * 8 + lane / 4, u = lane % 4;
-    if (r < rows && u * 8 < cols) *reinterpret_cast<uint4 *>(dst + r * ld + u * 8) = *slot(r, u);
+    if (r < rows && u * 8 < cols) *reinterpret_cast<uint4 *>(dst + r * ld + u * 8) = *chunk_slot(mine, r, u);
   }
+  __syncwarp();
+}
+// From each lane's row; and its mirror image, from each lane's column.
+__device__ __forceinline__ void store_rows(unsigned char *mine, __half *dst, int64_t ld, int rows, int cols,
+                                           const uint4 (&v)[4]) {
+  __syncwarp();
+#pragma unroll
+  for (int u = 0; u < 4; ++u) *chunk_slot(mine, threadIdx.x % 32, u) = v[u];
+  flush(mine, dst, ld, rows, cols);
+}
+__device__ __forceinline__ void store_columns(unsigned char *mine, __half *dst, int64_t ld, int rows, int cols,
+                                              const uint4 (&v)[4]) {
+  const int lane = threadIdx.x % 32;
+  const __half *h = reinterpret_cast<const __half *>(&v[0]);
+#pragma unroll
+  for (int x = 0; x < 32; ++x) reinterpret_cast<__half *>(chunk_slot(mine, x, lane / 8))[lane % 8] = h[x];
+  flush(mine, dst, ld, rows, cols);
 }
 
-__device__ __forceinline__ const __half *halves(const uint4 (&v)[4]) {
-  return reinterpret_cast<const __half *>(&v[0]);
+// The part of `in` under chunk c of the warp's columns, IN slices.
+template <int IN>
+__device__ __forceinline__ void fetch_in(const StepParams &p, int z, int row, int column, Chunk (&v)[IN + !IN]) {
+#pragma unroll
+  for (int q = 0; q < IN; ++q)
+    fetch(p.in.at(q, z, row, column), p.in.ld, p.rows - row, p.cols - column, v[q]);
 }
 
 // alpha * in + beta * accumulator for 32 columns of the lane's row.
-template <class Source>
+template <int IN, class Source>
 __device__ __forceinline__ void combine(const StepParams &p, const Source &source, int c, unsigned char *mine,
-                                        int z, int row, int column, int rows, int cols, float (&v)[32]) {
-  float acc[16];
+                                        Chunk (&in)[IN + !IN], float (&v)[32]) {
 #pragma unroll
   for (int h = 0; h < 32; h += 16) {
+    float acc[16];
     source.read(c + h, acc);
 #pragma unroll
     for (int x = 0; x < 16; ++x) v[h + x] = p.beta * acc[x];
   }
-  for (int q = 0; q < p.in_planes; ++q) {
-    uint4 in[4];
-    load_chunk(mine, p.in.at(q, z, row, column), p.in.ld, rows, cols, in);
+#pragma unroll
+  for (int q = 0; q < IN; ++q) {
+    to_rows(mine, in[q]);
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const __half2 *h = reinterpret_cast<const __half2 *>(&in[u]);
+      const __half2 *h = reinterpret_cast<const __half2 *>(&in[q].piece[u]);
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         const float2 f = __half22float2(h[x]);
@@ -234,15 +296,23 @@ __device__ __forceinline__ void slices_of(const float (&v)[32], uint4 (&high)[4]
 
 struct StepTile { int z, row, column; bool mirror; };
 
-// S = X X^T (in_planes 0) and P = b S + c S S: tiles (i, j) on and below the
-// diagonal, the others their mirror images.
-template <int PAIR_, int NT_, int PLANES_> struct SymmetricJob {
+// S = X X^T (IN 0) and P = b S + c S S (IN slices of S): tiles (i, j) on and
+// below the diagonal, the others their mirror images.
+template <int PAIR_, int NT_, int PLANES_, int IN> struct SymmetricJob {
   static constexpr int PAIR = PAIR_, NT = NT_, PLANES = PLANES_, PASS = (PLANES_ - 1) * 4;
   static constexpr bool AMN = false, BMN = false, RAGGED = false;
   static constexpr int R = kRows * PAIR / NT;           // column tiles as wide as a tile is high
   using Params = StepParams;
   using Extra = StepTile;
   static __device__ int plane_stride(const Params &p) { return p.batch; }
+  // The first chunk of `in` is fetched before the accumulators are there and
+  // each next one before the one in hand is used (passes need the registers).
+  struct Ahead { Chunk in[IN + !IN]; };
+  template <class Tile>
+  static __device__ void look_ahead(const Params &p, const Tile &t, int row, int column, Ahead &early) {
+    if (PASS == 0 && t.extra.row + row < p.rows && t.extra.column + column < p.cols)
+      fetch_in<IN>(p, t.extra.z, t.extra.row + row, t.extra.column + column, early.in);
+  }
   struct Walk {
     __device__ Walk(const Params &) {}
     __device__ bool find(const Params &p, int t, TileOf<Extra> &tile) {
@@ -264,28 +334,32 @@ template <int PAIR_, int NT_, int PLANES_> struct SymmetricJob {
   };
   template <class Source>
   static __device__ void epilogue(const Params &p, const TileOf<Extra> &t, const Source &source, int row,
-                                  int column, unsigned char *mine) {
-    const int r0 = t.extra.row + row, rows = p.rows - r0, lane = threadIdx.x % 32;
+                                  int column, unsigned char *mine, Ahead &early) {
+    const int r0 = t.extra.row + row, rows = p.rows - r0;
     if (rows <= 0) return;
 #pragma unroll
     for (int c = 0; c < NT / 2; c += 32) {
       const int c0 = t.extra.column + column + c, cols = p.cols - c0;
       if (cols <= 0) continue;
       float v[32];
-      combine(p, source, c, mine, t.extra.z, r0, c0, rows, cols, v);
+      Chunk in[IN + !IN];
+      if constexpr (PASS == 0) {
+#pragma unroll
+        for (int q = 0; q < IN; ++q) in[q] = early.in[q];
+        if (c + 32 < NT / 2 && cols > 32) fetch_in<IN>(p, t.extra.z, r0, c0 + 32, early.in);
+      } else {
+        fetch_in<IN>(p, t.extra.z, r0, c0, in);
+      }
+      combine<IN>(p, source, c, mine, in, v);
       uint4 high[4], low[4];
       slices_of(v, high, low);
-      store_chunk(mine, p.out.at(0, t.extra.z, r0, c0), p.out.ld, rows, cols, high);
+      store_rows(mine, p.out.at(0, t.extra.z, r0, c0), p.out.ld, rows, cols, high);
       if constexpr (PLANES == 2)
-        store_chunk(mine, p.out.at(1, t.extra.z, r0, c0), p.out.ld, rows, cols, low);
-      if (t.extra.mirror && lane < rows) {
-        __half *h = p.out.at(0, t.extra.z, c0, r0 + lane), *l = h + p.out.plane;
-#pragma unroll
-        for (int x = 0; x < 32; ++x)
-          if (x < cols) {
-            h[x * p.out.ld] = halves(high)[x];
-            if constexpr (PLANES == 2) l[x * p.out.ld] = halves(low)[x];
-          }
+        store_rows(mine, p.out.at(1, t.extra.z, r0, c0), p.out.ld, rows, cols, low);
+      if (t.extra.mirror) {
+        store_columns(mine, p.out.at(0, t.extra.z, c0, r0), p.out.ld, cols, rows, high);
+        if constexpr (PLANES == 2)
+          store_columns(mine, p.out.at(1, t.extra.z, c0, r0), p.out.ld, cols, rows, low);
       }
     }
   }
@@ -294,11 +368,20 @@ template <int PAIR_, int NT_, int PLANES_> struct SymmetricJob {
 
 // X <- a X + P X: A is the rows of P, B the columns of X.
 template <int PAIR_, int NT_, int PLANES_> struct UpdateJob {
+  static constexpr int IN = 2;
   static constexpr int PAIR = PAIR_, NT = NT_, PLANES = PLANES_, PASS = (PLANES_ - 1) * 4;
   static constexpr bool AMN = false, BMN = true, RAGGED = false;
   using Params = StepParams;
   using Extra = StepTile;
   static __device__ int plane_stride(const Params &p) { return p.batch; }
+  // The first chunk of `in` is fetched before the accumulators are there and
+  // each next one before the one in hand is used (passes need the registers).
+  struct Ahead { Chunk in[IN + !IN]; };
+  template <class Tile>
+  static __device__ void look_ahead(const Params &p, const Tile &t, int row, int column, Ahead &early) {
+    if (PASS == 0 && t.extra.row + row < p.rows && t.extra.column + column < p.cols)
+      fetch_in<IN>(p, t.extra.z, t.extra.row + row, t.extra.column + column, early.in);
+  }
   struct Walk {
     __device__ Walk(const Params &) {}
     __device__ bool find(const Params &p, int t, TileOf<Extra> &tile) {
@@ -317,7 +400,7 @@ template <int PAIR_, int NT_, int PLANES_> struct UpdateJob {
   };
   template <class Source>
   static __device__ void epilogue(const Params &p, const TileOf<Extra> &t, const Source &source, int row,
-                                  int column, unsigned char *mine) {
+                                  int column, unsigned char *mine, Ahead &early) {
     const int r0 = t.extra.row + row, rows = p.rows - r0, lane = threadIdx.x % 32;
     if (rows <= 0) return;
 #pragma unroll
@@ -325,12 +408,20 @@ template <int PAIR_, int NT_, int PLANES_> struct UpdateJob {
       const int c0 = t.extra.column + column + c, cols = p.cols - c0;
       if (cols <= 0) continue;
       float v[32];
-      combine(p, source, c, mine, t.extra.z, r0, c0, rows, cols, v);
+      Chunk in[IN + !IN];
+      if constexpr (PASS == 0) {
+#pragma unroll
+        for (int q = 0; q < IN; ++q) in[q] = early.in[q];
+        if (c + 32 < NT / 2 && cols > 32) fetch_in<IN>(p, t.extra.z, r0, c0 + 32, early.in);
+      } else {
+        fetch_in<IN>(p, t.extra.z, r0, c0, in);
+      }
+      combine<IN>(p, source, c, mine, in, v);
       if (!p.last) {
         uint4 high[4], low[4];
         slices_of(v, high, low);
-        store_chunk(mine, p.out.at(0, t.extra.z, r0, c0), p.out.ld, rows, cols, high);
-        store_chunk(mine, p.out.at(1, t.extra.z, r0, c0), p.out.ld, rows, cols, low);
+        store_rows(mine, p.out.at(0, t.extra.z, r0, c0), p.out.ld, rows, cols, high);
+        store_rows(mine, p.out.at(1, t.extra.z, r0, c0), p.out.ld, rows, cols, low);
       } else {
         // the result: through the staging where it is stored along the rows,
         // from the lanes where it is stored across them
@@ -463,7 +554,7 @@ int run(const InitParams &init, const Layout &l, int batch, int steps, const dou
   squares_kernel<<<dim3((unsigned)init.partials, (unsigned)batch), 256, 0, st>>>(init);
   if (int rc = check_cuda(cudaGetLastError(), "squares_kernel launch")) return rc;
   count_launch();
-  normalise_kernel<<<dim3((unsigned)((cols + 31) / 32), (unsigned)((rows + 31) / 32), (unsigned)batch), 256, 0,
+  normalise_kernel<<<dim3((unsigned)((cols + 63) / 64), (unsigned)((rows + 63) / 64), (unsigned)batch), 256, 0,
                      st>>>(init);
   if (int rc = check_cuda(cudaGetLastError(), "normalise_kernel launch")) return rc;
 
@@ -495,21 +586,19 @@ int run(const InitParams &init, const Layout &l, int batch, int steps, const dou
     const double slack = 1 + 1.0 / 64;
     const int es = exponent(most * most * slack), ep = exponent(largest_poly(b, c, most) * slack);
     sym.k = cols;
-    sym.in_planes = 0;
     sym.alpha = 0;
     sym.beta = (float)std::ldexp(1.0, es - 2 * ex);
     sym.out = s;
-    int rc = pair_s ? step_product<SymmetricJob<2, 256, SPLITS>>(xa[cur], xb[cur], sym, true, st)
-                    : step_product<SymmetricJob<1, 64, SPLITS>>(xa[cur], xb[cur], sym, true, st);
+    int rc = pair_s ? step_product<SymmetricJob<2, 256, SPLITS, 0>>(xa[cur], xb[cur], sym, true, st)
+                    : step_product<SymmetricJob<1, 64, SPLITS, 0>>(xa[cur], xb[cur], sym, true, st);
     if (rc) return rc;
     sym.k = rows;
-    sym.in_planes = SPLITS;
     sym.in = s;
     sym.alpha = (float)std::ldexp(b, ep - es);
     sym.beta = (float)std::ldexp(c, ep - 2 * es);
     sym.out = q;
-    rc = pair_s ? step_product<SymmetricJob<2, 256, SPLITS>>(sa, sb, sym, true, st)
-                : step_product<SymmetricJob<1, 64, SPLITS>>(sa, sb, sym, true, st);
+    rc = pair_s ? step_product<SymmetricJob<2, 256, SPLITS, SPLITS>>(sa, sb, sym, true, st)
+                : step_product<SymmetricJob<1, 64, SPLITS, SPLITS>>(sa, sb, sym, true, st);
     if (rc) return rc;
     most = std::min(largest_value(a, b, c, most) * slack, 1e15);
     const bool end = i + 1 == steps;
@@ -521,7 +610,6 @@ int run(const InitParams &init, const Layout &l, int batch, int steps, const dou
     up.rows = rows;
     up.cols = cols;
     up.k = rows;
-    up.in_planes = 2;
     up.in = x[cur];
     up.out = x[cur ^ 1];
     up.alpha = (float)std::ldexp(a, en - ex);
@@ -576,7 +664,11 @@ extern "C" int oz_orthogonalize(const void *g, int dtype, int64_t batch, int64_t
   unsigned char *ws = static_cast<unsigned char *>(workspace);
   const bool tall = m > n;
   const int64_t blocks = (l.rows * l.cols + 4095) / 4096;
-  InitParams init{g, dtype, (int)std::min<int64_t>(blocks, kMostPartials), (int)l.rows, (int)l.cols, g_sb,
+  const int64_t line = std::max(g_sr, g_sc), step = std::min(g_sr, g_sc);
+  const int64_t in_line = g_sr < g_sc ? m : n, per16 = 16 / dtype_size(dtype);
+  const bool vectors = (uintptr_t)g % 16 == 0 && step == 1 && line % per16 == 0 && (batch == 1 || g_sb % per16 == 0);
+  const bool flat = vectors && line == in_line && m * n % 8 == 0;
+  InitParams init{g, dtype, (int)std::min<int64_t>(blocks, kMostPartials), flat, vectors, (int)l.rows, (int)l.cols, g_sb,
                   tall ? g_sc : g_sr, tall ? g_sr : g_sc, reinterpret_cast<double *>(ws),
                   Planes{reinterpret_cast<__half *>(ws + l.x0), pitch(l.cols), l.x_mat, l.x_mat * batch}, eps,
                   std::ldexp(1.0, exponent(1 + 1e-6))};

@@ -52,6 +52,12 @@ constexpr int kStagingBytes = 4096;     // of each epilogue warp: 32 rows of 128
 constexpr int kBarrierBytes = 512;
 constexpr int kSmemLimit = 227 * 1024;
 
+// For jobs whose epilogue reads nothing but the accumulators.
+struct NoLookAhead {
+  struct Ahead {};
+  template <class P, class T> static __device__ void look_ahead(const P &, const T &, int, int, Ahead &) {}
+};
+
 template <class J> __host__ __device__ constexpr int a_bytes() { return kRows * kLine; }
 template <class J> __host__ __device__ constexpr int b_bytes() { return J::NT / J::PAIR * kLine; }
 template <class J> __host__ __device__ constexpr int stage_bytes() { return J::PLANES * (a_bytes<J>() + b_bytes<J>()); }
@@ -478,6 +484,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     for (int i = unit; walk.find(p, i, t); i += units) {
       const int row = (int)rank * kRows + sub * 32, column = half * (NT / 2);
+      typename J::Ahead early;                        // what the epilogue reads besides the accumulators
+      J::look_ahead(p, t, row, column, early);
       if constexpr (J::PASS > 0) {
         float sum[NT / 2];
 #pragma unroll
@@ -499,11 +507,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           hand_back();
         }
         if (!ok) break;
-        J::epilogue(p, t, Registers<NT / 2>{sum}, row, column, mine);
+        J::epilogue(p, t, Registers<NT / 2>{sum}, row, column, mine, early);
       } else {
         const bool some = t.k_len > 0;
         if (some && !acquire()) break;
-        J::epilogue(p, t, Columns{some, columns + (uint32_t)((done & 1) * NT)}, row, column, mine);
+        J::epilogue(p, t, Columns{some, columns + (uint32_t)((done & 1) * NT)}, row, column, mine, early);
         if (some) hand_back();
       }
     }
