@@ -100,7 +100,7 @@ struct RowTile { int row, rows, column; };   // first row, rows from there to th
 
 // y = x w: A is the rows of x, B the columns of w[e].
 template <typename O, int PAIR_, int NT_, bool BMN_> struct RowsJob : NoLookAhead {
-  static constexpr int PAIR = PAIR_, NT = NT_, PLANES = 1, PASS = sizeof(O) == 4 ? 8 : 0;
+  static constexpr int PAIR = PAIR_, NT = NT_, EW = NT_ >= 128 ? 16 : 8, PLANES = 1, PASS = sizeof(O) == 4 ? 8 : 0;
   static constexpr bool AMN = false, BMN = BMN_, RAGGED = false;
   using Params = GroupedParams;
   using Extra = RowTile;
@@ -124,7 +124,7 @@ template <typename O, int PAIR_, int NT_, bool BMN_> struct RowsJob : NoLookAhea
   static __device__ void epilogue(const Params &p, const TileOf<Extra> &t, const Source &source, int row,
                                   int column, unsigned char *mine, Ahead &) {
     const int64_t c0 = t.extra.column + column;
-    write_rows<O, NT / 2>(source, mine,
+    write_rows<O, NT * 4 / EW>(source, mine,
                           static_cast<O *>(p.out) + (int64_t)(t.extra.row + row) * p.ld + c0, p.ld,
                           t.extra.rows - row, p.n - c0, p.vectors);
   }
@@ -135,7 +135,7 @@ template <typename O, int PAIR_, int NT_, bool BMN_> struct RowsJob : NoLookAhea
 // 128 columns of w[e], B up to NT rows of x, so a tile's weights are read
 // once and hardly any of the staged bytes belong to rows that are not there.
 template <typename O, int NT_, bool AMN_> struct ColumnsJob : NoLookAhead {
-  static constexpr int PAIR = 1, NT = NT_, PLANES = 1, PASS = sizeof(O) == 4 ? 8 : 0;
+  static constexpr int PAIR = 1, NT = NT_, EW = 8, PLANES = 1, PASS = sizeof(O) == 4 ? 8 : 0;
   static constexpr bool AMN = AMN_, BMN = false, RAGGED = false;
   using Params = GroupedParams;
   using Extra = RowTile;
@@ -179,7 +179,7 @@ struct WeightTile { int row, column, group; };
 // dw[e] = x^T dy over the group's rows: both operands are stored across the
 // contraction, whose range is the group.
 template <typename O, int PAIR_, int NT_> struct WeightsJob : NoLookAhead {
-  static constexpr int PAIR = PAIR_, NT = NT_, PLANES = 1, PASS = sizeof(O) == 4 ? 8 : 0;
+  static constexpr int PAIR = PAIR_, NT = NT_, EW = NT_ >= 128 ? 16 : 8, PLANES = 1, PASS = sizeof(O) == 4 ? 8 : 0;
   static constexpr bool AMN = true, BMN = true, RAGGED = true;
   using Params = GroupedParams;
   using Extra = WeightTile;
@@ -210,7 +210,7 @@ template <typename O, int PAIR_, int NT_> struct WeightsJob : NoLookAhead {
   static __device__ void epilogue(const Params &p, const TileOf<Extra> &t, const Source &source, int row,
                                   int column, unsigned char *mine, Ahead &) {
     const int64_t r0 = t.extra.row + row, c0 = t.extra.column + column;
-    write_rows<O, NT / 2>(source, mine,
+    write_rows<O, NT * 4 / EW>(source, mine,
                           static_cast<O *>(p.out) + ((int64_t)t.extra.group * p.k + r0) * p.ld + c0,
                           p.ld, (int)(p.k - r0), p.n - c0, p.vectors);
   }

@@ -12,11 +12,10 @@
 // step by step (the singular values start in [0, 1] and a step's polynomial
 // is known), so e puts the bound at 2^15 and nothing can overflow; no data
 // is looked at.  With one slice the products use `high` alone (11 bits) and
-// only the term a X keeps X's 22: that term carries the directions that the
-// products hardly touch, and rounding it as well as P X makes both sides of
-// the sum consistent only for full-rank G (measured on a low-rank gradient:
-// 2.2e-2 with 11 bits there, 4.5e-4 with 22).  With two slices the products add
-// high*high + high*low + low*high.  S and P are symmetric: only the tiles on
+// only the term a X keeps an fp32 X: that term carries the directions that
+// the products hardly touch (in a model of the roundings on a low-rank gradient
+// the result is 2.2e-2 off with 11 bits there, 4.5e-4 with 22 or more).  With two
+// slices the products add high*high + high*low + low*high.  S and P are symmetric: only the tiles on
 // and below the diagonal are multiplied, each written twice.
 
 #include <algorithm>
@@ -55,6 +54,7 @@ struct InitParams {
   int64_t g_sb, g_sr, g_sc;         // strides of G's member, and of X's rows and columns in G
   double *partial;                  // (batch, partials) sums of squares
   Planes x;
+  float *x32;                       // with one slice: X in fp32 beside it, same pitches
   double eps, scale;
 };
 
@@ -172,7 +172,13 @@ __global__ void __launch_bounds__(256) normalise_kernel(const InitParams p) {
       low[x] = pack2<__half>(a - f.x, b - f.y);
     }
     *reinterpret_cast<uint4 *>(p.x.at(0, blockIdx.z, r0 + r, c0 + u)) = make_uint4(high[0], high[1], high[2], high[3]);
-    *reinterpret_cast<uint4 *>(p.x.at(1, blockIdx.z, r0 + r, c0 + u)) = make_uint4(low[0], low[1], low[2], low[3]);
+    if (p.x32) {
+      float4 *x32 = reinterpret_cast<float4 *>(p.x32 + blockIdx.z * p.x.mat + (r0 + r) * p.x.ld + c0 + u);
+      x32[0] = make_float4(tile[r][u], tile[r][u + 1], tile[r][u + 2], tile[r][u + 3]);
+      x32[1] = make_float4(tile[r][u + 4], tile[r][u + 5], tile[r][u + 6], tile[r][u + 7]);
+    } else {
+      *reinterpret_cast<uint4 *>(p.x.at(1, blockIdx.z, r0 + r, c0 + u)) = make_uint4(low[0], low[1], low[2], low[3]);
+    }
   }
 }
 
@@ -182,115 +188,113 @@ struct StepParams {
   int row_tiles, column_tiles, tiles;   // tiles of one member
   float alpha, beta;                // result = alpha * in + beta * accumulator
   Planes in, out;
+  const float *in32;                // with one slice the update reads and writes X in fp32,
+  float *out32;                     // with the pitches of `in` and `out`
   // the last step's result instead of `out`: element (z, r, c) of the type
   void *last;
   int last_dtype;
   int64_t last_sb, last_sr, last_sc;
 };
 
-// 32 rows x 32 fp16 columns: each lane 4 pieces of 8 columns, 64 bytes of a
-// row by 4 lanes; the warp's staging turns them into each lane's own row.
-struct Chunk { uint4 piece[4]; };
-
-__device__ __forceinline__ uint4 *chunk_slot(unsigned char *mine, int r, int u) {
-  return reinterpret_cast<uint4 *>(mine + r * 64 + ((u ^ ((r >> 1) & 3)) << 4));
+// 32 bytes of a lane's row at a time: a whole sector, so that the lanes of a
+// warp can each read and write their own row without staging.
+__device__ __forceinline__ void load32(const void *p, uint32_t *v) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+               : "l"(p));
 }
-__device__ __forceinline__ void fetch(const __half *src, int64_t ld, int rows, int cols, Chunk &v) {
-  const int lane = threadIdx.x % 32;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = i * 8 + lane / 4, u = lane % 4;
-    v.piece[i] = r < rows && u * 8 < cols ? *reinterpret_cast<const uint4 *>(src + r * ld + u * 8)
-                                          : make_uint4(0, 0, 0, 0);
-  }
-}
-__device__ __forceinline__ void to_rows(unsigned char *mine, Chunk &v) {
-  const int lane = threadIdx.x % 32;
-  __syncwarp();
-#pragma unroll
-  for (int i = 0; i < 4; ++i) *chunk_slot(mine, i * 8 + lane / 4, lane % 4) = v.piece[i];
-  __syncwarp();
-#pragma unroll
-  for (int u = 0; u < 4; ++u) v.piece[u] = *chunk_slot(mine, lane, u);
+__device__ __forceinline__ void store32(void *p, const uint32_t *v) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
 }
 
-// The way back: the chunk in the staging to memory.
-__device__ __forceinline__ void flush(unsigned char *mine, __half *dst, int64_t ld, int rows, int cols) {
-  const int lane = threadIdx.x % 32;
-  __syncwarp();
+// WORDS words of the lane's row (fp16 pairs or fp32), the pieces that begin
+// before column `cols`; rows are padded to whole pieces.
+template <int WORDS, int PER>
+__device__ __forceinline__ void load_row(const void *p, int cols, uint32_t (&v)[WORDS]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = i * 8 + lane / 4, u = lane % 4;
-    if (r < rows && u * 8 < cols) *reinterpret_cast<uint4 *>(dst + r * ld + u * 8) = *chunk_slot(mine, r, u);
+  for (int i = 0; i < WORDS; i += 8) {
+    if (i * PER < cols) {
+      load32(static_cast<const uint32_t *>(p) + i, v + i);
+    } else {
+#pragma unroll
+      for (int x = 0; x < 8; ++x) v[i + x] = 0;
+    }
   }
-  __syncwarp();
 }
-// From each lane's row; and its mirror image, from each lane's column.
-__device__ __forceinline__ void store_rows(unsigned char *mine, __half *dst, int64_t ld, int rows, int cols,
-                                           const uint4 (&v)[4]) {
-  __syncwarp();
+template <int WORDS, int PER>
+__device__ __forceinline__ void store_row(void *p, int cols, const uint32_t (&v)[WORDS]) {
 #pragma unroll
-  for (int u = 0; u < 4; ++u) *chunk_slot(mine, threadIdx.x % 32, u) = v[u];
-  flush(mine, dst, ld, rows, cols);
+  for (int i = 0; i < WORDS; i += 8)
+    if (i * PER < cols) store32(static_cast<uint32_t *>(p) + i, v + i);
 }
+
+// The mirror image of 32 fp16 columns of each lane's row: the lanes' rows are
+// columns there, so the staging turns them, 64 bytes of a row by 4 lanes.
 __device__ __forceinline__ void store_columns(unsigned char *mine, __half *dst, int64_t ld, int rows, int cols,
-                                              const uint4 (&v)[4]) {
+                                              const uint32_t (&v)[16]) {
   const int lane = threadIdx.x % 32;
-  const __half *h = reinterpret_cast<const __half *>(&v[0]);
 #pragma unroll
-  for (int x = 0; x < 32; ++x) reinterpret_cast<__half *>(chunk_slot(mine, x, lane / 8))[lane % 8] = h[x];
-  flush(mine, dst, ld, rows, cols);
-}
-
-// The part of `in` under chunk c of the warp's columns, IN slices.
-template <int IN>
-__device__ __forceinline__ void fetch_in(const StepParams &p, int z, int row, int column, Chunk (&v)[IN + !IN]) {
+  for (int x = 0; x < 32; ++x)
+    reinterpret_cast<unsigned short *>(staged(mine, x, lane / 8))[lane % 8] =
+        (unsigned short)(x % 2 ? v[x / 2] >> 16 : v[x / 2]);
+  __half *to = dst + (lane / 4) * ld + (lane % 4) * 8;
+  __syncwarp();
+  if (rows >= 32 && cols >= 32) {
 #pragma unroll
-  for (int q = 0; q < IN; ++q)
-    fetch(p.in.at(q, z, row, column), p.in.ld, p.rows - row, p.cols - column, v[q]);
-}
-
-// alpha * in + beta * accumulator for 32 columns of the lane's row.
-template <int IN, class Source>
-__device__ __forceinline__ void combine(const StepParams &p, const Source &source, int c, unsigned char *mine,
-                                        Chunk (&in)[IN + !IN], float (&v)[32]) {
+    for (int i = 0; i < 4; ++i)
+      *reinterpret_cast<uint4 *>(to + i * 8 * ld) = *staged(mine, i * 8 + lane / 4, lane % 4);
+  } else {
 #pragma unroll
-  for (int h = 0; h < 32; h += 16) {
-    float acc[16];
-    source.read(c + h, acc);
-#pragma unroll
-    for (int x = 0; x < 16; ++x) v[h + x] = p.beta * acc[x];
+    for (int i = 0; i < 4; ++i)
+      if (i * 8 + lane / 4 < rows && lane % 4 * 8 < cols)
+        *reinterpret_cast<uint4 *>(to + i * 8 * ld) = *staged(mine, i * 8 + lane / 4, lane % 4);
   }
+  __syncwarp();
+}
+
+// What the epilogue adds to the accumulators: IN slices of `in` (0: nothing), or
+// `in32` (IN = -1), 32 columns of the lane's row.
+template <int IN> struct Addend {
+  static constexpr int kSlices = IN < 0 ? 0 : IN, kWords = IN < 0 ? 32 : IN == 0 ? 1 : 16 * IN;
+  uint32_t w[kWords];
+  __device__ __forceinline__ void fetch(const StepParams &p, int z, int row, int column) {
+    const int r = row + threadIdx.x % 32, cols = p.cols - column;
+    if constexpr (IN < 0) {
+      if (r < p.rows) load_row<32, 1>(p.in32 + z * p.in.mat + r * p.in.ld + column, cols, w);
+    } else if constexpr (IN > 0) {
 #pragma unroll
-  for (int q = 0; q < IN; ++q) {
-    to_rows(mine, in[q]);
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const __half2 *h = reinterpret_cast<const __half2 *>(&in[q].piece[u]);
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const float2 f = __half22float2(h[x]);
-        v[u * 8 + x * 2] += p.alpha * f.x;
-        v[u * 8 + x * 2 + 1] += p.alpha * f.y;
-      }
+      for (int q = 0; q < IN; ++q)
+        if (r < p.rows)
+          load_row<16, 2>(p.in.at(q, z, r, column), cols, *reinterpret_cast<uint32_t(*)[16]>(w + q * 16));
     }
   }
-}
-
-__device__ __forceinline__ void slices_of(const float (&v)[32], uint4 (&high)[4], uint4 (&low)[4]) {
+  __device__ __forceinline__ void add(float alpha, float (&v)[32]) const {
+    if constexpr (IN < 0) {
 #pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    uint32_t h[4], l[4];
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const float a = v[u * 8 + x * 2], b = v[u * 8 + x * 2 + 1];
-      const __half2 hh = __floats2half2_rn(a, b);
-      const float2 f = __half22float2(hh);
-      h[x] = *reinterpret_cast<const uint32_t *>(&hh);
-      l[x] = pack2<__half>(a - f.x, b - f.y);
+      for (int x = 0; x < 32; ++x) v[x] += alpha * __uint_as_float(w[x]);
     }
-    high[u] = make_uint4(h[0], h[1], h[2], h[3]);
-    low[u] = make_uint4(l[0], l[1], l[2], l[3]);
+#pragma unroll
+    for (int i = 0; i < 16 * kSlices; ++i) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+      v[i % 16 * 2] += alpha * f.x;
+      v[i % 16 * 2 + 1] += alpha * f.y;
+    }
+  }
+};
+
+// The slices of 32 values, as pairs.
+template <bool LOW>
+__device__ __forceinline__ void slices_of(const float (&v)[32], uint32_t (&high)[16], uint32_t (&low)[16]) {
+#pragma unroll
+  for (int x = 0; x < 16; ++x) {
+    const __half2 h = __floats2half2_rn(v[2 * x], v[2 * x + 1]);
+    high[x] = *reinterpret_cast<const uint32_t *>(&h);
+    if constexpr (LOW) {
+      const float2 f = __half22float2(h);
+      low[x] = pack2<__half>(v[2 * x] - f.x, v[2 * x + 1] - f.y);
+    }
   }
 }
 
@@ -299,19 +303,38 @@ struct StepTile { int z, row, column; bool mirror; };
 // S = X X^T (IN 0) and P = b S + c S S (IN slices of S): tiles (i, j) on and
 // below the diagonal, the others their mirror images.
 template <int PAIR_, int NT_, int PLANES_, int IN> struct SymmetricJob {
-  static constexpr int PAIR = PAIR_, NT = NT_, PLANES = PLANES_, PASS = (PLANES_ - 1) * 4;
+  static constexpr int PAIR = PAIR_, NT = NT_, EW = NT_ >= 128 ? 16 : 8, PLANES = PLANES_, PASS = (PLANES_ - 1) * 4;
   static constexpr bool AMN = false, BMN = false, RAGGED = false;
   static constexpr int R = kRows * PAIR / NT;           // column tiles as wide as a tile is high
   using Params = StepParams;
   using Extra = StepTile;
   static __device__ int plane_stride(const Params &p) { return p.batch; }
-  // The first chunk of `in` is fetched before the accumulators are there and
-  // each next one before the one in hand is used (passes need the registers).
-  struct Ahead { Chunk in[IN + !IN]; };
+  // The first columns of `in` are fetched before the accumulators are there and
+  // each next ones before those in hand are used (passes need the registers).
+  struct Ahead { Addend<IN> in; };
   template <class Tile>
   static __device__ void look_ahead(const Params &p, const Tile &t, int row, int column, Ahead &early) {
     if (PASS == 0 && t.extra.row + row < p.rows && t.extra.column + column < p.cols)
-      fetch_in<IN>(p, t.extra.z, t.extra.row + row, t.extra.column + column, early.in);
+      early.in.fetch(p, t.extra.z, t.extra.row + row, t.extra.column + column);
+  }
+  template <class Source>
+  static __device__ __forceinline__ void values(const Params &p, const TileOf<Extra> &t, const Source &source, int c,
+                                                int r0, int c0, Ahead &early, float (&v)[32]) {
+    Addend<IN> in;
+    if constexpr (PASS == 0) {
+      in = early.in;
+      if (c + 32 < NT * 4 / EW && c0 + 32 < p.cols) early.in.fetch(p, t.extra.z, r0, c0 + 32);
+    } else {
+      in.fetch(p, t.extra.z, r0, c0);
+    }
+#pragma unroll
+    for (int h = 0; h < 32; h += 16) {
+      float acc[16];
+      source.read(c + h, acc);
+#pragma unroll
+      for (int x = 0; x < 16; ++x) v[h + x] = p.beta * acc[x];
+    }
+    in.add(p.alpha, v);
   }
   struct Walk {
     __device__ Walk(const Params &) {}
@@ -335,27 +358,18 @@ template <int PAIR_, int NT_, int PLANES_, int IN> struct SymmetricJob {
   template <class Source>
   static __device__ void epilogue(const Params &p, const TileOf<Extra> &t, const Source &source, int row,
                                   int column, unsigned char *mine, Ahead &early) {
-    const int r0 = t.extra.row + row, rows = p.rows - r0;
+    const int r0 = t.extra.row + row, rows = p.rows - r0, lane = threadIdx.x % 32;
     if (rows <= 0) return;
 #pragma unroll
-    for (int c = 0; c < NT / 2; c += 32) {
+    for (int c = 0; c < NT * 4 / EW; c += 32) {
       const int c0 = t.extra.column + column + c, cols = p.cols - c0;
       if (cols <= 0) continue;
       float v[32];
-      Chunk in[IN + !IN];
-      if constexpr (PASS == 0) {
-#pragma unroll
-        for (int q = 0; q < IN; ++q) in[q] = early.in[q];
-        if (c + 32 < NT / 2 && cols > 32) fetch_in<IN>(p, t.extra.z, r0, c0 + 32, early.in);
-      } else {
-        fetch_in<IN>(p, t.extra.z, r0, c0, in);
-      }
-      combine<IN>(p, source, c, mine, in, v);
-      uint4 high[4], low[4];
-      slices_of(v, high, low);
-      store_rows(mine, p.out.at(0, t.extra.z, r0, c0), p.out.ld, rows, cols, high);
-      if constexpr (PLANES == 2)
-        store_rows(mine, p.out.at(1, t.extra.z, r0, c0), p.out.ld, rows, cols, low);
+      values(p, t, source, c, r0, c0, early, v);
+      uint32_t high[16], low[16];
+      slices_of<PLANES == 2>(v, high, low);
+      if (lane < rows) store_row<16, 2>(p.out.at(0, t.extra.z, r0 + lane, c0), cols, high);
+      if (PLANES == 2 && lane < rows) store_row<16, 2>(p.out.at(1, t.extra.z, r0 + lane, c0), cols, low);
       if (t.extra.mirror) {
         store_columns(mine, p.out.at(0, t.extra.z, c0, r0), p.out.ld, cols, rows, high);
         if constexpr (PLANES == 2)
@@ -368,19 +382,38 @@ template <int PAIR_, int NT_, int PLANES_, int IN> struct SymmetricJob {
 
 // X <- a X + P X: A is the rows of P, B the columns of X.
 template <int PAIR_, int NT_, int PLANES_> struct UpdateJob {
-  static constexpr int IN = 2;
-  static constexpr int PAIR = PAIR_, NT = NT_, PLANES = PLANES_, PASS = (PLANES_ - 1) * 4;
+  static constexpr int IN = PLANES_ == 2 ? 2 : -1;
+  static constexpr int PAIR = PAIR_, NT = NT_, EW = NT_ >= 128 ? 16 : 8, PLANES = PLANES_, PASS = (PLANES_ - 1) * 4;
   static constexpr bool AMN = false, BMN = true, RAGGED = false;
   using Params = StepParams;
   using Extra = StepTile;
   static __device__ int plane_stride(const Params &p) { return p.batch; }
-  // The first chunk of `in` is fetched before the accumulators are there and
-  // each next one before the one in hand is used (passes need the registers).
-  struct Ahead { Chunk in[IN + !IN]; };
+  // The first columns of `in` are fetched before the accumulators are there and
+  // each next ones before those in hand are used (passes need the registers).
+  struct Ahead { Addend<IN> in; };
   template <class Tile>
   static __device__ void look_ahead(const Params &p, const Tile &t, int row, int column, Ahead &early) {
     if (PASS == 0 && t.extra.row + row < p.rows && t.extra.column + column < p.cols)
-      fetch_in<IN>(p, t.extra.z, t.extra.row + row, t.extra.column + column, early.in);
+      early.in.fetch(p, t.extra.z, t.extra.row + row, t.extra.column + column);
+  }
+  template <class Source>
+  static __device__ __forceinline__ void values(const Params &p, const TileOf<Extra> &t, const Source &source, int c,
+                                                int r0, int c0, Ahead &early, float (&v)[32]) {
+    Addend<IN> in;
+    if constexpr (PASS == 0) {
+      in = early.in;
+      if (c + 32 < NT * 4 / EW && c0 + 32 < p.cols) early.in.fetch(p, t.extra.z, r0, c0 + 32);
+    } else {
+      in.fetch(p, t.extra.z, r0, c0);
+    }
+#pragma unroll
+    for (int h = 0; h < 32; h += 16) {
+      float acc[16];
+      source.read(c + h, acc);
+#pragma unroll
+      for (int x = 0; x < 16; ++x) v[h + x] = p.beta * acc[x];
+    }
+    in.add(p.alpha, v);
   }
   struct Walk {
     __device__ Walk(const Params &) {}
@@ -404,24 +437,22 @@ template <int PAIR_, int NT_, int PLANES_> struct UpdateJob {
     const int r0 = t.extra.row + row, rows = p.rows - r0, lane = threadIdx.x % 32;
     if (rows <= 0) return;
 #pragma unroll
-    for (int c = 0; c < NT / 2; c += 32) {
+    for (int c = 0; c < NT * 4 / EW; c += 32) {
       const int c0 = t.extra.column + column + c, cols = p.cols - c0;
       if (cols <= 0) continue;
       float v[32];
-      Chunk in[IN + !IN];
-      if constexpr (PASS == 0) {
-#pragma unroll
-        for (int q = 0; q < IN; ++q) in[q] = early.in[q];
-        if (c + 32 < NT / 2 && cols > 32) fetch_in<IN>(p, t.extra.z, r0, c0 + 32, early.in);
-      } else {
-        fetch_in<IN>(p, t.extra.z, r0, c0, in);
-      }
-      combine<IN>(p, source, c, mine, in, v);
+      values(p, t, source, c, r0, c0, early, v);
       if (!p.last) {
-        uint4 high[4], low[4];
-        slices_of(v, high, low);
-        store_rows(mine, p.out.at(0, t.extra.z, r0, c0), p.out.ld, rows, cols, high);
-        store_rows(mine, p.out.at(1, t.extra.z, r0, c0), p.out.ld, rows, cols, low);
+        uint32_t high[16], low[16];
+        slices_of<PLANES == 2>(v, high, low);
+        if (lane < rows) {
+          store_row<16, 2>(p.out.at(0, t.extra.z, r0 + lane, c0), cols, high);
+          if constexpr (PLANES == 2)
+            store_row<16, 2>(p.out.at(1, t.extra.z, r0 + lane, c0), cols, low);
+          else
+            store_row<32, 1>(p.out32 + t.extra.z * p.out.mat + (r0 + lane) * p.out.ld + c0, cols,
+                             *reinterpret_cast<const uint32_t(*)[32]>(v));
+        }
       } else {
         // the result: through the staging where it is stored along the rows,
         // from the lanes where it is stored across them
@@ -443,18 +474,22 @@ template <int PAIR_, int NT_, int PLANES_> struct UpdateJob {
               }
           }
         } else {
-          __syncwarp();
 #pragma unroll
-          for (int u = 0; u < 8; ++u)
-            *staged(mine, lane, u) = *reinterpret_cast<const uint4 *>(&v[u * 4]);
-          __syncwarp();
+          for (int h = 0; h < 32; h += 16) {
+            __syncwarp();
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              *staged(mine, lane, u) = *reinterpret_cast<const uint4 *>(&v[h + u * 4]);
+            __syncwarp();
 #pragma unroll 4
-          for (int r = 0; r < 32; ++r)
-            if (r < rows && lane < cols) {
-              const float f = reinterpret_cast<const float *>(staged(mine, r, lane / 4))[lane % 4];
-              if (wide) out32[r * p.last_sr + lane] = f;
-              else out16[r * p.last_sr + lane] = bits(f);
-            }
+            for (int r = lane / 16; r < 32; r += 2)
+              if (r < rows && h + lane % 16 < cols) {
+                const float f = reinterpret_cast<const float *>(staged(mine, r, lane % 16 / 4))[lane % 4];
+                const int64_t to = r * p.last_sr + h + lane % 16;
+                if (wide) out32[to] = f;
+                else out16[to] = bits(f);
+              }
+          }
         }
       }
     }
@@ -463,11 +498,12 @@ template <int PAIR_, int NT_, int PLANES_> struct UpdateJob {
 };
 
 int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
-int64_t pitch(int64_t n) { return (n + 7) / 8 * 8; }
+int64_t pitch(int64_t n) { return (n + 15) / 16 * 16; }   // rows of whole 32-byte pieces
 
-// Workspace of a call: sums of squares, two X's, S and P in slices.
+// Workspace of a call: sums of squares, two X's (two slices, or one and fp32), S
+// and P in slices.
 struct Layout {
-  int64_t rows, cols, x_mat, s_mat, x0, x1, s, p, total;
+  int64_t rows, cols, x_mat, s_mat, x0, x1, x32, s, p, total;   // x32: from an X's slice to its fp32
 };
 Layout layout(int64_t batch, int64_t m, int64_t n, int splits) {
   Layout l{};
@@ -476,7 +512,8 @@ Layout layout(int64_t batch, int64_t m, int64_t n, int splits) {
   l.x_mat = l.rows * pitch(l.cols);
   l.s_mat = l.rows * pitch(l.rows);
   int64_t at = align256(batch * kMostPartials * 8);
-  const int64_t x = align256(2 * batch * l.x_mat * 2), s = align256(splits * batch * l.s_mat * 2);
+  l.x32 = splits == 1 ? align256(batch * l.x_mat * 2) : 0;
+  const int64_t x = l.x32 + align256(batch * l.x_mat * 4), s = align256(splits * batch * l.s_mat * 2);
   l.x0 = at;
   l.x1 = l.x0 + x;
   l.s = l.x1 + x;
@@ -566,9 +603,9 @@ int run(const InitParams &init, const Layout &l, int batch, int steps, const dou
   };
   CUtensorMap xa[2], xb[2], xu[2], sa, sb, pa;
   for (int i = 0; i < 2; ++i) {
-    if (int rc = map(&xa[i], x[i], cols, 2, kRows)) return rc;
-    if (int rc = map(&xb[i], x[i], cols, 2, pair_s ? 128 : 64)) return rc;
-    if (int rc = map(&xu[i], x[i], cols, 2, kBlock)) return rc;
+    if (int rc = map(&xa[i], x[i], cols, SPLITS, kRows)) return rc;
+    if (int rc = map(&xb[i], x[i], cols, SPLITS, pair_s ? 128 : 64)) return rc;
+    if (int rc = map(&xu[i], x[i], cols, SPLITS, kBlock)) return rc;
   }
   if (int rc = map(&sa, s, rows, SPLITS, kRows)) return rc;
   if (int rc = map(&sb, s, rows, SPLITS, pair_s ? 128 : 64)) return rc;
@@ -612,6 +649,10 @@ int run(const InitParams &init, const Layout &l, int batch, int steps, const dou
     up.k = rows;
     up.in = x[cur];
     up.out = x[cur ^ 1];
+    if (SPLITS == 1) {
+      up.in32 = reinterpret_cast<const float *>(ws + (cur ? l.x1 : l.x0) + l.x32);
+      up.out32 = reinterpret_cast<float *>(ws + (cur ? l.x0 : l.x1) + l.x32);
+    }
     up.alpha = (float)std::ldexp(a, en - ex);
     up.beta = (float)std::ldexp(1.0, en - ep - ex);
     rc = pair_x ? step_product<UpdateJob<2, 256, SPLITS>>(pa, xu[cur], up, false, st)
@@ -670,7 +711,8 @@ extern "C" int oz_orthogonalize(const void *g, int dtype, int64_t batch, int64_t
   const bool flat = vectors && line == in_line && m * n % 8 == 0;
   InitParams init{g, dtype, (int)std::min<int64_t>(blocks, kMostPartials), flat, vectors, (int)l.rows, (int)l.cols, g_sb,
                   tall ? g_sc : g_sr, tall ? g_sr : g_sc, reinterpret_cast<double *>(ws),
-                  Planes{reinterpret_cast<__half *>(ws + l.x0), pitch(l.cols), l.x_mat, l.x_mat * batch}, eps,
+                  Planes{reinterpret_cast<__half *>(ws + l.x0), pitch(l.cols), l.x_mat, l.x_mat * batch},
+                  num_splits == 1 ? reinterpret_cast<float *>(ws + l.x0 + l.x32) : nullptr, eps,
                   std::ldexp(1.0, exponent(1 + 1e-6))};
   StepParams last{};
   last.last = out;

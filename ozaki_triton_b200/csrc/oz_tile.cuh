@@ -6,8 +6,11 @@
 // moves the data and issues the matrix instructions:
 //   warp 0     TMA producer: 64-deep blocks of A and B into a ring of stages;
 //   warp 1     TMEM allocator and the one thread that issues tcgen05.mma;
-//   warps 2-9  epilogue: the job's, from TMEM (fp32 accumulators, two buffers,
+//   warps 2..  epilogue: the job's, from TMEM (fp32 accumulators, two buffers,
 //              so the epilogue of one tile runs under the products of the next).
+//              EW = 8 or 16 warps: a warp's epilogue is one chain of dependent
+//              steps, so more warps shorten it until it hides (the update of
+//              2048 x 2816 took 27,000 cycles a tile with 8, its products 16,400).
 // A tile is 128 * PAIR rows by NT columns; with PAIR = 2 two CTAs of a
 // cluster hold half of A's rows and half of B's columns each and one
 // cta_group::2 instruction multiplies both halves: each CTA then feeds 256
@@ -46,9 +49,7 @@ constexpr int kRows = 128;              // rows of one CTA's part of a tile
 constexpr int kBlock = 64;              // contraction elements of a stage
 constexpr int kLine = 128;              // bytes of a swizzled row
 constexpr int kMaxStages = 10;
-constexpr int kEpilogueWarps = 8;
-constexpr int kThreads = 64 + 32 * kEpilogueWarps;
-constexpr int kStagingBytes = 4096;     // of each epilogue warp: 32 rows of 128 bytes
+constexpr int kStagingBytes = 2048;     // of each epilogue warp: 32 rows of 64 bytes
 constexpr int kBarrierBytes = 512;
 constexpr int kSmemLimit = 227 * 1024;
 
@@ -58,16 +59,19 @@ struct NoLookAhead {
   template <class P, class T> static __device__ void look_ahead(const P &, const T &, int, int, Ahead &) {}
 };
 
+template <class J> __host__ __device__ constexpr int threads() { return 64 + 32 * J::EW; }
+// columns of an epilogue warp (4 warps share the rows of a tile, a quarter each)
+template <class J> __host__ __device__ constexpr int warp_columns() { return J::NT * 4 / J::EW; }
 template <class J> __host__ __device__ constexpr int a_bytes() { return kRows * kLine; }
 template <class J> __host__ __device__ constexpr int b_bytes() { return J::NT / J::PAIR * kLine; }
 template <class J> __host__ __device__ constexpr int stage_bytes() { return J::PLANES * (a_bytes<J>() + b_bytes<J>()); }
 template <class J> __host__ __device__ constexpr int stages() {
-  constexpr int room = kSmemLimit - 1024 - kBarrierBytes - kEpilogueWarps * kStagingBytes;
+  constexpr int room = kSmemLimit - 1024 - kBarrierBytes - J::EW * kStagingBytes;
   constexpr int n = room / stage_bytes<J>();
   return n < kMaxStages ? n : kMaxStages;
 }
 template <class J> __host__ __device__ constexpr int smem_bytes() {
-  return 1024 + stages<J>() * stage_bytes<J>() + kEpilogueWarps * kStagingBytes + kBarrierBytes;
+  return 1024 + stages<J>() * stage_bytes<J>() + J::EW * kStagingBytes + kBarrierBytes;
 }
 
 // Where a tile's operands lie: first row (or column) and matrix of A and B in
@@ -162,7 +166,7 @@ __device__ __forceinline__ bool wait_cluster(uint64_t *bar, uint32_t parity, vol
 }
 
 // Where an epilogue finds its warp's accumulators, 32 rows (one a lane) by
-// NT / 2 columns, 16 columns at a time: in TMEM (zeros for an empty
+// its columns, 16 at a time: in TMEM (zeros for an empty
 // contraction), or summed over the passes in registers.
 struct Columns {
   bool some;
@@ -188,8 +192,15 @@ template <int N> struct Registers {
   }
 };
 
+// Tell the pair's leader that this warp has read its accumulators.  No memory is
+// handed over (TMEM is ordered by the tcgen05 fence before), so the arrival is not
+// a release over the cluster, which would wait for the warp's stores to land.
+__device__ __forceinline__ void arrive_at_leader(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
 template <class J>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(threads<J>(), 1)
     tile_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                 const typename J::Params p) {
   using Tile = TileOf<typename J::Extra>;
@@ -203,7 +214,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ unsigned char smem_raw[];
   unsigned char *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   unsigned char *staging = smem + S * SB;
-  uint64_t *full = reinterpret_cast<uint64_t *>(staging + kEpilogueWarps * kStagingBytes);
+  uint64_t *full = reinterpret_cast<uint64_t *>(staging + J::EW * kStagingBytes);
   uint64_t *empty = full + kMaxStages;
   uint64_t *acc_full = empty + kMaxStages;            // [2]
   uint64_t *acc_empty = acc_full + 2;                 // [2]
@@ -227,7 +238,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], PAIR * kEpilogueWarps);
+      mbar_init(&acc_empty[i], PAIR * J::EW);
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -460,9 +471,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     // ------------------------------------------------------------ epilogue
-    const int sub = warp & 3, half = (warp - 2) >> 2;
+    constexpr int CW = warp_columns<J>();
+    const int sub = warp & 3, part = (warp - 2) >> 2;
     unsigned char *mine = staging + (warp - 2) * kStagingBytes;
-    const uint32_t columns = tmem + ((uint32_t)(sub * 32) << 16) + (uint32_t)(half * (NT / 2));
+    const uint32_t columns = tmem + ((uint32_t)(sub * 32) << 16) + (uint32_t)(part * CW);
     typename J::Walk walk(p);
     Tile t;
     uint32_t done = 0;
@@ -478,36 +490,34 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) {
         if (leader) mbar_arrive(&acc_empty[done & 1]);
-        else mbar_arrive_remote(leader_addr(&acc_empty[done & 1]));
+        else arrive_at_leader(leader_addr(&acc_empty[done & 1]));
       }
       ++done;
     };
     for (int i = unit; walk.find(p, i, t); i += units) {
-      const int row = (int)rank * kRows + sub * 32, column = half * (NT / 2);
+      const int row = (int)rank * kRows + sub * 32, column = part * CW;
       typename J::Ahead early;                        // what the epilogue reads besides the accumulators
       J::look_ahead(p, t, row, column, early);
       if constexpr (J::PASS > 0) {
-        float sum[NT / 2];
+        float sum[CW];
 #pragma unroll
-        for (int c = 0; c < NT / 2; ++c) sum[c] = 0.f;
+        for (int c = 0; c < CW; ++c) sum[c] = 0.f;
         const int blocks = (int)((t.k_len + kBlock - 1) / kBlock);
         bool ok = true;
         for (int kb = 0; ok && kb < blocks; kb += J::PASS) {
           if (!(ok = acquire())) break;
 #pragma unroll
-          for (int c = 0; c < NT / 2; c += 32) {
-            uint32_t r[32];
+          for (int c = 0; c < CW; c += 16) {
+            uint32_t r[16];
             tmem_ld16_at(columns + (uint32_t)((done & 1) * NT + c), r);
-            tmem_ld16_at(columns + (uint32_t)((done & 1) * NT + c + 16), r + 16);
-            tmem_ld_wait16(*reinterpret_cast<uint32_t(*)[16]>(r));
-            tmem_ld_wait16(*reinterpret_cast<uint32_t(*)[16]>(r + 16));
+            tmem_ld_wait16(r);
 #pragma unroll
-            for (int x = 0; x < 32; ++x) sum[c + x] += __uint_as_float(r[x]);
+            for (int x = 0; x < 16; ++x) sum[c + x] += __uint_as_float(r[x]);
           }
           hand_back();
         }
         if (!ok) break;
-        J::epilogue(p, t, Registers<NT / 2>{sum}, row, column, mine, early);
+        J::epilogue(p, t, Registers<CW>{sum}, row, column, mine, early);
       } else {
         const bool some = t.k_len > 0;
         if (some && !acquire()) break;
@@ -515,7 +525,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (some) hand_back();
       }
     }
-    J::finish(p, (blockIdx.x * kEpilogueWarps + warp - 2), gridDim.x * kEpilogueWarps);
+    J::finish(p, (blockIdx.x * J::EW + warp - 2), gridDim.x * J::EW);
   }
 
   tc_fence_before();
@@ -538,7 +548,7 @@ int launch(const CUtensorMap &a, const CUtensorMap &b, const typename J::Params 
   const int64_t most = sm_count() / J::PAIR;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((tiles < most ? tiles : most) * J::PAIR));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(threads<J>());
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
@@ -567,21 +577,22 @@ template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, fl
   return *reinterpret_cast<const uint32_t *>(&v);
 }
 
-// The 16-byte piece u of row r in a warp's staging (32 rows of 128 bytes,
+// The 16-byte piece u of row r in a warp's staging (32 rows of 64 bytes,
 // pieces swizzled so that neither row-wise nor piece-wise access conflicts).
 __device__ __forceinline__ uint4 *staged(unsigned char *mine, int r, int u) {
-  return reinterpret_cast<uint4 *>(mine + r * 128 + ((u ^ (r & 7)) << 4));
+  return reinterpret_cast<uint4 *>(mine + r * 64 + ((u ^ ((r >> 1) & 3)) << 4));
 }
 
 // Rounds the warp's 32 x COLS accumulators to O and writes the first `rows`
 // rows and `cols` columns of them to out (row pitch ld): every lane rounds
-// its row into the staging, then 8 lanes write 128 consecutive bytes of a row.
+// its row into the staging, then 4 lanes write 64 consecutive bytes of a row.
 template <typename O, int COLS, class Source>
-__device__ __forceinline__ void write_rows(const Source &source, unsigned char *mine, O *out, int64_t ld, int rows, int64_t cols, bool vectors) {
-  constexpr int ES = (int)sizeof(O);
-  constexpr int CH = 128 / ES < COLS ? 128 / ES : COLS;   // columns staged at a time
-  constexpr int PIECES = CH * ES / 16;
+__device__ __forceinline__ void write_rows(const Source &source, unsigned char *mine, O *out, int64_t ld,
+                                           int rows, int64_t cols, bool vectors) {
+  constexpr int ES = (int)sizeof(O), CH = 64 / ES;        // columns staged at a time
   const int lane = threadIdx.x % 32;
+  O *to = out + (lane / 4) * ld + (lane % 4) * (16 / ES);
+  const bool whole = vectors && rows >= 32;
 #pragma unroll
   for (int c0 = 0; c0 < COLS; c0 += CH) {
     if (c0 >= cols || rows <= 0) continue;
@@ -592,7 +603,7 @@ __device__ __forceinline__ void write_rows(const Source &source, unsigned char *
       if constexpr (ES == 4) {
 #pragma unroll
         for (int u = 0; u < 4; ++u)
-          *staged(mine, lane, c / 4 + u) = *reinterpret_cast<uint4 *>(&v[u * 4]);
+          *staged(mine, lane, u) = *reinterpret_cast<uint4 *>(&v[u * 4]);
       } else {
 #pragma unroll
         for (int u = 0; u < 2; ++u)
@@ -602,18 +613,20 @@ __device__ __forceinline__ void write_rows(const Source &source, unsigned char *
       }
     }
     __syncwarp();
-    if (vectors && c0 + CH <= cols) {
+    if (whole && c0 + CH <= cols) {
 #pragma unroll
-      for (int v = lane; v < 32 * PIECES; v += 32) {
-        const int r = v / PIECES, u = v % PIECES;
-        if (r < rows)
-          *reinterpret_cast<uint4 *>(out + r * ld + c0 + u * (16 / ES)) = *staged(mine, r, u);
-      }
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<uint4 *>(to + c0 + i * 8 * ld) = *staged(mine, i * 8 + lane / 4, lane % 4);
+    } else if (vectors && c0 + CH <= cols) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i * 8 + lane / 4 < rows)
+          *reinterpret_cast<uint4 *>(to + c0 + i * 8 * ld) = *staged(mine, i * 8 + lane / 4, lane % 4);
     } else {
-      for (int r = 0; r < rows && r < 32; ++r)
-        for (int c = lane; c < CH && c0 + c < cols; c += 32)
-          out[r * ld + c0 + c] =
-              reinterpret_cast<const O *>(staged(mine, r, c * ES / 16))[c % (16 / ES)];
+      for (int r = 32 / CH > 1 ? lane / CH : 0; r < rows && r < 32; r += 32 / CH > 1 ? 32 / CH : 1)
+        if (c0 + lane % CH < cols)
+          out[r * ld + c0 + lane % CH] =
+              reinterpret_cast<const O *>(staged(mine, r, lane % CH * ES / 16))[lane % CH % (16 / ES)];
     }
     __syncwarp();
   }
