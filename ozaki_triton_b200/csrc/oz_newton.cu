@@ -12,10 +12,11 @@
 // step by step (the singular values start in [0, 1] and a step's polynomial
 // is known), so e puts the bound at 2^15 and nothing can overflow; no data
 // is looked at.  With one slice the products use `high` alone (11 bits) and
-// only the term a X keeps an fp32 X: that term carries the directions that
-// the products hardly touch (in a model of the roundings on a low-rank gradient
-// the result is 2.2e-2 off with 11 bits there, 4.5e-4 with 22 or more).  With two
-// slices the products add high*high + high*low + low*high.  S and P are symmetric: only the tiles on
+// only the term a X keeps X's 22: that term carries the directions that the
+// products hardly touch, and rounding it as well as P X makes both sides of
+// the sum consistent only for full-rank G (measured on a low-rank gradient:
+// 2.2e-2 with 11 bits there, 4.5e-4 with 22).  With two slices the products add
+// high*high + high*low + low*high.  S and P are symmetric: only the tiles on
 // and below the diagonal are multiplied, each written twice.
 
 #include <algorithm>
@@ -54,7 +55,6 @@ struct InitParams {
   int64_t g_sb, g_sr, g_sc;         // strides of G's member, and of X's rows and columns in G
   double *partial;                  // (batch, partials) sums of squares
   Planes x;
-  float *x32;                       // with one slice: X in fp32 beside it, same pitches
   double eps, scale;
 };
 
@@ -172,13 +172,7 @@ __global__ void __launch_bounds__(256) normalise_kernel(const InitParams p) {
       low[x] = pack2<__half>(a - f.x, b - f.y);
     }
     *reinterpret_cast<uint4 *>(p.x.at(0, blockIdx.z, r0 + r, c0 + u)) = make_uint4(high[0], high[1], high[2], high[3]);
-    if (p.x32) {
-      float4 *x32 = reinterpret_cast<float4 *>(p.x32 + blockIdx.z * p.x.mat + (r0 + r) * p.x.ld + c0 + u);
-      x32[0] = make_float4(tile[r][u], tile[r][u + 1], tile[r][u + 2], tile[r][u + 3]);
-      x32[1] = make_float4(tile[r][u + 4], tile[r][u + 5], tile[r][u + 6], tile[r][u + 7]);
-    } else {
-      *reinterpret_cast<uint4 *>(p.x.at(1, blockIdx.z, r0 + r, c0 + u)) = make_uint4(low[0], low[1], low[2], low[3]);
-    }
+    *reinterpret_cast<uint4 *>(p.x.at(1, blockIdx.z, r0 + r, c0 + u)) = make_uint4(low[0], low[1], low[2], low[3]);
   }
 }
 
@@ -188,57 +182,43 @@ struct StepParams {
   int row_tiles, column_tiles, tiles;   // tiles of one member
   float alpha, beta;                // result = alpha * in + beta * accumulator
   Planes in, out;
-  const float *in32;                // with one slice the update reads and writes X in fp32,
-  float *out32;                     // with the pitches of `in` and `out`
   // the last step's result instead of `out`: element (z, r, c) of the type
   void *last;
   int last_dtype;
   int64_t last_sb, last_sr, last_sc;
 };
 
-// 32 bytes of a lane's row at a time: a whole sector, so that the lanes of a
-// warp can each read and write their own row without staging.
-__device__ __forceinline__ void load32(const void *p, uint32_t *v) {
-  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
-               : "l"(p));
-}
-__device__ __forceinline__ void store32(void *p, const uint32_t *v) {
-  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
-               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-               : "memory");
-}
+// 32 rows x 32 fp16 columns: each lane 4 pieces of 8 columns, 64 bytes of a
+// row by 4 lanes; the warp's staging turns them into each lane's own row.
+struct Chunk { uint4 piece[4]; };
 
-// WORDS words of the lane's row (fp16 pairs or fp32), the pieces that begin
-// before column `cols`; rows are padded to whole pieces.
-template <int WORDS, int PER>
-__device__ __forceinline__ void load_row(const void *p, int cols, uint32_t (&v)[WORDS]) {
+__device__ __forceinline__ void fetch(const __half *src, int64_t ld, int rows, int cols, Chunk &v) {
+  const int lane = threadIdx.x % 32;
+  const __half *from = src + (lane / 4) * ld + (lane % 4) * 8;
+  if (rows >= 32 && cols >= 32) {
 #pragma unroll
-  for (int i = 0; i < WORDS; i += 8) {
-    if (i * PER < cols) {
-      load32(static_cast<const uint32_t *>(p) + i, v + i);
-    } else {
+    for (int i = 0; i < 4; ++i) v.piece[i] = *reinterpret_cast<const uint4 *>(from + i * 8 * ld);
+  } else {
 #pragma unroll
-      for (int x = 0; x < 8; ++x) v[i + x] = 0;
-    }
+    for (int i = 0; i < 4; ++i)
+      v.piece[i] = i * 8 + lane / 4 < rows && lane % 4 * 8 < cols
+                       ? *reinterpret_cast<const uint4 *>(from + i * 8 * ld)
+                       : make_uint4(0, 0, 0, 0);
   }
 }
-template <int WORDS, int PER>
-__device__ __forceinline__ void store_row(void *p, int cols, const uint32_t (&v)[WORDS]) {
+__device__ __forceinline__ void to_rows(unsigned char *mine, Chunk &v) {
+  const int lane = threadIdx.x % 32;
+  __syncwarp();
 #pragma unroll
-  for (int i = 0; i < WORDS; i += 8)
-    if (i * PER < cols) store32(static_cast<uint32_t *>(p) + i, v + i);
+  for (int i = 0; i < 4; ++i) *staged(mine, i * 8 + lane / 4, lane % 4) = v.piece[i];
+  __syncwarp();
+#pragma unroll
+  for (int u = 0; u < 4; ++u) v.piece[u] = *staged(mine, lane, u);
 }
 
-// The mirror image of 32 fp16 columns of each lane's row: the lanes' rows are
-// columns there, so the staging turns them, 64 bytes of a row by 4 lanes.
-__device__ __forceinline__ void store_columns(unsigned char *mine, __half *dst, int64_t ld, int rows, int cols,
-                                              const uint32_t (&v)[16]) {
+// The way back: the chunk in the staging to memory.
+__device__ __forceinline__ void flush(unsigned char *mine, __half *dst, int64_t ld, int rows, int cols) {
   const int lane = threadIdx.x % 32;
-#pragma unroll
-  for (int x = 0; x < 32; ++x)
-    reinterpret_cast<unsigned short *>(staged(mine, x, lane / 8))[lane % 8] =
-        (unsigned short)(x % 2 ? v[x / 2] >> 16 : v[x / 2]);
   __half *to = dst + (lane / 4) * ld + (lane % 4) * 8;
   __syncwarp();
   if (rows >= 32 && cols >= 32) {
@@ -253,48 +233,72 @@ __device__ __forceinline__ void store_columns(unsigned char *mine, __half *dst, 
   }
   __syncwarp();
 }
-
-// What the epilogue adds to the accumulators: IN slices of `in` (0: nothing), or
-// `in32` (IN = -1), 32 columns of the lane's row.
-template <int IN> struct Addend {
-  static constexpr int kSlices = IN < 0 ? 0 : IN, kWords = IN < 0 ? 32 : IN == 0 ? 1 : 16 * IN;
-  uint32_t w[kWords];
-  __device__ __forceinline__ void fetch(const StepParams &p, int z, int row, int column) {
-    const int r = row + threadIdx.x % 32, cols = p.cols - column;
-    if constexpr (IN < 0) {
-      if (r < p.rows) load_row<32, 1>(p.in32 + z * p.in.mat + r * p.in.ld + column, cols, w);
-    } else if constexpr (IN > 0) {
+// From each lane's row; and its mirror image, from each lane's column.
+__device__ __forceinline__ void store_rows(unsigned char *mine, __half *dst, int64_t ld, int rows, int cols,
+                                           const uint4 (&v)[4]) {
+  __syncwarp();
 #pragma unroll
-      for (int q = 0; q < IN; ++q)
-        if (r < p.rows)
-          load_row<16, 2>(p.in.at(q, z, r, column), cols, *reinterpret_cast<uint32_t(*)[16]>(w + q * 16));
+  for (int u = 0; u < 4; ++u) *staged(mine, threadIdx.x % 32, u) = v[u];
+  flush(mine, dst, ld, rows, cols);
+}
+__device__ __forceinline__ void store_columns(unsigned char *mine, __half *dst, int64_t ld, int rows, int cols,
+                                              const uint4 (&v)[4]) {
+  const int lane = threadIdx.x % 32;
+  const __half *h = reinterpret_cast<const __half *>(&v[0]);
+#pragma unroll
+  for (int x = 0; x < 32; ++x) reinterpret_cast<__half *>(staged(mine, x, lane / 8))[lane % 8] = h[x];
+  flush(mine, dst, ld, rows, cols);
+}
+
+// The part of `in` under chunk c of the warp's columns, IN slices.
+template <int IN>
+__device__ __forceinline__ void fetch_in(const StepParams &p, int z, int row, int column, Chunk (&v)[IN + !IN]) {
+#pragma unroll
+  for (int q = 0; q < IN; ++q)
+    fetch(p.in.at(q, z, row, column), p.in.ld, p.rows - row, p.cols - column, v[q]);
+}
+
+// alpha * in + beta * accumulator for 32 columns of the lane's row.
+template <int IN, class Source>
+__device__ __forceinline__ void combine(const StepParams &p, const Source &source, int c, unsigned char *mine,
+                                        Chunk (&in)[IN + !IN], float (&v)[32]) {
+#pragma unroll
+  for (int h = 0; h < 32; h += 16) {
+    float acc[16];
+    source.read(c + h, acc);
+#pragma unroll
+    for (int x = 0; x < 16; ++x) v[h + x] = p.beta * acc[x];
+  }
+#pragma unroll
+  for (int q = 0; q < IN; ++q) {
+    to_rows(mine, in[q]);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const __half2 *h = reinterpret_cast<const __half2 *>(&in[q].piece[u]);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const float2 f = __half22float2(h[x]);
+        v[u * 8 + x * 2] += p.alpha * f.x;
+        v[u * 8 + x * 2 + 1] += p.alpha * f.y;
+      }
     }
   }
-  __device__ __forceinline__ void add(float alpha, float (&v)[32]) const {
-    if constexpr (IN < 0) {
-#pragma unroll
-      for (int x = 0; x < 32; ++x) v[x] += alpha * __uint_as_float(w[x]);
-    }
-#pragma unroll
-    for (int i = 0; i < 16 * kSlices; ++i) {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
-      v[i % 16 * 2] += alpha * f.x;
-      v[i % 16 * 2 + 1] += alpha * f.y;
-    }
-  }
-};
+}
 
-// The slices of 32 values, as pairs.
-template <bool LOW>
-__device__ __forceinline__ void slices_of(const float (&v)[32], uint32_t (&high)[16], uint32_t (&low)[16]) {
+__device__ __forceinline__ void slices_of(const float (&v)[32], uint4 (&high)[4], uint4 (&low)[4]) {
 #pragma unroll
-  for (int x = 0; x < 16; ++x) {
-    const __half2 h = __floats2half2_rn(v[2 * x], v[2 * x + 1]);
-    high[x] = *reinterpret_cast<const uint32_t *>(&h);
-    if constexpr (LOW) {
-      const float2 f = __half22float2(h);
-      low[x] = pack2<__half>(v[2 * x] - f.x, v[2 * x + 1] - f.y);
+  for (int u = 0; u < 4; ++u) {
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const float a = v[u * 8 + x * 2], b = v[u * 8 + x * 2 + 1];
+      const __half2 hh = __floats2half2_rn(a, b);
+      const float2 f = __half22float2(hh);
+      h[x] = *reinterpret_cast<const uint32_t *>(&hh);
+      l[x] = pack2<__half>(a - f.x, b - f.y);
     }
+    high[u] = make_uint4(h[0], h[1], h[2], h[3]);
+    low[u] = make_uint4(l[0], l[1], l[2], l[3]);
   }
 }
 
@@ -303,38 +307,19 @@ struct StepTile { int z, row, column; bool mirror; };
 // S = X X^T (IN 0) and P = b S + c S S (IN slices of S): tiles (i, j) on and
 // below the diagonal, the others their mirror images.
 template <int PAIR_, int NT_, int PLANES_, int IN> struct SymmetricJob {
-  static constexpr int PAIR = PAIR_, NT = NT_, EW = NT_ >= 128 ? 16 : 8, PLANES = PLANES_, PASS = (PLANES_ - 1) * 4;
+  static constexpr int PAIR = PAIR_, NT = NT_, EW = 8, PLANES = PLANES_, PASS = (PLANES_ - 1) * 4;
   static constexpr bool AMN = false, BMN = false, RAGGED = false;
   static constexpr int R = kRows * PAIR / NT;           // column tiles as wide as a tile is high
   using Params = StepParams;
   using Extra = StepTile;
   static __device__ int plane_stride(const Params &p) { return p.batch; }
-  // The first columns of `in` are fetched before the accumulators are there and
-  // each next ones before those in hand are used (passes need the registers).
-  struct Ahead { Addend<IN> in; };
+  // The first chunk of `in` is fetched before the accumulators are there and
+  // each next one before the one in hand is used (passes need the registers).
+  struct Ahead { Chunk in[IN + !IN]; };
   template <class Tile>
   static __device__ void look_ahead(const Params &p, const Tile &t, int row, int column, Ahead &early) {
     if (PASS == 0 && t.extra.row + row < p.rows && t.extra.column + column < p.cols)
-      early.in.fetch(p, t.extra.z, t.extra.row + row, t.extra.column + column);
-  }
-  template <class Source>
-  static __device__ __forceinline__ void values(const Params &p, const TileOf<Extra> &t, const Source &source, int c,
-                                                int r0, int c0, Ahead &early, float (&v)[32]) {
-    Addend<IN> in;
-    if constexpr (PASS == 0) {
-      in = early.in;
-      if (c + 32 < NT * 4 / EW && c0 + 32 < p.cols) early.in.fetch(p, t.extra.z, r0, c0 + 32);
-    } else {
-      in.fetch(p, t.extra.z, r0, c0);
-    }
-#pragma unroll
-    for (int h = 0; h < 32; h += 16) {
-      float acc[16];
-      source.read(c + h, acc);
-#pragma unroll
-      for (int x = 0; x < 16; ++x) v[h + x] = p.beta * acc[x];
-    }
-    in.add(p.alpha, v);
+      fetch_in<IN>(p, t.extra.z, t.extra.row + row, t.extra.column + column, early.in);
   }
   struct Walk {
     __device__ Walk(const Params &) {}
@@ -358,18 +343,27 @@ template <int PAIR_, int NT_, int PLANES_, int IN> struct SymmetricJob {
   template <class Source>
   static __device__ void epilogue(const Params &p, const TileOf<Extra> &t, const Source &source, int row,
                                   int column, unsigned char *mine, Ahead &early) {
-    const int r0 = t.extra.row + row, rows = p.rows - r0, lane = threadIdx.x % 32;
+    const int r0 = t.extra.row + row, rows = p.rows - r0;
     if (rows <= 0) return;
 #pragma unroll
     for (int c = 0; c < NT * 4 / EW; c += 32) {
       const int c0 = t.extra.column + column + c, cols = p.cols - c0;
       if (cols <= 0) continue;
       float v[32];
-      values(p, t, source, c, r0, c0, early, v);
-      uint32_t high[16], low[16];
-      slices_of<PLANES == 2>(v, high, low);
-      if (lane < rows) store_row<16, 2>(p.out.at(0, t.extra.z, r0 + lane, c0), cols, high);
-      if (PLANES == 2 && lane < rows) store_row<16, 2>(p.out.at(1, t.extra.z, r0 + lane, c0), cols, low);
+      Chunk in[IN + !IN];
+      if constexpr (PASS == 0) {
+#pragma unroll
+        for (int q = 0; q < IN; ++q) in[q] = early.in[q];
+        if (c + 32 < NT * 4 / EW && cols > 32) fetch_in<IN>(p, t.extra.z, r0, c0 + 32, early.in);
+      } else {
+        fetch_in<IN>(p, t.extra.z, r0, c0, in);
+      }
+      combine<IN>(p, source, c, mine, in, v);
+      uint4 high[4], low[4];
+      slices_of(v, high, low);
+      store_rows(mine, p.out.at(0, t.extra.z, r0, c0), p.out.ld, rows, cols, high);
+      if constexpr (PLANES == 2)
+        store_rows(mine, p.out.at(1, t.extra.z, r0, c0), p.out.ld, rows, cols, low);
       if (t.extra.mirror) {
         store_columns(mine, p.out.at(0, t.extra.z, c0, r0), p.out.ld, cols, rows, high);
         if constexpr (PLANES == 2)
@@ -382,38 +376,19 @@ template <int PAIR_, int NT_, int PLANES_, int IN> struct SymmetricJob {
 
 // X <- a X + P X: A is the rows of P, B the columns of X.
 template <int PAIR_, int NT_, int PLANES_> struct UpdateJob {
-  static constexpr int IN = PLANES_ == 2 ? 2 : -1;
-  static constexpr int PAIR = PAIR_, NT = NT_, EW = NT_ >= 128 ? 16 : 8, PLANES = PLANES_, PASS = (PLANES_ - 1) * 4;
+  static constexpr int IN = 2;
+  static constexpr int PAIR = PAIR_, NT = NT_, EW = 8, PLANES = PLANES_, PASS = (PLANES_ - 1) * 4;
   static constexpr bool AMN = false, BMN = true, RAGGED = false;
   using Params = StepParams;
   using Extra = StepTile;
   static __device__ int plane_stride(const Params &p) { return p.batch; }
-  // The first columns of `in` are fetched before the accumulators are there and
-  // each next ones before those in hand are used (passes need the registers).
-  struct Ahead { Addend<IN> in; };
+  // The first chunk of `in` is fetched before the accumulators are there and
+  // each next one before the one in hand is used (passes need the registers).
+  struct Ahead { Chunk in[IN + !IN]; };
   template <class Tile>
   static __device__ void look_ahead(const Params &p, const Tile &t, int row, int column, Ahead &early) {
     if (PASS == 0 && t.extra.row + row < p.rows && t.extra.column + column < p.cols)
-      early.in.fetch(p, t.extra.z, t.extra.row + row, t.extra.column + column);
-  }
-  template <class Source>
-  static __device__ __forceinline__ void values(const Params &p, const TileOf<Extra> &t, const Source &source, int c,
-                                                int r0, int c0, Ahead &early, float (&v)[32]) {
-    Addend<IN> in;
-    if constexpr (PASS == 0) {
-      in = early.in;
-      if (c + 32 < NT * 4 / EW && c0 + 32 < p.cols) early.in.fetch(p, t.extra.z, r0, c0 + 32);
-    } else {
-      in.fetch(p, t.extra.z, r0, c0);
-    }
-#pragma unroll
-    for (int h = 0; h < 32; h += 16) {
-      float acc[16];
-      source.read(c + h, acc);
-#pragma unroll
-      for (int x = 0; x < 16; ++x) v[h + x] = p.beta * acc[x];
-    }
-    in.add(p.alpha, v);
+      fetch_in<IN>(p, t.extra.z, t.extra.row + row, t.extra.column + column, early.in);
   }
   struct Walk {
     __device__ Walk(const Params &) {}
@@ -441,18 +416,20 @@ template <int PAIR_, int NT_, int PLANES_> struct UpdateJob {
       const int c0 = t.extra.column + column + c, cols = p.cols - c0;
       if (cols <= 0) continue;
       float v[32];
-      values(p, t, source, c, r0, c0, early, v);
+      Chunk in[IN + !IN];
+      if constexpr (PASS == 0) {
+#pragma unroll
+        for (int q = 0; q < IN; ++q) in[q] = early.in[q];
+        if (c + 32 < NT * 4 / EW && cols > 32) fetch_in<IN>(p, t.extra.z, r0, c0 + 32, early.in);
+      } else {
+        fetch_in<IN>(p, t.extra.z, r0, c0, in);
+      }
+      combine<IN>(p, source, c, mine, in, v);
       if (!p.last) {
-        uint32_t high[16], low[16];
-        slices_of<PLANES == 2>(v, high, low);
-        if (lane < rows) {
-          store_row<16, 2>(p.out.at(0, t.extra.z, r0 + lane, c0), cols, high);
-          if constexpr (PLANES == 2)
-            store_row<16, 2>(p.out.at(1, t.extra.z, r0 + lane, c0), cols, low);
-          else
-            store_row<32, 1>(p.out32 + t.extra.z * p.out.mat + (r0 + lane) * p.out.ld + c0, cols,
-                             *reinterpret_cast<const uint32_t(*)[32]>(v));
-        }
+        uint4 high[4], low[4];
+        slices_of(v, high, low);
+        store_rows(mine, p.out.at(0, t.extra.z, r0, c0), p.out.ld, rows, cols, high);
+        store_rows(mine, p.out.at(1, t.extra.z, r0, c0), p.out.ld, rows, cols, low);
       } else {
         // the result: through the staging where it is stored along the rows,
         // from the lanes where it is stored across them
@@ -498,12 +475,11 @@ template <int PAIR_, int NT_, int PLANES_> struct UpdateJob {
 };
 
 int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
-int64_t pitch(int64_t n) { return (n + 15) / 16 * 16; }   // rows of whole 32-byte pieces
+int64_t pitch(int64_t n) { return (n + 7) / 8 * 8; }
 
-// Workspace of a call: sums of squares, two X's (two slices, or one and fp32), S
-// and P in slices.
+// Workspace of a call: sums of squares, two X's, S and P in slices.
 struct Layout {
-  int64_t rows, cols, x_mat, s_mat, x0, x1, x32, s, p, total;   // x32: from an X's slice to its fp32
+  int64_t rows, cols, x_mat, s_mat, x0, x1, s, p, total;
 };
 Layout layout(int64_t batch, int64_t m, int64_t n, int splits) {
   Layout l{};
@@ -512,8 +488,7 @@ Layout layout(int64_t batch, int64_t m, int64_t n, int splits) {
   l.x_mat = l.rows * pitch(l.cols);
   l.s_mat = l.rows * pitch(l.rows);
   int64_t at = align256(batch * kMostPartials * 8);
-  l.x32 = splits == 1 ? align256(batch * l.x_mat * 2) : 0;
-  const int64_t x = l.x32 + align256(batch * l.x_mat * 4), s = align256(splits * batch * l.s_mat * 2);
+  const int64_t x = align256(2 * batch * l.x_mat * 2), s = align256(splits * batch * l.s_mat * 2);
   l.x0 = at;
   l.x1 = l.x0 + x;
   l.s = l.x1 + x;
@@ -603,9 +578,9 @@ int run(const InitParams &init, const Layout &l, int batch, int steps, const dou
   };
   CUtensorMap xa[2], xb[2], xu[2], sa, sb, pa;
   for (int i = 0; i < 2; ++i) {
-    if (int rc = map(&xa[i], x[i], cols, SPLITS, kRows)) return rc;
-    if (int rc = map(&xb[i], x[i], cols, SPLITS, pair_s ? 128 : 64)) return rc;
-    if (int rc = map(&xu[i], x[i], cols, SPLITS, kBlock)) return rc;
+    if (int rc = map(&xa[i], x[i], cols, 2, kRows)) return rc;
+    if (int rc = map(&xb[i], x[i], cols, 2, pair_s ? 128 : 64)) return rc;
+    if (int rc = map(&xu[i], x[i], cols, 2, kBlock)) return rc;
   }
   if (int rc = map(&sa, s, rows, SPLITS, kRows)) return rc;
   if (int rc = map(&sb, s, rows, SPLITS, pair_s ? 128 : 64)) return rc;
@@ -649,10 +624,6 @@ int run(const InitParams &init, const Layout &l, int batch, int steps, const dou
     up.k = rows;
     up.in = x[cur];
     up.out = x[cur ^ 1];
-    if (SPLITS == 1) {
-      up.in32 = reinterpret_cast<const float *>(ws + (cur ? l.x1 : l.x0) + l.x32);
-      up.out32 = reinterpret_cast<float *>(ws + (cur ? l.x0 : l.x1) + l.x32);
-    }
     up.alpha = (float)std::ldexp(a, en - ex);
     up.beta = (float)std::ldexp(1.0, en - ep - ex);
     rc = pair_x ? step_product<UpdateJob<2, 256, SPLITS>>(pa, xu[cur], up, false, st)
@@ -711,8 +682,7 @@ extern "C" int oz_orthogonalize(const void *g, int dtype, int64_t batch, int64_t
   const bool flat = vectors && line == in_line && m * n % 8 == 0;
   InitParams init{g, dtype, (int)std::min<int64_t>(blocks, kMostPartials), flat, vectors, (int)l.rows, (int)l.cols, g_sb,
                   tall ? g_sc : g_sr, tall ? g_sr : g_sc, reinterpret_cast<double *>(ws),
-                  Planes{reinterpret_cast<__half *>(ws + l.x0), pitch(l.cols), l.x_mat, l.x_mat * batch},
-                  num_splits == 1 ? reinterpret_cast<float *>(ws + l.x0 + l.x32) : nullptr, eps,
+                  Planes{reinterpret_cast<__half *>(ws + l.x0), pitch(l.cols), l.x_mat, l.x_mat * batch}, eps,
                   std::ldexp(1.0, exponent(1 + 1e-6))};
   StepParams last{};
   last.last = out;
