@@ -38,6 +38,7 @@ struct W4Params {
   int64_t ldy;
   int64_t s_se, s_sn;                  // scales (and zeros): expert and row strides, elements
   int along;                           // warps that share the k of a tile (1, 2, 4 or 8)
+  uint32_t per_group;                  // 2^32 / (group / 32), rounded up
   int column_tiles;
 };
 
@@ -155,9 +156,10 @@ template <int RT, int NB, bool WHOLE> struct W4Shape {
   static constexpr int kWeights = kRows * kChunk / 2;      // bytes of a chunk
   static constexpr int kX = 8 * NB * kChunk * 2;
   static constexpr int kStage = kWeights + kX;
-  static constexpr int kSums = kRows * 8 * NB * 4;         // of a warp
   static constexpr int kEntries = kRows * (WHOLE ? 1 : 4); // scales of a chunk
-  static constexpr int kWarpBytes = kDepth * kStage + kEntries * 16 + kSums;
+  static constexpr int kSumRows = kRows < 32 ? kRows : 32; // summed over the warps at a time
+  static constexpr int kSums = kSumRows * 8 * NB * 4;      // of a warp
+  static constexpr int kWarpBytes = kDepth * kStage + kEntries * 12 + kSums;
   static constexpr int kBytes = 512 + kWarps * kWarpBytes + kWarps * kDepth * 8 + 16;
   static constexpr int kCtas = 2 * (kBytes + 1024) <= 228 * 1024 ? 2 : 1;
 };
@@ -175,8 +177,11 @@ __global__ void __launch_bounds__(kWarps * 32, (W4Shape<RT, NB, WHOLE>::kCtas))
   unsigned char *smem = raw + ((512 - (smem_u32(raw) & 511)) & 511);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
   unsigned char *ring = smem + warp * kDepth * Shape::kStage;
-  uint4 *entries = reinterpret_cast<uint4 *>(smem + kWarps * kDepth * Shape::kStage) + warp * Shape::kEntries;
-  float *sums = reinterpret_cast<float *>(smem + kWarps * (kDepth * Shape::kStage + Shape::kEntries * 16));
+  // of the chunk in hand: zeros as Unpack wants them, and scales
+  uint2 *zeros = reinterpret_cast<uint2 *>(smem + kWarps * kDepth * Shape::kStage) + warp * Shape::kEntries;
+  float *scales = reinterpret_cast<float *>(smem + kWarps * (kDepth * Shape::kStage + Shape::kEntries * 8)) +
+                  warp * Shape::kEntries;
+  float *sums = reinterpret_cast<float *>(smem + kWarps * (kDepth * Shape::kStage + Shape::kEntries * 12));
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + kWarps * Shape::kWarpBytes);
   uint64_t *full = bars + warp * kDepth;
   volatile int *abort_flag = reinterpret_cast<volatile int *>(bars + kWarps * kDepth);
@@ -208,6 +213,7 @@ __global__ void __launch_bounds__(kWarps * 32, (W4Shape<RT, NB, WHOLE>::kCtas))
   uint32_t scale_bits[kMine], zero_bits[kMine];
 #pragma unroll
   for (int i = 0; i < kMine; ++i) scale_bits[i] = zero_bits[i] = 0;
+  const uint2 eight = Unpack<T>::zero(8);
   auto issue = [&]() {
 #pragma unroll
     for (int i = 0; i < kMine; ++i) {
@@ -215,9 +221,10 @@ __global__ void __launch_bounds__(kWarps * 32, (W4Shape<RT, NB, WHOLE>::kCtas))
       const float f = p.scale_dtype == OZ_F32 ? __uint_as_float(bits)
                       : p.scale_dtype == OZ_BF16 ? __uint_as_float(bits << 16)
                                                  : __half2float(__ushort_as_half((unsigned short)bits));
-      const uint2 z = Unpack<T>::zero(zero_bits[i]);
-      if (Shape::kEntries >= 32 || lane < Shape::kEntries)
-        entries[i * 32 + lane] = make_uint4(__float_as_uint(f), z.x, z.y, 0);
+      if (Shape::kEntries >= 32 || lane < Shape::kEntries) {
+        scales[i * 32 + lane] = f;
+        if (p.zeros) zeros[i * 32 + lane] = Unpack<T>::zero(zero_bits[i]);
+      }
     }
     while (a_more && a_chunk >= chunks) {
       a_tile += units;
@@ -232,17 +239,19 @@ __global__ void __launch_bounds__(kWarps * 32, (W4Shape<RT, NB, WHOLE>::kCtas))
         tma_load_3d(st, &tm_w, bar, a_chunk * (kChunk / 2), a_column * Shape::kRows, a_e);
         tma_load_3d(st + Shape::kWeights, &tm_x, bar, 0, a_row, a_chunk * (kChunk / 32));
       }
+      const int64_t at0 = a_e * p.s_se + a_column * (Shape::kRows * p.s_sn);
 #pragma unroll
       for (int i = 0; i < kMine; ++i) {
-        const int entry = i * 32 + lane, n = a_column * Shape::kRows + entry % Shape::kRows;
-        const int group = (a_chunk * kChunk + entry / Shape::kRows * 32) / p.group;
-        scale_bits[i] = 0;
-        zero_bits[i] = 8;
-        if (n < p.n && group < p.groups && (Shape::kEntries >= 32 || lane < Shape::kEntries)) {
-          const int64_t at = a_e * p.s_se + n * p.s_sn + group;
+        const int entry = i * 32 + lane, r = entry % Shape::kRows;
+        const uint32_t k32 = (uint32_t)(a_chunk * (kChunk / 32) + entry / Shape::kRows);
+        const int group = p.group == kChunk ? (int)(k32 / 4) : p.group == 32 ? (int)k32 : (int)__umulhi(k32, p.per_group);
+        if ((Shape::kEntries >= 32 || lane < Shape::kEntries) && a_column * Shape::kRows + r < p.n && group < p.groups) {
+          const int64_t at = at0 + r * p.s_sn + group;
           if (p.scale_dtype == OZ_F32) scale_bits[i] = __ldg(static_cast<const uint32_t *>(p.scales) + at);
           else scale_bits[i] = __ldg(static_cast<const unsigned short *>(p.scales) + at);
           if (p.zeros) zero_bits[i] = __ldg(p.zeros + at);
+        } else {
+          scale_bits[i] = 0;                              // nothing there: adds nothing
         }
       }
       a_chunk += p.along;
@@ -252,6 +261,12 @@ __global__ void __launch_bounds__(kWarps * 32, (W4Shape<RT, NB, WHOLE>::kCtas))
   };
   issue();
   issue();
+
+  // the lane's word of the 32-k piece i of a row, and its 8 k of x
+  uint32_t piece[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) piece[i] = g * 64 + ((i ^ ((g >> 1) & 3)) << 4) + t * 4;
+  const uint32_t x_at = Shape::kWeights + g * 64 + t * 16;
 
   W4Walk walk;
   uint32_t used = 0;
@@ -284,17 +299,16 @@ __global__ void __launch_bounds__(kWarps * 32, (W4Shape<RT, NB, WHOLE>::kCtas))
           for (int r = 0; r < RT; ++r)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const uint4 v = entries[(WHOLE ? 0 : i * Shape::kRows) + r * 16 + h * 8 + g];
-              scale[r][h] = __uint_as_float(v.x);
-              zero[r][h] = make_uint2(v.y, v.z);
+              const int entry = (WHOLE ? 0 : i * Shape::kRows) + r * 16 + h * 8 + g;
+              scale[r][h] = scales[entry];
+              zero[r][h] = p.zeros ? zeros[entry] : eight;
             }
         }
         // x: row g of each block of 8, the lane's 8 k, as the pairs (0 4) (1 5) (2 6) (3 7)
         uint32_t x[NB][4];
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-          const uint4 v = *reinterpret_cast<const uint4 *>(st + Shape::kWeights + i * (NB * 512) + b * 512 +
-                                                           g * 64 + t * 16);
+          const uint4 v = *reinterpret_cast<const uint4 *>(st + x_at + i * (NB * 512) + b * 512);
           x[b][0] = __byte_perm(v.x, v.z, 0x5410);
           x[b][1] = __byte_perm(v.x, v.z, 0x7632);
           x[b][2] = __byte_perm(v.y, v.w, 0x5410);
@@ -305,10 +319,8 @@ __global__ void __launch_bounds__(kWarps * 32, (W4Shape<RT, NB, WHOLE>::kCtas))
           uint32_t w[2][4];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const int rr = r * 16 + h * 8 + g;
-            Unpack<T>::values(
-                *reinterpret_cast<const uint32_t *>(st + rr * 64 + ((i ^ ((rr >> 1) & 3)) << 4) + t * 4),
-                zero[r][h], w[h]);
+            Unpack<T>::values(*reinterpret_cast<const uint32_t *>(st + piece[i] + (r * 16 + h * 8) * 64), zero[r][h],
+                              w[h]);
           }
 #pragma unroll
           for (int b = 0; b < NB; ++b) {
@@ -333,24 +345,28 @@ __global__ void __launch_bounds__(kWarps * 32, (W4Shape<RT, NB, WHOLE>::kCtas))
       ++used;
       issue();                                            // into the slot just read
     }
-    // the team's sums: rows of x by weight rows, summed in the order of the warps
+    // the team's sums, 32 weight rows (by rows of x) at a time, in the order of the warps
     float *own = sums + warp * (Shape::kSums / 4);
-#pragma unroll
-    for (int r = 0; r < RT; ++r)
-#pragma unroll
-      for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          own[(b * 8 + t * 2 + (c & 1)) * Shape::kRows + r * 16 + (c >> 1) * 8 + g] = acc[r][b][c];
-    asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(p.along * 32) : "memory");
     const float *all = sums + team * p.along * (Shape::kSums / 4);
-    for (int v = member * 32 + lane; v < rows * Shape::kRows; v += p.along * 32) {
-      float sum = 0.f;
-      for (int w = 0; w < p.along; ++w) sum += all[w * (Shape::kSums / 4) + v];
-      const int n = n0 + v % Shape::kRows;
-      if (n < p.n) put(p, (row + v / Shape::kRows) * p.ldy + n, sum);
+    constexpr int kSumRows = Shape::kSumRows;
+#pragma unroll
+    for (int r0 = 0; r0 < RT; r0 += kSumRows / 16) {
+#pragma unroll
+      for (int r = r0; r < r0 + kSumRows / 16; ++r)
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            own[(b * 8 + t * 2 + (c & 1)) * kSumRows + (r - r0) * 16 + (c >> 1) * 8 + g] = acc[r][b][c];
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(p.along * 32) : "memory");
+      for (int v = member * 32 + lane; v < rows * kSumRows; v += p.along * 32) {
+        float sum = 0.f;
+        for (int w = 0; w < p.along; ++w) sum += all[w * (Shape::kSums / 4) + v];
+        const int n = n0 + r0 * 16 + v % kSumRows;
+        if (n < p.n) put(p, (row + v / kSumRows) * p.ldy + n, sum);
+      }
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(p.along * 32) : "memory");
     }
-    asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(p.along * 32) : "memory");
     ok = !*abort_flag;
   }
   // copies still in flight after a wait gave up
@@ -446,7 +462,8 @@ extern "C" int oz_matmul_w4(const void *x, const void *packed, const void *scale
     return set_error(OZ_ERR_UNSUPPORTED, "unsupported output dtype %d", out_dtype);
   if (experts < 1) return set_error(OZ_ERR_INVALID, "at least one expert is needed, got %d", experts);
   if (rows < 0 || k < 0 || n < 0) return set_error(OZ_ERR_INVALID, "negative size");
-  if (rows > (1 << 30) || k > (1 << 30) || n > (1 << 30) || experts > (1 << 24))
+  // (k / 32) (group / 32) < 2^32 keeps the kernel's division by a product exact
+  if (rows > (1 << 30) || k > (1 << 20) || n > (1 << 30) || experts > (1 << 24))
     return set_error(OZ_ERR_INVALID, "size out of range");
   if (k == 0 || group < 32 || group % 32 != 0 || k % group != 0)
     return set_error(OZ_ERR_INVALID, "the group size must be a multiple of 32 that divides k (group=%d k=%lld)",
@@ -465,7 +482,8 @@ extern "C" int oz_matmul_w4(const void *x, const void *packed, const void *scale
   const int64_t chunks = (k + kChunk - 1) / kChunk;
   W4Params p{scales, offsets, static_cast<const uint8_t *>(zeros), y, offsets_64, experts, group,
              (int)(k / group), scale_dtype, out_dtype, (int)rows, (int)k, (int)n, ldy, s_se, s_sn,
-             chunks >= 8 ? 8 : chunks >= 4 ? 4 : chunks >= 2 ? 2 : 1, 0};
+             chunks >= 8 ? 8 : chunks >= 4 ? 4 : chunks >= 2 ? 2 : 1,
+             group == 32 ? 0 : (uint32_t)(((1ull << 32) + group / 32 - 1) / (group / 32)), 0};
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   return dtype == OZ_F16 ? choose<__half>(packed, x, p, dtype, x_sr, p_se, p_sn, st)
                          : choose<__nv_bfloat16>(packed, x, p, dtype, x_sr, p_se, p_sn, st);
