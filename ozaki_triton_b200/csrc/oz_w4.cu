@@ -96,6 +96,12 @@ struct W4Walk {
 // 16-19 first), exactly: a field becomes the low mantissa bits of a constant
 // that is a power of two, and the same constant plus z is subtracted.  fp16
 // has room for a field in bits 4-7 too (64 + q beside 1024 + q), bf16 has not.
+// (w & m) | c in one instruction: the compiler makes two of it when both are immediates
+__device__ __forceinline__ uint32_t field(uint32_t w, uint32_t m, uint32_t c) {
+  uint32_t v;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(v) : "r"(w), "r"(m), "r"(c));
+  return v;
+}
 template <typename T> struct Unpack;
 template <> struct Unpack<__half> {
   static __device__ __forceinline__ uint2 zero(uint32_t z) {
@@ -107,11 +113,11 @@ template <> struct Unpack<__half> {
     return *reinterpret_cast<const uint32_t *>(&d);
   }
   static __device__ __forceinline__ void values(uint32_t w, uint2 z, uint32_t (&v)[4]) {
-    v[0] = less((w & 0x000f000fu) | 0x64006400u, z.x);
-    v[1] = less((w & 0x00f000f0u) | 0x54005400u, z.y);
+    v[0] = less(field(w, 0x000f000fu, 0x64006400u), z.x);
+    v[1] = less(field(w, 0x00f000f0u, 0x54005400u), z.y);
     w >>= 8;
-    v[2] = less((w & 0x000f000fu) | 0x64006400u, z.x);
-    v[3] = less((w & 0x00f000f0u) | 0x54005400u, z.y);
+    v[2] = less(field(w, 0x000f000fu, 0x64006400u), z.x);
+    v[3] = less(field(w, 0x00f000f0u, 0x54005400u), z.y);
   }
 };
 template <> struct Unpack<__nv_bfloat16> {
@@ -121,7 +127,7 @@ template <> struct Unpack<__nv_bfloat16> {
   static __device__ __forceinline__ void values(uint32_t w, uint2 z, uint32_t (&v)[4]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t u = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+      const uint32_t u = field(w >> (4 * i), 0x000f000fu, 0x43004300u);
       const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&u),
                                        *reinterpret_cast<const __nv_bfloat162 *>(&z.x));
       v[i] = *reinterpret_cast<const uint32_t *>(&d);
@@ -151,12 +157,12 @@ __device__ __forceinline__ void put(const W4Params &p, int64_t i, float v) {
   else static_cast<__nv_bfloat16 *>(p.y)[i] = __float2bfloat16_rn(v);
 }
 
-template <int RT, int NB, bool WHOLE> struct W4Shape {
+template <int RT, int NB, int PER> struct W4Shape {
   static constexpr int kRows = 16 * RT;                    // weight rows of a tile
   static constexpr int kWeights = kRows * kChunk / 2;      // bytes of a chunk
   static constexpr int kX = 8 * NB * kChunk * 2;
   static constexpr int kStage = kWeights + kX;
-  static constexpr int kEntries = kRows * (WHOLE ? 1 : 4); // scales of a chunk
+  static constexpr int kEntries = kRows * PER;             // scales of a chunk
   static constexpr int kSumRows = kRows < 32 ? kRows : 32; // summed over the warps at a time
   static constexpr int kSums = kSumRows * 8 * NB * 4;      // of a warp
   static constexpr int kWarpBytes = kDepth * kStage + kEntries * 12 + kSums;
@@ -165,13 +171,13 @@ template <int RT, int NB, bool WHOLE> struct W4Shape {
 };
 
 // RT: 16-row blocks of weights of a tile; NB: 8-row blocks of x.
-// WHOLE: a group covers whole chunks (g a multiple of 128), one scale a chunk
-// and row; otherwise one for every 32 k.
-template <typename T, int RT, int NB, bool WHOLE>
-__global__ void __launch_bounds__(kWarps * 32, (W4Shape<RT, NB, WHOLE>::kCtas))
+// PER: scales of a chunk and row: 1 where a group covers whole chunks (g a
+// multiple of 128), 2 where g is a multiple of 64, otherwise one for every 32 k.
+template <typename T, int RT, int NB, int PER>
+__global__ void __launch_bounds__(kWarps * 32, (W4Shape<RT, NB, PER>::kCtas))
     w4_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
               const W4Params p) {
-  using Shape = W4Shape<RT, NB, WHOLE>;
+  using Shape = W4Shape<RT, NB, PER>;
   static_assert(kDepth == 2, "the scales of a chunk are loaded two chunks ahead");
   extern __shared__ unsigned char raw[];
   unsigned char *smem = raw + ((512 - (smem_u32(raw) & 511)) & 511);
@@ -212,8 +218,10 @@ __global__ void __launch_bounds__(kWarps * 32, (W4Shape<RT, NB, WHOLE>::kCtas))
   uint32_t issued = 0;
   uint32_t scale_bits[kMine], zero_bits[kMine];
 #pragma unroll
-  for (int i = 0; i < kMine; ++i) scale_bits[i] = zero_bits[i] = 0;
-  const uint2 eight = Unpack<T>::zero(8);
+  for (int i = 0; i < kMine; ++i) {
+    scale_bits[i] = 0;
+    zero_bits[i] = 8;
+  }
   auto issue = [&]() {
 #pragma unroll
     for (int i = 0; i < kMine; ++i) {
@@ -223,7 +231,7 @@ __global__ void __launch_bounds__(kWarps * 32, (W4Shape<RT, NB, WHOLE>::kCtas))
                                                  : __half2float(__ushort_as_half((unsigned short)bits));
       if (Shape::kEntries >= 32 || lane < Shape::kEntries) {
         scales[i * 32 + lane] = f;
-        if (p.zeros) zeros[i * 32 + lane] = Unpack<T>::zero(zero_bits[i]);
+        zeros[i * 32 + lane] = Unpack<T>::zero(zero_bits[i]);
       }
     }
     while (a_more && a_chunk >= chunks) {
@@ -243,7 +251,7 @@ __global__ void __launch_bounds__(kWarps * 32, (W4Shape<RT, NB, WHOLE>::kCtas))
 #pragma unroll
       for (int i = 0; i < kMine; ++i) {
         const int entry = i * 32 + lane, r = entry % Shape::kRows;
-        const uint32_t k32 = (uint32_t)(a_chunk * (kChunk / 32) + entry / Shape::kRows);
+        const uint32_t k32 = (uint32_t)(a_chunk * (kChunk / 32) + entry / Shape::kRows * (4 / PER));
         const int group = p.group == kChunk ? (int)(k32 / 4) : p.group == 32 ? (int)k32 : (int)__umulhi(k32, p.per_group);
         if ((Shape::kEntries >= 32 || lane < Shape::kEntries) && a_column * Shape::kRows + r < p.n && group < p.groups) {
           const int64_t at = at0 + r * p.s_sn + group;
@@ -294,14 +302,14 @@ __global__ void __launch_bounds__(kWarps * 32, (W4Shape<RT, NB, WHOLE>::kCtas))
       float scale[RT][2];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {                       // 32 k at a time
-        if (!WHOLE || i == 0) {
+        if (i % (4 / PER) == 0) {
 #pragma unroll
           for (int r = 0; r < RT; ++r)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const int entry = (WHOLE ? 0 : i * Shape::kRows) + r * 16 + h * 8 + g;
+              const int entry = i / (4 / PER) * Shape::kRows + r * 16 + h * 8 + g;
               scale[r][h] = scales[entry];
-              zero[r][h] = p.zeros ? zeros[entry] : eight;
+              zero[r][h] = zeros[entry];
             }
         }
         // x: row g of each block of 8, the lane's 8 k, as the pairs (0 4) (1 5) (2 6) (3 7)
@@ -325,14 +333,14 @@ __global__ void __launch_bounds__(kWarps * 32, (W4Shape<RT, NB, WHOLE>::kCtas))
 #pragma unroll
           for (int b = 0; b < NB; ++b) {
             float(&d)[4] = part[r][b];
-            if (!WHOLE || i == 0)
+            if (i % (4 / PER) == 0)
               mma<T>(d, w[0][0], w[1][0], w[0][1], w[1][1], x[b][0], x[b][1], 0.f, 0.f, 0.f, 0.f);
             else
               mma<T>(d, w[0][0], w[1][0], w[0][1], w[1][1], x[b][0], x[b][1], d[0], d[1], d[2], d[3]);
             mma<T>(d, w[0][2], w[1][2], w[0][3], w[1][3], x[b][2], x[b][3], d[0], d[1], d[2], d[3]);
           }
         }
-        if (!WHOLE || i == 3) {
+        if ((i + 1) % (4 / PER) == 0) {
 #pragma unroll
           for (int r = 0; r < RT; ++r)
 #pragma unroll
@@ -393,10 +401,10 @@ int make_maps(CUtensorMap *w, CUtensorMap *x, const void *packed, const void *xp
                       kChunk / 32, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
-template <typename T, int RT, int NB, bool WHOLE>
+template <typename T, int RT, int NB, int PER>
 int run_shape(const void *packed, const void *x, W4Params p, int dtype, int64_t x_sr, int64_t p_se, int64_t p_sn,
               cudaStream_t st) {
-  using Shape = W4Shape<RT, NB, WHOLE>;
+  using Shape = W4Shape<RT, NB, PER>;
   CUtensorMap tw, tx;
   if (int rc = make_maps(&tw, &tx, packed, x, p, dtype, x_sr, p_se, p_sn, Shape::kRows, 8 * NB)) return rc;
   p.column_tiles = (p.n + Shape::kRows - 1) / Shape::kRows;
@@ -406,7 +414,7 @@ int run_shape(const void *packed, const void *x, W4Params p, int dtype, int64_t 
   const int teams = kWarps / p.along;
   const int64_t most = Shape::kCtas * (int64_t)tile::sm_count();
   const int64_t need = (tiles + teams - 1) / teams;
-  auto kernel = w4_kernel<T, RT, NB, WHOLE>;
+  auto kernel = w4_kernel<T, RT, NB, PER>;
   static_assert(Shape::kBytes <= 227 * 1024, "shared memory");
   if (int rc = set_smem_once((const void *)kernel, Shape::kBytes, "w4_kernel shared memory")) return rc;
   cudaLaunchConfig_t cfg = {};
@@ -426,8 +434,9 @@ int run_shape(const void *packed, const void *x, W4Params p, int dtype, int64_t 
 template <typename T, int RT, int NB>
 int run(const void *packed, const void *x, const W4Params &p, int dtype, int64_t x_sr, int64_t p_se, int64_t p_sn,
         cudaStream_t st) {
-  return p.group % kChunk == 0 ? run_shape<T, RT, NB, true>(packed, x, p, dtype, x_sr, p_se, p_sn, st)
-                               : run_shape<T, RT, NB, false>(packed, x, p, dtype, x_sr, p_se, p_sn, st);
+  return p.group % 128 == 0  ? run_shape<T, RT, NB, 1>(packed, x, p, dtype, x_sr, p_se, p_sn, st)
+         : p.group % 64 == 0 ? run_shape<T, RT, NB, 2>(packed, x, p, dtype, x_sr, p_se, p_sn, st)
+                             : run_shape<T, RT, NB, 4>(packed, x, p, dtype, x_sr, p_se, p_sn, st);
 }
 
 template <typename T>
