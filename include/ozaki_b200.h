@@ -262,10 +262,13 @@ int oz_cross_gemm_arrivals(const void *a_slices, const void *b_slices, const flo
  * Operands start on 16-byte boundaries and their other strides are multiples
  * of 8 elements.  Sums are held in fp32 and rounded once.
  */
-int oz_grouped_matmul(const void *x, const void *w, const void *offsets, int offsets_64, int dtype,
-                      int out_dtype, int32_t groups, int64_t rows, int64_t k, int64_t n,
-                      int64_t x_sr, int64_t w_se, int64_t w_sk, int64_t w_sn, void *y, int64_t ldy,
-                      void *stream);
+typedef struct {
+  const void *x, *w, *offsets;
+  void *y;
+  int64_t rows, k, n, x_sr, w_se, w_sk, w_sn, ldy;
+  int32_t groups, offsets_64, dtype, out_dtype;
+} oz_grouped_args;
+int oz_grouped_matmul(const oz_grouped_args *args, void *stream);
 
 /*
  * Weight gradient of oz_grouped_matmul:
@@ -273,9 +276,13 @@ int oz_grouped_matmul(const void *x, const void *w, const void *offsets, int off
  * x (rows, k) and dy (rows, n) as x there, row pitches x_sr and dy_sr; dw:
  * contiguous (groups, k, n) of the operands' type or fp32 (out_dtype).
  */
-int oz_grouped_wgrad(const void *x, const void *dy, const void *offsets, int offsets_64, int dtype,
-                     int out_dtype, int32_t groups, int64_t rows, int64_t k, int64_t n,
-                     int64_t x_sr, int64_t dy_sr, void *dw, void *stream);
+typedef struct {
+  const void *x, *dy, *offsets;
+  void *dw;
+  int64_t rows, k, n, x_sr, dy_sr;
+  int32_t groups, offsets_64, dtype, out_dtype;
+} oz_grouped_wgrad_args;
+int oz_grouped_wgrad(const oz_grouped_wgrad_args *args, void *stream);
 
 /*
  * Product of a few rows with 4-bit weights (no counterpart in the reference):
@@ -293,11 +300,13 @@ int oz_grouped_wgrad(const void *x, const void *dy, const void *offsets, int off
  * boundaries and their row pitches are multiples of 16 bytes.  y: (rows, n),
  * row pitch ldy, of x's type or fp32.
  */
-int oz_matmul_w4(const void *x, const void *packed, const void *scales, const void *zeros,
-                 const void *offsets, int offsets_64, int dtype, int scale_dtype, int out_dtype,
-                 int32_t experts, int64_t rows, int64_t k, int64_t n, int32_t group, int64_t x_sr,
-                 int64_t p_se, int64_t p_sn, int64_t s_se, int64_t s_sn, void *y, int64_t ldy,
-                 void *stream);
+typedef struct {
+  const void *x, *packed, *scales, *zeros, *offsets;
+  void *y;
+  int64_t rows, k, n, x_sr, p_se, p_sn, s_se, s_sn, ldy;
+  int32_t experts, group, offsets_64, dtype, scale_dtype, out_dtype;
+} oz_w4_args;
+int oz_matmul_w4(const oz_w4_args *args, void *stream);
 
 /*
  * Newton-Schulz orthogonalisation (no counterpart in the reference) of a

@@ -26,6 +26,21 @@ OZ_IPC_HANDLE_BYTES = 64
 
 # every function the header declares: name -> (restype, argtypes)
 _i64, _i32, _u32, _vp, _int = ctypes.c_int64, ctypes.c_int32, ctypes.c_uint32, ctypes.c_void_p, ctypes.c_int
+
+
+def _struct(name, pointers, int64s, int32s):
+    """A structure of the header: pointers, then 64-bit, then 32-bit integers."""
+    fields = [(f, t) for names, t in ((pointers, _vp), (int64s, _i64), (int32s, _i32)) for f in names.split()]
+    return type(name, (ctypes.Structure,), {"_fields_": fields})
+
+
+GroupedArgs = _struct("GroupedArgs", "x w offsets y", "rows k n x_sr w_se w_sk w_sn ldy",
+                      "groups offsets_64 dtype out_dtype")
+GroupedWgradArgs = _struct("GroupedWgradArgs", "x dy offsets dw", "rows k n x_sr dy_sr",
+                           "groups offsets_64 dtype out_dtype")
+W4Args = _struct("W4Args", "x packed scales zeros offsets y", "rows k n x_sr p_se p_sn s_se s_sn ldy",
+                 "experts group offsets_64 dtype scale_dtype out_dtype")
+
 SIGNATURES = {
     "oz_compute_split_bits": (_int, [_i64, _int, ctypes.POINTER(_i32)]),
     "oz_slice_row_bytes": (_i64, [_i64, _int]),
@@ -48,12 +63,9 @@ SIGNATURES = {
     "oz_matmul": (_int, [_vp, _vp, _int, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _i64,
                          _i64, _i64, _i64, _i64, _i64, _i32, _int, _int, _vp, _i64, _u32, _vp,
                          _i64, _vp]),
-    "oz_grouped_matmul": (_int, [_vp, _vp, _vp, _int, _int, _int, _i32, _i64, _i64, _i64, _i64,
-                                 _i64, _i64, _i64, _vp, _i64, _vp]),
-    "oz_grouped_wgrad": (_int, [_vp, _vp, _vp, _int, _int, _int, _i32, _i64, _i64, _i64, _i64,
-                                _i64, _vp, _vp]),
-    "oz_matmul_w4": (_int, [_vp, _vp, _vp, _vp, _vp, _int, _int, _int, _int, _i32, _i64, _i64,
-                            _i64, _i32, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _vp]),
+    "oz_grouped_matmul": (_int, [ctypes.POINTER(GroupedArgs), _vp]),
+    "oz_grouped_wgrad": (_int, [ctypes.POINTER(GroupedWgradArgs), _vp]),
+    "oz_matmul_w4": (_int, [ctypes.POINTER(W4Args), _vp]),
     "oz_orthogonalize_workspace_bytes": (_i64, [_int, _i64, _i64, _i64, _i32]),
     "oz_orthogonalize": (_int, [_vp, _int, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _vp,
                                 ctypes.c_double, _i32, _vp, _vp, _i64, _vp]),

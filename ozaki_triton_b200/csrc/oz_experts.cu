@@ -301,10 +301,10 @@ int wgrad(const void *x, const void *dy, int64_t x_sr, int64_t dy_sr, const Grou
 }  // namespace
 }  // namespace oz
 
-extern "C" int oz_grouped_matmul(const void *x, const void *w, const void *offsets,
-                                 int offsets_64, int dtype, int out_dtype, int32_t groups,
-                                 int64_t rows, int64_t k, int64_t n, int64_t x_sr, int64_t w_se,
-                                 int64_t w_sk, int64_t w_sn, void *y, int64_t ldy, void *stream) {
+extern "C" int oz_grouped_matmul(const oz_grouped_args *args, void *stream) {
+  if (!args) return oz::set_error(OZ_ERR_INVALID, "null arguments");
+  const auto [x, w, offsets, y, rows, k, n, x_sr, w_se, w_sk, w_sn, ldy, groups, offsets_64, dtype,
+              out_dtype] = *args;
   using namespace oz;
   if (int rc = check_grouped(dtype, out_dtype, groups, rows, k, n)) return rc;
   if (rows == 0 || n == 0) return OZ_OK;
@@ -330,10 +330,9 @@ extern "C" int oz_grouped_matmul(const void *x, const void *w, const void *offse
   return grouped<__nv_bfloat16>(x, w, x_sr, w_se, across, w_row, p, st);
 }
 
-extern "C" int oz_grouped_wgrad(const void *x, const void *dy, const void *offsets,
-                                int offsets_64, int dtype, int out_dtype, int32_t groups,
-                                int64_t rows, int64_t k, int64_t n, int64_t x_sr, int64_t dy_sr,
-                                void *dw, void *stream) {
+extern "C" int oz_grouped_wgrad(const oz_grouped_wgrad_args *args, void *stream) {
+  if (!args) return oz::set_error(OZ_ERR_INVALID, "null arguments");
+  const auto [x, dy, offsets, dw, rows, k, n, x_sr, dy_sr, groups, offsets_64, dtype, out_dtype] = *args;
   using namespace oz;
   if (int rc = check_grouped(dtype, out_dtype, groups, rows, k, n)) return rc;
   if (k == 0 || n == 0) return OZ_OK;

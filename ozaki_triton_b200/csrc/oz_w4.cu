@@ -96,7 +96,14 @@ struct W4Walk {
 // 16-19 first), exactly: a field becomes the low mantissa bits of a constant
 // that is a power of two, and the same constant plus z is subtracted.  fp16
 // has room for a field in bits 4-7 too (64 + q beside 1024 + q), bf16 has not.
-// (w & m) | c in one instruction: the compiler makes two of it when both are immediates
+// A constant that stays in a register (as an immediate it is moved there again at
+// each use, and a mask and an or with two immediates become two instructions).
+__device__ __forceinline__ uint32_t kept(uint32_t c) {
+  uint32_t v;
+  asm volatile("mov.b32 %0, %1;" : "=r"(v) : "r"(c));
+  return v;
+}
+// (w & m) | c
 __device__ __forceinline__ uint32_t field(uint32_t w, uint32_t m, uint32_t c) {
   uint32_t v;
   asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(v) : "r"(w), "r"(m), "r"(c));
@@ -104,6 +111,7 @@ __device__ __forceinline__ uint32_t field(uint32_t w, uint32_t m, uint32_t c) {
 }
 template <typename T> struct Unpack;
 template <> struct Unpack<__half> {
+  uint32_t m0 = kept(0x000f000fu), c0 = kept(0x64006400u), m1 = kept(0x00f000f0u), c1 = kept(0x54005400u);
   static __device__ __forceinline__ uint2 zero(uint32_t z) {
     z *= 0x10001u;
     return make_uint2(0x64006400u | z, 0x54005400u | z << 4);
@@ -112,22 +120,23 @@ template <> struct Unpack<__half> {
     const __half2 d = __hsub2(*reinterpret_cast<const __half2 *>(&v), *reinterpret_cast<const __half2 *>(&z));
     return *reinterpret_cast<const uint32_t *>(&d);
   }
-  static __device__ __forceinline__ void values(uint32_t w, uint2 z, uint32_t (&v)[4]) {
-    v[0] = less(field(w, 0x000f000fu, 0x64006400u), z.x);
-    v[1] = less(field(w, 0x00f000f0u, 0x54005400u), z.y);
+  __device__ __forceinline__ void values(uint32_t w, uint2 z, uint32_t (&v)[4]) const {
+    v[0] = less(field(w, m0, c0), z.x);
+    v[1] = less(field(w, m1, c1), z.y);
     w >>= 8;
-    v[2] = less(field(w, 0x000f000fu, 0x64006400u), z.x);
-    v[3] = less(field(w, 0x00f000f0u, 0x54005400u), z.y);
+    v[2] = less(field(w, m0, c0), z.x);
+    v[3] = less(field(w, m1, c1), z.y);
   }
 };
 template <> struct Unpack<__nv_bfloat16> {
+  uint32_t m0 = kept(0x000f000fu), c0 = kept(0x43004300u);
   static __device__ __forceinline__ uint2 zero(uint32_t z) {
     return make_uint2(0x43004300u | z * 0x10001u, 0);
   }
-  static __device__ __forceinline__ void values(uint32_t w, uint2 z, uint32_t (&v)[4]) {
+  __device__ __forceinline__ void values(uint32_t w, uint2 z, uint32_t (&v)[4]) const {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t u = field(w >> (4 * i), 0x000f000fu, 0x43004300u);
+      const uint32_t u = field(w >> (4 * i), m0, c0);
       const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&u),
                                        *reinterpret_cast<const __nv_bfloat162 *>(&z.x));
       v[i] = *reinterpret_cast<const uint32_t *>(&d);
@@ -140,12 +149,12 @@ template <typename T>
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                     uint32_t b1, float c0, float c1, float c2, float c3) {
   if constexpr (__is_same(T, __half))
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
                  "{%8, %9}, {%10, %11, %12, %13};"
                  : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
   else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
                  "{%8, %9}, {%10, %11, %12, %13};"
                  : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
@@ -217,6 +226,22 @@ __global__ void __launch_bounds__(kWarps * 32, (W4Shape<RT, NB, PER>::kCtas))
   bool a_more = ahead.find(p, 8 * NB, a_tile, a_e, a_row, a_rows, a_column);
   uint32_t issued = 0;
   uint32_t scale_bits[kMine], zero_bits[kMine];
+  // the tile's scales of this lane's entries (null: no such row), and what a
+  // chunk's group index has to be multiplied by
+  const char *scale_at[kMine];
+  const uint8_t *zero_at[kMine];
+  const int scale_bytes = p.scale_dtype == OZ_F32 ? 4 : 2;
+  auto enter = [&]() {                                    // the tile that is copied next
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const int r = (i * 32 + lane) % Shape::kRows, n = a_column * Shape::kRows + r;
+      const int64_t at = a_e * p.s_se + n * p.s_sn;
+      const bool in = n < p.n && (Shape::kEntries >= 32 || lane < Shape::kEntries);
+      scale_at[i] = in ? static_cast<const char *>(p.scales) + at * scale_bytes : nullptr;
+      zero_at[i] = in && p.zeros ? p.zeros + at : nullptr;
+    }
+  };
+  if (a_more) enter();
 #pragma unroll
   for (int i = 0; i < kMine; ++i) {
     scale_bits[i] = 0;
@@ -238,6 +263,7 @@ __global__ void __launch_bounds__(kWarps * 32, (W4Shape<RT, NB, PER>::kCtas))
       a_tile += units;
       a_chunk = member;
       a_more = ahead.find(p, 8 * NB, a_tile, a_e, a_row, a_rows, a_column);
+      if (a_more) enter();
     }
     if (a_more) {
       if (lane == 0) {
@@ -247,17 +273,15 @@ __global__ void __launch_bounds__(kWarps * 32, (W4Shape<RT, NB, PER>::kCtas))
         tma_load_3d(st, &tm_w, bar, a_chunk * (kChunk / 2), a_column * Shape::kRows, a_e);
         tma_load_3d(st + Shape::kWeights, &tm_x, bar, 0, a_row, a_chunk * (kChunk / 32));
       }
-      const int64_t at0 = a_e * p.s_se + a_column * (Shape::kRows * p.s_sn);
 #pragma unroll
       for (int i = 0; i < kMine; ++i) {
-        const int entry = i * 32 + lane, r = entry % Shape::kRows;
-        const uint32_t k32 = (uint32_t)(a_chunk * (kChunk / 32) + entry / Shape::kRows * (4 / PER));
-        const int group = p.group == kChunk ? (int)(k32 / 4) : p.group == 32 ? (int)k32 : (int)__umulhi(k32, p.per_group);
-        if ((Shape::kEntries >= 32 || lane < Shape::kEntries) && a_column * Shape::kRows + r < p.n && group < p.groups) {
-          const int64_t at = at0 + r * p.s_sn + group;
-          if (p.scale_dtype == OZ_F32) scale_bits[i] = __ldg(static_cast<const uint32_t *>(p.scales) + at);
-          else scale_bits[i] = __ldg(static_cast<const unsigned short *>(p.scales) + at);
-          if (p.zeros) zero_bits[i] = __ldg(p.zeros + at);
+        const uint32_t k32 = (uint32_t)(a_chunk * (kChunk / 32) + (i * 32 + lane) / Shape::kRows * (4 / PER));
+        const uint32_t group = p.group == kChunk ? k32 / 4 : p.group == 32 ? k32 : __umulhi(k32, p.per_group);
+        if (scale_at[i] && (int)group < p.groups) {
+          const char *at = scale_at[i] + group * scale_bytes;
+          scale_bits[i] = scale_bytes == 4 ? __ldg(reinterpret_cast<const uint32_t *>(at))
+                                           : __ldg(reinterpret_cast<const unsigned short *>(at));
+          if (zero_at[i]) zero_bits[i] = __ldg(zero_at[i] + group);
         } else {
           scale_bits[i] = 0;                              // nothing there: adds nothing
         }
@@ -276,6 +300,7 @@ __global__ void __launch_bounds__(kWarps * 32, (W4Shape<RT, NB, PER>::kCtas))
   for (int i = 0; i < 4; ++i) piece[i] = g * 64 + ((i ^ ((g >> 1) & 3)) << 4) + t * 4;
   const uint32_t x_at = Shape::kWeights + g * 64 + t * 16;
 
+  const Unpack<T> unpack;
   W4Walk walk;
   uint32_t used = 0;
   bool ok = true;
@@ -327,7 +352,7 @@ __global__ void __launch_bounds__(kWarps * 32, (W4Shape<RT, NB, PER>::kCtas))
           uint32_t w[2][4];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            Unpack<T>::values(*reinterpret_cast<const uint32_t *>(st + piece[i] + (r * 16 + h * 8) * 64), zero[r][h],
+            unpack.values(*reinterpret_cast<const uint32_t *>(st + piece[i] + (r * 16 + h * 8) * 64), zero[r][h],
                               w[h]);
           }
 #pragma unroll
@@ -456,12 +481,10 @@ int choose(const void *packed, const void *x, const W4Params &p, int dtype, int6
 }  // namespace
 }  // namespace oz
 
-extern "C" int oz_matmul_w4(const void *x, const void *packed, const void *scales,
-                            const void *zeros, const void *offsets, int offsets_64, int dtype,
-                            int scale_dtype, int out_dtype, int32_t experts, int64_t rows,
-                            int64_t k, int64_t n, int32_t group, int64_t x_sr, int64_t p_se,
-                            int64_t p_sn, int64_t s_se, int64_t s_sn, void *y, int64_t ldy,
-                            void *stream) {
+extern "C" int oz_matmul_w4(const oz_w4_args *args, void *stream) {
+  if (!args) return oz::set_error(OZ_ERR_INVALID, "null arguments");
+  auto [x, packed, scales, zeros, offsets, y, rows, k, n, x_sr, p_se, p_sn, s_se, s_sn, ldy, experts, group,
+        offsets_64, dtype, scale_dtype, out_dtype] = *args;
   using namespace oz;
   if (dtype != OZ_F16 && dtype != OZ_BF16)
     return set_error(OZ_ERR_UNSUPPORTED, "unsupported operand dtype %d (fp16 or bf16)", dtype);

@@ -17,6 +17,8 @@ All calls enqueue their work on the current stream of their tensors' device.
 
 from __future__ import annotations
 
+import ctypes
+import threading
 from typing import Optional, Tuple
 
 import torch
@@ -42,7 +44,7 @@ def _check_places(x: torch.Tensor, *ts: Optional[torch.Tensor]) -> int:
 
 
 class _OnDevice:
-    """Makes a device current for a call, at no cost where it is already."""
+    """Makes a device current for a call."""
 
     __slots__ = ("index", "other")
 
@@ -90,59 +92,29 @@ def _copied(t: torch.Tensor) -> torch.Tensor:
     return laid[..., :inner].copy_(t)
 
 
-def _as_operand(t: torch.Tensor) -> torch.Tensor:
-    """t, or a copy where the copy unit cannot read its layout: it wants a unit
-    stride along the last dimension, 16-byte boundaries and no repeated rows."""
+def _readable(t: torch.Tensor) -> bool:
+    """Whether the copy unit can read t's layout: it wants a unit stride along the
+    last dimension, 16-byte boundaries and no repeated rows."""
     shape, strides = t.shape, t.stride()
-    if (strides[-1] == 1 or shape[-1] == 1) and t.data_ptr() % 16 == 0:
-        for n, s in zip(shape[:-1], strides):
-            if n > 1 and (s <= 0 or s % 8):
-                break
-        else:
-            return t
-    return _copied(t)
+    if (strides[-1] != 1 and shape[-1] != 1) or t.data_ptr() % 16:
+        return False
+    return all(n <= 1 or (s > 0 and s % 8 == 0) for n, s in zip(shape[:-1], strides))
+
+
+def _as_operand(t: torch.Tensor) -> torch.Tensor:
+    return t if _readable(t) else _copied(t)
+
+
+def _along(w: torch.Tensor) -> torch.Tensor:
+    """(E, K, N) weights with the dimension they are stored along last."""
+    return w.transpose(1, 2) if w.stride(1) == 1 and w.stride(2) != 1 else w
 
 
 def _as_weights(w: torch.Tensor) -> torch.Tensor:
-    """The same for (E, K, N) weights, which may be stored along K or along N."""
-    if w.stride(1) == 1 and w.stride(2) != 1:
-        return _as_operand(w.transpose(1, 2)).transpose(1, 2)
-    return _as_operand(w)
-
-
-def _product(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, out_dtype: torch.dtype,
-             device: int) -> torch.Tensor:
-    rows, k = x.shape
-    groups, _, n = w.shape
-    y = x.new_empty((rows, n), dtype=out_dtype)
-    if rows == 0 or n == 0:
-        return y
-    if k > 0:
-        x, w = _as_operand(x), _as_weights(w)
-    w_se, w_sk, w_sn = w.stride()
-    with _OnDevice(device):
-        _lib.check(_lib.load().oz_grouped_matmul(
-            x.data_ptr(), w.data_ptr(), offsets.data_ptr(), offsets.dtype is torch.int64,
-            _OZ_DTYPE[x.dtype], _OZ_DTYPE[out_dtype], groups, rows, k, n, x.stride(0),
-            w_se, w_sk, w_sn, y.data_ptr(), n, _stream_of(device)))
-    return y
-
-
-def _weight_gradient(x: torch.Tensor, dy: torch.Tensor, offsets: torch.Tensor, groups: int,
-                     out_dtype: torch.dtype, device: int) -> torch.Tensor:
-    rows, k = x.shape
-    n = dy.shape[1]
-    dw = x.new_empty((groups, k, n), dtype=out_dtype)
-    if k == 0 or n == 0:
-        return dw
-    if rows > 0:
-        x, dy = _as_operand(x), _as_operand(dy)
-    with _OnDevice(device):
-        _lib.check(_lib.load().oz_grouped_wgrad(
-            x.data_ptr(), dy.data_ptr(), offsets.data_ptr(), offsets.dtype is torch.int64,
-            _OZ_DTYPE[x.dtype], _OZ_DTYPE[out_dtype], groups, rows, k, n, x.stride(0),
-            dy.stride(0), dw.data_ptr(), _stream_of(device)))
-    return dw
+    if _readable(_along(w)):
+        return w
+    across = w.stride(1) == 1 and w.stride(2) != 1
+    return _copied(w.transpose(1, 2)).transpose(1, 2) if across else _copied(w)
 
 
 def _check_grouped(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor) -> None:
@@ -154,19 +126,123 @@ def _check_grouped(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor) -> N
     _check_offsets(offsets, w.shape[0])
 
 
+class _Plan:
+    """What a call derives from its tensors' types, shapes, strides and devices
+    alone: the checks passed, the library's arguments but for the addresses,
+    and the result's shape.  Kept per distinct call signature and thread, so
+    that a repeated small product pays for its allocation and one library
+    call (checking and converting everything again took 5 us of 13)."""
+
+    __slots__ = ("args", "ref", "call", "shape", "dtype", "empty", "copy", "device")
+
+
+class _Plans(threading.local):
+    def __init__(self):
+        self.kept = {}
+
+    def keep(self, key, plan: _Plan) -> _Plan:
+        if len(self.kept) >= 256:
+            self.kept.clear()
+        self.kept[key] = plan
+        return plan
+
+
+_PLANS = _Plans()
+_CURRENT_DEVICE = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _launch(plan: _Plan) -> None:
+    """The plan's library call on the current stream of its device."""
+    device = plan.device
+    if _CURRENT_DEVICE() == device:
+        status = plan.call(plan.ref, _stream_of(device))
+    else:
+        with _OnDevice(device):
+            status = plan.call(plan.ref, _stream_of(device))
+    if status:
+        _lib.check(status)
+
+
+def _make_plan(call: str, args: ctypes.Structure, shape: Tuple[int, ...], dtype: torch.dtype, device: int,
+               empty: bool, copy: bool) -> _Plan:
+    plan = _Plan()
+    plan.args, plan.ref = args, ctypes.byref(args)
+    plan.call = getattr(_lib.load(), call) if not empty else None
+    plan.shape, plan.dtype, plan.device, plan.empty, plan.copy = shape, dtype, device, empty, copy
+    return plan
+
+
+def _plan_product(key, x, w, offsets, out_dtype) -> _Plan:
+    _check_grouped(x, w, offsets)
+    out_dtype = _out_dtype(out_dtype, x.dtype)
+    device = _check_places(x, w, offsets)
+    rows, k = x.shape
+    groups, _, n = w.shape
+    copy = k > 0 and not (_readable(x) and _readable(_along(w)))
+    args = _lib.GroupedArgs(None, None, None, None, rows, k, n, x.stride(0), *w.stride(), n, groups,
+                            offsets.dtype is torch.int64, _OZ_DTYPE[x.dtype], _OZ_DTYPE[out_dtype])
+    return _PLANS.keep(key, _make_plan("oz_grouped_matmul", args, (rows, n), out_dtype, device,
+                                       rows == 0 or n == 0, copy))
+
+
+def _product(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor,
+             out_dtype: Optional[torch.dtype]) -> torch.Tensor:
+    # the addresses' alignment is part of the signature: _as_operand looks at it
+    xp, wp = x.data_ptr(), w.data_ptr()
+    key = (x.shape, x.stride(), x.dtype, w.shape, w.stride(), w.dtype, offsets.shape, offsets.stride(),
+           offsets.dtype, out_dtype, x.get_device(), w.get_device(), offsets.get_device(), xp % 16, wp % 16)
+    plan = _PLANS.kept.get(key) or _plan_product(key, x, w, offsets, out_dtype)
+    if plan.copy:
+        return _product(_as_operand(x), _as_weights(w), offsets, out_dtype)
+    y = x.new_empty(plan.shape, dtype=plan.dtype)
+    if not plan.empty:
+        args = plan.args
+        args.x, args.w, args.offsets, args.y = xp, wp, offsets.data_ptr(), y.data_ptr()
+        _launch(plan)
+    return y
+
+
+def _plan_weight_gradient(key, x, dy, offsets, groups, out_dtype) -> _Plan:
+    out_dtype = _out_dtype(out_dtype, x.dtype)
+    device = _check_places(x, dy, offsets)
+    rows, k = x.shape
+    n = dy.shape[1]
+    copy = rows > 0 and not (_readable(x) and _readable(dy))
+    args = _lib.GroupedWgradArgs(None, None, None, None, rows, k, n, x.stride(0), dy.stride(0), groups,
+                                 offsets.dtype is torch.int64, _OZ_DTYPE[x.dtype], _OZ_DTYPE[out_dtype])
+    return _PLANS.keep(key, _make_plan("oz_grouped_wgrad", args, (groups, k, n), out_dtype, device,
+                                       k == 0 or n == 0, copy))
+
+
+def _weight_gradient(x: torch.Tensor, dy: torch.Tensor, offsets: torch.Tensor, groups: int,
+                     out_dtype: Optional[torch.dtype]) -> torch.Tensor:
+    xp, dp = x.data_ptr(), dy.data_ptr()
+    key = (groups, x.shape, x.stride(), x.dtype, dy.shape, dy.stride(), offsets.dtype, out_dtype,
+           x.get_device(), dy.get_device(), offsets.get_device(), xp % 16, dp % 16)
+    plan = _PLANS.kept.get(key) or _plan_weight_gradient(key, x, dy, offsets, groups, out_dtype)
+    if plan.copy:
+        return _weight_gradient(_as_operand(x), _as_operand(dy), offsets, groups, out_dtype)
+    dw = x.new_empty(plan.shape, dtype=plan.dtype)
+    if not plan.empty:
+        args = plan.args
+        args.x, args.dy, args.offsets, args.dw = xp, dp, offsets.data_ptr(), dw.data_ptr()
+        _launch(plan)
+    return dw
+
+
 class _GroupedMatmul(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, offsets, out_dtype):
         ctx.save_for_backward(x, w, offsets)
-        return _product(x, w, offsets, out_dtype, x.get_device())
+        return _product(x, w, offsets, out_dtype)
 
     @staticmethod
     def backward(ctx, dy):
         x, w, offsets = ctx.saved_tensors
-        dy, device = dy.to(x.dtype), x.get_device()
+        dy = dy.to(x.dtype)
         need_x, need_w = ctx.needs_input_grad[:2]
-        dx = _product(dy, w.transpose(1, 2), offsets, x.dtype, device) if need_x else None
-        dw = _weight_gradient(x, dy, offsets, w.shape[0], w.dtype, device) if need_w else None
+        dx = _product(dy, w.transpose(1, 2), offsets, None) if need_x else None
+        dw = _weight_gradient(x, dy, offsets, w.shape[0], None) if need_w else None
         return dx, dw, None, None
 
 
@@ -181,12 +257,9 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, *,
     fp32 with ``out_dtype=torch.float32``.  Sums are held in fp32 and rounded
     once.  Differentiable in x and w.
     """
-    _check_grouped(x, w, offsets)
-    out_dtype = _out_dtype(out_dtype, x.dtype)
-    device = _check_places(x, w, offsets)
-    if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
+    if (x.requires_grad or w.requires_grad) and torch.is_grad_enabled():
         return _GroupedMatmul.apply(x, w, offsets, out_dtype)
-    return _product(x, w, offsets, out_dtype, device)
+    return _product(x, w, offsets, out_dtype)
 
 
 def grouped_matmul_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor,
@@ -198,16 +271,16 @@ def grouped_matmul_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor,
     with ``dw_dtype=torch.float32``, in fp32.  The gradient of an expert without
     rows is zero.
     """
-    _check_grouped(x, w, offsets)
-    _check_rows(dy, "dy")
-    assert dy.dtype == x.dtype, f"x/dy dtype mismatch: {x.dtype} vs {dy.dtype}"
-    assert tuple(dy.shape) == (x.shape[0], w.shape[2]), \
+    assert dy.dim() == 2 and x.dim() == 2 and w.dim() == 3, "x and dy must have 2 dimensions, w 3"
+    assert dy.dtype is x.dtype, f"x/dy dtype mismatch: {x.dtype} vs {dy.dtype}"
+    assert dy.shape[0] == x.shape[0] and dy.shape[1] == w.shape[2], \
         f"dy must be {(x.shape[0], w.shape[2])}, got {tuple(dy.shape)}"
+    assert x.shape[1] == w.shape[1], f"contraction dim mismatch: x K={x.shape[1]}, w K={w.shape[1]}"
     dw_dtype = _out_dtype(dw_dtype, x.dtype)
-    device = _check_places(x, w, offsets, dy)
-    x, dy = _as_operand(x), _as_operand(dy)               # once for both products
-    return (_product(dy, w.transpose(1, 2), offsets, x.dtype, device),
-            _weight_gradient(x, dy, offsets, w.shape[0], dw_dtype, device))
+    if x.is_cuda and dy.is_cuda:
+        x, dy = _as_operand(x), _as_operand(dy)           # once for both products
+    return (_product(dy, w.transpose(1, 2), offsets, None),
+            _weight_gradient(x, dy, offsets, w.shape[0], dw_dtype))
 
 
 def quantize_w4(w: torch.Tensor, group_size: int = 128, *, symmetric: bool = True,
@@ -242,18 +315,7 @@ def quantize_w4(w: torch.Tensor, group_size: int = 128, *, symmetric: bool = Tru
     return (q[..., 0::2] | (q[..., 1::2] << 4)).contiguous(), scales, zeros
 
 
-def matmul_w4(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor,
-              zeros: Optional[torch.Tensor] = None, *, offsets: Optional[torch.Tensor] = None,
-              out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
-    """y = x @ W^T with W[n, k] = (q[n, k] - z[n, k / g]) s[n, k / g] held in 4 bits.
-
-    x (T, K) bf16 or fp16; packed (N, K / 2) uint8, two values a byte, the even
-    k in the low half; scales (N, K / g) fp16, bf16 or fp32; zeros (N, K / g)
-    uint8, or None for 8 everywhere (the layout ``quantize_w4`` returns).
-    With ``offsets`` the weights have a leading expert dimension and the rows
-    of x come in groups.  Returns (T, N) in x's dtype or fp32.  Made for few
-    rows a matrix (the weights' bytes bound it); any number is right.
-    """
+def _plan_w4(key, x, packed, scales, zeros, offsets, out_dtype) -> _Plan:
     _check_rows(x, "x")
     lead = 2 if offsets is None else 3
     p_shape, s_shape = packed.shape, scales.shape
@@ -278,22 +340,44 @@ def matmul_w4(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor,
     if offsets is not None:
         _check_offsets(offsets, experts)
     device = _check_places(x, packed, scales, zeros, offsets)
-    y = x.new_empty((rows, n), dtype=out_dtype)
-    if rows == 0 or n == 0:
-        return y
-    x = _as_operand(x)
-    packed, scales = packed.contiguous(), scales.contiguous()
-    if packed.data_ptr() % 16:
-        packed = packed.clone()
-    if zeros is not None:
-        zeros = zeros.contiguous()
-    with _OnDevice(device):
-        _lib.check(_lib.load().oz_matmul_w4(
-            x.data_ptr(), packed.data_ptr(), scales.data_ptr(),
-            zeros.data_ptr() if zeros is not None else None,
-            offsets.data_ptr() if offsets is not None else None,
-            offsets is not None and offsets.dtype is torch.int64, _OZ_DTYPE[x.dtype],
-            _OZ_DTYPE[scales.dtype], _OZ_DTYPE[out_dtype], experts, rows, k, n, k // groups,
-            x.stride(0), n * (k // 2), k // 2, n * groups, groups, y.data_ptr(), n,
-            _stream_of(device)))
+    copy = (not _readable(x) or not packed.is_contiguous() or not scales.is_contiguous()
+            or packed.data_ptr() % 16 != 0 or (zeros is not None and not zeros.is_contiguous()))
+    args = _lib.W4Args(None, None, None, None, None, None, rows, k, n, x.stride(0), n * (k // 2), k // 2,
+                       n * groups, groups, n, experts, k // groups,
+                       offsets is not None and offsets.dtype is torch.int64, _OZ_DTYPE[x.dtype],
+                       _OZ_DTYPE[scales.dtype], _OZ_DTYPE[out_dtype])
+    return _PLANS.keep(key, _make_plan("oz_matmul_w4", args, (rows, n), out_dtype, device,
+                                       rows == 0 or n == 0, copy))
+
+
+def matmul_w4(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor,
+              zeros: Optional[torch.Tensor] = None, *, offsets: Optional[torch.Tensor] = None,
+              out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """y = x @ W^T with W[n, k] = (q[n, k] - z[n, k / g]) s[n, k / g] held in 4 bits.
+
+    x (T, K) bf16 or fp16; packed (N, K / 2) uint8, two values a byte, the even
+    k in the low half; scales (N, K / g) fp16, bf16 or fp32; zeros (N, K / g)
+    uint8, or None for 8 everywhere (the layout ``quantize_w4`` returns).
+    With ``offsets`` the weights have a leading expert dimension and the rows
+    of x come in groups.  Returns (T, N) in x's dtype or fp32.  Made for few
+    rows a matrix (the weights' bytes bound it); any number is right.
+    """
+    xp, pp = x.data_ptr(), packed.data_ptr()
+    key = (x.shape, x.stride(), x.dtype, packed.shape, packed.stride(), packed.dtype, scales.shape,
+           scales.stride(), scales.dtype, out_dtype, x.get_device(), packed.get_device(), scales.get_device(),
+           xp % 16, pp % 16,
+           None if zeros is None else (zeros.shape, zeros.stride(), zeros.dtype, zeros.get_device()),
+           None if offsets is None else (offsets.shape, offsets.stride(), offsets.dtype, offsets.get_device()))
+    plan = _PLANS.kept.get(key) or _plan_w4(key, x, packed, scales, zeros, offsets, out_dtype)
+    if plan.copy and not plan.empty:
+        packed = packed.contiguous()
+        return matmul_w4(_as_operand(x), packed.clone() if packed.data_ptr() % 16 else packed, scales.contiguous(),
+                         None if zeros is None else zeros.contiguous(), offsets=offsets, out_dtype=out_dtype)
+    y = x.new_empty(plan.shape, dtype=plan.dtype)
+    if not plan.empty:
+        args = plan.args
+        args.x, args.packed, args.scales, args.y = xp, pp, scales.data_ptr(), y.data_ptr()
+        args.zeros = None if zeros is None else zeros.data_ptr()
+        args.offsets = None if offsets is None else offsets.data_ptr()
+        _launch(plan)
     return y

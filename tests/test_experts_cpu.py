@@ -99,7 +99,9 @@ def test_library_entries_validate_without_a_launch():
     n0 = lib.oz_launch_count()
 
     def grouped(dtype=_lib.OZ_F16, out=_lib.OZ_F16, groups=2, rows=4, k=8, n=8, x=p, y=p, ldy=8):
-        return lib.oz_grouped_matmul(x, p, p, 0, dtype, out, groups, rows, k, n, k, k * n, n, 1, y, ldy, None)
+        return lib.oz_grouped_matmul(_lib.GroupedArgs(x, p, p, y, rows, k, n, k, k * n, n, 1, ldy, groups, 0,
+                                                      dtype, out), None)
+    assert lib.oz_grouped_matmul(None, None) == _lib.OZ_ERR_INVALID
     assert grouped(dtype=_lib.OZ_F32) == _lib.OZ_ERR_UNSUPPORTED
     assert grouped(out=_lib.OZ_BF16) == _lib.OZ_ERR_UNSUPPORTED
     assert grouped(groups=0) == _lib.OZ_ERR_INVALID
@@ -113,15 +115,17 @@ def test_library_entries_validate_without_a_launch():
     assert grouped(k=12) == _lib.OZ_ERR_INVALID          # rows 24 bytes apart
 
     def wgrad(dtype=_lib.OZ_F16, groups=2, dw=p, k=8):
-        return lib.oz_grouped_wgrad(p, p, p, 0, dtype, dtype, groups, 4, k, 8, 8, 8, dw, None)
+        return lib.oz_grouped_wgrad(_lib.GroupedWgradArgs(p, p, p, dw, 4, k, 8, 8, 8, groups, 0, dtype, dtype), None)
+    assert lib.oz_grouped_wgrad(None, None) == _lib.OZ_ERR_INVALID
     assert wgrad(dtype=_lib.OZ_I8) == _lib.OZ_ERR_UNSUPPORTED
     assert wgrad(groups=-1) == _lib.OZ_ERR_INVALID
     assert wgrad(dw=None) == _lib.OZ_ERR_INVALID
     assert wgrad(k=0, dw=None) == _lib.OZ_OK
 
     def four(dtype=_lib.OZ_F16, scale=_lib.OZ_F16, experts=1, group=32, k=64, offsets=None, y=p, rows=1):
-        return lib.oz_matmul_w4(p, p, p, None, offsets, 0, dtype, scale, dtype, experts, rows, k, 8, group, k,
-                                4 * k, k // 2, 8 * 2, 2, y, 8, None)
+        return lib.oz_matmul_w4(_lib.W4Args(p, p, p, None, offsets, y, rows, k, 8, k, 4 * k, k // 2, 8 * 2, 2, 8,
+                                            experts, group, 0, dtype, scale, dtype), None)
+    assert lib.oz_matmul_w4(None, None) == _lib.OZ_ERR_INVALID
     assert four(dtype=_lib.OZ_F64) == _lib.OZ_ERR_UNSUPPORTED
     assert four(scale=_lib.OZ_I8) == _lib.OZ_ERR_UNSUPPORTED
     assert four(group=16) == _lib.OZ_ERR_INVALID
