@@ -23,8 +23,10 @@
 // With RAGGED the contraction runs over a tile's own range of rows
 // [k_begin, k_begin + k_len) of longer operands: the rows of the last block
 // past the range are overwritten with zeros in shared memory before they are
-// multiplied (in both operands: a zero times a stray NaN is a NaN), by each
-// CTA's MMA warp, so that the producer runs on to the next tile's blocks.
+// multiplied (in both operands: a zero times a stray NaN is a NaN), as far as
+// the last instruction of 16 reads.  A warp of its own does that as soon as the
+// block is there, ahead of the products (done by the MMA warp in its turn it
+// cost 8 of 48 us on 256 tiles of 4 blocks).
 //
 // With PASS > 0 an accumulator takes at most PASS blocks and the epilogue adds
 // the passes in registers: the tensor core cuts each sum off instead of
@@ -59,7 +61,7 @@ struct NoLookAhead {
   template <class P, class T> static __device__ void look_ahead(const P &, const T &, int, int, Ahead &) {}
 };
 
-template <class J> __host__ __device__ constexpr int threads() { return 64 + 32 * J::EW; }
+template <class J> __host__ __device__ constexpr int threads() { return 64 + 32 * J::EW + (J::RAGGED ? 32 : 0); }
 // columns of an epilogue warp (4 warps share the rows of a tile, a quarter each)
 template <class J> __host__ __device__ constexpr int warp_columns() { return J::NT * 4 / J::EW; }
 template <class J> __host__ __device__ constexpr int a_bytes() { return kRows * kLine; }
@@ -288,14 +290,13 @@ __global__ void __launch_bounds__(threads<J>(), 1)
                                        DEV_TIMEOUT_PRODUCER)))
             break;
           // a block's bytes count on the leader's barrier; those of a block
-          // that ends the range count on each CTA's own, for its MMA warp
+          // that ends the range count on each CTA's own, for its clearing warp
           const bool last = ragged && kb == blocks - 1;
           const uint32_t bar = leader_addr(&full[slot]);
           if (last) {
             mbar_arrive_expect_tx(&tail[slot], SB);
             turn ^= ((ended >> slot) & 1) << slot;
             ended |= 1u << slot;
-            if (leader) mbar_arrive(&full[slot]);
           } else if (leader) {
             mbar_arrive_expect_tx(&full[slot], PAIR * SB);
           }
@@ -333,7 +334,8 @@ __global__ void __launch_bounds__(threads<J>(), 1)
       }
       ok = __shfl_sync(0xffffffffu, (int)ok, 0);
     }
-    // every load must have landed before shared memory goes away
+    // every load must have landed before shared memory goes away (a block that ends a
+    // range counts on `full` only through the clearing warp)
     if (lane == 0)
       for (int slot = 0; J::RAGGED && slot < S; ++slot)
         if ((ended >> slot) & 1)
@@ -365,7 +367,7 @@ __global__ void __launch_bounds__(threads<J>(), 1)
     const uint64_t a_desc = operand_desc<J::AMN>(base);
     const uint64_t b_desc = operand_desc<J::BMN>(base + J::PLANES * a_bytes<J>());
     uint32_t slot = 0, phase = 0;
-    auto multiply = [&](uint32_t d, bool first) {
+    auto multiply = [&](uint32_t d, bool first, int steps) {
       const uint64_t ad = a_desc + slot * (SB >> 4), bd = b_desc + slot * (SB >> 4);
 #pragma unroll
       for (int q = 0; q < (J::PLANES == 2 ? 3 : 1); ++q) {
@@ -374,6 +376,7 @@ __global__ void __launch_bounds__(threads<J>(), 1)
         const uint64_t bq = bd + (q == 1 ? b_bytes<J>() >> 4 : 0);
 #pragma unroll
         for (int kk = 0; kk < kBlock / 16; ++kk) {
+          if (J::RAGGED && kk >= steps) break;
           const uint32_t add = (kk | q) ? 1u : (first ? 0u : 1u);
           if constexpr (PAIR == 2) tc_mma_pair<1>(d, aq + kk * a_step, bq + kk * b_step, idesc, add);
           else tc_mma<1>(d, aq + kk * a_step, bq + kk * b_step, idesc, add);
@@ -381,85 +384,31 @@ __global__ void __launch_bounds__(threads<J>(), 1)
       }
       release(&empty[slot]);
     };
-    auto advance = [&]() {
-      if (++slot == S) {
-        slot = 0;
-        phase ^= 1;
-      }
-    };
-    uint32_t tails = 0;                               // parity of each slot's tail barriers
     for (int i = unit; ok && walk.find(p, i, t); i += units) {
-      const int blocks = (int)((t.k_len + kBlock - 1) / kBlock);   // none: the epilogue writes zeros
-      const int rest = J::RAGGED ? (int)(t.k_len % kBlock) : 0;
-      const int whole = blocks - (rest ? 1 : 0);
-      const uint32_t slot0 = slot, phase0 = phase;
-      uint32_t d = 0;
-      auto start = [&]() {
-        const int buf = done & 1;
-        if (!wait(&acc_empty[buf], ((done >> 1) & 1) ^ 1)) return false;
-        tc_fence_after();
-        d = tmem + (uint32_t)(buf * NT);
-        return true;
-      };
-      auto end = [&]() {
-        release(&acc_full[done & 1]);
-        ++done;
-      };
       if (lane == 0 && leader) {
+        const int blocks = (int)((t.k_len + kBlock - 1) / kBlock);   // none: the epilogue writes zeros
+        const int rest = J::RAGGED ? (int)(t.k_len % kBlock) : 0;
         // accumulator by accumulator: all blocks, or PASS at a time
         int kb = 0;
-        while (kb < whole) {
-          const int stop = J::PASS ? min(whole, kb + J::PASS) : whole;
-          if (!(ok = start())) break;
+        while (kb < blocks) {
+          const int stop = J::PASS ? min(blocks, kb + J::PASS) : blocks;
+          const int buf = done & 1;
+          if (!(ok = wait(&acc_empty[buf], ((done >> 1) & 1) ^ 1))) break;
+          tc_fence_after();
+          const uint32_t d = tmem + (uint32_t)(buf * NT);
           bool first = true;
           for (; kb < stop; ++kb) {
             if (!(ok = wait(&full[slot], phase))) break;
-            multiply(d, first);
+            multiply(d, first, rest && kb == blocks - 1 ? (rest + 15) / 16 : kBlock / 16);
             first = false;
-            advance();
-          }
-          if (!ok) break;
-          if (kb < whole || !rest || (J::PASS && kb % (J::PASS + !J::PASS) == 0)) end();
-        }
-      }
-      if (whole > 0) {                                // the other lanes, and where this one stopped
-        const uint32_t n = slot0 + (uint32_t)whole;
-        slot = n % S;
-        phase = phase0 ^ (n / S & 1);
-      }
-      if constexpr (J::RAGGED) {
-        if (rest) {
-          unsigned char *st = smem + slot * SB;
-          const uint32_t parity = (tails >> slot) & 1;
-          ok = __shfl_sync(0xffffffffu, (int)ok, 0);
-          ok = ok && mbar_wait_bounded(&tail[slot], parity, abort_flag, DEV_TIMEOUT_MMA);
-          ok = __all_sync(0xffffffffu, ok);
-          if (ok) {
-            // rows [rest, 64) of every chunk: whole 128-byte lines, so the swizzle does not matter
-            constexpr int chunks = SB / (kBlock * kLine);
-            const int pieces = (kBlock - rest) * 8;          // 16-byte pieces of a chunk's lines
-            for (int c = 0; c < chunks; ++c)
-              for (int v = lane; v < pieces; v += 32)
-                *reinterpret_cast<uint4 *>(st + c * (kBlock * kLine) + rest * kLine + v * 16) =
-                    make_uint4(0, 0, 0, 0);
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-              if (leader) {
-                const bool first = whole == 0 || (J::PASS && whole % (J::PASS + !J::PASS) == 0);
-                ok = (!first || start()) && wait(&full[slot], phase);
-                if constexpr (PAIR == 2) ok = ok && wait(&peer_tail[slot], parity);
-                if (ok) {
-                  multiply(d, first);
-                  end();
-                }
-              } else {
-                mbar_arrive_remote(leader_addr(&peer_tail[slot]));
-              }
+            if (++slot == S) {
+              slot = 0;
+              phase ^= 1;
             }
           }
-          tails ^= 1u << slot;
-          advance();
+          if (!ok) break;
+          release(&acc_full[buf]);
+          ++done;
         }
       }
       ok = __shfl_sync(0xffffffffu, (int)ok, 0);
@@ -468,6 +417,41 @@ __global__ void __launch_bounds__(threads<J>(), 1)
       if constexpr (PAIR == 2) tc_commit_pair(smem_u32(drain));
       else tc_commit(drain);
       mbar_wait_bounded(drain, 0, abort_flag, DEV_TIMEOUT_MMA);
+    }
+  } else if (J::RAGGED && warp == 2 + J::EW) {
+    // ------------------------------------------------------------ clearing
+    typename J::Walk walk(p);
+    Tile t;
+    uint32_t it = 0, turn = 0;                        // parity of each slot's tail barriers
+    bool ok = true;
+    for (int i = unit; ok && walk.find(p, i, t); i += units) {
+      const int blocks = (int)((t.k_len + kBlock - 1) / kBlock), rest = (int)(t.k_len % kBlock);
+      it += blocks;
+      if (rest == 0) continue;
+      const uint32_t slot = (it - 1) % S, parity = (turn >> slot) & 1;
+      turn ^= 1u << slot;
+      unsigned char *st = smem + slot * SB;
+      ok = mbar_wait_bounded(&tail[slot], parity, abort_flag, DEV_TIMEOUT_PRODUCER);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      // rows [rest, up to a multiple of 16) of every chunk: whole 128-byte lines, so
+      // the swizzle does not matter
+      constexpr int chunks = SB / (kBlock * kLine);
+      const int pieces = ((rest + 15) / 16 * 16 - rest) * 8;  // 16-byte pieces of a chunk's lines
+      for (int c = 0; c < chunks; ++c)
+        for (int v = lane; v < pieces; v += 32)
+          *reinterpret_cast<uint4 *>(st + c * (kBlock * kLine) + rest * kLine + v * 16) = make_uint4(0, 0, 0, 0);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        if (leader) {
+          if constexpr (PAIR == 2) ok = wait_cluster(&peer_tail[slot], parity, abort_flag, DEV_TIMEOUT_PRODUCER);
+          if (ok) mbar_arrive(&full[slot]);
+        } else {
+          mbar_arrive_remote(leader_addr(&peer_tail[slot]));
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, (int)ok, 0);
     }
   } else {
     // ------------------------------------------------------------ epilogue
