@@ -259,13 +259,19 @@ int oz_cross_gemm_arrivals(const void *a_slices, const void *b_slices, const flo
  *   offsets   : device int32 (or int64, offsets_64 != 0) [groups + 1], read on
  *               the device only and clamped to [0, rows]
  *   y         : (rows, n), row pitch ldy, of x's type or fp32 (out_dtype)
- * Operands start on 16-byte boundaries and their other strides are multiples
- * of 8 elements.  Sums are held in fp32 and rounded once.
+ *   workspace : an operand that does not start on a 16-byte boundary, or whose
+ *               other strides are not positive multiples of 8 elements, is
+ *               copied here first (256-byte aligned): its rows padded to
+ *               multiples of 8 elements, each copy to a multiple of 256 bytes;
+ *               NULL where none is needed
+ * Sums are held in fp32 and rounded once.
  */
 typedef struct {
   const void *x, *w, *offsets;
   void *y;
   int64_t rows, k, n, x_sr, w_se, w_sk, w_sn, ldy;
+  void *workspace;
+  int64_t workspace_bytes;
   int32_t groups, offsets_64, dtype, out_dtype;
 } oz_grouped_args;
 int oz_grouped_matmul(const oz_grouped_args *args, void *stream);
@@ -273,13 +279,15 @@ int oz_grouped_matmul(const oz_grouped_args *args, void *stream);
 /*
  * Weight gradient of oz_grouped_matmul:
  *   dw[e] = sum over the rows r of group e of x[r]^T dy[r]   (0 for an empty group)
- * x (rows, k) and dy (rows, n) as x there, row pitches x_sr and dy_sr; dw:
+ * x (rows, k) and dy (rows, n) as x there, row pitches x_sr and dy_sr, workspace as there; dw:
  * contiguous (groups, k, n) of the operands' type or fp32 (out_dtype).
  */
 typedef struct {
   const void *x, *dy, *offsets;
   void *dw;
   int64_t rows, k, n, x_sr, dy_sr;
+  void *workspace;
+  int64_t workspace_bytes;
   int32_t groups, offsets_64, dtype, out_dtype;
 } oz_grouped_wgrad_args;
 int oz_grouped_wgrad(const oz_grouped_wgrad_args *args, void *stream);

@@ -28,18 +28,20 @@ OZ_IPC_HANDLE_BYTES = 64
 _i64, _i32, _u32, _vp, _int = ctypes.c_int64, ctypes.c_int32, ctypes.c_uint32, ctypes.c_void_p, ctypes.c_int
 
 
-def _struct(name, pointers, int64s, int32s):
-    """A structure of the header: pointers, then 64-bit, then 32-bit integers."""
-    fields = [(f, t) for names, t in ((pointers, _vp), (int64s, _i64), (int32s, _i32)) for f in names.split()]
-    return type(name, (ctypes.Structure,), {"_fields_": fields})
+def _struct(name, *fields):
+    """A structure of the header: ("names", type) groups in its order."""
+    return type(name, (ctypes.Structure,), {"_fields_": [(f, t) for names, t in fields for f in names.split()]})
 
 
-GroupedArgs = _struct("GroupedArgs", "x w offsets y", "rows k n x_sr w_se w_sk w_sn ldy",
-                      "groups offsets_64 dtype out_dtype")
-GroupedWgradArgs = _struct("GroupedWgradArgs", "x dy offsets dw", "rows k n x_sr dy_sr",
-                           "groups offsets_64 dtype out_dtype")
-W4Args = _struct("W4Args", "x packed scales zeros offsets y", "rows k n x_sr p_se p_sn s_se s_sn ldy",
-                 "experts group offsets_64 dtype scale_dtype out_dtype")
+GroupedArgs = _struct("GroupedArgs", ("x w offsets y", _vp), ("rows k n x_sr w_se w_sk w_sn ldy", _i64),
+                      ("workspace", _vp), ("workspace_bytes", _i64),
+                      ("groups offsets_64 dtype out_dtype", _i32))
+GroupedWgradArgs = _struct("GroupedWgradArgs", ("x dy offsets dw", _vp), ("rows k n x_sr dy_sr", _i64),
+                           ("workspace", _vp), ("workspace_bytes", _i64),
+                           ("groups offsets_64 dtype out_dtype", _i32))
+W4Args = _struct("W4Args", ("x packed scales zeros offsets y", _vp),
+                 ("rows k n x_sr p_se p_sn s_se s_sn ldy", _i64),
+                 ("experts group offsets_64 dtype scale_dtype out_dtype", _i32))
 
 SIGNATURES = {
     "oz_compute_split_bits": (_int, [_i64, _int, ctypes.POINTER(_i32)]),

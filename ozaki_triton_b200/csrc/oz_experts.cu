@@ -100,7 +100,7 @@ struct RowTile { int row, rows, column; };   // first row, rows from there to th
 
 // y = x w: A is the rows of x, B the columns of w[e].
 template <typename O, int PAIR_, int NT_, bool BMN_> struct RowsJob : NoLookAhead {
-  static constexpr int PAIR = PAIR_, NT = NT_, EW = NT_ >= 128 ? 16 : 8, PLANES = 1, PASS = sizeof(O) == 4 ? 8 : 0;
+  static constexpr int PAIR = PAIR_, NT = NT_, PLANES = 1, PASS = sizeof(O) == 4 ? 8 : 0;
   static constexpr bool AMN = false, BMN = BMN_, RAGGED = false;
   using Params = GroupedParams;
   using Extra = RowTile;
@@ -124,7 +124,7 @@ template <typename O, int PAIR_, int NT_, bool BMN_> struct RowsJob : NoLookAhea
   static __device__ void epilogue(const Params &p, const TileOf<Extra> &t, const Source &source, int row,
                                   int column, unsigned char *mine, Ahead &) {
     const int64_t c0 = t.extra.column + column;
-    write_rows<O, NT * 4 / EW>(source, mine,
+    write_rows<O, NT / 2>(source, mine,
                           static_cast<O *>(p.out) + (int64_t)(t.extra.row + row) * p.ld + c0, p.ld,
                           t.extra.rows - row, p.n - c0, p.vectors);
   }
@@ -135,7 +135,7 @@ template <typename O, int PAIR_, int NT_, bool BMN_> struct RowsJob : NoLookAhea
 // 128 columns of w[e], B up to NT rows of x, so a tile's weights are read
 // once and hardly any of the staged bytes belong to rows that are not there.
 template <typename O, int NT_, bool AMN_> struct ColumnsJob : NoLookAhead {
-  static constexpr int PAIR = 1, NT = NT_, EW = 8, PLANES = 1, PASS = sizeof(O) == 4 ? 8 : 0;
+  static constexpr int PAIR = 1, NT = NT_, PLANES = 1, PASS = sizeof(O) == 4 ? 8 : 0;
   static constexpr bool AMN = AMN_, BMN = false, RAGGED = false;
   using Params = GroupedParams;
   using Extra = RowTile;
@@ -179,7 +179,7 @@ struct WeightTile { int row, column, group; };
 // dw[e] = x^T dy over the group's rows: both operands are stored across the
 // contraction, whose range is the group.
 template <typename O, int PAIR_, int NT_> struct WeightsJob : NoLookAhead {
-  static constexpr int PAIR = PAIR_, NT = NT_, EW = NT_ >= 128 ? 16 : 8, PLANES = 1, PASS = sizeof(O) == 4 ? 8 : 0;
+  static constexpr int PAIR = PAIR_, NT = NT_, PLANES = 1, PASS = sizeof(O) == 4 ? 8 : 0;
   static constexpr bool AMN = true, BMN = true, RAGGED = true;
   using Params = GroupedParams;
   using Extra = WeightTile;
@@ -210,7 +210,7 @@ template <typename O, int PAIR_, int NT_> struct WeightsJob : NoLookAhead {
   static __device__ void epilogue(const Params &p, const TileOf<Extra> &t, const Source &source, int row,
                                   int column, unsigned char *mine, Ahead &) {
     const int64_t r0 = t.extra.row + row, c0 = t.extra.column + column;
-    write_rows<O, NT * 4 / EW>(source, mine,
+    write_rows<O, NT / 2>(source, mine,
                           static_cast<O *>(p.out) + ((int64_t)t.extra.group * p.k + r0) * p.ld + c0,
                           p.ld, (int)(p.k - r0), p.n - c0, p.vectors);
   }
@@ -237,14 +237,81 @@ int64_t pitch_bytes(int64_t stride, int64_t count, int64_t inner) {
   return 2 * (count <= 1 ? (inner + 7) / 8 * 8 : stride);
 }
 
-int check_operand(const char *name, const void *p, int64_t rows, int64_t row_stride, int64_t mats,
-                  int64_t mat_stride) {
-  if ((uintptr_t)p % 16 != 0 || !pitch_ok(row_stride, rows) || !pitch_ok(mat_stride, mats))
-    return set_error(OZ_ERR_INVALID,
-                     "%s must start on a 16-byte boundary, its strides must be multiples of 16 bytes "
-                     "(row %lld, matrix %lld elements)",
-                     name, (long long)row_stride, (long long)mat_stride);
-  return OZ_OK;
+bool readable(const void *p, int64_t rows, int64_t row_stride, int64_t mats, int64_t mat_stride) {
+  return (uintptr_t)p % 16 == 0 && pitch_ok(row_stride, rows) && pitch_ok(mat_stride, mats);
+}
+
+// Copies of operands whose rows the copy unit cannot address (16-byte boundaries
+// and pitches): rows of 2-byte elements with unit stride to rows 16 bytes apart,
+// both operands of a call in one launch.  A warp takes 128 pairs of a row.
+struct Repitch {
+  const unsigned short *from;
+  unsigned short *to;
+  int64_t from_row, from_mat, rows, mats, to_row;
+  int inner;
+};
+struct RepitchTwo { Repitch job[2]; };
+
+__global__ void __launch_bounds__(256) repitch_kernel(const RepitchTwo two) {
+  const Repitch &p = two.job[blockIdx.y];
+  const int lane = threadIdx.x % 32, pieces = (p.inner + 255) / 256;
+  const int64_t all = p.rows * p.mats * pieces;
+  for (int64_t v = (int64_t)blockIdx.x * 8 + threadIdx.x / 32; v < all; v += (int64_t)gridDim.x * 8) {
+    const int64_t line = v / pieces, mat = line / p.rows;
+    const int first = (int)(v - line * pieces) * 256 + lane * 2;
+    const unsigned short *from = p.from + mat * p.from_mat + (line - mat * p.rows) * p.from_row;
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int c = first + i * 64;
+      const uint32_t a = c < p.inner ? __ldg(from + c) : 0, b = c + 1 < p.inner ? __ldg(from + c + 1) : 0;
+      w[i] = a | b << 16;
+    }
+    uint32_t *to = reinterpret_cast<uint32_t *>(p.to + line * p.to_row);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (first + i * 64 < p.inner) to[(first + i * 64) / 2] = w[i];
+  }
+}
+
+// An operand as it is, or its copy in the workspace.
+struct Operand {
+  const void *p;
+  int64_t rows, row, mats, mat;
+  int inner;
+};
+int64_t copy_bytes(const Operand &o) {
+  if (o.p && readable(o.p, o.rows, o.row, o.mats, o.mat)) return 0;
+  return (o.rows * o.mats * ((o.inner + 7) / 8 * 8) * 2 + 255) / 256 * 256;
+}
+int lay_out(Operand *ops, void *workspace, int64_t workspace_bytes, cudaStream_t st) {
+  RepitchTwo two{};
+  int n = 0;
+  int64_t at = 0, most = 0;
+  for (int i = 0; i < 2; ++i) {
+    Operand &o = ops[i];
+    const int64_t bytes = copy_bytes(o);
+    if (!bytes) continue;
+    if (!workspace || (uintptr_t)workspace % 256 != 0 || workspace_bytes < at + bytes)
+      return set_error(OZ_ERR_INVALID,
+                       "an operand off the 16-byte boundaries needs a workspace of %lld bytes (256-byte "
+                       "aligned), got %lld at %p",
+                       (long long)(at + bytes), (long long)workspace_bytes, workspace);
+    if ((uintptr_t)o.p % 2 != 0) return set_error(OZ_ERR_INVALID, "an operand is not aligned to its elements");
+    unsigned char *to = static_cast<unsigned char *>(workspace) + at;
+    const int64_t pitch = (o.inner + 7) / 8 * 8;
+    two.job[n++] = Repitch{static_cast<const unsigned short *>(o.p), reinterpret_cast<unsigned short *>(to), o.row,
+                           o.mat, o.rows, o.mats, pitch, o.inner};
+    o.p = to;
+    o.row = pitch;
+    o.mat = pitch * o.rows;
+    at += bytes;
+    most = max(most, (o.rows * o.mats * ((o.inner + 255) / 256) + 7) / 8);
+  }
+  if (!n) return OZ_OK;
+  count_launch();
+  repitch_kernel<<<dim3((unsigned)min(most, (int64_t)sm_count() * 16), n), 256, 0, st>>>(two);
+  return check_cuda(cudaGetLastError(), "repitch_kernel launch");
 }
 
 template <class J>
@@ -303,8 +370,8 @@ int wgrad(const void *x, const void *dy, int64_t x_sr, int64_t dy_sr, const Grou
 
 extern "C" int oz_grouped_matmul(const oz_grouped_args *args, void *stream) {
   if (!args) return oz::set_error(OZ_ERR_INVALID, "null arguments");
-  const auto [x, w, offsets, y, rows, k, n, x_sr, w_se, w_sk, w_sn, ldy, groups, offsets_64, dtype,
-              out_dtype] = *args;
+  const auto [x, w, offsets, y, rows, k, n, x_sr, w_se, w_sk, w_sn, ldy, workspace, workspace_bytes, groups,
+              offsets_64, dtype, out_dtype] = *args;
   using namespace oz;
   if (int rc = check_grouped(dtype, out_dtype, groups, rows, k, n)) return rc;
   if (rows == 0 || n == 0) return OZ_OK;
@@ -320,19 +387,20 @@ extern "C" int oz_grouped_matmul(const oz_grouped_args *args, void *stream) {
   const bool across = w_sn == 1 || (n == 1 && w_sk != 1);
   if (!across && w_sk != 1 && k != 1)
     return set_error(OZ_ERR_INVALID, "w must have a unit stride along k or n");
-  const int64_t w_row = across ? w_sk : w_sn;
-  if (int rc = check_operand("x", x, rows, x_sr, 1, 0)) return rc;
-  if (int rc = check_operand("w", w, across ? k : n, w_row, groups, w_se)) return rc;
+  Operand ops[2] = {{x, rows, x_sr, 1, 0, (int)k},
+                    {w, across ? k : n, across ? w_sk : w_sn, groups, w_se, (int)(across ? n : k)}};
+  if (int rc = lay_out(ops, workspace, workspace_bytes, st)) return rc;
   GroupedParams p{offsets, y, ldy, offsets_64, groups, (int)rows, (int)k, (int)n, 0,
                   (uintptr_t)y % 16 == 0 && ldy * es % 16 == 0, tile::instruction(dtype)};
-  if (out_dtype == OZ_F32) return grouped<float>(x, w, x_sr, w_se, across, w_row, p, st);
-  if (dtype == OZ_F16) return grouped<__half>(x, w, x_sr, w_se, across, w_row, p, st);
-  return grouped<__nv_bfloat16>(x, w, x_sr, w_se, across, w_row, p, st);
+  if (out_dtype == OZ_F32) return grouped<float>(ops[0].p, ops[1].p, ops[0].row, ops[1].mat, across, ops[1].row, p, st);
+  if (dtype == OZ_F16) return grouped<__half>(ops[0].p, ops[1].p, ops[0].row, ops[1].mat, across, ops[1].row, p, st);
+  return grouped<__nv_bfloat16>(ops[0].p, ops[1].p, ops[0].row, ops[1].mat, across, ops[1].row, p, st);
 }
 
 extern "C" int oz_grouped_wgrad(const oz_grouped_wgrad_args *args, void *stream) {
   if (!args) return oz::set_error(OZ_ERR_INVALID, "null arguments");
-  const auto [x, dy, offsets, dw, rows, k, n, x_sr, dy_sr, groups, offsets_64, dtype, out_dtype] = *args;
+  const auto [x, dy, offsets, dw, rows, k, n, x_sr, dy_sr, workspace, workspace_bytes, groups, offsets_64, dtype,
+              out_dtype] = *args;
   using namespace oz;
   if (int rc = check_grouped(dtype, out_dtype, groups, rows, k, n)) return rc;
   if (k == 0 || n == 0) return OZ_OK;
@@ -342,11 +410,11 @@ extern "C" int oz_grouped_wgrad(const oz_grouped_wgrad_args *args, void *stream)
   if (rows == 0)
     return check_cuda(cudaMemsetAsync(dw, 0, (size_t)(groups * k * n * es), st), "cudaMemsetAsync");
   if (!offsets || !x || !dy) return set_error(OZ_ERR_INVALID, "null pointer");
-  if (int rc = check_operand("x", x, rows, x_sr, 1, 0)) return rc;
-  if (int rc = check_operand("dy", dy, rows, dy_sr, 1, 0)) return rc;
+  Operand ops[2] = {{x, rows, x_sr, 1, 0, (int)k}, {dy, rows, dy_sr, 1, 0, (int)n}};
+  if (int rc = lay_out(ops, workspace, workspace_bytes, st)) return rc;
   GroupedParams p{offsets, dw, n, offsets_64, groups, (int)rows, (int)k, (int)n, 0,
                   (uintptr_t)dw % 16 == 0 && n * es % 16 == 0, tile::instruction(dtype)};
-  if (out_dtype == OZ_F32) return wgrad<float>(x, dy, x_sr, dy_sr, p, st);
-  if (dtype == OZ_F16) return wgrad<__half>(x, dy, x_sr, dy_sr, p, st);
-  return wgrad<__nv_bfloat16>(x, dy, x_sr, dy_sr, p, st);
+  if (out_dtype == OZ_F32) return wgrad<float>(ops[0].p, ops[1].p, ops[0].row, ops[1].row, p, st);
+  if (dtype == OZ_F16) return wgrad<__half>(ops[0].p, ops[1].p, ops[0].row, ops[1].row, p, st);
+  return wgrad<__nv_bfloat16>(ops[0].p, ops[1].p, ops[0].row, ops[1].row, p, st);
 }

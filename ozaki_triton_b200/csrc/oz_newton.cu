@@ -307,7 +307,7 @@ struct StepTile { int z, row, column; bool mirror; };
 // S = X X^T (IN 0) and P = b S + c S S (IN slices of S): tiles (i, j) on and
 // below the diagonal, the others their mirror images.
 template <int PAIR_, int NT_, int PLANES_, int IN> struct SymmetricJob {
-  static constexpr int PAIR = PAIR_, NT = NT_, EW = 8, PLANES = PLANES_, PASS = (PLANES_ - 1) * 4;
+  static constexpr int PAIR = PAIR_, NT = NT_, PLANES = PLANES_, PASS = (PLANES_ - 1) * 4;
   static constexpr bool AMN = false, BMN = false, RAGGED = false;
   static constexpr int R = kRows * PAIR / NT;           // column tiles as wide as a tile is high
   using Params = StepParams;
@@ -346,7 +346,7 @@ template <int PAIR_, int NT_, int PLANES_, int IN> struct SymmetricJob {
     const int r0 = t.extra.row + row, rows = p.rows - r0;
     if (rows <= 0) return;
 #pragma unroll
-    for (int c = 0; c < NT * 4 / EW; c += 32) {
+    for (int c = 0; c < NT / 2; c += 32) {
       const int c0 = t.extra.column + column + c, cols = p.cols - c0;
       if (cols <= 0) continue;
       float v[32];
@@ -354,7 +354,7 @@ template <int PAIR_, int NT_, int PLANES_, int IN> struct SymmetricJob {
       if constexpr (PASS == 0) {
 #pragma unroll
         for (int q = 0; q < IN; ++q) in[q] = early.in[q];
-        if (c + 32 < NT * 4 / EW && cols > 32) fetch_in<IN>(p, t.extra.z, r0, c0 + 32, early.in);
+        if (c + 32 < NT / 2 && cols > 32) fetch_in<IN>(p, t.extra.z, r0, c0 + 32, early.in);
       } else {
         fetch_in<IN>(p, t.extra.z, r0, c0, in);
       }
@@ -377,7 +377,7 @@ template <int PAIR_, int NT_, int PLANES_, int IN> struct SymmetricJob {
 // X <- a X + P X: A is the rows of P, B the columns of X.
 template <int PAIR_, int NT_, int PLANES_> struct UpdateJob {
   static constexpr int IN = 2;
-  static constexpr int PAIR = PAIR_, NT = NT_, EW = 8, PLANES = PLANES_, PASS = (PLANES_ - 1) * 4;
+  static constexpr int PAIR = PAIR_, NT = NT_, PLANES = PLANES_, PASS = (PLANES_ - 1) * 4;
   static constexpr bool AMN = false, BMN = true, RAGGED = false;
   using Params = StepParams;
   using Extra = StepTile;
@@ -412,7 +412,7 @@ template <int PAIR_, int NT_, int PLANES_> struct UpdateJob {
     const int r0 = t.extra.row + row, rows = p.rows - r0, lane = threadIdx.x % 32;
     if (rows <= 0) return;
 #pragma unroll
-    for (int c = 0; c < NT * 4 / EW; c += 32) {
+    for (int c = 0; c < NT / 2; c += 32) {
       const int c0 = t.extra.column + column + c, cols = p.cols - c0;
       if (cols <= 0) continue;
       float v[32];
@@ -420,7 +420,7 @@ template <int PAIR_, int NT_, int PLANES_> struct UpdateJob {
       if constexpr (PASS == 0) {
 #pragma unroll
         for (int q = 0; q < IN; ++q) in[q] = early.in[q];
-        if (c + 32 < NT * 4 / EW && cols > 32) fetch_in<IN>(p, t.extra.z, r0, c0 + 32, early.in);
+        if (c + 32 < NT / 2 && cols > 32) fetch_in<IN>(p, t.extra.z, r0, c0 + 32, early.in);
       } else {
         fetch_in<IN>(p, t.extra.z, r0, c0, in);
       }

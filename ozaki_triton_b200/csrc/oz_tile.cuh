@@ -6,11 +6,9 @@
 // moves the data and issues the matrix instructions:
 //   warp 0     TMA producer: 64-deep blocks of A and B into a ring of stages;
 //   warp 1     TMEM allocator and the one thread that issues tcgen05.mma;
-//   warps 2..  epilogue: the job's, from TMEM (fp32 accumulators, two buffers,
-//              so the epilogue of one tile runs under the products of the next).
-//              EW = 8 or 16 warps: a warp's epilogue is one chain of dependent
-//              steps, so more warps shorten it until it hides (the update of
-//              2048 x 2816 took 27,000 cycles a tile with 8, its products 16,400).
+//   warps 2-9  epilogue: the job's, from TMEM (fp32 accumulators, two buffers,
+//              so the epilogue of one tile runs under the products of the next;
+//              16 warps and a stage less were 2% slower forward, 10% for dw).
 // A tile is 128 * PAIR rows by NT columns; with PAIR = 2 two CTAs of a
 // cluster hold half of A's rows and half of B's columns each and one
 // cta_group::2 instruction multiplies both halves: each CTA then feeds 256
@@ -51,6 +49,7 @@ constexpr int kRows = 128;              // rows of one CTA's part of a tile
 constexpr int kBlock = 64;              // contraction elements of a stage
 constexpr int kLine = 128;              // bytes of a swizzled row
 constexpr int kMaxStages = 10;
+constexpr int kEpilogueWarps = 8;
 constexpr int kStagingBytes = 2048;     // of each epilogue warp: 32 rows of 64 bytes
 constexpr int kBarrierBytes = 512;
 constexpr int kSmemLimit = 227 * 1024;
@@ -61,19 +60,19 @@ struct NoLookAhead {
   template <class P, class T> static __device__ void look_ahead(const P &, const T &, int, int, Ahead &) {}
 };
 
-template <class J> __host__ __device__ constexpr int threads() { return 64 + 32 * J::EW + (J::RAGGED ? 32 : 0); }
+template <class J> __host__ __device__ constexpr int threads() { return 64 + 32 * kEpilogueWarps + (J::RAGGED ? 32 : 0); }
 // columns of an epilogue warp (4 warps share the rows of a tile, a quarter each)
-template <class J> __host__ __device__ constexpr int warp_columns() { return J::NT * 4 / J::EW; }
+template <class J> __host__ __device__ constexpr int warp_columns() { return J::NT * 4 / kEpilogueWarps; }
 template <class J> __host__ __device__ constexpr int a_bytes() { return kRows * kLine; }
 template <class J> __host__ __device__ constexpr int b_bytes() { return J::NT / J::PAIR * kLine; }
 template <class J> __host__ __device__ constexpr int stage_bytes() { return J::PLANES * (a_bytes<J>() + b_bytes<J>()); }
 template <class J> __host__ __device__ constexpr int stages() {
-  constexpr int room = kSmemLimit - 1024 - kBarrierBytes - J::EW * kStagingBytes;
+  constexpr int room = kSmemLimit - 1024 - kBarrierBytes - kEpilogueWarps * kStagingBytes;
   constexpr int n = room / stage_bytes<J>();
   return n < kMaxStages ? n : kMaxStages;
 }
 template <class J> __host__ __device__ constexpr int smem_bytes() {
-  return 1024 + stages<J>() * stage_bytes<J>() + J::EW * kStagingBytes + kBarrierBytes;
+  return 1024 + stages<J>() * stage_bytes<J>() + kEpilogueWarps * kStagingBytes + kBarrierBytes;
 }
 
 // Where a tile's operands lie: first row (or column) and matrix of A and B in
@@ -216,7 +215,7 @@ __global__ void __launch_bounds__(threads<J>(), 1)
   extern __shared__ unsigned char smem_raw[];
   unsigned char *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   unsigned char *staging = smem + S * SB;
-  uint64_t *full = reinterpret_cast<uint64_t *>(staging + J::EW * kStagingBytes);
+  uint64_t *full = reinterpret_cast<uint64_t *>(staging + kEpilogueWarps * kStagingBytes);
   uint64_t *empty = full + kMaxStages;
   uint64_t *acc_full = empty + kMaxStages;            // [2]
   uint64_t *acc_empty = acc_full + 2;                 // [2]
@@ -240,7 +239,7 @@ __global__ void __launch_bounds__(threads<J>(), 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], PAIR * J::EW);
+      mbar_init(&acc_empty[i], PAIR * kEpilogueWarps);
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -418,7 +417,7 @@ __global__ void __launch_bounds__(threads<J>(), 1)
       else tc_commit(drain);
       mbar_wait_bounded(drain, 0, abort_flag, DEV_TIMEOUT_MMA);
     }
-  } else if (J::RAGGED && warp == 2 + J::EW) {
+  } else if (J::RAGGED && warp == 2 + kEpilogueWarps) {
     // ------------------------------------------------------------ clearing
     typename J::Walk walk(p);
     Tile t;
@@ -509,7 +508,7 @@ __global__ void __launch_bounds__(threads<J>(), 1)
         if (some) hand_back();
       }
     }
-    J::finish(p, (blockIdx.x * J::EW + warp - 2), gridDim.x * J::EW);
+    J::finish(p, (blockIdx.x * kEpilogueWarps + warp - 2), gridDim.x * kEpilogueWarps);
   }
 
   tc_fence_before();

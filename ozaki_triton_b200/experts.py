@@ -110,11 +110,15 @@ def _along(w: torch.Tensor) -> torch.Tensor:
     return w.transpose(1, 2) if w.stride(1) == 1 and w.stride(2) != 1 else w
 
 
-def _as_weights(w: torch.Tensor) -> torch.Tensor:
-    if _readable(_along(w)):
-        return w
-    across = w.stride(1) == 1 and w.stride(2) != 1
-    return _copied(w.transpose(1, 2)).transpose(1, 2) if across else _copied(w)
+def _unit(t: torch.Tensor) -> bool:
+    return t.stride(-1) == 1 or t.shape[-1] == 1
+
+
+def _copy_bytes(t: torch.Tensor) -> int:
+    """Workspace of the library's copy of t, none where it can be read as it is."""
+    if _readable(t):
+        return 0
+    return (t[..., 0].numel() * ((t.shape[-1] + 7) // 8 * 8) * 2 + 255) // 256 * 256
 
 
 def _check_grouped(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor) -> None:
@@ -133,7 +137,7 @@ class _Plan:
     that a repeated small product pays for its allocation and one library
     call (checking and converting everything again took 5 us of 13)."""
 
-    __slots__ = ("args", "ref", "call", "shape", "dtype", "empty", "copy", "device")
+    __slots__ = ("args", "ref", "call", "shape", "dtype", "empty", "copy", "device", "workspace")
 
 
 class _Plans(threading.local):
@@ -164,11 +168,12 @@ def _launch(plan: _Plan) -> None:
 
 
 def _make_plan(call: str, args: ctypes.Structure, shape: Tuple[int, ...], dtype: torch.dtype, device: int,
-               empty: bool, copy: bool) -> _Plan:
+               empty: bool, copy: bool, workspace: int = 0) -> _Plan:
     plan = _Plan()
     plan.args, plan.ref = args, ctypes.byref(args)
     plan.call = getattr(_lib.load(), call) if not empty else None
     plan.shape, plan.dtype, plan.device, plan.empty, plan.copy = shape, dtype, device, empty, copy
+    plan.workspace = workspace
     return plan
 
 
@@ -178,26 +183,31 @@ def _plan_product(key, x, w, offsets, out_dtype) -> _Plan:
     device = _check_places(x, w, offsets)
     rows, k = x.shape
     groups, _, n = w.shape
-    copy = k > 0 and not (_readable(x) and _readable(_along(w)))
-    args = _lib.GroupedArgs(None, None, None, None, rows, k, n, x.stride(0), *w.stride(), n, groups,
-                            offsets.dtype is torch.int64, _OZ_DTYPE[x.dtype], _OZ_DTYPE[out_dtype])
+    copy, workspace = k > 0 and not (_unit(x) and _unit(_along(w))), 0
+    if k > 0 and rows > 0 and n > 0 and not copy:
+        workspace = _copy_bytes(x) + _copy_bytes(_along(w))
+    args = _lib.GroupedArgs(None, None, None, None, rows, k, n, x.stride(0), *w.stride(), n, None, workspace,
+                            groups, offsets.dtype is torch.int64, _OZ_DTYPE[x.dtype], _OZ_DTYPE[out_dtype])
     return _PLANS.keep(key, _make_plan("oz_grouped_matmul", args, (rows, n), out_dtype, device,
-                                       rows == 0 or n == 0, copy))
+                                       rows == 0 or n == 0, copy, workspace))
 
 
 def _product(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor,
              out_dtype: Optional[torch.dtype]) -> torch.Tensor:
-    # the addresses' alignment is part of the signature: _as_operand looks at it
+    # the addresses' alignment is part of the signature: it decides what is copied
     xp, wp = x.data_ptr(), w.data_ptr()
     key = (x.shape, x.stride(), x.dtype, w.shape, w.stride(), w.dtype, offsets.shape, offsets.stride(),
            offsets.dtype, out_dtype, x.get_device(), w.get_device(), offsets.get_device(), xp % 16, wp % 16)
     plan = _PLANS.kept.get(key) or _plan_product(key, x, w, offsets, out_dtype)
     if plan.copy:
-        return _product(_as_operand(x), _as_weights(w), offsets, out_dtype)
+        return _product(x if _unit(x) else _copied(x), w if _unit(_along(w)) else _copied(w), offsets, out_dtype)
     y = x.new_empty(plan.shape, dtype=plan.dtype)
     if not plan.empty:
         args = plan.args
         args.x, args.w, args.offsets, args.y = xp, wp, offsets.data_ptr(), y.data_ptr()
+        if plan.workspace:
+            workspace = x.new_empty((plan.workspace,), dtype=torch.uint8)
+            args.workspace = workspace.data_ptr()
         _launch(plan)
     return y
 
@@ -207,11 +217,13 @@ def _plan_weight_gradient(key, x, dy, offsets, groups, out_dtype) -> _Plan:
     device = _check_places(x, dy, offsets)
     rows, k = x.shape
     n = dy.shape[1]
-    copy = rows > 0 and not (_readable(x) and _readable(dy))
-    args = _lib.GroupedWgradArgs(None, None, None, None, rows, k, n, x.stride(0), dy.stride(0), groups,
-                                 offsets.dtype is torch.int64, _OZ_DTYPE[x.dtype], _OZ_DTYPE[out_dtype])
+    copy, workspace = rows > 0 and not (_unit(x) and _unit(dy)), 0
+    if rows > 0 and k > 0 and n > 0 and not copy:
+        workspace = _copy_bytes(x) + _copy_bytes(dy)
+    args = _lib.GroupedWgradArgs(None, None, None, None, rows, k, n, x.stride(0), dy.stride(0), None, workspace,
+                                 groups, offsets.dtype is torch.int64, _OZ_DTYPE[x.dtype], _OZ_DTYPE[out_dtype])
     return _PLANS.keep(key, _make_plan("oz_grouped_wgrad", args, (groups, k, n), out_dtype, device,
-                                       k == 0 or n == 0, copy))
+                                       k == 0 or n == 0, copy, workspace))
 
 
 def _weight_gradient(x: torch.Tensor, dy: torch.Tensor, offsets: torch.Tensor, groups: int,
@@ -221,11 +233,15 @@ def _weight_gradient(x: torch.Tensor, dy: torch.Tensor, offsets: torch.Tensor, g
            x.get_device(), dy.get_device(), offsets.get_device(), xp % 16, dp % 16)
     plan = _PLANS.kept.get(key) or _plan_weight_gradient(key, x, dy, offsets, groups, out_dtype)
     if plan.copy:
-        return _weight_gradient(_as_operand(x), _as_operand(dy), offsets, groups, out_dtype)
+        return _weight_gradient(x if _unit(x) else _copied(x), dy if _unit(dy) else _copied(dy), offsets, groups,
+                                out_dtype)
     dw = x.new_empty(plan.shape, dtype=plan.dtype)
     if not plan.empty:
         args = plan.args
         args.x, args.dy, args.offsets, args.dw = xp, dp, offsets.data_ptr(), dw.data_ptr()
+        if plan.workspace:
+            workspace = x.new_empty((plan.workspace,), dtype=torch.uint8)
+            args.workspace = workspace.data_ptr()
         _launch(plan)
     return dw
 
@@ -277,8 +293,8 @@ def grouped_matmul_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor,
         f"dy must be {(x.shape[0], w.shape[2])}, got {tuple(dy.shape)}"
     assert x.shape[1] == w.shape[1], f"contraction dim mismatch: x K={x.shape[1]}, w K={w.shape[1]}"
     dw_dtype = _out_dtype(dw_dtype, x.dtype)
-    if x.is_cuda and dy.is_cuda:
-        x, dy = _as_operand(x), _as_operand(dy)           # once for both products
+    if dy.is_cuda and not _readable(dy):
+        dy = _copied(dy)                                  # once for both products
     return (_product(dy, w.transpose(1, 2), offsets, None),
             _weight_gradient(x, dy, offsets, w.shape[0], dw_dtype))
 

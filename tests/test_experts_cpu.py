@@ -99,8 +99,8 @@ def test_library_entries_validate_without_a_launch():
     n0 = lib.oz_launch_count()
 
     def grouped(dtype=_lib.OZ_F16, out=_lib.OZ_F16, groups=2, rows=4, k=8, n=8, x=p, y=p, ldy=8):
-        return lib.oz_grouped_matmul(_lib.GroupedArgs(x, p, p, y, rows, k, n, k, k * n, n, 1, ldy, groups, 0,
-                                                      dtype, out), None)
+        return lib.oz_grouped_matmul(_lib.GroupedArgs(x, p, p, y, rows, k, n, k, k * n, n, 1, ldy, None, 0, groups,
+                                                      0, dtype, out), None)
     assert lib.oz_grouped_matmul(None, None) == _lib.OZ_ERR_INVALID
     assert grouped(dtype=_lib.OZ_F32) == _lib.OZ_ERR_UNSUPPORTED
     assert grouped(out=_lib.OZ_BF16) == _lib.OZ_ERR_UNSUPPORTED
@@ -112,10 +112,12 @@ def test_library_entries_validate_without_a_launch():
     assert grouped(y=None) == _lib.OZ_ERR_INVALID
     assert grouped(rows=0, y=None) == _lib.OZ_OK
     assert grouped(x=ctypes.c_void_p(264)) == _lib.OZ_ERR_INVALID
-    assert grouped(k=12) == _lib.OZ_ERR_INVALID          # rows 24 bytes apart
+    assert grouped(k=12) == _lib.OZ_ERR_INVALID          # rows 24 bytes apart, and no workspace
+    assert "workspace" in lib.oz_last_error().decode()
 
     def wgrad(dtype=_lib.OZ_F16, groups=2, dw=p, k=8):
-        return lib.oz_grouped_wgrad(_lib.GroupedWgradArgs(p, p, p, dw, 4, k, 8, 8, 8, groups, 0, dtype, dtype), None)
+        return lib.oz_grouped_wgrad(_lib.GroupedWgradArgs(p, p, p, dw, 4, k, 8, 8, 8, None, 0, groups, 0, dtype,
+                                                          dtype), None)
     assert lib.oz_grouped_wgrad(None, None) == _lib.OZ_ERR_INVALID
     assert wgrad(dtype=_lib.OZ_I8) == _lib.OZ_ERR_UNSUPPORTED
     assert wgrad(groups=-1) == _lib.OZ_ERR_INVALID
