@@ -326,10 +326,13 @@ int oz_matmul_w4(const oz_w4_args *args, void *stream);
  *   coefficients : host array of `steps` triples (a, b, c)
  *   num_splits   : fp16 slices of a matrix in the products, 1 or 2
  *   out          : contiguous (batch, m, n) of g's type
- *   workspace    : oz_orthogonalize_workspace_bytes() bytes, 256-byte aligned
+ *                  (small matrices, up to 128 rows or columns, are worked on in
+ *                  fp32 whatever it is)
+ *   workspace    : oz_orthogonalize_workspace_bytes() bytes, 256-byte aligned;
+ *                  may be 0 bytes and NULL
  */
 int64_t oz_orthogonalize_workspace_bytes(int dtype, int64_t batch, int64_t m, int64_t n,
-                                         int32_t num_splits);
+                                         int32_t steps, int32_t num_splits);
 int oz_orthogonalize(const void *g, int dtype, int64_t batch, int64_t m, int64_t n, int64_t g_sb,
                      int64_t g_sr, int64_t g_sc, int32_t steps, const double *coefficients,
                      double eps, int32_t num_splits, void *out, void *workspace,

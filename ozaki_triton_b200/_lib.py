@@ -68,7 +68,7 @@ SIGNATURES = {
     "oz_grouped_matmul": (_int, [ctypes.POINTER(GroupedArgs), _vp]),
     "oz_grouped_wgrad": (_int, [ctypes.POINTER(GroupedWgradArgs), _vp]),
     "oz_matmul_w4": (_int, [ctypes.POINTER(W4Args), _vp]),
-    "oz_orthogonalize_workspace_bytes": (_i64, [_int, _i64, _i64, _i64, _i32]),
+    "oz_orthogonalize_workspace_bytes": (_i64, [_int, _i64, _i64, _i64, _i32, _i32]),
     "oz_orthogonalize": (_int, [_vp, _int, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _vp,
                                 ctypes.c_double, _i32, _vp, _vp, _i64, _vp]),
     "oz_ipc_export": (_int, [_vp, _vp, ctypes.POINTER(_i64)]),

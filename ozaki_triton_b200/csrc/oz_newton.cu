@@ -474,6 +474,272 @@ template <int PAIR_, int NT_, int PLANES_> struct UpdateJob {
   static __device__ void finish(const Params &, int, int) {}
 };
 
+// ---------------------------------------------------------------------------
+// small matrices: all steps in one launch
+// ---------------------------------------------------------------------------
+// 17 launches of products that take a microsecond each cost 85 us for 12
+// matrices of 64 x 250; here a cluster of up to 8 CTAs keeps one matrix in
+// shared memory in fp32, a panel of X's columns in each CTA and S and P in
+// all of them: the panels' X X^T are added in the order of the ranks, P is
+// computed a few rows a CTA and handed to the others, and a X + P X needs
+// nothing of another panel.  fp32 FMAs are enough here (and rounded sums more
+// exact than the tensor core's): a step of 64 x 250 is 0.4 M FMAs a CTA.
+constexpr int kSmallRows = 128;
+constexpr int kSmallThreads = 256;
+
+struct SmallParams {
+  const void *g;
+  void *out;
+  int dtype, rows, cols, panel;     // columns of a CTA, a multiple of 4
+  int steps;
+  int x_ld, s_ld;                   // pitches in shared memory: odd multiples of 4 floats
+  int64_t g_sb, g_sr, g_sc, o_sb, o_sr, o_sc;
+  double eps;
+  float abc[3 * 16];
+};
+constexpr int kSmallSteps = 16;
+
+__device__ __forceinline__ float4 peer_load(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ void peer_store(uint32_t addr, float4 v) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z),
+               "f"(v.w)
+               : "memory");
+}
+
+// MT x MT tile of sum over k of a[k][i] b[k][j], k = first, first + step, ..
+template <int MT>
+__device__ __forceinline__ void tile_along(const float *a, int lda, const float *b, int ldb, int first, int step,
+                                           int n, float (&acc)[MT][MT]) {
+  for (int k = first; k < n; k += step) {
+    float x[MT], y[MT];
+#pragma unroll
+    for (int u = 0; u < MT; u += 4) {
+      *reinterpret_cast<float4 *>(x + u) = *reinterpret_cast<const float4 *>(a + k * lda + u);
+      *reinterpret_cast<float4 *>(y + u) = *reinterpret_cast<const float4 *>(b + k * ldb + u);
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < MT; ++j) acc[i][j] = fmaf(x[i], y[j], acc[i][j]);
+  }
+}
+
+// Threads that share the terms of a tile when there are fewer tiles than threads.
+__device__ __forceinline__ int sharing(int tiles) {
+  int n = 1;
+  while (n < 32 && tiles * n * 2 <= kSmallThreads) n *= 2;
+  return n;
+}
+
+template <int MT>
+__device__ __forceinline__ void add_shared(float (&acc)[MT][MT], int share) {
+  for (int o = 1; o < share; o *= 2)
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < MT; ++j) acc[i][j] += __shfl_xor_sync(0xffffffffu, acc[i][j], o);
+}
+
+template <int MT> __global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const SmallParams p) {
+  extern __shared__ __align__(16) float smem_f[];
+  __shared__ double norms[8], part[8];
+  const int ranks = (int)cluster_nctarank(), rank = (int)cluster_ctarank();
+  const int tid = threadIdx.x, lane = tid % 32;
+  const int member = blockIdx.x / ranks;
+  const int rm = (p.rows + MT - 1) / MT * MT;           // rows, padded with zeros
+  float *x = smem_f, *s = x + rm * p.x_ld, *q = s + rm * p.s_ld;   // q: partial S, then P
+  const int c0 = rank * p.panel, width = max(0, min(p.panel, p.cols - c0));
+
+  // X = G's panel, its squares, and zeros around it
+  double sum = 0;
+  const bool across = p.g_sr < p.g_sc;                  // G is stored along X's columns
+  const int inner = across ? p.rows : width, outer = across ? width : p.rows;
+  const int64_t from = member * p.g_sb + c0 * p.g_sc;
+  for (int i = tid; i < rm * p.x_ld; i += kSmallThreads) x[i] = 0.f;
+  __syncthreads();
+  if (inner > 0) {
+    const int per = inner >= 256 ? 256 : inner >= 128 ? 128 : inner >= 64 ? 64 : 32;
+    for (int o = tid / per; o < outer; o += kSmallThreads / per)
+      for (int i = tid % per; i < inner; i += per) {
+        const int r = across ? i : o, c = across ? o : i;
+        const float v = load_value(p.g, p.dtype, from + r * p.g_sr + c * p.g_sc);
+        sum += (double)v * v;
+        x[r * p.x_ld + c] = v;
+      }
+  }
+  sum = block_sum(sum, part);
+  if (tid < ranks) {
+    const uint32_t to = map_to_cta(smem_u32(&norms[rank]), (uint32_t)tid);
+    asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(to), "d"(sum) : "memory");
+  }
+  cluster_sync();
+  sum = 0;
+  for (int r = 0; r < ranks; ++r) sum += norms[r];
+  const double scale = sum == 0 && p.eps == 0 ? 0.0 : 1.0 / (sqrt(sum) + p.eps);
+  for (int i = tid; i < rm * p.x_ld; i += kSmallThreads) x[i] = (float)(x[i] * scale);
+  __syncthreads();
+
+  const int side = rm / MT;
+  const int slice = (side + ranks - 1) / ranks * MT;    // rows of S and P that this CTA makes
+  const int first = min(rank * slice, rm), last = min(first + slice, rm);
+  for (int step = 0; step < p.steps; ++step) {
+    const float a = p.abc[3 * step], b = p.abc[3 * step + 1], c = p.abc[3 * step + 2];
+    {   // this panel's X X^T
+      const int tiles = side * side, share = sharing(tiles), kq = tid % share;
+      for (int t0 = 0; t0 < tiles; t0 += kSmallThreads / share) {
+        const int t = t0 + tid / share, i0 = t / side * MT, j0 = t % side * MT;
+        float acc[MT][MT] = {};
+        if (t < tiles)
+          for (int k = kq * 4; k < p.panel; k += share * 4) {
+            float4 u[MT], w[MT];
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+              u[i] = *reinterpret_cast<const float4 *>(x + (i0 + i) * p.x_ld + k);
+              w[i] = *reinterpret_cast<const float4 *>(x + (j0 + i) * p.x_ld + k);
+            }
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+              for (int j = 0; j < MT; ++j)
+                acc[i][j] = fmaf(u[i].w, w[j].w, fmaf(u[i].z, w[j].z, fmaf(u[i].y, w[j].y, fmaf(u[i].x, w[j].x, acc[i][j]))));
+          }
+        add_shared<MT>(acc, share);
+        if (t < tiles && kq == 0)
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < MT; j += 4)
+              *reinterpret_cast<float4 *>(q + (i0 + i) * p.s_ld + j0 + j) = *reinterpret_cast<float4 *>(&acc[i][j]);
+      }
+    }
+    cluster_sync();
+    // S, rows [first, last) of it here, for everyone
+    for (int v = tid; v < (last - first) * (rm / 4); v += kSmallThreads) {
+      const int at = (first + v / (rm / 4)) * p.s_ld + v % (rm / 4) * 4;
+      const uint32_t from_q = smem_u32(q + at), to_s = smem_u32(s + at);
+      float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int r = 0; r < ranks; ++r) {
+        const float4 o = peer_load(map_to_cta(from_q, (uint32_t)r));
+        f.x += o.x, f.y += o.y, f.z += o.z, f.w += o.w;
+      }
+      for (int r = 0; r < ranks; ++r) peer_store(map_to_cta(to_s, (uint32_t)r), f);
+    }
+    cluster_sync();
+    {   // the same rows of P = b S + c S S
+      const int tiles = (last - first) / MT * side, share = sharing(max(tiles, 1)), kq = tid % share;
+      for (int t0 = 0; t0 < tiles; t0 += kSmallThreads / share) {
+        const int t = t0 + tid / share, i0 = first + t / side * MT, j0 = t % side * MT;
+        float acc[MT][MT] = {};
+        if (t < tiles) tile_along<MT>(s + i0, p.s_ld, s + j0, p.s_ld, kq, share, rm, acc);
+        add_shared<MT>(acc, share);
+        if (t < tiles && kq == 0)
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < MT; j += 4) {
+              const int at = (i0 + i) * p.s_ld + j0 + j;
+              const float4 o = *reinterpret_cast<const float4 *>(s + at);
+              const float4 f = make_float4(b * o.x + c * acc[i][j], b * o.y + c * acc[i][j + 1],
+                                           b * o.z + c * acc[i][j + 2], b * o.w + c * acc[i][j + 3]);
+              const uint32_t to = smem_u32(q + at);
+              for (int r = 0; r < ranks; ++r) peer_store(map_to_cta(to, (uint32_t)r), f);
+            }
+      }
+    }
+    cluster_sync();
+    // X <- a X + P X, the columns of a round from registers once all have read them
+    const int per_round = max(1, kSmallThreads / side) * MT;
+    for (int base = 0; base < p.panel; base += per_round) {
+      const int i0 = tid % side * MT, j0 = base + tid / side * MT;
+      const bool mine = tid / side < per_round / MT && j0 < p.panel;
+      float acc[MT][MT] = {};
+      if (mine) tile_along<MT>(q + i0, p.s_ld, x + j0, p.x_ld, 0, 1, rm, acc);
+      __syncthreads();
+      if (mine)
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int j = 0; j < MT; j += 4) {
+            float4 *at = reinterpret_cast<float4 *>(x + (i0 + i) * p.x_ld + j0 + j);
+            const float4 o = *at;
+            *at = make_float4(fmaf(a, o.x, acc[i][j]), fmaf(a, o.y, acc[i][j + 1]), fmaf(a, o.z, acc[i][j + 2]),
+                              fmaf(a, o.w, acc[i][j + 3]));
+          }
+    }
+    __syncthreads();
+  }
+
+  const int64_t to = member * p.o_sb + c0 * p.o_sc;
+  const bool rows_in = p.o_sr < p.o_sc;                 // the result is stored along X's columns
+  const int o_inner = rows_in ? p.rows : width, all = p.rows * width;
+  for (int i = tid; i < all; i += kSmallThreads) {
+    const int r = rows_in ? i % o_inner : i / o_inner, cc = rows_in ? i / o_inner : i % o_inner;
+    const float v = x[r * p.x_ld + cc];
+    const int64_t at = to + r * p.o_sr + cc * p.o_sc;
+    if (p.dtype == OZ_F32) static_cast<float *>(p.out)[at] = v;
+    else if (p.dtype == OZ_F16) static_cast<__half *>(p.out)[at] = __float2half_rn(v);
+    else static_cast<__nv_bfloat16 *>(p.out)[at] = __float2bfloat16_rn(v);
+  }
+}
+
+// CTAs of a small matrix's cluster, 0 where the tiles of the general path are
+// expected to be faster.  Time in cycles of a step: the FMAs of a CTA at half of
+// the 128 a cycle, and about 4000 for its three cluster barriers and
+// exchanges; the general path takes about 15 us a step whatever its size here.
+struct SmallShape { int ranks, panel, x_ld, s_ld, mt, bytes; };
+SmallShape small_shape(int64_t batch, int64_t rows, int64_t cols, int steps) {
+  SmallShape best{};
+  if (rows > kSmallRows || steps > kSmallSteps || batch > 4096) return best;
+  double least = 15.0 * 1900;
+  for (int ranks = 1; ranks <= 8; ranks *= 2) {
+    const int mt = rows > 64 ? 8 : 4;
+    const int64_t rm = (rows + mt - 1) / mt * mt, panel = ((cols + ranks - 1) / ranks + mt - 1) / mt * mt;
+    auto odd = [](int64_t n) { return n / 4 % 2 ? n : n + 4; };
+    const int64_t x_ld = odd(panel), s_ld = odd(rm), bytes = 4 * rm * (x_ld + 2 * s_ld);
+    if (bytes > 220 * 1024) continue;
+    const double fmas = (double)rm * rm * (2 * panel) + (double)rm * rm * rm / ranks;
+    const int64_t waves = (batch * ranks + sm_count() - 1) / sm_count();
+    const double t = (double)waves * (fmas / 64 + 4000);
+    if (t < least) {
+      least = t;
+      best = SmallShape{ranks, (int)panel, (int)x_ld, (int)s_ld, mt, (int)bytes};
+    }
+  }
+  return best;
+}
+
+int run_small(const SmallShape &shape, SmallParams p, int64_t batch, cudaStream_t st) {
+  p.panel = shape.panel;
+  p.x_ld = shape.x_ld;
+  p.s_ld = shape.s_ld;
+  auto kernel = shape.mt == 8 ? small_kernel<8> : small_kernel<4>;
+  if (int rc = set_smem_once((const void *)kernel, shape.bytes, "small_kernel shared memory")) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(batch * shape.ranks));
+  cfg.blockDim = dim3(kSmallThreads);
+  cfg.dynamicSmemBytes = shape.bytes;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = shape.ranks;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  count_launch();
+  return check_cuda(cudaLaunchKernelEx(&cfg, kernel, p), "small_kernel launch");
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
 int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
 int64_t pitch(int64_t n) { return (n + 7) / 8 * 8; }
 
@@ -644,9 +910,11 @@ bool valid(int dtype, int64_t batch, int64_t m, int64_t n, int splits) {
 }  // namespace oz
 
 extern "C" int64_t oz_orthogonalize_workspace_bytes(int dtype, int64_t batch, int64_t m, int64_t n,
-                                                    int32_t num_splits) {
-  if (!oz::valid(dtype, batch, m, n, num_splits)) return OZ_ERR_INVALID;
-  return oz::layout(batch, m, n, num_splits).total;
+                                                    int32_t steps, int32_t num_splits) {
+  using namespace oz;
+  if (!valid(dtype, batch, m, n, num_splits) || steps < 1) return OZ_ERR_INVALID;
+  if (batch == 0 || m == 0 || n == 0 || small_shape(batch, std::min(m, n), std::max(m, n), steps).ranks) return 0;
+  return layout(batch, m, n, num_splits).total;
 }
 
 extern "C" int oz_orthogonalize(const void *g, int dtype, int64_t batch, int64_t m, int64_t n,
@@ -668,13 +936,32 @@ extern "C" int oz_orthogonalize(const void *g, int dtype, int64_t batch, int64_t
     if (!std::isfinite(coefficients[i])) return set_error(OZ_ERR_INVALID, "coefficients must be finite");
   if (batch == 0 || m == 0 || n == 0) return OZ_OK;
   if (!g || !out) return set_error(OZ_ERR_INVALID, "null pointer");
+  const bool tall = m > n;
+  const SmallShape small = small_shape(batch, m < n ? m : n, m < n ? n : m, steps);
+  if (small.ranks) {
+    SmallParams p{};
+    p.g = g;
+    p.out = out;
+    p.dtype = dtype;
+    p.rows = (int)(tall ? n : m);
+    p.cols = (int)(tall ? m : n);
+    p.steps = steps;
+    p.g_sb = g_sb;
+    p.g_sr = tall ? g_sc : g_sr;
+    p.g_sc = tall ? g_sr : g_sc;
+    p.o_sb = m * n;
+    p.o_sr = tall ? 1 : n;
+    p.o_sc = tall ? n : 1;
+    p.eps = eps;
+    for (int i = 0; i < 3 * steps; ++i) p.abc[i] = (float)coefficients[i];
+    return run_small(small, p, batch, reinterpret_cast<cudaStream_t>(stream));
+  }
   const Layout l = layout(batch, m, n, num_splits);
   if (!workspace || workspace_bytes < l.total || (uintptr_t)workspace % 256 != 0)
     return set_error(OZ_ERR_INVALID,
                      "workspace of %lld bytes (256-byte aligned) needed, got %lld at %p",
                      (long long)l.total, (long long)workspace_bytes, workspace);
   unsigned char *ws = static_cast<unsigned char *>(workspace);
-  const bool tall = m > n;
   const int64_t blocks = (l.rows * l.cols + 4095) / 4096;
   const int64_t line = std::max(g_sr, g_sc), step = std::min(g_sr, g_sc);
   const int64_t in_line = g_sr < g_sc ? m : n, per16 = 16 / dtype_size(dtype);

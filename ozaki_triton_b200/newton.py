@@ -3,23 +3,53 @@
 from __future__ import annotations
 
 import ctypes
+import math
 from typing import Optional, Sequence, Union
 
 import torch
 
 from . import _lib
 from .api import _OZ_DTYPE, _check_cuda
-from .experts import _OnDevice, _stream_of
+from .experts import _CURRENT_DEVICE, _OnDevice, _Plans, _stream_of
 
 ORTHOGONALIZE_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
-def _coefficients(coefficients, steps: int):
-    rows = [tuple(c) for c in coefficients] if hasattr(coefficients[0], "__len__") else \
-        [tuple(coefficients)] * steps
+class _Plan:
+    """What a call derives from its matrices' type, shape and strides and from
+    its other arguments: the checks passed and the library's arguments."""
+
+    __slots__ = ("matrices", "rest", "workspace", "empty", "device")
+
+
+_PLANS = _Plans()
+
+
+def _plan(key, g, steps, coefficients, eps, num_splits) -> _Plan:
+    assert g.dim() >= 2, f"g must be a matrix or a stack of them, got shape {tuple(g.shape)}"
+    assert g.dtype in ORTHOGONALIZE_DTYPES, f"unsupported dtype: {g.dtype}"
+    assert steps >= 1, f"at least one step is needed, got {steps}"
+    assert eps >= 0, f"eps must not be negative, got {eps}"
+    if num_splits is None:
+        num_splits = 1 if g.dtype == torch.bfloat16 else 2
+    assert num_splits in (1, 2), f"num_splits must be 1 or 2, got {num_splits}"
+    rows = list(coefficients) if hasattr(coefficients[0], "__len__") else [coefficients] * steps
     assert len(rows) == steps and all(len(r) == 3 for r in rows), \
         f"coefficients must be one (a, b, c) or one for each of the {steps} steps"
-    return (ctypes.c_double * (3 * steps))(*[float(v) for r in rows for v in r])
+    values = [float(v) for r in rows for v in r]
+    assert all(math.isfinite(v) for v in values), "coefficients must be finite"
+    _check_cuda(g)
+    plan = _Plan()
+    plan.device, plan.empty, plan.workspace = g.get_device(), g.numel() == 0, 0
+    plan.matrices = plan.rest = None
+    if not plan.empty:
+        m, n = g.shape[-2:]
+        code, batch = _OZ_DTYPE[g.dtype], g.numel() // (m * n)
+        strides = g.stride() if g.dim() == 3 else (0, *g.stride()) if g.dim() == 2 else (m * n, n, 1)
+        plan.matrices = (code, batch, m, n, *strides, steps, (ctypes.c_double * len(values))(*values), float(eps),
+                         num_splits)
+        plan.workspace = _lib.load().oz_orthogonalize_workspace_bytes(code, batch, m, n, steps, num_splits)
+    return _PLANS.keep(key, plan)
 
 
 def orthogonalize(g: torch.Tensor, steps: int = 5,
@@ -36,29 +66,28 @@ def orthogonalize(g: torch.Tensor, steps: int = 5,
 
     ``num_splits`` is how many fp16 slices of each matrix the products use: 1
     (11 bits, the default for bf16 whose result has 8) or 2 (22 bits, the
-    default for fp32 and fp16).  Sums are held in fp32.
+    default for fp32 and fp16).  Sums are held in fp32.  Small matrices (up to
+    128 rows or columns) are worked on in fp32 whatever it is.
     """
-    assert g.dim() >= 2, f"g must be a matrix or a stack of them, got shape {tuple(g.shape)}"
-    assert g.dtype in ORTHOGONALIZE_DTYPES, f"unsupported dtype: {g.dtype}"
-    assert steps >= 1, f"at least one step is needed, got {steps}"
-    assert eps >= 0, f"eps must not be negative, got {eps}"
-    if num_splits is None:
-        num_splits = 1 if g.dtype == torch.bfloat16 else 2
-    assert num_splits in (1, 2), f"num_splits must be 1 or 2, got {num_splits}"
-    coeffs = _coefficients(coefficients, steps)
-    _check_cuda(g)
-    out = torch.empty(g.shape, dtype=g.dtype, device=g.device)
-    if g.numel() == 0:
+    if not isinstance(coefficients, tuple) or hasattr(coefficients[0], "__len__"):
+        coefficients = tuple(tuple(c) if hasattr(c, "__len__") else c for c in coefficients)
+    if g.dim() > 3:
+        g3 = g.reshape(-1, *g.shape[-2:]) if g.numel() else g
+        return orthogonalize(g3, steps, coefficients, eps, num_splits=num_splits).view(g.shape) if g.numel() \
+            else g.new_empty(g.shape)
+    key = (g.shape, g.stride(), g.dtype, g.get_device(), steps, coefficients, eps, num_splits)
+    plan = _PLANS.kept.get(key) or _plan(key, g, steps, coefficients, eps, num_splits)
+    out = g.new_empty(g.shape)
+    if plan.empty:
         return out
-    m, n = g.shape[-2:]
-    g3 = g.reshape(-1, m, n)
-    lib = _lib.load()
-    code = _OZ_DTYPE[g.dtype]
-    ws_bytes = lib.oz_orthogonalize_workspace_bytes(code, g3.shape[0], m, n, num_splits)
-    ws = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=g.device)
-    device = g.get_device()
-    with _OnDevice(device):
-        _lib.check(lib.oz_orthogonalize(
-            g3.data_ptr(), code, g3.shape[0], m, n, *g3.stride(), steps, coeffs, float(eps),
-            num_splits, out.data_ptr(), ws.data_ptr(), ws_bytes, _stream_of(device)))
+    ws = g.new_empty((plan.workspace,), dtype=torch.uint8) if plan.workspace else None
+    args = (g.data_ptr(), *plan.matrices, out.data_ptr(), ws.data_ptr() if ws is not None else None, plan.workspace)
+    call, device = _lib.load().oz_orthogonalize, plan.device
+    if _CURRENT_DEVICE() == device:
+        status = call(*args, _stream_of(device))
+    else:
+        with _OnDevice(device):
+            status = call(*args, _stream_of(device))
+    if status:
+        _lib.check(status)
     return out

@@ -139,12 +139,13 @@ def test_library_entries_validate_without_a_launch():
 
     abc = (ctypes.c_double * 3)(1.5, -0.5, 0.0)
 
-    def ortho(dtype=_lib.OZ_F32, batch=1, m=4, n=4, steps=1, c=abc, eps=0.0, splits=2, ws=p, ws_bytes=1 << 30):
+    def ortho(dtype=_lib.OZ_F32, batch=1, m=512, n=512, steps=1, c=abc, eps=0.0, splits=2, ws=p, ws_bytes=1 << 30):
         return lib.oz_orthogonalize(p, dtype, batch, m, n, 16, 4, 1, steps, c, eps, splits, p, ws, ws_bytes, None)
     assert ortho(dtype=_lib.OZ_F64) == _lib.OZ_ERR_UNSUPPORTED
     assert ortho(m=-1) == _lib.OZ_ERR_INVALID
     assert ortho(steps=0) == _lib.OZ_ERR_INVALID
     assert ortho(c=None) == _lib.OZ_ERR_INVALID
+    assert ortho(c=(ctypes.c_double * 3)(1.5, float("inf"), 0.0)) == _lib.OZ_ERR_INVALID
     assert ortho(eps=-1.0) == _lib.OZ_ERR_INVALID
     assert ortho(eps=float("nan")) == _lib.OZ_ERR_INVALID
     assert ortho(splits=3) == _lib.OZ_ERR_INVALID
@@ -152,8 +153,11 @@ def test_library_entries_validate_without_a_launch():
     assert ortho(ws=ctypes.c_void_p(128)) == _lib.OZ_ERR_INVALID
     assert ortho(ws_bytes=10) == _lib.OZ_ERR_INVALID
     assert ortho(n=0) == _lib.OZ_OK
-    assert lib.oz_orthogonalize_workspace_bytes(_lib.OZ_F32, 1, 4, 4, 0) == _lib.OZ_ERR_INVALID
-    assert lib.oz_orthogonalize_workspace_bytes(_lib.OZ_F32, 2, 64, 32, 2) > 0
+    need = lib.oz_orthogonalize_workspace_bytes
+    assert need(_lib.OZ_F32, 1, 4, 4, 1, 0) == _lib.OZ_ERR_INVALID
+    assert need(_lib.OZ_F32, 1, 512, 512, 0, 1) == _lib.OZ_ERR_INVALID
+    assert need(_lib.OZ_F32, 2, 640, 320, 5, 2) > need(_lib.OZ_F32, 2, 640, 320, 5, 1) > 0
+    assert need(_lib.OZ_F32, 2, 64, 32, 5, 2) == 0       # small: kept on chip
     assert lib.oz_launch_count() == n0
 
 
