@@ -486,6 +486,7 @@ template <int PAIR_, int NT_, int PLANES_> struct UpdateJob {
 // exact than the tensor core's): a step of 64 x 250 is 0.4 M FMAs a CTA.
 constexpr int kSmallRows = 128;
 constexpr int kSmallThreads = 256;
+constexpr int kMicro = 4;                // rows and columns of a thread's tile
 
 struct SmallParams {
   const void *g;
@@ -503,8 +504,7 @@ __device__ __forceinline__ float4 peer_load(uint32_t addr) {
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
                : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(addr)
-               : "memory");
+               : "r"(addr));
   return v;
 }
 __device__ __forceinline__ void peer_store(uint32_t addr, float4 v) {
@@ -513,21 +513,17 @@ __device__ __forceinline__ void peer_store(uint32_t addr, float4 v) {
                : "memory");
 }
 
-// MT x MT tile of sum over k of a[k][i] b[k][j], k = first, first + step, ..
-template <int MT>
+// 4 x 4 tile of sum over k of a[k][i] b[k][j], k = first, first + step, ..
 __device__ __forceinline__ void tile_along(const float *a, int lda, const float *b, int ldb, int first, int step,
-                                           int n, float (&acc)[MT][MT]) {
+                                           int n, float (&acc)[kMicro][kMicro]) {
+#pragma unroll 4
   for (int k = first; k < n; k += step) {
-    float x[MT], y[MT];
+    const float4 u = *reinterpret_cast<const float4 *>(a + k * lda), w = *reinterpret_cast<const float4 *>(b + k * ldb);
+    const float x[4] = {u.x, u.y, u.z, u.w}, y[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int u = 0; u < MT; u += 4) {
-      *reinterpret_cast<float4 *>(x + u) = *reinterpret_cast<const float4 *>(a + k * lda + u);
-      *reinterpret_cast<float4 *>(y + u) = *reinterpret_cast<const float4 *>(b + k * ldb + u);
-    }
+    for (int i = 0; i < kMicro; ++i)
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int j = 0; j < MT; ++j) acc[i][j] = fmaf(x[i], y[j], acc[i][j]);
+      for (int j = 0; j < kMicro; ++j) acc[i][j] = fmaf(x[i], y[j], acc[i][j]);
   }
 }
 
@@ -538,22 +534,21 @@ __device__ __forceinline__ int sharing(int tiles) {
   return n;
 }
 
-template <int MT>
-__device__ __forceinline__ void add_shared(float (&acc)[MT][MT], int share) {
+__device__ __forceinline__ void add_shared(float (&acc)[kMicro][kMicro], int share) {
   for (int o = 1; o < share; o *= 2)
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int i = 0; i < kMicro; ++i)
 #pragma unroll
-      for (int j = 0; j < MT; ++j) acc[i][j] += __shfl_xor_sync(0xffffffffu, acc[i][j], o);
+      for (int j = 0; j < kMicro; ++j) acc[i][j] += __shfl_xor_sync(0xffffffffu, acc[i][j], o);
 }
 
-template <int MT> __global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const SmallParams p) {
+__global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const SmallParams p) {
   extern __shared__ __align__(16) float smem_f[];
   __shared__ double norms[8], part[8];
   const int ranks = (int)cluster_nctarank(), rank = (int)cluster_ctarank();
   const int tid = threadIdx.x, lane = tid % 32;
   const int member = blockIdx.x / ranks;
-  const int rm = (p.rows + MT - 1) / MT * MT;           // rows, padded with zeros
+  const int rm = (p.rows + kMicro - 1) / kMicro * kMicro;           // rows, padded with zeros
   float *x = smem_f, *s = x + rm * p.x_ld, *q = s + rm * p.s_ld;   // q: partial S, then P
   const int c0 = rank * p.panel, width = max(0, min(p.panel, p.cols - c0));
 
@@ -586,37 +581,39 @@ template <int MT> __global__ void __launch_bounds__(kSmallThreads, 1) small_kern
   for (int i = tid; i < rm * p.x_ld; i += kSmallThreads) x[i] = (float)(x[i] * scale);
   __syncthreads();
 
-  const int side = rm / MT;
-  const int slice = (side + ranks - 1) / ranks * MT;    // rows of S and P that this CTA makes
+  const int side = rm / kMicro;
+  const int slice = (side + ranks - 1) / ranks * kMicro;    // rows of S and P that this CTA makes
   const int first = min(rank * slice, rm), last = min(first + slice, rm);
   for (int step = 0; step < p.steps; ++step) {
     const float a = p.abc[3 * step], b = p.abc[3 * step + 1], c = p.abc[3 * step + 2];
-    {   // this panel's X X^T
+    {   // this panel's X X^T; a tile takes every side-th row, so that the threads of
+        // a warp read neighbouring rows (whose pitch is odd: no bank conflicts)
       const int tiles = side * side, share = sharing(tiles), kq = tid % share;
       for (int t0 = 0; t0 < tiles; t0 += kSmallThreads / share) {
-        const int t = t0 + tid / share, i0 = t / side * MT, j0 = t % side * MT;
-        float acc[MT][MT] = {};
-        if (t < tiles)
+        const int t = t0 + tid / share, ti = t / side, tj = t - ti * side;
+        float acc[kMicro][kMicro] = {};
+        if (t < tiles) {
+          const float *xi = x + ti * p.x_ld, *xj = x + tj * p.x_ld;
           for (int k = kq * 4; k < p.panel; k += share * 4) {
-            float4 u[MT], w[MT];
+            float4 u[kMicro], w[kMicro];
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-              u[i] = *reinterpret_cast<const float4 *>(x + (i0 + i) * p.x_ld + k);
-              w[i] = *reinterpret_cast<const float4 *>(x + (j0 + i) * p.x_ld + k);
+            for (int i = 0; i < kMicro; ++i) {
+              u[i] = *reinterpret_cast<const float4 *>(xi + i * side * p.x_ld + k);
+              w[i] = *reinterpret_cast<const float4 *>(xj + i * side * p.x_ld + k);
             }
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
+            for (int i = 0; i < kMicro; ++i)
 #pragma unroll
-              for (int j = 0; j < MT; ++j)
+              for (int j = 0; j < kMicro; ++j)
                 acc[i][j] = fmaf(u[i].w, w[j].w, fmaf(u[i].z, w[j].z, fmaf(u[i].y, w[j].y, fmaf(u[i].x, w[j].x, acc[i][j]))));
           }
-        add_shared<MT>(acc, share);
+        }
+        add_shared(acc, share);
         if (t < tiles && kq == 0)
 #pragma unroll
-          for (int i = 0; i < MT; ++i)
+          for (int i = 0; i < kMicro; ++i)
 #pragma unroll
-            for (int j = 0; j < MT; j += 4)
-              *reinterpret_cast<float4 *>(q + (i0 + i) * p.s_ld + j0 + j) = *reinterpret_cast<float4 *>(&acc[i][j]);
+            for (int j = 0; j < kMicro; ++j) q[(ti + i * side) * p.s_ld + tj + j * side] = acc[i][j];
       }
     }
     cluster_sync();
@@ -624,26 +621,28 @@ template <int MT> __global__ void __launch_bounds__(kSmallThreads, 1) small_kern
     for (int v = tid; v < (last - first) * (rm / 4); v += kSmallThreads) {
       const int at = (first + v / (rm / 4)) * p.s_ld + v % (rm / 4) * 4;
       const uint32_t from_q = smem_u32(q + at), to_s = smem_u32(s + at);
-      float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int r = 0; r < ranks; ++r) {
-        const float4 o = peer_load(map_to_cta(from_q, (uint32_t)r));
-        f.x += o.x, f.y += o.y, f.z += o.z, f.w += o.w;
-      }
+      float4 o[8], f = make_float4(0.f, 0.f, 0.f, 0.f);   // all on their way before the first is used
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        if (r < ranks) o[r] = peer_load(map_to_cta(from_q, (uint32_t)r));
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        if (r < ranks) f.x += o[r].x, f.y += o[r].y, f.z += o[r].z, f.w += o[r].w;
       for (int r = 0; r < ranks; ++r) peer_store(map_to_cta(to_s, (uint32_t)r), f);
     }
     cluster_sync();
     {   // the same rows of P = b S + c S S
-      const int tiles = (last - first) / MT * side, share = sharing(max(tiles, 1)), kq = tid % share;
+      const int tiles = (last - first) / kMicro * side, share = sharing(max(tiles, 1)), kq = tid % share;
       for (int t0 = 0; t0 < tiles; t0 += kSmallThreads / share) {
-        const int t = t0 + tid / share, i0 = first + t / side * MT, j0 = t % side * MT;
-        float acc[MT][MT] = {};
-        if (t < tiles) tile_along<MT>(s + i0, p.s_ld, s + j0, p.s_ld, kq, share, rm, acc);
-        add_shared<MT>(acc, share);
+        const int t = t0 + tid / share, i0 = first + t / side * kMicro, j0 = t % side * kMicro;
+        float acc[kMicro][kMicro] = {};
+        if (t < tiles) tile_along(s + i0, p.s_ld, s + j0, p.s_ld, kq, share, rm, acc);
+        add_shared(acc, share);
         if (t < tiles && kq == 0)
 #pragma unroll
-          for (int i = 0; i < MT; ++i)
+          for (int i = 0; i < kMicro; ++i)
 #pragma unroll
-            for (int j = 0; j < MT; j += 4) {
+            for (int j = 0; j < kMicro; j += 4) {
               const int at = (i0 + i) * p.s_ld + j0 + j;
               const float4 o = *reinterpret_cast<const float4 *>(s + at);
               const float4 f = make_float4(b * o.x + c * acc[i][j], b * o.y + c * acc[i][j + 1],
@@ -655,18 +654,20 @@ template <int MT> __global__ void __launch_bounds__(kSmallThreads, 1) small_kern
     }
     cluster_sync();
     // X <- a X + P X, the columns of a round from registers once all have read them
-    const int per_round = max(1, kSmallThreads / side) * MT;
-    for (int base = 0; base < p.panel; base += per_round) {
-      const int i0 = tid % side * MT, j0 = base + tid / side * MT;
-      const bool mine = tid / side < per_round / MT && j0 < p.panel;
-      float acc[MT][MT] = {};
-      if (mine) tile_along<MT>(q + i0, p.s_ld, x + j0, p.x_ld, 0, 1, rm, acc);
+    const int share = sharing(side * (p.panel / kMicro)), kq = tid % share, t = tid / share;
+    const int abreast = kSmallThreads / share / side;      // column tiles of a round
+    for (int base = 0; base < p.panel; base += abreast * kMicro) {
+      const int i0 = t % side * kMicro, j0 = base + t / side * kMicro;
+      const bool mine = t / side < abreast && j0 < p.panel;
+      float acc[kMicro][kMicro] = {};
+      if (mine) tile_along(q + i0, p.s_ld, x + j0, p.x_ld, kq, share, rm, acc);
+      add_shared(acc, share);
       __syncthreads();
-      if (mine)
+      if (mine && kq == 0)
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
+        for (int i = 0; i < kMicro; ++i)
 #pragma unroll
-          for (int j = 0; j < MT; j += 4) {
+          for (int j = 0; j < kMicro; j += 4) {
             float4 *at = reinterpret_cast<float4 *>(x + (i0 + i) * p.x_ld + j0 + j);
             const float4 o = *at;
             *at = make_float4(fmaf(a, o.x, acc[i][j]), fmaf(a, o.y, acc[i][j + 1]), fmaf(a, o.z, acc[i][j + 2]),
@@ -693,14 +694,13 @@ template <int MT> __global__ void __launch_bounds__(kSmallThreads, 1) small_kern
 // expected to be faster.  Time in cycles of a step: the FMAs of a CTA at half of
 // the 128 a cycle, and about 4000 for its three cluster barriers and
 // exchanges; the general path takes about 15 us a step whatever its size here.
-struct SmallShape { int ranks, panel, x_ld, s_ld, mt, bytes; };
+struct SmallShape { int ranks, panel, x_ld, s_ld, bytes; };
 SmallShape small_shape(int64_t batch, int64_t rows, int64_t cols, int steps) {
   SmallShape best{};
   if (rows > kSmallRows || steps > kSmallSteps || batch > 4096) return best;
   double least = 15.0 * 1900;
   for (int ranks = 1; ranks <= 8; ranks *= 2) {
-    const int mt = rows > 64 ? 8 : 4;
-    const int64_t rm = (rows + mt - 1) / mt * mt, panel = ((cols + ranks - 1) / ranks + mt - 1) / mt * mt;
+    const int64_t rm = (rows + 3) / 4 * 4, panel = ((cols + ranks - 1) / ranks + 3) / 4 * 4;
     auto odd = [](int64_t n) { return n / 4 % 2 ? n : n + 4; };
     const int64_t x_ld = odd(panel), s_ld = odd(rm), bytes = 4 * rm * (x_ld + 2 * s_ld);
     if (bytes > 220 * 1024) continue;
@@ -709,7 +709,7 @@ SmallShape small_shape(int64_t batch, int64_t rows, int64_t cols, int steps) {
     const double t = (double)waves * (fmas / 64 + 4000);
     if (t < least) {
       least = t;
-      best = SmallShape{ranks, (int)panel, (int)x_ld, (int)s_ld, mt, (int)bytes};
+      best = SmallShape{ranks, (int)panel, (int)x_ld, (int)s_ld, (int)bytes};
     }
   }
   return best;
@@ -719,7 +719,7 @@ int run_small(const SmallShape &shape, SmallParams p, int64_t batch, cudaStream_
   p.panel = shape.panel;
   p.x_ld = shape.x_ld;
   p.s_ld = shape.s_ld;
-  auto kernel = shape.mt == 8 ? small_kernel<8> : small_kernel<4>;
+  auto kernel = small_kernel;
   if (int rc = set_smem_once((const void *)kernel, shape.bytes, "small_kernel shared memory")) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(batch * shape.ranks));
