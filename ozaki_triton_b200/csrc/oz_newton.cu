@@ -82,7 +82,7 @@ __device__ double block_sum(double sum, double *part) {
   if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = sum;
   __syncthreads();
   sum = 0;
-  for (int w = 0; w < 8; ++w) sum += part[w];
+  for (int w = 0; w < (int)blockDim.x / 32; ++w) sum += part[w];
   return sum;
 }
 
@@ -530,7 +530,7 @@ __device__ __forceinline__ void tile_along(const float *a, int lda, const float 
 // Threads that share the terms of a tile when there are fewer tiles than threads.
 __device__ __forceinline__ int sharing(int tiles) {
   int n = 1;
-  while (n < 32 && tiles * n * 2 <= kSmallThreads) n *= 2;
+  while (n < 8 && tiles * n * 2 <= kSmallThreads) n *= 2;
   return n;
 }
 
@@ -544,10 +544,14 @@ __device__ __forceinline__ void add_shared(float (&acc)[kMicro][kMicro], int sha
 
 __global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const SmallParams p) {
   extern __shared__ __align__(16) float smem_f[];
-  __shared__ double norms[8], part[8];
+  __shared__ double norms[8], part[kSmallThreads / 32];
   const int ranks = (int)cluster_nctarank(), rank = (int)cluster_ctarank();
-  const int tid = threadIdx.x, lane = tid % 32;
+  const int tid = threadIdx.x;
   const int member = blockIdx.x / ranks;
+  auto together = [&]() {
+    if (ranks > 1) cluster_sync();
+    else __syncthreads();
+  };
   const int rm = (p.rows + kMicro - 1) / kMicro * kMicro;           // rows, padded with zeros
   float *x = smem_f, *s = x + rm * p.x_ld, *q = s + rm * p.s_ld;   // q: partial S, then P
   const int c0 = rank * p.panel, width = max(0, min(p.panel, p.cols - c0));
@@ -560,7 +564,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const SmallPara
   for (int i = tid; i < rm * p.x_ld; i += kSmallThreads) x[i] = 0.f;
   __syncthreads();
   if (inner > 0) {
-    const int per = inner >= 256 ? 256 : inner >= 128 ? 128 : inner >= 64 ? 64 : 32;
+    const int per = inner >= 256 ? 256 : inner >= 128 ? 128 : inner >= 64 ? 64 : inner >= 32 ? 32 : 16;
     for (int o = tid / per; o < outer; o += kSmallThreads / per)
       for (int i = tid % per; i < inner; i += per) {
         const int r = across ? i : o, c = across ? o : i;
@@ -574,7 +578,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const SmallPara
     const uint32_t to = map_to_cta(smem_u32(&norms[rank]), (uint32_t)tid);
     asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(to), "d"(sum) : "memory");
   }
-  cluster_sync();
+  together();
   sum = 0;
   for (int r = 0; r < ranks; ++r) sum += norms[r];
   const double scale = sum == 0 && p.eps == 0 ? 0.0 : 1.0 / (sqrt(sum) + p.eps);
@@ -616,7 +620,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const SmallPara
             for (int j = 0; j < kMicro; ++j) q[(ti + i * side) * p.s_ld + tj + j * side] = acc[i][j];
       }
     }
-    cluster_sync();
+    together();
     // S, rows [first, last) of it here, for everyone
     for (int v = tid; v < (last - first) * (rm / 4); v += kSmallThreads) {
       const int at = (first + v / (rm / 4)) * p.s_ld + v % (rm / 4) * 4;
@@ -630,7 +634,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const SmallPara
         if (r < ranks) f.x += o[r].x, f.y += o[r].y, f.z += o[r].z, f.w += o[r].w;
       for (int r = 0; r < ranks; ++r) peer_store(map_to_cta(to_s, (uint32_t)r), f);
     }
-    cluster_sync();
+    together();
     {   // the same rows of P = b S + c S S
       const int tiles = (last - first) / kMicro * side, share = sharing(max(tiles, 1)), kq = tid % share;
       for (int t0 = 0; t0 < tiles; t0 += kSmallThreads / share) {
@@ -652,7 +656,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const SmallPara
             }
       }
     }
-    cluster_sync();
+    together();
     // X <- a X + P X, the columns of a round from registers once all have read them
     const int share = sharing(side * (p.panel / kMicro)), kq = tid % share, t = tid / share;
     const int abreast = kSmallThreads / share / side;      // column tiles of a round
@@ -691,14 +695,17 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const SmallPara
 }
 
 // CTAs of a small matrix's cluster, 0 where the tiles of the general path are
-// expected to be faster.  Time in cycles of a step: the FMAs of a CTA at half of
-// the 128 a cycle, and about 4000 for its three cluster barriers and
-// exchanges; the general path takes about 15 us a step whatever its size here.
+// expected to be faster.  Cycles of a step: the FMAs of a CTA at 46 a cycle
+// (shared memory feeds no more of these 4 x 4 tiles), 4000 for barriers and
+// sums, and the exchange of S and P, which slows down once many clusters do
+// it; the general path takes about 40,000 whatever its size here.  Measured, us a
+// call of 5 steps: 64 x 512 with 1, 2, 4, 8 CTAs 254, 144, 86, 60; 16 matrices
+// of 128 x 128 332, 183, 115, 179; the general path 105.
 struct SmallShape { int ranks, panel, x_ld, s_ld, bytes; };
 SmallShape small_shape(int64_t batch, int64_t rows, int64_t cols, int steps) {
   SmallShape best{};
   if (rows > kSmallRows || steps > kSmallSteps || batch > 4096) return best;
-  double least = 15.0 * 1900;
+  double least = 40000;
   for (int ranks = 1; ranks <= 8; ranks *= 2) {
     const int64_t rm = (rows + 3) / 4 * 4, panel = ((cols + ranks - 1) / ranks + 3) / 4 * 4;
     auto odd = [](int64_t n) { return n / 4 % 2 ? n : n + 4; };
@@ -706,7 +713,9 @@ SmallShape small_shape(int64_t batch, int64_t rows, int64_t cols, int steps) {
     if (bytes > 220 * 1024) continue;
     const double fmas = (double)rm * rm * (2 * panel) + (double)rm * rm * rm / ranks;
     const int64_t waves = (batch * ranks + sm_count() - 1) / sm_count();
-    const double t = (double)waves * (fmas / 64 + 4000);
+    const double crowd = std::max(1.0, (double)(batch * ranks) * (batch * ranks) / (80.0 * 80.0));
+    const double exchange = ranks > 1 ? 0.7 * rm * rm * std::min(crowd, 3.0) : 0;
+    const double t = (double)waves * (fmas / 46 + 4000 + exchange);
     if (t < least) {
       least = t;
       best = SmallShape{ranks, (int)panel, (int)x_ld, (int)s_ld, (int)bytes};
