@@ -11,6 +11,8 @@
 // [0, rows] before they are used as row numbers.  Products of fp16 / bf16
 // values are exact in fp32; sums are held in fp32 and rounded once.
 
+#include <cmath>
+
 #include "oz_tile.cuh"
 
 namespace oz {
@@ -326,11 +328,23 @@ int run(const CUtensorMap &a, const CUtensorMap &b, GroupedParams p, int64_t row
 template <typename O>
 int grouped(const void *x, const void *w, int64_t x_sr, int64_t w_se, bool across, int64_t w_row,
             const GroupedParams &p, cudaStream_t st) {
-  // Columns as A (at most 32 rows of a group a tile) while the mean group has no
-  // more than 32 rows; pairs of CTAs (256-row tiles) from 192 rows on.
-  const int64_t mean = p.rows / p.groups;
-  const int pair = mean >= 192 ? 2 : 1;
-  const bool few = mean <= 32;
+  // The least estimated time of three tile shapes: waves of tiles over the GPU,
+  // from the mean group (half a tile of each group is empty on average), times a
+  // tile's blocks and four more for its start and end, times the bytes a CTA loads a
+  // block: 128 columns by at most 32 rows (20 KB), 128 rows by 128 columns (32),
+  // pairs of CTAs 256 by 256 (32 each).  Measured, us: 1003 rows / 12 experts,
+  // 1000 x 1407 (GROUPED_A); 16 rows / 8 experts, 1024 x 2048 (GROUPED_B).
+  const int64_t groups = min(p.groups, p.rows);
+  const double mean = (double)p.rows / groups;
+  const double blocks64 = (p.k + kBlock - 1) / kBlock + 4;
+  auto time = [&](int high, int wide, int bytes, int ctas) {
+    const double tiles = groups * max(1.0, mean / high + 0.5) * ((p.n + wide - 1) / wide);
+    return ceil(tiles * ctas / sm_count()) * blocks64 * bytes;
+  };
+  const double few_time = time(32, kRows, 20, 1), one_time = time(kRows, 128, 32, 1);
+  const double two_time = time(2 * kRows, 256, 32, 2);
+  const bool few = few_time <= one_time && few_time <= two_time;
+  const int pair = two_time <= one_time ? 2 : 1;
   CUtensorMap tx, tw;
   const int64_t wr = across ? p.k : p.n, wi = across ? p.n : p.k;
   const int nt = pair == 2 ? 256 : 128;

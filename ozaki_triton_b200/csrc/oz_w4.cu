@@ -112,10 +112,8 @@ __device__ __forceinline__ uint32_t field(uint32_t w, uint32_t m, uint32_t c) {
 template <typename T> struct Unpack;
 template <> struct Unpack<__half> {
   uint32_t m0 = kept(0x000f000fu), c0 = kept(0x64006400u), m1 = kept(0x00f000f0u), c1 = kept(0x54005400u);
-  static __device__ __forceinline__ uint2 zero(uint32_t z) {
-    z *= 0x10001u;
-    return make_uint2(0x64006400u | z, 0x54005400u | z << 4);
-  }
+  static __device__ __forceinline__ uint32_t zero(uint32_t z) { return 0x64006400u | z * 0x10001u; }
+  __device__ __forceinline__ uint2 both(uint32_t z) const { return make_uint2(z, field(z << 4, m1, c1)); }
   static __device__ __forceinline__ uint32_t less(uint32_t v, uint32_t z) {
     const __half2 d = __hsub2(*reinterpret_cast<const __half2 *>(&v), *reinterpret_cast<const __half2 *>(&z));
     return *reinterpret_cast<const uint32_t *>(&d);
@@ -130,9 +128,8 @@ template <> struct Unpack<__half> {
 };
 template <> struct Unpack<__nv_bfloat16> {
   uint32_t m0 = kept(0x000f000fu), c0 = kept(0x43004300u);
-  static __device__ __forceinline__ uint2 zero(uint32_t z) {
-    return make_uint2(0x43004300u | z * 0x10001u, 0);
-  }
+  static __device__ __forceinline__ uint32_t zero(uint32_t z) { return 0x43004300u | z * 0x10001u; }
+  __device__ __forceinline__ uint2 both(uint32_t z) const { return make_uint2(z, 0); }
   __device__ __forceinline__ void values(uint32_t w, uint2 z, uint32_t (&v)[4]) const {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -174,7 +171,7 @@ template <int RT, int NB, int PER> struct W4Shape {
   static constexpr int kEntries = kRows * PER;             // scales of a chunk
   static constexpr int kSumRows = kRows < 32 ? kRows : 32; // summed over the warps at a time
   static constexpr int kSums = kSumRows * 8 * NB * 4;      // of a warp
-  static constexpr int kWarpBytes = kDepth * kStage + kEntries * 12 + kSums;
+  static constexpr int kWarpBytes = kDepth * kStage + kEntries * 8 + kSums;
   static constexpr int kBytes = 512 + kWarps * kWarpBytes + kWarps * kDepth * 8 + 16;
   static constexpr int kCtas = 2 * (kBytes + 1024) <= 228 * 1024 ? 2 : 1;
 };
@@ -192,11 +189,9 @@ __global__ void __launch_bounds__(kWarps * 32, (W4Shape<RT, NB, PER>::kCtas))
   unsigned char *smem = raw + ((512 - (smem_u32(raw) & 511)) & 511);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
   unsigned char *ring = smem + warp * kDepth * Shape::kStage;
-  // of the chunk in hand: zeros as Unpack wants them, and scales
-  uint2 *zeros = reinterpret_cast<uint2 *>(smem + kWarps * kDepth * Shape::kStage) + warp * Shape::kEntries;
-  float *scales = reinterpret_cast<float *>(smem + kWarps * (kDepth * Shape::kStage + Shape::kEntries * 8)) +
-                  warp * Shape::kEntries;
-  float *sums = reinterpret_cast<float *>(smem + kWarps * (kDepth * Shape::kStage + Shape::kEntries * 12));
+  // of the chunk in hand: scale and zero of each row and group
+  uint2 *entries = reinterpret_cast<uint2 *>(smem + kWarps * kDepth * Shape::kStage) + warp * Shape::kEntries;
+  float *sums = reinterpret_cast<float *>(smem + kWarps * (kDepth * Shape::kStage + Shape::kEntries * 8));
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + kWarps * Shape::kWarpBytes);
   uint64_t *full = bars + warp * kDepth;
   volatile int *abort_flag = reinterpret_cast<volatile int *>(bars + kWarps * kDepth);
@@ -255,8 +250,7 @@ __global__ void __launch_bounds__(kWarps * 32, (W4Shape<RT, NB, PER>::kCtas))
                       : p.scale_dtype == OZ_BF16 ? __uint_as_float(bits << 16)
                                                  : __half2float(__ushort_as_half((unsigned short)bits));
       if (Shape::kEntries >= 32 || lane < Shape::kEntries) {
-        scales[i * 32 + lane] = f;
-        zeros[i * 32 + lane] = Unpack<T>::zero(zero_bits[i]);
+        entries[i * 32 + lane] = make_uint2(__float_as_uint(f), Unpack<T>::zero(zero_bits[i]));
       }
     }
     while (a_more && a_chunk >= chunks) {
@@ -333,8 +327,9 @@ __global__ void __launch_bounds__(kWarps * 32, (W4Shape<RT, NB, PER>::kCtas))
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const int entry = i / (4 / PER) * Shape::kRows + r * 16 + h * 8 + g;
-              scale[r][h] = scales[entry];
-              zero[r][h] = zeros[entry];
+              const uint2 v = entries[entry];
+              scale[r][h] = __uint_as_float(v.x);
+              zero[r][h] = unpack.both(v.y);
             }
         }
         // x: row g of each block of 8, the lane's 8 k, as the pairs (0 4) (1 5) (2 6) (3 7)
@@ -465,17 +460,40 @@ int run(const void *packed, const void *x, const W4Params &p, int dtype, int64_t
 }
 
 template <typename T>
-int choose(const void *packed, const void *x, const W4Params &p, int dtype, int64_t x_sr, int64_t p_se,
+int choose(const void *packed, const void *x, W4Params p, int dtype, int64_t x_sr, int64_t p_se,
            int64_t p_sn, cudaStream_t st) {
-  // rows of x a tile: as many as the mean group has (more would be read for nothing)
-  const int64_t mean = (p.rows + p.experts - 1) / p.experts;
-  if (mean > 16) return run<T, 2, 4>(packed, x, p, dtype, x_sr, p_se, p_sn, st);
-  if (mean > 8) return run<T, 4, 2>(packed, x, p, dtype, x_sr, p_se, p_sn, st);
-  // 64 weight rows a tile share the reading of x; 16 where that would leave SMs idle
-  const int64_t used = min(p.experts, p.rows);
-  if (used * ((p.n + 63) / 64) * p.along >= 2 * kWarps * (int64_t)tile::sm_count())
-    return run<T, 4, 1>(packed, x, p, dtype, x_sr, p_se, p_sn, st);
-  return run<T, 1, 1>(packed, x, p, dtype, x_sr, p_se, p_sn, st);
+  // Rows of x a tile: as many as the mean group has (more would be read for
+  // nothing).  Weight rows and warps a tile: the least estimated time, rounds of
+  // tiles over the GPU times a warp's chunks of a tile and half a one for the
+  // tile itself; a chunk of 16 weight rows takes 0.58 of one of 64 (instructions
+  // counted: 411 and 714).  9 rows / 64 experts, 1088 x 15288, 9 chunks: 8 warps a
+  // tile 61 us, 1 warp 37 us; 30 rows, 3520 x 11715: 8 warps 27 us, 2 warps 38 us.
+  const int64_t mean = (p.rows + p.experts - 1) / p.experts, used = min(p.experts, p.rows);
+  const int wide = mean > 16 ? 4 : mean > 8 ? 2 : 1;
+  const int64_t chunks = (p.k + kChunk - 1) / kChunk;
+  const int per = p.group % 128 == 0 ? 1 : p.group % 64 == 0 ? 2 : 4;
+  auto time = [&](int rt, int nb, int ctas, int along) {
+    const int64_t tiles = used * ((mean + 8 * nb - 1) / (8 * nb)) * ((p.n + 16 * rt - 1) / (16 * rt));
+    const int64_t teams = (int64_t)tile::sm_count() * ctas * (kWarps / along);
+    return (double)((tiles + teams - 1) / teams) * ((double)((chunks + along - 1) / along) + 0.5);
+  };
+  double best = 0;
+  bool narrow = false;
+  p.along = 0;
+  for (int along = kWarps; along; along /= 2) {
+    if (along > 1 && along > chunks) continue;
+    const double t = wide == 1 ? time(4, 1, per == 4 ? 1 : 2, along) : time(wide == 2 ? 4 : 2, wide, 1, along);
+    const double u = wide == 1 ? 0.58 * time(1, 1, 2, along) : t;
+    if (!p.along || min(t, u) < 0.93 * best) {           // more warps a tile unless it pays
+      best = min(t, u);
+      narrow = u < t;
+      p.along = along;
+    }
+  }
+  if (wide == 4) return run<T, 2, 4>(packed, x, p, dtype, x_sr, p_se, p_sn, st);
+  if (wide == 2) return run<T, 4, 2>(packed, x, p, dtype, x_sr, p_se, p_sn, st);
+  return narrow ? run<T, 1, 1>(packed, x, p, dtype, x_sr, p_se, p_sn, st)
+                : run<T, 4, 1>(packed, x, p, dtype, x_sr, p_se, p_sn, st);
 }
 
 }  // namespace
@@ -511,10 +529,9 @@ extern "C" int oz_matmul_w4(const oz_w4_args *args, void *stream) {
       p_sn % 16 != 0 || (experts > 1 && (p_se <= 0 || p_se % 16 != 0)))
     return set_error(OZ_ERR_INVALID,
                      "x and packed must start on 16-byte boundaries with row pitches of multiples of 16 bytes");
-  const int64_t chunks = (k + kChunk - 1) / kChunk;
   W4Params p{scales, offsets, static_cast<const uint8_t *>(zeros), y, offsets_64, experts, group,
              (int)(k / group), scale_dtype, out_dtype, (int)rows, (int)k, (int)n, ldy, s_se, s_sn,
-             chunks >= 8 ? 8 : chunks >= 4 ? 4 : chunks >= 2 ? 2 : 1,
+             0,
              group == 32 ? 0 : (uint32_t)(((1ull << 32) + group / 32 - 1) / (group / 32)), 0};
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   return dtype == OZ_F16 ? choose<__half>(packed, x, p, dtype, x_sr, p_se, p_sn, st)
