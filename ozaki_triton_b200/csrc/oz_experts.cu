@@ -245,34 +245,51 @@ bool readable(const void *p, int64_t rows, int64_t row_stride, int64_t mats, int
 
 // Copies of operands whose rows the copy unit cannot address (16-byte boundaries
 // and pitches): rows of 2-byte elements with unit stride to rows 16 bytes apart,
-// both operands of a call in one launch.  A warp takes 128 pairs of a row.
+// both operands of a call in one launch.  A warp takes up to 2048 elements of a
+// row, 9 words a lane on their way at a time (34 MB of odd rows: 20 us; 22 us
+// with loads of single elements).
 struct Repitch {
   const unsigned short *from;
   unsigned short *to;
-  int64_t from_row, from_mat, rows, mats, to_row;
+  int64_t from_row, from_mat, to_row;
+  uint32_t rows, lines, parts;         // rows of a matrix, of all, and parts of 2048 elements of a row
   int inner;
 };
 struct RepitchTwo { Repitch job[2]; };
+constexpr int kPart = 2048;
 
 __global__ void __launch_bounds__(256) repitch_kernel(const RepitchTwo two) {
   const Repitch &p = two.job[blockIdx.y];
-  const int lane = threadIdx.x % 32, pieces = (p.inner + 255) / 256;
-  const int64_t all = p.rows * p.mats * pieces;
-  for (int64_t v = (int64_t)blockIdx.x * 8 + threadIdx.x / 32; v < all; v += (int64_t)gridDim.x * 8) {
-    const int64_t line = v / pieces, mat = line / p.rows;
-    const int first = (int)(v - line * pieces) * 256 + lane * 2;
-    const unsigned short *from = p.from + mat * p.from_mat + (line - mat * p.rows) * p.from_row;
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int c = first + i * 64;
-      const uint32_t a = c < p.inner ? __ldg(from + c) : 0, b = c + 1 < p.inner ? __ldg(from + c + 1) : 0;
-      w[i] = a | b << 16;
-    }
+  const int lane = threadIdx.x % 32;
+  const uint64_t all = (uint64_t)p.lines * p.parts;
+  for (uint64_t v = (uint64_t)blockIdx.x * 8 + threadIdx.x / 32; v < all; v += (uint64_t)gridDim.x * 8) {
+    const uint32_t line = p.parts == 1 ? (uint32_t)v : (uint32_t)(v / p.parts);
+    const int first = p.parts == 1 ? 0 : (int)(v - (uint64_t)line * p.parts) * kPart;
+    const uint32_t mat = line / p.rows;
+    const unsigned short *from = p.from + mat * p.from_mat + (int64_t)(line - mat * p.rows) * p.from_row;
     uint32_t *to = reinterpret_cast<uint32_t *>(p.to + line * p.to_row);
+    const int count = min(p.inner - first, kPart);
+    // aligned words: a row that starts in the middle of one gets its pairs from two
+    // neighbouring words (the halves that belong to neither row nor part stay unused;
+    // they share their word with an element, so they can be read)
+    const unsigned short *start = from + first;
+    const int off = (int)((uintptr_t)start >> 1 & 1);
+    const uint32_t *words = reinterpret_cast<const uint32_t *>(start - off);
+    to += first / 2;
+    for (int j0 = 0; j0 * 2 < count; j0 += 256) {
+      uint32_t w[9];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (first + i * 64 < p.inner) to[(first + i * 64) / 2] = w[i];
+      for (int i = 0; i < 9; ++i) {
+        const int j = j0 + i * 32 + lane;
+        w[i] = 2 * j - off < count && (i < 8 || lane == 0) ? __ldg(words + j) : 0;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t down = __shfl_down_sync(0xffffffffu, w[i], 1), over = __shfl_sync(0xffffffffu, w[i + 1], 0);
+        const int j = j0 + i * 32 + lane;
+        if (2 * j < count) to[j] = off ? __funnelshift_r(w[i], lane == 31 ? over : down, 16) : w[i];
+      }
+    }
   }
 }
 
@@ -302,13 +319,15 @@ int lay_out(Operand *ops, void *workspace, int64_t workspace_bytes, cudaStream_t
     if ((uintptr_t)o.p % 2 != 0) return set_error(OZ_ERR_INVALID, "an operand is not aligned to its elements");
     unsigned char *to = static_cast<unsigned char *>(workspace) + at;
     const int64_t pitch = (o.inner + 7) / 8 * 8;
+    const int64_t parts = (o.inner + kPart - 1) / kPart;
+    if (o.rows * o.mats > INT32_MAX) return set_error(OZ_ERR_INVALID, "size out of range");
     two.job[n++] = Repitch{static_cast<const unsigned short *>(o.p), reinterpret_cast<unsigned short *>(to), o.row,
-                           o.mat, o.rows, o.mats, pitch, o.inner};
+                           o.mat, pitch, (uint32_t)o.rows, (uint32_t)(o.rows * o.mats), (uint32_t)parts, o.inner};
     o.p = to;
     o.row = pitch;
     o.mat = pitch * o.rows;
     at += bytes;
-    most = max(most, (o.rows * o.mats * ((o.inner + 255) / 256) + 7) / 8);
+    most = max(most, (o.rows * o.mats * parts + 7) / 8);
   }
   if (!n) return OZ_OK;
   count_launch();
@@ -332,8 +351,9 @@ int grouped(const void *x, const void *w, int64_t x_sr, int64_t w_se, bool acros
   // from the mean group (half a tile of each group is empty on average), times a
   // tile's blocks and four more for its start and end, times the bytes a CTA loads a
   // block: 128 columns by at most 32 rows (20 KB), 128 rows by 128 columns (32),
-  // pairs of CTAs 256 by 256 (32 each).  Measured, us: 1003 rows / 12 experts,
-  // 1000 x 1407 (GROUPED_A); 16 rows / 8 experts, 1024 x 2048 (GROUPED_B).
+  // pairs of CTAs 256 by 256 (32 each).  Measured, 128 x 128 against pairs: 256
+  // rows / 8 experts, 2048 x 2048, 23 and 16 us; 1003 rows / 12 experts, 1000 x 1408,
+  // 14 and 12 us.
   const int64_t groups = min(p.groups, p.rows);
   const double mean = (double)p.rows / groups;
   const double blocks64 = (p.k + kBlock - 1) / kBlock + 4;

@@ -606,8 +606,11 @@ __device__ __forceinline__ void write_rows(const Source &source, unsigned char *
         if (i * 8 + lane / 4 < rows)
           *reinterpret_cast<uint4 *>(to + c0 + i * 8 * ld) = *staged(mine, i * 8 + lane / 4, lane % 4);
     } else {
-      for (int r = 32 / CH > 1 ? lane / CH : 0; r < rows && r < 32; r += 32 / CH > 1 ? 32 / CH : 1)
-        if (c0 + lane % CH < cols)
+      // rows off the 16-byte boundaries: element by element (pairs from 4-byte
+      // boundary to 4-byte boundary took 30 us where this takes 23)
+#pragma unroll 8
+      for (int r = lane / CH; r < 32; r += 32 / CH)
+        if (r < rows && c0 + lane % CH < cols)
           out[r * ld + c0 + lane % CH] =
               reinterpret_cast<const O *>(staged(mine, r, lane % CH * ES / 16))[lane % CH % (16 / ES)];
     }
