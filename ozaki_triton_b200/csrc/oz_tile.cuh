@@ -282,31 +282,16 @@ __global__ void __launch_bounds__(threads<J>(), 1)
       const bool ragged = J::RAGGED && t.k_len % kBlock;
       if (lane == 0) {
         const int ar = t.a_row + (int)rank * kRows, br = t.b_row + (int)rank * BR;
-        for (int kb = 0; kb < blocks; ++kb, ++it) {
-          const int slot = it % S;
-          unsigned char *st = smem + slot * SB;
-          if (!(ok = mbar_wait_bounded(&empty[slot], ((it / S) & 1) ^ 1, abort_flag,
-                                       DEV_TIMEOUT_PRODUCER)))
-            break;
-          // a block's bytes count on the leader's barrier; those of a block
-          // that ends the range count on each CTA's own, for its clearing warp
-          const bool last = ragged && kb == blocks - 1;
-          const uint32_t bar = leader_addr(&full[slot]);
-          if (last) {
-            mbar_arrive_expect_tx(&tail[slot], SB);
-            turn ^= ((ended >> slot) & 1) << slot;
-            ended |= 1u << slot;
-          } else if (leader) {
-            mbar_arrive_expect_tx(&full[slot], PAIR * SB);
-          }
+        // the boxes of block kb: into this CTA, counted on the leader's barrier, or for a
+        // block that ends the range on each CTA's own, for its clearing warp
+        auto block = [&](int kb, unsigned char *st, uint32_t bar, uint64_t *own) {
           auto load = [&](void *dst, const CUtensorMap *map, int c0, int c1, int c2) {
             if constexpr (PAIR == 2) {
-              if (!last) {
-                tma_load_3d_pair(dst, map, bar, c0, c1, c2);
-                return;
-              }
+              if (!own) tma_load_3d_pair(dst, map, bar, c0, c1, c2);
+              else tma_load_3d(dst, map, own, c0, c1, c2);
+            } else {
+              tma_load_3d(dst, map, own, c0, c1, c2);
             }
-            tma_load_3d(dst, map, last ? &tail[slot] : &full[slot], c0, c1, c2);
           };
           const int k = (int)(t.k_begin + (int64_t)kb * kBlock);
 #pragma unroll
@@ -328,6 +313,24 @@ __global__ void __launch_bounds__(threads<J>(), 1)
             } else {
               load(sb, &tm_b, k, br, bm);
             }
+          }
+        };
+        const int whole = blocks - (ragged ? 1 : 0);
+        for (int kb = 0; kb < whole; ++kb, ++it) {
+          const int slot = it % S;
+          if (!(ok = mbar_wait_bounded(&empty[slot], ((it / S) & 1) ^ 1, abort_flag, DEV_TIMEOUT_PRODUCER))) break;
+          if (leader) mbar_arrive_expect_tx(&full[slot], PAIR * SB);
+          block(kb, smem + slot * SB, leader_addr(&full[slot]), PAIR == 2 ? nullptr : &full[slot]);
+        }
+        if (ragged && ok) {
+          const int slot = it % S;
+          ok = mbar_wait_bounded(&empty[slot], ((it / S) & 1) ^ 1, abort_flag, DEV_TIMEOUT_PRODUCER);
+          if (ok) {
+            mbar_arrive_expect_tx(&tail[slot], SB);
+            turn ^= ((ended >> slot) & 1) << slot;
+            ended |= 1u << slot;
+            block(whole, smem + slot * SB, 0, &tail[slot]);
+            ++it;
           }
         }
       }
@@ -366,7 +369,11 @@ __global__ void __launch_bounds__(threads<J>(), 1)
     const uint64_t a_desc = operand_desc<J::AMN>(base);
     const uint64_t b_desc = operand_desc<J::BMN>(base + J::PLANES * a_bytes<J>());
     uint32_t slot = 0, phase = 0;
-    auto multiply = [&](uint32_t d, bool first, int steps) {
+    auto instruction = [&](uint32_t d, uint64_t ad, uint64_t bd, uint32_t add) {
+      if constexpr (PAIR == 2) tc_mma_pair<1>(d, ad, bd, idesc, add);
+      else tc_mma<1>(d, ad, bd, idesc, add);
+    };
+    auto multiply = [&](uint32_t d, bool first) {
       const uint64_t ad = a_desc + slot * (SB >> 4), bd = b_desc + slot * (SB >> 4);
 #pragma unroll
       for (int q = 0; q < (J::PLANES == 2 ? 3 : 1); ++q) {
@@ -374,19 +381,22 @@ __global__ void __launch_bounds__(threads<J>(), 1)
         const uint64_t aq = ad + (J::PLANES == 2 && q == 0 ? a_bytes<J>() >> 4 : 0);
         const uint64_t bq = bd + (q == 1 ? b_bytes<J>() >> 4 : 0);
 #pragma unroll
-        for (int kk = 0; kk < kBlock / 16; ++kk) {
-          if (J::RAGGED && kk >= steps) break;
-          const uint32_t add = (kk | q) ? 1u : (first ? 0u : 1u);
-          if constexpr (PAIR == 2) tc_mma_pair<1>(d, aq + kk * a_step, bq + kk * b_step, idesc, add);
-          else tc_mma<1>(d, aq + kk * a_step, bq + kk * b_step, idesc, add);
-        }
+        for (int kk = 0; kk < kBlock / 16; ++kk)
+          instruction(d, aq + kk * a_step, bq + kk * b_step, (kk | q) ? 1u : (first ? 0u : 1u));
       }
       release(&empty[slot]);
+    };
+    auto advance = [&]() {
+      if (++slot == S) {
+        slot = 0;
+        phase ^= 1;
+      }
     };
     for (int i = unit; ok && walk.find(p, i, t); i += units) {
       if (lane == 0 && leader) {
         const int blocks = (int)((t.k_len + kBlock - 1) / kBlock);   // none: the epilogue writes zeros
         const int rest = J::RAGGED ? (int)(t.k_len % kBlock) : 0;
+        const int whole = blocks - (rest ? 1 : 0);
         // accumulator by accumulator: all blocks, or PASS at a time
         int kb = 0;
         while (kb < blocks) {
@@ -396,13 +406,24 @@ __global__ void __launch_bounds__(threads<J>(), 1)
           tc_fence_after();
           const uint32_t d = tmem + (uint32_t)(buf * NT);
           bool first = true;
-          for (; kb < stop; ++kb) {
+          for (const int to = min(stop, whole); kb < to; ++kb) {
             if (!(ok = wait(&full[slot], phase))) break;
-            multiply(d, first, rest && kb == blocks - 1 ? (rest + 15) / 16 : kBlock / 16);
+            multiply(d, first);
             first = false;
-            if (++slot == S) {
-              slot = 0;
-              phase ^= 1;
+            advance();
+          }
+          // a block that ends the range: the instructions that hold some of it.  Apart
+          // from the loop above, whose instructions have to come without a pause (with
+          // a test in it 8192^3 took 1084 us, without 715)
+          if (J::RAGGED && ok && kb < stop) {
+            ok = wait(&full[slot], phase);
+            if (ok) {
+              for (int kk = 0; kk * 16 < rest; ++kk)
+                instruction(d, a_desc + slot * (SB >> 4) + kk * a_step, b_desc + slot * (SB >> 4) + kk * b_step,
+                            kk ? 1u : (first ? 0u : 1u));
+              release(&empty[slot]);
+              advance();
+              ++kb;
             }
           }
           if (!ok) break;
