@@ -176,6 +176,45 @@ template <typename O, int NT_, bool AMN_> struct ColumnsJob : NoLookAhead {
   static __device__ void finish(const Params &p, int me, int warps) { clear_outside<O>(p, me, warps); }
 };
 
+// The exchanged roles for pairs of CTAs: 256 columns of w[e] by up to 256 rows of
+// x.  A group's rows are dealt out evenly to as few tiles as hold them, in multiples
+// of 32: with rows as A every group ends in a tile of 256 rows whatever is left
+// (32768 rows over 64 experts, 2048 x 2816: 356 us, this 344; 8192 rows over 64,
+// 2048 x 1408: 93 and 78).  Its epilogue turns the tile, which a short contraction
+// does not hide.
+template <typename O, bool AMN_> struct PairsJob : NoLookAhead {
+  static constexpr int PAIR = 2, NT = 256, PLANES = 1, PASS = sizeof(O) == 4 ? 8 : 0;
+  static constexpr bool AMN = AMN_, BMN = false, RAGGED = false, VARIABLE = true;
+  using Params = GroupedParams;
+  using Extra = RowTile;
+  static __device__ int plane_stride(const Params &) { return 0; }
+  struct Walk : GroupWalk {
+    using GroupWalk::GroupWalk;
+    __device__ bool find(const Params &p, int i, TileOf<Extra> &t) {
+      int e, lo, hi, block, column;
+      if (!GroupWalk::find(p, NT, 8, i, e, lo, hi, block, column)) return false;
+      const int blocks = (hi - lo + NT - 1) / NT, each = (hi - lo + blocks - 1) / blocks;
+      t.n = (each + 31) / 32 * 32;
+      t.a_row = column * 2 * kRows;
+      t.a_mat = e;
+      t.b_row = lo + block * t.n;
+      t.b_mat = 0;
+      t.k_begin = 0;
+      t.k_len = p.k;
+      t.extra = RowTile{t.b_row, min(t.n, hi - t.b_row), t.a_row};
+      return true;
+    }
+  };
+  template <class Source>
+  static __device__ void epilogue(const Params &p, const TileOf<Extra> &t, const Source &source, int row,
+                                  int column, unsigned char *mine, Ahead &) {
+    const int64_t c = t.extra.column + row;
+    write_columns<O, NT / 2>(source, mine, static_cast<O *>(p.out) + (int64_t)(t.extra.row + column) * p.ld + c, p.ld,
+                             t.extra.rows - column, p.n - c, p.vectors);
+  }
+  static __device__ void finish(const Params &p, int me, int warps) { clear_outside<O>(p, me, warps); }
+};
+
 struct WeightTile { int row, column, group; };
 
 // dw[e] = x^T dy over the group's rows: both operands are stored across the
@@ -362,28 +401,32 @@ int grouped(const void *x, const void *w, int64_t x_sr, int64_t w_se, bool acros
     return ceil(tiles * ctas / sm_count()) * blocks64 * bytes;
   };
   const double few_time = time(32, kRows, 20, 1), one_time = time(kRows, 128, 32, 1);
-  const double two_time = time(2 * kRows, 256, 32, 2);
+  const double two_time = time(256, 2 * kRows, 32, 2);
   const bool few = few_time <= one_time && few_time <= two_time;
   const int pair = two_time <= one_time ? 2 : 1;
+  // columns as A: 32 experts of 256 rows on average, 4096 columns: k 256 32 us (rows as
+  // A 30), k 512 45 (47), k 2048 143 (152); one of 20000 rows, k 2048: 234 (226)
+  const bool turned = pair == 2 && p.k >= 512 && mean < 2048;
   CUtensorMap tx, tw;
   const int64_t wr = across ? p.k : p.n, wi = across ? p.n : p.k;
-  const int nt = pair == 2 ? 256 : 128;
   const int64_t xb = pitch_bytes(x_sr, p.rows, p.k), wb = pitch_bytes(w_row, wr, wi);
-  if (int rc = make_map(&tx, x, p.k, p.rows, 1, xb, xb, few ? 32 : kRows))
-    return rc;
-  if (int rc = make_map(&tw, w, wi, wr, p.groups, wb, p.groups > 1 ? 2 * w_se : wb, across ? kBlock : few ? kRows : nt / pair))
+  if (int rc = make_map(&tx, x, p.k, p.rows, 1, xb, xb, few ? 32 : turned ? 64 : kRows)) return rc;
+  if (int rc = make_map(&tw, w, wi, wr, p.groups, wb, p.groups > 1 ? 2 * w_se : wb, across ? kBlock : kRows))
     return rc;
   const char *what = "grouped product launch";
   const int64_t per = few ? 32 : kRows * pair;
-  const int64_t blocks = p.rows / per + min((int64_t)p.groups, (int64_t)p.rows);
+  const int64_t blocks = p.rows / per + groups;
   if (few)
     return across ? run<ColumnsJob<O, 32, true>>(tw, tx, p, blocks, p.n, kRows, st, what)
                   : run<ColumnsJob<O, 32, false>>(tw, tx, p, blocks, p.n, kRows, st, what);
   if (pair == 1)
     return across ? run<RowsJob<O, 1, 128, true>>(tx, tw, p, blocks, p.n, 128, st, what)
                   : run<RowsJob<O, 1, 128, false>>(tx, tw, p, blocks, p.n, 128, st, what);
-  return across ? run<RowsJob<O, 2, 256, true>>(tx, tw, p, blocks, p.n, 256, st, what)
-                : run<RowsJob<O, 2, 256, false>>(tx, tw, p, blocks, p.n, 256, st, what);
+  if (!turned)
+    return across ? run<RowsJob<O, 2, 256, true>>(tx, tw, p, blocks, p.n, 256, st, what)
+                  : run<RowsJob<O, 2, 256, false>>(tx, tw, p, blocks, p.n, 256, st, what);
+  return across ? run<PairsJob<O, true>>(tw, tx, p, blocks, p.n, 256, st, what)
+                : run<PairsJob<O, false>>(tw, tx, p, blocks, p.n, 256, st, what);
 }
 
 template <typename O>

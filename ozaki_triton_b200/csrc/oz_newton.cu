@@ -308,7 +308,7 @@ struct StepTile { int z, row, column; bool mirror; };
 // below the diagonal, the others their mirror images.
 template <int PAIR_, int NT_, int PLANES_, int IN> struct SymmetricJob {
   static constexpr int PAIR = PAIR_, NT = NT_, PLANES = PLANES_, PASS = (PLANES_ - 1) * 4;
-  static constexpr bool AMN = false, BMN = false, RAGGED = false;
+  static constexpr bool AMN = false, BMN = false, RAGGED = false, VARIABLE = false;
   static constexpr int R = kRows * PAIR / NT;           // column tiles as wide as a tile is high
   using Params = StepParams;
   using Extra = StepTile;
@@ -378,7 +378,7 @@ template <int PAIR_, int NT_, int PLANES_, int IN> struct SymmetricJob {
 template <int PAIR_, int NT_, int PLANES_> struct UpdateJob {
   static constexpr int IN = 2;
   static constexpr int PAIR = PAIR_, NT = NT_, PLANES = PLANES_, PASS = (PLANES_ - 1) * 4;
-  static constexpr bool AMN = false, BMN = true, RAGGED = false;
+  static constexpr bool AMN = false, BMN = true, RAGGED = false, VARIABLE = false;
   using Params = StepParams;
   using Extra = StepTile;
   static __device__ int plane_stride(const Params &p) { return p.batch; }

@@ -26,6 +26,9 @@
 // block is there, ahead of the products (done by the MMA warp in its turn it
 // cost 8 of 48 us on 256 tiles of 4 blocks).
 //
+// With VARIABLE a tile has t.n <= NT columns, a multiple of 32, and both the loads
+// (B's rows in one or two boxes of 64) and the instructions go by that.
+//
 // With PASS > 0 an accumulator takes at most PASS blocks and the epilogue adds
 // the passes in registers: the tensor core cuts each sum off instead of
 // rounding it, an error that grows with the number of blocks (relative 1.1e-6
@@ -56,6 +59,7 @@ constexpr int kSmemLimit = 227 * 1024;
 
 // For jobs whose epilogue reads nothing but the accumulators.
 struct NoLookAhead {
+  static constexpr bool VARIABLE = false;
   struct Ahead {};
   template <class P, class T> static __device__ void look_ahead(const P &, const T &, int, int, Ahead &) {}
 };
@@ -78,7 +82,7 @@ template <class J> __host__ __device__ constexpr int smem_bytes() {
 // Where a tile's operands lie: first row (or column) and matrix of A and B in
 // their tensor maps, the contraction range, and what the job's epilogue wants.
 template <class Extra> struct TileOf {
-  int a_row, a_mat, b_row, b_mat;
+  int a_row, a_mat, b_row, b_mat, n;
   int64_t k_begin, k_len;
   Extra extra;
 };
@@ -144,8 +148,7 @@ template <bool MN> __device__ __forceinline__ uint64_t operand_desc(uint32_t add
 __device__ __forceinline__ bool wait_cluster(uint64_t *bar, uint32_t parity, volatile int *abort,
                                              int code) {
   const uint32_t a = smem_u32(bar);
-  const long long t0 = clock64();
-  for (uint32_t it = 0;; ++it) {
+  auto there = [&]() {
     uint32_t ok;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
@@ -154,7 +157,12 @@ __device__ __forceinline__ bool wait_cluster(uint64_t *bar, uint32_t parity, vol
         : "=r"(ok)
         : "r"(a), "r"(parity)
         : "memory");
-    if (ok) return true;
+    return ok != 0;
+  };
+  if (there()) return true;
+  const long long t0 = clock64();
+  for (uint32_t it = 0;; ++it) {
+    if (there()) return true;
     if ((it & 63u) == 63u) {
       if (*abort) return false;
       if (clock64() - t0 > kWaitBoundCycles) {
@@ -281,7 +289,10 @@ __global__ void __launch_bounds__(threads<J>(), 1)
       const int blocks = (int)((t.k_len + kBlock - 1) / kBlock);
       const bool ragged = J::RAGGED && t.k_len % kBlock;
       if (lane == 0) {
-        const int ar = t.a_row + (int)rank * kRows, br = t.b_row + (int)rank * BR;
+        const int ar = t.a_row + (int)rank * kRows;
+        const int br = t.b_row + (int)rank * (J::VARIABLE ? t.n / PAIR : BR);
+        const bool two = t.n / PAIR > 64;
+        const uint32_t bytes = J::VARIABLE ? J::PLANES * (a_bytes<J>() + (two ? 128 : 64) * kLine) : SB;
         // the boxes of block kb: into this CTA, counted on the leader's barrier, or for a
         // block that ends the range on each CTA's own, for its clearing warp
         auto block = [&](int kb, unsigned char *st, uint32_t bar, uint64_t *own) {
@@ -310,6 +321,9 @@ __global__ void __launch_bounds__(threads<J>(), 1)
 #pragma unroll
               for (int c = 0; c < BR / 64; ++c)
                 load(sb + c * kBlock * kLine, &tm_b, br + c * 64, k, bm);
+            } else if constexpr (J::VARIABLE) {
+              load(sb, &tm_b, k, br, bm);
+              if (two) load(sb + 64 * kLine, &tm_b, k, br + 64, bm);
             } else {
               load(sb, &tm_b, k, br, bm);
             }
@@ -319,7 +333,7 @@ __global__ void __launch_bounds__(threads<J>(), 1)
         for (int kb = 0; kb < whole; ++kb, ++it) {
           const int slot = it % S;
           if (!(ok = mbar_wait_bounded(&empty[slot], ((it / S) & 1) ^ 1, abort_flag, DEV_TIMEOUT_PRODUCER))) break;
-          if (leader) mbar_arrive_expect_tx(&full[slot], PAIR * SB);
+          if (leader) mbar_arrive_expect_tx(&full[slot], PAIR * bytes);
           block(kb, smem + slot * SB, leader_addr(&full[slot]), PAIR == 2 ? nullptr : &full[slot]);
         }
         if (ragged && ok) {
@@ -352,7 +366,7 @@ __global__ void __launch_bounds__(threads<J>(), 1)
     uint32_t done = 0;
     bool ok = true;
     const uint32_t base = smem_u32(smem);
-    const uint32_t idesc = p.idesc | ((uint32_t)(NT >> 3) << 17) |
+    const uint32_t fixed = p.idesc | (J::VARIABLE ? 0u : (uint32_t)(NT >> 3) << 17) |
                            ((uint32_t)((kRows * PAIR) >> 4) << 24) | (J::AMN ? 1u << 15 : 0u) |
                            (J::BMN ? 1u << 16 : 0u);
     constexpr uint64_t a_step = J::AMN ? (16 * kLine) >> 4 : 2, b_step = J::BMN ? (16 * kLine) >> 4 : 2;
@@ -369,6 +383,7 @@ __global__ void __launch_bounds__(threads<J>(), 1)
     const uint64_t a_desc = operand_desc<J::AMN>(base);
     const uint64_t b_desc = operand_desc<J::BMN>(base + J::PLANES * a_bytes<J>());
     uint32_t slot = 0, phase = 0;
+    uint32_t idesc = fixed;
     auto instruction = [&](uint32_t d, uint64_t ad, uint64_t bd, uint32_t add) {
       if constexpr (PAIR == 2) tc_mma_pair<1>(d, ad, bd, idesc, add);
       else tc_mma<1>(d, ad, bd, idesc, add);
@@ -397,6 +412,7 @@ __global__ void __launch_bounds__(threads<J>(), 1)
         const int blocks = (int)((t.k_len + kBlock - 1) / kBlock);   // none: the epilogue writes zeros
         const int rest = J::RAGGED ? (int)(t.k_len % kBlock) : 0;
         const int whole = blocks - (rest ? 1 : 0);
+        if constexpr (J::VARIABLE) idesc = fixed | (uint32_t)(t.n >> 3) << 17;
         // accumulator by accumulator: all blocks, or PASS at a time
         int kb = 0;
         while (kb < blocks) {
@@ -634,6 +650,47 @@ __device__ __forceinline__ void write_rows(const Source &source, unsigned char *
         if (r < rows && c0 + lane % CH < cols)
           out[r * ld + c0 + lane % CH] =
               reinterpret_cast<const O *>(staged(mine, r, lane % CH * ES / 16))[lane % CH % (16 / ES)];
+    }
+    __syncwarp();
+  }
+}
+
+// The same where the lanes hold columns of the output and the accumulator
+// columns are its rows: `rows` of them from out on, 32 columns wide.
+template <typename O, int COLS, class Source>
+__device__ __forceinline__ void write_columns(const Source &source, unsigned char *mine, O *out, int64_t ld,
+                                              int rows, int64_t cols, bool vectors) {
+  constexpr int ES = (int)sizeof(O), RH = 64 / ES;        // rows staged at a time, 32 ES bytes each
+  constexpr int PIECES = 32 * ES / 16, PER = 32 / PIECES;
+  const int lane = threadIdx.x % 32;
+  O *to = out + (int64_t)(lane / PIECES) * ld + lane % PIECES * (16 / ES);
+  // 16-byte piece u of row r: shifted by the row, so that a row's write and the
+  // pieces' reads touch every bank once
+  auto piece = [&](int r, int u) {
+    return reinterpret_cast<uint4 *>(mine + r * (32 * ES) + ((ES == 2 ? u ^ (r >> 1 & 3) : u ^ (r & 7)) << 4));
+  };
+#pragma unroll
+  for (int r0 = 0; r0 < COLS; r0 += RH) {
+    if (r0 >= rows || cols <= 0) continue;
+#pragma unroll
+    for (int c = 0; c < RH; c += 16) {
+      float v[16];
+      source.read(r0 + c, v);
+#pragma unroll
+      for (int x = 0; x < 16; ++x)
+        reinterpret_cast<O *>(piece(c + x, lane * ES / 16))[lane % (16 / ES)] = O(v[x]);
+    }
+    __syncwarp();
+    if (vectors && cols >= 32) {
+#pragma unroll
+      for (int i = 0; i < RH; i += PER)
+        if (r0 + i + lane / PIECES < rows)
+          *reinterpret_cast<uint4 *>(to + (r0 + i) * ld) = *piece(i + lane / PIECES, lane % PIECES);
+    } else {
+#pragma unroll 8
+      for (int r = 0; r < RH; ++r)
+        if (r0 + r < rows && lane < cols)
+          out[(r0 + r) * ld + lane] = reinterpret_cast<const O *>(piece(r, lane * ES / 16))[lane % (16 / ES)];
     }
     __syncwarp();
   }
