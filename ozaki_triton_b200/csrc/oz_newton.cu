@@ -59,7 +59,8 @@ struct InitParams {
 };
 
 // 8 consecutive elements from a 16-byte boundary.
-__device__ __forceinline__ void load8(const void *p, int dtype, int64_t i, float (&v)[8]) {
+template <int DTYPE> __device__ __forceinline__ void load8(const void *p, int64_t i, float (&v)[8]) {
+  constexpr int dtype = DTYPE;
   if (dtype == OZ_F32) {
     const float4 *q = reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i);
     const float4 a = __ldg(q), b = __ldg(q + 1);
@@ -88,23 +89,28 @@ __device__ double block_sum(double sum, double *part) {
 
 // Sums of squares in fp64 (fp32 would overflow from 1.8e19 on), each block a
 // fixed part: the order of the sum does not depend on the launch.
-__global__ void __launch_bounds__(256) squares_kernel(const InitParams p) {
+template <int DTYPE> __global__ void __launch_bounds__(256) squares_kernel(const InitParams p) {
   __shared__ double part[8];
   const int64_t base = blockIdx.y * p.g_sb, stride = (int64_t)gridDim.x * 256;
   double sum = 0;
   if (p.flat) {
     const int64_t pieces = (int64_t)p.rows * p.cols / 8;
     int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    for (; i < pieces; i += 2 * stride) {
-      float v[2][8];
-      load8(p.g, p.dtype, base + i * 8, v[0]);
-      const bool two = i + stride < pieces;
-      if (two) load8(p.g, p.dtype, base + (i + stride) * 8, v[1]);
+    for (; i < pieces; i += 4 * stride) {
+      float v[4][8];
 #pragma unroll
-      for (int x = 0; x < 8; ++x) sum += (double)v[0][x] * v[0][x];
-      if (two)
+      for (int u = 0; u < 4; ++u) {
+        if (i + u * stride < pieces) {
+          load8<DTYPE>(p.g, base + (i + u * stride) * 8, v[u]);
+        } else {
 #pragma unroll
-        for (int x = 0; x < 8; ++x) sum += (double)v[1][x] * v[1][x];
+          for (int x = 0; x < 8; ++x) v[u][x] = 0.f;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int x = 0; x < 8; ++x) sum += (double)v[u][x] * v[u][x];
     }
   } else {
     // a line at a time, consecutive threads along the smaller stride
@@ -114,7 +120,7 @@ __global__ void __launch_bounds__(256) squares_kernel(const InitParams p) {
     const int wide = inner >= 256 ? 256 : 32;                // threads of a line
     for (int o = blockIdx.x * (256 / wide) + threadIdx.x / wide; o < outer; o += gridDim.x * (256 / wide))
       for (int i = threadIdx.x % wide; i < inner; i += wide) {
-        const double v = load_value(p.g, p.dtype, base + o * s_out + i * s_in);
+        const double v = load_value(p.g, DTYPE, base + o * s_out + i * s_in);
         sum += v * v;
       }
   }
@@ -125,14 +131,25 @@ __global__ void __launch_bounds__(256) squares_kernel(const InitParams p) {
 // X_0 in slices, 64 x 64 tiles: 8 elements at a time from G along its smaller
 // stride, through shared memory where that is across X's rows, and 8 at a
 // time to X along its rows (whose pitch is a multiple of 8).
-__global__ void __launch_bounds__(256) normalise_kernel(const InitParams p) {
+template <int DTYPE> __global__ void __launch_bounds__(256) normalise_kernel(const InitParams p) {
   __shared__ double part[8];
   __shared__ float tile[64][65];
   double sum = 0;
   for (int i = threadIdx.x; i < p.partials; i += 256) sum += p.partial[(int64_t)blockIdx.z * p.partials + i];
   sum = block_sum(sum, part);
-  const double scale = p.scale / (sqrt(sum) + p.eps);
-  const bool zero = sum == 0 && p.eps == 0;             // 0 / 0: a zero matrix stays zero
+  // the scale as a float in [1, 2) and two powers of two, which together have its
+  // range: the product with each element is rounded once (the scale itself 2^-24 off)
+  __shared__ float factors[3];
+  if (threadIdx.x == 0) {
+    const double scale = sum == 0 && p.eps == 0 ? 0.0 : p.scale / (sqrt(sum) + p.eps);   // a zero matrix stays zero
+    int e = 0;
+    factors[0] = isfinite(scale) ? (float)(2 * frexp(scale, &e)) : (float)scale;
+    e = max(-250, min(250, e - 1));
+    factors[1] = (float)ldexp(1.0, e / 2);
+    factors[2] = (float)ldexp(1.0, e - e / 2);
+  }
+  __syncthreads();
+  const float f0 = factors[0], f1 = factors[1], f2 = factors[2];
   const bool across = p.g_sr < p.g_sc;
   const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
 #pragma unroll
@@ -145,14 +162,14 @@ __global__ void __launch_bounds__(256) normalise_kernel(const InitParams p) {
     const int64_t at = blockIdx.z * p.g_sb + r * p.g_sr + c * p.g_sc, step = across ? p.g_sr : p.g_sc;
     float v[8];
     if (p.vectors && left >= 8) {
-      load8(p.g, p.dtype, at, v);
+      load8<DTYPE>(p.g, at, v);
     } else {
 #pragma unroll
-      for (int x = 0; x < 8; ++x) v[x] = x < left ? load_value(p.g, p.dtype, at + x * step) : 0.f;
+      for (int x = 0; x < 8; ++x) v[x] = x < left ? load_value(p.g, DTYPE, at + x * step) : 0.f;
     }
 #pragma unroll
     for (int x = 0; x < 8; ++x) {
-      const float f = zero ? 0.f : (float)(v[x] * scale);
+      const float f = v[x] * f1 * f0 * f2;
       if (across) tile[u + x][line] = f;
       else tile[line][u + x] = f;
     }
@@ -826,6 +843,16 @@ int step_product(const CUtensorMap &a, const CUtensorMap &b, StepParams p, bool 
   return launch<J>(a, b, p, tiles * p.batch, st, "newton step launch");
 }
 
+template <int DTYPE> int start(const InitParams &init, int batch, cudaStream_t st) {
+  count_launch();
+  squares_kernel<DTYPE><<<dim3((unsigned)init.partials, (unsigned)batch), 256, 0, st>>>(init);
+  if (int rc = check_cuda(cudaGetLastError(), "squares_kernel launch")) return rc;
+  const dim3 grid((unsigned)((init.cols + 63) / 64), (unsigned)((init.rows + 63) / 64), (unsigned)batch);
+  count_launch();
+  normalise_kernel<DTYPE><<<grid, 256, 0, st>>>(init);
+  return check_cuda(cudaGetLastError(), "normalise_kernel launch");
+}
+
 template <int SPLITS>
 int run(const InitParams &init, const Layout &l, int batch, int steps, const double *coefficients,
         unsigned char *ws, StepParams last, cudaStream_t st) {
@@ -837,13 +864,10 @@ int run(const InitParams &init, const Layout &l, int batch, int steps, const dou
   Planes x[2] = {planes(l.x0, ldx, l.x_mat), planes(l.x1, ldx, l.x_mat)};
   const Planes s = planes(l.s, lds, l.s_mat), q = planes(l.p, lds, l.s_mat);
 
-  count_launch();
-  squares_kernel<<<dim3((unsigned)init.partials, (unsigned)batch), 256, 0, st>>>(init);
-  if (int rc = check_cuda(cudaGetLastError(), "squares_kernel launch")) return rc;
-  count_launch();
-  normalise_kernel<<<dim3((unsigned)((cols + 63) / 64), (unsigned)((rows + 63) / 64), (unsigned)batch), 256, 0,
-                     st>>>(init);
-  if (int rc = check_cuda(cudaGetLastError(), "normalise_kernel launch")) return rc;
+  if (int rc = init.dtype == OZ_F32   ? start<OZ_F32>(init, batch, st)
+               : init.dtype == OZ_F16 ? start<OZ_F16>(init, batch, st)
+                                      : start<OZ_BF16>(init, batch, st))
+    return rc;
 
   const bool pair_s = use_pairs(true, batch, rows, rows), pair_x = use_pairs(false, batch, rows, cols);
   // each matrix in the boxes its products read: 128 rows (A), the columns of a

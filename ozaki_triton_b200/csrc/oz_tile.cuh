@@ -219,6 +219,7 @@ __global__ void __launch_bounds__(threads<J>(), 1)
   static_assert((NT & (NT - 1)) == 0 && NT >= 32 && NT <= 256 && 2 * NT <= 512, "tile columns");
   static_assert(!J::BMN || BR % 64 == 0, "an MN-major B comes in chunks of 64");
   static_assert(S >= 3, "too few stages");
+  static_assert(!J::VARIABLE || !J::BMN, "a variable B is stored along the contraction");
 
   extern __shared__ unsigned char smem_raw[];
   unsigned char *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
