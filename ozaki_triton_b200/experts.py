@@ -271,7 +271,8 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, *,
     boundaries, are copied first);
     offsets (E + 1,) int32 or int64.  Returns (T, N) in the operands' dtype, or
     fp32 with ``out_dtype=torch.float32``.  Sums are held in fp32 and rounded
-    once.  Differentiable in x and w.
+    once.  Differentiable in x and w: the gradient is rounded to the operands'
+    dtype before it is multiplied.
     """
     if (x.requires_grad or w.requires_grad) and torch.is_grad_enabled():
         return _GroupedMatmul.apply(x, w, offsets, out_dtype)
@@ -376,7 +377,9 @@ def matmul_w4(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor,
     uint8, or None for 8 everywhere (the layout ``quantize_w4`` returns).
     With ``offsets`` the weights have a leading expert dimension and the rows
     of x come in groups.  Returns (T, N) in x's dtype or fp32.  Made for few
-    rows a matrix (the weights' bytes bound it); any number is right.
+    rows a matrix (the weights' bytes bound it); any number is right.  Layouts
+    that the copy unit cannot read are copied first.  For serving: no gradient
+    is recorded.
     """
     xp, pp = x.data_ptr(), packed.data_ptr()
     key = (x.shape, x.stride(), x.dtype, packed.shape, packed.stride(), packed.dtype, scales.shape,

@@ -62,7 +62,8 @@ def orthogonalize(g: torch.Tensor, steps: int = 5,
     independent.  X = g / (|g|_F + eps), then ``steps`` times with A = X X^T
     X <- a X + (b A + c A^2) X, which drives the singular values of X towards
     1 (``coefficients``: one (a, b, c) for all steps or one for each).  Returns
-    a contiguous tensor of g's shape and dtype.
+    a contiguous tensor of g's shape and dtype.  For updates: no gradient is
+    recorded.
 
     ``num_splits`` is how many fp16 slices of each matrix the products use: 1
     (11 bits, the default for bf16 whose result has 8) or 2 (22 bits, the

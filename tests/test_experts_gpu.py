@@ -77,6 +77,9 @@ RAGGED = [
     ([2] * 70, 0, 0, 64, 256),
     ([40] * 40, 0, 0, 256, 320),
     ([1100, 900], 0, 0, 520, 776),
+    ([100] * 100, 0, 0, 200, 100),
+    ([900, 1100, 700], 3, 5, 200, 1000),
+    ([1300, 0, 901], 1, 0, 264, 1003),
 ]
 
 
@@ -103,7 +106,7 @@ def test_grouped_products_of_whole_numbers_are_exact(sizes, before, after, k, n,
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
-@pytest.mark.parametrize("sizes,before,after,k,n", RAGGED[2:5] + RAGGED[7:9])
+@pytest.mark.parametrize("sizes,before,after,k,n", RAGGED[2:5] + RAGGED[7:9] + RAGGED[11:])
 def test_grouped_products_of_normal_values(sizes, before, after, k, n, dtype):
     g = generator(k * n)
     rows = before + sum(sizes) + after
@@ -252,7 +255,8 @@ def weights(packed, scales, zeros):
 
 
 W4 = [(1, 32, 1, 32), (1, 256, 64, 32), (2, 64, 7, 64), (3, 4256, 517, 32), (8, 1024, 129, 128), (9, 2048, 256, 128),
-      (1, 4096, 300, 256), (17, 96, 1000, 96), (40, 384, 33, 192), (5, 16384, 24, 128), (1, 8192, 2048, 64)]
+      (1, 4096, 300, 256), (17, 96, 1000, 96), (40, 384, 33, 192), (5, 16384, 24, 128), (1, 8192, 2048, 64),
+      (4, 1024, 20000, 64), (4, 1024, 20000, 128), (2, 1024, 20011, 32), (12, 320, 20000, 64), (20, 256, 9000, 128)]
 
 
 @pytest.mark.parametrize("zeros", [False, True], ids=["symmetric", "zeros"])
