@@ -323,8 +323,8 @@ struct StepTile { int z, row, column; bool mirror; };
 
 // S = X X^T (IN 0) and P = b S + c S S (IN slices of S): tiles (i, j) on and
 // below the diagonal, the others their mirror images.
-template <int PAIR_, int NT_, int PLANES_, int IN> struct SymmetricJob {
-  static constexpr int PAIR = PAIR_, NT = NT_, PLANES = PLANES_, PASS = (PLANES_ - 1) * 4;
+template <int PAIR_, int NT_, int PLANES_, int IN, int PASS_> struct SymmetricJob {
+  static constexpr int PAIR = PAIR_, NT = NT_, PLANES = PLANES_, PASS = PASS_;
   static constexpr bool AMN = false, BMN = false, RAGGED = false, VARIABLE = false;
   static constexpr int R = kRows * PAIR / NT;           // column tiles as wide as a tile is high
   using Params = StepParams;
@@ -392,9 +392,9 @@ template <int PAIR_, int NT_, int PLANES_, int IN> struct SymmetricJob {
 };
 
 // X <- a X + P X: A is the rows of P, B the columns of X.
-template <int PAIR_, int NT_, int PLANES_> struct UpdateJob {
+template <int PAIR_, int NT_, int PLANES_, int PASS_> struct UpdateJob {
   static constexpr int IN = 2;
-  static constexpr int PAIR = PAIR_, NT = NT_, PLANES = PLANES_, PASS = (PLANES_ - 1) * 4;
+  static constexpr int PAIR = PAIR_, NT = NT_, PLANES = PLANES_, PASS = PASS_;
   static constexpr bool AMN = false, BMN = true, RAGGED = false, VARIABLE = false;
   using Params = StepParams;
   using Extra = StepTile;
@@ -853,7 +853,8 @@ template <int DTYPE> int start(const InitParams &init, int batch, cudaStream_t s
   return check_cuda(cudaGetLastError(), "normalise_kernel launch");
 }
 
-template <int SPLITS>
+// PASS: blocks an accumulator takes before it is added in registers (0: all of them).
+template <int SPLITS, int PASS>
 int run(const InitParams &init, const Layout &l, int batch, int steps, const double *coefficients,
         unsigned char *ws, StepParams last, cudaStream_t st) {
   const int rows = (int)l.rows, cols = (int)l.cols;
@@ -900,16 +901,16 @@ int run(const InitParams &init, const Layout &l, int batch, int steps, const dou
     sym.alpha = 0;
     sym.beta = (float)std::ldexp(1.0, es - 2 * ex);
     sym.out = s;
-    int rc = pair_s ? step_product<SymmetricJob<2, 256, SPLITS, 0>>(xa[cur], xb[cur], sym, true, st)
-                    : step_product<SymmetricJob<1, 64, SPLITS, 0>>(xa[cur], xb[cur], sym, true, st);
+    int rc = pair_s ? step_product<SymmetricJob<2, 256, SPLITS, 0, PASS>>(xa[cur], xb[cur], sym, true, st)
+                    : step_product<SymmetricJob<1, 64, SPLITS, 0, PASS>>(xa[cur], xb[cur], sym, true, st);
     if (rc) return rc;
     sym.k = rows;
     sym.in = s;
     sym.alpha = (float)std::ldexp(b, ep - es);
     sym.beta = (float)std::ldexp(c, ep - 2 * es);
     sym.out = q;
-    rc = pair_s ? step_product<SymmetricJob<2, 256, SPLITS, SPLITS>>(sa, sb, sym, true, st)
-                : step_product<SymmetricJob<1, 64, SPLITS, SPLITS>>(sa, sb, sym, true, st);
+    rc = pair_s ? step_product<SymmetricJob<2, 256, SPLITS, SPLITS, PASS>>(sa, sb, sym, true, st)
+                : step_product<SymmetricJob<1, 64, SPLITS, SPLITS, PASS>>(sa, sb, sym, true, st);
     if (rc) return rc;
     most = std::min(largest_value(a, b, c, most) * slack, 1e15);
     const bool end = i + 1 == steps;
@@ -925,8 +926,8 @@ int run(const InitParams &init, const Layout &l, int batch, int steps, const dou
     up.out = x[cur ^ 1];
     up.alpha = (float)std::ldexp(a, en - ex);
     up.beta = (float)std::ldexp(1.0, en - ep - ex);
-    rc = pair_x ? step_product<UpdateJob<2, 256, SPLITS>>(pa, xu[cur], up, false, st)
-                : step_product<UpdateJob<1, 64, SPLITS>>(pa, xu[cur], up, false, st);
+    rc = pair_x ? step_product<UpdateJob<2, 256, SPLITS, PASS>>(pa, xu[cur], up, false, st)
+                : step_product<UpdateJob<1, 64, SPLITS, PASS>>(pa, xu[cur], up, false, st);
     if (rc) return rc;
     cur ^= 1;
     ex = en;
@@ -1011,6 +1012,12 @@ extern "C" int oz_orthogonalize(const void *g, int dtype, int64_t batch, int64_t
   last.last_sr = tall ? 1 : n;
   last.last_sc = tall ? n : 1;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  return num_splits == 1 ? run<1>(init, l, (int)batch, steps, coefficients, ws, last, st)
-                         : run<2>(init, l, (int)batch, steps, coefficients, ws, last, st);
+  if (num_splits == 1) return run<1, 0>(init, l, (int)batch, steps, coefficients, ws, last, st);
+  // Two slices: sums cut off every block where the launches and not the products take
+  // the time, every 4 blocks where it would cost (4096 x 4096: 4682 us and 6.4e-7 off
+  // against 3531 us and 1.3e-6; fp32 sums 3.7e-6.  200 x 800: 3.7e-6 with 4, 1.0e-6
+  // with 1, fp32 sums 1.5e-6)
+  const double work = (double)batch * l.rows * l.rows * (3.0 * l.cols + l.rows);
+  return work < 2e10 ? run<2, 1>(init, l, (int)batch, steps, coefficients, ws, last, st)
+                     : run<2, 4>(init, l, (int)batch, steps, coefficients, ws, last, st);
 }

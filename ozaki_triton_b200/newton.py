@@ -31,7 +31,9 @@ def _plan(key, g, steps, coefficients, eps, num_splits) -> _Plan:
     assert steps >= 1, f"at least one step is needed, got {steps}"
     assert eps >= 0, f"eps must not be negative, got {eps}"
     if num_splits is None:
-        num_splits = 1 if g.dtype == torch.bfloat16 else 2
+        rows, cols = sorted(g.shape[-2:])
+        work = g.numel() * rows * (3 + rows / max(cols, 1))           # of a step
+        num_splits = 1 if g.dtype == torch.bfloat16 and work >= 5e9 else 2
     assert num_splits in (1, 2), f"num_splits must be 1 or 2, got {num_splits}"
     rows = list(coefficients) if hasattr(coefficients[0], "__len__") else [coefficients] * steps
     assert len(rows) == steps and all(len(r) == 3 for r in rows), \
@@ -66,9 +68,10 @@ def orthogonalize(g: torch.Tensor, steps: int = 5,
     recorded.
 
     ``num_splits`` is how many fp16 slices of each matrix the products use: 1
-    (11 bits, the default for bf16 whose result has 8) or 2 (22 bits, the
-    default for fp32 and fp16).  Sums are held in fp32.  Small matrices (up to
-    128 rows or columns) are worked on in fp32 whatever it is.
+    (11 bits, the default for bf16, whose result has 8, where the products'
+    time counts: batch M N min(M, N) above 2e9 or so) or 2 (22 bits, the default
+    elsewhere).  Sums are held in fp32.  Small matrices (up to 128 rows or
+    columns) are worked on in fp32 whatever it is.
     """
     if not isinstance(coefficients, tuple) or hasattr(coefficients[0], "__len__"):
         coefficients = tuple(tuple(c) if hasattr(c, "__len__") else c for c in coefficients)
