@@ -199,6 +199,11 @@ struct StepParams {
   int row_tiles, column_tiles, tiles;   // tiles of one member
   float alpha, beta;                // result = alpha * in + beta * accumulator
   Planes in, out;
+  // S of few rows and many columns: `parts` CTAs a tile, each `part_blocks` blocks of
+  // the contraction, whose sums go to partial (parts, batch, rows, part_ld)
+  int parts, part_blocks;
+  int64_t part_ld;
+  float *partial;
   // the last step's result instead of `out`: element (z, r, c) of the type
   void *last;
   int last_dtype;
@@ -390,6 +395,65 @@ template <int PAIR_, int NT_, int PLANES_, int IN, int PASS_> struct SymmetricJo
   }
   static __device__ void finish(const Params &, int, int) {}
 };
+
+// S of few rows and many columns: the same tiles, each with a part of the
+// contraction; its sums are left to add_parts_kernel.
+template <int PLANES, int PASS> struct PartsJob : SymmetricJob<1, 64, PLANES, 0, PASS> {
+  using Whole = SymmetricJob<1, 64, PLANES, 0, PASS>;
+  using typename Whole::Params;
+  using typename Whole::Extra;
+  using typename Whole::Ahead;
+  struct Walk : Whole::Walk {
+    __device__ Walk(const Params &p) : Whole::Walk(p) {}
+    __device__ bool find(const Params &p, int t, TileOf<Extra> &tile) {
+      const int part = t / (p.tiles * p.batch);
+      if (part >= p.parts || !Whole::Walk::find(p, t - part * p.tiles * p.batch, tile)) return false;
+      tile.k_begin = (int64_t)part * p.part_blocks * kBlock;
+      tile.k_len = min((int64_t)p.part_blocks * kBlock, p.k - tile.k_begin);
+      tile.extra.z += part * p.batch;
+      return true;
+    }
+  };
+  template <class Source>
+  static __device__ void epilogue(const Params &p, const TileOf<Extra> &t, const Source &source, int row,
+                                  int column, unsigned char *mine, Ahead &) {
+    const int r0 = t.extra.row + row, c0 = t.extra.column + column;
+    if (r0 < p.rows && c0 < p.cols)
+      write_rows<float, 32>(source, mine, p.partial + ((int64_t)t.extra.z * p.rows + r0) * p.part_ld + c0,
+                            p.part_ld, p.rows - r0, p.cols - c0, true);
+  }
+};
+
+// The parts of S added up in their order, sliced, and mirrored: 32 x 32 tiles on
+// and below the diagonal.
+__global__ void __launch_bounds__(256) add_parts_kernel(const StepParams p, int planes) {
+  __shared__ float tile[32][33];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int r0 = blockIdx.y * 32, c0 = blockIdx.x * 32, z = blockIdx.z;
+  if (c0 > r0) return;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  for (int i = warp; i < 32; i += 8) {
+    float sum = 0.f;
+    // above the diagonal of a diagonal tile: the element below it (both are there)
+    const int r = max(r0 + i, c0 + lane), c = min(r0 + i, c0 + lane);
+    if (r < p.rows)
+      for (int part = 0; part < p.parts; ++part)
+        sum += p.partial[((int64_t)(part * p.batch + z) * p.rows + r) * p.part_ld + c];
+    tile[i][lane] = p.beta * sum;
+  }
+  __syncthreads();
+  for (int i = warp; i < 32; i += 8) {
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {
+      const int r = (side ? c0 : r0) + i, c = (side ? r0 : c0) + lane;
+      if (r >= p.rows || c >= p.rows || (side && r0 == c0)) continue;
+      const float v = side ? tile[lane][i] : tile[i][lane];
+      const __half high = __float2half_rn(v);
+      *p.out.at(0, z, r, c) = high;
+      if (planes == 2) *p.out.at(1, z, r, c) = __float2half_rn(v - __half2float(high));
+    }
+  }
+}
 
 // X <- a X + P X: A is the rows of P, B the columns of X.
 template <int PAIR_, int NT_, int PLANES_, int PASS_> struct UpdateJob {
@@ -771,8 +835,11 @@ int64_t pitch(int64_t n) { return (n + 7) / 8 * 8; }
 
 // Workspace of a call: sums of squares, two X's, S and P in slices.
 struct Layout {
-  int64_t rows, cols, x_mat, s_mat, x0, x1, s, p, total;
+  int64_t rows, cols, x_mat, s_mat, x0, x1, s, p, partial, total;
+  int parts, part_blocks;           // of S's contraction
 };
+int64_t member_tiles(bool symmetric, int64_t rows, int64_t cols, int high, int wide);
+bool use_pairs(bool symmetric, int64_t batch, int64_t rows, int64_t cols);
 Layout layout(int64_t batch, int64_t m, int64_t n, int splits) {
   Layout l{};
   l.rows = m < n ? m : n;
@@ -785,7 +852,17 @@ Layout layout(int64_t batch, int64_t m, int64_t n, int splits) {
   l.x1 = l.x0 + x;
   l.s = l.x1 + x;
   l.p = l.s + s;
-  l.total = l.p + s;
+  l.partial = l.p + s;
+  // S of few rows: parts of at least 8 blocks on the SMs that its tiles leave idle
+  // (68 x 3686, 5 matrices: 309 us a call in one part, 178 in 10)
+  const int64_t blocks = (l.cols + kBlock - 1) / kBlock;
+  int64_t parts = 1;
+  if (batch && l.rows && blocks >= 32 && !use_pairs(true, batch, l.rows, l.rows))
+    parts = std::max<int64_t>(
+        1, std::min<int64_t>({16, sm_count() / (batch * member_tiles(true, l.rows, l.rows, 128, 64)), blocks / 8}));
+  l.part_blocks = (int)((blocks + parts - 1) / parts);
+  l.parts = (int)((blocks + l.part_blocks - 1) / std::max(l.part_blocks, 1));  // none is empty
+  l.total = l.partial + (l.parts > 1 ? align256(l.parts * batch * l.rows * pitch(l.rows) * 4) : 0);
   return l;
 }
 
@@ -840,7 +917,22 @@ int step_product(const CUtensorMap &a, const CUtensorMap &b, StepParams p, bool 
   p.row_tiles = (p.rows + kRows * J::PAIR - 1) / (kRows * J::PAIR);
   p.column_tiles = (p.cols + J::NT - 1) / J::NT;
   p.tiles = (int)tiles;
-  return launch<J>(a, b, p, tiles * p.batch, st, "newton step launch");
+  return launch<J>(a, b, p, tiles * p.batch * max(p.parts, 1), st, "newton step launch");
+}
+
+int add_parts(const StepParams &p, int planes, cudaStream_t st) {
+  const unsigned side = (unsigned)((p.rows + 31) / 32);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(side, side, (unsigned)p.batch);
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  count_launch();
+  return check_cuda(cudaLaunchKernelEx(&cfg, add_parts_kernel, p, planes), "add_parts_kernel launch");
 }
 
 template <int DTYPE> int start(const InitParams &init, int batch, cudaStream_t st) {
@@ -901,9 +993,17 @@ int run(const InitParams &init, const Layout &l, int batch, int steps, const dou
     sym.alpha = 0;
     sym.beta = (float)std::ldexp(1.0, es - 2 * ex);
     sym.out = s;
+    sym.parts = l.parts;
+    sym.part_blocks = l.part_blocks;
+    sym.part_ld = pitch(rows);
+    sym.partial = reinterpret_cast<float *>(ws + l.partial);
     int rc = pair_s ? step_product<SymmetricJob<2, 256, SPLITS, 0, PASS>>(xa[cur], xb[cur], sym, true, st)
-                    : step_product<SymmetricJob<1, 64, SPLITS, 0, PASS>>(xa[cur], xb[cur], sym, true, st);
+             : l.parts > 1
+                 ? step_product<PartsJob<SPLITS, PASS>>(xa[cur], xb[cur], sym, true, st)
+                 : step_product<SymmetricJob<1, 64, SPLITS, 0, PASS>>(xa[cur], xb[cur], sym, true, st);
+    if (rc == OZ_OK && l.parts > 1) rc = add_parts(sym, SPLITS, st);
     if (rc) return rc;
+    sym.parts = 1;
     sym.k = rows;
     sym.in = s;
     sym.alpha = (float)std::ldexp(b, ep - es);
