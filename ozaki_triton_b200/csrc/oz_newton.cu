@@ -65,25 +65,44 @@ struct InitParams {
   double eps, scale;
 };
 
-// 8 consecutive elements from a 16-byte boundary.
-template <int DTYPE> __device__ __forceinline__ void load8(const void *p, int64_t i, float (&v)[8]) {
-  constexpr int dtype = DTYPE;
-  if (dtype == OZ_F32) {
-    const float4 *q = reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i);
-    const float4 a = __ldg(q), b = __ldg(q + 1);
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-    return;
-  }
-  const uint4 a = __ldg(reinterpret_cast<const uint4 *>(static_cast<const __half *>(p) + i));
-  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+// 8 elements of G as they are stored.
+template <int DTYPE> struct Eight {
+  static constexpr int kWords = DTYPE == OZ_F32 ? 8 : 4;
+  uint32_t w[kWords];
+  // from a 16-byte boundary, one after the other
+  __device__ __forceinline__ void load(const void *p, int64_t i) {
+    const uint4 *q = reinterpret_cast<const uint4 *>(static_cast<const char *>(p) + i * (kWords / 2));
 #pragma unroll
-  for (int x = 0; x < 4; ++x) {
-    const float2 f = dtype == OZ_F16 ? __half22float2(*reinterpret_cast<const __half2 *>(&w[x]))
-                                     : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&w[x]));
-    v[2 * x] = f.x;
-    v[2 * x + 1] = f.y;
+    for (int x = 0; x < kWords / 4; ++x) {
+      const uint4 a = __ldg(q + x);
+      w[4 * x] = a.x, w[4 * x + 1] = a.y, w[4 * x + 2] = a.z, w[4 * x + 3] = a.w;
+    }
   }
-}
+  // the first `left`, `step` apart; the others are zero
+  __device__ __forceinline__ void load(const void *p, int64_t i, int64_t step, int left) {
+#pragma unroll
+    for (int x = 0; x < kWords; ++x) w[x] = 0;
+#pragma unroll
+    for (int x = 0; x < 8; ++x)
+      if (x < left) {
+        if (DTYPE == OZ_F32) w[x % kWords] = __ldg(static_cast<const uint32_t *>(p) + i + x * step);
+        else w[x / 2 % kWords] |= (uint32_t)__ldg(static_cast<const unsigned short *>(p) + i + x * step) << x % 2 * 16;
+      }
+  }
+  __device__ __forceinline__ void floats(float (&v)[8]) const {
+#pragma unroll
+    for (int x = 0; x < kWords; ++x) {
+      if (DTYPE == OZ_F32) {
+        v[x] = __uint_as_float(w[x]);
+        continue;
+      }
+      const float2 f = DTYPE == OZ_F16 ? __half22float2(*reinterpret_cast<const __half2 *>(&w[x]))
+                                       : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&w[x]));
+      v[2 * x % 8] = f.x;
+      v[(2 * x + 1) % 8] = f.y;
+    }
+  }
+};
 
 __device__ double block_sum(double sum, double *part) {
   for (int o = 16; o; o /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -94,30 +113,45 @@ __device__ double block_sum(double sum, double *part) {
   return sum;
 }
 
-// Sums of squares in fp64 (fp32 would overflow from 1.8e19 on), each block a
-// fixed part: the order of the sum does not depend on the launch.
+// sum + the squares of 8 elements: in fp32 where neither an overflow nor the loss of
+// small ones beside the largest can matter (a group's sum is then 2^-22 off at most),
+// since conversions to fp64 are slow (46 MB of bf16 in 25 us with one an element), else
+// in fp64.
+template <int DTYPE> __device__ __forceinline__ double add_squares(double sum, const float (&v)[8]) {
+  float most = 0.f;
+#pragma unroll
+  for (int x = 0; x < 8; ++x) most = fmaxf(most, fabsf(v[x]));
+  if (DTYPE == OZ_F16 || (most >= 0x1p-40f && most <= 0x1p60f)) {
+    const float a = fmaf(v[3], v[3], fmaf(v[2], v[2], fmaf(v[1], v[1], v[0] * v[0])));
+    const float b = fmaf(v[7], v[7], fmaf(v[6], v[6], fmaf(v[5], v[5], v[4] * v[4])));
+    return sum + (double)(a + b);
+  }
+#pragma unroll
+  for (int x = 0; x < 8; ++x) sum += (double)v[x] * v[x];
+  return sum;
+}
+
+// Sums of squares, held in fp64, each block a fixed part: the order of the sum does
+// not depend on the launch.
 template <int DTYPE> __global__ void __launch_bounds__(256) squares_kernel(const InitParams p) {
   __shared__ double part[8];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int64_t base = blockIdx.y * p.g_sb, stride = (int64_t)gridDim.x * 256;
   double sum = 0;
   if (p.flat) {
     const int64_t pieces = (int64_t)p.rows * p.cols / 8;
     int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     for (; i < pieces; i += 4 * stride) {
-      float v[4][8];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        if (i + u * stride < pieces) {
-          load8<DTYPE>(p.g, base + (i + u * stride) * 8, v[u]);
-        } else {
-#pragma unroll
-          for (int x = 0; x < 8; ++x) v[u][x] = 0.f;
-        }
-      }
+      Eight<DTYPE> some[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u)
+        if (i + u * stride < pieces) some[u].load(p.g, base + (i + u * stride) * 8);
 #pragma unroll
-        for (int x = 0; x < 8; ++x) sum += (double)v[u][x] * v[u][x];
+      for (int u = 0; u < 4; ++u) {
+        float v[8];
+        some[u].floats(v);
+        if (i + u * stride < pieces) sum = add_squares<DTYPE>(sum, v);
+      }
     }
   } else {
     // a line at a time, consecutive threads along the smaller stride
@@ -137,10 +171,32 @@ template <int DTYPE> __global__ void __launch_bounds__(256) squares_kernel(const
 
 // X_0 in slices, 64 x 64 tiles: 8 elements at a time from G along its smaller
 // stride, through shared memory where that is across X's rows, and 8 at a
-// time to X along its rows (whose pitch is a multiple of 8).
-template <int DTYPE> __global__ void __launch_bounds__(256) normalise_kernel(const InitParams p) {
+// time to X along its rows (whose pitch is a multiple of 8).  A block takes many tiles,
+// each one's elements on their way while the one before is written (a block for
+// each tile added up the partial sums 5632 times for 4 x 2048 x 2816 bf16: 35 us, this 29).
+template <int DTYPE> __global__ void __launch_bounds__(256, 6) normalise_kernel(const InitParams p) {
   __shared__ double part[8];
   __shared__ float tile[64][65];
+  const bool across = p.g_sr < p.g_sc;
+  const int64_t step = across ? p.g_sr : p.g_sc;
+  const int wide = (p.cols + 63) / 64, tiles = wide * ((p.rows + 63) / 64);
+  Eight<DTYPE> next[2];
+  auto fetch = [&](int t) {
+    const int r0 = t / wide * 64, c0 = t % wide * 64;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      // line and piece of G's tile
+      const int line = threadIdx.x / 8 + h * 32, u = threadIdx.x % 8 * 8;
+      const int r = r0 + (across ? u : line), c = c0 + (across ? line : u);
+      const int left = r >= p.rows || c >= p.cols ? 0 : across ? p.rows - r : p.cols - c;
+      const int64_t at = blockIdx.z * p.g_sb + r * p.g_sr + c * p.g_sc;
+      if (p.vectors && left >= 8) next[h].load(p.g, at);
+      else next[h].load(p.g, at, step, left);
+    }
+  };
+  if (blockIdx.x < tiles) fetch(blockIdx.x);
+  asm volatile("griddepcontrol.wait;" ::: "memory");      // the partial sums
+
   double sum = 0;
   for (int i = threadIdx.x; i < p.partials; i += 256) sum += p.partial[(int64_t)blockIdx.z * p.partials + i];
   sum = block_sum(sum, part);
@@ -157,46 +213,39 @@ template <int DTYPE> __global__ void __launch_bounds__(256) normalise_kernel(con
   }
   __syncthreads();
   const float f0 = factors[0], f1 = factors[1], f2 = factors[2];
-  const bool across = p.g_sr < p.g_sc;
-  const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
+  for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
 #pragma unroll
-  for (int i = threadIdx.x; i < 512; i += 256) {
-    // line and piece of G's tile
-    const int line = i / 8, u = i % 8 * 8;
-    const int r = r0 + (across ? u : line), c = c0 + (across ? line : u);
-    if (r >= p.rows || c >= p.cols) continue;
-    const int left = across ? p.rows - r : p.cols - c;
-    const int64_t at = blockIdx.z * p.g_sb + r * p.g_sr + c * p.g_sc, step = across ? p.g_sr : p.g_sc;
-    float v[8];
-    if (p.vectors && left >= 8) {
-      load8<DTYPE>(p.g, at, v);
-    } else {
+    for (int h = 0; h < 2; ++h) {
+      const int line = threadIdx.x / 8 + h * 32, u = threadIdx.x % 8 * 8;
+      float v[8];
+      next[h].floats(v);
 #pragma unroll
-      for (int x = 0; x < 8; ++x) v[x] = x < left ? load_value(p.g, DTYPE, at + x * step) : 0.f;
+      for (int x = 0; x < 8; ++x) {
+        const float f = v[x] * f1 * f0 * f2;
+        if (across) tile[u + x][line] = f;
+        else tile[line][u + x] = f;
+      }
     }
+    __syncthreads();
+    if (t + gridDim.x < tiles) fetch(t + gridDim.x);
+    const int r0 = t / wide * 64, c0 = t % wide * 64;
 #pragma unroll
-    for (int x = 0; x < 8; ++x) {
-      const float f = v[x] * f1 * f0 * f2;
-      if (across) tile[u + x][line] = f;
-      else tile[line][u + x] = f;
+    for (int h = 0; h < 2; ++h) {
+      const int r = threadIdx.x / 8 + h * 32, u = threadIdx.x % 8 * 8;
+      if (r0 + r >= p.rows || c0 + u >= p.cols) continue;
+      uint32_t high[4], low[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const float a = tile[r][u + 2 * x], b = tile[r][u + 2 * x + 1];
+        const __half2 high2 = __floats2half2_rn(a, b);
+        const float2 f = __half22float2(high2);
+        high[x] = *reinterpret_cast<const uint32_t *>(&high2);
+        low[x] = pack2<__half>(a - f.x, b - f.y);
+      }
+      *reinterpret_cast<uint4 *>(p.x.at(0, blockIdx.z, r0 + r, c0 + u)) = make_uint4(high[0], high[1], high[2], high[3]);
+      *reinterpret_cast<uint4 *>(p.x.at(1, blockIdx.z, r0 + r, c0 + u)) = make_uint4(low[0], low[1], low[2], low[3]);
     }
-  }
-  __syncthreads();
-#pragma unroll
-  for (int i = threadIdx.x; i < 512; i += 256) {
-    const int r = i / 8, u = i % 8 * 8;
-    if (r0 + r >= p.rows || c0 + u >= p.cols) continue;
-    uint32_t high[4], low[4];
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const float a = tile[r][u + 2 * x], b = tile[r][u + 2 * x + 1];
-      const __half2 h = __floats2half2_rn(a, b);
-      const float2 f = __half22float2(h);
-      high[x] = *reinterpret_cast<const uint32_t *>(&h);
-      low[x] = pack2<__half>(a - f.x, b - f.y);
-    }
-    *reinterpret_cast<uint4 *>(p.x.at(0, blockIdx.z, r0 + r, c0 + u)) = make_uint4(high[0], high[1], high[2], high[3]);
-    *reinterpret_cast<uint4 *>(p.x.at(1, blockIdx.z, r0 + r, c0 + u)) = make_uint4(low[0], low[1], low[2], low[3]);
+    __syncthreads();
   }
 }
 
@@ -927,10 +976,11 @@ int step_product(const CUtensorMap &a, const CUtensorMap &b, StepParams p, bool 
   return launch<J>(a, b, p, tiles * p.batch * max(p.parts, 1), st, "newton step launch");
 }
 
-int add_parts(const StepParams &p, int planes, cudaStream_t st) {
-  const unsigned side = (unsigned)((p.rows + 31) / 32);
+// A launch of 256 threads that may start before the one before it has ended.
+template <class... A>
+int launch_after(void (*kernel)(A...), dim3 grid, const char *what, cudaStream_t st, A... args) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(side, side, (unsigned)p.batch);
+  cfg.gridDim = grid;
   cfg.blockDim = dim3(256);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -939,17 +989,22 @@ int add_parts(const StepParams &p, int planes, cudaStream_t st) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   count_launch();
-  return check_cuda(cudaLaunchKernelEx(&cfg, add_parts_kernel, p, planes), "add_parts_kernel launch");
+  return check_cuda(cudaLaunchKernelEx(&cfg, kernel, args...), what);
+}
+
+int add_parts(const StepParams &p, int planes, cudaStream_t st) {
+  const unsigned side = (unsigned)((p.rows + 31) / 32);
+  return launch_after(add_parts_kernel, dim3(side, side, (unsigned)p.batch), "add_parts_kernel launch", st, p, planes);
 }
 
 template <int DTYPE> int start(const InitParams &init, int batch, cudaStream_t st) {
   count_launch();
   squares_kernel<DTYPE><<<dim3((unsigned)init.partials, (unsigned)batch), 256, 0, st>>>(init);
   if (int rc = check_cuda(cudaGetLastError(), "squares_kernel launch")) return rc;
-  const dim3 grid((unsigned)((init.cols + 63) / 64), (unsigned)((init.rows + 63) / 64), (unsigned)batch);
-  count_launch();
-  normalise_kernel<DTYPE><<<grid, 256, 0, st>>>(init);
-  return check_cuda(cudaGetLastError(), "normalise_kernel launch");
+  const int64_t tiles = (int64_t)((init.cols + 63) / 64) * ((init.rows + 63) / 64);
+  const int64_t most = std::max<int64_t>(1, 6 * sm_count() / batch);          // tiles at a time of a member
+  return launch_after(normalise_kernel<DTYPE>, dim3((unsigned)std::min(tiles, most), 1, (unsigned)batch),
+                      "normalise_kernel launch", st, init);
 }
 
 // PASS: blocks an accumulator takes before it is added in registers (0: all of them).
