@@ -22,7 +22,7 @@
 // 5 steps measured: 4096 x 4096 fp32 (two slices) 3.45 ms, 1200 TFLOP/s of fp16
 // products (2.46 ms at the burst rate), bound by the tensor cores under the power
 // limit and by 136 tiles of S and P for 74 pairs of CTAs; 4 x 2048 x 2816 bf16
-// (one slice) 0.91 ms (0.52 at the burst rate), bound by what the products and the
+// (one slice) 0.89 ms (0.52 at the burst rate), bound by what the products and the
 // epilogues' slices move between L2 and the SMs; up to 1000 or so rows the launches'
 // length (17 of 7 us or so).
 
@@ -264,6 +264,7 @@ struct StepParams {
   void *last;
   int last_dtype;
   int64_t last_sb, last_sr, last_sc;
+  bool last_vectors;                // its rows start on 16-byte boundaries
 };
 
 // 32 rows x 32 fp16 columns: each lane 4 pieces of 8 columns, 64 bytes of a
@@ -586,6 +587,25 @@ template <int PAIR_, int NT_, int PLANES_, int PASS_> struct UpdateJob {
                 if (wide) out32[lane + x * p.last_sc] = v[x];
                 else out16[lane + x * p.last_sc] = bits(v[x]);
               }
+          }
+        } else if (p.last_vectors) {
+          // 64 bytes of a row at a time (4 x 2048 x 2816 bf16: the last product 105 us with single elements,
+          // 83 so)
+          uint4 w[4];
+          if (wide) {
+#pragma unroll
+            for (int h = 0; h < 32; h += 16) {
+#pragma unroll
+              for (int u = 0; u < 4; ++u) w[u] = *reinterpret_cast<const uint4 *>(&v[h + u * 4]);
+              store_rows(mine, reinterpret_cast<__half *>(out32 + h), 2 * p.last_sr, rows, 2 * (cols - h), w);
+            }
+          } else {
+            __half h[32];
+#pragma unroll
+            for (int x = 0; x < 32; ++x) h[x] = bits(v[x]);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) w[u] = *reinterpret_cast<const uint4 *>(&h[u * 8]);
+            store_rows(mine, out16, p.last_sr, rows, cols, w);
           }
         } else {
 #pragma unroll
@@ -1173,6 +1193,7 @@ extern "C" int oz_orthogonalize(const void *g, int dtype, int64_t batch, int64_t
   last.last_sb = m * n;
   last.last_sr = tall ? 1 : n;
   last.last_sc = tall ? n : 1;
+  last.last_vectors = !tall && (uintptr_t)out % 16 == 0 && n * (dtype == OZ_F32 ? 4 : 2) % 16 == 0;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (num_splits == 1) return run<1, 0>(init, l, (int)batch, steps, coefficients, ws, last, st);
   // Two slices: sums cut off every block where the launches and not the products take
