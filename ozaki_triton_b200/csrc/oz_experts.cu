@@ -292,8 +292,9 @@ bool readable(const void *p, int64_t rows, int64_t row_stride, int64_t mats, int
 // Copies of operands whose rows the copy unit cannot address (16-byte boundaries
 // and pitches): rows of 2-byte elements with unit stride to rows 16 bytes apart,
 // both operands of a call in one launch.  A warp takes up to 2048 elements of a
-// row, 9 words a lane on their way at a time (34 MB of odd rows: 20 us; 22 us
-// with loads of single elements).
+// row, 9 words a lane on their way at a time.  1003 rows / 12 experts, 1000 x 1407,
+// most of whose time is this copy of 34 MB: 33.1 us with 6 blocks an SM, 39.4
+// with 4, 35.3 with 8 (and so fewer registers), 34.5 with 13 words.
 struct Repitch {
   const unsigned short *from;
   unsigned short *to;
@@ -304,7 +305,7 @@ struct Repitch {
 struct RepitchTwo { Repitch job[2]; };
 constexpr int kPart = 2048;
 
-__global__ void __launch_bounds__(256) repitch_kernel(const RepitchTwo two) {
+__global__ void __launch_bounds__(256, 6) repitch_kernel(const __grid_constant__ RepitchTwo two) {
   const Repitch &p = two.job[blockIdx.y];
   const int lane = threadIdx.x % 32;
   const uint64_t all = (uint64_t)p.lines * p.parts;
