@@ -640,7 +640,8 @@ template <int PAIR_, int NT_, int PLANES_, int PASS_> struct UpdateJob {
 // all of them: the panels' X X^T are added in the order of the ranks, P is
 // computed a few rows a CTA and handed to the others, and a X + P X needs
 // nothing of another panel.  fp32 FMAs are enough here (and rounded sums more
-// exact than the tensor core's): a step of 64 x 250 is 0.4 M FMAs a CTA.
+// exact than the tensor core's): a step of 64 x 250 is 0.23 M FMAs a CTA.  12 of
+// them take 42 us, 16 x 16 takes 13 us: barriers, exchanges and the latency of each part.
 constexpr int kSmallRows = 128;
 constexpr int kSmallThreads = 256;
 constexpr int kMicro = 4;                // rows and columns of a thread's tile
@@ -684,15 +685,15 @@ __device__ __forceinline__ void tile_along(const float *a, int lda, const float 
   }
 }
 
-// Threads that share the terms of a tile when there are fewer tiles than threads.
+// log2 of the threads (up to 8) that share the terms of a tile when there are fewer
+// tiles than threads.
 __device__ __forceinline__ int sharing(int tiles) {
-  int n = 1;
-  while (n < 8 && tiles * n * 2 <= kSmallThreads) n *= 2;
-  return n;
+  static_assert(kSmallThreads == 256, "the limits below");
+  return tiles <= 32 ? 3 : tiles <= 64 ? 2 : tiles <= 128 ? 1 : 0;
 }
 
-__device__ __forceinline__ void add_shared(float (&acc)[kMicro][kMicro], int share) {
-  for (int o = 1; o < share; o *= 2)
+__device__ __forceinline__ void add_shared(float (&acc)[kMicro][kMicro], int log) {
+  for (int o = 1; o < 1 << log; o *= 2)
 #pragma unroll
     for (int i = 0; i < kMicro; ++i)
 #pragma unroll
@@ -742,98 +743,121 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const SmallPara
   for (int i = tid; i < rm * p.x_ld; i += kSmallThreads) x[i] = (float)(x[i] * scale);
   __syncthreads();
 
+  // What does not change from step to step is computed here: a step of a small
+  // matrix is bound by latencies, and divisions by variables have long ones
+  // (12 matrices of 64 x 250: 8.0 us a step with them in it, 7.1 so).
   const int side = rm / kMicro;
+  const uint32_t inverse = ((1u << 20) + side - 1) / side;
+  auto by_side = [&](int v) { return (int)((uint32_t)v * inverse >> 20); };   // v / side for v < 2^20 / side
+  auto below = [&](int t, int &i, int &j) {                 // tile t on and below the diagonal
+    i = (int)((sqrtf(8.f * t + 1.f) - 1.f) * 0.5f);
+    while ((i + 1) * (i + 2) / 2 <= t) ++i;
+    while (i * (i + 1) / 2 > t) --i;
+    j = t - i * (i + 1) / 2;
+  };
   const int slice = (side + ranks - 1) / ranks * kMicro;    // rows of S and P that this CTA makes
   const int first = min(rank * slice, rm), last = min(first + slice, rm);
+  const int s_tiles = side * (side + 1) / 2, p_tiles = (last - first) / kMicro * side;
+  const int p_log = sharing(p_tiles), x_log = sharing(side * (p.panel / kMicro));
+  const int abreast = by_side(kSmallThreads >> x_log);      // column tiles of a round of the update
+  const int x_column = by_side(tid >> x_log), x_row = (tid >> x_log) - x_column * side;
+  int first_i, first_j;
+  below(tid >> sharing(s_tiles), first_i, first_j);
   for (int step = 0; step < p.steps; ++step) {
     const float a = p.abc[3 * step], b = p.abc[3 * step + 1], c = p.abc[3 * step + 2];
-    {   // this panel's X X^T; a tile takes every side-th row, so that the threads of
-        // a warp read neighbouring rows (whose pitch is odd: no bank conflicts)
-      const int tiles = side * side, share = sharing(tiles), kq = tid % share;
-      for (int t0 = 0; t0 < tiles; t0 += kSmallThreads / share) {
-        const int t = t0 + tid / share, ti = t / side, tj = t - ti * side;
-        float acc[kMicro][kMicro] = {};
-        if (t < tiles) {
-          const float *xi = x + ti * p.x_ld, *xj = x + tj * p.x_ld;
-          for (int k = kq * 4; k < p.panel; k += share * 4) {
-            float4 u[kMicro], w[kMicro];
-#pragma unroll
-            for (int i = 0; i < kMicro; ++i) {
-              u[i] = *reinterpret_cast<const float4 *>(xi + i * side * p.x_ld + k);
-              w[i] = *reinterpret_cast<const float4 *>(xj + i * side * p.x_ld + k);
-            }
-#pragma unroll
-            for (int i = 0; i < kMicro; ++i)
-#pragma unroll
-              for (int j = 0; j < kMicro; ++j)
-                acc[i][j] = fmaf(u[i].w, w[j].w, fmaf(u[i].z, w[j].z, fmaf(u[i].y, w[j].y, fmaf(u[i].x, w[j].x, acc[i][j]))));
-          }
-        }
-        add_shared(acc, share);
-        if (t < tiles && kq == 0)
-#pragma unroll
-          for (int i = 0; i < kMicro; ++i)
-#pragma unroll
-            for (int j = 0; j < kMicro; ++j) q[(ti + i * side) * p.s_ld + tj + j * side] = acc[i][j];
-      }
-    }
-    together();
-    // S, rows [first, last) of it here, for everyone
-    for (int v = tid; v < (last - first) * (rm / 4); v += kSmallThreads) {
-      const int at = (first + v / (rm / 4)) * p.s_ld + v % (rm / 4) * 4;
-      const uint32_t from_q = smem_u32(q + at), to_s = smem_u32(s + at);
-      float4 o[8], f = make_float4(0.f, 0.f, 0.f, 0.f);   // all on their way before the first is used
-#pragma unroll
-      for (int r = 0; r < 8; ++r)
-        if (r < ranks) o[r] = peer_load(map_to_cta(from_q, (uint32_t)r));
-#pragma unroll
-      for (int r = 0; r < 8; ++r)
-        if (r < ranks) f.x += o[r].x, f.y += o[r].y, f.z += o[r].z, f.w += o[r].w;
-      for (int r = 0; r < ranks; ++r) peer_store(map_to_cta(to_s, (uint32_t)r), f);
-    }
-    together();
-    {   // the same rows of P = b S + c S S
-      const int tiles = (last - first) / kMicro * side, share = sharing(max(tiles, 1)), kq = tid % share;
-      for (int t0 = 0; t0 < tiles; t0 += kSmallThreads / share) {
-        const int t = t0 + tid / share, i0 = first + t / side * kMicro, j0 = t % side * kMicro;
-        float acc[kMicro][kMicro] = {};
-        if (t < tiles) tile_along(s + i0, p.s_ld, s + j0, p.s_ld, kq, share, rm, acc);
-        add_shared(acc, share);
-        if (t < tiles && kq == 0)
-#pragma unroll
-          for (int i = 0; i < kMicro; ++i)
-#pragma unroll
-            for (int j = 0; j < kMicro; j += 4) {
-              const int at = (i0 + i) * p.s_ld + j0 + j;
-              const float4 o = *reinterpret_cast<const float4 *>(s + at);
-              const float4 f = make_float4(b * o.x + c * acc[i][j], b * o.y + c * acc[i][j + 1],
-                                           b * o.z + c * acc[i][j + 2], b * o.w + c * acc[i][j + 3]);
-              const uint32_t to = smem_u32(q + at);
-              for (int r = 0; r < ranks; ++r) peer_store(map_to_cta(to, (uint32_t)r), f);
-            }
-      }
-    }
-    together();
-    // X <- a X + P X, the columns of a round from registers once all have read them
-    const int share = sharing(side * (p.panel / kMicro)), kq = tid % share, t = tid / share;
-    const int abreast = kSmallThreads / share / side;      // column tiles of a round
-    for (int base = 0; base < p.panel; base += abreast * kMicro) {
-      const int i0 = t % side * kMicro, j0 = base + t / side * kMicro;
-      const bool mine = t / side < abreast && j0 < p.panel;
+    // This panel's X X^T, tiles on and below the diagonal and their mirror images; a
+    // tile takes every side-th row, so that the threads of a warp read neighbouring
+    // rows (whose pitch is odd: no bank conflicts).  One CTA's is S itself.
+    float *sums = ranks > 1 ? q : s;
+    for (int t0 = 0; t0 < s_tiles;) {
+      const int log = sharing(s_tiles - t0), kq = tid & ((1 << log) - 1), t = t0 + (tid >> log);
+      int ti = first_i, tj = first_j;
+      if (t0) below(t, ti, tj);
       float acc[kMicro][kMicro] = {};
-      if (mine) tile_along(q + i0, p.s_ld, x + j0, p.x_ld, kq, share, rm, acc);
-      add_shared(acc, share);
-      __syncthreads();
-      if (mine && kq == 0)
+      if (t < s_tiles) {
+        const float *xi = x + ti * p.x_ld, *xj = x + tj * p.x_ld;
+        for (int k = kq * 4; k < p.panel; k += 4 << log) {
+          float4 u[kMicro], w[kMicro];
+#pragma unroll
+          for (int i = 0; i < kMicro; ++i) {
+            u[i] = *reinterpret_cast<const float4 *>(xi + i * side * p.x_ld + k);
+            w[i] = *reinterpret_cast<const float4 *>(xj + i * side * p.x_ld + k);
+          }
+#pragma unroll
+          for (int i = 0; i < kMicro; ++i)
+#pragma unroll
+            for (int j = 0; j < kMicro; ++j)
+              acc[i][j] = fmaf(u[i].w, w[j].w, fmaf(u[i].z, w[j].z, fmaf(u[i].y, w[j].y, fmaf(u[i].x, w[j].x, acc[i][j]))));
+        }
+      }
+      add_shared(acc, log);
+      if (t < s_tiles && kq == 0)
 #pragma unroll
         for (int i = 0; i < kMicro; ++i)
 #pragma unroll
-          for (int j = 0; j < kMicro; j += 4) {
-            float4 *at = reinterpret_cast<float4 *>(x + (i0 + i) * p.x_ld + j0 + j);
-            const float4 o = *at;
-            *at = make_float4(fmaf(a, o.x, acc[i][j]), fmaf(a, o.y, acc[i][j + 1]), fmaf(a, o.z, acc[i][j + 2]),
-                              fmaf(a, o.w, acc[i][j + 3]));
+          for (int j = 0; j < kMicro; ++j) {
+            sums[(ti + i * side) * p.s_ld + tj + j * side] = acc[i][j];
+            sums[(tj + j * side) * p.s_ld + ti + i * side] = acc[i][j];
           }
+      t0 += kSmallThreads >> log;
+    }
+    together();
+    if (ranks > 1) {
+      // S, rows [first, last) of it here, for everyone
+      for (int v = tid; v < (last - first) * side; v += kSmallThreads) {
+        const int row = by_side(v), at = (first + row) * p.s_ld + (v - row * side) * 4;
+        const uint32_t from_q = smem_u32(q + at), to_s = smem_u32(s + at);
+        float4 o[8], f = make_float4(0.f, 0.f, 0.f, 0.f);   // all on their way before the first is used
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+          if (r < ranks) o[r] = peer_load(map_to_cta(from_q, (uint32_t)r));
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+          if (r < ranks) f.x += o[r].x, f.y += o[r].y, f.z += o[r].z, f.w += o[r].w;
+        for (int r = 0; r < ranks; ++r) peer_store(map_to_cta(to_s, (uint32_t)r), f);
+      }
+      cluster_sync();
+    }
+    // the same rows of P = b S + c S S
+    for (int t0 = 0; t0 < p_tiles; t0 += kSmallThreads >> p_log) {
+      const int kq = tid & ((1 << p_log) - 1), t = t0 + (tid >> p_log), row = by_side(t);
+      const int i0 = first + row * kMicro, j0 = (t - row * side) * kMicro;
+      float acc[kMicro][kMicro] = {};
+      if (t < p_tiles) tile_along(s + i0, p.s_ld, s + j0, p.s_ld, kq, 1 << p_log, rm, acc);
+      add_shared(acc, p_log);
+      if (t < p_tiles && kq == 0)
+#pragma unroll
+        for (int i = 0; i < kMicro; ++i) {
+          const int at = (i0 + i) * p.s_ld + j0;
+          const float4 o = *reinterpret_cast<const float4 *>(s + at);
+          const float4 f = make_float4(b * o.x + c * acc[i][0], b * o.y + c * acc[i][1], b * o.z + c * acc[i][2],
+                                       b * o.w + c * acc[i][3]);
+          if (ranks == 1) {
+            *reinterpret_cast<float4 *>(q + at) = f;
+          } else {
+            const uint32_t to = smem_u32(q + at);
+            for (int r = 0; r < ranks; ++r) peer_store(map_to_cta(to, (uint32_t)r), f);
+          }
+        }
+    }
+    together();
+    // X <- a X + P X, the columns of a round from registers once all have read them
+    const int kq = tid & ((1 << x_log) - 1);
+    for (int base = 0; base < p.panel; base += abreast * kMicro) {
+      const int i0 = x_row * kMicro, j0 = base + x_column * kMicro;
+      const bool mine = x_column < abreast && j0 < p.panel;
+      float acc[kMicro][kMicro] = {};
+      if (mine) tile_along(q + i0, p.s_ld, x + j0, p.x_ld, kq, 1 << x_log, rm, acc);
+      add_shared(acc, x_log);
+      __syncthreads();
+      if (mine && kq == 0)
+#pragma unroll
+        for (int i = 0; i < kMicro; ++i) {
+          float4 *at = reinterpret_cast<float4 *>(x + (i0 + i) * p.x_ld + j0);
+          const float4 o = *at;
+          *at = make_float4(fmaf(a, o.x, acc[i][0]), fmaf(a, o.y, acc[i][1]), fmaf(a, o.z, acc[i][2]),
+                            fmaf(a, o.w, acc[i][3]));
+        }
     }
     __syncthreads();
   }
@@ -853,11 +877,12 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const SmallPara
 
 // CTAs of a small matrix's cluster, 0 where the tiles of the general path are
 // expected to be faster.  Cycles of a step: the FMAs of a CTA at 46 a cycle
-// (shared memory feeds no more of these 4 x 4 tiles), 4000 for barriers and
-// sums, and the exchange of S and P, which slows down once many clusters do
-// it; the general path takes about 40,000 whatever its size here.  Measured, us a
-// call of 5 steps: 64 x 512 with 1, 2, 4, 8 CTAs 254, 144, 86, 60; 16 matrices
-// of 128 x 128 332, 183, 115, 179; the general path 105.
+// (shared memory feeds no more of these 4 x 4 tiles); 3500 for barriers and
+// sums; with a cluster 2500 more and the exchange of S and P, which both slow down
+// once many clusters are there.  The general path takes about 40,000 whatever its size
+// here.  Measured, cycles a step with 1, 2, 4, 8 CTAs: 16 x 16 3769, 5683, 6367, 6584;
+// 64 x 250 41637, 25490, 16577, 13215, and 37 of them 41659, 25608, 25799, 38276;
+// 128 x 128 92266, 54462, 34929, 28684.
 struct SmallShape { int ranks, panel, x_ld, s_ld, bytes; };
 SmallShape small_shape(int64_t batch, int64_t rows, int64_t cols, int steps) {
   SmallShape best{};
@@ -868,11 +893,11 @@ SmallShape small_shape(int64_t batch, int64_t rows, int64_t cols, int steps) {
     auto odd = [](int64_t n) { return n / 4 % 2 ? n : n + 4; };
     const int64_t x_ld = odd(panel), s_ld = odd(rm), bytes = 4 * rm * (x_ld + 2 * s_ld);
     if (bytes > 220 * 1024) continue;
-    const double fmas = (double)rm * rm * (2 * panel) + (double)rm * rm * rm / ranks;
+    const double fmas = (double)rm * rm * (1.5 * panel) + (double)rm * rm * rm / ranks;
     const int64_t waves = (batch * ranks + sm_count() - 1) / sm_count();
     const double crowd = std::max(1.0, (double)(batch * ranks) * (batch * ranks) / (80.0 * 80.0));
-    const double exchange = ranks > 1 ? 0.7 * rm * rm * std::min(crowd, 3.0) : 0;
-    const double t = (double)waves * (fmas / 46 + 4000 + exchange);
+    const double exchange = ranks > 1 ? (2500 + 0.6 * rm * rm) * std::min(crowd, 3.0) : 0;
+    const double t = (double)waves * (fmas / 46 + 3500 + exchange);
     if (t < least) {
       least = t;
       best = SmallShape{ranks, (int)panel, (int)x_ld, (int)s_ld, (int)bytes};
