@@ -1224,8 +1224,11 @@ extern "C" int oz_orthogonalize(const void *g, int dtype, int64_t batch, int64_t
   // Two slices: sums cut off every block where the launches and not the products take
   // the time, every 4 blocks where it would cost (4096 x 4096: 4682 us and 6.4e-7 off
   // against 3531 us and 1.3e-6; fp32 sums 3.7e-6.  200 x 800: 3.7e-6 with 4, 1.0e-6
-  // with 1, fp32 sums 1.5e-6)
+  // with 1, fp32 sums 1.5e-6), and every 2 for fewer rows, whose singular values start
+  // nearer to 1, so that more steps feel S and P (6 x 1024 x 1536: 782 us and 5.1e-6
+  // with 4, 800 us and 2.8e-6 with 2, fp32 sums 3.2e-6)
   const double work = (double)batch * l.rows * l.rows * (3.0 * l.cols + l.rows);
-  return work < 2e10 ? run<2, 1>(init, l, (int)batch, steps, coefficients, ws, last, st)
-                     : run<2, 4>(init, l, (int)batch, steps, coefficients, ws, last, st);
+  return work < 2e10     ? run<2, 1>(init, l, (int)batch, steps, coefficients, ws, last, st)
+         : l.rows < 1536 ? run<2, 2>(init, l, (int)batch, steps, coefficients, ws, last, st)
+                         : run<2, 4>(init, l, (int)batch, steps, coefficients, ws, last, st);
 }
