@@ -63,7 +63,7 @@ def gradient(seed, *shape, kind="normal"):
 
 SHAPES = [(1, 1), (1, 40), (33, 1), (3, 5, 7), (16, 64), (2, 64, 16), (130, 257), (2, 3, 129, 100), (256, 256),
           (511, 300), (300, 1000), (5, 128, 384), (1030, 520), (640, 1288), (1900, 2100),
-          (2, 70, 2600), (4200, 130), (1, 33, 9000), (3, 300, 2050)]
+          (2, 70, 2600), (4200, 130), (1, 33, 9000), (3, 300, 2050), (1400, 3500)]
 
 
 @pytest.mark.parametrize("kind", ["normal", "low rank"])
