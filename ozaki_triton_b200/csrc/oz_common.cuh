@@ -263,6 +263,14 @@ __device__ __forceinline__ void st_async_f32(uint32_t addr, float v, uint32_t ba
                "r"(__float_as_uint(v)), "r"(bar)
                : "memory");
 }
+// The two halves of a barrier over the cluster that hands over no memory: what lies
+// between them hides its latency.
+__device__ __forceinline__ void cluster_arrive_relaxed() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
                    : "memory");

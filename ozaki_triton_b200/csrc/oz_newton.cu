@@ -706,6 +706,9 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const SmallPara
   const int ranks = (int)cluster_nctarank(), rank = (int)cluster_ctarank();
   const int tid = threadIdx.x;
   const int member = blockIdx.x / ranks;
+  // another CTA's shared memory may be used once that CTA is known to have started:
+  // waited for below, before the first remote store
+  if (ranks > 1) cluster_arrive_relaxed();
   auto together = [&]() {
     if (ranks > 1) cluster_sync();
     else __syncthreads();
@@ -732,6 +735,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const SmallPara
       }
   }
   sum = block_sum(sum, part);
+  if (ranks > 1) cluster_wait();
   if (tid < ranks) {
     const uint32_t to = map_to_cta(smem_u32(&norms[rank]), (uint32_t)tid);
     asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(to), "d"(sum) : "memory");
