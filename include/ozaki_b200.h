@@ -323,7 +323,9 @@ int oz_matmul_w4(const oz_w4_args *args, void *stream);
  *   X <- a X + (b A + c A^2) X
  *
  *   g            : fp32, fp16 or bf16, element (z, i, j) at z*g_sb + i*g_sr + j*g_sc
- *   coefficients : host array of `steps` triples (a, b, c)
+ *   coefficients : host array of `steps` triples (a, b, c).  Where the products take
+ *                  fp16 slices, singular values starting in [0, 1] may grow to 8 at
+ *                  most before the last step (OZ_ERR_UNSUPPORTED otherwise)
  *   num_splits   : fp16 slices of a matrix in the products, 1 or 2
  *   out          : contiguous (batch, m, n) of g's type
  *                  (small matrices, up to 128 rows or columns, are worked on in

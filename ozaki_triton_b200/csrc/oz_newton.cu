@@ -9,9 +9,15 @@
 //
 // Every matrix is held as fp16 slices at a power-of-two scale of its own:
 // high = fp16(v 2^e), low = fp16(v 2^e - high).  The host bounds the norms
-// step by step (the singular values start in [0, 1] and a step's polynomial
-// is known), so e puts the bound at 2^15 and nothing can overflow; no data
-// is looked at.  With one slice the products use `high` alone (11 bits) and
+// step by step: the singular values start in [0, 1] and a step's polynomial
+// is known, so their largest value after it is too; no data is looked at.  It
+// is the bound of exact steps: rounded ones go a little beyond it, and a factor
+// for that must not enter the next step's bound, since polynomials chosen for
+// an interval may be steep just outside it (1/64 a step took the bound of one such
+// schedule from 2 to 10^15 in 5 steps, and the matrices to zero).  Instead e puts the bound
+// at 2^12, which leaves a factor of 16 below the largest fp16 and, two slices
+// having 22 bits down to 2^-3, one of 2^15 above the entries that keep them all.  Schedules
+// whose bound leaves [0, 8] before their last step are refused.  With one slice the products use `high` alone (11 bits) and
 // only the term a X keeps X's 22: that term carries the directions that the
 // products hardly touch, and rounding it as well as P X makes both sides of
 // the sum consistent only for full-rank G (measured on a low-rank gradient:
@@ -971,12 +977,13 @@ Layout layout(int64_t batch, int64_t m, int64_t n, int splits) {
   return l;
 }
 
-// The exponent that puts a bound on a matrix's entries at 2^15.
+// The exponent that puts a bound on a matrix's entries at 2^12.  Past 100 (a bound below
+// 2^-88) the entries sink below fp16's; the other end is not reached (bounded_steps).
 int exponent(double bound) {
-  if (!(bound > 0)) return 15;
+  if (!(bound > 0)) return 12;
   int e;
   frexp(bound, &e);                                    // bound <= 2^e
-  return std::min(std::max(15 - e, -40), 40);
+  return std::min(std::max(12 - e, -100), 100);
 }
 
 // Largest |a s + b s^3 + c s^5| for s in [0, most], and |b u + c u^2| for u = s^2.
@@ -999,6 +1006,25 @@ double largest_poly(double b, double c, double most) {
   double v = f(end);
   if (c != 0 && -b / (2 * c) > 0 && -b / (2 * c) < end) v = std::max(v, f(-b / (2 * c)));
   return v;
+}
+
+// Whether the slices can hold every matrix of the steps: S grows with the square of the
+// bound and P with its fourth power, while their entries may stay near 1, so X's bound
+// before a step may be 8 at most (P's entries then still lie 2^12 above the 2^-12 that
+// costs them bits), and P's 2^60.
+constexpr double kMostNorm = 8, kMostPoly = 0x1p60;
+constexpr double kFirstNorm = 1 + 1e-6;                // of X = G / (|G| + eps)
+int bounded_steps(int steps, const double *coefficients) {
+  double most = kFirstNorm;
+  for (int i = 0; i < steps; ++i) {
+    const double a = coefficients[3 * i], b = coefficients[3 * i + 1], c = coefficients[3 * i + 2];
+    if (!(most <= kMostNorm) || !(largest_poly(b, c, most) <= kMostPoly))
+      return set_error(OZ_ERR_UNSUPPORTED,
+                       "the coefficients let singular values grow to %g before step %d of %d; fp16 slices hold %g",
+                       most, i + 1, steps, kMostNorm);
+    most = largest_value(a, b, c, most);
+  }
+  return OZ_OK;
 }
 
 // Tile counts of a member, and the estimated time of all tiles: waves over the
@@ -1093,13 +1119,11 @@ int run(const InitParams &init, const Layout &l, int batch, int steps, const dou
   sym.idesc = instruction(OZ_F16);
   sym.batch = batch;
   sym.rows = sym.cols = rows;
-  double most = 1 + 1e-6;                              // largest singular value of X
+  double most = kFirstNorm;                            // largest singular value of X
   int ex = exponent(most), cur = 0;
   for (int i = 0; i < steps; ++i) {
     const double a = coefficients[3 * i], b = coefficients[3 * i + 1], c = coefficients[3 * i + 2];
-    // rounded operands give a little more than the exact bounds
-    const double slack = 1 + 1.0 / 64;
-    const int es = exponent(most * most * slack), ep = exponent(largest_poly(b, c, most) * slack);
+    const int es = exponent(most * most), ep = exponent(largest_poly(b, c, most));
     sym.k = cols;
     sym.alpha = 0;
     sym.beta = (float)std::ldexp(1.0, es - 2 * ex);
@@ -1123,7 +1147,7 @@ int run(const InitParams &init, const Layout &l, int batch, int steps, const dou
     rc = pair_s ? step_product<SymmetricJob<2, 256, SPLITS, SPLITS, PASS>>(sa, sb, sym, true, st)
                 : step_product<SymmetricJob<1, 64, SPLITS, SPLITS, PASS>>(sa, sb, sym, true, st);
     if (rc) return rc;
-    most = std::min(largest_value(a, b, c, most) * slack, 1e15);
+    most = largest_value(a, b, c, most);
     const bool end = i + 1 == steps;
     const int en = end ? 0 : exponent(most);
     StepParams up = last;
@@ -1201,6 +1225,7 @@ extern "C" int oz_orthogonalize(const void *g, int dtype, int64_t batch, int64_t
     for (int i = 0; i < 3 * steps; ++i) p.abc[i] = (float)coefficients[i];
     return run_small(small, p, batch, reinterpret_cast<cudaStream_t>(stream));
   }
+  if (int rc = bounded_steps(steps, coefficients)) return rc;
   const Layout l = layout(batch, m, n, num_splits);
   if (!workspace || workspace_bytes < l.total || (uintptr_t)workspace % 256 != 0)
     return set_error(OZ_ERR_INVALID,
@@ -1215,7 +1240,7 @@ extern "C" int oz_orthogonalize(const void *g, int dtype, int64_t batch, int64_t
   InitParams init{g, dtype, (int)std::min<int64_t>(blocks, kMostPartials), flat, vectors, (int)l.rows, (int)l.cols, g_sb,
                   tall ? g_sc : g_sr, tall ? g_sr : g_sc, reinterpret_cast<double *>(ws),
                   Planes{reinterpret_cast<__half *>(ws + l.x0), pitch(l.cols), l.x_mat, l.x_mat * batch}, eps,
-                  std::ldexp(1.0, exponent(1 + 1e-6))};
+                  std::ldexp(1.0, exponent(kFirstNorm))};
   StepParams last{};
   last.last = out;
   last.last_dtype = dtype;

@@ -70,8 +70,10 @@ def orthogonalize(g: torch.Tensor, steps: int = 5,
     ``num_splits`` is how many fp16 slices of each matrix the products use: 1
     (11 bits, the default for bf16, whose result has 8, where the products'
     time counts: batch M N min(M, N) above 2e9 or so) or 2 (22 bits, the default
-    elsewhere).  Sums are held in fp32.  Small matrices (up to 128 rows or
-    columns) are worked on in fp32 whatever it is.
+    elsewhere).  Their scales follow from the largest singular value that the
+    coefficients allow, so a schedule that lets one starting in [0, 1] grow past
+    8 before its last step is refused (OzakiError).  Sums are held in fp32.  Small matrices (up to 128 rows or
+    columns) are worked on in fp32 whatever it is, with any coefficients.
     """
     if not isinstance(coefficients, tuple) or hasattr(coefficients[0], "__len__"):
         coefficients = tuple(tuple(c) if hasattr(c, "__len__") else c for c in coefficients)
