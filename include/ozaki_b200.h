@@ -301,7 +301,7 @@ int oz_grouped_wgrad(const oz_grouped_wgrad_args *args, void *stream);
  *               half); byte strides p_se, p_sn, unit stride along k
  *   scales    : (experts, n, k / group) fp16, bf16 or fp32 (scale_dtype);
  *               element strides s_se, s_sn
- *   zeros     : uint8 with the scales' strides, or NULL: z = 8
+ *   zeros     : uint8 (0 to 255) with the scales' strides, or NULL: z = 8
  *   offsets   : row groups of the experts as in oz_grouped_matmul, or NULL
  *               for one expert with every row
  * group is a multiple of 32 that divides k.  x and packed start on 16-byte

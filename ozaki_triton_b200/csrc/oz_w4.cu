@@ -101,6 +101,11 @@ struct W4Walk {
 // 16-19 first), exactly: a field becomes the low mantissa bits of a constant
 // that is a power of two, and the same constant plus z is subtracted.  fp16
 // has room for a field in bits 4-7 too (64 + q beside 1024 + q), bf16 has not.
+// z is any byte.  fp16 holds 1024 + z and 64 + z exactly.  bf16 holds 128 + z up to z =
+// 127 only; from there on the field's bits are flipped in the mantissa of -255, which
+// makes q - 255, and z - 255 is subtracted (24 rows / 64 experts, 2816 x 2048: 32.1 us;
+// 30.4 if z stopped at 127; a product of its own for the upper bit of z, behind a test,
+// took 34 to 38).
 // A constant that stays in a register (as an immediate it is moved there again at
 // each use, and a mask and an or with two immediates become two instructions).
 __device__ __forceinline__ uint32_t kept(uint32_t c) {
@@ -108,17 +113,18 @@ __device__ __forceinline__ uint32_t kept(uint32_t c) {
   asm volatile("mov.b32 %0, %1;" : "=r"(v) : "r"(c));
   return v;
 }
-// (w & m) | c
+// (w & m) ^ c
 __device__ __forceinline__ uint32_t field(uint32_t w, uint32_t m, uint32_t c) {
   uint32_t v;
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(v) : "r"(w), "r"(m), "r"(c));
+  asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(v) : "r"(w), "r"(m), "r"(c));
   return v;
 }
 template <typename T> struct Unpack;
 template <> struct Unpack<__half> {
   uint32_t m0 = kept(0x000f000fu), c0 = kept(0x64006400u), m1 = kept(0x00f000f0u), c1 = kept(0x54005400u);
   static __device__ __forceinline__ uint32_t zero(uint32_t z) { return 0x64006400u | z * 0x10001u; }
-  __device__ __forceinline__ uint2 both(uint32_t z) const { return make_uint2(z, field(z << 4, m1, c1)); }
+  // 1024 + z and 64 + z
+  __device__ __forceinline__ uint2 both(uint32_t z) const { return make_uint2(z, less(z, 0x63806380u)); }
   static __device__ __forceinline__ uint32_t less(uint32_t v, uint32_t z) {
     const __half2 d = __hsub2(*reinterpret_cast<const __half2 *>(&v), *reinterpret_cast<const __half2 *>(&z));
     return *reinterpret_cast<const uint32_t *>(&d);
@@ -132,13 +138,21 @@ template <> struct Unpack<__half> {
   }
 };
 template <> struct Unpack<__nv_bfloat16> {
-  uint32_t m0 = kept(0x000f000fu), c0 = kept(0x43004300u);
-  static __device__ __forceinline__ uint32_t zero(uint32_t z) { return 0x43004300u | z * 0x10001u; }
-  __device__ __forceinline__ uint2 both(uint32_t z) const { return make_uint2(z, 0); }
+  uint32_t m0 = kept(0x000f000fu);
+  // 128 + z, or z - 255 with its sign (-0 too)
+  static __device__ __forceinline__ uint32_t zero(uint32_t z) {
+    return (z < 128 ? 0x4300u | z : 0x8000u | __float_as_uint((float)(255 - z)) >> 16) * 0x10001u;
+  }
+  // and what the fields are put into: 128, or -255 where the sign is there
+  __device__ __forceinline__ uint2 both(uint32_t z) const {
+    uint32_t sign;                                        // of the upper half, in every bit
+    asm("prmt.b32 %0, %1, %1, 0xbbbb;" : "=r"(sign) : "r"(z));
+    return make_uint2(z, 0x43004300u ^ (sign & 0x807f807fu));
+  }
   __device__ __forceinline__ void values(uint32_t w, uint2 z, uint32_t (&v)[4]) const {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t u = field(w >> (4 * i), m0, c0);
+      const uint32_t u = field(w >> (4 * i), m0, z.y);
       const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&u),
                                        *reinterpret_cast<const __nv_bfloat162 *>(&z.x));
       v[i] = *reinterpret_cast<const uint32_t *>(&d);
@@ -226,19 +240,16 @@ __global__ void __launch_bounds__(kWarps * 32, (W4Shape<RT, NB, PER>::kCtas))
   bool a_more = ahead.find(p, 8 * NB, a_tile, a_e, a_row, a_rows, a_column);
   uint32_t issued = 0;
   uint32_t scale_bits[kMine], zero_bits[kMine];
-  // the tile's scales of this lane's entries (null: no such row), and what a
-  // chunk's group index has to be multiplied by
-  const char *scale_at[kMine];
-  const uint8_t *zero_at[kMine];
+  // where the scales and zeros of this lane's entries start (kNowhere: no such row)
+  constexpr int64_t kNowhere = INT64_MIN;
+  int64_t entry_at[kMine];
   const int scale_bytes = p.scale_dtype == OZ_F32 ? 4 : 2;
   auto enter = [&]() {                                    // the tile that is copied next
 #pragma unroll
     for (int i = 0; i < kMine; ++i) {
       const int r = (i * 32 + lane) % Shape::kRows, n = a_column * Shape::kRows + r;
-      const int64_t at = a_e * p.s_se + n * p.s_sn;
       const bool in = n < p.n && (Shape::kEntries >= 32 || lane < Shape::kEntries);
-      scale_at[i] = in ? static_cast<const char *>(p.scales) + at * scale_bytes : nullptr;
-      zero_at[i] = in && p.zeros ? p.zeros + at : nullptr;
+      entry_at[i] = in ? a_e * p.s_se + n * p.s_sn : kNowhere;
     }
   };
   if (a_more) enter();
@@ -276,11 +287,11 @@ __global__ void __launch_bounds__(kWarps * 32, (W4Shape<RT, NB, PER>::kCtas))
       for (int i = 0; i < kMine; ++i) {
         const uint32_t k32 = (uint32_t)(a_chunk * (kChunk / 32) + (i * 32 + lane) / Shape::kRows * (4 / PER));
         const uint32_t group = p.group == kChunk ? k32 / 4 : p.group == 32 ? k32 : __umulhi(k32, p.per_group);
-        if (scale_at[i] && (int)group < p.groups) {
-          const char *at = scale_at[i] + group * scale_bytes;
-          scale_bits[i] = scale_bytes == 4 ? __ldg(reinterpret_cast<const uint32_t *>(at))
-                                           : __ldg(reinterpret_cast<const unsigned short *>(at));
-          if (zero_at[i]) zero_bits[i] = __ldg(zero_at[i] + group);
+        if (entry_at[i] != kNowhere && (int)group < p.groups) {
+          const int64_t at = entry_at[i] + group;
+          scale_bits[i] = scale_bytes == 4 ? __ldg(static_cast<const uint32_t *>(p.scales) + at)
+                                           : __ldg(static_cast<const unsigned short *>(p.scales) + at);
+          if (p.zeros) zero_bits[i] = __ldg(p.zeros + at);
         } else {
           scale_bits[i] = 0;                              // nothing there: adds nothing
         }

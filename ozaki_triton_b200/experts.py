@@ -377,7 +377,7 @@ def matmul_w4(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor,
 
     x (T, K) bf16 or fp16; packed (N, K / 2) uint8, two values a byte, the even
     k in the low half; scales (N, K / g) fp16, bf16 or fp32; zeros (N, K / g)
-    uint8, or None for 8 everywhere (the layout ``quantize_w4`` returns).
+    uint8 (any value), or None for 8 everywhere (the layout ``quantize_w4`` returns).
     With ``offsets`` the weights have a leading expert dimension and the rows
     of x come in groups.  Returns (T, N) in x's dtype or fp32.  Made for few
     rows a matrix (the weights' bytes bound it); any number is right.  Layouts
