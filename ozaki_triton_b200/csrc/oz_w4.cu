@@ -313,8 +313,10 @@ __global__ void __launch_bounds__(kWarps * 32, (W4Shape<RT, NB, PER>::kCtas))
   const Unpack<T> unpack;
   W4Walk walk;
   uint32_t used = 0;
+  // Once a wait has given up a warp multiplies nothing more but goes through all its
+  // tiles: the other warps of its team wait for it at each tile's barriers.
   bool ok = true;
-  for (int tile = unit; ok; tile += units) {
+  for (int tile = unit;; tile += units) {
     int e, row, rows, column;
     if (!walk.find(p, 8 * NB, tile, e, row, rows, column)) break;
     const int n0 = column * Shape::kRows;
@@ -325,13 +327,11 @@ __global__ void __launch_bounds__(kWarps * 32, (W4Shape<RT, NB, PER>::kCtas))
       for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int c = 0; c < 4; ++c) acc[r][b][c] = 0.f;
-    for (int chunk = member; chunk < chunks; chunk += p.along) {
+    for (int chunk = member; ok && chunk < chunks; chunk += p.along) {
       const unsigned char *st = ring + (used & 1) * Shape::kStage;
       ok = mbar_wait_bounded(&full[used & 1], used >> 1 & 1, abort_flag, DEV_TIMEOUT_PRODUCER);
-      if (!__all_sync(0xffffffffu, ok)) {
-        ok = false;
-        break;
-      }
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
       float part[RT][NB][4];
       uint2 zero[RT][2];
       float scale[RT][2];
@@ -411,7 +411,6 @@ __global__ void __launch_bounds__(kWarps * 32, (W4Shape<RT, NB, PER>::kCtas))
       }
       asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(p.along * 32) : "memory");
     }
-    ok = !*abort_flag;
   }
   // copies still in flight after a wait gave up
   if (lane == 0)
