@@ -223,6 +223,18 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t *bar, uint32_t parity
   }
 }
 
+// The wait before shared or tensor memory goes away, for copies and products still under
+// way: where another role has aborted, *abort no longer ends it, but a limit of its own
+// (0.5 s) does.
+constexpr long long kSettleBoundCycles = kWaitBoundCycles / 4;
+__device__ __forceinline__ bool mbar_settle(uint64_t *bar, uint32_t parity, volatile int *abort, int code) {
+  if (mbar_wait_bounded(bar, parity, abort, code)) return true;
+  const long long t0 = clock64();
+  while (clock64() - t0 < kSettleBoundCycles)
+    if (mbar_try_wait(smem_u32(bar), parity)) return true;
+  return false;
+}
+
 // 3-D tiled TMA load global -> shared, completion counted on `bar`.
 __device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, uint64_t *bar,
                                             int c0, int c1, int c2) {

@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       // before shared memory is released
       if (leader)
         for (uint32_t k = (it > (uint32_t)S ? it - S : 0); k < it; ++k)
-          mbar_wait_bounded(&full[k % S], (k / S) & 1, abort_flag, DEV_TIMEOUT_PRODUCER);
+          if (!mbar_settle(&full[k % S], (k / S) & 1, abort_flag, DEV_TIMEOUT_PRODUCER)) break;
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
@@ -374,7 +374,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       // wait for all issued MMAs before TMEM / shared memory go away
       if constexpr (PAIR == 2) tc_commit_pair(smem_u32(drain));
       else tc_commit(drain);
-      mbar_wait_bounded(drain, 0, abort_flag, DEV_TIMEOUT_MMA);
+      mbar_settle(drain, 0, abort_flag, DEV_TIMEOUT_MMA);
     }
   } else {
     // ------------------------------------------------------------ epilogue

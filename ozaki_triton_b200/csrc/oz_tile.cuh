@@ -352,14 +352,15 @@ __global__ void __launch_bounds__(threads<J>(), 1)
       ok = __shfl_sync(0xffffffffu, (int)ok, 0);
     }
     // every load must have landed before shared memory goes away (a block that ends a
-    // range counts on `full` only through the clearing warp)
+    // range counts on `full` only through the clearing warp); past the first that does not
+    // within its limit, nothing can still be under way
     if (lane == 0)
       for (int slot = 0; J::RAGGED && slot < S; ++slot)
-        if ((ended >> slot) & 1)
-          mbar_wait_bounded(&tail[slot], (turn >> slot) & 1, abort_flag, DEV_TIMEOUT_PRODUCER);
+        if (((ended >> slot) & 1) && !mbar_settle(&tail[slot], (turn >> slot) & 1, abort_flag, DEV_TIMEOUT_PRODUCER))
+          break;
     if (lane == 0 && leader)
       for (uint32_t k = (it > (uint32_t)S ? it - S : 0); k < it; ++k)
-        mbar_wait_bounded(&full[k % S], (k / S) & 1, abort_flag, DEV_TIMEOUT_PRODUCER);
+        if (!mbar_settle(&full[k % S], (k / S) & 1, abort_flag, DEV_TIMEOUT_PRODUCER)) break;
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
     typename J::Walk walk(p);
@@ -453,7 +454,7 @@ __global__ void __launch_bounds__(threads<J>(), 1)
     if (lane == 0 && leader) {
       if constexpr (PAIR == 2) tc_commit_pair(smem_u32(drain));
       else tc_commit(drain);
-      mbar_wait_bounded(drain, 0, abort_flag, DEV_TIMEOUT_MMA);
+      mbar_settle(drain, 0, abort_flag, DEV_TIMEOUT_MMA);
     }
   } else if (J::RAGGED && warp == 2 + kEpilogueWarps) {
     // ------------------------------------------------------------ clearing

@@ -415,7 +415,7 @@ __global__ void __launch_bounds__(kWarps * 32, (W4Shape<RT, NB, PER>::kCtas))
   // copies still in flight after a wait gave up
   if (lane == 0)
     for (; used < issued; ++used)
-      mbar_wait_bounded(&full[used & 1], used >> 1 & 1, abort_flag, DEV_TIMEOUT_PRODUCER);
+      mbar_settle(&full[used & 1], used >> 1 & 1, abort_flag, DEV_TIMEOUT_PRODUCER);
 
   if (p.offsets) {                                        // rows that no group holds are zero
     int first, last, a, b;
