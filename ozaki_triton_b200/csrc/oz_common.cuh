@@ -4,6 +4,7 @@
 #pragma once
 
 #include <cuda.h>
+#include <cudaTypedefs.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -48,6 +49,36 @@ inline int set_smem_once(const void *kern, int smem, const char *what) {
     if (v < smem) v = smem;
   }
   return rc;
+}
+
+// cuTensorMapEncodeTiled for a 3-D map without interleave, element strides of 1 and zeros
+// outside.  The driver refuses it on a thread without a context, and a thread that has made
+// no runtime call that needs one has none (a worker of the autograd engine whose first
+// operator this is, any new thread): it is bound to the runtime's current device then.
+inline int encode_tiled(CUtensorMap *map, CUtensorMapDataType type, const void *base, const cuuint64_t (&dims)[3],
+                        const cuuint64_t (&strides)[2], const cuuint32_t (&box)[3], CUtensorMapSwizzle swizzle,
+                        CUtensorMapL2promotion promotion) {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  if (!fn) {
+    void *ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &ptr, 12000, cudaEnableDefault,
+                                         &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      return set_error(OZ_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+    fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+  }
+  const cuuint32_t steps[3] = {1, 1, 1};
+  auto encode = [&]() {
+    return fn(map, type, 3, const_cast<void *>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              swizzle, promotion, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  int dev = 0;
+  if (r == CUDA_ERROR_INVALID_CONTEXT && cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess)
+    r = encode();
+  if (r != CUDA_SUCCESS) return set_error(OZ_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return OZ_OK;
 }
 
 // Device-side status word of this translation unit: kernels write a nonzero

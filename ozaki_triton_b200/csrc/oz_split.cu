@@ -44,7 +44,6 @@
 #include <cstring>
 #include <mutex>
 #include <type_traits>
-#include <cudaTypedefs.h>
 
 #include "oz_common.cuh"
 #include "oz_log2_table.h"
@@ -1535,19 +1534,6 @@ int launch_rows(const TIn *in, int64_t sb, int64_t sl, int64_t batch, int lines,
   return OZ_OK;
 }
 
-PFN_cuTensorMapEncodeTiled_v12000 split_encode_fn() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  if (!fn) {
-    void *ptr = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &ptr, 12000,
-                                         cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
-  }
-  return fn;
-}
-
 template <typename TIn, int SK, bool EXACT, int V>
 int launch_cols_v(const TIn *in, int64_t sb, int64_t sk, int64_t batch, int lines, int K, int ld,
                   int s, int alpha, void *slices, float *scales, cudaStream_t st, bool *done) {
@@ -1562,8 +1548,6 @@ int launch_cols_v(const TIn *in, int64_t sb, int64_t sk, int64_t batch, int line
   const int NS = min(4, (kColSmem - fixed) / STAGE);
   if (NS < 1) return OZ_OK;
   *done = true;
-  auto enc = split_encode_fn();
-  if (!enc) return set_error(OZ_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
   CUtensorMap map;
   const CUtensorMapDataType dt = sizeof(TIn) == 8 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT64
                                  : sizeof(TIn) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
@@ -1572,12 +1556,9 @@ int launch_cols_v(const TIn *in, int64_t sb, int64_t sk, int64_t batch, int line
   cuuint64_t strides[2] = {(cuuint64_t)(sk * (int64_t)sizeof(TIn)),
                            (cuuint64_t)(sb * (int64_t)sizeof(TIn))};
   cuuint32_t box[3] = {(cuuint32_t)W, (cuuint32_t)(KC < 256 ? KC : 256), 1};
-  cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = enc(&map, dt, 3, const_cast<TIn *>(in), dims, strides, box, estr,
-                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
-                   CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS)
-    return set_error(OZ_ERR_CUDA, "cuTensorMapEncodeTiled (split) failed (%d)", (int)r);
+  if (int rc = encode_tiled(&map, dt, in, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_128B))
+    return rc;
   const int smem = NS * STAGE + fixed;
   auto kern = split_cols_tma<TIn, SK, V, EXACT>;
   if (int rc = set_smem_once((const void *)kern, smem, "cudaFuncSetAttribute(split_cols)"))
@@ -1619,18 +1600,13 @@ int launch_colpairs(const double *in, int64_t sb, int64_t sk, int64_t batch, int
   const int nch = nch0 <= 1 ? 1 : nch0 <= 2 ? 2 : 4;
   const int NS = std::min(kPairMaxStages, (kPairSmem - 1024) / kPairStage);
   if (NS < nch) return OZ_OK;                    // a panel's chunks must fit the ring
-  auto enc = split_encode_fn();
-  if (!enc) return set_error(OZ_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
   CUtensorMap map;
   cuuint64_t dims[3] = {(cuuint64_t)lines, (cuuint64_t)K, (cuuint64_t)batch};
   cuuint64_t strides[2] = {(cuuint64_t)(sk * 8), (cuuint64_t)(sb * 8)};
   cuuint32_t box[3] = {2, 256, 1};
-  cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = enc(&map, CU_TENSOR_MAP_DATA_TYPE_FLOAT64, 3, const_cast<double *>(in), dims,
-                   strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
-                   CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS)
-    return set_error(OZ_ERR_CUDA, "cuTensorMapEncodeTiled (column pairs) failed (%d)", (int)r);
+  if (int rc = encode_tiled(&map, CU_TENSOR_MAP_DATA_TYPE_FLOAT64, in, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_128B))
+    return rc;
   const int ppb = (lines + 1) / 2;
   const int64_t panels = (int64_t)ppb * batch;
   const int smem = NS * kPairStage + kPairMaxStages * 8 + 2 * 16 * 4;
@@ -1683,19 +1659,13 @@ int launch_colpairs_kx(const double *in, int64_t sb, int64_t sk, int64_t batch, 
     resident = nb;
   }
   if (resident < kPairKPerSM) return OZ_OK;
-  auto enc = split_encode_fn();
-  if (!enc) return set_error(OZ_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
   CUtensorMap map;
   cuuint64_t dims[3] = {(cuuint64_t)lines, (cuuint64_t)K, (cuuint64_t)batch};
   cuuint64_t strides[2] = {(cuuint64_t)(sk * 8), (cuuint64_t)(sb * 8)};
   cuuint32_t box[3] = {2, 256, 1};
-  cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = enc(&map, CU_TENSOR_MAP_DATA_TYPE_FLOAT64, 3, const_cast<double *>(in), dims,
-                   strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
-                   CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS)
-    return set_error(OZ_ERR_CUDA, "cuTensorMapEncodeTiled (column pairs, K split) failed (%d)",
-                     (int)r);
+  if (int rc = encode_tiled(&map, CU_TENSOR_MAP_DATA_TYPE_FLOAT64, in, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_128B))
+    return rc;
   const int ppb = (lines + 1) / 2;
   const int64_t panels = (int64_t)ppb * batch;
   const int clusters =

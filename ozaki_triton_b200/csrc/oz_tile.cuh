@@ -41,8 +41,6 @@
 // Every wait is bounded (oz_common.cuh).
 #pragma once
 
-#include <cudaTypedefs.h>
-
 #include "oz_common.cuh"
 
 namespace oz {
@@ -92,25 +90,10 @@ template <class Extra> struct TileOf {
 inline int encode(CUtensorMap *map, CUtensorMapDataType type, const void *base, int64_t inner, int64_t rows,
                   int64_t mats, int64_t row_bytes, int64_t mat_bytes, int box_inner, int box_rows, int box_mats,
                   CUtensorMapSwizzle swizzle) {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  if (!fn) {
-    void *ptr = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &ptr, 12000, cudaEnableDefault,
-                                         &q) != cudaSuccess ||
-        q != cudaDriverEntryPointSuccess)
-      return set_error(OZ_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
-    fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
-  }
-  cuuint64_t dims[3] = {(cuuint64_t)inner, (cuuint64_t)rows, (cuuint64_t)mats};
-  cuuint64_t strides[2] = {(cuuint64_t)row_bytes, (cuuint64_t)mat_bytes};
-  cuuint32_t box[3] = {(cuuint32_t)box_inner, (cuuint32_t)box_rows, (cuuint32_t)box_mats};
-  cuuint32_t steps[3] = {1, 1, 1};
-  const CUresult r = fn(map, type, 3, const_cast<void *>(base), dims, strides, box, steps,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return set_error(OZ_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
-  return OZ_OK;
+  const cuuint64_t dims[3] = {(cuuint64_t)inner, (cuuint64_t)rows, (cuuint64_t)mats};
+  const cuuint64_t strides[2] = {(cuuint64_t)row_bytes, (cuuint64_t)mat_bytes};
+  const cuuint32_t box[3] = {(cuuint32_t)box_inner, (cuuint32_t)box_rows, (cuuint32_t)box_mats};
+  return encode_tiled(map, type, base, dims, strides, box, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
 }
 
 // A 16-bit operand of the engine: boxes of 64 elements x box_rows, swizzled.
