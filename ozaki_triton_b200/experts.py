@@ -258,11 +258,35 @@ class _GroupedMatmul(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         x, w, offsets = ctx.saved_tensors
+        # by functions that record gradients themselves: a graph of the gradient is whole
         dy = dy.to(x.dtype)
         need_x, need_w = ctx.needs_input_grad[:2]
-        dx = _product(dy, w.transpose(1, 2), offsets, None) if need_x else None
-        dw = _weight_gradient(x, dy, offsets, w.shape[0], None) if need_w else None
+        dx = grouped_matmul(dy, w.transpose(1, 2), offsets) if need_x else None
+        dw = _differentiable_weight_gradient(x, dy, offsets, w.shape[0]) if need_w else None
         return dx, dw, None, None
+
+
+class _WeightGradient(torch.autograd.Function):
+    """dw[e] = sum_r x[r]^T dy[r], bilinear like the product: its gradients are products."""
+
+    @staticmethod
+    def forward(ctx, x, dy, offsets, groups):
+        ctx.save_for_backward(x, dy, offsets)
+        return _weight_gradient(x, dy, offsets, groups, None)
+
+    @staticmethod
+    def backward(ctx, v):
+        x, dy, offsets = ctx.saved_tensors
+        v = v.to(x.dtype)
+        need_x, need_dy = ctx.needs_input_grad[:2]
+        return (grouped_matmul(dy, v.transpose(1, 2), offsets) if need_x else None,
+                grouped_matmul(x, v, offsets) if need_dy else None, None, None)
+
+
+def _differentiable_weight_gradient(x, dy, offsets, groups):
+    if (x.requires_grad or dy.requires_grad) and torch.is_grad_enabled():
+        return _WeightGradient.apply(x, dy, offsets, groups)
+    return _weight_gradient(x, dy, offsets, groups, None)
 
 
 def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, *,
@@ -274,8 +298,8 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, *,
     boundaries, are copied first);
     offsets (E + 1,) int32 or int64.  Returns (T, N) in the operands' dtype, or
     fp32 with ``out_dtype=torch.float32``.  Sums are held in fp32 and rounded
-    once.  Differentiable in x and w: the gradient is rounded to the operands'
-    dtype before it is multiplied.
+    once.  Differentiable in x and w, to any order: a gradient is rounded to the
+    operands' dtype before it is multiplied.
     """
     if (x.requires_grad or w.requires_grad) and torch.is_grad_enabled():
         return _GroupedMatmul.apply(x, w, offsets, out_dtype)
@@ -289,7 +313,8 @@ def grouped_matmul_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor,
 
     Returns (dx, dw): dx (T, K) in the operands' dtype, dw (E, K, N) in it or,
     with ``dw_dtype=torch.float32``, in fp32.  The gradient of an expert without
-    rows is zero.
+    rows is zero.  No gradient of the gradients is recorded here; autograd of
+    ``grouped_matmul`` records it.
     """
     assert dy.dim() == 2 and x.dim() == 2 and w.dim() == 3, "x and dy must have 2 dimensions, w 3"
     assert dy.dtype is x.dtype, f"x/dy dtype mismatch: {x.dtype} vs {dy.dtype}"
