@@ -23,6 +23,7 @@ import threading
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .api import _OZ_DTYPE, _RAW_STREAM, _check_cuda
@@ -42,6 +43,15 @@ def _check_places(x: torch.Tensor, *ts: Optional[torch.Tensor]) -> int:
         if t is not None and (not t.is_cuda or t.get_device() != index):
             raise ValueError(f"tensors on different devices: {x.device} and {t.device}")
     return index
+
+
+def _check_tangents(*ts: Optional[torch.Tensor]) -> None:
+    """Refuses tensors that carry a forward-mode derivative: it would be lost, since the
+    library reads their values only."""
+    if getattr(forward_ad, "_current_level", 0) >= 0:      # inside a dual level
+        for t in ts:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError("no forward-mode derivative of this operator: an argument has a tangent")
 
 
 class _OnDevice:
@@ -284,6 +294,7 @@ class _WeightGradient(torch.autograd.Function):
 
 
 def _differentiable_weight_gradient(x, dy, offsets, groups):
+    _check_tangents(x, dy)
     if (x.requires_grad or dy.requires_grad) and torch.is_grad_enabled():
         return _WeightGradient.apply(x, dy, offsets, groups)
     return _weight_gradient(x, dy, offsets, groups, None)
@@ -299,8 +310,9 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, *,
     offsets (E + 1,) int32 or int64.  Returns (T, N) in the operands' dtype, or
     fp32 with ``out_dtype=torch.float32``.  Sums are held in fp32 and rounded
     once.  Differentiable in x and w, to any order: a gradient is rounded to the
-    operands' dtype before it is multiplied.
+    operands' dtype before it is multiplied.  Forward-mode derivatives are refused.
     """
+    _check_tangents(x, w)
     if (x.requires_grad or w.requires_grad) and torch.is_grad_enabled():
         return _GroupedMatmul.apply(x, w, offsets, out_dtype)
     return _product(x, w, offsets, out_dtype)
@@ -314,8 +326,9 @@ def grouped_matmul_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor,
     Returns (dx, dw): dx (T, K) in the operands' dtype, dw (E, K, N) in it or,
     with ``dw_dtype=torch.float32``, in fp32.  The gradient of an expert without
     rows is zero.  No gradient of the gradients is recorded here; autograd of
-    ``grouped_matmul`` records it.
+    ``grouped_matmul`` records it.  Forward-mode derivatives are refused.
     """
+    _check_tangents(dy, x, w)
     assert dy.dim() == 2 and x.dim() == 2 and w.dim() == 3, "x and dy must have 2 dimensions, w 3"
     assert dy.dtype is x.dtype, f"x/dy dtype mismatch: {x.dtype} vs {dy.dtype}"
     assert dy.shape[0] == x.shape[0] and dy.shape[1] == w.shape[2], \
@@ -407,8 +420,9 @@ def matmul_w4(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor,
     of x come in groups.  Returns (T, N) in x's dtype or fp32.  Made for few
     rows a matrix (the weights' bytes bound it); any number is right.  Layouts
     that the copy unit cannot read are copied first.  For serving: no gradient
-    is recorded.
+    is recorded, and forward-mode derivatives are refused.
     """
+    _check_tangents(x, scales)
     xp, pp = x.data_ptr(), packed.data_ptr()
     key = (x.shape, x.stride(), x.dtype, packed.shape, packed.stride(), packed.dtype, scales.shape,
            scales.stride(), scales.dtype, out_dtype, x.get_device(), packed.get_device(), scales.get_device(),

@@ -10,7 +10,7 @@ import torch
 
 from . import _lib
 from .api import _OZ_DTYPE, _check_cuda
-from .experts import _CURRENT_DEVICE, _OnDevice, _Plans, _stream_of
+from .experts import _CURRENT_DEVICE, _OnDevice, _Plans, _check_tangents, _stream_of
 
 ORTHOGONALIZE_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 
@@ -65,7 +65,7 @@ def orthogonalize(g: torch.Tensor, steps: int = 5,
     X <- a X + (b A + c A^2) X, which drives the singular values of X towards
     1 (``coefficients``: one (a, b, c) for all steps or one for each).  Returns
     a contiguous tensor of g's shape and dtype.  For updates: no gradient is
-    recorded.
+    recorded, and forward-mode derivatives are refused.
 
     ``num_splits`` is how many fp16 slices of each matrix the products use: 1
     (11 bits, the default for bf16, whose result has 8, where the products'
@@ -75,6 +75,7 @@ def orthogonalize(g: torch.Tensor, steps: int = 5,
     8 before its last step is refused (OzakiError).  Sums are held in fp32.  Small matrices (up to 128 rows or
     columns) are worked on in fp32 whatever it is, with any coefficients.
     """
+    _check_tangents(g)
     if not isinstance(coefficients, tuple) or hasattr(coefficients[0], "__len__"):
         coefficients = tuple(tuple(c) if hasattr(c, "__len__") else c for c in coefficients)
     if g.dim() > 3:
