@@ -23,7 +23,7 @@ int set_error(int code, const char *fmt, ...) {
 }
 
 static std::atomic<int64_t> g_launches{0};
-void count_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
+void count_library_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
 
 int check_cuda(cudaError_t e, const char *what) {
   if (e == cudaSuccess) return OZ_OK;

@@ -10,6 +10,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <mutex>
 #include <unordered_map>
 
@@ -23,8 +24,13 @@ namespace oz {
 int set_error(int code, const char *fmt, ...);
 int check_cuda(cudaError_t e, const char *what);
 // Kernel launches issued by the library (oz_launch_count), counted at each
-// launch site.
-void count_launch();
+// launch site, and whether this translation unit has issued any.
+void count_library_launch();
+static std::atomic<bool> g_unit_launched{false};
+static inline void count_launch() {
+  g_unit_launched.store(true, std::memory_order_relaxed);
+  count_library_launch();
+}
 
 // cudaFuncSetAttribute(MaxDynamicSharedMemorySize) for a kernel, issued only
 // when this device has not yet allowed the kernel that much shared memory
@@ -104,9 +110,14 @@ int split_two_small_impl(int in_dtype, const void *a, int64_t a_batches, int64_t
                          float *a_scales, void *b_slices, float *b_scales, int64_t ld,
                          void *stream, bool *done);
 
-// Read (and optionally clear) this translation unit's status word.
+// Read (and optionally clear) this translation unit's status word.  A unit without
+// launches has nothing to report and is not read (a copy from the device each).
 static inline int read_status_word(int *value, bool clear) {
   int v = 0;
+  if (!g_unit_launched.load(std::memory_order_relaxed)) {
+    *value = 0;
+    return OZ_OK;
+  }
   if (int rc = check_cuda(cudaMemcpyFromSymbol(&v, g_device_status, sizeof(int)),
                           "read device status"))
     return rc;
