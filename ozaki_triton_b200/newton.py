@@ -63,17 +63,21 @@ def orthogonalize(g: torch.Tensor, steps: int = 5,
     g (..., M, N) fp32, bf16 or fp16, any strides; batch members are
     independent.  X = g / (|g|_F + eps), then ``steps`` times with A = X X^T
     X <- a X + (b A + c A^2) X, which drives the singular values of X towards
-    1 (``coefficients``: one (a, b, c) for all steps or one for each).  Returns
-    a contiguous tensor of g's shape and dtype.  For updates: no gradient is
+    1 (``coefficients``: one (a, b, c) for all steps or one for each).  A zero
+    matrix stays zero, also with eps = 0.  Returns a contiguous tensor of g's
+    shape and dtype (at most 65535 matrices of at most 2^20 rows and columns).  For updates: no gradient is
     recorded, and forward-mode derivatives are refused.
 
     ``num_splits`` is how many fp16 slices of each matrix the products use: 1
     (11 bits, the default for bf16, whose result has 8, where the products'
     time counts: batch M N min(M, N) above 2e9 or so) or 2 (22 bits, the default
-    elsewhere).  Their scales follow from the largest singular value that the
-    coefficients allow, so a schedule that lets one starting in [0, 1] grow past
-    8 before its last step is refused (OzakiError).  Sums are held in fp32.  Small matrices (up to 128 rows or
-    columns) are worked on in fp32 whatever it is, with any coefficients.
+    elsewhere).  One slice leaves a bf16 result 1.15 to 1.4 times as far from the
+    exact one as its rounding alone does; ask for 2 where that matters.  Sums are
+    held in fp32.  The slices' scales follow from the largest singular value
+    that the coefficients allow, so a schedule that lets one starting in [0, 1]
+    grow past 8 before its last step is refused (OzakiError).  Small matrices (up
+    to 128 rows or columns) are worked on in fp32 whatever ``num_splits`` is, with
+    any coefficients.
     """
     _check_tangents(g)
     if not isinstance(coefficients, tuple) or hasattr(coefficients[0], "__len__"):
