@@ -308,6 +308,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       if (leader)
         for (uint32_t k = (it > (uint32_t)S ? it - S : 0); k < it; ++k)
           if (!mbar_settle(&full[k % S], (k / S) & 1, abort_flag, DEV_TIMEOUT_PRODUCER)) break;
+      // nor may this CTA leave while the pair's leader still reports a stage as read to its
+      // barriers (the reports come from the other SM)
+      for (uint32_t k = (it > (uint32_t)S ? it - S : 0); k < it; ++k)
+        if (!mbar_settle(&empty[k % S], (k / S) & 1, abort_flag, DEV_TIMEOUT_PRODUCER)) break;
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer

@@ -344,6 +344,11 @@ __global__ void __launch_bounds__(threads<J>(), 1)
     if (lane == 0 && leader)
       for (uint32_t k = (it > (uint32_t)S ? it - S : 0); k < it; ++k)
         if (!mbar_settle(&full[k % S], (k / S) & 1, abort_flag, DEV_TIMEOUT_PRODUCER)) break;
+    // nor may this CTA leave while the pair's leader still reports a stage as read to its
+    // barriers (the reports come from the other SM)
+    if (lane == 0)
+      for (uint32_t k = (it > (uint32_t)S ? it - S : 0); k < it; ++k)
+        if (!mbar_settle(&empty[k % S], (k / S) & 1, abort_flag, DEV_TIMEOUT_PRODUCER)) break;
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
     typename J::Walk walk(p);
