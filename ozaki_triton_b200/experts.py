@@ -20,6 +20,7 @@ from __future__ import annotations
 import ctypes
 import math
 import threading
+import types
 from typing import Optional, Tuple
 
 import torch
@@ -45,13 +46,16 @@ def _check_places(x: torch.Tensor, *ts: Optional[torch.Tensor]) -> int:
     return index
 
 
+# inside a forward-mode level >= 0 (where torch does not say, tensors are always looked at)
+_LEVEL = forward_ad if hasattr(forward_ad, "_current_level") else types.SimpleNamespace(_current_level=0)
+
+
 def _check_tangents(*ts: Optional[torch.Tensor]) -> None:
     """Refuses tensors that carry a forward-mode derivative: it would be lost, since the
     library reads their values only."""
-    if getattr(forward_ad, "_current_level", 0) >= 0:      # inside a dual level
-        for t in ts:
-            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
-                raise NotImplementedError("no forward-mode derivative of this operator: an argument has a tangent")
+    for t in ts:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError("no forward-mode derivative of this operator: an argument has a tangent")
 
 
 class _OnDevice:
@@ -294,7 +298,8 @@ class _WeightGradient(torch.autograd.Function):
 
 
 def _differentiable_weight_gradient(x, dy, offsets, groups):
-    _check_tangents(x, dy)
+    if _LEVEL._current_level >= 0:
+        _check_tangents(x, dy)
     if (x.requires_grad or dy.requires_grad) and torch.is_grad_enabled():
         return _WeightGradient.apply(x, dy, offsets, groups)
     return _weight_gradient(x, dy, offsets, groups, None)
@@ -312,7 +317,8 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, *,
     once.  Differentiable in x and w, to any order: a gradient is rounded to the
     operands' dtype before it is multiplied.  Forward-mode derivatives are refused.
     """
-    _check_tangents(x, w)
+    if _LEVEL._current_level >= 0:
+        _check_tangents(x, w)
     if (x.requires_grad or w.requires_grad) and torch.is_grad_enabled():
         return _GroupedMatmul.apply(x, w, offsets, out_dtype)
     return _product(x, w, offsets, out_dtype)
@@ -328,7 +334,8 @@ def grouped_matmul_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor,
     rows is zero.  No gradient of the gradients is recorded here; autograd of
     ``grouped_matmul`` records it.  Forward-mode derivatives are refused.
     """
-    _check_tangents(dy, x, w)
+    if _LEVEL._current_level >= 0:
+        _check_tangents(dy, x, w)
     assert dy.dim() == 2 and x.dim() == 2 and w.dim() == 3, "x and dy must have 2 dimensions, w 3"
     assert dy.dtype is x.dtype, f"x/dy dtype mismatch: {x.dtype} vs {dy.dtype}"
     assert dy.shape[0] == x.shape[0] and dy.shape[1] == w.shape[2], \
@@ -422,7 +429,8 @@ def matmul_w4(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor,
     that the copy unit cannot read are copied first.  For serving: no gradient
     is recorded, and forward-mode derivatives are refused.
     """
-    _check_tangents(x, scales)
+    if _LEVEL._current_level >= 0:
+        _check_tangents(x, scales)
     xp, pp = x.data_ptr(), packed.data_ptr()
     key = (x.shape, x.stride(), x.dtype, packed.shape, packed.stride(), packed.dtype, scales.shape,
            scales.stride(), scales.dtype, out_dtype, x.get_device(), packed.get_device(), scales.get_device(),
