@@ -101,11 +101,10 @@ struct W4Walk {
 // 16-19 first), exactly: a field becomes the low mantissa bits of a constant
 // that is a power of two, and the same constant plus z is subtracted.  fp16
 // has room for a field in bits 4-7 too (64 + q beside 1024 + q), bf16 has not.
-// z is any byte.  fp16 holds 1024 + z and 64 + z exactly.  bf16 holds 128 + z up to z =
-// 127 only; from there on the field's bits are flipped in the mantissa of -255, which
-// makes q - 255, and z - 255 is subtracted (24 rows / 64 experts, 2816 x 2048: 32.1 us;
-// 30.4 if z stopped at 127; a product of its own for the upper bit of z, behind a test,
-// took 34 to 38).
+// z is any byte.  fp16 holds 1024 + z and 64 + z exactly.  bf16 holds whole numbers up to
+// 256, and 128 + z is more from 129 on: there the fields are flipped in the mantissa of
+// -255, which makes q - 255, and z - 255 is subtracted (24 rows / 64 experts, 2816 x 2048:
+// 30.9 us; 128 + q below z = 128 and q - 255 above 31.6).
 // A constant that stays in a register (as an immediate it is moved there again at
 // each use, and a mask and an or with two immediates become two instructions).
 __device__ __forceinline__ uint32_t kept(uint32_t c) {
@@ -138,21 +137,16 @@ template <> struct Unpack<__half> {
   }
 };
 template <> struct Unpack<__nv_bfloat16> {
-  uint32_t m0 = kept(0x000f000fu);
-  // 128 + z, or z - 255 with its sign (-0 too)
+  uint32_t m0 = kept(0x000f000fu), c0 = kept(0xc37fc37fu);
+  // z - 255
   static __device__ __forceinline__ uint32_t zero(uint32_t z) {
-    return (z < 128 ? 0x4300u | z : 0x8000u | __float_as_uint((float)(255 - z)) >> 16) * 0x10001u;
+    return (__float_as_uint((float)((int)z - 255)) >> 16) * 0x10001u;
   }
-  // and what the fields are put into: 128, or -255 where the sign is there
-  __device__ __forceinline__ uint2 both(uint32_t z) const {
-    uint32_t sign;                                        // of the upper half, in every bit
-    asm("prmt.b32 %0, %1, %1, 0xbbbb;" : "=r"(sign) : "r"(z));
-    return make_uint2(z, 0x43004300u ^ (sign & 0x807f807fu));
-  }
+  __device__ __forceinline__ uint2 both(uint32_t z) const { return make_uint2(z, 0); }
   __device__ __forceinline__ void values(uint32_t w, uint2 z, uint32_t (&v)[4]) const {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t u = field(w >> (4 * i), m0, z.y);
+      const uint32_t u = field(w >> (4 * i), m0, c0);
       const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&u),
                                        *reinterpret_cast<const __nv_bfloat162 *>(&z.x));
       v[i] = *reinterpret_cast<const uint32_t *>(&d);
