@@ -102,7 +102,7 @@ struct RowTile { int row, rows, column; };   // first row, rows from there to th
 
 // y = x w: A is the rows of x, B the columns of w[e].  For groups of many rows:
 // one of 8192 rows, 8192 x 8192, runs at the rate of the tensor cores under the
-// power limit (715 us, 1540 TFLOP/s).
+// power limit (715 us in short runs, 1540 TFLOP/s).
 template <typename O, int PAIR_, int NT_, bool BMN_> struct RowsJob : NoLookAhead {
   static constexpr int PAIR = PAIR_, NT = NT_, PLANES = 1, PASS = sizeof(O) == 4 ? 8 : 0;
   static constexpr bool AMN = false, BMN = BMN_, RAGGED = false;
@@ -183,9 +183,11 @@ template <typename O, int NT_, bool AMN_> struct ColumnsJob : NoLookAhead {
 // The exchanged roles for pairs of CTAs: 256 columns of w[e] by up to 256 rows of
 // x.  A group's rows are dealt out evenly to as few tiles as hold them, in multiples
 // of 32: with rows as A every group ends in a tile of 256 rows whatever is left
-// (32768 rows over 64 experts, 2048 x 2816: 356 us, this 344; 8192 rows over 64,
-// 2048 x 1408: 93 and 78).  Its epilogue turns the tile, which a short contraction
-// does not hide.
+// (32768 rows over 64 experts, 2048 x 2816, in short runs: 356 us, this 344; 8192 rows
+// over 64, 2048 x 1408: 93 and 78).  Under lasting load the power limit makes the first
+// 405 us.  Its epilogue turns the tile, which a short contraction does not hide.  With
+// fp32 results the sums of the passes spill 28 bytes under 168 registers (15% slower: 369
+// us where bf16 results take 320).
 template <typename O, bool AMN_> struct PairsJob : NoLookAhead {
   static constexpr int PAIR = 2, NT = 256, PLANES = 1, PASS = sizeof(O) == 4 ? 8 : 0;
   static constexpr bool AMN = AMN_, BMN = false, RAGGED = false, VARIABLE = true;
@@ -224,8 +226,10 @@ struct WeightTile { int row, column, group; };
 // dw[e] = x^T dy over the group's rows: both operands are stored across the
 // contraction, whose range is the group.  32768 rows over 16 groups, 4096 x 2048, with
 // dx: 855 us (both are 1100 GFLOP: 1290 TFLOP/s; under lasting load the power limit makes
-// it 1000), bound by the tensor cores; 3989 rows over 16, 1024 x 1536, with dx:
-// 63 us, bound by the 100 MB of fp32 results and by tiles of only 4 blocks.
+// it 1010; with bf16 results 826 where fp32 ones take 869), bound by the tensor cores; 3989
+// rows over 16, 1024 x 1536, with dx: 63 us, bound by the 100 MB of fp32 results and by tiles
+// of only 4 blocks.  The contraction is not divided: few tiles of many rows leave SMs idle
+// (one group of 32768 rows, 256 x 256: 245 us with dx, which takes 18).
 template <typename O, int PAIR_, int NT_> struct WeightsJob : NoLookAhead {
   static constexpr int PAIR = PAIR_, NT = NT_, PLANES = 1, PASS = sizeof(O) == 4 ? 8 : 0;
   static constexpr bool AMN = true, BMN = true, RAGGED = true;

@@ -17,7 +17,9 @@
 // schedule from 2 to 10^15 in 5 steps, and the matrices to zero).  Instead e puts the bound
 // at 2^12, which leaves a factor of 16 below the largest fp16 and, two slices
 // having 22 bits down to 2^-3, one of 2^15 above the entries that keep them all.  Schedules
-// whose bound leaves [0, 8] before their last step are refused.  With one slice the products use `high` alone (11 bits) and
+// whose bound leaves [0, 8] before their last step are refused.
+//
+// With one slice the products use `high` alone (11 bits) and
 // only the term a X keeps X's 22: that term carries the directions that the
 // products hardly touch, and rounding it as well as P X makes both sides of
 // the sum consistent only for full-rank G (measured on a low-rank gradient:
@@ -25,12 +27,14 @@
 // high*high + high*low + low*high.  S and P are symmetric: only the tiles on
 // and below the diagonal are multiplied, each written twice.
 //
-// 5 steps measured: 4096 x 4096 fp32 (two slices) 3.45 ms, 1200 TFLOP/s of fp16
-// products (2.46 ms at the burst rate), bound by the tensor cores under the power
-// limit and by 136 tiles of S and P for 74 pairs of CTAs; 4 x 2048 x 2816 bf16
-// (one slice) 0.89 ms (0.52 at the burst rate), bound by what the products and the
-// epilogues' slices move between L2 and the SMs; up to 1000 or so rows the launches'
-// length (17 of 7 us or so).
+// 5 steps measured: 4096 x 4096 fp32 (two slices) 3.71 ms under lasting load, 1110 TFLOP/s
+// of fp16 products (3.45 ms in short runs; 2.46 at the burst rate), bound by the tensor cores
+// under the power limit and by 136 tiles of S and P for 74 pairs of CTAs; 4 x 2048 x 2816
+// bf16 (one slice) 1.04 ms under lasting load (0.89 in short runs; 0.52 at the burst rate),
+// bound by what the products and the epilogues' slices move between L2 and the SMs; up to
+// 1000 or so rows the launches' length (17 of 7 us or more: 256 x 256 122 us, 300 x 1000
+// 173, 1024 x 1024 261).  The pairs' tiles with passes hold 128 sums a thread under a cap of
+// 168 registers and spill 108 to 172 bytes.
 
 #include <algorithm>
 #include <cmath>
@@ -647,7 +651,7 @@ template <int PAIR_, int NT_, int PLANES_, int PASS_> struct UpdateJob {
 // computed a few rows a CTA and handed to the others, and a X + P X needs
 // nothing of another panel.  fp32 FMAs are enough here (and rounded sums more
 // exact than the tensor core's): a step of 64 x 250 is 0.23 M FMAs a CTA.  12 of
-// them take 42 us, 16 x 16 takes 13 us: barriers, exchanges and the latency of each part.
+// them take 44 us, one of 16 x 16 13: barriers, exchanges and the latency of each part.
 constexpr int kSmallRows = 128;
 constexpr int kSmallThreads = 256;
 constexpr int kMicro = 4;                // rows and columns of a thread's tile

@@ -18,10 +18,13 @@
 // (0 4, 1 5, 2 6, 3 7) on both sides.  A group's sum is scaled in fp32.
 // The warps of a tile share k and are summed in shared memory in a fixed order.
 //
-// 8 rows, 28672 x 8192, groups of 128: 49.5 us (123 MB: 2.5 TB/s); 24 rows over 64
-// experts of 2816 x 2048: 30 us; one row, 2048 x 2048: 5.4 us on the device, 11 a call.
-// The warps' own instructions bound it, 700 a chunk of 64 x 128 weights (four warps a
-// scheduler do not cover their latencies) and the last round of tiles.
+// 8 rows, 28672 x 8192, groups of 128: 46.7 us (123 MB: 2.6 TB/s); 24 rows over 64
+// experts of 2816 x 2048: 31 us; one row, 2048 x 2048: 5.4 us on the device, 11 a call.
+// The warps' own instructions bound it, 690 a chunk of 64 x 128 weights (four warps a
+// scheduler do not cover their latencies) and the last round of tiles.  Two blocks an SM
+// leave 128 registers: with 64 weight rows, groups of 64 spill 32 (fp16) and 44 bytes
+// (bf16), groups of 128 spill 4 (fp16).  Many rows are not what it is for: 4096 x 11008, 64
+// rows 47 us, 512 291, 2048 934 (each 32 of them unpack the weights again).
 
 #include "oz_tile.cuh"
 
