@@ -328,8 +328,9 @@ int oz_matmul_w4(const oz_w4_args *args, void *stream);
  *                  most before the last step (OZ_ERR_UNSUPPORTED otherwise)
  *   num_splits   : fp16 slices of a matrix in the products, 1 or 2
  *   out          : contiguous (batch, m, n) of g's type
- *                  (small matrices, up to 128 rows or columns, are worked on in
- *                  fp32 whatever it is)
+ *                  (small matrices, at most 128 rows or columns, are worked on in
+ *                  fp32 whatever num_splits is where that is faster: those whose
+ *                  workspace is 0 bytes)
  *   workspace    : oz_orthogonalize_workspace_bytes() bytes, 256-byte aligned;
  *                  may be 0 bytes and NULL
  */
