@@ -148,8 +148,7 @@ def prepare(case, seed):
     if case["op"] == "route":
         return state
     # what the forward pass returned
-    weights, experts, slots, offsets, counts, loss = _plain_route(state["logits"], picks, case.get("normalize", False))
-    state["routing"] = (weights, experts.int(), slots.int(), offsets.int(), counts.int(), loss)
+    state["routing"] = _plain_route(state["logits"], picks, case.get("normalize", False))
     if case["op"] == "route_grad":
         state["dweights"] = torch.randn(t, picks, generator=g, device="cuda")
         state["dloss"] = torch.rand((), generator=g, device="cuda") + 0.5
@@ -239,18 +238,19 @@ def _plain_route(logits, picks, normalize):
     offsets = torch.cat([counts.new_zeros(1), torch.cumsum(counts, 0)])
     mean = p.sum(0) / held.sum().clamp(min=1)
     share = counts.float() / counts.sum().clamp(min=1)
-    return weights, experts, slots, offsets, counts, e * (share * mean).sum()
+    whole = (v.int() for v in (experts, slots, offsets, counts, held.sum()))
+    return weights, *whole, e * (share * mean).sum()
 
 
 def _plain_route_grad(state):
     logits, normalize = state["logits"], state["case"]["normalize"]
-    weights, experts, _, _, counts, _ = state["routing"]
-    p, held = _probabilities(logits)
+    weights, experts, _, _, counts, tokens, _ = state["routing"]
+    p, _ = _probabilities(logits)
     real = experts >= 0
     at = torch.where(real, experts, torch.zeros_like(experts)).long()
     dw = torch.where(real, state["dweights"], torch.zeros_like(state["dweights"]))
     share = counts.float() / counts.sum().clamp(min=1)
-    slope = (state["dloss"] * logits.shape[1] / held.sum().clamp(min=1)) * share
+    slope = (state["dloss"] * logits.shape[1] / tokens.clamp(min=1)) * share
     slope = slope.expand_as(p)
     if normalize:
         # the picks' weights are a softmax over themselves
@@ -355,7 +355,7 @@ def work(case):
                                + (4 * n if case["bias"] else 0)), "flops": 4.0 * t * k * n}
     e, picks, held = case["e"], case["picks"], case["t"] - case["padded"]
     if case["op"] == "route":
-        return {"bytes": float(t * e * es + 12 * t * picks + 8 * e + 8), "flops": float(t * e * (4 + picks))}
+        return {"bytes": float(t * e * es + 12 * t * picks + 8 * e + 12), "flops": float(t * e * (4 + picks))}
     if case["op"] == "route_grad":
         return {"bytes": float(2 * t * e * es + 12 * t * picks + 4 * e), "flops": 10.0 * t * e}
     d = case["d"]
@@ -432,13 +432,13 @@ def _exact_route(case, logits):
     row = offsets[:-1] + before
     slots = torch.where(experts >= 0, row.gather(1, experts.clamp(min=0)), -1)
     loss = e * (counts.double() / max(1, int(counts.sum())) * p.sum(0) / max(1, int(held.sum()))).sum()
-    return weights, experts, slots, offsets, counts, loss
+    return weights, experts, slots, offsets, counts, held.sum(), loss
 
 
 def _exact_route_grad(state):
     """By differentiation of the weights and the loss."""
     case = state["case"]
-    _, experts, _, _, counts, _ = state["routing"]
+    _, experts, _, _, counts, _, _ = state["routing"]
     v = state["logits"].double()
     held = (v > float("-inf")).any(1)
     v = v[held].requires_grad_()
