@@ -342,6 +342,135 @@ int oz_orthogonalize(const void *g, int dtype, int64_t batch, int64_t m, int64_t
                      int64_t workspace_bytes, void *stream);
 
 /*
+ * Product with bias, activation and residual (no counterpart in the reference):
+ *   u = x w + bias,  y = act(u) + residual
+ *
+ *   x        : (rows, k) fp16 or bf16, unit stride along k, row pitch x_sr
+ *   w        : (k, n) of x's type, element strides w_sk, w_sn, one of them 1
+ *   bias     : n elements of x's type or fp32 (bias_dtype), or NULL
+ *   residual : (rows, n) of y's type, unit stride along n, row pitch residual_sr, or NULL
+ *   y        : contiguous (rows, n) of x's type or fp32 (out_dtype)
+ *   pre      : contiguous (rows, n) of x's type for u, or NULL
+ *   workspace: as in oz_grouped_matmul, for copies of operands off the 16-byte boundaries
+ */
+enum oz_activation { OZ_ACT_NONE = 0, OZ_ACT_RELU = 1, OZ_ACT_GELU = 2, OZ_ACT_SILU = 3 };
+typedef struct {
+  const void *x, *w, *bias, *residual;
+  void *y, *pre, *workspace;
+  int64_t rows, k, n, x_sr, w_sk, w_sn, residual_sr, workspace_bytes;
+  int32_t dtype, out_dtype, bias_dtype, act;
+} oz_linear_args;
+int oz_linear(const oz_linear_args *args, void *stream);
+
+/*
+ * Gradients of oz_linear:
+ *   du = dy act'(pre),  dx = du w^T,  dw = x^T du,  db = sum over the rows of du
+ * dy (rows, n) and pre (rows, n; NULL without activation) of x's type with row pitches dy_sr,
+ * pre_sr; x and w as there.  dx: contiguous (rows, k) of x's type; dw: contiguous (k, n) of
+ * x's type or fp32 (dw_dtype); db: n fp32; each may be NULL (x is read for dw only, w for dx
+ * only).  workspace: oz_linear_backward_workspace_bytes() bytes (`sums`: db is wanted), then
+ * room for copies of operands off the 16-byte boundaries; 256-byte aligned.
+ */
+typedef struct {
+  const void *dy, *x, *w, *pre;
+  void *dx, *dw;
+  float *db;
+  void *workspace;
+  int64_t rows, k, n, dy_sr, x_sr, w_sk, w_sn, pre_sr, workspace_bytes;
+  int32_t dtype, dw_dtype, act, unused;
+} oz_linear_backward_args;
+int64_t oz_linear_backward_workspace_bytes(int64_t rows, int64_t n, int32_t act, int32_t sums);
+int oz_linear_backward(const oz_linear_backward_args *args, void *stream);
+
+/*
+ * Router of an expert layer (no counterpart in the reference).  For every row of logits:
+ * softmax (zeros for a row that is -inf throughout), the `picks` largest entries (the lowest
+ * index first among equals; entries of -inf are no picks), and over all rows
+ *
+ *   weights  : (rows, picks) fp32, the picks' probabilities, or with `normalize` those over
+ *              their sum in the row; 0 where there is no pick
+ *   chosen   : (rows, picks) int32 experts, -1 where there is no pick
+ *   slots    : (rows, picks) int32, the pick's row in the order of experts, then of rows
+ *   offsets  : experts + 1 int32, first row of each expert
+ *   counts   : experts int32;  tokens: int32, rows with a pick
+ *   loss     : fp32, experts * sum_e (counts[e] / sum of counts) (sum of p[., e] / tokens)
+ *
+ * logits: fp32, fp16 or bf16 (dtype), element (r, e) at r * row + e * col.  Up to 1024
+ * experts and 32 picks.  workspace: oz_route_workspace_bytes() bytes, 16-byte aligned; may be
+ * 0 bytes and NULL.
+ */
+typedef struct {
+  const void *logits;
+  float *weights, *loss;
+  int32_t *chosen, *slots, *offsets, *counts, *tokens;
+  void *workspace;
+  int64_t rows, row, col, workspace_bytes;
+  int32_t experts, picks, normalize, dtype;
+} oz_route_args;
+int64_t oz_route_workspace_bytes(int64_t rows, int32_t experts);
+int oz_route(const oz_route_args *args, void *stream);
+
+/*
+ * Gradient of oz_route's weights and loss: dlogits, contiguous (rows, experts) of the logits'
+ * type, from dweights (rows, picks) fp32 and dloss, fp32 on the device (either may be NULL).
+ */
+typedef struct {
+  const void *logits;
+  const float *dweights, *dloss, *weights;
+  const int32_t *chosen, *counts, *tokens;
+  void *dlogits;
+  int64_t rows, row, col;
+  int32_t experts, picks, normalize, dtype;
+} oz_route_backward_args;
+int oz_route_backward(const oz_route_backward_args *args, void *stream);
+
+/*
+ * Rows of tokens to their experts and back (no counterpart in the reference), `picks` rows a
+ * token, tokens * picks rows in all:
+ *   oz_dispatch         : rows_out[slots[t, j]] = x[t]; zeros in the rows from offsets[experts] on
+ *   oz_combine          : x_out[t] = sum_j weights[t, j] rows[slots[t, j]] (weights NULL: 1)
+ *   oz_combine_backward : rows_out[slots[t, j]] = weights[t, j] x[t], zeros as in oz_dispatch;
+ *                         dweights[t, j] = x[t] . rows[slots[t, j]]
+ * A slot outside [0, tokens * picks) is no row.  x and rows: fp32, fp16 or bf16 with unit
+ * stride along d and row pitches x_row, rows_row; results contiguous.  Sums are fp32.
+ */
+typedef struct {
+  const void *x, *rows;
+  void *x_out, *rows_out;
+  const int32_t *slots, *offsets;
+  const float *weights;
+  float *dweights;
+  int64_t tokens, d, x_row, rows_row;
+  int32_t experts, picks, dtype, unused;
+} oz_rows_args;
+int oz_dispatch(const oz_rows_args *args, void *stream);
+int oz_combine(const oz_rows_args *args, void *stream);
+int oz_combine_backward(const oz_rows_args *args, void *stream);
+
+/*
+ * Gradients scaled to a common norm (no counterpart in the reference):
+ *   *norm = sqrt(sum of the squares of all tensors),
+ *   outs[i] = grads[i] * min(1, max_norm / (*norm + eps))
+ * Host arrays of `tensors` addresses, sizes (contiguous elements) and types (fp32, fp16 or
+ * bf16).  outs[i] may be grads[i] where the types agree; results that share memory otherwise are
+ * refused.  norm: fp32 on the device.  workspace: oz_clip_workspace_bytes() bytes, 16-byte
+ * aligned.
+ */
+typedef struct {
+  const void *const *grads;
+  void *const *outs;
+  const int64_t *sizes;
+  const int32_t *dtypes, *out_dtypes;
+  float *norm;
+  void *workspace;
+  int64_t workspace_bytes;
+  double max_norm, eps;
+  int32_t tensors, unused;
+} oz_clip_args;
+int64_t oz_clip_workspace_bytes(int32_t tensors);
+int oz_clip(const oz_clip_args *args, void *stream);
+
+/*
  * Peer mappings for the multi-GPU gather (no counterpart in the reference,
  * which has no multi-GPU path).  One process per GPU: a rank exports the
  * allocation holding its slice buffer, each peer imports it once and pulls

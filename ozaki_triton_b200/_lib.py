@@ -42,6 +42,23 @@ GroupedWgradArgs = _struct("GroupedWgradArgs", ("x dy offsets dw", _vp), ("rows 
 W4Args = _struct("W4Args", ("x packed scales zeros offsets y", _vp),
                  ("rows k n x_sr p_se p_sn s_se s_sn ldy", _i64),
                  ("experts group offsets_64 dtype scale_dtype out_dtype", _i32))
+LinearArgs = _struct("LinearArgs", ("x w bias residual y pre workspace", _vp),
+                     ("rows k n x_sr w_sk w_sn residual_sr workspace_bytes", _i64),
+                     ("dtype out_dtype bias_dtype act", _i32))
+LinearBackwardArgs = _struct("LinearBackwardArgs", ("dy x w pre dx dw db workspace", _vp),
+                             ("rows k n dy_sr x_sr w_sk w_sn pre_sr workspace_bytes", _i64),
+                             ("dtype dw_dtype act unused", _i32))
+RouteArgs = _struct("RouteArgs", ("logits weights loss chosen slots offsets counts tokens workspace", _vp),
+                    ("rows row col workspace_bytes", _i64), ("experts picks normalize dtype", _i32))
+RouteBackwardArgs = _struct("RouteBackwardArgs", ("logits dweights dloss weights chosen counts tokens dlogits", _vp),
+                            ("rows row col", _i64), ("experts picks normalize dtype", _i32))
+RowsArgs = _struct("RowsArgs", ("x rows x_out rows_out slots offsets weights dweights", _vp),
+                   ("tokens d x_row rows_row", _i64), ("experts picks dtype unused", _i32))
+ClipArgs = _struct("ClipArgs", ("grads outs sizes dtypes out_dtypes norm workspace", _vp), ("workspace_bytes", _i64),
+                   ("max_norm eps", ctypes.c_double), ("tensors unused", _i32))
+
+# activation codes (enum oz_activation)
+ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "silu": 3}
 
 SIGNATURES = {
     "oz_compute_split_bits": (_int, [_i64, _int, ctypes.POINTER(_i32)]),
@@ -71,6 +88,17 @@ SIGNATURES = {
     "oz_orthogonalize_workspace_bytes": (_i64, [_int, _i64, _i64, _i64, _i32, _i32]),
     "oz_orthogonalize": (_int, [_vp, _int, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _vp,
                                 ctypes.c_double, _i32, _vp, _vp, _i64, _vp]),
+    "oz_linear": (_int, [ctypes.POINTER(LinearArgs), _vp]),
+    "oz_linear_backward_workspace_bytes": (_i64, [_i64, _i64, _i32, _i32]),
+    "oz_linear_backward": (_int, [ctypes.POINTER(LinearBackwardArgs), _vp]),
+    "oz_route_workspace_bytes": (_i64, [_i64, _i32]),
+    "oz_route": (_int, [ctypes.POINTER(RouteArgs), _vp]),
+    "oz_route_backward": (_int, [ctypes.POINTER(RouteBackwardArgs), _vp]),
+    "oz_dispatch": (_int, [ctypes.POINTER(RowsArgs), _vp]),
+    "oz_combine": (_int, [ctypes.POINTER(RowsArgs), _vp]),
+    "oz_combine_backward": (_int, [ctypes.POINTER(RowsArgs), _vp]),
+    "oz_clip_workspace_bytes": (_i64, [_i32]),
+    "oz_clip": (_int, [ctypes.POINTER(ClipArgs), _vp]),
     "oz_ipc_export": (_int, [_vp, _vp, ctypes.POINTER(_i64)]),
     "oz_ipc_import": (_int, [_vp, _i64, ctypes.POINTER(_vp)]),
     "oz_ipc_close": (_int, [_vp, _i64]),

@@ -1,0 +1,301 @@
+// oz_clip.cu -- gradients of many tensors, scaled so that their common norm is at
+// most max_norm:
+//
+//   norm = sqrt(sum of all squares),  out = g min(1, max_norm / (norm + eps))
+//
+// Two launches read the gradients: the first sums squares (fp32 in a thread's
+// piece, fp64 across pieces, in an order that does not depend on timing), the
+// second has every block add up the first's sums and scales.  Bound by memory:
+// the gradients are read twice and the results written once.
+
+#include <algorithm>
+#include <cmath>
+#include <vector>
+
+#include "oz_stream.cuh"
+
+namespace oz {
+namespace {
+using namespace stream;
+
+constexpr int kThreads = 256;
+constexpr int kPiece = 8192;          // elements of a block's turn
+
+struct Tensor {
+  const void *g;
+  void *out;
+  int64_t n;
+  int first;                          // pieces of the tensors before it
+  int types;                          // type of g, of out (4 bits each), 16-byte runs (bit 8)
+};
+template <int N> struct Table {
+  Tensor t[N];
+  int tensors, pieces;
+};
+struct Sums {
+  double *partial;                    // one of each block of each summing launch
+  float *norm;
+  int blocks;
+  float max_norm, eps;
+};
+
+template <int N> __device__ __forceinline__ const Tensor &tensor_of(const Table<N> &table, int piece) {
+  int low = 0, high = table.tensors - 1;      // the last tensor whose first piece is not after it
+  while (low < high) {
+    const int mid = (low + high + 1) / 2;
+    if (table.t[mid].first <= piece) low = mid;
+    else high = mid - 1;
+  }
+  return table.t[low];
+}
+
+// Calls f(offset, values, how many) for this thread's elements of a piece: V at a time
+// with 4 loads on their way, or one by one.
+template <typename T, typename F>
+__device__ __forceinline__ void each_run(const T *g, int64_t n, bool runs, F f) {
+  constexpr int V = 16 / sizeof(T), AT_ONCE = 4;
+  if (runs) {
+    for (int64_t i0 = (int64_t)threadIdx.x * V; i0 < n; i0 += (int64_t)kThreads * V * AT_ONCE) {
+      uint4 u[AT_ONCE];
+#pragma unroll
+      for (int j = 0; j < AT_ONCE; ++j) {
+        const int64_t i = i0 + (int64_t)j * kThreads * V;
+        if (i + V <= n) u[j] = *reinterpret_cast<const uint4 *>(g + i);
+      }
+#pragma unroll
+      for (int j = 0; j < AT_ONCE; ++j) {
+        const int64_t i = i0 + (int64_t)j * kThreads * V;
+        if (i + V <= n) {
+          float v[V];
+          unpack<T>(u[j], v);
+          f(i, v, V);
+        } else {
+          for (int64_t x = i; x < n; ++x) {
+            float v[V];
+            v[0] = to_f32(g[x]);
+            f(x, v, 1);
+          }
+        }
+      }
+    }
+  } else {
+    for (int64_t i = threadIdx.x; i < n; i += kThreads) {
+      float v[V];
+      v[0] = to_f32(g[i]);
+      f(i, v, 1);
+    }
+  }
+}
+
+template <typename T> __device__ __forceinline__ float squares(const T *g, int64_t n, bool runs) {
+  float s = 0.f;
+  each_run<T>(g, n, runs, [&](int64_t, const auto &v, int m) {
+    if (m == 1) s = fmaf(v[0], v[0], s);
+    else
+#pragma unroll
+      for (int x = 0; x < (int)(16 / sizeof(T)); ++x) s = fmaf(v[x], v[x], s);
+  });
+  return s;
+}
+
+template <int N>
+__global__ void __launch_bounds__(kThreads) norm_kernel(const __grid_constant__ Table<N> table, double *partial) {
+  start_after_earlier_kernels();
+  double all = 0;
+  for (int piece = blockIdx.x; piece < table.pieces; piece += gridDim.x) {
+    const Tensor &t = tensor_of(table, piece);
+    const int64_t at = (int64_t)(piece - t.first) * kPiece;
+    const int64_t n = min(t.n - at, (int64_t)kPiece);
+    const int type = t.types & 15;
+    const bool runs = t.types >> 8 & 1;
+    if (type == OZ_F32) all += squares(static_cast<const float *>(t.g) + at, n, runs);
+    else if (type == OZ_F16) all += squares(static_cast<const __half *>(t.g) + at, n, runs);
+    else all += squares(static_cast<const __nv_bfloat16 *>(t.g) + at, n, runs);
+  }
+  __shared__ double warp_sum[kThreads / 32];
+#pragma unroll
+  for (int o = 16; o > 0; o /= 2) all += __shfl_xor_sync(0xffffffffu, all, o);
+  if (threadIdx.x % 32 == 0) warp_sum[threadIdx.x / 32] = all;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < kThreads / 32; ++w) all += warp_sum[w];
+    partial[blockIdx.x] = all;
+  }
+}
+
+template <typename T, typename O>
+__device__ __forceinline__ void scaled(const T *g, O *out, int64_t n, bool runs, float scale) {
+  constexpr int V = 16 / sizeof(T), W = 16 / sizeof(O);
+  each_run<T>(g, n, runs, [&](int64_t i, const auto &v, int m) {
+    if (m == 1) {
+      out[i] = from_f32<O>(v[0] * scale);
+      return;
+    }
+    if constexpr (V >= W) {
+#pragma unroll
+      for (int h = 0; h < V / W; ++h) {
+        float w[W];
+#pragma unroll
+        for (int x = 0; x < W; ++x) w[x] = v[h * W + x] * scale;
+        *reinterpret_cast<uint4 *>(out + i + h * W) = pack<O>(w);
+      }
+    } else {                              // 4 fp32 values to 8 bytes
+      O w[V];
+#pragma unroll
+      for (int x = 0; x < V; ++x) w[x] = from_f32<O>(v[x] * scale);
+      *reinterpret_cast<uint2 *>(out + i) = *reinterpret_cast<const uint2 *>(w);
+    }
+  });
+}
+
+template <int N>
+__global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__ Table<N> table, const Sums sums) {
+  __shared__ float shared_scale;
+  __shared__ double warp_sum[kThreads / 32];
+  start_after_earlier_kernels();
+  double all = 0;
+  for (int i = threadIdx.x; i < sums.blocks; i += kThreads) all += __ldg(sums.partial + i);
+#pragma unroll
+  for (int o = 16; o > 0; o /= 2) all += __shfl_xor_sync(0xffffffffu, all, o);
+  if (threadIdx.x % 32 == 0) warp_sum[threadIdx.x / 32] = all;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < kThreads / 32; ++w) all += warp_sum[w];
+    const float norm = (float)sqrt(all);
+    const float ratio = sums.max_norm / (norm + sums.eps);
+    shared_scale = ratio >= 1.f ? 1.f : ratio;                 // NaN stays
+    if (blockIdx.x == 0) *sums.norm = norm;
+  }
+  __syncthreads();
+  const float scale = shared_scale;
+  // the pieces read last are the first here: some of them are still in L2
+  for (int piece = table.pieces - 1 - (int)blockIdx.x; piece >= 0; piece -= gridDim.x) {
+    const Tensor &t = tensor_of(table, piece);
+    const int64_t at = (int64_t)(piece - t.first) * kPiece;
+    const int64_t n = min(t.n - at, (int64_t)kPiece);
+    const int type = t.types & 15, to = t.types >> 4 & 15;
+    const bool runs = t.types >> 8 & 1;
+    auto from = [&](auto g0) {
+      using T = decltype(g0);
+      const T *g = static_cast<const T *>(t.g) + at;
+      if (to == OZ_F32) scaled(g, static_cast<float *>(t.out) + at, n, runs, scale);
+      else if (to == OZ_F16) scaled(g, static_cast<__half *>(t.out) + at, n, runs, scale);
+      else scaled(g, static_cast<__nv_bfloat16 *>(t.out) + at, n, runs, scale);
+    };
+    if (type == OZ_F32) from(float{});
+    else if (type == OZ_F16) from(__half{});
+    else from(__nv_bfloat16{});
+  }
+}
+
+// A launch takes the addresses of at most this many tensors as arguments.
+constexpr int kFew = 64, kMany = 640;
+constexpr int kBlocksPerSm = 4;
+
+int sum_blocks(int64_t pieces) { return (int)std::min<int64_t>(pieces, (int64_t)sm_count() * kBlocksPerSm); }
+
+template <int N> Table<N> table_of(const oz_clip_args &a, int first, int count) {
+  Table<N> table;
+  int64_t pieces = 0;
+  table.tensors = 0;
+  for (int i = first; i < first + count; ++i) {
+    const int64_t n = a.sizes[i];
+    if (n == 0) continue;
+    const int es = dtype_size(a.dtypes[i]), os = dtype_size(a.out_dtypes[i]);
+    const bool runs = (uintptr_t)a.grads[i] % 16 == 0 && (uintptr_t)a.outs[i] % (es == 4 && os == 2 ? 8 : 16) == 0;
+    table.t[table.tensors++] = Tensor{a.grads[i], a.outs[i], n, (int)pieces,
+                                      a.dtypes[i] | a.out_dtypes[i] << 4 | (runs ? 1 << 8 : 0)};
+    pieces += (n + kPiece - 1) / kPiece;
+  }
+  table.pieces = (int)pieces;
+  return table;
+}
+int64_t pieces_of(const oz_clip_args &a, int first, int count) {
+  int64_t pieces = 0;
+  for (int i = first; i < first + count; ++i) pieces += (a.sizes[i] + kPiece - 1) / kPiece;
+  return pieces;
+}
+
+template <int N> int run(const oz_clip_args &a, Sums sums, cudaStream_t st) {
+  sums.blocks = 0;
+  for (int i = 0; i < a.tensors; i += N) {
+    const auto table = table_of<N>(a, i, std::min(N, a.tensors - i));
+    if (!table.pieces) continue;
+    const int blocks = sum_blocks(table.pieces);
+    if (int rc = launch(norm_kernel<N>, dim3(blocks), kThreads, 0, st, "norm_kernel launch", table,
+                        sums.partial + sums.blocks))
+      return rc;
+    sums.blocks += blocks;
+  }
+  // the last tensors first, like the pieces in a launch
+  const int last = a.tensors ? (a.tensors - 1) / N * N : 0;
+  for (int i = last; i >= 0; i -= N) {
+    const auto table = table_of<N>(a, i, std::min(N, a.tensors - i));
+    if (!table.pieces && i != last) continue;                   // one launch at least writes the norm
+    if (int rc = launch(scale_kernel<N>, dim3(std::max(1, sum_blocks(table.pieces))), kThreads, 0, st,
+                        "scale_kernel launch", table, sums))
+      return rc;
+  }
+  return OZ_OK;
+}
+
+}  // namespace
+}  // namespace oz
+
+extern "C" int64_t oz_clip_workspace_bytes(int32_t tensors) {
+  if (tensors < 0) return OZ_ERR_INVALID;
+  const int64_t launches = tensors <= oz::kFew ? 1 : (tensors + oz::kMany - 1) / oz::kMany;
+  return launches * oz::stream::sm_count() * oz::kBlocksPerSm * 8;
+}
+
+extern "C" int oz_clip(const oz_clip_args *args, void *stream) {
+  if (!args) return oz::set_error(OZ_ERR_INVALID, "null arguments");
+  using namespace oz;
+  const oz_clip_args &a = *args;
+  if (a.tensors < 0) return set_error(OZ_ERR_INVALID, "negative size");
+  if (!a.norm || (a.tensors > 0 && (!a.grads || !a.outs || !a.sizes || !a.dtypes || !a.out_dtypes)))
+    return set_error(OZ_ERR_INVALID, "null pointer");
+  if (!(a.max_norm >= 0) || !(a.eps >= 0)) return set_error(OZ_ERR_INVALID, "max_norm and eps must not be negative");
+  const int64_t bytes = oz_clip_workspace_bytes(a.tensors);
+  if (!a.workspace || (uintptr_t)a.workspace % 16 != 0 || a.workspace_bytes < bytes)
+    return set_error(OZ_ERR_INVALID, "workspace of %lld bytes (16-byte aligned) needed, got %lld at %p",
+                     (long long)bytes, (long long)a.workspace_bytes, a.workspace);
+  struct Range { uintptr_t from, to; };
+  thread_local std::vector<Range> ranges;
+  try {
+    ranges.clear();
+    ranges.reserve(a.tensors);
+    for (int i = 0; i < a.tensors; ++i) {
+      for (int dt : {a.dtypes[i], a.out_dtypes[i]})
+        if (dt != OZ_F32 && dt != OZ_F16 && dt != OZ_BF16)
+          return set_error(OZ_ERR_UNSUPPORTED, "unsupported dtype %d of tensor %d (fp32, fp16 or bf16)", dt, i);
+      if (a.sizes[i] < 0) return set_error(OZ_ERR_INVALID, "negative size of tensor %d", i);
+      if (a.sizes[i] == 0) continue;
+      if (!a.grads[i] || !a.outs[i]) return set_error(OZ_ERR_INVALID, "null pointer of tensor %d", i);
+      const int es = dtype_size(a.dtypes[i]), os = dtype_size(a.out_dtypes[i]);
+      if ((uintptr_t)a.grads[i] % es || (uintptr_t)a.outs[i] % os)
+        return set_error(OZ_ERR_INVALID, "tensor %d is not aligned to its elements", i);
+      ranges.push_back({(uintptr_t)a.outs[i], (uintptr_t)a.outs[i] + (uintptr_t)a.sizes[i] * os});
+    }
+  } catch (...) {
+    return set_error(OZ_ERR_INVALID, "out of host memory");
+  }
+  if (pieces_of(a, 0, a.tensors) > INT32_MAX / 2) return set_error(OZ_ERR_INVALID, "size out of range");
+  // results that share memory would be scaled twice, or in parts
+  std::sort(ranges.begin(), ranges.end(), [](const Range &x, const Range &y) { return x.from < y.from; });
+  for (size_t i = 1; i < ranges.size(); ++i)
+    if (ranges[i].from < ranges[i - 1].to) return set_error(OZ_ERR_INVALID, "two results share memory");
+  // and so would a result over another tensor's gradient, which is read again
+  for (int i = 0; i < a.tensors; ++i) {
+    if (a.sizes[i] == 0) continue;
+    const uintptr_t g0 = (uintptr_t)a.grads[i], g1 = g0 + (uintptr_t)a.sizes[i] * dtype_size(a.dtypes[i]);
+    const uintptr_t o0 = (uintptr_t)a.outs[i];
+    auto it = std::upper_bound(ranges.begin(), ranges.end(), g0, [](uintptr_t v, const Range &r) { return v < r.to; });
+    for (; it != ranges.end() && it->from < g1; ++it)
+      if (!(it->from == o0 && g0 == o0 && a.dtypes[i] == a.out_dtypes[i]))
+        return set_error(OZ_ERR_INVALID, "a result shares memory with a gradient, and is not that gradient");
+  }
+  const Sums sums{static_cast<double *>(a.workspace), a.norm, 0, (float)a.max_norm, (float)a.eps};
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  return a.tensors <= kFew ? run<kFew>(a, sums, st) : run<kMany>(a, sums, st);
+}

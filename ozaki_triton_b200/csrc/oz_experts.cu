@@ -13,7 +13,7 @@
 
 #include <cmath>
 
-#include "oz_tile.cuh"
+#include "oz_operands.cuh"
 
 namespace oz {
 int status_experts(int *value, bool clear) { return read_status_word(value, clear); }
@@ -281,111 +281,6 @@ int check_grouped(int dtype, int out_dtype, int32_t groups, int64_t rows, int64_
   return OZ_OK;
 }
 
-// Whether the copy unit can read rows (and matrices) that far apart.
-bool pitch_ok(int64_t stride, int64_t count) {
-  return count <= 1 || (stride > 0 && stride % 8 == 0 && stride < ((int64_t)1 << 38));
-}
-int64_t pitch_bytes(int64_t stride, int64_t count, int64_t inner) {
-  return 2 * (count <= 1 ? (inner + 7) / 8 * 8 : stride);
-}
-
-bool readable(const void *p, int64_t rows, int64_t row_stride, int64_t mats, int64_t mat_stride) {
-  return (uintptr_t)p % 16 == 0 && pitch_ok(row_stride, rows) && pitch_ok(mat_stride, mats);
-}
-
-// Copies of operands whose rows the copy unit cannot address (16-byte boundaries
-// and pitches): rows of 2-byte elements with unit stride to rows 16 bytes apart,
-// both operands of a call in one launch.  A warp takes up to 2048 elements of a
-// row, 9 words a lane on their way at a time.  1003 rows / 12 experts, 1000 x 1407,
-// most of whose time is this copy of 34 MB: 33.1 us with 6 blocks an SM, 39.4
-// with 4, 35.3 with 8 (and so fewer registers), 34.5 with 13 words.
-struct Repitch {
-  const unsigned short *from;
-  unsigned short *to;
-  int64_t from_row, from_mat, to_row;
-  uint32_t rows, lines, parts;         // rows of a matrix, of all, and parts of 2048 elements of a row
-  int inner;
-};
-struct RepitchTwo { Repitch job[2]; };
-constexpr int kPart = 2048;
-
-__global__ void __launch_bounds__(256, 6) repitch_kernel(const __grid_constant__ RepitchTwo two) {
-  const Repitch &p = two.job[blockIdx.y];
-  const int lane = threadIdx.x % 32;
-  const uint64_t all = (uint64_t)p.lines * p.parts;
-  for (uint64_t v = (uint64_t)blockIdx.x * 8 + threadIdx.x / 32; v < all; v += (uint64_t)gridDim.x * 8) {
-    const uint32_t line = p.parts == 1 ? (uint32_t)v : (uint32_t)(v / p.parts);
-    const int first = p.parts == 1 ? 0 : (int)(v - (uint64_t)line * p.parts) * kPart;
-    const uint32_t mat = line / p.rows;
-    const unsigned short *from = p.from + mat * p.from_mat + (int64_t)(line - mat * p.rows) * p.from_row;
-    uint32_t *to = reinterpret_cast<uint32_t *>(p.to + line * p.to_row);
-    const int count = min(p.inner - first, kPart);
-    // aligned words: a row that starts in the middle of one gets its pairs from two
-    // neighbouring words (the halves that belong to neither row nor part stay unused;
-    // they share their word with an element, so they can be read)
-    const unsigned short *start = from + first;
-    const int off = (int)((uintptr_t)start >> 1 & 1);
-    const uint32_t *words = reinterpret_cast<const uint32_t *>(start - off);
-    to += first / 2;
-    for (int j0 = 0; j0 * 2 < count; j0 += 256) {
-      uint32_t w[9];
-#pragma unroll
-      for (int i = 0; i < 9; ++i) {
-        const int j = j0 + i * 32 + lane;
-        w[i] = 2 * j - off < count && (i < 8 || lane == 0) ? __ldg(words + j) : 0;
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t down = __shfl_down_sync(0xffffffffu, w[i], 1), over = __shfl_sync(0xffffffffu, w[i + 1], 0);
-        const int j = j0 + i * 32 + lane;
-        if (2 * j < count) to[j] = off ? __funnelshift_r(w[i], lane == 31 ? over : down, 16) : w[i];
-      }
-    }
-  }
-}
-
-// An operand as it is, or its copy in the workspace.
-struct Operand {
-  const void *p;
-  int64_t rows, row, mats, mat;
-  int inner;
-};
-int64_t copy_bytes(const Operand &o) {
-  if (o.p && readable(o.p, o.rows, o.row, o.mats, o.mat)) return 0;
-  return (o.rows * o.mats * ((o.inner + 7) / 8 * 8) * 2 + 255) / 256 * 256;
-}
-int lay_out(Operand *ops, void *workspace, int64_t workspace_bytes, cudaStream_t st) {
-  RepitchTwo two{};
-  int n = 0;
-  int64_t at = 0, most = 0;
-  for (int i = 0; i < 2; ++i) {
-    Operand &o = ops[i];
-    const int64_t bytes = copy_bytes(o);
-    if (!bytes) continue;
-    if (!workspace || (uintptr_t)workspace % 256 != 0 || workspace_bytes < at + bytes)
-      return set_error(OZ_ERR_INVALID,
-                       "an operand off the 16-byte boundaries needs a workspace of %lld bytes (256-byte "
-                       "aligned), got %lld at %p",
-                       (long long)(at + bytes), (long long)workspace_bytes, workspace);
-    if ((uintptr_t)o.p % 2 != 0) return set_error(OZ_ERR_INVALID, "an operand is not aligned to its elements");
-    unsigned char *to = static_cast<unsigned char *>(workspace) + at;
-    const int64_t pitch = (o.inner + 7) / 8 * 8;
-    const int64_t parts = (o.inner + kPart - 1) / kPart;
-    if (o.rows * o.mats > INT32_MAX) return set_error(OZ_ERR_INVALID, "size out of range");
-    two.job[n++] = Repitch{static_cast<const unsigned short *>(o.p), reinterpret_cast<unsigned short *>(to), o.row,
-                           o.mat, pitch, (uint32_t)o.rows, (uint32_t)(o.rows * o.mats), (uint32_t)parts, o.inner};
-    o.p = to;
-    o.row = pitch;
-    o.mat = pitch * o.rows;
-    at += bytes;
-    most = max(most, (o.rows * o.mats * parts + 7) / 8);
-  }
-  if (!n) return OZ_OK;
-  count_launch();
-  repitch_kernel<<<dim3((unsigned)min(most, (int64_t)sm_count() * 16), n), 256, 0, st>>>(two);
-  return check_cuda(cudaGetLastError(), "repitch_kernel launch");
-}
-
 template <class J>
 int run(const CUtensorMap &a, const CUtensorMap &b, GroupedParams p, int64_t row_tiles, int64_t n_side,
         int n_per_tile, cudaStream_t st, const char *what) {
@@ -478,7 +373,7 @@ extern "C" int oz_grouped_matmul(const oz_grouped_args *args, void *stream) {
     return set_error(OZ_ERR_INVALID, "w must have a unit stride along k or n");
   Operand ops[2] = {{x, rows, x_sr, 1, 0, (int)k},
                     {w, across ? k : n, across ? w_sk : w_sn, groups, w_se, (int)(across ? n : k)}};
-  if (int rc = lay_out(ops, workspace, workspace_bytes, st)) return rc;
+  if (int rc = lay_out(ops, 2, workspace, workspace_bytes, st)) return rc;
   GroupedParams p{offsets, y, ldy, offsets_64, groups, (int)rows, (int)k, (int)n, 0,
                   (uintptr_t)y % 16 == 0 && ldy * es % 16 == 0, tile::instruction(dtype)};
   if (out_dtype == OZ_F32) return grouped<float>(ops[0].p, ops[1].p, ops[0].row, ops[1].mat, across, ops[1].row, p, st);
@@ -500,7 +395,7 @@ extern "C" int oz_grouped_wgrad(const oz_grouped_wgrad_args *args, void *stream)
     return check_cuda(cudaMemsetAsync(dw, 0, (size_t)(groups * k * n * es), st), "cudaMemsetAsync");
   if (!offsets || !x || !dy) return set_error(OZ_ERR_INVALID, "null pointer");
   Operand ops[2] = {{x, rows, x_sr, 1, 0, (int)k}, {dy, rows, dy_sr, 1, 0, (int)n}};
-  if (int rc = lay_out(ops, workspace, workspace_bytes, st)) return rc;
+  if (int rc = lay_out(ops, 2, workspace, workspace_bytes, st)) return rc;
   GroupedParams p{offsets, dw, n, offsets_64, groups, (int)rows, (int)k, (int)n, 0,
                   (uintptr_t)dw % 16 == 0 && n * es % 16 == 0, tile::instruction(dtype)};
   if (out_dtype == OZ_F32) return wgrad<float>(ops[0].p, ops[1].p, ops[0].row, ops[1].row, p, st);

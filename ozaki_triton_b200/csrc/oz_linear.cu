@@ -1,0 +1,432 @@
+// oz_linear.cu -- a product with what follows it, and its gradients:
+//
+//   u  = x w + bias,  y = act(u) + residual
+//   du = dy act'(u),  dx = du w^T,  dw = x^T du,  dbias = sum of du's rows
+//
+// The products run on the tile engine (oz_tile.cuh), their epilogues read the
+// accumulators from tensor memory and write y (and u, rounded, for the backward
+// pass).  Operands are fp16 or bf16, sums fp32; bias, activation and residual are
+// applied in fp32 and rounded once.  du is rounded to the operands' type before
+// it is multiplied, its sum is not.
+
+#include <cmath>
+
+#include "oz_operands.cuh"
+#include "oz_stream.cuh"
+
+namespace oz {
+int status_linear(int *value, bool clear) { return read_status_word(value, clear); }
+
+namespace {
+using namespace tile;
+using stream::from_f32;
+using stream::to_f32;
+
+// ---------------------------------------------------------------------------
+// activations
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ float activated(float u, int act) {
+  switch (act) {
+    case OZ_ACT_RELU: return u > 0.f ? u : u != u ? u : 0.f;
+    case OZ_ACT_GELU: return u * normcdff(u);
+    case OZ_ACT_SILU: return u / (1.f + expf(-u));
+    default: return u;
+  }
+}
+// The same as a call, for epilogues whose columns are in registers and so not in a loop.
+__device__ __noinline__ float activated_call(float u, int act) { return activated(u, act); }
+__device__ __forceinline__ float slope(float u, int act) {
+  switch (act) {
+    case OZ_ACT_RELU: return u > 0.f ? 1.f : u != u ? u : 0.f;
+    case OZ_ACT_GELU: return normcdff(u) + u * (0.3989422804014327f * expf(-0.5f * u * u));
+    case OZ_ACT_SILU: {
+      const float s = 1.f / (1.f + expf(-u));
+      return s * (1.f + u * (1.f - s));
+    }
+    default: return 1.f;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// products
+// ---------------------------------------------------------------------------
+struct LinearParams {
+  void *out, *pre;
+  const void *bias, *residual;
+  int64_t ld, residual_ld;
+  int rows, k, n;              // of the result, and the contraction
+  int row_tiles, column_tiles;
+  int vectors;                 // rows of out and pre may be written 16 bytes at a time
+  int bias_f32, act;
+  uint32_t idesc;
+};
+
+template <typename O> __device__ __forceinline__ float bias_at(const LinearParams &p, int64_t c) {
+  // the bias has the operands' type, which is the result's unless that is fp32
+  if (p.bias_f32) return __ldg(static_cast<const float *>(p.bias) + c);
+  return to_f32(__ldg(static_cast<const O *>(p.bias) + c));
+}
+
+struct OutTile { int row, column; };
+
+// A warp's accumulators plus bias: u.
+template <typename O, typename B, class Source> struct WithBias {
+  const Source &source;
+  const LinearParams &p;
+  int64_t column;
+  __device__ __forceinline__ void read(int c, float (&v)[16]) const {
+    source.read(c, v);
+    if (!p.bias) return;
+#pragma unroll
+    for (int x = 0; x < 16; ++x)
+      if (column + c + x < p.n) v[x] += bias_at<B>(p, column + c + x);
+  }
+};
+// act(u) + residual, a lane's row of it.
+template <typename O, class Source> struct Finished {
+  const Source &source;
+  const LinearParams &p;
+  const O *residual;           // this lane's row from the warp's first column on, or none
+  int64_t columns;
+  __device__ __forceinline__ void read(int c, float (&v)[16]) const {
+    source.read(c, v);
+    if (p.act)
+#pragma unroll
+      for (int x = 0; x < 16; ++x) v[x] = sizeof(O) == 4 ? activated_call(v[x], p.act) : activated(v[x], p.act);
+    if (!residual) return;
+#pragma unroll
+    for (int x = 0; x < 16; ++x)
+      if (c + x < columns) v[x] += to_f32(__ldg(residual + c + x));
+  }
+};
+
+// A along the result's rows, B along its columns.
+template <typename O, typename B, int PAIR_, int NT_, bool AMN_, bool BMN_, bool PLAIN> struct LinearJob : NoLookAhead {
+  static constexpr int PAIR = PAIR_, NT = NT_, PLANES = 1, PASS = sizeof(O) == 4 ? 8 : 0;
+  static constexpr bool AMN = AMN_, BMN = BMN_, RAGGED = false;
+  using Params = LinearParams;
+  using Extra = OutTile;
+  static __device__ int plane_stride(const Params &) { return 0; }
+  struct Walk {
+    __device__ Walk(const Params &) {}
+    // 8 row tiles at a time sweep the columns: their operands stay in L2
+    __device__ bool find(const Params &p, int i, TileOf<Extra> &t) {
+      if (i >= p.row_tiles * p.column_tiles) return false;
+      const int sweep = i / (8 * p.column_tiles), in = i - sweep * 8 * p.column_tiles;
+      const int size = min(p.row_tiles - sweep * 8, 8);
+      t.a_row = (sweep * 8 + in % size) * kRows * PAIR;
+      t.b_row = in / size * NT;
+      t.a_mat = t.b_mat = 0;
+      t.k_begin = 0;
+      t.k_len = p.k;
+      t.extra = OutTile{t.a_row, t.b_row};
+      return true;
+    }
+  };
+  template <class Source>
+  static __device__ void epilogue(const Params &p, const TileOf<Extra> &t, const Source &source, int row, int column,
+                                  unsigned char *mine, Ahead &) {
+    const int64_t r0 = t.extra.row + row, c0 = t.extra.column + column;
+    const int rows = (int)(p.rows - r0);
+    O *out = static_cast<O *>(p.out) + r0 * p.ld + c0;
+    if constexpr (PLAIN) {
+      write_rows<O, NT / 2>(source, mine, out, p.ld, rows, p.n - c0, p.vectors);
+    } else {
+      constexpr int UNROLL = PASS ? NT / 2 : 1;
+      const WithBias<O, B, Source> u{source, p, c0};
+      if (p.pre) write_rows<B, NT / 2, UNROLL>(u, mine, static_cast<B *>(p.pre) + r0 * p.ld + c0, p.ld, rows, p.n - c0, p.vectors);
+      const int lane = threadIdx.x % 32;
+      const O *residual = p.residual && lane < rows
+                              ? static_cast<const O *>(p.residual) + (r0 + lane) * p.residual_ld + c0 : nullptr;
+      write_rows<O, NT / 2, UNROLL>(Finished<O, WithBias<O, B, Source>>{u, p, residual, p.n - c0}, mine, out, p.ld, rows,
+                            p.n - c0, p.vectors);
+    }
+  }
+  static __device__ void finish(const Params &, int, int) {}
+};
+
+// Two operands: rows of A along the result's rows, rows of B along its columns, each
+// `mn` (stored across the contraction) or along it, with its row pitch.
+struct Side {
+  const void *p;
+  int64_t pitch;               // elements
+  bool mn;
+};
+
+template <class J>
+int run_job(const Side &a, const Side &b, LinearParams p, cudaStream_t st, const char *what) {
+  CUtensorMap ta, tb;
+  const int64_t ai = J::AMN ? p.rows : p.k, ar = J::AMN ? p.k : p.rows;
+  const int64_t bi = J::BMN ? p.n : p.k, br = J::BMN ? p.k : p.n;
+  const int64_t ap = pitch_bytes(a.pitch, ar, ai), bp = pitch_bytes(b.pitch, br, bi);
+  if (int rc = make_map(&ta, a.p, ai, ar, 1, ap, ap, J::AMN ? kBlock : kRows)) return rc;
+  if (int rc = make_map(&tb, b.p, bi, br, 1, bp, bp, J::BMN ? kBlock : J::NT / J::PAIR)) return rc;
+  const int64_t rows = (p.rows + kRows * J::PAIR - 1) / (kRows * J::PAIR), columns = (p.n + J::NT - 1) / J::NT;
+  if (rows * columns > INT32_MAX / 2) return set_error(OZ_ERR_INVALID, "too many tiles");
+  p.row_tiles = (int)rows;
+  p.column_tiles = (int)columns;
+  return launch<J>(ta, tb, p, rows * columns, st, what);
+}
+
+template <typename O, typename B, bool PLAIN>
+int product(const Side &a, const Side &b, const LinearParams &p, cudaStream_t st, const char *what) {
+  const bool pair = p.rows > kRows && p.n > 128;
+  if (a.mn) {
+    if constexpr (PLAIN)
+      return pair ? run_job<LinearJob<O, B, 2, 256, true, true, true>>(a, b, p, st, what)
+                  : run_job<LinearJob<O, B, 1, 128, true, true, true>>(a, b, p, st, what);
+    return set_error(OZ_ERR_UNSUPPORTED, "operand layout");
+  }
+  if (b.mn)
+    return pair ? run_job<LinearJob<O, B, 2, 256, false, true, PLAIN>>(a, b, p, st, what)
+                : run_job<LinearJob<O, B, 1, 128, false, true, PLAIN>>(a, b, p, st, what);
+  return pair ? run_job<LinearJob<O, B, 2, 256, false, false, PLAIN>>(a, b, p, st, what)
+              : run_job<LinearJob<O, B, 1, 128, false, false, PLAIN>>(a, b, p, st, what);
+}
+
+template <bool PLAIN>
+int product_of(int dtype, int out_dtype, const Side &a, const Side &b, const LinearParams &p, cudaStream_t st,
+               const char *what) {
+  if (dtype == OZ_F16)
+    return out_dtype == OZ_F32 ? product<float, __half, PLAIN>(a, b, p, st, what)
+                               : product<__half, __half, PLAIN>(a, b, p, st, what);
+  return out_dtype == OZ_F32 ? product<float, __nv_bfloat16, PLAIN>(a, b, p, st, what)
+                             : product<__nv_bfloat16, __nv_bfloat16, PLAIN>(a, b, p, st, what);
+}
+
+// ---------------------------------------------------------------------------
+// du = dy act'(u) and the sums of its columns
+// ---------------------------------------------------------------------------
+struct SlopeParams {
+  const void *dy, *pre;
+  void *du;                    // may be none (no activation)
+  float *sums;                 // a row for each block row; none: no sums
+  int64_t dy_sr, pre_sr, du_sr;
+  int64_t rows;
+  int n, act, per;             // rows of a block
+};
+
+constexpr int kSlopeRows = 8;  // rows of a block's pass, a warp each
+
+// 32 lanes take 32 V columns of a row, 4 rows of a warp on their way at a time.
+template <typename T, int V> __global__ void __launch_bounds__(256) slope_kernel(const SlopeParams p) {
+  __shared__ float part[kSlopeRows][32 * V];
+  stream::start_after_earlier_kernels();
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int c = (blockIdx.x * 32 + lane) * V;
+  const int64_t r0 = (int64_t)blockIdx.y * p.per, r1 = min(r0 + p.per, p.rows);
+  float sum[V] = {};
+  if (c < p.n) {
+    for (int64_t r = r0 + warp; r < r1; r += 4 * kSlopeRows) {
+      float dy[4][V], u[4][V];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int64_t at = r + q * kSlopeRows;
+        if (at >= r1) continue;
+        stream::Run<T, V>::load(static_cast<const T *>(p.dy) + at * p.dy_sr + c, dy[q]);
+        if (p.pre) stream::Run<T, V>::load(static_cast<const T *>(p.pre) + at * p.pre_sr + c, u[q]);
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int64_t at = r + q * kSlopeRows;
+        if (at >= r1) continue;
+        if (p.pre)
+#pragma unroll
+          for (int x = 0; x < V; ++x) dy[q][x] *= slope(u[q][x], p.act);
+#pragma unroll
+        for (int x = 0; x < V; ++x) sum[x] += dy[q][x];
+        if (p.du) stream::Run<T, V>::store(static_cast<T *>(p.du) + at * p.du_sr + c, dy[q]);
+      }
+    }
+  }
+  if (!p.sums) return;
+#pragma unroll
+  for (int x = 0; x < V; ++x) part[warp][lane * V + x] = sum[x];
+  __syncthreads();
+  for (int i = threadIdx.x; i < 32 * V; i += 256) {
+    const int column = blockIdx.x * 32 * V + i;
+    if (column >= p.n) continue;
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < kSlopeRows; ++w) s += part[w][i];
+    p.sums[(int64_t)blockIdx.y * p.n + column] = s;
+  }
+}
+
+__global__ void __launch_bounds__(256) sums_kernel(const float *sums, float *out, int rows, int n) {
+  stream::start_after_earlier_kernels();
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= n) return;
+  double s = 0;
+#pragma unroll 8
+  for (int r = 0; r < rows; ++r) s += __ldg(sums + (int64_t)r * n + c);
+  out[c] = (float)s;
+}
+
+int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
+
+// Rows of a block of slope_kernel: as many blocks as keep the GPU's memory busy.
+int slope_rows(int64_t rows, int n) {
+  const int64_t columns = (n + 255) / 256;
+  const int64_t want = std::max<int64_t>(1, stream::sm_count() * 8 / columns);
+  const int64_t per = std::max<int64_t>(64, (rows + want - 1) / want);
+  return (int)((per + 31) / 32 * 32);
+}
+
+int check_linear(int dtype, int out_dtype, int act, int64_t rows, int64_t k, int64_t n) {
+  if (dtype != OZ_F16 && dtype != OZ_BF16)
+    return set_error(OZ_ERR_UNSUPPORTED, "unsupported operand dtype %d (fp16 or bf16)", dtype);
+  if (out_dtype != dtype && out_dtype != OZ_F32)
+    return set_error(OZ_ERR_UNSUPPORTED, "unsupported output dtype %d", out_dtype);
+  if (act < OZ_ACT_NONE || act > OZ_ACT_SILU) return set_error(OZ_ERR_UNSUPPORTED, "unsupported activation %d", act);
+  if (rows < 0 || k < 0 || n < 0) return set_error(OZ_ERR_INVALID, "negative size");
+  if (rows > (1 << 30) || k > (1 << 30) || n > (1 << 30)) return set_error(OZ_ERR_INVALID, "size out of range");
+  return OZ_OK;
+}
+
+// A weight (k, n) as an operand: stored across its rows' dimension or along it.
+bool stored_across(int64_t n, int64_t w_sk, int64_t w_sn) { return w_sn == 1 || (n == 1 && w_sk != 1); }
+
+// y of an empty contraction: the epilogue on zeros.
+template <typename O, typename B> __global__ void __launch_bounds__(256) empty_kernel(const LinearParams p) {
+  stream::start_after_earlier_kernels();
+  const int64_t end = (int64_t)p.rows * p.n;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < end; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / p.n, c = i - r * p.n;
+    const float u = p.bias ? bias_at<B>(p, c) : 0.f;
+    if (p.pre) static_cast<B *>(p.pre)[r * p.ld + c] = from_f32<B>(u);
+    float y = activated(u, p.act);
+    if (p.residual) y += to_f32(static_cast<const O *>(p.residual)[r * p.residual_ld + c]);
+    static_cast<O *>(p.out)[r * p.ld + c] = from_f32<O>(y);
+  }
+}
+
+}  // namespace
+}  // namespace oz
+
+extern "C" int oz_linear(const oz_linear_args *args, void *stream) {
+  if (!args) return oz::set_error(OZ_ERR_INVALID, "null arguments");
+  using namespace oz;
+  const oz_linear_args &a = *args;
+  if (int rc = check_linear(a.dtype, a.out_dtype, a.act, a.rows, a.k, a.n)) return rc;
+  if (a.bias && a.bias_dtype != a.dtype && a.bias_dtype != OZ_F32)
+    return set_error(OZ_ERR_UNSUPPORTED, "unsupported bias dtype %d", a.bias_dtype);
+  if (a.rows == 0 || a.n == 0) return OZ_OK;
+  if (!a.y) return set_error(OZ_ERR_INVALID, "null pointer");
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const int es = dtype_size(a.out_dtype);
+  LinearParams p{a.y, a.pre, a.bias, a.residual, a.n, a.residual_sr, (int)a.rows, (int)a.k, (int)a.n, 0, 0,
+                 (uintptr_t)a.y % 16 == 0 && a.n * es % 16 == 0 &&
+                     (!a.pre || ((uintptr_t)a.pre % 16 == 0 && a.n * 2 % 16 == 0)),
+                 a.bias_dtype == OZ_F32, a.act, tile::instruction(a.dtype)};
+  if (a.k == 0) {
+    const dim3 grid((unsigned)std::min<int64_t>((a.rows * a.n + 255) / 256, stream::sm_count() * 8));
+    const char *what = "empty product launch";
+    if (a.dtype == OZ_F16)
+      return a.out_dtype == OZ_F32 ? stream::launch(empty_kernel<float, __half>, grid, 256, 0, st, what, p)
+                                   : stream::launch(empty_kernel<__half, __half>, grid, 256, 0, st, what, p);
+    return a.out_dtype == OZ_F32 ? stream::launch(empty_kernel<float, __nv_bfloat16>, grid, 256, 0, st, what, p)
+                                 : stream::launch(empty_kernel<__nv_bfloat16, __nv_bfloat16>, grid, 256, 0, st, what, p);
+  }
+  if (!a.x || !a.w) return set_error(OZ_ERR_INVALID, "null pointer");
+  const bool across = stored_across(a.n, a.w_sk, a.w_sn);
+  if (!across && a.w_sk != 1 && a.k != 1) return set_error(OZ_ERR_INVALID, "w must have a unit stride along k or n");
+  Operand ops[2] = {{a.x, a.rows, a.x_sr, 1, 0, (int)a.k},
+                    {a.w, across ? a.k : a.n, across ? a.w_sk : a.w_sn, 1, 0, (int)(across ? a.n : a.k)}};
+  if (int rc = lay_out(ops, 2, a.workspace, a.workspace_bytes, st)) return rc;
+  return product_of<false>(a.dtype, a.out_dtype, Side{ops[0].p, ops[0].row, false}, Side{ops[1].p, ops[1].row, across}, p,
+                           st, "product launch");
+}
+
+// Workspace of the backward pass beside the operands' copies: du and partial sums.
+extern "C" int64_t oz_linear_backward_workspace_bytes(int64_t rows, int64_t n, int32_t act, int32_t sums) {
+  using namespace oz;
+  if (rows < 0 || n < 0) return OZ_ERR_INVALID;
+  if (rows == 0 || n == 0) return 0;
+  const int64_t blocks = (rows + slope_rows(rows, (int)n) - 1) / slope_rows(rows, (int)n);
+  return (act ? align256(rows * ((n + 7) / 8 * 8) * 2) : 0) + (sums && blocks > 1 ? align256(blocks * n * 4) : 0);
+}
+
+extern "C" int oz_linear_backward(const oz_linear_backward_args *args, void *stream) {
+  if (!args) return oz::set_error(OZ_ERR_INVALID, "null arguments");
+  using namespace oz;
+  const oz_linear_backward_args &a = *args;
+  if (int rc = check_linear(a.dtype, a.dw_dtype, a.act, a.rows, a.k, a.n)) return rc;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const int dw_size = dtype_size(a.dw_dtype);
+  if (a.rows == 0 || a.n == 0) {
+    if (a.dx && a.rows * a.k)
+      if (int rc = check_cuda(cudaMemsetAsync(a.dx, 0, (size_t)(a.rows * a.k * 2), st), "cudaMemsetAsync")) return rc;
+    if (a.dw && a.k * a.n)
+      if (int rc = check_cuda(cudaMemsetAsync(a.dw, 0, (size_t)(a.k * a.n * dw_size), st), "cudaMemsetAsync")) return rc;
+    if (a.db && a.n) return check_cuda(cudaMemsetAsync(a.db, 0, (size_t)(a.n * 4), st), "cudaMemsetAsync");
+    return OZ_OK;
+  }
+  if (!a.dy || (a.act && !a.pre)) return set_error(OZ_ERR_INVALID, "null pointer");
+  const bool want_x = a.dx && a.k > 0, want_w = a.dw && a.k > 0;
+  if ((want_x && !a.w) || (want_w && !a.x)) return set_error(OZ_ERR_INVALID, "null pointer");
+  const int64_t own = oz_linear_backward_workspace_bytes(a.rows, a.n, a.act, a.db != nullptr);
+  if (own && (!a.workspace || (uintptr_t)a.workspace % 256 != 0 || a.workspace_bytes < own))
+    return set_error(OZ_ERR_INVALID, "workspace of %lld bytes (256-byte aligned) needed, got %lld at %p", (long long)own,
+                     (long long)a.workspace_bytes, a.workspace);
+  unsigned char *space = static_cast<unsigned char *>(a.workspace);
+  const int per = slope_rows(a.rows, (int)a.n);
+  const int64_t blocks = (a.rows + per - 1) / per;
+  Operand du{a.dy, a.rows, a.dy_sr, 1, 0, (int)a.n};
+  if (a.act || a.db) {
+    const int64_t pitch = (a.n + 7) / 8 * 8;
+    void *out = a.act ? space : nullptr;
+    float *sums = !a.db ? nullptr : blocks == 1 ? a.db
+                  : reinterpret_cast<float *>(space + (a.act ? align256(a.rows * pitch * 2) : 0));
+    const SlopeParams s{a.dy, a.act ? a.pre : nullptr, out, sums, a.dy_sr, a.pre_sr, pitch, a.rows, (int)a.n, a.act, per};
+    auto fits = [&](const void *base, int64_t sr) { return !base || ((uintptr_t)base % 16 == 0 && (a.rows == 1 || sr % 8 == 0)); };
+    const bool wide = fits(s.dy, s.dy_sr) && fits(s.pre, s.pre_sr) && a.n % 8 == 0;
+    const int v = wide ? 8 : 1;
+    if (blocks > 65535) return set_error(OZ_ERR_INVALID, "size out of range");
+    const dim3 grid((unsigned)((a.n + 32 * v - 1) / (32 * v)), (unsigned)blocks);
+    const char *what = "slope_kernel launch";
+    int rc;
+    if (a.dtype == OZ_F16)
+      rc = wide ? stream::launch(slope_kernel<__half, 8>, grid, 256, 0, st, what, s)
+                : stream::launch(slope_kernel<__half, 1>, grid, 256, 0, st, what, s);
+    else
+      rc = wide ? stream::launch(slope_kernel<__nv_bfloat16, 8>, grid, 256, 0, st, what, s)
+                : stream::launch(slope_kernel<__nv_bfloat16, 1>, grid, 256, 0, st, what, s);
+    if (rc) return rc;
+    if (a.db && blocks > 1) {
+      rc = stream::launch(sums_kernel, dim3((unsigned)((a.n + 255) / 256)), 256, 0, st, "sums_kernel launch",
+                          (const float *)sums, a.db, (int)blocks, (int)a.n);
+      if (rc) return rc;
+    }
+    if (a.act) {
+      du.p = out;
+      du.row = pitch;
+    }
+  }
+  if (!want_x && !want_w) return OZ_OK;
+  const bool across = stored_across(a.n, a.w_sk, a.w_sn);
+  if (want_x && !across && a.w_sk != 1 && a.k != 1)
+    return set_error(OZ_ERR_INVALID, "w must have a unit stride along k or n");
+  Operand ops[3] = {du};
+  int count = 1, at_w = 0, at_x = 0;
+  if (want_x) {
+    ops[at_w = count++] = Operand{a.w, across ? a.k : a.n, across ? a.w_sk : a.w_sn, 1, 0, (int)(across ? a.n : a.k)};
+  }
+  if (want_w) ops[at_x = count++] = Operand{a.x, a.rows, a.x_sr, 1, 0, (int)a.k};
+  if (int rc = lay_out(ops, count, space + own, a.workspace_bytes - own, st)) return rc;
+  if (want_x) {
+    // dx (rows, k) = du (rows, n) w^T: w's rows along n where it is stored across
+    LinearParams p{a.dx, nullptr, nullptr, nullptr, a.k, 0, (int)a.rows, (int)a.n, (int)a.k, 0, 0,
+                   (uintptr_t)a.dx % 16 == 0 && a.k % 8 == 0, 0, OZ_ACT_NONE, tile::instruction(a.dtype)};
+    if (int rc = product_of<true>(a.dtype, a.dtype, Side{ops[0].p, ops[0].row, false},
+                                  Side{ops[at_w].p, ops[at_w].row, !across}, p, st, "dx launch"))
+      return rc;
+  }
+  if (want_w) {
+    LinearParams p{a.dw, nullptr, nullptr, nullptr, a.n, 0, (int)a.k, (int)a.rows, (int)a.n, 0, 0,
+                   (uintptr_t)a.dw % 16 == 0 && a.n * dw_size % 16 == 0, 0, OZ_ACT_NONE, tile::instruction(a.dtype)};
+    return product_of<true>(a.dtype, a.dw_dtype, Side{ops[at_x].p, ops[at_x].row, true},
+                            Side{ops[0].p, ops[0].row, true}, p, st, "dw launch");
+  }
+  return OZ_OK;
+}

@@ -1,0 +1,93 @@
+// oz_stream.cuh -- pieces of the kernels that stream through memory: elements
+// in 32 bits, 16 bytes of them at a time, and launches that overlap their start
+// with the end of the kernel before.
+#pragma once
+
+#include "oz_common.cuh"
+
+namespace oz {
+namespace stream {
+
+template <typename T> __device__ __forceinline__ float to_f32(T v);
+template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+template <typename T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// 16 bytes of T as fp32 values and back.
+template <typename T> __device__ __forceinline__ void unpack(const uint4 &u, float (&v)[16 / sizeof(T)]) {
+  const T *e = reinterpret_cast<const T *>(&u);
+#pragma unroll
+  for (int i = 0; i < (int)(16 / sizeof(T)); ++i) v[i] = to_f32(e[i]);
+}
+template <typename T> __device__ __forceinline__ uint4 pack(const float (&v)[16 / sizeof(T)]) {
+  uint4 u;
+  T *e = reinterpret_cast<T *>(&u);
+#pragma unroll
+  for (int i = 0; i < (int)(16 / sizeof(T)); ++i) e[i] = from_f32<T>(v[i]);
+  return u;
+}
+
+// V consecutive elements of T: 16 bytes, or one element where rows do not start
+// on 16-byte boundaries.  Read once (no use of them is left for L1).
+template <typename T, int V> struct Run {
+  static_assert(V == 1 || V * sizeof(T) == 16, "one element or 16 bytes");
+  static __device__ __forceinline__ void load(const T *p, float (&v)[V]) {
+    if constexpr (V == 1) v[0] = to_f32(*p);
+    else unpack<T>(__ldg(reinterpret_cast<const uint4 *>(p)), v);
+  }
+  static __device__ __forceinline__ void store(T *p, const float (&v)[V]) {
+    if constexpr (V == 1) *p = from_f32<T>(v[0]);
+    else *reinterpret_cast<uint4 *>(p) = pack<T>(v);
+  }
+};
+
+__device__ __forceinline__ void start_after_earlier_kernels() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+// A launch whose blocks may start while the kernel before ends; every kernel
+// launched so calls start_after_earlier_kernels() before it touches memory.
+template <typename... P, typename... A>
+int launch(void (*kernel)(P...), dim3 grid, int threads, int smem, cudaStream_t st, const char *what, A... args) {
+  if (smem > 48 * 1024)
+    if (int rc = set_smem_once((const void *)kernel, smem, what)) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  count_launch();
+  return check_cuda(cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...), what);
+}
+
+inline int sm_count() {
+  static const int n = [] {
+    int dev = 0, v = 0;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev);
+    return v > 0 ? v : 148;
+  }();
+  return n;
+}
+
+// Calls f with a value of the element type that `dtype` names.
+template <typename F> int with_type(int dtype, F f) {
+  if (dtype == OZ_F32) return f(float{});
+  if (dtype == OZ_F16) return f(__half{});
+  if (dtype == OZ_BF16) return f(__nv_bfloat16{});
+  return set_error(OZ_ERR_UNSUPPORTED, "unsupported dtype %d (fp32, fp16 or bf16)", dtype);
+}
+
+}  // namespace stream
+}  // namespace oz
