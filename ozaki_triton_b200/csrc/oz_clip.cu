@@ -20,6 +20,7 @@ using namespace stream;
 
 constexpr int kThreads = 256;
 constexpr int kPiece = 8192;          // elements of a block's turn
+constexpr int kAtOnce = 4;            // 16-byte loads of a thread on their way
 
 struct Tensor {
   const void *g;
@@ -39,78 +40,81 @@ struct Sums {
   float max_norm, eps;
 };
 
-template <int N> __device__ __forceinline__ const Tensor &tensor_of(const Table<N> &table, int piece) {
+// The pieces of this block, one after the other in memory, and the tensor of the first.
+struct Share { int first, end; };
+template <int N> __device__ __forceinline__ Share share_of(const Table<N> &table) {
+  return {(int)((int64_t)table.pieces * blockIdx.x / gridDim.x),
+          (int)((int64_t)table.pieces * (blockIdx.x + 1) / gridDim.x)};
+}
+template <int N> __device__ __forceinline__ int tensor_of(const Table<N> &table, int piece) {
   int low = 0, high = table.tensors - 1;      // the last tensor whose first piece is not after it
   while (low < high) {
     const int mid = (low + high + 1) / 2;
     if (table.t[mid].first <= piece) low = mid;
     else high = mid - 1;
   }
-  return table.t[low];
+  return low;
 }
 
-// Calls f(offset, values, how many) for this thread's elements of a piece: V at a time
-// with 4 loads on their way, or one by one.
-template <typename T, typename F>
-__device__ __forceinline__ void each_run(const T *g, int64_t n, bool runs, F f) {
-  constexpr int V = 16 / sizeof(T), AT_ONCE = 4;
-  if (runs) {
-    for (int64_t i0 = (int64_t)threadIdx.x * V; i0 < n; i0 += (int64_t)kThreads * V * AT_ONCE) {
-      uint4 u[AT_ONCE];
+template <typename T> __device__ __forceinline__ float squares(const uint4 &u) {
+  constexpr int V = 16 / sizeof(T);
+  float v[V], s = 0.f;
+  unpack<T>(u, v);
 #pragma unroll
-      for (int j = 0; j < AT_ONCE; ++j) {
-        const int64_t i = i0 + (int64_t)j * kThreads * V;
-        if (i + V <= n) u[j] = *reinterpret_cast<const uint4 *>(g + i);
-      }
+  for (int x = 0; x < V; ++x) s = fmaf(v[x], v[x], s);
+  return s;
+}
+// An element of a type known at run time.
+__device__ __forceinline__ float element(const void *g, int64_t i, int type) {
+  if (type == OZ_F32) return static_cast<const float *>(g)[i];
+  if (type == OZ_F16) return to_f32(static_cast<const __half *>(g)[i]);
+  return to_f32(static_cast<const __nv_bfloat16 *>(g)[i]);
+}
+__device__ __forceinline__ void set_element(void *out, int64_t i, int type, float v) {
+  if (type == OZ_F32) static_cast<float *>(out)[i] = v;
+  else if (type == OZ_F16) static_cast<__half *>(out)[i] = from_f32<__half>(v);
+  else static_cast<__nv_bfloat16 *>(out)[i] = from_f32<__nv_bfloat16>(v);
+}
+
+// Loads 16-byte runs j of [0, runs) of a piece kAtOnce at a time, calls f(run, bits).
+template <typename F> __device__ __forceinline__ void each_run(const uint4 *g, int runs, F f) {
+#pragma unroll 1
+  for (int i0 = threadIdx.x; i0 < runs; i0 += kThreads * kAtOnce) {
+    uint4 u[kAtOnce];
 #pragma unroll
-      for (int j = 0; j < AT_ONCE; ++j) {
-        const int64_t i = i0 + (int64_t)j * kThreads * V;
-        if (i + V <= n) {
-          float v[V];
-          unpack<T>(u[j], v);
-          f(i, v, V);
-        } else {
-          for (int64_t x = i; x < n; ++x) {
-            float v[V];
-            v[0] = to_f32(g[x]);
-            f(x, v, 1);
-          }
-        }
-      }
-    }
-  } else {
-    for (int64_t i = threadIdx.x; i < n; i += kThreads) {
-      float v[V];
-      v[0] = to_f32(g[i]);
-      f(i, v, 1);
-    }
+    for (int j = 0; j < kAtOnce; ++j)
+      if (i0 + j * kThreads < runs) u[j] = g[i0 + j * kThreads];
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j)
+      if (i0 + j * kThreads < runs) f(i0 + j * kThreads, u[j]);
   }
 }
 
-template <typename T> __device__ __forceinline__ float squares(const T *g, int64_t n, bool runs) {
-  float s = 0.f;
-  each_run<T>(g, n, runs, [&](int64_t, const auto &v, int m) {
-    if (m == 1) s = fmaf(v[0], v[0], s);
-    else
-#pragma unroll
-      for (int x = 0; x < (int)(16 / sizeof(T)); ++x) s = fmaf(v[x], v[x], s);
-  });
-  return s;
-}
-
 template <int N>
-__global__ void __launch_bounds__(kThreads) norm_kernel(const __grid_constant__ Table<N> table, double *partial) {
+__global__ void __launch_bounds__(kThreads, 6) norm_kernel(const __grid_constant__ Table<N> table, double *partial) {
   start_after_earlier_kernels();
   double all = 0;
-  for (int piece = blockIdx.x; piece < table.pieces; piece += gridDim.x) {
-    const Tensor &t = tensor_of(table, piece);
-    const int64_t at = (int64_t)(piece - t.first) * kPiece;
-    const int64_t n = min(t.n - at, (int64_t)kPiece);
-    const int type = t.types & 15;
-    const bool runs = t.types >> 8 & 1;
-    if (type == OZ_F32) all += squares(static_cast<const float *>(t.g) + at, n, runs);
-    else if (type == OZ_F16) all += squares(static_cast<const __half *>(t.g) + at, n, runs);
-    else all += squares(static_cast<const __nv_bfloat16 *>(t.g) + at, n, runs);
+  const Share share = share_of(table);
+  int at = tensor_of(table, share.first);
+  for (int piece = share.first; piece < share.end; ++piece) {
+    while (at + 1 < table.tensors && table.t[at + 1].first <= piece) ++at;
+    const Tensor &t = table.t[at];
+    const int64_t from = (int64_t)(piece - t.first) * kPiece;
+    const int n = (int)min(t.n - from, (int64_t)kPiece), type = t.types & 15, es = type == OZ_F32 ? 4 : 2;
+    const char *g = static_cast<const char *>(t.g) + from * es;
+    const int runs = t.types >> 8 & 1 ? n * es / 16 : 0;
+    float s = 0.f;
+    each_run(reinterpret_cast<const uint4 *>(g), runs, [&](int, const uint4 &u) {
+      if (type == OZ_F32) s += squares<float>(u);
+      else if (type == OZ_F16) s += squares<__half>(u);
+      else s += squares<__nv_bfloat16>(u);
+    });
+#pragma unroll 1
+    for (int i = runs * (16 / es) + threadIdx.x; i < n; i += kThreads) {
+      const float v = element(g, i, type);
+      s = fmaf(v, v, s);
+    }
+    all += s;
   }
   __shared__ double warp_sum[kThreads / 32];
 #pragma unroll
@@ -123,33 +127,29 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const __grid_constant__ 
   }
 }
 
-template <typename T, typename O>
-__device__ __forceinline__ void scaled(const T *g, O *out, int64_t n, bool runs, float scale) {
-  constexpr int V = 16 / sizeof(T), W = 16 / sizeof(O);
-  each_run<T>(g, n, runs, [&](int64_t i, const auto &v, int m) {
-    if (m == 1) {
-      out[i] = from_f32<O>(v[0] * scale);
-      return;
-    }
-    if constexpr (V >= W) {
+// A run of T, scaled, to run r of out (its size is V elements of O, 8 to 32 bytes).
+template <typename T, typename O> __device__ __forceinline__ void scaled(const uint4 &u, O *out, int r, float scale) {
+  constexpr int V = 16 / sizeof(T);
+  float v[V];
+  unpack<T>(u, v);
 #pragma unroll
-      for (int h = 0; h < V / W; ++h) {
-        float w[W];
+  for (int x = 0; x < V; ++x) v[x] *= scale;
+  out += (int64_t)r * V;
+  if constexpr (sizeof(O) == sizeof(T)) {
+    __stcs(reinterpret_cast<uint4 *>(out), pack<O>(v));
+  } else if constexpr (sizeof(O) == 4) {
+    __stcs(reinterpret_cast<float4 *>(out), make_float4(v[0], v[1], v[2], v[3]));
+    __stcs(reinterpret_cast<float4 *>(out) + 1, make_float4(v[4], v[5], v[6], v[7]));
+  } else {
+    O w[V];
 #pragma unroll
-        for (int x = 0; x < W; ++x) w[x] = v[h * W + x] * scale;
-        *reinterpret_cast<uint4 *>(out + i + h * W) = pack<O>(w);
-      }
-    } else {                              // 4 fp32 values to 8 bytes
-      O w[V];
-#pragma unroll
-      for (int x = 0; x < V; ++x) w[x] = from_f32<O>(v[x] * scale);
-      *reinterpret_cast<uint2 *>(out + i) = *reinterpret_cast<const uint2 *>(w);
-    }
-  });
+    for (int x = 0; x < V; ++x) w[x] = from_f32<O>(v[x]);
+    __stcs(reinterpret_cast<uint2 *>(out), *reinterpret_cast<const uint2 *>(w));
+  }
 }
 
 template <int N>
-__global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__ Table<N> table, const Sums sums) {
+__global__ void __launch_bounds__(kThreads, 4) scale_kernel(const __grid_constant__ Table<N> table, const Sums sums) {
   __shared__ float shared_scale;
   __shared__ double warp_sum[kThreads / 32];
   start_after_earlier_kernels();
@@ -168,29 +168,39 @@ __global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__
   }
   __syncthreads();
   const float scale = shared_scale;
+  const Share share = share_of(table);
+  if (share.first >= share.end) return;
   // the pieces read last are the first here: some of them are still in L2
-  for (int piece = table.pieces - 1 - (int)blockIdx.x; piece >= 0; piece -= gridDim.x) {
-    const Tensor &t = tensor_of(table, piece);
-    const int64_t at = (int64_t)(piece - t.first) * kPiece;
-    const int64_t n = min(t.n - at, (int64_t)kPiece);
-    const int type = t.types & 15, to = t.types >> 4 & 15;
-    const bool runs = t.types >> 8 & 1;
-    auto from = [&](auto g0) {
-      using T = decltype(g0);
-      const T *g = static_cast<const T *>(t.g) + at;
-      if (to == OZ_F32) scaled(g, static_cast<float *>(t.out) + at, n, runs, scale);
-      else if (to == OZ_F16) scaled(g, static_cast<__half *>(t.out) + at, n, runs, scale);
-      else scaled(g, static_cast<__nv_bfloat16 *>(t.out) + at, n, runs, scale);
-    };
-    if (type == OZ_F32) from(float{});
-    else if (type == OZ_F16) from(__half{});
-    else from(__nv_bfloat16{});
+  int at = tensor_of(table, share.end - 1);
+  for (int piece = share.end - 1; piece >= share.first; --piece) {
+    while (table.t[at].first > piece) --at;
+    const Tensor &t = table.t[at];
+    const int64_t from = (int64_t)(piece - t.first) * kPiece;
+    const int n = (int)min(t.n - from, (int64_t)kPiece), type = t.types & 15, to = t.types >> 4 & 15;
+    const int es = type == OZ_F32 ? 4 : 2, os = to == OZ_F32 ? 4 : 2;
+    const char *g = static_cast<const char *>(t.g) + from * es;
+    char *out = static_cast<char *>(t.out) + from * os;
+    const int runs = t.types >> 8 & 1 ? n * es / 16 : 0;
+    each_run(reinterpret_cast<const uint4 *>(g), runs, [&](int r, const uint4 &u) {
+      auto run = [&](auto g0) {
+        using T = decltype(g0);
+        if (to == OZ_F32) scaled<T>(u, reinterpret_cast<float *>(out), r, scale);
+        else if (to == OZ_F16) scaled<T>(u, reinterpret_cast<__half *>(out), r, scale);
+        else scaled<T>(u, reinterpret_cast<__nv_bfloat16 *>(out), r, scale);
+      };
+      if (type == OZ_F32) run(float{});
+      else if (type == OZ_F16) run(__half{});
+      else run(__nv_bfloat16{});
+    });
+#pragma unroll 1
+    for (int i = runs * (16 / es) + threadIdx.x; i < n; i += kThreads)
+      set_element(out, i, to, element(g, i, type) * scale);
   }
 }
 
 // A launch takes the addresses of at most this many tensors as arguments.
 constexpr int kFew = 64, kMany = 640;
-constexpr int kBlocksPerSm = 4;
+constexpr int kBlocksPerSm = 6;
 
 int sum_blocks(int64_t pieces) { return (int)std::min<int64_t>(pieces, (int64_t)sm_count() * kBlocksPerSm); }
 

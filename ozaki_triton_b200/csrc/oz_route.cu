@@ -15,6 +15,7 @@
 // Softmax and all sums are in fp32 (the sums over tokens of all blocks in
 // fp64); results do not depend on the order in which blocks run.
 
+#include <algorithm>
 #include <cmath>
 
 #include "oz_stream.cuh"
@@ -510,7 +511,7 @@ struct RowsParams {
   const float *weights;
   float *dweights;
   int64_t tokens, row_count, x_row, rows_row;   // row pitches of the inputs
-  int d, k, experts, parts;    // parts: blocks or groups of threads a token
+  int d, k, experts;
 };
 
 // A slot that is a row, else -1.
@@ -529,129 +530,172 @@ template <typename T, int V> __device__ __forceinline__ void clear_rest(const Ro
     Run<T, V>::store(static_cast<T *>(p.rows_out) + i * V, zero);
 }
 
-// The token and the first column of this thread: `parts` blocks a token, or
-// 1 / -parts of a block.
-template <int V> __device__ __forceinline__ bool place(const RowsParams &p, int64_t &t, int &c) {
-  if (p.parts > 0) {
-    t = blockIdx.x / p.parts;
-    c = ((int)(blockIdx.x - t * p.parts) * (int)blockDim.x + (int)threadIdx.x) * V;
-  } else {
-    const int each = (int)blockDim.x / -p.parts, g = (int)threadIdx.x / each;
-    t = (int64_t)blockIdx.x * -p.parts + g;
-    c = ((int)threadIdx.x - g * each) * V;
-    if (g >= -p.parts) return false;
-  }
-  return t < p.tokens && c < p.d;
-}
+// How the threads of a block lie over tokens and columns: `tokens` tokens side by side,
+// `threads` threads each, which take the columns in steps of threads * V.
+struct Spread { int tokens, threads; };
 
-template <typename T, int V> __global__ void __launch_bounds__(256) dispatch_kernel(const RowsParams p, int blocks) {
-  start_after_earlier_kernels();
-  if ((int)blockIdx.x >= blocks) return clear_rest<T, V>(p, blocks);
-  int64_t t;
-  int c;
-  if (!place<V>(p, t, c)) return;
-  float v[V];
-  Run<T, V>::load(static_cast<const T *>(p.x) + t * p.x_row + c, v);
-  T *to = static_cast<T *>(p.rows_out) + c;
-#pragma unroll 4
-  for (int j = 0; j < p.k; ++j) {
-    const int64_t s = slot_of(p, t * p.k + j);
-    if (s >= 0) Run<T, V>::store(to + s * p.d, v);
-  }
-}
-
-// y[t] = sum_j w rows[slot], in the order of j, 8 loads on their way at a time.
-template <typename T, int V> __global__ void __launch_bounds__(256) combine_kernel(const RowsParams p) {
-  start_after_earlier_kernels();
-  int64_t t;
-  int c;
-  if (!place<V>(p, t, c)) return;
-  float y[V] = {};
-  const T *from = static_cast<const T *>(p.rows) + c;
-  for (int j0 = 0; j0 < p.k; j0 += 8) {
-    float v[8][V], w[8];
+// The slots of a token's picks, -1 where there is no row, loaded ahead of the rows they name.
+template <int K> struct Picks {
+  int slot[K];
+  __device__ __forceinline__ void load(const RowsParams &p, int64_t t, int j0) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int64_t s = j0 + j < p.k ? slot_of(p, t * p.k + j0 + j) : -1;
-      w[j] = s < 0 ? 0.f : p.weights ? __ldg(p.weights + t * p.k + j0 + j) : 1.f;
-      if (s >= 0) Run<T, V>::load(from + s * p.rows_row, v[j]);
-      else
-#pragma unroll
-        for (int i = 0; i < V; ++i) v[j][i] = 0.f;
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-#pragma unroll
-      for (int i = 0; i < V; ++i) y[i] = fmaf(w[j], v[j][i], y[i]);
-  }
-  Run<T, V>::store(static_cast<T *>(p.x_out) + t * p.d + c, y);
-}
-
-// drows[slot] = w dy[t], dw[t, j] = dy[t] . rows[slot]: `parts` warps a token.
-template <typename T, int V>
-__global__ void __launch_bounds__(256) combine_backward_kernel(const RowsParams p, int blocks) {
-  __shared__ float sums[8][8];
-  start_after_earlier_kernels();
-  if ((int)blockIdx.x >= blocks) return clear_rest<T, V>(p, blocks);
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, in = warp % p.parts, each = 8 / p.parts;
-  const int64_t t = (int64_t)blockIdx.x * each + warp / p.parts;
-  for (int j0 = 0; j0 < p.k; j0 += 4) {
-    float dot[4] = {0.f, 0.f, 0.f, 0.f};
-    if (t < p.tokens) {
-      int64_t s[4];
-      float w[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        s[j] = j0 + j < p.k ? slot_of(p, t * p.k + j0 + j) : -1;
-        w[j] = s[j] >= 0 ? __ldg(p.weights + t * p.k + j0 + j) : 0.f;
+    for (int j = 0; j < K; ++j) {
+      slot[j] = -1;
+      if (t < p.tokens && j0 + j < p.k) {
+        const int s = __ldg(p.slots + t * p.k + j0 + j);
+        slot[j] = s >= 0 && s < p.row_count ? s : -1;
       }
-      for (int c = (in * 32 + lane) * V; c < p.d; c += p.parts * 32 * V) {
-        float dy[V], v[4][V];
-        Run<T, V>::load(static_cast<const T *>(p.x) + t * p.x_row + c, dy);
+    }
+  }
+};
+
+template <typename T, int V> __global__ void __launch_bounds__(256, 6) dispatch_kernel(const RowsParams p, const Spread at,
+                                                                                       int blocks) {
+  start_after_earlier_kernels();
+  if ((int)blockIdx.x >= blocks) return clear_rest<T, V>(p, blocks);
+  const int group = (int)threadIdx.x / at.threads, in = (int)threadIdx.x - group * at.threads;
+  if (group >= at.tokens) return;
+  for (int64_t t = (int64_t)blockIdx.x * at.tokens + group; t < p.tokens; t += (int64_t)blocks * at.tokens) {
+    for (int c = in * V; c < p.d; c += at.threads * V) {
+      const auto v = Raw<T, V>::load(static_cast<const T *>(p.x) + t * p.x_row + c);
+      T *to = static_cast<T *>(p.rows_out) + c;
+#pragma unroll 4
+      for (int j = 0; j < p.k; ++j) {
+        const int64_t s = slot_of(p, t * p.k + j);
+        if (s >= 0) Raw<T, V>::store(to + s * p.d, v);
+      }
+    }
+  }
+}
+
+// y[t] = sum_j w rows[slot], in the order of j, K loads on their way at a time; the next
+// token's slots are loaded before this one's rows arrive.
+template <typename T, int V, int K> __global__ void __launch_bounds__(256, K >= 8 ? 3 : K >= 4 ? 4 : 5) combine_kernel(
+    const RowsParams p, const Spread at) {
+  start_after_earlier_kernels();
+  const int group = (int)threadIdx.x / at.threads, in = (int)threadIdx.x - group * at.threads;
+  if (group >= at.tokens) return;
+  const int64_t step = (int64_t)gridDim.x * at.tokens;
+  int64_t t = (int64_t)blockIdx.x * at.tokens + group;
+  Picks<K> picks, next;
+  picks.load(p, t, 0);
+  for (; t < p.tokens; t += step) {
+    next.load(p, t + step, 0);
+#pragma unroll 1
+    for (int c = in * V; c < p.d; c += at.threads * V) {
+      const T *from = static_cast<const T *>(p.rows) + c;
+      float y[V] = {};
+#pragma unroll 1
+      for (int j0 = 0; j0 < p.k; j0 += K) {
+        if (p.k > K) picks.load(p, t, j0);
+        typename Raw<T, V>::Type v[K];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (s[j] >= 0) Run<T, V>::load(static_cast<const T *>(p.rows) + s[j] * p.rows_row + c, v[j]);
+        for (int j = 0; j < K; ++j)
+          if (picks.slot[j] >= 0) v[j] = Raw<T, V>::load(from + (int64_t)picks.slot[j] * p.rows_row);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (s[j] < 0) continue;
-          float out[V];
+        for (int j = 0; j < K; ++j)
+          if (picks.slot[j] >= 0) {
+            const float w = p.weights ? __ldg(p.weights + t * p.k + j0 + j) : 1.f;
+            float u[V];
+            Raw<T, V>::values(v[j], u);
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
-            dot[j] = fmaf(dy[i], v[j][i], dot[j]);
-            out[i] = w[j] * dy[i];
+            for (int i = 0; i < V; ++i) y[i] = fmaf(w, u[i], y[i]);
           }
-          Run<T, V>::store(static_cast<T *>(p.rows_out) + s[j] * p.d + c, out);
+      }
+      Run<T, V>::store(static_cast<T *>(p.x_out) + t * p.d + c, y);
+    }
+    picks = next;
+  }
+}
+
+// drows[slot] = w dy[t], dw[t, j] = dy[t] . rows[slot]: `at.threads` threads (whole warps) a
+// token, K picks at a time.
+template <typename T, int V, int K>
+__global__ void __launch_bounds__(256, 3) combine_backward_kernel(const RowsParams p, const Spread at, int blocks) {
+  __shared__ float sums[8][K];
+  start_after_earlier_kernels();
+  if ((int)blockIdx.x >= blocks) return clear_rest<T, V>(p, blocks);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, parts = at.threads / 32;
+  const int group = warp / parts, in = (int)threadIdx.x - group * at.threads;
+  const int64_t step = (int64_t)blocks * at.tokens;
+  int64_t t = (int64_t)blockIdx.x * at.tokens + group;
+  Picks<K> picks, next;
+  picks.load(p, t, 0);
+  // every warp takes part in every round: the sums are shared
+  for (int64_t t0 = (int64_t)blockIdx.x * at.tokens; t0 < p.tokens; t0 += step, t += step) {
+    next.load(p, t + step, 0);
+    for (int j0 = 0; j0 < p.k; j0 += K) {
+      if (j0) picks.load(p, t, j0);
+      float dot[K], weight[K];
+#pragma unroll
+      for (int j = 0; j < K; ++j) {
+        dot[j] = 0.f;
+        weight[j] = picks.slot[j] >= 0 ? __ldg(p.weights + t * p.k + j0 + j) : 0.f;
+      }
+      if (t < p.tokens) {
+        for (int c = in * V; c < p.d; c += at.threads * V) {
+          typename Raw<T, V>::Type v[K];
+          const auto raw = Raw<T, V>::load(static_cast<const T *>(p.x) + t * p.x_row + c);
+#pragma unroll
+          for (int j = 0; j < K; ++j)
+            if (picks.slot[j] >= 0)
+              v[j] = Raw<T, V>::load(static_cast<const T *>(p.rows) + (int64_t)picks.slot[j] * p.rows_row + c);
+          float dy[V];
+          Raw<T, V>::values(raw, dy);
+#pragma unroll
+          for (int j = 0; j < K; ++j) {
+            if (picks.slot[j] < 0) continue;
+            float u[V];
+            Raw<T, V>::values(v[j], u);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              dot[j] = fmaf(dy[i], u[i], dot[j]);
+              u[i] = weight[j] * dy[i];
+            }
+            Run<T, V>::store(static_cast<T *>(p.rows_out) + (int64_t)picks.slot[j] * p.d + c, u);
+          }
         }
       }
-    }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < K; ++j) {
 #pragma unroll
-      for (int o = 16; o > 0; o /= 2) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], o);
-      if (lane == 0) sums[warp][j] = dot[j];
+        for (int o = 16; o > 0; o /= 2) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], o);
+        if (parts > 1 && lane == 0) sums[warp][j] = dot[j];
+      }
+      if (parts == 1) {
+        if (t < p.tokens && lane == 0)
+#pragma unroll
+          for (int j = 0; j < K; ++j)
+            if (j0 + j < p.k) p.dweights[t * p.k + j0 + j] = dot[j];
+      } else {
+        __syncthreads();
+        if (in < K && j0 + in < p.k && t < p.tokens) {
+          float all = 0.f;
+          for (int w = 0; w < parts; ++w) all += sums[warp + w][in];
+          p.dweights[t * p.k + j0 + in] = all;
+        }
+        __syncthreads();
+      }
     }
-    __syncthreads();
-    if (in == 0 && lane < 4 && j0 + lane < p.k && t < p.tokens) {
-      float all = 0.f;
-      for (int w = 0; w < p.parts; ++w) all += sums[warp + w][lane];
-      p.dweights[t * p.k + j0 + lane] = all;
-    }
-    __syncthreads();
+    picks = next;
   }
 }
 
-// Threads and blocks for a token's d / V runs: blocks of 256 for wide rows, several tokens
-// a block for narrow ones.
-void shape_rows(RowsParams &p, int v, int64_t &blocks) {
-  const int64_t runs = p.d / v;
-  if (runs >= 256 || p.tokens < 2) {
-    p.parts = (int)((runs + 255) / 256);
-    blocks = p.tokens * p.parts;
+// Threads for a token's `runs` runs of V columns, whole warps where `warps`, and blocks
+// for all tokens: as many as the GPU holds, so that each takes several tokens in turn.
+Spread spread_over(int64_t runs, int64_t tokens, bool warps, int resident, int64_t &blocks) {
+  Spread s;
+  if (warps) {
+    // 3 steps over a row and more: a warp's sums cost 5 exchanges a pick however long they are
+    s.threads = runs <= 96 ? 32 : runs <= 192 ? 64 : runs <= 640 ? 128 : 256;
   } else {
-    const int each = (int)(256 / runs);
-    p.parts = -each;
-    blocks = (p.tokens + each - 1) / each;
+    // the fewest steps over a row that fit, with as few idle threads as may be
+    const int64_t steps = (runs + 255) / 256;
+    s.threads = (int)((runs + steps - 1) / steps);
   }
+  s.tokens = 256 / s.threads;
+  blocks = std::min<int64_t>((tokens + s.tokens - 1) / s.tokens, (int64_t)sm_count() * resident);
+  return s;
 }
 
 bool vectors_ok(const void *base, int64_t pitch, int64_t rows, int es) {
@@ -740,18 +784,17 @@ extern "C" int oz_dispatch(const oz_rows_args *args, void *stream) {
   if (!a.x || !a.rows_out || !a.slots || !a.offsets) return set_error(OZ_ERR_INVALID, "null pointer");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   RowsParams p{a.x, nullptr, nullptr, a.rows_out, a.slots, a.offsets, nullptr, nullptr, a.tokens, a.tokens * a.picks,
-               a.x_row, 0, (int)a.d, a.picks, a.experts, 0};
+               a.x_row, 0, (int)a.d, a.picks, a.experts};
   return with_type(a.dtype, [&](auto z) {
     using T = decltype(z);
     constexpr int ES = sizeof(T);
     const bool wide = vectors_ok(a.x, a.x_row, a.tokens, ES) && vectors_ok(a.rows_out, a.d, a.tokens * a.picks, ES) &&
                       a.d * ES % 16 == 0;
     int64_t blocks;
-    shape_rows(p, wide ? 16 / ES : 1, blocks);
-    if (blocks + kClearBlocks > INT32_MAX) return set_error(OZ_ERR_INVALID, "size out of range");
+    const Spread at = spread_over(a.d / (wide ? 16 / ES : 1), a.tokens, false, 6, blocks);
     const dim3 grid((unsigned)(blocks + kClearBlocks));
-    return wide ? launch(dispatch_kernel<T, 16 / ES>, grid, 256, 0, st, "dispatch_kernel launch", p, (int)blocks)
-                : launch(dispatch_kernel<T, 1>, grid, 256, 0, st, "dispatch_kernel launch", p, (int)blocks);
+    return wide ? launch(dispatch_kernel<T, 16 / ES>, grid, 256, 0, st, "dispatch_kernel launch", p, at, (int)blocks)
+                : launch(dispatch_kernel<T, 1>, grid, 256, 0, st, "dispatch_kernel launch", p, at, (int)blocks);
   });
 }
 
@@ -764,18 +807,23 @@ extern "C" int oz_combine(const oz_rows_args *args, void *stream) {
   if (!a.rows || !a.x_out || !a.slots) return set_error(OZ_ERR_INVALID, "null pointer");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   RowsParams p{nullptr, a.rows, a.x_out, nullptr, a.slots, nullptr, a.weights, nullptr, a.tokens, a.tokens * a.picks,
-               0, a.rows_row, (int)a.d, a.picks, a.experts, 0};
+               0, a.rows_row, (int)a.d, a.picks, a.experts};
   return with_type(a.dtype, [&](auto z) {
     using T = decltype(z);
     constexpr int ES = sizeof(T);
     const bool wide = vectors_ok(a.rows, a.rows_row, a.tokens * a.picks, ES) && vectors_ok(a.x_out, a.d, a.tokens, ES) &&
                       a.d * ES % 16 == 0;
     int64_t blocks;
-    shape_rows(p, wide ? 16 / ES : 1, blocks);
-    if (blocks > INT32_MAX) return set_error(OZ_ERR_INVALID, "size out of range");
-    const dim3 grid((unsigned)blocks);
-    return wide ? launch(combine_kernel<T, 16 / ES>, grid, 256, 0, st, "combine_kernel launch", p)
-                : launch(combine_kernel<T, 1>, grid, 256, 0, st, "combine_kernel launch", p);
+    const Spread at = spread_over(a.d / (wide ? 16 / ES : 1), a.tokens, false, a.picks > 4 ? 3 : a.picks > 2 ? 4 : 5, blocks);
+    auto with = [&](auto k) {
+      constexpr int K = decltype(k)::value;
+      const dim3 grid((unsigned)blocks);
+      return wide ? launch(combine_kernel<T, 16 / ES, K>, grid, 256, 0, st, "combine_kernel launch", p, at)
+                  : launch(combine_kernel<T, 1, K>, grid, 256, 0, st, "combine_kernel launch", p, at);
+    };
+    if (a.picks <= 2) return with(std::integral_constant<int, 2>{});
+    if (a.picks <= 4) return with(std::integral_constant<int, 4>{});
+    return with(std::integral_constant<int, 8>{});
   });
 }
 
@@ -789,21 +837,18 @@ extern "C" int oz_combine_backward(const oz_rows_args *args, void *stream) {
     return set_error(OZ_ERR_INVALID, "null pointer");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   RowsParams p{a.x, a.rows, nullptr, a.rows_out, a.slots, a.offsets, a.weights, a.dweights, a.tokens,
-               a.tokens * a.picks, a.x_row, a.rows_row, (int)a.d, a.picks, a.experts, 0};
+               a.tokens * a.picks, a.x_row, a.rows_row, (int)a.d, a.picks, a.experts};
   return with_type(a.dtype, [&](auto z) {
     using T = decltype(z);
     constexpr int ES = sizeof(T);
     const int64_t n = a.tokens * a.picks;
     const bool wide = vectors_ok(a.x, a.x_row, a.tokens, ES) && vectors_ok(a.rows, a.rows_row, n, ES) &&
                       vectors_ok(a.rows_out, a.d, n, ES) && a.d * ES % 16 == 0;
-    const int64_t runs = a.d / (wide ? 16 / ES : 1);
-    p.parts = runs <= 64 ? 1 : runs <= 128 ? 2 : runs <= 256 ? 4 : 8;
-    const int64_t blocks = (a.tokens * p.parts + 7) / 8;
-    if (blocks + kClearBlocks > INT32_MAX) return set_error(OZ_ERR_INVALID, "size out of range");
+    int64_t blocks;
+    const Spread at = spread_over(a.d / (wide ? 16 / ES : 1), a.tokens, true, 3, blocks);
     const dim3 grid((unsigned)(blocks + kClearBlocks));
-    return wide ? launch(combine_backward_kernel<T, 16 / ES>, grid, 256, 0, st, "combine_backward_kernel launch", p,
-                         (int)blocks)
-                : launch(combine_backward_kernel<T, 1>, grid, 256, 0, st, "combine_backward_kernel launch", p,
-                         (int)blocks);
+    const char *what = "combine_backward_kernel launch";
+    return wide ? launch(combine_backward_kernel<T, 16 / ES, 4>, grid, 256, 0, st, what, p, at, (int)blocks)
+                : launch(combine_backward_kernel<T, 1, 4>, grid, 256, 0, st, what, p, at, (int)blocks);
   });
 }

@@ -3,6 +3,8 @@
 // with the end of the kernel before.
 #pragma once
 
+#include <type_traits>
+
 #include "oz_common.cuh"
 
 namespace oz {
@@ -43,6 +45,20 @@ template <typename T, int V> struct Run {
   static __device__ __forceinline__ void store(T *p, const float (&v)[V]) {
     if constexpr (V == 1) *p = from_f32<T>(v[0]);
     else *reinterpret_cast<uint4 *>(p) = pack<T>(v);
+  }
+};
+
+// The same as it lies in memory: few registers for loads on their way.
+template <typename T, int V> struct Raw {
+  using Type = typename std::conditional<V == 1, T, uint4>::type;
+  static __device__ __forceinline__ Type load(const T *p) {
+    if constexpr (V == 1) return *p;
+    else return __ldg(reinterpret_cast<const uint4 *>(p));
+  }
+  static __device__ __forceinline__ void store(T *p, const Type &v) { *reinterpret_cast<Type *>(p) = v; }
+  static __device__ __forceinline__ void values(const Type &r, float (&v)[V]) {
+    if constexpr (V == 1) v[0] = to_f32(r);
+    else unpack<T>(r, v);
   }
 };
 
