@@ -20,8 +20,8 @@ ROOT = os.path.dirname(PKG)
 LIB = os.path.join(PKG, "liboz_b200.so")
 UNITS = ["oz_api.cu", "oz_split.cu", "oz_gemm.cu", "oz_peer.cu",
          "oz_experts.cu", "oz_w4.cu", "oz_newton.cu",
-         "oz_linear.cu", "oz_route.cu", "oz_clip.cu"]
-SOURCES = UNITS + ["oz_common.cuh", "oz_tile.cuh", "oz_operands.cuh", "oz_stream.cuh",
+         "oz_linear.cu", "oz_linear_split.cu", "oz_route.cu", "oz_clip.cu"]
+SOURCES = UNITS + ["oz_common.cuh", "oz_tile.cuh", "oz_operands.cuh", "oz_stream.cuh", "oz_linear.cuh",
                    "oz_log2_table.h", "oz_tile_table.h"]
 BUILD_DIR = os.path.join(PKG, "_build")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]

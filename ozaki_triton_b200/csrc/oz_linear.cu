@@ -9,70 +9,26 @@
 // applied in fp32 and rounded once.  du is rounded to the operands' type before
 // it is multiplied, its sum is not.
 
-#include <cmath>
+#include <algorithm>
 
-#include "oz_operands.cuh"
-#include "oz_stream.cuh"
+#include "oz_linear.cuh"
 
 namespace oz {
 int status_linear(int *value, bool clear) { return read_status_word(value, clear); }
 
 namespace {
 using namespace tile;
-using stream::from_f32;
-using stream::to_f32;
+using namespace linear;
 
-// ---------------------------------------------------------------------------
-// activations
-// ---------------------------------------------------------------------------
-__device__ __forceinline__ float activated(float u, int act) {
-  switch (act) {
-    case OZ_ACT_RELU: return u > 0.f ? u : u != u ? u : 0.f;
-    case OZ_ACT_GELU: return u * normcdff(u);
-    case OZ_ACT_SILU: return u / (1.f + expf(-u));
-    default: return u;
-  }
-}
 // The same as a call, for epilogues whose columns are in registers and so not in a loop.
 __device__ __noinline__ float activated_call(float u, int act) { return activated(u, act); }
-__device__ __forceinline__ float slope(float u, int act) {
-  switch (act) {
-    case OZ_ACT_RELU: return u > 0.f ? 1.f : u != u ? u : 0.f;
-    case OZ_ACT_GELU: return normcdff(u) + u * (0.3989422804014327f * expf(-0.5f * u * u));
-    case OZ_ACT_SILU: {
-      const float s = 1.f / (1.f + expf(-u));
-      return s * (1.f + u * (1.f - s));
-    }
-    default: return 1.f;
-  }
-}
-
-// ---------------------------------------------------------------------------
-// products
-// ---------------------------------------------------------------------------
-struct LinearParams {
-  void *out, *pre;
-  const void *bias, *residual;
-  int64_t ld, residual_ld;
-  int rows, k, n;              // of the result, and the contraction
-  int row_tiles, column_tiles;
-  int vectors;                 // rows of out and pre may be written 16 bytes at a time
-  int bias_f32, act;
-  uint32_t idesc;
-};
-
-template <typename O> __device__ __forceinline__ float bias_at(const LinearParams &p, int64_t c) {
-  // the bias has the operands' type, which is the result's unless that is fp32
-  if (p.bias_f32) return __ldg(static_cast<const float *>(p.bias) + c);
-  return to_f32(__ldg(static_cast<const O *>(p.bias) + c));
-}
 
 struct OutTile { int row, column; };
 
 // A warp's accumulators plus bias: u.
 template <typename O, typename B, class Source> struct WithBias {
   const Source &source;
-  const LinearParams &p;
+  const Params &p;
   int64_t column;
   __device__ __forceinline__ void read(int c, float (&v)[16]) const {
     source.read(c, v);
@@ -85,7 +41,7 @@ template <typename O, typename B, class Source> struct WithBias {
 // act(u) + residual, a lane's row of it.
 template <typename O, class Source> struct Finished {
   const Source &source;
-  const LinearParams &p;
+  const Params &p;
   const O *residual;           // this lane's row from the warp's first column on, or none
   int64_t columns;
   __device__ __forceinline__ void read(int c, float (&v)[16]) const {
@@ -104,7 +60,7 @@ template <typename O, class Source> struct Finished {
 template <typename O, typename B, int PAIR_, int NT_, bool AMN_, bool BMN_, bool PLAIN> struct LinearJob : NoLookAhead {
   static constexpr int PAIR = PAIR_, NT = NT_, PLANES = 1, PASS = sizeof(O) == 4 ? 8 : 0;
   static constexpr bool AMN = AMN_, BMN = BMN_, RAGGED = false;
-  using Params = LinearParams;
+  using Params = linear::Params;
   using Extra = OutTile;
   static __device__ int plane_stride(const Params &) { return 0; }
   struct Walk {
@@ -145,16 +101,8 @@ template <typename O, typename B, int PAIR_, int NT_, bool AMN_, bool BMN_, bool
   static __device__ void finish(const Params &, int, int) {}
 };
 
-// Two operands: rows of A along the result's rows, rows of B along its columns, each
-// `mn` (stored across the contraction) or along it, with its row pitch.
-struct Side {
-  const void *p;
-  int64_t pitch;               // elements
-  bool mn;
-};
-
 template <class J>
-int run_job(const Side &a, const Side &b, LinearParams p, cudaStream_t st, const char *what) {
+int run_job(const Side &a, const Side &b, Params p, cudaStream_t st, const char *what) {
   CUtensorMap ta, tb;
   const int64_t ai = J::AMN ? p.rows : p.k, ar = J::AMN ? p.k : p.rows;
   const int64_t bi = J::BMN ? p.n : p.k, br = J::BMN ? p.k : p.n;
@@ -169,7 +117,7 @@ int run_job(const Side &a, const Side &b, LinearParams p, cudaStream_t st, const
 }
 
 template <typename O, typename B, bool PLAIN>
-int product(const Side &a, const Side &b, const LinearParams &p, cudaStream_t st, const char *what) {
+int product(const Side &a, const Side &b, const Params &p, cudaStream_t st, const char *what) {
   const bool pair = p.rows > kRows && p.n > 128;
   if (a.mn) {
     if constexpr (PLAIN)
@@ -185,8 +133,10 @@ int product(const Side &a, const Side &b, const LinearParams &p, cudaStream_t st
 }
 
 template <bool PLAIN>
-int product_of(int dtype, int out_dtype, const Side &a, const Side &b, const LinearParams &p, cudaStream_t st,
+int product_of(int dtype, int out_dtype, const Side &a, const Side &b, const Params &p, cudaStream_t st,
                const char *what) {
+  const SplitPlan plan = split_plan(p.rows, p.k, p.n, a.mn);
+  if (plan.tile_rows) return split_product(plan, dtype, out_dtype, a, b, p, st, what);
   if (dtype == OZ_F16)
     return out_dtype == OZ_F32 ? product<float, __half, PLAIN>(a, b, p, st, what)
                                : product<__half, __half, PLAIN>(a, b, p, st, what);
@@ -288,7 +238,7 @@ int check_linear(int dtype, int out_dtype, int act, int64_t rows, int64_t k, int
 bool stored_across(int64_t n, int64_t w_sk, int64_t w_sn) { return w_sn == 1 || (n == 1 && w_sk != 1); }
 
 // y of an empty contraction: the epilogue on zeros.
-template <typename O, typename B> __global__ void __launch_bounds__(256) empty_kernel(const LinearParams p) {
+template <typename O, typename B> __global__ void __launch_bounds__(256) empty_kernel(const Params p) {
   stream::start_after_earlier_kernels();
   const int64_t end = (int64_t)p.rows * p.n;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < end; i += (int64_t)gridDim.x * 256) {
@@ -315,7 +265,7 @@ extern "C" int oz_linear(const oz_linear_args *args, void *stream) {
   if (!a.y) return set_error(OZ_ERR_INVALID, "null pointer");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int es = dtype_size(a.out_dtype);
-  LinearParams p{a.y, a.pre, a.bias, a.residual, a.n, a.residual_sr, (int)a.rows, (int)a.k, (int)a.n, 0, 0,
+  Params p{a.y, a.pre, a.bias, a.residual, a.n, a.residual_sr, (int)a.rows, (int)a.k, (int)a.n, 0, 0,
                  (uintptr_t)a.y % 16 == 0 && a.n * es % 16 == 0 &&
                      (!a.pre || ((uintptr_t)a.pre % 16 == 0 && a.n * 2 % 16 == 0)),
                  a.bias_dtype == OZ_F32, a.act, tile::instruction(a.dtype)};
@@ -416,14 +366,14 @@ extern "C" int oz_linear_backward(const oz_linear_backward_args *args, void *str
   if (int rc = lay_out(ops, count, space + own, a.workspace_bytes - own, st)) return rc;
   if (want_x) {
     // dx (rows, k) = du (rows, n) w^T: w's rows along n where it is stored across
-    LinearParams p{a.dx, nullptr, nullptr, nullptr, a.k, 0, (int)a.rows, (int)a.n, (int)a.k, 0, 0,
+    Params p{a.dx, nullptr, nullptr, nullptr, a.k, 0, (int)a.rows, (int)a.n, (int)a.k, 0, 0,
                    (uintptr_t)a.dx % 16 == 0 && a.k % 8 == 0, 0, OZ_ACT_NONE, tile::instruction(a.dtype)};
     if (int rc = product_of<true>(a.dtype, a.dtype, Side{ops[0].p, ops[0].row, false},
                                   Side{ops[at_w].p, ops[at_w].row, !across}, p, st, "dx launch"))
       return rc;
   }
   if (want_w) {
-    LinearParams p{a.dw, nullptr, nullptr, nullptr, a.n, 0, (int)a.k, (int)a.rows, (int)a.n, 0, 0,
+    Params p{a.dw, nullptr, nullptr, nullptr, a.n, 0, (int)a.k, (int)a.rows, (int)a.n, 0, 0,
                    (uintptr_t)a.dw % 16 == 0 && a.n * dw_size % 16 == 0, 0, OZ_ACT_NONE, tile::instruction(a.dtype)};
     return product_of<true>(a.dtype, a.dw_dtype, Side{ops[at_x].p, ops[at_x].row, true},
                             Side{ops[0].p, ops[0].row, true}, p, st, "dw launch");

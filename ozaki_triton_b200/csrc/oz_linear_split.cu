@@ -1,0 +1,317 @@
+// oz_linear_split.cu -- fused products whose result has few tiles: one token against
+// a weight matrix, a short chunk, the gradient of a small weight.
+//
+//   y = act(x w + bias) + residual     (or a plain product)
+//
+// What bounds them is the way of the operands' bytes to the SMs, so the contraction is
+// divided over the CTAs of a cluster (up to 8), each with 128 columns of the result
+// by up to 128 of its rows: tcgen05 products with the columns as A (their weights are
+// read once, however few rows there are), fp32 sums in tensor memory.  The CTAs
+// then put their sums into shared memory and each adds up, over the cluster, the
+// rows that are its own, in the order of the CTAs, and finishes them.  No second
+// launch, no atomics.  Two CTAs share an SM, so that one's start and end run under
+// the other's loads.
+
+#include <algorithm>
+
+#include "oz_linear.cuh"
+
+namespace oz {
+int status_linear_split(int *value, bool clear) { return read_status_word(value, clear); }
+
+namespace {
+using namespace tile;
+using namespace linear;
+
+constexpr int kSplitThreads = 192;            // producer, MMA, 4 warps that finish
+constexpr int kSplitRoom = 106 * 1024;        // shared memory of a CTA: two an SM
+constexpr int kMostSplits = 8;
+constexpr int kPassBlocks = 8;                // of an accumulator where the result is fp32
+
+template <int NT> __host__ __device__ constexpr int split_stage() { return kRows * kLine + NT * kLine; }
+template <int NT> __host__ __device__ constexpr int split_stages() {
+  return (kSplitRoom - 2048) / split_stage<NT>() < 8 ? (kSplitRoom - 2048) / split_stage<NT>() : 8;
+}
+template <int NT> __host__ __device__ constexpr int split_smem() { return 1024 + split_stages<NT>() * split_stage<NT>() + 256; }
+
+__device__ __forceinline__ float load_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// A: 128 columns of the result, B: NT rows.  O: the result's type, T: the operands'.
+template <typename O, typename T, int NT, bool AMN, bool BMN>
+__global__ void __launch_bounds__(kSplitThreads, 2)
+    split_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const Params p,
+                 const int splits) {
+  constexpr int S = split_stages<NT>(), SB = split_stage<NT>(), A_BYTES = kRows * kLine;
+  constexpr int PASS = sizeof(O) == 4 ? kPassBlocks : 1 << 28;
+  constexpr int kTmemColumns = 2 * NT < 32 ? 32 : 2 * NT;
+  static_assert(S >= 3 && NT * kRows * 4 <= S * SB, "shared memory");
+  static_assert(NT % 16 == 0 && (!BMN || NT % 64 == 0), "rows of a tile");
+
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  float *partial = reinterpret_cast<float *>(smem);            // [NT][128], after the products
+  uint64_t *full = reinterpret_cast<uint64_t *>(smem + S * SB);
+  uint64_t *empty = full + S;
+  uint64_t *acc_full = empty + S;                              // [2]
+  uint64_t *acc_empty = acc_full + 2;                          // [2]
+  uint64_t *drain = acc_empty + 2;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int rank = splits > 1 ? (int)cluster_ctarank() : 0;
+  const int tile = blockIdx.x / splits;
+  const int column0 = tile / p.row_tiles * kRows, row0 = tile % p.row_tiles * NT;
+  const int blocks = (p.k + kBlock - 1) / kBlock;
+  const int first = (int)((int64_t)blocks * rank / splits), last = (int)((int64_t)blocks * (rank + 1) / splits);
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], 4);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    prefetch_tmap(&tm_a);
+    prefetch_tmap(&tm_b);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, kTmemColumns);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  stream::start_after_earlier_kernels();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int it = 0;
+      for (int kb = first; kb < last; ++kb, ++it) {
+        const int slot = it % S;
+        if (!mbar_wait_bounded(&empty[slot], ((it / S) & 1) ^ 1, abort_flag, DEV_TIMEOUT_PRODUCER)) break;
+        unsigned char *sa = smem + slot * SB, *sb = sa + A_BYTES;
+        mbar_arrive_expect_tx(&full[slot], SB);
+        if constexpr (AMN) {
+          tma_load_3d(sa, &tm_a, &full[slot], column0, kb * kBlock, 0);
+          tma_load_3d(sa + kBlock * kLine, &tm_a, &full[slot], column0 + 64, kb * kBlock, 0);
+        } else {
+          tma_load_3d(sa, &tm_a, &full[slot], kb * kBlock, column0, 0);
+        }
+        if constexpr (BMN) {
+#pragma unroll
+          for (int c = 0; c < NT / 64; ++c)
+            tma_load_3d(sb + c * kBlock * kLine, &tm_b, &full[slot], row0 + c * 64, kb * kBlock, 0);
+        } else {
+          tma_load_3d(sb, &tm_b, &full[slot], kb * kBlock, row0, 0);
+        }
+      }
+      // every load has landed before shared memory is used for something else or goes away
+      for (int k = max(it - S, 0); k < it; ++k)
+        if (!mbar_settle(&full[k % S], (k / S) & 1, abort_flag, DEV_TIMEOUT_PRODUCER)) break;
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint32_t base = smem_u32(smem);
+      const uint64_t a_desc = operand_desc<AMN>(base), b_desc = operand_desc<BMN>(base + A_BYTES);
+      constexpr uint64_t a_step = AMN ? (16 * kLine) >> 4 : 2, b_step = BMN ? (16 * kLine) >> 4 : 2;
+      const uint32_t idesc = p.idesc | (uint32_t)(NT >> 3) << 17 | (uint32_t)(kRows >> 4) << 24 |
+                             (AMN ? 1u << 15 : 0u) | (BMN ? 1u << 16 : 0u);
+      int slot = 0;
+      uint32_t phase = 0, done = 0;
+      bool ok = true;
+      for (int kb = first; ok && kb < last;) {
+        const int stop = min(last - kb, PASS) + kb, buf = done & 1;
+        if (!(ok = mbar_wait_bounded(&acc_empty[buf], ((done >> 1) & 1) ^ 1, abort_flag, DEV_TIMEOUT_MMA))) break;
+        tc_fence_after();
+        const uint32_t d = tmem + (uint32_t)(buf * NT);
+        for (const int from = kb; kb < stop; ++kb) {
+          if (!(ok = mbar_wait_bounded(&full[slot], phase, abort_flag, DEV_TIMEOUT_MMA))) break;
+          tc_fence_after();
+          const uint64_t ad = a_desc + slot * (SB >> 4), bd = b_desc + slot * (SB >> 4);
+#pragma unroll
+          for (int kk = 0; kk < kBlock / 16; ++kk)
+            tc_mma<1>(d, ad + kk * a_step, bd + kk * b_step, idesc, kk || kb > from ? 1u : 0u);
+          tc_commit(&empty[slot]);
+          if (++slot == S) {
+            slot = 0;
+            phase ^= 1;
+          }
+        }
+        if (!ok) break;
+        tc_commit(&acc_full[buf]);
+        ++done;
+      }
+      tc_commit(drain);
+      mbar_settle(drain, 0, abort_flag, DEV_TIMEOUT_MMA);
+    }
+  } else {
+    // sums to shared memory: the last accumulator is there, so the products are done with it
+    const int sub = warp & 3, rows = min(p.rows - row0, NT);
+    const uint32_t columns = tmem + ((uint32_t)(sub * 32) << 16);
+    const int c = sub * 32 + lane;
+    uint32_t done = 0;
+    auto acquire = [&]() {
+      const bool ok = mbar_wait_bounded(&acc_full[done & 1], (done >> 1) & 1, abort_flag, DEV_TIMEOUT_EPILOGUE);
+      if (!__all_sync(0xffffffffu, ok)) return false;
+      tc_fence_after();
+      return true;
+    };
+    if constexpr (sizeof(O) == 4) {
+      float sum[NT];
+#pragma unroll
+      for (int r = 0; r < NT; ++r) sum[r] = 0.f;
+      for (int kb = first; kb < last; kb += PASS) {
+        if (!acquire()) break;
+#pragma unroll
+        for (int r0 = 0; r0 < NT; r0 += 16) {
+          uint32_t v[16];
+          tmem_ld16_at(columns + (uint32_t)((done & 1) * NT + r0), v);
+          tmem_ld_wait16(v);
+#pragma unroll
+          for (int x = 0; x < 16; ++x) sum[r0 + x] += __uint_as_float(v[x]);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&acc_empty[done & 1]);
+        ++done;
+      }
+#pragma unroll
+      for (int r = 0; r < NT; ++r)
+        if (r < rows) partial[r * kRows + c] = sum[r];
+    } else {
+      acquire();
+#pragma unroll 1
+      for (int r0 = 0; r0 < rows; r0 += 16) {
+        uint32_t v[16];
+        tmem_ld16_at(columns + (uint32_t)r0, v);
+        tmem_ld_wait16(v);
+#pragma unroll
+        for (int x = 0; x < 16; ++x)
+          if (r0 + x < rows) partial[(r0 + x) * kRows + c] = __uint_as_float(v[x]);
+      }
+    }
+  }
+  if (splits > 1) cluster_sync();
+  if (warp >= 2) {
+    const int sub = warp & 3, rows = min(p.rows - row0, NT);
+    const int c = sub * 32 + lane, column = column0 + c;
+    const uint32_t mine = smem_u32(partial) + (uint32_t)c * 4;
+    const bool there = column < p.n;
+    const float bias = p.bias && there ? bias_at<T>(p, column) : 0.f;
+    for (int r = rank; r < rows; r += splits) {
+      const int64_t row = row0 + r;
+      float residual = 0.f;
+      if (p.residual && there) residual = to_f32(__ldg(static_cast<const O *>(p.residual) + row * p.residual_ld + column));
+      float u;
+      if (splits > 1) {
+        float v[kMostSplits];
+#pragma unroll
+        for (int s = 0; s < kMostSplits; ++s)
+          v[s] = s < splits ? load_cluster(map_to_cta(mine + (uint32_t)(r * kRows * 4), s)) : 0.f;
+        u = v[0];
+#pragma unroll
+        for (int s = 1; s < kMostSplits; ++s) u += v[s];
+      } else {
+        u = partial[r * kRows + c];
+      }
+      if (!there) continue;
+      u += bias;
+      if (p.pre) static_cast<T *>(p.pre)[row * p.ld + column] = from_f32<T>(u);
+      static_cast<O *>(p.out)[row * p.ld + column] = from_f32<O>(activated(u, p.act) + residual);
+    }
+  }
+  tc_fence_before();
+  if (splits > 1) cluster_sync();              // nobody's sums go away while they are read
+  else __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemColumns);
+  }
+}
+
+template <typename O, typename T, int NT, bool AMN, bool BMN>
+int run_split(const Side &a, const Side &b, Params p, int splits, cudaStream_t st, const char *what) {
+  // a lies along the result's rows: the kernel's B
+  CUtensorMap tc, tr;
+  const int64_t ci = AMN ? p.n : p.k, cr = AMN ? p.k : p.n, ri = BMN ? p.rows : p.k, rr = BMN ? p.k : p.rows;
+  const int64_t cp = pitch_bytes(b.pitch, cr, ci), rp = pitch_bytes(a.pitch, rr, ri);
+  if (int rc = make_map(&tc, b.p, ci, cr, 1, cp, cp, AMN ? kBlock : kRows)) return rc;
+  if (int rc = make_map(&tr, a.p, ri, rr, 1, rp, rp, BMN ? kBlock : NT)) return rc;
+  const int64_t rows = (p.rows + NT - 1) / NT, columns = (p.n + kRows - 1) / kRows;
+  if (rows * columns * splits > INT32_MAX / 2) return set_error(OZ_ERR_INVALID, "too many tiles");
+  p.row_tiles = (int)rows;
+  p.column_tiles = (int)columns;
+  auto kernel = split_kernel<O, T, NT, AMN, BMN>;
+  constexpr int smem = split_smem<NT>();
+  if (int rc = set_smem_once((const void *)kernel, smem, what)) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(rows * columns * splits));
+  cfg.blockDim = dim3(kSplitThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = splits;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  count_launch();
+  return check_cuda(cudaLaunchKernelEx(&cfg, kernel, tc, tr, p, splits), what);
+}
+
+template <typename O, typename T>
+int split_of(const SplitPlan &plan, const Side &a, const Side &b, const Params &p, cudaStream_t st, const char *what) {
+  const int s = plan.splits;
+  if (a.mn) {
+    if (!b.mn) return set_error(OZ_ERR_UNSUPPORTED, "operand layout");
+    return plan.tile_rows <= 64 ? run_split<O, T, 64, true, true>(a, b, p, s, st, what)
+                                : run_split<O, T, 128, true, true>(a, b, p, s, st, what);
+  }
+  if (b.mn)
+    return plan.tile_rows <= 16   ? run_split<O, T, 16, true, false>(a, b, p, s, st, what)
+           : plan.tile_rows <= 64 ? run_split<O, T, 64, true, false>(a, b, p, s, st, what)
+                                  : run_split<O, T, 128, true, false>(a, b, p, s, st, what);
+  return plan.tile_rows <= 16   ? run_split<O, T, 16, false, false>(a, b, p, s, st, what)
+         : plan.tile_rows <= 64 ? run_split<O, T, 64, false, false>(a, b, p, s, st, what)
+                                : run_split<O, T, 128, false, false>(a, b, p, s, st, what);
+}
+
+}  // namespace
+
+namespace linear {
+
+SplitPlan split_plan(int64_t rows, int64_t k, int64_t n, bool rows_mn) {
+  SplitPlan plan{rows <= 16 && !rows_mn ? 16 : rows <= 64 ? 64 : 128, 1};
+  const int64_t tiles = (rows + plan.tile_rows - 1) / plan.tile_rows * ((n + kRows - 1) / kRows);
+  const int64_t blocks = (k + kBlock - 1) / kBlock, sms = tile::sm_count();
+  // up to two CTAs an SM, two blocks a CTA at least
+  while (plan.splits < kMostSplits && tiles * plan.splits * 2 <= 2 * sms && blocks >= plan.splits * 4) plan.splits *= 2;
+  if (rows > 128 && tiles * plan.splits > 2 * sms) plan.tile_rows = 0;
+  return plan;
+}
+
+int split_product(const SplitPlan &plan, int dtype, int out_dtype, const Side &a, const Side &b, const Params &p,
+                  cudaStream_t st, const char *what) {
+  if (dtype == OZ_F16)
+    return out_dtype == OZ_F32 ? split_of<float, __half>(plan, a, b, p, st, what)
+                               : split_of<__half, __half>(plan, a, b, p, st, what);
+  return out_dtype == OZ_F32 ? split_of<float, __nv_bfloat16>(plan, a, b, p, st, what)
+                             : split_of<__nv_bfloat16, __nv_bfloat16>(plan, a, b, p, st, what);
+}
+
+}  // namespace linear
+}  // namespace oz
