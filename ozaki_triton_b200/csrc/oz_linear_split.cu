@@ -34,10 +34,47 @@ template <int NT> __host__ __device__ constexpr int split_stages() {
 }
 template <int NT> __host__ __device__ constexpr int split_smem() { return 1024 + split_stages<NT>() * split_stage<NT>() + 256; }
 
-__device__ __forceinline__ float load_cluster(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+__device__ __forceinline__ float4 load_cluster(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
   return v;
+}
+// 4 consecutive columns, at once or, up to `count`, one by one.
+template <typename E> __device__ __forceinline__ void load4(const E *from, bool vectors, int count, float (&v)[4]) {
+  if (vectors && count >= 4) {
+    if constexpr (sizeof(E) == 4) {
+      const float4 a = __ldg(reinterpret_cast<const float4 *>(from));
+      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+    } else {
+      const uint2 a = __ldg(reinterpret_cast<const uint2 *>(from));
+      const E *e = reinterpret_cast<const E *>(&a);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) v[x] = to_f32(e[x]);
+    }
+  } else {
+#pragma unroll
+    for (int x = 0; x < 4; ++x) v[x] = x < count ? to_f32(__ldg(from + x)) : 0.f;
+  }
+}
+template <typename E> __device__ __forceinline__ void store4(E *to, bool vectors, int count, const float (&v)[4]) {
+  if (vectors && count >= 4) {
+    if constexpr (sizeof(E) == 4) {
+      *reinterpret_cast<float4 *>(to) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+      uint2 a;
+      E *e = reinterpret_cast<E *>(&a);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) e[x] = from_f32<E>(v[x]);
+      *reinterpret_cast<uint2 *>(to) = a;
+    }
+  } else {
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      if (x < count) to[x] = from_f32<E>(v[x]);
+  }
 }
 
 // A: 128 columns of the result, B: NT rows.  O: the result's type, T: the operands'.
@@ -203,32 +240,44 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
     }
   }
   if (splits > 1) cluster_sync();
+  else __syncthreads();
   if (warp >= 2) {
-    const int sub = warp & 3, rows = min(p.rows - row0, NT);
-    const int c = sub * 32 + lane, column = column0 + c;
-    const uint32_t mine = smem_u32(partial) + (uint32_t)c * 4;
-    const bool there = column < p.n;
-    const float bias = p.bias && there ? bias_at<T>(p, column) : 0.f;
-    for (int r = rank; r < rows; r += splits) {
+    // a warp a row, 4 columns a lane
+    const int rows = min(p.rows - row0, NT), column = column0 + lane * 4, count = min(p.n - column, 4);
+    const uint32_t mine = smem_u32(partial) + (uint32_t)lane * 16;
+    float bias[4] = {};
+    if (p.bias && count > 0) {
+      if (p.bias_f32) load4(static_cast<const float *>(p.bias) + column, p.vectors & kBiasVectors, count, bias);
+      else load4(static_cast<const T *>(p.bias) + column, p.vectors & kBiasVectors, count, bias);
+    }
+    for (int r = rank + (warp - 2) * splits; r < rows; r += 4 * splits) {
       const int64_t row = row0 + r;
-      float residual = 0.f;
-      if (p.residual && there) residual = to_f32(__ldg(static_cast<const O *>(p.residual) + row * p.residual_ld + column));
-      float u;
+      float residual[4] = {};
+      if (p.residual && count > 0)
+        load4(static_cast<const O *>(p.residual) + row * p.residual_ld + column, p.vectors & kResidualVectors, count,
+              residual);
+      float u[4];
       if (splits > 1) {
-        float v[kMostSplits];
+        float4 v[kMostSplits];
 #pragma unroll
         for (int s = 0; s < kMostSplits; ++s)
-          v[s] = s < splits ? load_cluster(map_to_cta(mine + (uint32_t)(r * kRows * 4), s)) : 0.f;
-        u = v[0];
+          if (s < splits) v[s] = load_cluster(map_to_cta(mine + (uint32_t)(r * kRows * 4), s));
+        u[0] = v[0].x, u[1] = v[0].y, u[2] = v[0].z, u[3] = v[0].w;
 #pragma unroll
-        for (int s = 1; s < kMostSplits; ++s) u += v[s];
+        for (int s = 1; s < kMostSplits; ++s)
+          if (s < splits) u[0] += v[s].x, u[1] += v[s].y, u[2] += v[s].z, u[3] += v[s].w;
       } else {
-        u = partial[r * kRows + c];
+        const float4 v = *reinterpret_cast<const float4 *>(partial + r * kRows + lane * 4);
+        u[0] = v.x, u[1] = v.y, u[2] = v.z, u[3] = v.w;
       }
-      if (!there) continue;
-      u += bias;
-      if (p.pre) static_cast<T *>(p.pre)[row * p.ld + column] = from_f32<T>(u);
-      static_cast<O *>(p.out)[row * p.ld + column] = from_f32<O>(activated(u, p.act) + residual);
+      if (count <= 0) continue;
+      const int64_t at = row * p.ld + column;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) u[x] += bias[x];
+      if (p.pre) store4(static_cast<T *>(p.pre) + at, p.vectors & kVectors, count, u);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) u[x] = activated(u[x], p.act) + residual[x];
+      store4(static_cast<O *>(p.out) + at, p.vectors & kVectors, count, u);
     }
   }
   tc_fence_before();
