@@ -164,8 +164,7 @@ int run_job(const Side &a, const Side &b, Params p, cudaStream_t st, const char 
 }
 
 template <typename O, typename B, bool PLAIN>
-int product(const Side &a, const Side &b, const Params &p, cudaStream_t st, const char *what) {
-  const bool pair = p.rows > kRows && p.n > 128;
+int product(bool pair, const Side &a, const Side &b, const Params &p, cudaStream_t st, const char *what) {
   if (a.mn) {
     if constexpr (PLAIN)
       return pair ? run_job<LinearJob<O, B, 2, 256, true, true, true>>(a, b, p, st, what)
@@ -179,24 +178,59 @@ int product(const Side &a, const Side &b, const Params &p, cudaStream_t st, cons
               : run_job<LinearJob<O, B, 1, 128, false, false, PLAIN>>(a, b, p, st, what);
 }
 
+// How a product is divided, by the least estimated time (us, one B200, fitted to 690
+// measured times of 90 sizes, 1 to 16000 rows, 8 to 8192 terms and columns: half of them
+// within 10%; the choice is 3% slower than the best one on average).  Engine: its start, and for
+// each wave of tiles a tile's blocks of 64 terms and its end.  Split: for each CTA of the two
+// that an SM holds its start and end, for each CTA of an SM its blocks.  Some pairs (bf16, us):
+//   rows x terms x columns    128 x 128   256 x 256   split (rows of a tile, CTAs)
+//   4 x 3904 x 2600              22.3        25.1      7.2 (16, 8)    9.0 (16, 4)
+//   131 x 7504 x 2688            45          49       16.7 (64, 4)   20.4 (128, 4)
+//   432 x 72 x 2136               4.2         5.9      5.5 (64, 1)    7.4 (128, 1)
+//   720 x 7904 x 3616            76.8        45.2     67.0 (128, 4)
+//   2317 x 3056 x 3360           65.5        41.3     60.2 (128, 1)
+struct Plan {
+  bool pair;                   // the engine's tiles: 256 x 256 by pairs of CTAs, or 128 x 128
+  SplitPlan split;             // of 0 rows: the engine
+};
+Plan plan_product(int64_t rows, int64_t k, int64_t n, bool rows_mn) {
+  const int64_t sms = tile::sm_count(), blocks = (k + kBlock - 1) / kBlock;
+  auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
+  Plan plan{false, {0, 1}};
+  double best = 3.3 + up(up(rows, 128) * up(n, 128), sms) * (0.32 * blocks + 0.9);
+  const double pairs = 3.6 + up(up(rows, 256) * up(n, 256) * 2, sms) * (0.347 * blocks + 1.9);
+  if (pairs < best) plan.pair = true, best = pairs;
+  for (int shape = rows_mn ? 1 : 0; shape < 3; ++shape) {
+    const int tile_rows = shape == 0 ? 16 : shape == 1 ? 64 : 128;
+    const double end = shape == 0 ? 3.2 : shape == 1 ? 4.5 : 5.8, block = shape == 0 ? 0.224 : shape == 1 ? 0.269 : 0.345;
+    const int64_t tiles = up(rows, tile_rows) * up(n, 128);
+    for (int splits = 1; splits <= kMostSplits && splits <= blocks; splits *= 2) {
+      const double time = up(tiles * splits, 2 * sms) * end + up(tiles * splits, sms) * up(blocks, splits) * block +
+                          (splits > 1 ? 0.7 : 0.0);
+      if (time < best) plan.split = SplitPlan{tile_rows, splits}, best = time;
+    }
+  }
+  return plan;
+}
+
 template <bool PLAIN>
 int product_of(int dtype, int out_dtype, const Side &a, const Side &b, const Params &p, cudaStream_t st,
                const char *what) {
-  const SplitPlan plan = split_plan(p.rows, p.k, p.n, a.mn);
-  if (plan.tile_rows) return split_product(plan, dtype, out_dtype, a, b, p, st, what);
+  const Plan plan = plan_product(p.rows, p.k, p.n, a.mn);
+  if (plan.split.tile_rows) return split_product(plan.split, dtype, out_dtype, a, b, p, st, what);
   if (dtype == OZ_F16)
-    return out_dtype == OZ_F32 ? product<float, __half, PLAIN>(a, b, p, st, what)
-                               : product<__half, __half, PLAIN>(a, b, p, st, what);
-  return out_dtype == OZ_F32 ? product<float, __nv_bfloat16, PLAIN>(a, b, p, st, what)
-                             : product<__nv_bfloat16, __nv_bfloat16, PLAIN>(a, b, p, st, what);
+    return out_dtype == OZ_F32 ? product<float, __half, PLAIN>(plan.pair, a, b, p, st, what)
+                               : product<__half, __half, PLAIN>(plan.pair, a, b, p, st, what);
+  return out_dtype == OZ_F32 ? product<float, __nv_bfloat16, PLAIN>(plan.pair, a, b, p, st, what)
+                             : product<__nv_bfloat16, __nv_bfloat16, PLAIN>(plan.pair, a, b, p, st, what);
 }
 
 // ---------------------------------------------------------------------------
 // du = dy act'(u) and the sums of its columns
 // ---------------------------------------------------------------------------
 struct SlopeParams {
-  const void *dy, *pre;
-  void *du;                    // may be none (no activation)
+  const void *dy, *pre;        // pre: none without an activation
+  void *du;                    // written where there is an activation
   float *sums;                 // a row for each block row; none: no sums
   int64_t dy_sr, pre_sr, du_sr;
   int64_t rows;
@@ -205,34 +239,54 @@ struct SlopeParams {
 
 constexpr int kSlopeRows = 8;  // rows of a block's pass, a warp each
 
-// 32 lanes take 32 V columns of a row, 4 rows of a warp on their way at a time.
-template <typename T, int V> __global__ void __launch_bounds__(256) slope_kernel(const SlopeParams p) {
+// 32 lanes take 32 V columns of a row; a warp's next two rows are on their way while it
+// works on the two before.
+template <typename T, int V> __global__ void __launch_bounds__(256, 5) slope_kernel(const SlopeParams p) {
+  constexpr int AT_ONCE = 2;
+  using R = stream::Raw<T, V>;
   __shared__ float part[kSlopeRows][32 * V];
   stream::start_after_earlier_kernels();
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int c = (blockIdx.x * 32 + lane) * V;
-  const int64_t r0 = (int64_t)blockIdx.y * p.per, r1 = min(r0 + p.per, p.rows);
+  const int64_t r0 = (int64_t)blockIdx.y * p.per;
+  const int rows = (int)min((int64_t)p.per, p.rows - r0);
   float sum[V] = {};
   if (c < p.n) {
-    for (int64_t r = r0 + warp; r < r1; r += 4 * kSlopeRows) {
-      float dy[4][V], u[4][V];
+    const T *dy = static_cast<const T *>(p.dy) + r0 * p.dy_sr + c, *pre = static_cast<const T *>(p.pre) + r0 * p.pre_sr + c;
+    T *du = static_cast<T *>(p.du) + r0 * p.du_sr + c;
+    typename R::Type a[AT_ONCE], b[AT_ONCE], next_a[AT_ONCE], next_b[AT_ONCE];
+    auto load = [&](int r, auto &to_a, auto &to_b) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int64_t at = r + q * kSlopeRows;
-        if (at >= r1) continue;
-        stream::Run<T, V>::load(static_cast<const T *>(p.dy) + at * p.dy_sr + c, dy[q]);
-        if (p.pre) stream::Run<T, V>::load(static_cast<const T *>(p.pre) + at * p.pre_sr + c, u[q]);
+      for (int q = 0; q < AT_ONCE; ++q) {
+        const int at = r + q * kSlopeRows;
+        if (at >= rows) continue;
+        to_a[q] = R::load(dy + at * p.dy_sr);
+        if (p.pre) to_b[q] = R::load(pre + at * p.pre_sr);
+      }
+    };
+    load(warp, a, b);
+#pragma unroll 1
+    for (int r = warp; r < rows; r += AT_ONCE * kSlopeRows) {
+      load(r + AT_ONCE * kSlopeRows, next_a, next_b);
+#pragma unroll
+      for (int q = 0; q < AT_ONCE; ++q) {
+        const int at = r + q * kSlopeRows;
+        if (at >= rows) continue;
+        float v[V], u[V];
+        R::values(a[q], v);
+        if (p.pre) {
+          R::values(b[q], u);
+#pragma unroll
+          for (int x = 0; x < V; ++x) v[x] *= slope(u[x], p.act);
+          stream::Run<T, V>::store(du + at * p.du_sr, v);
+        }
+#pragma unroll
+        for (int x = 0; x < V; ++x) sum[x] += v[x];
       }
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int64_t at = r + q * kSlopeRows;
-        if (at >= r1) continue;
-        if (p.pre)
-#pragma unroll
-          for (int x = 0; x < V; ++x) dy[q][x] *= slope(u[q][x], p.act);
-#pragma unroll
-        for (int x = 0; x < V; ++x) sum[x] += dy[q][x];
-        if (p.du) stream::Run<T, V>::store(static_cast<T *>(p.du) + at * p.du_sr + c, dy[q]);
+      for (int q = 0; q < AT_ONCE; ++q) {
+        a[q] = next_a[q];
+        b[q] = next_b[q];
       }
     }
   }
@@ -250,24 +304,30 @@ template <typename T, int V> __global__ void __launch_bounds__(256) slope_kernel
   }
 }
 
+// A block adds up 32 columns of the block rows' sums, a warp every eighth row.
 __global__ void __launch_bounds__(256) sums_kernel(const float *sums, float *out, int rows, int n) {
+  __shared__ double part[8][33];
   stream::start_after_earlier_kernels();
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c >= n) return;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, c = blockIdx.x * 32 + lane;
   double s = 0;
+  if (c < n)
 #pragma unroll 8
-  for (int r = 0; r < rows; ++r) s += __ldg(sums + (int64_t)r * n + c);
+    for (int r = warp; r < rows; r += 8) s += __ldg(sums + (int64_t)r * n + c);
+  part[warp][lane] = s;
+  __syncthreads();
+  if (warp || c >= n) return;
+  for (int w = 1; w < 8; ++w) s += part[w][lane];
   out[c] = (float)s;
 }
 
 int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
 
-// Rows of a block of slope_kernel: as many blocks as keep the GPU's memory busy.
+// Rows of a block of slope_kernel: as many blocks as the GPU holds at once.
 int slope_rows(int64_t rows, int n) {
   const int64_t columns = (n + 255) / 256;
-  const int64_t want = std::max<int64_t>(1, stream::sm_count() * 8 / columns);
+  const int64_t want = std::max<int64_t>(1, stream::sm_count() * 5 / columns);
   const int64_t per = std::max<int64_t>(64, (rows + want - 1) / want);
-  return (int)((per + 31) / 32 * 32);
+  return (int)((per + 15) / 16 * 16);
 }
 
 int check_linear(int dtype, int out_dtype, int act, int64_t rows, int64_t k, int64_t n) {
@@ -333,6 +393,9 @@ extern "C" int oz_linear(const oz_linear_args *args, void *stream) {
   Operand ops[2] = {{a.x, a.rows, a.x_sr, 1, 0, (int)a.k},
                     {a.w, across ? a.k : a.n, across ? a.w_sk : a.w_sn, 1, 0, (int)(across ? a.n : a.k)}};
   if (int rc = lay_out(ops, 2, a.workspace, a.workspace_bytes, st)) return rc;
+  if (!a.bias && !a.act && !a.residual && !a.pre)
+    return product_of<true>(a.dtype, a.out_dtype, Side{ops[0].p, ops[0].row, false}, Side{ops[1].p, ops[1].row, across},
+                            p, st, "product launch");
   return product_of<false>(a.dtype, a.out_dtype, Side{ops[0].p, ops[0].row, false}, Side{ops[1].p, ops[1].row, across}, p,
                            st, "product launch");
 }
@@ -393,7 +456,7 @@ extern "C" int oz_linear_backward(const oz_linear_backward_args *args, void *str
                 : stream::launch(slope_kernel<__nv_bfloat16, 1>, grid, 256, 0, st, what, s);
     if (rc) return rc;
     if (a.db && blocks > 1) {
-      rc = stream::launch(sums_kernel, dim3((unsigned)((a.n + 255) / 256)), 256, 0, st, "sums_kernel launch",
+      rc = stream::launch(sums_kernel, dim3((unsigned)((a.n + 31) / 32)), 256, 0, st, "sums_kernel launch",
                           (const float *)sums, a.db, (int)blocks, (int)a.n);
       if (rc) return rc;
     }

@@ -17,8 +17,8 @@ using stream::to_f32;
 // ratio: Phi(-z) = exp(-z^2 / 2) t Q(t), t = 1 / (1 + 0.3 z), z >= 0.  Q (degree 7) is a
 // weighted least-squares fit of erfcx(z / sqrt 2) / 2, off by at most 1.5e-7 of its value up
 // to z = 14 (4.8e-7 as evaluated in fp32), so the tails keep their relative accuracy; above 14
-// the exponential is below fp32's smallest.  17 instructions where normcdff, erff and a
-// division took the epilogue of 8192 x 8192 results of 4096 terms from 365 us to 516.
+// the exponential is below fp32's smallest.  16 instructions; with normcdff 8192 x 8192 results of 4096
+// terms took 516 us where they take 365 without an activation.
 __device__ __forceinline__ float exp2_of(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -44,21 +44,29 @@ __device__ __forceinline__ float normal_tail(float z, float &e) {
   e = exp2_of(z * z * (-0.5f * kLog2E));
   return t * q * e;
 }
-// |u| up to a bound, past which nothing changes (so that infinities give the limit); NaN stays.
-__device__ __forceinline__ float bounded(float u, float most) { return u > most ? most : u < -most ? -most : u; }
+// Smaller and larger of two, NaN if one is.
+__device__ __forceinline__ float smaller(float a, float b) {
+  float y;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+__device__ __forceinline__ float larger(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+// 1 / (1 + exp(-u)); below -88 the exponential is infinite and the result 0.
+__device__ __forceinline__ float sigmoid(float u) { return reciprocal(1.f + exp2_of(u * -kLog2E)); }
 
 __device__ __forceinline__ float activated(float u, int act) {
   switch (act) {
-    case OZ_ACT_RELU: return u > 0.f ? u : u != u ? u : 0.f;
+    case OZ_ACT_RELU: return larger(u, 0.f);
     case OZ_ACT_GELU: {                       // u Phi(u) = max(u, 0) - |u| Phi(-|u|)
       float e;
-      const float z = fabsf(bounded(u, 40.f));
-      return fmaxf(u, 0.f) - z * normal_tail(z, e);
+      const float z = smaller(fabsf(u), 40.f);
+      return larger(u, 0.f) - z * normal_tail(z, e);
     }
-    case OZ_ACT_SILU: {                       // with exp(-|u|): no overflow
-      const float e = exp2_of(fabsf(u) * -kLog2E), r = reciprocal(1.f + e);
-      return u >= 0.f ? u * r : (u < -200.f ? -200.f : u) * (e * r);
-    }
+    case OZ_ACT_SILU: return u * sigmoid(u);
     default: return u;
   }
 }
@@ -67,15 +75,12 @@ __device__ __forceinline__ float slope(float u, int act) {
     case OZ_ACT_RELU: return u > 0.f ? 1.f : u != u ? u : 0.f;
     case OZ_ACT_GELU: {
       float e;
-      u = bounded(u, 40.f);
-      const float h = normal_tail(fabsf(u), e);
-      return fmaf(u * 0.3989422804014327f, e, u >= 0.f ? 1.f - h : h);
+      const float z = smaller(fabsf(u), 40.f), h = normal_tail(z, e);
+      return fmaf(copysignf(z, u) * 0.3989422804014327f, e, u >= 0.f ? 1.f - h : h);
     }
     case OZ_ACT_SILU: {
-      u = bounded(u, 200.f);
-      const float e = exp2_of(fabsf(u) * -kLog2E), r = reciprocal(1.f + e);
-      const float s = u >= 0.f ? r : e * r, rest = u >= 0.f ? e * r : r;    // sigmoid(u), sigmoid(-u)
-      return s * fmaf(u, rest, 1.f);
+      const float s = sigmoid(u);
+      return s * fmaf(u, 1.f - s, 1.f);
     }
     default: return 1.f;
   }
@@ -108,11 +113,11 @@ struct Side {
   bool mn;
 };
 
-// oz_linear_split.cu: results of few tiles, the contraction over the CTAs of a cluster.
-// `plan` says how (rows of a tile, CTAs of a cluster), or 0 rows where the tile engine is
-// the faster way.
+// oz_linear_split.cu: results of few tiles of 128 columns by `tile_rows` (16, 64 or 128; 16
+// only where the rows are not stored across the contraction), the contraction over `splits`
+// CTAs of a cluster.
+constexpr int kMostSplits = 8;
 struct SplitPlan { int tile_rows, splits; };
-SplitPlan split_plan(int64_t rows, int64_t k, int64_t n, bool rows_mn);
 int split_product(const SplitPlan &plan, int dtype, int out_dtype, const Side &a, const Side &b, const Params &p,
                   cudaStream_t st, const char *what);
 

@@ -23,9 +23,9 @@ namespace {
 using namespace tile;
 using namespace linear;
 
-constexpr int kSplitThreads = 192;            // producer, MMA, 4 warps that finish
+constexpr int kFinishWarps = 8;               // they read the sums, join and finish them
+constexpr int kSplitThreads = 64 + 32 * kFinishWarps;
 constexpr int kSplitRoom = 106 * 1024;        // shared memory of a CTA: two an SM
-constexpr int kMostSplits = 8;
 constexpr int kPassBlocks = 8;                // of an accumulator where the result is fp32
 
 template <int NT> __host__ __device__ constexpr int split_stage() { return kRows * kLine + NT * kLine; }
@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], 4);
+      mbar_init(&acc_empty[i], kFinishWarps);
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -193,10 +193,12 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
       mbar_settle(drain, 0, abort_flag, DEV_TIMEOUT_MMA);
     }
   } else {
-    // sums to shared memory: the last accumulator is there, so the products are done with it
-    const int sub = warp & 3, rows = min(p.rows - row0, NT);
-    const uint32_t columns = tmem + ((uint32_t)(sub * 32) << 16);
-    const int c = sub * 32 + lane;
+    // sums to shared memory (once the last accumulator is there, the products are done with
+    // it): two warps a quarter of the lanes, half of the rows each
+    constexpr int HALF = NT / 2 < 16 ? 16 : NT / 2;
+    const int sub = warp & 3, from = (warp - 2) / 4 * HALF, rows = min(min(p.rows - row0, NT) - from, min(HALF, NT - from));
+    const uint32_t columns = tmem + ((uint32_t)(sub * 32) << 16) + (uint32_t)from;
+    float *to = partial + from * kRows + sub * 32 + lane;
     uint32_t done = 0;
     auto acquire = [&]() {
       const bool ok = mbar_wait_bounded(&acc_full[done & 1], (done >> 1) & 1, abort_flag, DEV_TIMEOUT_EPILOGUE);
@@ -205,18 +207,20 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
       return true;
     };
     if constexpr (sizeof(O) == 4) {
-      float sum[NT];
+      float sum[HALF];
 #pragma unroll
-      for (int r = 0; r < NT; ++r) sum[r] = 0.f;
+      for (int r = 0; r < HALF; ++r) sum[r] = 0.f;
       for (int kb = first; kb < last; kb += PASS) {
         if (!acquire()) break;
+        if (rows > 0) {
 #pragma unroll
-        for (int r0 = 0; r0 < NT; r0 += 16) {
-          uint32_t v[16];
-          tmem_ld16_at(columns + (uint32_t)((done & 1) * NT + r0), v);
-          tmem_ld_wait16(v);
+          for (int r0 = 0; r0 < HALF; r0 += 16) {
+            uint32_t v[16];
+            tmem_ld16_at(columns + (uint32_t)((done & 1) * NT + r0), v);
+            tmem_ld_wait16(v);
 #pragma unroll
-          for (int x = 0; x < 16; ++x) sum[r0 + x] += __uint_as_float(v[x]);
+            for (int x = 0; x < 16; ++x) sum[r0 + x] += __uint_as_float(v[x]);
+          }
         }
         tc_fence_before();
         __syncwarp();
@@ -224,8 +228,8 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
         ++done;
       }
 #pragma unroll
-      for (int r = 0; r < NT; ++r)
-        if (r < rows) partial[r * kRows + c] = sum[r];
+      for (int r = 0; r < HALF; ++r)
+        if (r < rows) to[r * kRows] = sum[r];
     } else {
       acquire();
 #pragma unroll 1
@@ -235,7 +239,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
         tmem_ld_wait16(v);
 #pragma unroll
         for (int x = 0; x < 16; ++x)
-          if (r0 + x < rows) partial[(r0 + x) * kRows + c] = __uint_as_float(v[x]);
+          if (r0 + x < rows) to[(r0 + x) * kRows] = __uint_as_float(v[x]);
       }
     }
   }
@@ -250,34 +254,53 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
       if (p.bias_f32) load4(static_cast<const float *>(p.bias) + column, p.vectors & kBiasVectors, count, bias);
       else load4(static_cast<const T *>(p.bias) + column, p.vectors & kBiasVectors, count, bias);
     }
-    for (int r = rank + (warp - 2) * splits; r < rows; r += 4 * splits) {
-      const int64_t row = row0 + r;
-      float residual[4] = {};
-      if (p.residual && count > 0)
-        load4(static_cast<const O *>(p.residual) + row * p.residual_ld + column, p.vectors & kResidualVectors, count,
-              residual);
-      float u[4];
-      if (splits > 1) {
-        float4 v[kMostSplits];
+    if (count > 0) {
+      // two rows side by side: one's way through the instructions hides the other's
+      constexpr int AT_ONCE = 2;
+      const int step = kFinishWarps * splits;
+      for (int r0 = rank + (warp - 2) * splits; r0 < rows; r0 += AT_ONCE * step) {
+        float u[AT_ONCE][4], residual[AT_ONCE][4];
+        if (p.residual)
 #pragma unroll
-        for (int s = 0; s < kMostSplits; ++s)
-          if (s < splits) v[s] = load_cluster(map_to_cta(mine + (uint32_t)(r * kRows * 4), s));
-        u[0] = v[0].x, u[1] = v[0].y, u[2] = v[0].z, u[3] = v[0].w;
+          for (int i = 0; i < AT_ONCE; ++i)
+            if (r0 + i * step < rows)
+              load4(static_cast<const O *>(p.residual) + (int64_t)(row0 + r0 + i * step) * p.residual_ld + column,
+                    p.vectors & kResidualVectors, count, residual[i]);
+        float4 v[AT_ONCE][kMostSplits];
 #pragma unroll
-        for (int s = 1; s < kMostSplits; ++s)
-          if (s < splits) u[0] += v[s].x, u[1] += v[s].y, u[2] += v[s].z, u[3] += v[s].w;
-      } else {
-        const float4 v = *reinterpret_cast<const float4 *>(partial + r * kRows + lane * 4);
-        u[0] = v.x, u[1] = v.y, u[2] = v.z, u[3] = v.w;
+        for (int i = 0; i < AT_ONCE; ++i) {
+          const int r = min(r0 + i * step, rows - 1);
+          if (splits > 1) {
+#pragma unroll
+            for (int s = 0; s < kMostSplits; ++s)
+              if (s < splits) v[i][s] = load_cluster(map_to_cta(mine + (uint32_t)(r * kRows * 4), s));
+          } else {
+            v[i][0] = *reinterpret_cast<const float4 *>(partial + r * kRows + lane * 4);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+          u[i][0] = v[i][0].x, u[i][1] = v[i][0].y, u[i][2] = v[i][0].z, u[i][3] = v[i][0].w;
+#pragma unroll
+          for (int s = 1; s < kMostSplits; ++s)
+            if (s < splits) u[i][0] += v[i][s].x, u[i][1] += v[i][s].y, u[i][2] += v[i][s].z, u[i][3] += v[i][s].w;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) u[i][x] += bias[x];
+        }
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+          if (r0 + i * step >= rows) continue;
+          const int64_t at = (int64_t)(row0 + r0 + i * step) * p.ld + column;
+          if (p.pre) store4(static_cast<T *>(p.pre) + at, p.vectors & kVectors, count, u[i]);
+          if (p.act)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) u[i][x] = activated(u[i][x], p.act);
+          if (p.residual)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) u[i][x] += residual[i][x];
+          store4(static_cast<O *>(p.out) + at, p.vectors & kVectors, count, u[i]);
+        }
       }
-      if (count <= 0) continue;
-      const int64_t at = row * p.ld + column;
-#pragma unroll
-      for (int x = 0; x < 4; ++x) u[x] += bias[x];
-      if (p.pre) store4(static_cast<T *>(p.pre) + at, p.vectors & kVectors, count, u);
-#pragma unroll
-      for (int x = 0; x < 4; ++x) u[x] = activated(u[x], p.act) + residual[x];
-      store4(static_cast<O *>(p.out) + at, p.vectors & kVectors, count, u);
     }
   }
   tc_fence_before();
@@ -342,16 +365,6 @@ int split_of(const SplitPlan &plan, const Side &a, const Side &b, const Params &
 }  // namespace
 
 namespace linear {
-
-SplitPlan split_plan(int64_t rows, int64_t k, int64_t n, bool rows_mn) {
-  SplitPlan plan{rows <= 16 && !rows_mn ? 16 : rows <= 64 ? 64 : 128, 1};
-  const int64_t tiles = (rows + plan.tile_rows - 1) / plan.tile_rows * ((n + kRows - 1) / kRows);
-  const int64_t blocks = (k + kBlock - 1) / kBlock, sms = tile::sm_count();
-  // up to two CTAs an SM, two blocks a CTA at least
-  while (plan.splits < kMostSplits && tiles * plan.splits * 2 <= 2 * sms && blocks >= plan.splits * 4) plan.splits *= 2;
-  if (rows > 128 && tiles * plan.splits > 2 * sms) plan.tile_rows = 0;
-  return plan;
-}
 
 int split_product(const SplitPlan &plan, int dtype, int out_dtype, const Side &a, const Side &b, const Params &p,
                   cudaStream_t st, const char *what) {

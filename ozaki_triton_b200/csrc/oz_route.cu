@@ -26,40 +26,76 @@ using namespace stream;
 
 constexpr int kMaxPicks = 32, kMaxExperts = 1024;
 constexpr int kMaxChunk = 256;                // tokens of a block's round
-constexpr uint32_t kNothing = 0x007FFFFFu;    // ordered form of -inf
+constexpr int kNothing = (int)0x807FFFFF;     // key of -inf; INT_MIN: no expert
 
-// Order-preserving whole numbers of fp32 values: NaN above all, the two zeros equal.
-__device__ __forceinline__ uint32_t ordered(float f) {
-  const uint32_t u = __float_as_uint(f + 0.f);
-  if (f != f) return 0xFFFFFFFFu;
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+// Whole numbers in the order of fp32 values: NaN above all (an addition gives the positive
+// one), the two zeros equal.
+__device__ __forceinline__ int key_of(float f) {
+  const int u = __float_as_int(f + 0.f);
+  return u ^ (u >> 31 & 0x7FFFFFFF);
 }
-__device__ __forceinline__ float unordered(uint32_t u) {
-  return __uint_as_float(u & 0x80000000u ? u & 0x7FFFFFFFu : ~u);
+__device__ __forceinline__ float value_of(int key) { return __int_as_float(key ^ (key >> 31 & 0x7FFFFFFF)); }
+// exp(x) for x <= 0: off by |x| + 3 units of 2^-24 of its value.
+__device__ __forceinline__ float exp_of(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
+  return y;
+}
+
+// Where logits lie: LPT lanes take a token, 4 consecutive experts each in turn, so lane l's
+// element 4 q + x is expert 4 (q LPT + l) + x.
+struct Logits {
+  const void *p;
+  int64_t rows, row, col;
+  int e, dtype, vectors;       // rows may be read 4 elements at a time
+};
+template <int LPT> __device__ __forceinline__ int expert_of(int i, int l) { return (i / 4 * LPT + l) * 4 + i % 4; }
+
+template <int LPT, int VPL, typename T>
+__device__ __forceinline__ void load_row(const Logits &g, int64_t t, bool there, int l, float (&v)[VPL]) {
+  const T *from = static_cast<const T *>(g.p) + t * g.row;
+#pragma unroll
+  for (int i = 0; i < VPL; i += 4) {
+    const int e = expert_of<LPT>(i, l);
+    if (g.vectors) {                          // whole groups of 4
+      if (there && e < g.e) {
+        if constexpr (sizeof(T) == 4) {
+          const float4 u = __ldg(reinterpret_cast<const float4 *>(from + e));
+          v[i] = u.x, v[i + 1] = u.y, v[i + 2] = u.z, v[i + 3] = u.w;
+        } else {
+          const uint2 u = __ldg(reinterpret_cast<const uint2 *>(from + e));
+          const T *w = reinterpret_cast<const T *>(&u);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) v[i + x] = to_f32(w[x]);
+        }
+      } else {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) v[i + x] = -INFINITY;
+      }
+    } else {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) v[i + x] = there && e + x < g.e ? to_f32(from[(e + x) * g.col]) : -INFINITY;
+    }
+  }
+}
+template <int LPT, int VPL>
+__device__ __forceinline__ void load_row(const Logits &g, int64_t t, bool there, int l, float (&v)[VPL]) {
+  if (g.dtype == OZ_F32) load_row<LPT, VPL, float>(g, t, there, l, v);
+  else if (g.dtype == OZ_F16) load_row<LPT, VPL, __half>(g, t, there, l, v);
+  else load_row<LPT, VPL, __nv_bfloat16>(g, t, there, l, v);
 }
 
 struct RouteParams {
-  const void *logits;
+  Logits logits;
   float *weights, *loss;
   int *experts, *slots, *offsets, *counts, *tokens;
   int *hist;                   // picks of each block and expert, and ...
   float *psum;                 // ... its sums of p, and its tokens
   int *held;
-  int64_t rows, row, col;
+  int64_t rows;
   int e, k, normalize, chunk, per, blocks;    // tokens of a round, rounds of a block
 };
 
-// A token's logits lie in LPT lanes, value i of lane l being expert i * LPT + l.
-template <typename T, int LPT, int VPL> struct Row {
-  static __device__ __forceinline__ void load(const RouteParams &p, int64_t t, bool there, int l, float (&v)[VPL]) {
-    const T *from = static_cast<const T *>(p.logits) + t * p.row;
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      const int e = i * LPT + l;
-      v[i] = there && e < p.e ? to_f32(from[e * p.col]) : -INFINITY;
-    }
-  }
-};
 template <int LPT, typename F> __device__ __forceinline__ float over_lanes(float v, F f) {
 #pragma unroll
   for (int o = LPT / 2; o > 0; o /= 2) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
@@ -68,6 +104,59 @@ template <int LPT, typename F> __device__ __forceinline__ float over_lanes(float
 template <int LPT> __device__ __forceinline__ float lanes_sum(float v) {
   return over_lanes<LPT>(v, [](float a, float b) { return a + b; });
 }
+
+// The K largest of what has been put in, the largest first, the lowest expert first among
+// equals.
+template <int K> struct Largest {
+  int key[K], expert[K];
+  __device__ __forceinline__ Largest() {
+#pragma unroll
+    for (int j = 0; j < K; ++j) key[j] = (int)0x80000000, expert[j] = 0;
+  }
+  // Elements come in the order of their experts: an equal one goes behind, and from its
+  // place on all others move by one.
+  __device__ __forceinline__ void put(int x, int e) {
+    bool before = false;
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+      before = before || x > key[j];
+      const int k0 = key[j], e0 = expert[j];
+      key[j] = before ? x : k0;
+      expert[j] = before ? e : e0;
+      x = before ? k0 : x;
+      e = before ? e0 : e;
+    }
+  }
+  static __device__ __forceinline__ bool precedes(int k0, int e0, int k1, int e1) {
+    return k0 > k1 || (k0 == k1 && e0 < e1);
+  }
+  // Joins the lists of LPT lanes: of two sorted lists the better of the j-th and the
+  // other's j-th from the end are the K best, falling then rising, and are sorted in
+  // log K steps.  Both lanes of a pair end with the same list.
+  template <int LPT> __device__ __forceinline__ void join() {
+#pragma unroll 1
+    for (int o = 1; o < LPT; o *= 2) {
+      int k1[K], e1[K];
+#pragma unroll
+      for (int j = 0; j < K; ++j) {
+        k1[j] = __shfl_xor_sync(0xffffffffu, key[K - 1 - j], o);
+        e1[j] = __shfl_xor_sync(0xffffffffu, expert[K - 1 - j], o);
+      }
+#pragma unroll
+      for (int j = 0; j < K; ++j)
+        if (precedes(k1[j], e1[j], key[j], expert[j])) key[j] = k1[j], expert[j] = e1[j];
+#pragma unroll
+      for (int s = K / 2; s > 0; s /= 2)
+#pragma unroll
+        for (int j = 0; j < K; ++j)
+          if ((j & s) == 0 && precedes(key[j + s], expert[j + s], key[j], expert[j])) {
+            const int k0 = key[j], e0 = expert[j];
+            key[j] = key[j + s], expert[j] = expert[j + s];
+            key[j + s] = k0, expert[j + s] = e0;
+          }
+    }
+  }
+};
 
 // Exclusive prefix sums of n counts in shared memory, by the first warp; total in from[n].
 __device__ __forceinline__ void scan(int *from, int n) {
@@ -94,13 +183,17 @@ int route_smem(int e, int k, int chunk, int warps) {
   return 4 * (e * (chunk / 32) + 2 * (e + 1) + warps * e + chunk * k + chunk + 1) + 2 * chunk * k;
 }
 
-// Picks of `per` rounds of `chunk` tokens a block.  A token's picks are found by k
-// maxima over its lanes; ranks among the tokens of a round come from one bit a
-// token and expert in shared memory (set in any order, counted by popc), so there
-// is no sort.  With one block of one round the rows are final, else they count
-// from the block's first pick of the expert and route_place adds the rest.
-template <typename T, int LPT, int VPL>
-__global__ void __launch_bounds__(VPL <= 8 ? 1024 : VPL == 16 ? 512 : 256) route_pick(const RouteParams p) {
+template <int VPL, int K> __host__ __device__ constexpr int pick_threads() { return VPL == 16 && K <= 8 ? 512 : 256; }
+
+// Picks of `per` rounds of `chunk` tokens a block.  A lane puts its part of a token's logits
+// into a sorted list of K, and the LPT lanes of the token join their lists: 5
+// instructions an expert and place of the list (k maxima over all lanes took 2440
+// instructions for 4 tokens of 64 experts and 8 picks, this 700).  Ranks among the tokens of
+// a round come from one bit a token and expert in shared memory (set in any order, counted
+// by popc), so there is no sort.  With one block of one round the rows are final, else
+// they count from the block's first pick of the expert and route_place adds the rest.
+template <int LPT, int VPL, int K>
+__global__ void __launch_bounds__(pick_threads<VPL, K>()) route_pick(const RouteParams p) {
   extern __shared__ unsigned char smem[];
   const int words = p.chunk / 32, warps = blockDim.x / 32;
   uint32_t *bits = reinterpret_cast<uint32_t *>(smem);              // [e][words]
@@ -130,77 +223,45 @@ __global__ void __launch_bounds__(VPL <= 8 ? 1024 : VPL == 16 ? 512 : 256) route
     for (int w0 = warp * GROUPS; w0 < here; w0 += warps * GROUPS) {
       const int tl = w0 + lane / LPT;
       float v[VPL];
-      Row<T, LPT, VPL>::load(p, t0 + tl, tl < here, l, v);
-      uint32_t key[VPL], best = 0;
-      int at = 0;
-      auto rescan = [&]() {
-        best = 0;
-        at = 0;
+      load_row<LPT, VPL>(p.logits, t0 + tl, tl < here, l, v);
+      Largest<K> best;
 #pragma unroll
-        for (int i = 0; i < VPL; ++i)
-          if (key[i] > best) {
-            best = key[i];
-            at = i;
-          }
-      };
-#pragma unroll
-      for (int i = 0; i < VPL; ++i) key[i] = ordered(v[i]);
-      rescan();
-      // the largest of all lanes and its expert
-      auto largest = [&](uint32_t &m, int &e) {
-        m = best;
-        e = at * LPT + l;
-        if constexpr (LPT == 32) {
-          m = __reduce_max_sync(0xffffffffu, best);
-          e = (int)__reduce_min_sync(0xffffffffu, best == m ? (uint32_t)e : 0xFFFFu);
-        } else {
-#pragma unroll
-          for (int o = LPT / 2; o > 0; o /= 2) {
-            const uint32_t other = __shfl_xor_sync(0xffffffffu, m, o);
-            const int index = __shfl_xor_sync(0xffffffffu, e, o);
-            if (other > m || (other == m && index < e)) {
-              m = other;
-              e = index;
-            }
-          }
+      for (int i = 0; i < VPL; ++i)
+        if (i / 4 * 4 * LPT < p.e) {                    // the same for all lanes
+          const int e = expert_of<LPT>(i, l);
+          best.put(e < p.e ? key_of(v[i]) : (int)0x80000000, e);
         }
-      };
-      uint32_t m;
-      int e;
-      largest(m, e);
-      const bool real_row = m > kNothing;
-      const float top = real_row ? unordered(m) : 0.f;
+      best.template join<LPT>();
+      const bool real_row = best.key[0] > kNothing;
+      const float top = real_row ? value_of(best.key[0]) : 0.f;
       float sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < VPL; ++i) {
-        v[i] = expf(v[i] - top);
-        sum += v[i];
-      }
+      for (int i = 0; i < VPL; ++i)
+        if (i / 4 * 4 * LPT < p.e) {
+          v[i] = exp_of(v[i] - top);
+          sum += v[i];
+        }
       sum = lanes_sum<LPT>(sum);
       const float inverse = real_row ? 1.f / sum : 0.f;
 #pragma unroll
-      for (int i = 0; i < VPL; ++i) acc[i] += real_row ? v[i] * inverse : 0.f;
+      for (int i = 0; i < VPL; ++i)
+        if (i / 4 * 4 * LPT < p.e) acc[i] += real_row ? v[i] * inverse : 0.f;
+      // picks l, l + LPT, ... are this lane's to write
       float picked = 0.f;
-      for (int j = 0; j < p.k; ++j) {
-        if (j) largest(m, e);
-        const bool real = m > kNothing;
-        const float x = real ? expf(unordered(m) - top) : 0.f;
-        picked += x;
-        if (l == 0 && tl < here) {
-          pick_e[tl * p.k + j] = real ? (int16_t)e : (int16_t)-1;
-          pick_w[tl * p.k + j] = x;
-          if (real) atomicOr(&bits[e * words + tl / 32], 1u << (tl % 32));
-        }
-        if (e % LPT == l) {
 #pragma unroll
-          for (int i = 0; i < VPL; ++i)
-            if (i == e / LPT) key[i] = 0;
-          rescan();
-        }
-        __syncwarp();
+      for (int j = 0; j < K; ++j) {
+        if (j % LPT != l || j >= p.k || tl >= here) continue;
+        const bool real = best.key[j] > kNothing;
+        const int e = best.expert[j];
+        const float x = real ? exp_of(value_of(best.key[j]) - top) : 0.f;
+        picked += x;
+        pick_e[tl * p.k + j] = real ? (int16_t)e : (int16_t)-1;
+        pick_w[tl * p.k + j] = x;
+        if (real) atomicOr(&bits[e * words + tl / 32], 1u << (tl % 32));
       }
+      if (p.normalize) sum = lanes_sum<LPT>(picked);
       if (l == 0 && tl < here) {
-        total[tl] = real_row ? (p.normalize ? picked : sum) : 1.f;
+        total[tl] = real_row ? sum : 1.f;
         if (real_row) atomicAdd(held, 1);
       }
     }
@@ -243,7 +304,7 @@ __global__ void __launch_bounds__(VPL <= 8 ? 1024 : VPL == 16 ? 512 : 256) route
   for (int i = 0; i < VPL; ++i) {
 #pragma unroll
     for (int o = LPT; o < 32; o *= 2) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], o);
-    if (lane < LPT && i * LPT + l < p.e) sums[warp * p.e + i * LPT + l] = acc[i];
+    if (lane < LPT && expert_of<LPT>(i, l) < p.e) sums[warp * p.e + expert_of<LPT>(i, l)] = acc[i];
   }
   __syncthreads();
   if (p.blocks > 1) {
@@ -284,6 +345,15 @@ __global__ void __launch_bounds__(512) route_place(const RouteParams p) {
   int *part = base + p.e + 1;                                       // [2][groups][e]
   start_after_earlier_kernels();
   const bool last = blockIdx.x == p.blocks;
+  // this block's picks, up to 8 a thread, are on their way while the counts are added up
+  const int64_t span = (int64_t)p.chunk * p.per * p.k, i0 = blockIdx.x * span, end = min(i0 + span, p.rows * p.k);
+  int expert[8], slot[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int64_t i = i0 + threadIdx.x + j * (int64_t)blockDim.x;
+    expert[j] = !last && i < end ? p.experts[i] : -1;
+    slot[j] = expert[j] >= 0 ? p.slots[i] : 0;
+  }
   const int lanes = groups * p.e;                                   // threads at work where e < blockDim
   for (int i = threadIdx.x; i < lanes; i += blockDim.x) {
     const int e = i % p.e, g = i / p.e;
@@ -310,9 +380,10 @@ __global__ void __launch_bounds__(512) route_place(const RouteParams p) {
   __syncthreads();
   scan(total, p.e);
   if (!last) {
-    const int64_t span = (int64_t)p.chunk * p.per * p.k, i0 = blockIdx.x * span;
-    const int64_t end = min(i0 + span, p.rows * p.k);
-    for (int64_t i = i0 + threadIdx.x; i < end; i += blockDim.x) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (expert[j] >= 0) p.slots[i0 + threadIdx.x + j * (int64_t)blockDim.x] = slot[j] + total[expert[j]] + base[expert[j]];
+    for (int64_t i = i0 + threadIdx.x + 8 * (int64_t)blockDim.x; i < end; i += blockDim.x) {
       const int e = p.experts[i];
       if (e >= 0) p.slots[i] += total[e] + base[e];
     }
@@ -356,26 +427,33 @@ __global__ void __launch_bounds__(512) route_place(const RouteParams p) {
   }
 }
 
-// Lanes of a token and values of a lane for e experts, then f.run<T, LPT, VPL>().
-template <typename T, typename F> int with_layout(int e, F f) {
-  if (e <= 8) return f.template run<T, 1, 8>();
-  if (e <= 16) return f.template run<T, 2, 8>();
-  if (e <= 32) return f.template run<T, 4, 8>();
-  if (e <= 64) return f.template run<T, 8, 8>();
-  if (e <= 128) return f.template run<T, 16, 8>();
-  if (e <= 256) return f.template run<T, 32, 8>();
-  if (e <= 512) return f.template run<T, 32, 16>();
-  return f.template run<T, 32, 32>();
+// Lanes of a token and values of a lane for e experts, then f.run<LPT, VPL>().
+template <typename F> int with_layout(int e, const F &f) {
+  if (e <= 16) return f.template run<1, 16>();
+  if (e <= 32) return f.template run<2, 16>();
+  if (e <= 64) return f.template run<4, 16>();
+  if (e <= 128) return f.template run<8, 16>();
+  if (e <= 256) return f.template run<16, 16>();
+  if (e <= 512) return f.template run<32, 16>();
+  return f.template run<32, 32>();
+}
+int lanes_of(int e) {
+  int lanes = 1;
+  while (lanes < 32 && lanes * 16 < e) lanes *= 2;
+  return lanes;
+}
+Logits logits_of(const void *p, int64_t rows, int64_t row, int64_t col, int e, int dtype) {
+  const int es = dtype_size(dtype);
+  return {p, rows, row, col, e, dtype, e % 4 == 0 && col == 1 && (uintptr_t)p % (4 * es) == 0 && (rows <= 1 || row % 4 == 0)};
 }
 
 struct RoutePlan { int chunk, per, blocks; };
-// Rounds of 256 tokens, or fewer (down to 32) while that leaves SMs without a block.
+// One block where that takes 2 turns of its threads or fewer.  Else rounds of 256 tokens, or
+// fewer (down to 32) while that leaves SMs without a block.
 RoutePlan route_plan(int64_t rows, int e) {
-  const int lpt = e <= 8 ? 1 : e <= 256 ? (e <= 16 ? 2 : e <= 32 ? 4 : e <= 64 ? 8 : e <= 128 ? 16 : 32) : 32;
-  const int most = e <= 256 ? 1024 : e <= 512 ? 512 : 256;
   RoutePlan r{kMaxChunk, 1, 1};
-  if (rows <= kMaxChunk && rows <= 4 * most / lpt) {
-    r.chunk = (int)((rows + 31) / 32 * 32);
+  if (rows <= kMaxChunk && rows * lanes_of(e) <= 1024) {
+    r.chunk = (int)(std::max<int64_t>(rows, 1) + 31) / 32 * 32;
     return r;
   }
   while (r.chunk > 32 && (rows + r.chunk - 1) / r.chunk < 128) r.chunk /= 2;
@@ -388,32 +466,38 @@ RoutePlan route_plan(int64_t rows, int e) {
 struct PickLaunch {
   const RouteParams &p;
   cudaStream_t st;
-  template <typename T, int LPT, int VPL> int run() const {
-    const int most = VPL <= 8 ? 1024 : VPL == 16 ? 512 : 256;
-    const int64_t busy = min((int64_t)p.chunk, p.rows) * LPT;
-    const int threads = (int)max((int64_t)32, min((int64_t)most, (busy + 31) / 32 * 32));
-    return launch(route_pick<T, LPT, VPL>, dim3(p.blocks), threads, route_smem(p.e, p.k, p.chunk, threads / 32), st,
+  template <int LPT, int VPL, int K> int launch_it() const {
+    const int64_t busy = std::min((int64_t)p.chunk, p.rows) * LPT;
+    const int threads = (int)std::max<int64_t>(32, std::min<int64_t>(pick_threads<VPL, K>(), (busy + 31) / 32 * 32));
+    return launch(route_pick<LPT, VPL, K>, dim3(p.blocks), threads, route_smem(p.e, p.k, p.chunk, threads / 32), st,
                   "route_pick launch", p);
+  }
+  template <int LPT, int VPL> int run() const {
+    if (p.k <= 2) return launch_it<LPT, VPL, 2>();
+    if (p.k <= 4) return launch_it<LPT, VPL, 4>();
+    if (p.k <= 8) return launch_it<LPT, VPL, 8>();
+    if (p.k <= 16) return launch_it<LPT, VPL, 16>();
+    return launch_it<LPT, VPL, 32>();
   }
 };
 
 struct RouteBackward {
-  const void *logits;
+  Logits logits;
   const float *dweights, *dloss, *weights;
   const int *experts, *counts, *tokens;
   void *dlogits;
-  int64_t rows, row, col;
+  int64_t rows;
   int e, k, normalize;
 };
 
-// dlogits, LPT lanes a token: the softmax again from the logits, the picks' part
-// added by the lanes that hold them.
-template <typename T, int LPT, int VPL>
-__global__ void __launch_bounds__(256) route_backward(const RouteBackward p) {
+// dlogits, LPT lanes a token: the softmax again from the logits; a token's row then goes
+// through shared memory, where one lane for each pick adds its part.
+template <int LPT, int VPL> __global__ void __launch_bounds__(256) route_backward(const RouteBackward p) {
   extern __shared__ unsigned char smem[];
-  float *slope = reinterpret_cast<float *>(smem);                   // [e]: the loss's part of g
-  constexpr int GROUPS = 32 / LPT;
+  constexpr int GROUPS = 32 / LPT, WIDE = LPT * VPL;
+  float *slope = reinterpret_cast<float *>(smem);                   // [WIDE]: the loss's part of g
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, l = lane % LPT;
+  float *line = slope + WIDE + (warp * GROUPS + lane / LPT) * WIDE; // this token's row
   start_after_earlier_kernels();
   // sum of the counts, by every warp for itself
   int sum_n = 0;
@@ -422,19 +506,20 @@ __global__ void __launch_bounds__(256) route_backward(const RouteBackward p) {
   for (int o = 16; o > 0; o /= 2) sum_n += __shfl_xor_sync(0xffffffffu, sum_n, o);
   const int tokens = *p.tokens;
   const double scale = p.dloss && tokens > 0 && sum_n > 0 ? (double)*p.dloss * p.e / ((double)tokens * sum_n) : 0.0;
-  for (int e = threadIdx.x; e < p.e; e += blockDim.x) slope[e] = (float)(scale * p.counts[e]);
+  for (int e = threadIdx.x; e < WIDE; e += blockDim.x) slope[e] = e < p.e ? (float)(scale * p.counts[e]) : 0.f;
   __syncthreads();
   const int64_t step = (int64_t)gridDim.x * (blockDim.x / 32) * GROUPS;
   for (int64_t w0 = ((int64_t)blockIdx.x * (blockDim.x / 32) + warp) * GROUPS; w0 < p.rows; w0 += step) {
     const int64_t t = w0 + lane / LPT;
     const bool there = t < p.rows;
     float v[VPL];
-    const T *from = static_cast<const T *>(p.logits) + t * p.row;
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      const int e = i * LPT + l;
-      v[i] = there && e < p.e ? to_f32(from[e * p.col]) : -INFINITY;
-    }
+    load_row<LPT, VPL>(p.logits, t, there, l, v);
+    // the picks' part by lanes l, l + LPT, ...: w dw over the row first
+    float dot = 0.f;
+    if (p.dweights && there)
+      for (int j = l; j < p.k; j += LPT)
+        if (p.experts[t * p.k + j] >= 0) dot = fmaf(p.weights[t * p.k + j], p.dweights[t * p.k + j], dot);
+    dot = lanes_sum<LPT>(dot);
     float top = v[0];
     bool odd = false;                                               // a NaN makes the sum one
 #pragma unroll
@@ -447,56 +532,71 @@ __global__ void __launch_bounds__(256) route_backward(const RouteBackward p) {
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
-      v[i] = real || odd ? expf(v[i] - top) : 0.f;
+      v[i] = real || odd ? exp_of(v[i] - top) : 0.f;
       sum += v[i];
     }
     sum = lanes_sum<LPT>(sum);
     const float inverse = sum != 0.f ? 1.f / sum : 0.f;
     float inner = 0.f;
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      v[i] *= inverse;
-      const int e = i * LPT + l;
-      inner += v[i] * (e < p.e ? slope[e] : 0.f);
+    for (int i = 0; i < VPL; i += 4) {
+      const float4 g = *reinterpret_cast<const float4 *>(slope + expert_of<LPT>(i, l));
+      v[i] *= inverse, v[i + 1] *= inverse, v[i + 2] *= inverse, v[i + 3] *= inverse;
+      inner = fmaf(v[i], g.x, fmaf(v[i + 1], g.y, fmaf(v[i + 2], g.z, fmaf(v[i + 3], g.w, inner))));
     }
     inner = lanes_sum<LPT>(inner);
-    // what the picks add: w dw over the row
-    float dot = 0.f;
-    if (p.dweights && there)
-      for (int j = l; j < p.k; j += LPT)
-        if (p.experts[t * p.k + j] >= 0) dot += p.weights[t * p.k + j] * p.dweights[t * p.k + j];
-    dot = lanes_sum<LPT>(dot);
     if (!p.normalize) inner += dot;
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      const int e = i * LPT + l;
-      v[i] *= (e < p.e ? slope[e] : 0.f) - inner;
+    for (int i = 0; i < VPL; i += 4) {
+      const float4 g = *reinterpret_cast<const float4 *>(slope + expert_of<LPT>(i, l));
+      *reinterpret_cast<float4 *>(line + expert_of<LPT>(i, l)) =
+          make_float4(v[i] * (g.x - inner), v[i + 1] * (g.y - inner), v[i + 2] * (g.z - inner), v[i + 3] * (g.w - inner));
     }
+    __syncwarp();
     if (p.dweights && there)
-      for (int j = 0; j < p.k; ++j) {
+      for (int j = l; j < p.k; j += LPT) {
         const int e = p.experts[t * p.k + j];
-        if (e < 0 || e % LPT != l) continue;
+        if (e < 0 || e >= p.e) continue;
         const float w = p.weights[t * p.k + j], d = p.dweights[t * p.k + j];
-        const float add = p.normalize ? w * (d - dot) : w * d;
-#pragma unroll
-        for (int i = 0; i < VPL; ++i)
-          if (i == e / LPT) v[i] += add;
+        line[e] += p.normalize ? w * (d - dot) : w * d;
       }
-    T *to = static_cast<T *>(p.dlogits) + t * p.e;
+    __syncwarp();
+    if (there) {
+      auto store = [&](auto z) {
+        using T = decltype(z);
+        T *to = static_cast<T *>(p.dlogits) + t * p.e;
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      const int e = i * LPT + l;
-      if (there && e < p.e) to[e] = from_f32<T>(v[i]);
+        for (int i = 0; i < VPL; i += 4) {
+          const int e = expert_of<LPT>(i, l);
+          if (e >= p.e) continue;
+          const float4 u = *reinterpret_cast<const float4 *>(line + e);
+          if (p.e % 4 == 0) {                                       // rows of whole groups, aligned
+            T w[4] = {from_f32<T>(u.x), from_f32<T>(u.y), from_f32<T>(u.z), from_f32<T>(u.w)};
+            if constexpr (sizeof(T) == 4) *reinterpret_cast<float4 *>(to + e) = u;
+            else *reinterpret_cast<uint2 *>(to + e) = *reinterpret_cast<const uint2 *>(w);
+          } else {
+            const float f[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              if (e + x < p.e) to[e + x] = from_f32<T>(f[x]);
+          }
+        }
+      };
+      if (p.logits.dtype == OZ_F32) store(float{});
+      else if (p.logits.dtype == OZ_F16) store(__half{});
+      else store(__nv_bfloat16{});
     }
+    __syncwarp();
   }
 }
 
 struct BackwardLaunch {
   const RouteBackward &p;
   cudaStream_t st;
-  template <typename T, int LPT, int VPL> int run() const {
+  template <int LPT, int VPL> int run() const {
     const int64_t blocks = (p.rows * LPT + 255) / 256;
-    return launch(route_backward<T, LPT, VPL>, dim3((unsigned)min(blocks, (int64_t)sm_count() * 8)), 256, p.e * 4, st,
+    constexpr int smem = (1 + 8 * (32 / LPT)) * LPT * VPL * 4;
+    return launch(route_backward<LPT, VPL>, dim3((unsigned)std::min(blocks, (int64_t)sm_count() * 4)), 256, smem, st,
                   "route_backward launch", p);
   }
 };
@@ -743,15 +843,17 @@ extern "C" int oz_route(const oz_route_args *args, void *stream) {
   if (bytes && (!a.workspace || (uintptr_t)a.workspace % 16 != 0 || a.workspace_bytes < bytes))
     return set_error(OZ_ERR_INVALID, "workspace of %lld bytes (16-byte aligned) needed, got %lld at %p",
                      (long long)bytes, (long long)a.workspace_bytes, a.workspace);
-  RouteParams p{a.logits, a.weights, a.loss, a.chosen, a.slots, a.offsets, a.counts, a.tokens, nullptr, nullptr,
-                nullptr, a.rows, a.row, a.col, a.experts, a.picks, a.normalize, r.chunk, r.per, r.blocks};
-  if (p.chunk == 0) p.chunk = 32;
+  if (a.dtype != OZ_F32 && a.dtype != OZ_F16 && a.dtype != OZ_BF16)
+    return set_error(OZ_ERR_UNSUPPORTED, "unsupported dtype %d (fp32, fp16 or bf16)", a.dtype);
+  RouteParams p{logits_of(a.logits, a.rows, a.row, a.col, a.experts, a.dtype), a.weights, a.loss, a.chosen, a.slots,
+                a.offsets, a.counts, a.tokens, nullptr, nullptr, nullptr, a.rows, a.experts, a.picks, a.normalize,
+                r.chunk, r.per, r.blocks};
   if (bytes) {
     p.hist = static_cast<int *>(a.workspace);
     p.psum = reinterpret_cast<float *>(p.hist + (int64_t)r.blocks * a.experts);
     p.held = reinterpret_cast<int *>(p.psum + (int64_t)r.blocks * a.experts);
   }
-  const int rc = with_type(a.dtype, [&](auto v) { return with_layout<decltype(v)>(a.experts, PickLaunch{p, st}); });
+  const int rc = with_layout(a.experts, PickLaunch{p, st});
   if (rc || r.blocks <= 1) return rc;
   const int groups = max(1, 512 / a.experts);
   return launch(route_place, dim3(r.blocks + 1), 512, 4 * (2 * (a.experts + 1) + 2 * groups * a.experts), st,
@@ -770,9 +872,12 @@ extern "C" int oz_route_backward(const oz_route_backward_args *args, void *strea
   if (!a.logits || !a.weights || !a.chosen || !a.counts || !a.tokens || !a.dlogits)
     return set_error(OZ_ERR_INVALID, "null pointer");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const RouteBackward p{a.logits, a.dweights, a.dloss, a.weights, a.chosen, a.counts, a.tokens, a.dlogits,
-                        a.rows, a.row, a.col, a.experts, a.picks, a.normalize};
-  return with_type(a.dtype, [&](auto v) { return with_layout<decltype(v)>(a.experts, BackwardLaunch{p, st}); });
+  if (a.dtype != OZ_F32 && a.dtype != OZ_F16 && a.dtype != OZ_BF16)
+    return set_error(OZ_ERR_UNSUPPORTED, "unsupported dtype %d (fp32, fp16 or bf16)", a.dtype);
+  if ((uintptr_t)a.dlogits % 16 != 0) return set_error(OZ_ERR_INVALID, "dlogits must start on a 16-byte boundary");
+  const RouteBackward p{logits_of(a.logits, a.rows, a.row, a.col, a.experts, a.dtype), a.dweights, a.dloss, a.weights,
+                        a.chosen, a.counts, a.tokens, a.dlogits, a.rows, a.experts, a.picks, a.normalize};
+  return with_layout(a.experts, BackwardLaunch{p, st});
 }
 
 extern "C" int oz_dispatch(const oz_rows_args *args, void *stream) {
