@@ -8,10 +8,11 @@ from typing import Iterable, Optional, Sequence
 import torch
 
 from . import _lib
-from .api import _OZ_DTYPE, _check_cuda
-from .experts import _CURRENT_DEVICE, _LEVEL, _OnDevice, _check_tangents, _stream_of
+from .api import _OZ_DTYPE
+from .experts import _CURRENT_DEVICE, _LEVEL, _OnDevice, _check_places, _check_tangents, _stream_of
 
 CLIP_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+_CODES = {t: _OZ_DTYPE[t] for t in CLIP_DTYPES}
 
 
 def _dense(t: torch.Tensor) -> bool:
@@ -52,26 +53,27 @@ def clip_gradients(grads: Iterable[torch.Tensor], max_norm: float, *, eps: float
     n = len(grads)
     device = grads[0].get_device()
     for t in grads if out is None else grads + outs:
-        assert t.dtype in CLIP_DTYPES, f"unsupported dtype: {t.dtype}"
-        _check_cuda(t)
-        if t.get_device() != device:
-            raise ValueError(f"tensors on different devices: cuda:{device} and {t.device}")
-        assert _dense(t), f"a gradient of shape {tuple(t.shape)} and strides {t.stride()} is not dense"
+        if t.dtype not in _CODES:
+            raise AssertionError(f"unsupported dtype: {t.dtype}")
+        if t.get_device() != device or device < 0:
+            _check_places(grads[0], t)
+        if not t.is_contiguous() and not _dense(t):
+            raise AssertionError(f"a gradient of shape {tuple(t.shape)} and strides {t.stride()} is not dense")
     if out is not None:
         for g, o in zip(grads, outs):
-            assert g.shape == o.shape and (g.stride() == o.stride() or (g.is_contiguous() and o.is_contiguous())), \
-                f"a result must be laid out like its gradient: {tuple(o.shape)}, strides {o.stride()} for " \
-                f"{tuple(g.shape)}, strides {g.stride()}"
+            if g.shape != o.shape or (g.stride() != o.stride() and not (g.is_contiguous() and o.is_contiguous())):
+                raise AssertionError(f"a result must be laid out like its gradient: {tuple(o.shape)}, strides "
+                                     f"{o.stride()} for {tuple(g.shape)}, strides {g.stride()}")
     lib = _lib.load()
-    norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
+    norm = grads[0].new_empty((), dtype=torch.float32)
     size = lib.oz_clip_workspace_bytes(n)
-    workspace = torch.empty((size,), dtype=torch.uint8, device=grads[0].device)
+    workspace = grads[0].new_empty((size,), dtype=torch.uint8)
     pointers = ctypes.c_void_p * n
     from_ = pointers(*[t.data_ptr() for t in grads])
     to = from_ if out is None else pointers(*[t.data_ptr() for t in outs])
     sizes = (ctypes.c_int64 * n)(*[t.numel() for t in grads])
-    types = (ctypes.c_int32 * n)(*[_OZ_DTYPE[t.dtype] for t in grads])
-    out_types = types if out is None else (ctypes.c_int32 * n)(*[_OZ_DTYPE[t.dtype] for t in outs])
+    types = (ctypes.c_int32 * n)(*[_CODES[t.dtype] for t in grads])
+    out_types = types if out is None else (ctypes.c_int32 * n)(*[_CODES[t.dtype] for t in outs])
     address = ctypes.addressof
     args = _lib.ClipArgs(address(from_), address(to), address(sizes), address(types), address(out_types),
                          norm.data_ptr(), workspace.data_ptr(), size, float(max_norm), float(eps), n, 0)

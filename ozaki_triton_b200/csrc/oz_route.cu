@@ -26,7 +26,6 @@ using namespace stream;
 
 constexpr int kMaxPicks = 32, kMaxExperts = 1024;
 constexpr int kMaxChunk = 256;                // tokens of a block's round
-constexpr int kNothing = (int)0x807FFFFF;     // key of -inf; INT_MIN: no expert
 
 // Whole numbers in the order of fp32 values: NaN above all (an addition gives the positive
 // one), the two zeros equal.
@@ -34,7 +33,6 @@ __device__ __forceinline__ int key_of(float f) {
   const int u = __float_as_int(f + 0.f);
   return u ^ (u >> 31 & 0x7FFFFFFF);
 }
-__device__ __forceinline__ float value_of(int key) { return __int_as_float(key ^ (key >> 31 & 0x7FFFFFFF)); }
 // exp(x) for x <= 0: off by |x| + 3 units of 2^-24 of its value.
 __device__ __forceinline__ float exp_of(float x) {
   float y;
@@ -85,13 +83,21 @@ __device__ __forceinline__ void load_row(const Logits &g, int64_t t, bool there,
   else load_row<LPT, VPL, __nv_bfloat16>(g, t, there, l, v);
 }
 
+__device__ __forceinline__ float logit(const Logits &g, int64_t t, int e) {
+  const int64_t at = t * g.row + e * g.col;
+  if (g.dtype == OZ_F32) return __ldg(static_cast<const float *>(g.p) + at);
+  if (g.dtype == OZ_F16) return to_f32(__ldg(static_cast<const __half *>(g.p) + at));
+  return to_f32(__ldg(static_cast<const __nv_bfloat16 *>(g.p) + at));
+}
+
 struct RouteParams {
   Logits logits;
   float *weights, *loss;
   int *experts, *slots, *offsets, *counts, *tokens;
-  int *hist;                   // picks of each block and expert, and ...
-  float *psum;                 // ... its sums of p, and its tokens
-  int *held;
+  int *hist;                   // [e][blocks]: picks of each block and expert, then those before,
+  float *psum;                 // [e][blocks]: sums of p
+  int *held, *all;             // tokens of each block; picks of each expert ...
+  double *mass;                // ... and its sum of p
   int64_t rows;
   int e, k, normalize, chunk, per, blocks;    // tokens of a round, rounds of a block
 };
@@ -106,29 +112,42 @@ template <int LPT> __device__ __forceinline__ float lanes_sum(float v) {
 }
 
 // The K largest of what has been put in, the largest first, the lowest expert first among
-// equals.
-template <int K> struct Largest {
-  int key[K], expert[K];
+// equals.  A key and its expert, or with PACKED (logits of 16 bits) one number for both:
+// the key above, the lower the expert the larger below.
+constexpr int kNone = (int)0x80000000;
+template <int K, bool PACKED> struct Largest {
+  int key[K], expert[PACKED ? 1 : K];
   __device__ __forceinline__ Largest() {
 #pragma unroll
-    for (int j = 0; j < K; ++j) key[j] = (int)0x80000000, expert[j] = 0;
+    for (int j = 0; j < K; ++j) key[j] = kNone;
+    if constexpr (!PACKED)
+#pragma unroll
+      for (int j = 0; j < K; ++j) expert[j] = 0;
   }
-  // Elements come in the order of their experts: an equal one goes behind, and from its
-  // place on all others move by one.
-  __device__ __forceinline__ void put(int x, int e) {
+  // The i-th element; they come in the order of their experts: an equal one goes behind, and
+  // from its place on all others move by one.
+  __device__ __forceinline__ void put(int i, int x, int e) {
     bool before = false;
 #pragma unroll
     for (int j = 0; j < K; ++j) {
-      before = before || x > key[j];
-      const int k0 = key[j], e0 = expert[j];
-      key[j] = before ? x : k0;
-      expert[j] = before ? e : e0;
-      x = before ? k0 : x;
-      e = before ? e0 : e;
+      if (j > i) continue;
+      const int k0 = key[j];
+      if constexpr (PACKED) {
+        key[j] = max(k0, x);
+        x = min(k0, x);
+      } else {
+        const int e0 = expert[j];
+        before = before || x > k0;
+        key[j] = before ? x : k0;
+        expert[j] = before ? e : e0;
+        x = before ? k0 : x;
+        e = before ? e0 : e;
+      }
     }
   }
-  static __device__ __forceinline__ bool precedes(int k0, int e0, int k1, int e1) {
-    return k0 > k1 || (k0 == k1 && e0 < e1);
+  __device__ __forceinline__ bool precedes(int k0, int e0, int k1, int e1) const {
+    if constexpr (PACKED) return k0 > k1;
+    else return k0 > k1 || (k0 == k1 && e0 < e1);
   }
   // Joins the lists of LPT lanes: of two sorted lists the better of the j-th and the
   // other's j-th from the end are the K best, falling then rising, and are sorted in
@@ -136,27 +155,61 @@ template <int K> struct Largest {
   template <int LPT> __device__ __forceinline__ void join() {
 #pragma unroll 1
     for (int o = 1; o < LPT; o *= 2) {
-      int k1[K], e1[K];
+      int k1[K], e1[PACKED ? 1 : K];
 #pragma unroll
       for (int j = 0; j < K; ++j) {
         k1[j] = __shfl_xor_sync(0xffffffffu, key[K - 1 - j], o);
-        e1[j] = __shfl_xor_sync(0xffffffffu, expert[K - 1 - j], o);
+        if constexpr (!PACKED) e1[j] = __shfl_xor_sync(0xffffffffu, expert[K - 1 - j], o);
       }
 #pragma unroll
-      for (int j = 0; j < K; ++j)
-        if (precedes(k1[j], e1[j], key[j], expert[j])) key[j] = k1[j], expert[j] = e1[j];
+      for (int j = 0; j < K; ++j) {
+        if constexpr (PACKED) key[j] = max(key[j], k1[j]);
+        else if (precedes(k1[j], e1[j], key[j], expert[j])) key[j] = k1[j], expert[j] = e1[j];
+      }
 #pragma unroll
       for (int s = K / 2; s > 0; s /= 2)
 #pragma unroll
-        for (int j = 0; j < K; ++j)
-          if ((j & s) == 0 && precedes(key[j + s], expert[j + s], key[j], expert[j])) {
-            const int k0 = key[j], e0 = expert[j];
+        for (int j = 0; j < K; ++j) {
+          if (j & s) continue;
+          const int k0 = key[j];
+          if constexpr (PACKED) {
+            key[j] = max(k0, key[j + s]);
+            key[j + s] = min(k0, key[j + s]);
+          } else if (precedes(key[j + s], expert[j + s], k0, expert[j])) {
+            const int e0 = expert[j];
             key[j] = key[j + s], expert[j] = expert[j + s];
             key[j + s] = k0, expert[j + s] = e0;
           }
+        }
     }
   }
+  // exp(value - high) of the j-th, 0 where there is none
+  __device__ __forceinline__ float share(int j, float high, int dtype) const {
+    if (key[j] == kNone) return 0.f;
+    float v;
+    if constexpr (PACKED) {
+      const int k16 = key[j] & (int)0xFFFF0000, bits = k16 ^ (k16 >> 31 & 0x7FFF0000);
+      v = dtype == OZ_F16 ? __half2float(__ushort_as_half((unsigned short)((uint32_t)bits >> 16))) : __int_as_float(bits);
+    } else {
+      v = __int_as_float(key[j] ^ (key[j] >> 31 & 0x7FFFFFFF));
+    }
+    return exp_of(v - high);
+  }
+  __device__ __forceinline__ int chosen(int j) const {
+    if (key[j] == kNone) return -1;
+    if constexpr (PACKED) return 0xFFFF - (key[j] & 0xFFFF);
+    else return expert[j];
+  }
 };
+// An element's key; none for -inf and past the last expert.
+template <bool PACKED> __device__ __forceinline__ int element_key(float v, int e, int experts, int dtype) {
+  if (e >= experts || v == -INFINITY) return kNone;
+  if constexpr (!PACKED) return key_of(v);
+  int bits;                                   // 16 of them above
+  if (dtype == OZ_F16) bits = (int)((uint32_t)__half_as_ushort(__float2half_rn(v + 0.f)) << 16);
+  else bits = __float_as_int(v + 0.f) & (int)0xFFFF0000;
+  return (bits ^ (bits >> 31 & 0x7FFF0000)) | (0xFFFF - e);
+}
 
 // Exclusive prefix sums of n counts in shared memory, by the first warp; total in from[n].
 __device__ __forceinline__ void scan(int *from, int n) {
@@ -179,40 +232,38 @@ __device__ __forceinline__ void scan(int *from, int n) {
   __syncthreads();
 }
 
-int route_smem(int e, int k, int chunk, int warps) {
-  return 4 * (e * (chunk / 32) + 2 * (e + 1) + warps * e + chunk * k + chunk + 1) + 2 * chunk * k;
+constexpr int kPickThreads = 256;
+int route_smem(int e, int k, int chunk) {
+  return 4 * (e * (chunk / 32) + 2 * (e + 1) + kPickThreads / 32 * e + 2 * chunk + 1) + 2 * chunk * k;
 }
 
-template <int VPL, int K> __host__ __device__ constexpr int pick_threads() { return VPL == 16 && K <= 8 ? 512 : 256; }
-
 // Picks of `per` rounds of `chunk` tokens a block.  A lane puts its part of a token's logits
-// into a sorted list of K, and the LPT lanes of the token join their lists: 5
-// instructions an expert and place of the list (k maxima over all lanes took 2440
-// instructions for 4 tokens of 64 experts and 8 picks, this 700).  Ranks among the tokens of
-// a round come from one bit a token and expert in shared memory (set in any order, counted
-// by popc), so there is no sort.  With one block of one round the rows are final, else
-// they count from the block's first pick of the expert and route_place adds the rest.
-template <int LPT, int VPL, int K>
-__global__ void __launch_bounds__(pick_threads<VPL, K>()) route_pick(const RouteParams p) {
+// into a sorted list of K, and the LPT lanes of the token join their lists: for each expert and
+// place of the list 6 instructions, or 2 for logits of 16 bits (k maxima over all lanes took 2440
+// for 4 tokens of 64 experts and 8 picks).  Ranks among the tokens of a round come from
+// one bit a token and expert in shared memory (set in any order, counted by popc), so there
+// is no sort.  With one block of one round the rows are final, else they count from the
+// block's first pick of the expert, and route_scan and route_place add the rest.
+template <int LPT, int VPL, int K, bool PACKED>
+__global__ void __launch_bounds__(kPickThreads, VPL == 16 && K <= 8 ? 4 : 1) route_pick(const RouteParams p) {
   extern __shared__ unsigned char smem[];
   const int words = p.chunk / 32, warps = blockDim.x / 32;
   uint32_t *bits = reinterpret_cast<uint32_t *>(smem);              // [e][words]
   int *count = reinterpret_cast<int *>(bits + p.e * words);         // [e + 1]
   int *first = count + p.e + 1;                                     // [e + 1]
   float *sums = reinterpret_cast<float *>(first + p.e + 1);         // [warps][e]
-  float *pick_w = sums + warps * p.e;                               // [chunk][k]
-  float *total = pick_w + p.chunk * p.k;                            // [chunk]
+  float *top = sums + kPickThreads / 32 * p.e;                      // [chunk]
+  float *total = top + p.chunk;                                     // [chunk]
   int *held = reinterpret_cast<int *>(total + p.chunk);
-  int16_t *pick_e = reinterpret_cast<int16_t *>(held + 1);          // [chunk][k]
+  int16_t *pick = reinterpret_cast<int16_t *>(held + 1);            // [chunk][k]
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, l = lane % LPT;
   constexpr int GROUPS = 32 / LPT;
+  const uint32_t per_pick = ((1u << 18) + p.k - 1) / p.k;           // i / k for i < 8192: i per_pick / 2^18
   start_after_earlier_kernels();
   if (threadIdx.x == 0) *held = 0;
   for (int e = threadIdx.x; e <= p.e; e += blockDim.x) count[e] = first[e] = 0;
-  float acc[VPL];
-#pragma unroll
-  for (int i = 0; i < VPL; ++i) acc[i] = 0.f;
+  for (int i = threadIdx.x; i < warps * p.e; i += blockDim.x) sums[i] = 0.f;
 
   for (int round = 0; round < p.per; ++round) {
     const int64_t t0 = ((int64_t)blockIdx.x * p.per + round) * p.chunk;
@@ -220,50 +271,71 @@ __global__ void __launch_bounds__(pick_threads<VPL, K>()) route_pick(const Route
     const int here = (int)min((int64_t)p.chunk, p.rows - t0);
     for (int i = threadIdx.x; i < p.e * words; i += blockDim.x) bits[i] = 0;
     __syncthreads();
+#pragma unroll 1
     for (int w0 = warp * GROUPS; w0 < here; w0 += warps * GROUPS) {
       const int tl = w0 + lane / LPT;
       float v[VPL];
       load_row<LPT, VPL>(p.logits, t0 + tl, tl < here, l, v);
-      Largest<K> best;
+      Largest<K, PACKED> best;
+      float high = -INFINITY;
 #pragma unroll
       for (int i = 0; i < VPL; ++i)
         if (i / 4 * 4 * LPT < p.e) {                    // the same for all lanes
           const int e = expert_of<LPT>(i, l);
-          best.put(e < p.e ? key_of(v[i]) : (int)0x80000000, e);
+          best.put(i, element_key<PACKED>(v[i], e, p.e, p.logits.dtype), e);
+          high = fmaxf(high, v[i]);
         }
       best.template join<LPT>();
-      const bool real_row = best.key[0] > kNothing;
-      const float top = real_row ? value_of(best.key[0]) : 0.f;
+      high = over_lanes<LPT>(high, [](float a, float b) { return fmaxf(a, b); });
+      const bool real = best.key[0] != kNone;
+      if (!real) high = 0.f;
       float sum = 0.f;
 #pragma unroll
       for (int i = 0; i < VPL; ++i)
         if (i / 4 * 4 * LPT < p.e) {
-          v[i] = exp_of(v[i] - top);
+          v[i] = exp_of(v[i] - high);
           sum += v[i];
         }
       sum = lanes_sum<LPT>(sum);
-      const float inverse = real_row ? 1.f / sum : 0.f;
+      const float inverse = real ? 1.f / sum : 0.f;
+      // this warp's sums of p: over its tokens, then to those of its tokens before
 #pragma unroll
       for (int i = 0; i < VPL; ++i)
-        if (i / 4 * 4 * LPT < p.e) acc[i] += real_row ? v[i] * inverse : 0.f;
-      // picks l, l + LPT, ... are this lane's to write
-      float picked = 0.f;
+        if (i / 4 * 4 * LPT < p.e) {
+          float q = real ? v[i] * inverse : 0.f;
 #pragma unroll
-      for (int j = 0; j < K; ++j) {
-        if (j % LPT != l || j >= p.k || tl >= here) continue;
-        const bool real = best.key[j] > kNothing;
-        const int e = best.expert[j];
-        const float x = real ? exp_of(value_of(best.key[j]) - top) : 0.f;
-        picked += x;
-        pick_e[tl * p.k + j] = real ? (int16_t)e : (int16_t)-1;
-        pick_w[tl * p.k + j] = x;
-        if (real) atomicOr(&bits[e * words + tl / 32], 1u << (tl % 32));
+          for (int o = LPT; o < 32; o *= 2) q += __shfl_xor_sync(0xffffffffu, q, o);
+          const int e = expert_of<LPT>(i, l);
+          if (lane < LPT && e < p.e) sums[warp * p.e + e] += q;
+        }
+      if (p.normalize) {
+        sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < K; ++j)
+          if (j < p.k) sum += best.share(j, high, p.logits.dtype);
       }
-      if (p.normalize) sum = lanes_sum<LPT>(picked);
+      // picks l, l + LPT, ... are this lane's to write
+#pragma unroll
+      for (int j = 0; j < K; ++j)
+        if (j % LPT == l && j < p.k && tl < here) pick[tl * p.k + j] = (int16_t)best.chosen(j);
       if (l == 0 && tl < here) {
-        total[tl] = real_row ? sum : 1.f;
-        if (real_row) atomicAdd(held, 1);
+        top[tl] = high;
+        total[tl] = real ? sum : 1.f;
       }
+      const uint32_t with = __ballot_sync(0xffffffffu, l == 0 && tl < here && real);
+      if (lane == 0) atomicAdd(held, __popc(with));
+    }
+    __syncthreads();
+    // a thread a pick: its probability and its bit
+    for (int i = threadIdx.x; i < here * p.k; i += blockDim.x) {
+      const int e = pick[i], tl = (int)((uint32_t)i * per_pick >> 18);
+      float x = 0.f;
+      if (e >= 0) {
+        x = exp_of(logit(p.logits, t0 + tl, e) - top[tl]) / total[tl];
+        atomicOr(&bits[e * words + tl / 32], 1u << (tl % 32));
+      }
+      p.experts[t0 * p.k + i] = e;
+      p.weights[t0 * p.k + i] = x;
     }
     __syncthreads();
     const bool alone = p.blocks == 1;
@@ -277,20 +349,17 @@ __global__ void __launch_bounds__(pick_threads<VPL, K>()) route_pick(const Route
       scan(first, p.e);
     }
     for (int i = threadIdx.x; i < here * p.k; i += blockDim.x) {
-      const int e = pick_e[i], tl = i / p.k;
-      const int64_t to = t0 * p.k + i;
-      p.experts[to] = e;
-      p.weights[to] = pick_w[i] / total[tl];
+      const int e = pick[i], tl = (int)((uint32_t)i * per_pick >> 18);
       int rank = -1;
       if (e >= 0) {
         rank = alone ? first[e] : count[e];
         for (int w = 0; w < tl / 32; ++w) rank += __popc(bits[e * words + w]);
         rank += __popc(bits[e * words + tl / 32] & ((1u << (tl % 32)) - 1));
       }
-      p.slots[to] = rank;
+      p.slots[t0 * p.k + i] = rank;
     }
-    __syncthreads();
     if (!alone) {
+      __syncthreads();
       for (int e = threadIdx.x; e < p.e; e += blockDim.x) {
         int n = count[e];
         for (int w = 0; w < words; ++w) n += __popc(bits[e * words + w]);
@@ -299,20 +368,13 @@ __global__ void __launch_bounds__(pick_threads<VPL, K>()) route_pick(const Route
       __syncthreads();
     }
   }
-  // sums of p over the groups of a warp, then over the warps
-#pragma unroll
-  for (int i = 0; i < VPL; ++i) {
-#pragma unroll
-    for (int o = LPT; o < 32; o *= 2) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], o);
-    if (lane < LPT && expert_of<LPT>(i, l) < p.e) sums[warp * p.e + expert_of<LPT>(i, l)] = acc[i];
-  }
   __syncthreads();
   if (p.blocks > 1) {
     for (int e = threadIdx.x; e < p.e; e += blockDim.x) {
       float s = 0.f;
       for (int w = 0; w < warps; ++w) s += sums[w * p.e + e];
-      p.psum[(int64_t)blockIdx.x * p.e + e] = s;
-      p.hist[(int64_t)blockIdx.x * p.e + e] = count[e];
+      p.psum[(int64_t)e * p.blocks + blockIdx.x] = s;
+      p.hist[(int64_t)e * p.blocks + blockIdx.x] = count[e];
     }
     if (threadIdx.x == 0) p.held[blockIdx.x] = *held;
     return;
@@ -334,100 +396,110 @@ __global__ void __launch_bounds__(pick_threads<VPL, K>()) route_pick(const Route
   }
 }
 
-// The rows of each block's picks: its first of an expert follows those of the
-// blocks before it.  Every block adds up the counts of all blocks for itself; the
-// last one (of blocks + 1) writes offsets, counts and loss.
-__global__ void __launch_bounds__(512) route_place(const RouteParams p) {
+// A warp an expert: the picks of the blocks before each, of all, and the sum of p.
+__global__ void __launch_bounds__(256) route_scan(const RouteParams p) {
+  start_after_earlier_kernels();
+  const int e = blockIdx.x * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
+  if (e >= p.e) return;
+  constexpr int MOST = 16;                    // of a lane: kMostBlocks / 32
+  const int each = (p.blocks + 31) / 32;
+  int *hist = p.hist + (int64_t)e * p.blocks;
+  int n[MOST], own = 0;
+  double mass = 0;
+#pragma unroll
+  for (int i = 0; i < MOST; ++i) {
+    const int b = lane * each + i;
+    n[i] = i < each && b < p.blocks ? hist[b] : 0;
+    if (i < each && b < p.blocks) mass += p.psum[(int64_t)e * p.blocks + b];
+    own += n[i];
+  }
+  int upto = own;
+#pragma unroll
+  for (int o = 1; o < 32; o *= 2) {
+    const int v = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += v;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o /= 2) mass += __shfl_xor_sync(0xffffffffu, mass, o);
+  int before = upto - own;
+#pragma unroll
+  for (int i = 0; i < MOST; ++i) {
+    const int b = lane * each + i;
+    if (i < each && b < p.blocks) hist[b] = before;
+    before += n[i];
+  }
+  if (lane == 31) p.all[e] = upto;
+  if (lane == 0) p.mass[e] = mass;
+}
+
+// The rows of each block's picks: the expert's first row and the picks of the blocks before.
+// The last block (of blocks + 1) writes offsets, counts and loss.
+__global__ void __launch_bounds__(256) route_place(const RouteParams p) {
   extern __shared__ unsigned char smem[];
-  const int groups = max(1, (int)blockDim.x / p.e);
-  int *total = reinterpret_cast<int *>(smem);                       // [e + 1]
-  int *base = total + p.e + 1;                                      // [e]
-  int *part = base + p.e + 1;                                       // [2][groups][e]
+  int *from = reinterpret_cast<int *>(smem);                        // [e + 1]
   start_after_earlier_kernels();
   const bool last = blockIdx.x == p.blocks;
-  // this block's picks, up to 8 a thread, are on their way while the counts are added up
+  // this block's picks, up to 4 a thread, are on their way meanwhile
   const int64_t span = (int64_t)p.chunk * p.per * p.k, i0 = blockIdx.x * span, end = min(i0 + span, p.rows * p.k);
-  int expert[8], slot[8];
+  int expert[4], slot[4];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int64_t i = i0 + threadIdx.x + j * (int64_t)blockDim.x;
-    expert[j] = !last && i < end ? p.experts[i] : -1;
-    slot[j] = expert[j] >= 0 ? p.slots[i] : 0;
+  for (int j = 0; j < 4; ++j) {
+    const int64_t i = i0 + threadIdx.x + j * 256;
+    const bool there = !last && i < end;
+    expert[j] = there ? p.experts[i] : -1;
+    slot[j] = there ? p.slots[i] : 0;
   }
-  const int lanes = groups * p.e;                                   // threads at work where e < blockDim
-  for (int i = threadIdx.x; i < lanes; i += blockDim.x) {
-    const int e = i % p.e, g = i / p.e;
-    int all = 0, before = 0;
-#pragma unroll 8
-    for (int b = g; b < p.blocks; b += groups) {
-      const int n = __ldg(p.hist + (int64_t)b * p.e + e);
-      all += n;
-      before += b < (int)blockIdx.x ? n : 0;
-    }
-    part[g * p.e + e] = all;
-    part[(groups + g) * p.e + e] = before;
+  int *before = from + p.e + 1;                                     // [e]
+  for (int e = threadIdx.x; e < p.e; e += 256) {
+    from[e] = p.all[e];
+    before[e] = last ? 0 : p.hist[(int64_t)e * p.blocks + blockIdx.x];
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < p.e; e += blockDim.x) {
-    int all = 0, before = 0;
-    for (int g = 0; g < groups; ++g) {
-      all += part[g * p.e + e];
-      before += part[(groups + g) * p.e + e];
-    }
-    total[e] = all;
-    base[e] = before;
-  }
-  __syncthreads();
-  scan(total, p.e);
+  scan(from, p.e);
   if (!last) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (expert[j] >= 0) p.slots[i0 + threadIdx.x + j * (int64_t)blockDim.x] = slot[j] + total[expert[j]] + base[expert[j]];
-    for (int64_t i = i0 + threadIdx.x + 8 * (int64_t)blockDim.x; i < end; i += blockDim.x) {
+    for (int j = 0; j < 4; ++j)
+      if (expert[j] >= 0) p.slots[i0 + threadIdx.x + j * 256] = slot[j] + from[expert[j]] + before[expert[j]];
+    for (int64_t i = i0 + threadIdx.x + 4 * 256; i < end; i += 256) {
       const int e = p.experts[i];
-      if (e >= 0) p.slots[i] += total[e] + base[e];
+      if (e >= 0) p.slots[i] += from[e] + before[e];
     }
     return;
   }
-  for (int e = threadIdx.x; e <= p.e; e += blockDim.x) {
-    p.offsets[e] = total[e];
-    if (e < p.e) p.counts[e] = total[e + 1] - total[e];
-  }
   double s = 0;
   int tokens = 0;
-  for (int i = threadIdx.x; i < lanes; i += blockDim.x) {
-    const int e = i % p.e, g = i / p.e;
-    double q = 0;
-#pragma unroll 8
-    for (int b = g; b < p.blocks; b += groups) q += __ldg(p.psum + (int64_t)b * p.e + e);
-    s += q * (total[e + 1] - total[e]);
+  for (int e = threadIdx.x; e <= p.e; e += 256) {
+    p.offsets[e] = from[e];
+    if (e == p.e) break;
+    const int n = from[e + 1] - from[e];
+    p.counts[e] = n;
+    s += p.mass[e] * n;
   }
-  for (int b = threadIdx.x; b < p.blocks; b += blockDim.x) tokens += p.held[b];
+  for (int b = threadIdx.x; b < p.blocks; b += 256) tokens += p.held[b];
+  __shared__ double warp_s[8];
+  __shared__ int warp_n[8];
 #pragma unroll
   for (int o = 16; o > 0; o /= 2) {
     s += __shfl_xor_sync(0xffffffffu, s, o);
     tokens += __shfl_xor_sync(0xffffffffu, tokens, o);
   }
-  __shared__ double warp_s[16];
-  __shared__ int warp_n[16];
   if (threadIdx.x % 32 == 0) {
     warp_s[threadIdx.x / 32] = s;
     warp_n[threadIdx.x / 32] = tokens;
   }
   __syncthreads();
   if (threadIdx.x == 0) {
-    s = 0;
-    tokens = 0;
-    for (int w = 0; w < (int)blockDim.x / 32; ++w) {
+    for (int w = 1; w < 8; ++w) {
       s += warp_s[w];
       tokens += warp_n[w];
     }
     *p.tokens = tokens;
-    *p.loss = tokens ? (float)(p.e * s / ((double)total[p.e] * tokens)) : 0.f;
+    *p.loss = tokens ? (float)(p.e * s / ((double)from[p.e] * tokens)) : 0.f;
   }
 }
 
-// Lanes of a token and values of a lane for e experts, then f.run<LPT, VPL>().
+// Lanes of a token and values of a lane for e experts, then f.run<LPT, VPL>().  More lanes
+// than e needs leave some of each lane's values unused.
 template <typename F> int with_layout(int e, const F &f) {
   if (e <= 16) return f.template run<1, 16>();
   if (e <= 32) return f.template run<2, 16>();
@@ -442,23 +514,30 @@ int lanes_of(int e) {
   while (lanes < 32 && lanes * 16 < e) lanes *= 2;
   return lanes;
 }
+// Twice the lanes (8 values each) where there are few tokens: a lane's list is what takes the
+// time then (8 tokens of 64 experts).
+int spread_experts(int64_t rows, int e) {
+  const int lanes = lanes_of(e);
+  return lanes < 16 && e > 4 && rows * lanes <= 4096 ? lanes * 32 : e;
+}
 Logits logits_of(const void *p, int64_t rows, int64_t row, int64_t col, int e, int dtype) {
   const int es = dtype_size(dtype);
   return {p, rows, row, col, e, dtype, e % 4 == 0 && col == 1 && (uintptr_t)p % (4 * es) == 0 && (rows <= 1 || row % 4 == 0)};
 }
 
+constexpr int kMostBlocks = 512;
 struct RoutePlan { int chunk, per, blocks; };
 // One block where that takes 2 turns of its threads or fewer.  Else rounds of 256 tokens, or
-// fewer (down to 32) while that leaves SMs without a block.
+// fewer (down to 32) while that leaves room on the GPU.
 RoutePlan route_plan(int64_t rows, int e) {
   RoutePlan r{kMaxChunk, 1, 1};
-  if (rows <= kMaxChunk && rows * lanes_of(e) <= 1024) {
+  if (rows <= kMaxChunk && rows * lanes_of(spread_experts(rows, e)) <= 2 * kPickThreads) {
     r.chunk = (int)(std::max<int64_t>(rows, 1) + 31) / 32 * 32;
     return r;
   }
-  while (r.chunk > 32 && (rows + r.chunk - 1) / r.chunk < 128) r.chunk /= 2;
+  while (r.chunk > 32 && (rows + r.chunk - 1) / r.chunk <= kMostBlocks / 2) r.chunk /= 2;
   const int64_t rounds = (rows + r.chunk - 1) / r.chunk;
-  r.per = (int)((rounds + 511) / 512);
+  r.per = (int)((rounds + kMostBlocks - 1) / kMostBlocks);
   r.blocks = (int)((rounds + r.per - 1) / r.per);
   return r;
 }
@@ -468,9 +547,11 @@ struct PickLaunch {
   cudaStream_t st;
   template <int LPT, int VPL, int K> int launch_it() const {
     const int64_t busy = std::min((int64_t)p.chunk, p.rows) * LPT;
-    const int threads = (int)std::max<int64_t>(32, std::min<int64_t>(pick_threads<VPL, K>(), (busy + 31) / 32 * 32));
-    return launch(route_pick<LPT, VPL, K>, dim3(p.blocks), threads, route_smem(p.e, p.k, p.chunk, threads / 32), st,
-                  "route_pick launch", p);
+    const int threads = (int)std::max<int64_t>(128, std::min<int64_t>(kPickThreads, (busy + 31) / 32 * 32));
+    const int smem = route_smem(p.e, p.k, p.chunk);
+    const char *what = "route_pick launch";
+    return p.logits.dtype == OZ_F32 ? launch(route_pick<LPT, VPL, K, false>, dim3(p.blocks), threads, smem, st, what, p)
+                                    : launch(route_pick<LPT, VPL, K, true>, dim3(p.blocks), threads, smem, st, what, p);
   }
   template <int LPT, int VPL> int run() const {
     if (p.k <= 2) return launch_it<LPT, VPL, 2>();
@@ -822,7 +903,8 @@ extern "C" int64_t oz_route_workspace_bytes(int64_t rows, int32_t experts) {
   using namespace oz;
   if (rows < 0 || experts < 1 || experts > kMaxExperts) return OZ_ERR_INVALID;
   const RoutePlan r = route_plan(rows, experts);
-  return r.blocks <= 1 ? 0 : (int64_t)r.blocks * (experts * 8 + 4);
+  // sums of p, then what the blocks counted
+  return r.blocks <= 1 ? 0 : (int64_t)experts * 8 + (int64_t)r.blocks * (experts * 8 + 4) + experts * 4;
 }
 
 extern "C" int oz_route(const oz_route_args *args, void *stream) {
@@ -846,18 +928,20 @@ extern "C" int oz_route(const oz_route_args *args, void *stream) {
   if (a.dtype != OZ_F32 && a.dtype != OZ_F16 && a.dtype != OZ_BF16)
     return set_error(OZ_ERR_UNSUPPORTED, "unsupported dtype %d (fp32, fp16 or bf16)", a.dtype);
   RouteParams p{logits_of(a.logits, a.rows, a.row, a.col, a.experts, a.dtype), a.weights, a.loss, a.chosen, a.slots,
-                a.offsets, a.counts, a.tokens, nullptr, nullptr, nullptr, a.rows, a.experts, a.picks, a.normalize,
-                r.chunk, r.per, r.blocks};
+                a.offsets, a.counts, a.tokens, nullptr, nullptr, nullptr, nullptr, nullptr, a.rows, a.experts, a.picks,
+                a.normalize, r.chunk, r.per, r.blocks};
   if (bytes) {
-    p.hist = static_cast<int *>(a.workspace);
+    p.mass = static_cast<double *>(a.workspace);
+    p.hist = reinterpret_cast<int *>(p.mass + a.experts);
     p.psum = reinterpret_cast<float *>(p.hist + (int64_t)r.blocks * a.experts);
     p.held = reinterpret_cast<int *>(p.psum + (int64_t)r.blocks * a.experts);
+    p.all = p.held + r.blocks;
   }
-  const int rc = with_layout(a.experts, PickLaunch{p, st});
+  int rc = with_layout(spread_experts(a.rows, a.experts), PickLaunch{p, st});
   if (rc || r.blocks <= 1) return rc;
-  const int groups = max(1, 512 / a.experts);
-  return launch(route_place, dim3(r.blocks + 1), 512, 4 * (2 * (a.experts + 1) + 2 * groups * a.experts), st,
-                "route_place launch", p);
+  rc = launch(route_scan, dim3((a.experts + 7) / 8), 256, 0, st, "route_scan launch", p);
+  if (rc) return rc;
+  return launch(route_place, dim3(r.blocks + 1), 256, 4 * (2 * a.experts + 1), st, "route_place launch", p);
 }
 
 extern "C" int oz_route_backward(const oz_route_backward_args *args, void *stream) {

@@ -17,6 +17,7 @@ enqueue their work on the current stream of their tensors' device.
 from __future__ import annotations
 
 import ctypes
+import math
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -24,7 +25,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .api import _OZ_DTYPE
-from .experts import _CURRENT_DEVICE, _LEVEL, _OnDevice, _check_places, _check_tangents, _stream_of
+from .experts import _LEVEL, _Plan, _Plans, _check_places, _check_tangents, _launch, _make_plan
 
 ROUTE_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 MAX_EXPERTS, MAX_PICKS = 1024, 32
@@ -48,15 +49,7 @@ class Routing(NamedTuple):
     balance_loss: torch.Tensor   # () fp32, differentiable
 
 
-def _call(name: str, args: ctypes.Structure, device: int) -> None:
-    call = getattr(_lib.load(), name)
-    if _CURRENT_DEVICE() == device:
-        status = call(ctypes.byref(args), _stream_of(device))
-    else:
-        with _OnDevice(device):
-            status = call(ctypes.byref(args), _stream_of(device))
-    if status:
-        _lib.check(status)
+_PLANS = _Plans()
 
 
 def _check_logits(logits: torch.Tensor, picks: int) -> None:
@@ -68,35 +61,78 @@ def _check_logits(logits: torch.Tensor, picks: int) -> None:
         f"picks must be in [1, {min(experts, MAX_PICKS)}], got {picks}"
 
 
-def _route(logits: torch.Tensor, picks: int, normalize: bool) -> Routing:
+def _strides(*shape: int) -> Tuple[int, ...]:
+    return tuple(math.prod(max(n, 1) for n in shape[i + 1:]) for i in range(len(shape)))
+
+
+def _plan_route(key, logits, picks, normalize) -> _Plan:
     _check_logits(logits, picks)
     device = _check_places(logits)
     rows, experts = logits.shape
-    lib = _lib.load()
-
-    def whole(*shape):
-        return logits.new_empty(shape, dtype=torch.int32)
-
-    out = Routing(logits.new_empty((rows, picks), dtype=torch.float32), whole(rows, picks), whole(rows, picks),
-                  whole(experts + 1), whole(experts), whole(), logits.new_empty((), dtype=torch.float32))
-    size = lib.oz_route_workspace_bytes(rows, experts)
-    workspace = logits.new_empty((size,), dtype=torch.uint8) if size else None
-    args = _lib.RouteArgs(logits.data_ptr(), out.weights.data_ptr(), out.balance_loss.data_ptr(), out.experts.data_ptr(),
-                          out.slots.data_ptr(), out.offsets.data_ptr(), out.counts.data_ptr(), out.tokens.data_ptr(),
-                          None if workspace is None else workspace.data_ptr(), rows, *logits.stride(), size, experts,
+    size = _lib.load().oz_route_workspace_bytes(rows, experts)
+    args = _lib.RouteArgs(None, None, None, None, None, None, None, None, None, rows, *logits.stride(), size, experts,
                           picks, bool(normalize), _OZ_DTYPE[logits.dtype])
-    _call("oz_route", args, device)
+    return _PLANS.keep(key, _make_plan("oz_route", args, (rows, picks), logits.dtype, device, False, False, size))
+
+
+def _route(logits: torch.Tensor, picks: int, normalize: bool) -> Routing:
+    key = ("route", logits.shape, logits.stride(), logits.dtype, logits.get_device(), picks, normalize)
+    plan = _PLANS.kept.get(key) or _plan_route(key, logits, picks, normalize)
+    shape, strides, args, new = plan.shape, plan.strides, plan.args, logits.new_empty_strided
+    experts, whole, real = args.experts, torch.int32, torch.float32
+    out = Routing(new(shape, strides, dtype=real), new(shape, strides, dtype=whole), new(shape, strides, dtype=whole),
+                  new((experts + 1,), (1,), dtype=whole), new((experts,), (1,), dtype=whole), new((), (), dtype=whole),
+                  new((), (), dtype=real))
+    args.logits, args.weights, args.chosen = logits.data_ptr(), out[0].data_ptr(), out[1].data_ptr()
+    args.slots, args.offsets, args.counts = out[2].data_ptr(), out[3].data_ptr(), out[4].data_ptr()
+    args.tokens, args.loss = out[5].data_ptr(), out[6].data_ptr()
+    if plan.workspace:
+        workspace = new((plan.workspace,), (1,), dtype=torch.uint8)
+        args.workspace = workspace.data_ptr()
+    _launch(plan)
     return out
 
 
+def _plan_route_gradient(key, dweights, dloss, logits, weights, experts, counts, tokens, normalize) -> _Plan:
+    assert experts.dim() == 2, f"routing.experts must have 2 dimensions, got shape {tuple(experts.shape)}"
+    _check_logits(logits, experts.shape[1])
+    shape = (logits.shape[0], experts.shape[1])
+    for name, t, dtype, want in (("dweights", dweights, torch.float32, shape), ("dloss", dloss, torch.float32, ()),
+                                 ("routing.weights", weights, torch.float32, shape),
+                                 ("routing.experts", experts, torch.int32, shape),
+                                 ("routing.counts", counts, torch.int32, (logits.shape[1],)),
+                                 ("routing.tokens", tokens, torch.int32, ())):
+        if t is not None:
+            assert t.dtype is dtype, f"{name} must be {dtype}, got {t.dtype}"
+            assert t.shape == want, f"{name} must have shape {want}, got {tuple(t.shape)}"
+    device = _check_places(logits, dweights, dloss, weights, experts, counts, tokens)
+    args = _lib.RouteBackwardArgs(None, None, None, None, None, None, None, None, logits.shape[0], *logits.stride(),
+                                  logits.shape[1], experts.shape[1], bool(normalize), _OZ_DTYPE[logits.dtype])
+    copy = not all(t is None or t.is_contiguous() for t in (dweights, weights, experts, counts))
+    return _PLANS.keep(key, _make_plan("oz_route_backward", args, tuple(logits.shape), logits.dtype, device,
+                                       logits.shape[0] == 0, copy))
+
+
+def _signature(t: Optional[torch.Tensor]):
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
+
+
 def _route_gradient(dweights, dloss, logits, weights, experts, counts, tokens, normalize) -> torch.Tensor:
-    out = logits.new_empty(logits.shape)
-    args = _lib.RouteBackwardArgs(logits.data_ptr(), None if dweights is None else dweights.data_ptr(),
-                                  None if dloss is None else dloss.data_ptr(), weights.data_ptr(), experts.data_ptr(),
-                                  counts.data_ptr(), tokens.data_ptr(), out.data_ptr(), logits.shape[0],
-                                  *logits.stride(), logits.shape[1], experts.shape[1], bool(normalize),
-                                  _OZ_DTYPE[logits.dtype])
-    _call("oz_route_backward", args, logits.get_device())
+    key = ("gradient", logits.shape, logits.stride(), logits.dtype, logits.get_device(), normalize, _signature(dweights),
+           _signature(dloss), _signature(weights), _signature(experts), _signature(counts), _signature(tokens))
+    plan = _PLANS.kept.get(key) or _plan_route_gradient(key, dweights, dloss, logits, weights, experts, counts, tokens,
+                                                        normalize)
+    if plan.copy:
+        return _route_gradient(None if dweights is None else dweights.contiguous(), dloss, logits, weights.contiguous(),
+                               experts.contiguous(), counts.contiguous(), tokens, normalize)
+    out = logits.new_empty_strided(plan.shape, plan.strides)
+    if not plan.empty:
+        args = plan.args
+        args.logits, args.weights, args.chosen = logits.data_ptr(), weights.data_ptr(), experts.data_ptr()
+        args.counts, args.tokens, args.dlogits = counts.data_ptr(), tokens.data_ptr(), out.data_ptr()
+        args.dweights = None if dweights is None else dweights.data_ptr()
+        args.dloss = None if dloss is None else dloss.data_ptr()
+        _launch(plan)
     return out
 
 
@@ -117,9 +153,7 @@ class _Route(torch.autograd.Function):
         if dweights is None and dloss is None:
             return None, None, None
         logits, weights, experts, counts, tokens = ctx.saved_tensors
-        dweights = None if dweights is None else dweights.float().contiguous()
-        return (_route_gradient(dweights, None if dloss is None else dloss.float(), logits, weights, experts, counts,
-                                tokens, ctx.normalize), None, None)
+        return (_route_gradient(dweights, dloss, logits, weights, experts, counts, tokens, ctx.normalize), None, None)
 
 
 def route(logits: torch.Tensor, picks: int, *, normalize: bool = False) -> Routing:
@@ -158,39 +192,24 @@ def route_backward(dweights: Optional[torch.Tensor], dloss: Optional[torch.Tenso
     """
     if _LEVEL._current_level >= 0:
         _check_tangents(dweights, dloss, logits, routing.weights)
-    experts = routing.experts
-    assert experts.dim() == 2, f"routing.experts must have 2 dimensions, got shape {tuple(experts.shape)}"
-    _check_logits(logits, experts.shape[1])
-    shape = (logits.shape[0], experts.shape[1])
-    for name, t, dtype, want in (("dweights", dweights, torch.float32, shape), ("dloss", dloss, torch.float32, ()),
-                                 ("routing.weights", routing.weights, torch.float32, shape),
-                                 ("routing.experts", experts, torch.int32, shape),
-                                 ("routing.counts", routing.counts, torch.int32, (logits.shape[1],)),
-                                 ("routing.tokens", routing.tokens, torch.int32, ())):
-        if t is not None:
-            assert t.dtype is dtype, f"{name} must be {dtype}, got {t.dtype}"
-            assert t.shape == want, f"{name} must have shape {want}, got {tuple(t.shape)}"
-    _check_places(logits, dweights, dloss, *routing[:2], routing.counts, routing.tokens)
-    return _route_gradient(None if dweights is None else dweights.contiguous(), dloss, logits,
-                           routing.weights.contiguous(), experts.contiguous(), routing.counts.contiguous(),
-                           routing.tokens, normalize)
+    return _route_gradient(dweights, dloss, logits, routing.weights, routing.experts, routing.counts, routing.tokens,
+                           normalize)
 
 
 # ---------------------------------------------------------------------------
 # rows
 # ---------------------------------------------------------------------------
-def _check_routing(routing: Routing, weights: bool) -> None:
-    slots, offsets = routing.slots, routing.offsets
+def _check_routing(slots: torch.Tensor, offsets: torch.Tensor, weights: Optional[torch.Tensor]) -> None:
     assert slots.dim() == 2 and slots.dtype is torch.int32, \
         f"routing.slots must be (tokens, picks) int32, got {tuple(slots.shape)} {slots.dtype}"
     assert 1 <= slots.shape[1] <= MAX_PICKS, f"picks must be in [1, {MAX_PICKS}], got {slots.shape[1]}"
+    assert slots.is_contiguous(), "routing.slots must be contiguous"
     assert offsets.dim() == 1 and offsets.shape[0] >= 2 and offsets.dtype is torch.int32, \
         f"routing.offsets must be (experts + 1,) int32, got {tuple(offsets.shape)} {offsets.dtype}"
-    assert slots.is_contiguous() and offsets.is_contiguous(), "routing.slots and offsets must be contiguous"
-    if weights:
-        w = routing.weights
-        assert w.dtype is torch.float32 and w.shape == slots.shape, \
-            f"routing.weights must be {tuple(slots.shape)} torch.float32, got {tuple(w.shape)} {w.dtype}"
+    assert offsets.is_contiguous(), "routing.offsets must be contiguous"
+    if weights is not None:
+        assert weights.dtype is torch.float32 and weights.shape == slots.shape, \
+            f"routing.weights must be {tuple(slots.shape)} torch.float32, got {tuple(weights.shape)} {weights.dtype}"
 
 
 def _check_matrix(t: torch.Tensor, rows: int, what: str) -> None:
@@ -199,66 +218,78 @@ def _check_matrix(t: torch.Tensor, rows: int, what: str) -> None:
     assert t.shape[0] == rows, f"{what} must have {rows} rows, got {t.shape[0]}"
 
 
-def _rowwise(t: torch.Tensor) -> torch.Tensor:
-    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+def _plan_rows(key, call, x, rows, slots, offsets, weights) -> _Plan:
+    """x: of tokens, rows: of picks; the one that a call does not read is None."""
+    _check_routing(slots, offsets, weights)
+    (tokens, picks), given = slots.shape, x if rows is None else rows
+    if rows is not None:
+        _check_matrix(rows, tokens * picks, "rows")
+    if x is not None:
+        _check_matrix(x, tokens, "x" if rows is None else "dy")
+        assert x.dtype is given.dtype and x.shape[1] == given.shape[1], \
+            f"dy must be {(tokens, given.shape[1])} {given.dtype}, got {tuple(x.shape)} {x.dtype}"
+    device = _check_places(given, x, slots, offsets, weights)
+    d = given.shape[1]
+    shape = (tokens, d) if call == "oz_combine" else (tokens * picks, d)
+    copy = not all(t is None or t.stride(1) == 1 or t.shape[1] == 1 for t in (x, rows)) \
+        or (weights is not None and not weights.is_contiguous())
+    args = _lib.RowsArgs(None, None, None, None, None, None, None, None, tokens, d, 0 if x is None else x.stride(0),
+                         0 if rows is None else rows.stride(0), offsets.shape[0] - 1, picks,
+                         _OZ_DTYPE[given.dtype], 0)
+    return _PLANS.keep(key, _make_plan(call, args, shape, given.dtype, device, tokens == 0, copy))
 
 
-def _dispatch(x: torch.Tensor, slots: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
-    x = _rowwise(x)
-    (tokens, d), picks = x.shape, slots.shape[1]
-    out = x.new_empty((tokens * picks, d))
-    _call("oz_dispatch", _lib.RowsArgs(x.data_ptr(), None, None, out.data_ptr(), slots.data_ptr(), offsets.data_ptr(),
-                                       None, None, tokens, d, x.stride(0), 0, offsets.shape[0] - 1, picks,
-                                       _OZ_DTYPE[x.dtype], 0), x.get_device())
-    return out
-
-
-def _combine(rows: torch.Tensor, slots: torch.Tensor, weights: Optional[torch.Tensor]) -> torch.Tensor:
-    rows = _rowwise(rows)
-    (tokens, picks), d = slots.shape, rows.shape[1]
-    out = rows.new_empty((tokens, d))
-    if weights is not None:
-        weights = weights.contiguous()
-    _call("oz_combine", _lib.RowsArgs(None, rows.data_ptr(), out.data_ptr(), None, slots.data_ptr(), None,
-                                      None if weights is None else weights.data_ptr(), None, tokens, d, 0,
-                                      rows.stride(0), 1, picks, _OZ_DTYPE[rows.dtype], 0), rows.get_device())
-    return out
-
-
-def _combine_gradient(dy, rows, slots, offsets, weights):
-    dy, rows, weights = _rowwise(dy), _rowwise(rows), weights.contiguous()
-    (tokens, picks), d = slots.shape, rows.shape[1]
-    drows, dweights = rows.new_empty(rows.shape), weights.new_empty(weights.shape)
-    _call("oz_combine_backward", _lib.RowsArgs(dy.data_ptr(), rows.data_ptr(), None, drows.data_ptr(), slots.data_ptr(),
-                                               offsets.data_ptr(), weights.data_ptr(), dweights.data_ptr(), tokens, d,
-                                               dy.stride(0), rows.stride(0), offsets.shape[0] - 1, picks,
-                                               _OZ_DTYPE[rows.dtype], 0), rows.get_device())
-    return drows, dweights
+def _rows(call, x, rows, slots, offsets, weights):
+    """The result of a call in rows or tokens; of ``oz_combine_backward`` (drows, dweights)."""
+    key = (call, _signature(x), _signature(rows), _signature(slots), _signature(offsets), _signature(weights))
+    plan = _PLANS.kept.get(key) or _plan_rows(key, call, x, rows, slots, offsets, weights)
+    if plan.copy:
+        return _rows(call, None if x is None else x.contiguous(), None if rows is None else rows.contiguous(), slots,
+                     offsets, None if weights is None else weights.contiguous())
+    given = x if rows is None else rows
+    out = given.new_empty_strided(plan.shape, plan.strides)
+    gradient = call == "oz_combine_backward"
+    dweights = slots.new_empty(slots.shape, dtype=torch.float32) if gradient else None
+    if not plan.empty:
+        args = plan.args
+        args.x = None if x is None else x.data_ptr()
+        args.rows = None if rows is None else rows.data_ptr()
+        args.slots = slots.data_ptr()
+        args.offsets = offsets.data_ptr()
+        args.weights = None if weights is None else weights.data_ptr()
+        if call == "oz_combine":
+            args.x_out = out.data_ptr()
+        else:
+            args.rows_out = out.data_ptr()
+        if gradient:
+            args.dweights = dweights.data_ptr()
+        _launch(plan)
+    return (out, dweights) if gradient else out
 
 
 class _Dispatch(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, slots, offsets):
-        ctx.save_for_backward(slots)
-        return _dispatch(x, slots, offsets)
+        ctx.save_for_backward(slots, offsets)
+        return _rows("oz_dispatch", x, None, slots, offsets, None)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, drows):
-        return _combine(drows, ctx.saved_tensors[0], None), None, None
+        return _rows("oz_combine", None, drows, *ctx.saved_tensors, None), None, None
 
 
 class _Combine(torch.autograd.Function):
     @staticmethod
     def forward(ctx, rows, weights, slots, offsets):
         ctx.save_for_backward(rows, weights, slots, offsets)
-        return _combine(rows, slots, weights)
+        return _rows("oz_combine", None, rows, slots, offsets, weights)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         rows, weights, slots, offsets = ctx.saved_tensors
-        drows, dweights = _combine_gradient(dy, rows, slots, offsets, weights)
+        drows, dweights = _rows("oz_combine_backward", dy, rows, slots, offsets, weights)
         return (drows if ctx.needs_input_grad[0] else None, dweights if ctx.needs_input_grad[1] else None, None, None)
 
 
@@ -272,22 +303,16 @@ def dispatch(x: torch.Tensor, routing: Routing) -> torch.Tensor:
     """
     if _LEVEL._current_level >= 0:
         _check_tangents(x)
-    _check_routing(routing, False)
-    _check_matrix(x, routing.slots.shape[0], "x")
-    _check_places(x, routing.slots, routing.offsets)
     if x.requires_grad and torch.is_grad_enabled():
         return _Dispatch.apply(x, routing.slots, routing.offsets)
-    return _dispatch(x, routing.slots, routing.offsets)
+    return _rows("oz_dispatch", x, None, routing.slots, routing.offsets, None)
 
 
 def dispatch_backward(drows: torch.Tensor, routing: Routing) -> torch.Tensor:
     """Gradient of ``dispatch``: dx[t] = the sum over j of drows[routing.slots[t, j]]."""
     if _LEVEL._current_level >= 0:
         _check_tangents(drows)
-    _check_routing(routing, False)
-    _check_matrix(drows, routing.slots.numel(), "drows")
-    _check_places(drows, routing.slots)
-    return _combine(drows, routing.slots, None)
+    return _rows("oz_combine", None, drows, routing.slots, routing.offsets, None)
 
 
 def combine(rows: torch.Tensor, routing: Routing) -> torch.Tensor:
@@ -300,13 +325,10 @@ def combine(rows: torch.Tensor, routing: Routing) -> torch.Tensor:
     """
     if _LEVEL._current_level >= 0:
         _check_tangents(rows, routing.weights)
-    _check_routing(routing, True)
-    _check_matrix(rows, routing.slots.numel(), "rows")
     weights = routing.weights
-    _check_places(rows, *routing[:4])
     if (rows.requires_grad or weights.requires_grad) and torch.is_grad_enabled():
         return _Combine.apply(rows, weights, routing.slots, routing.offsets)
-    return _combine(rows, routing.slots, weights)
+    return _rows("oz_combine", None, rows, routing.slots, routing.offsets, weights)
 
 
 def combine_backward(dy: torch.Tensor, rows: torch.Tensor, routing: Routing) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -318,10 +340,4 @@ def combine_backward(dy: torch.Tensor, rows: torch.Tensor, routing: Routing) -> 
     """
     if _LEVEL._current_level >= 0:
         _check_tangents(dy, rows, routing.weights)
-    _check_routing(routing, True)
-    _check_matrix(rows, routing.slots.numel(), "rows")
-    _check_matrix(dy, routing.slots.shape[0], "dy")
-    assert dy.dtype is rows.dtype and dy.shape[1] == rows.shape[1], \
-        f"dy must be {(routing.slots.shape[0], rows.shape[1])} {rows.dtype}, got {tuple(dy.shape)} {dy.dtype}"
-    _check_places(rows, dy, *routing[:4])
-    return _combine_gradient(dy, rows, routing.slots, routing.offsets, routing.weights)
+    return _rows("oz_combine_backward", dy, rows, routing.slots, routing.offsets, routing.weights)

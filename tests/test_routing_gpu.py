@@ -99,7 +99,8 @@ def test_ties_and_special_values(e, picks):
     g = generator(e)
     few = torch.randint(-1, 2, (300, e), generator=g, device=DEV).float()
     few[few == 0] = torch.where(torch.rand(int((few == 0).sum()), generator=g, device=DEV) < 0.5, 0.0, -0.0)
-    check(few, picks, False)                                         # the lowest index first, also among zeros
+    for dtype in DTYPES:
+        check(few.to(dtype), picks, False)                           # the lowest index first, also among zeros
     check(torch.zeros(300, e, device=DEV), picks, True)
     check(torch.full((70, e), -INF, device=DEV), picks, True)        # nothing but padding
     low = torch.full((70, e), torch.finfo(torch.float32).min, device=DEV)
