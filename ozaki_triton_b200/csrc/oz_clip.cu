@@ -200,9 +200,9 @@ __global__ void __launch_bounds__(kThreads, 4) scale_kernel(const __grid_constan
 
 // A launch takes the addresses of at most this many tensors as arguments.
 constexpr int kFew = 64, kMany = 640;
-constexpr int kBlocksPerSm = 6;
+constexpr int kBlocksPerSm = 6, kScaleBlocksPerSm = 4;      // resident together
 
-int sum_blocks(int64_t pieces) { return (int)std::min<int64_t>(pieces, (int64_t)sm_count() * kBlocksPerSm); }
+int blocks_of(int64_t pieces, int per_sm) { return (int)std::min<int64_t>(pieces, (int64_t)sm_count() * per_sm); }
 
 template <int N> Table<N> table_of(const oz_clip_args &a, int first, int count) {
   Table<N> table;
@@ -231,7 +231,7 @@ template <int N> int run(const oz_clip_args &a, Sums sums, cudaStream_t st) {
   for (int i = 0; i < a.tensors; i += N) {
     const auto table = table_of<N>(a, i, std::min(N, a.tensors - i));
     if (!table.pieces) continue;
-    const int blocks = sum_blocks(table.pieces);
+    const int blocks = blocks_of(table.pieces, kBlocksPerSm);
     if (int rc = launch(norm_kernel<N>, dim3(blocks), kThreads, 0, st, "norm_kernel launch", table,
                         sums.partial + sums.blocks))
       return rc;
@@ -242,7 +242,7 @@ template <int N> int run(const oz_clip_args &a, Sums sums, cudaStream_t st) {
   for (int i = last; i >= 0; i -= N) {
     const auto table = table_of<N>(a, i, std::min(N, a.tensors - i));
     if (!table.pieces && i != last) continue;                   // one launch at least writes the norm
-    if (int rc = launch(scale_kernel<N>, dim3(std::max(1, sum_blocks(table.pieces))), kThreads, 0, st,
+    if (int rc = launch(scale_kernel<N>, dim3(std::max(1, blocks_of(table.pieces, kScaleBlocksPerSm))), kThreads, 0, st,
                         "scale_kernel launch", table, sums))
       return rc;
   }

@@ -51,24 +51,43 @@ template <typename E> __device__ __forceinline__ void store8(E *to, bool vectors
   }
 }
 
+// The columns of a source 16 at a time, the next ones on their way (accumulators in tensor
+// memory) while the ones before are worked on.
+template <class Source> struct Ahead16;
+template <> struct Ahead16<Columns> {
+  const Columns &source;
+  uint32_t r[16];
+  __device__ __forceinline__ void start(int c) { tmem_ld16_at(source.addr + (uint32_t)c, r); }
+  __device__ __forceinline__ void finish(float (&v)[16]) {
+    tmem_ld_wait16(r);
+#pragma unroll
+    for (int x = 0; x < 16; ++x) v[x] = __uint_as_float(r[x]);
+  }
+};
+template <int N> struct Ahead16<Registers<N>> {
+  const Registers<N> &source;
+  int at;
+  __device__ __forceinline__ void start(int c) { at = c; }
+  __device__ __forceinline__ void finish(float (&v)[16]) { source.read(at, v); }
+};
+
 // Finishes the warp's 32 x COLS accumulators: 16 columns at a time go through its staging
 // in fp32, so that a lane has 8 columns of two rows, whose bias, residual and results are
-// 16 bytes each, next to the neighbouring lane's.  (A lane's own row instead, with the
-// bias and the residual read element by element, took 8192 x 8192 results of 4096 terms
-// from 338 us to 365 and 549.)
+// 16 bytes each, next to the neighbouring lane's.  Accumulators, bias and residual of the next
+// columns are on their way meanwhile.  (A lane's own row instead, with the bias and the
+// residual read element by element, took 8192 x 8192 results of 4096 terms from 338 us to
+// 365 and 549.)
 template <typename O, typename B, int COLS, int UNROLL, class Source>
 __device__ __forceinline__ void finish_rows(const Params &p, const Source &source, unsigned char *mine, int64_t r0,
                                             int64_t c0) {
   const int lane = threadIdx.x % 32, half = lane % 2;
-  const int rows = (int)min(p.rows - r0, (int64_t)32);
-  const int64_t columns = p.n - c0;
-  if (rows <= 0) return;
-#pragma unroll(UNROLL)
-  for (int c = 0; c < COLS; c += 16) {
-    if (c >= columns) continue;
+  const int rows = (int)min(p.rows - r0, (int64_t)32), columns = (int)min(p.n - c0, (int64_t)COLS);
+  if (rows <= 0 || columns <= 0) return;
+  float residual[2][8], bias[8] = {};
+  // what the columns from c on need besides the accumulators
+  auto fetch = [&](int c) {
     const int64_t column = c0 + c + half * 8;
     const int count = (int)min(p.n - column, (int64_t)8);
-    float residual[2][8], bias[8] = {};
     if (p.residual)
 #pragma unroll
       for (int i = 0; i < 2; ++i)
@@ -79,39 +98,71 @@ __device__ __forceinline__ void finish_rows(const Params &p, const Source &sourc
       if (p.bias_f32) load8(static_cast<const float *>(p.bias) + column, p.vectors & kBiasVectors, count, bias);
       else load8(static_cast<const B *>(p.bias) + column, p.vectors & kBiasVectors, count, bias);
     }
+  };
+  Ahead16<Source> ahead{source};
+  ahead.start(0);
+  fetch(0);
+  const bool whole = rows == 32 && columns == COLS && (p.vectors & kVectors);
+  const int64_t at = (r0 + lane / 2) * p.ld + c0 + half * 8, next_row = 16 * p.ld;
+  O *out = static_cast<O *>(p.out) + at;
+  B *pre = static_cast<B *>(p.pre) + at;
+#pragma unroll(UNROLL)
+  for (int c = 0; c < COLS; c += 16) {
+    if (c >= columns) continue;
     float v[16];
-    source.read(c, v);
+    ahead.finish(v);
 #pragma unroll
     for (int u = 0; u < 4; ++u) *staged(mine, lane, u) = *reinterpret_cast<uint4 *>(&v[u * 4]);
+    if (c + 16 < columns) ahead.start(c + 16);
     __syncwarp();
+    float u[2][8];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int r = i * 16 + lane / 2;
-      if (r >= rows) continue;
-      float u[8];
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const uint4 raw = *staged(mine, r, half * 2 + h);
+        const uint4 raw = *staged(mine, i * 16 + lane / 2, half * 2 + h);
         const float *f = reinterpret_cast<const float *>(&raw);
 #pragma unroll
-        for (int x = 0; x < 4; ++x) u[h * 4 + x] = f[x] + bias[h * 4 + x];
+        for (int x = 0; x < 4; ++x) u[i][h * 4 + x] = f[x] + bias[h * 4 + x];
       }
-      const int64_t at = (r0 + r) * p.ld + column;
-      if (p.pre) store8(static_cast<B *>(p.pre) + at, p.vectors & kVectors, count, u);
-      if (p.act)
-#pragma unroll
-        for (int x = 0; x < 8; ++x) u[x] = activated(u[x], p.act);
+    __syncwarp();
+    if (whole) {
+      if (p.pre) {
+        store8(pre + c, true, 8, u[0]);
+        store8(pre + c + next_row, true, 8, u[1]);
+      }
+      activate(u[0], p.act);
+      activate(u[1], p.act);
       if (p.residual)
 #pragma unroll
-        for (int x = 0; x < 8; ++x) u[x] += residual[i][x];
-      store8(static_cast<O *>(p.out) + at, p.vectors & kVectors, count, u);
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int x = 0; x < 8; ++x) u[i][x] += residual[i][x];
+      if (c + 16 < COLS) fetch(c + 16);
+      store8(out + c, true, 8, u[0]);
+      store8(out + c + next_row, true, 8, u[1]);
+    } else {
+      const int count = (int)min(p.n - c0 - c - half * 8, (int64_t)8);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (i * 16 + lane / 2 >= rows) continue;
+        if (p.pre) store8(pre + c + i * next_row, p.vectors & kVectors, count, u[i]);
+        activate(u[i], p.act);
+        if (p.residual)
+#pragma unroll
+          for (int x = 0; x < 8; ++x) u[i][x] += residual[i][x];
+        store8(out + c + i * next_row, p.vectors & kVectors, count, u[i]);
+      }
+      if (c + 16 < columns) fetch(c + 16);
     }
-    __syncwarp();
   }
 }
 
 // A along the result's rows, B along its columns.
+// What follows a product keeps 16 epilogue warps busy (a plain one's 8 wait for its stores;
+// the sums of passes of an fp32 result leave no registers for 16).
 template <typename O, typename B, int PAIR_, int NT_, bool AMN_, bool BMN_, bool PLAIN> struct LinearJob : NoLookAhead {
+  static constexpr int EPILOGUE_WARPS = PLAIN || NT_ < 256 || sizeof(O) == 4 ? 8 : 16;
   static constexpr int PAIR = PAIR_, NT = NT_, PLANES = 1, PASS = sizeof(O) == 4 ? 8 : 0;
   static constexpr bool AMN = AMN_, BMN = BMN_, RAGGED = false;
   using Params = linear::Params;
@@ -142,7 +193,7 @@ template <typename O, typename B, int PAIR_, int NT_, bool AMN_, bool BMN_, bool
     if constexpr (PLAIN) {
       write_rows<O, NT / 2>(source, mine, out, p.ld, rows, p.n - c0, p.vectors & kVectors);
     } else {
-      finish_rows<O, B, NT / 2, PASS ? NT / 2 : 1>(p, source, mine, r0, c0);
+      finish_rows<O, B, NT * 4 / EPILOGUE_WARPS, PASS ? NT / 2 : 1>(p, source, mine, r0, c0);
     }
   }
   static __device__ void finish(const Params &, int, int) {}
@@ -276,8 +327,7 @@ template <typename T, int V> __global__ void __launch_bounds__(256, 5) slope_ker
         R::values(a[q], v);
         if (p.pre) {
           R::values(b[q], u);
-#pragma unroll
-          for (int x = 0; x < V; ++x) v[x] *= slope(u[x], p.act);
+          times_slope(v, u, p.act);
           stream::Run<T, V>::store(du + at * p.du_sr, v);
         }
 #pragma unroll
@@ -352,7 +402,9 @@ template <typename O, typename B> __global__ void __launch_bounds__(256) empty_k
     const int64_t r = i / p.n, c = i - r * p.n;
     const float u = p.bias ? bias_at<B>(p, c) : 0.f;
     if (p.pre) static_cast<B *>(p.pre)[r * p.ld + c] = from_f32<B>(u);
-    float y = activated(u, p.act);
+    float v[1] = {u};
+    activate(v, p.act);
+    float y = v[0];
     if (p.residual) y += to_f32(static_cast<const O *>(p.residual)[r * p.residual_ld + c]);
     static_cast<O *>(p.out)[r * p.ld + c] = from_f32<O>(y);
   }

@@ -58,31 +58,56 @@ __device__ __forceinline__ float larger(float a, float b) {
 // 1 / (1 + exp(-u)); below -88 the exponential is infinite and the result 0.
 __device__ __forceinline__ float sigmoid(float u) { return reciprocal(1.f + exp2_of(u * -kLog2E)); }
 
-__device__ __forceinline__ float activated(float u, int act) {
+__device__ __forceinline__ float relu(float u) { return larger(u, 0.f); }
+__device__ __forceinline__ float gelu(float u) {          // u Phi(u) = max(u, 0) - |u| Phi(-|u|)
+  float e;
+  const float z = smaller(fabsf(u), 40.f);
+  return larger(u, 0.f) - z * normal_tail(z, e);
+}
+__device__ __forceinline__ float silu(float u) { return u * sigmoid(u); }
+__device__ __forceinline__ float relu_slope(float u) { return u > 0.f ? 1.f : u != u ? u : 0.f; }
+__device__ __forceinline__ float gelu_slope(float u) {
+  float e;
+  const float z = smaller(fabsf(u), 40.f), h = normal_tail(z, e);
+  return fmaf(copysignf(z, u) * 0.3989422804014327f, e, u >= 0.f ? 1.f - h : h);
+}
+__device__ __forceinline__ float silu_slope(float u) {
+  const float s = sigmoid(u);
+  return s * fmaf(u, 1.f - s, 1.f);
+}
+// act of each value; v times act' of each u.  One branch for all of them.
+template <int N> __device__ __forceinline__ void activate(float (&v)[N], int act) {
   switch (act) {
-    case OZ_ACT_RELU: return larger(u, 0.f);
-    case OZ_ACT_GELU: {                       // u Phi(u) = max(u, 0) - |u| Phi(-|u|)
-      float e;
-      const float z = smaller(fabsf(u), 40.f);
-      return larger(u, 0.f) - z * normal_tail(z, e);
-    }
-    case OZ_ACT_SILU: return u * sigmoid(u);
-    default: return u;
+    case OZ_ACT_RELU:
+#pragma unroll
+      for (int x = 0; x < N; ++x) v[x] = relu(v[x]);
+      break;
+    case OZ_ACT_GELU:
+#pragma unroll
+      for (int x = 0; x < N; ++x) v[x] = gelu(v[x]);
+      break;
+    case OZ_ACT_SILU:
+#pragma unroll
+      for (int x = 0; x < N; ++x) v[x] = silu(v[x]);
+      break;
+    default: break;
   }
 }
-__device__ __forceinline__ float slope(float u, int act) {
+template <int N> __device__ __forceinline__ void times_slope(float (&v)[N], const float (&u)[N], int act) {
   switch (act) {
-    case OZ_ACT_RELU: return u > 0.f ? 1.f : u != u ? u : 0.f;
-    case OZ_ACT_GELU: {
-      float e;
-      const float z = smaller(fabsf(u), 40.f), h = normal_tail(z, e);
-      return fmaf(copysignf(z, u) * 0.3989422804014327f, e, u >= 0.f ? 1.f - h : h);
-    }
-    case OZ_ACT_SILU: {
-      const float s = sigmoid(u);
-      return s * fmaf(u, 1.f - s, 1.f);
-    }
-    default: return 1.f;
+    case OZ_ACT_RELU:
+#pragma unroll
+      for (int x = 0; x < N; ++x) v[x] *= relu_slope(u[x]);
+      break;
+    case OZ_ACT_GELU:
+#pragma unroll
+      for (int x = 0; x < N; ++x) v[x] *= gelu_slope(u[x]);
+      break;
+    case OZ_ACT_SILU:
+#pragma unroll
+      for (int x = 0; x < N; ++x) v[x] *= silu_slope(u[x]);
+      break;
+    default: break;
   }
 }
 

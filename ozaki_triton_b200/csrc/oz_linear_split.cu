@@ -292,9 +292,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
           if (r0 + i * step >= rows) continue;
           const int64_t at = (int64_t)(row0 + r0 + i * step) * p.ld + column;
           if (p.pre) store4(static_cast<T *>(p.pre) + at, p.vectors & kVectors, count, u[i]);
-          if (p.act)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) u[i][x] = activated(u[i][x], p.act);
+          activate(u[i], p.act);
           if (p.residual)
 #pragma unroll
             for (int x = 0; x < 4; ++x) u[i][x] += residual[i][x];

@@ -50,7 +50,6 @@ constexpr int kRows = 128;              // rows of one CTA's part of a tile
 constexpr int kBlock = 64;              // contraction elements of a stage
 constexpr int kLine = 128;              // bytes of a swizzled row
 constexpr int kMaxStages = 10;
-constexpr int kEpilogueWarps = 8;
 constexpr int kStagingBytes = 2048;     // of each epilogue warp: 32 rows of 64 bytes
 constexpr int kBarrierBytes = 512;
 constexpr int kSmemLimit = 227 * 1024;
@@ -62,19 +61,23 @@ struct NoLookAhead {
   template <class P, class T> static __device__ void look_ahead(const P &, const T &, int, int, Ahead &) {}
 };
 
-template <class J> __host__ __device__ constexpr int threads() { return 64 + 32 * kEpilogueWarps + (J::RAGGED ? 32 : 0); }
+// epilogue warps: 8, or what the job says
+template <class J, class = void> struct EpilogueWarps { static constexpr int value = 8; };
+template <class J> struct EpilogueWarps<J, decltype((void)J::EPILOGUE_WARPS)> { static constexpr int value = J::EPILOGUE_WARPS; };
+template <class J> __host__ __device__ constexpr int epilogue_warps() { return EpilogueWarps<J>::value; }
+template <class J> __host__ __device__ constexpr int threads() { return 64 + 32 * epilogue_warps<J>() + (J::RAGGED ? 32 : 0); }
 // columns of an epilogue warp (4 warps share the rows of a tile, a quarter each)
-template <class J> __host__ __device__ constexpr int warp_columns() { return J::NT * 4 / kEpilogueWarps; }
+template <class J> __host__ __device__ constexpr int warp_columns() { return J::NT * 4 / epilogue_warps<J>(); }
 template <class J> __host__ __device__ constexpr int a_bytes() { return kRows * kLine; }
 template <class J> __host__ __device__ constexpr int b_bytes() { return J::NT / J::PAIR * kLine; }
 template <class J> __host__ __device__ constexpr int stage_bytes() { return J::PLANES * (a_bytes<J>() + b_bytes<J>()); }
 template <class J> __host__ __device__ constexpr int stages() {
-  constexpr int room = kSmemLimit - 1024 - kBarrierBytes - kEpilogueWarps * kStagingBytes;
+  constexpr int room = kSmemLimit - 1024 - kBarrierBytes - epilogue_warps<J>() * kStagingBytes;
   constexpr int n = room / stage_bytes<J>();
   return n < kMaxStages ? n : kMaxStages;
 }
 template <class J> __host__ __device__ constexpr int smem_bytes() {
-  return 1024 + stages<J>() * stage_bytes<J>() + kEpilogueWarps * kStagingBytes + kBarrierBytes;
+  return 1024 + stages<J>() * stage_bytes<J>() + epilogue_warps<J>() * kStagingBytes + kBarrierBytes;
 }
 
 // Where a tile's operands lie: first row (or column) and matrix of A and B in
@@ -197,6 +200,7 @@ __global__ void __launch_bounds__(threads<J>(), 1)
                 const typename J::Params p) {
   using Tile = TileOf<typename J::Extra>;
   constexpr int PAIR = J::PAIR, NT = J::NT, S = stages<J>(), SB = stage_bytes<J>();
+  constexpr int kEpilogueWarps = epilogue_warps<J>();
   constexpr int BR = NT / PAIR;                       // B rows (columns of the tile) of one CTA
   constexpr int kTmemColumns = 2 * NT < 32 ? 32 : 2 * NT;
   static_assert((NT & (NT - 1)) == 0 && NT >= 32 && NT <= 256 && 2 * NT <= 512, "tile columns");
