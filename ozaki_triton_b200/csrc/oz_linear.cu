@@ -51,6 +51,23 @@ template <typename E> __device__ __forceinline__ void store8(E *to, bool vectors
   }
 }
 
+// 8 aligned values of E as they lie in memory.
+template <typename E> struct Run8 {
+  struct Raw { uint4 u[sizeof(E) / 2]; };
+  static __device__ __forceinline__ Raw load(const E *p) {
+    Raw r;
+#pragma unroll
+    for (int h = 0; h < (int)sizeof(E) / 2; ++h) r.u[h] = __ldg(reinterpret_cast<const uint4 *>(p) + h);
+    return r;
+  }
+  static __device__ __forceinline__ void values(const Raw &r, float (&v)[8]) {
+    const E *e = reinterpret_cast<const E *>(&r);
+#pragma unroll
+    for (int x = 0; x < 8; ++x) v[x] = to_f32(e[x]);
+  }
+  static __device__ __forceinline__ void store(E *p, const float (&v)[8]) { store8(p, true, 8, v); }
+};
+
 // The columns of a source 16 at a time, the next ones on their way (accumulators in tensor
 // memory) while the ones before are worked on.
 template <class Source> struct Ahead16;
@@ -83,39 +100,25 @@ __device__ __forceinline__ void finish_rows(const Params &p, const Source &sourc
   const int lane = threadIdx.x % 32, half = lane % 2;
   const int rows = (int)min(p.rows - r0, (int64_t)32), columns = (int)min(p.n - c0, (int64_t)COLS);
   if (rows <= 0 || columns <= 0) return;
-  float residual[2][8], bias[8] = {};
-  // what the columns from c on need besides the accumulators
-  auto fetch = [&](int c) {
-    const int64_t column = c0 + c + half * 8;
-    const int count = (int)min(p.n - column, (int64_t)8);
-    if (p.residual)
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        if (i * 16 + lane / 2 < rows)
-          load8(static_cast<const O *>(p.residual) + (r0 + i * 16 + lane / 2) * p.residual_ld + column,
-                p.vectors & kResidualVectors, count, residual[i]);
-    if (p.bias) {
-      if (p.bias_f32) load8(static_cast<const float *>(p.bias) + column, p.vectors & kBiasVectors, count, bias);
-      else load8(static_cast<const B *>(p.bias) + column, p.vectors & kBiasVectors, count, bias);
-    }
-  };
+  const int64_t at = (r0 + lane / 2) * p.ld + c0 + half * 8, next_row = 16 * p.ld;
+  const int64_t residual_row = 16 * p.residual_ld;
+  O *out = static_cast<O *>(p.out) + at;
+  B *pre = p.pre ? static_cast<B *>(p.pre) + at : nullptr;
+  const O *residual = p.residual ? static_cast<const O *>(p.residual) + (r0 + lane / 2) * p.residual_ld + c0 + half * 8
+                                 : nullptr;
+  const B *bias = p.bias && !p.bias_f32 ? static_cast<const B *>(p.bias) + c0 + half * 8 : nullptr;
+  const float *bias_f32 = p.bias && p.bias_f32 ? static_cast<const float *>(p.bias) + c0 + half * 8 : nullptr;
+  const int act = p.act;
   Ahead16<Source> ahead{source};
   ahead.start(0);
-  fetch(0);
-  const bool whole = rows == 32 && columns == COLS && (p.vectors & kVectors);
-  const int64_t at = (r0 + lane / 2) * p.ld + c0 + half * 8, next_row = 16 * p.ld;
-  O *out = static_cast<O *>(p.out) + at;
-  B *pre = static_cast<B *>(p.pre) + at;
-#pragma unroll(UNROLL)
-  for (int c = 0; c < COLS; c += 16) {
-    if (c >= columns) continue;
+  // this lane's part of 16 columns' accumulators, through the staging
+  auto turn = [&](int c, bool more, float (&u)[2][8]) {
     float v[16];
     ahead.finish(v);
 #pragma unroll
-    for (int u = 0; u < 4; ++u) *staged(mine, lane, u) = *reinterpret_cast<uint4 *>(&v[u * 4]);
-    if (c + 16 < columns) ahead.start(c + 16);
+    for (int x = 0; x < 4; ++x) *staged(mine, lane, x) = *reinterpret_cast<uint4 *>(&v[x * 4]);
+    if (more) ahead.start(c + 16);
     __syncwarp();
-    float u[2][8];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -123,42 +126,89 @@ __device__ __forceinline__ void finish_rows(const Params &p, const Source &sourc
         const uint4 raw = *staged(mine, i * 16 + lane / 2, half * 2 + h);
         const float *f = reinterpret_cast<const float *>(&raw);
 #pragma unroll
-        for (int x = 0; x < 4; ++x) u[i][h * 4 + x] = f[x] + bias[h * 4 + x];
+        for (int x = 0; x < 4; ++x) u[i][h * 4 + x] = f[x];
       }
     __syncwarp();
-    if (whole) {
-      if (p.pre) {
-        store8(pre + c, true, 8, u[0]);
-        store8(pre + c + next_row, true, 8, u[1]);
+  };
+  constexpr int kAll = kVectors | kResidualVectors | kBiasVectors;
+  if (rows == 32 && columns == COLS && (p.vectors & kAll) == kAll) {
+    using Out = Run8<O>;
+    using In = Run8<B>;
+    typename In::Raw b{};
+    typename Out::Raw r[2]{};
+    float4 b32[2]{};
+    auto fetch = [&](int c) {
+      if (bias) b = In::load(bias + c);
+      if (bias_f32) {
+        b32[0] = __ldg(reinterpret_cast<const float4 *>(bias_f32 + c));
+        b32[1] = __ldg(reinterpret_cast<const float4 *>(bias_f32 + c) + 1);
       }
-      activate(u[0], p.act);
-      activate(u[1], p.act);
-      if (p.residual)
+      if (residual) {
+        r[0] = Out::load(residual + c);
+        r[1] = Out::load(residual + c + residual_row);
+      }
+    };
+    fetch(0);
+#pragma unroll(UNROLL)
+    for (int c = 0; c < COLS; c += 16) {
+      float u[2][8], add[8];
+      turn(c, c + 16 < COLS, u);
+      if (bias || bias_f32) {
+        if (bias) In::values(b, add);
+        else add[0] = b32[0].x, add[1] = b32[0].y, add[2] = b32[0].z, add[3] = b32[0].w, add[4] = b32[1].x,
+             add[5] = b32[1].y, add[6] = b32[1].z, add[7] = b32[1].w;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int x = 0; x < 8; ++x) u[0][x] += add[x], u[1][x] += add[x];
+      }
+      if (pre) {
+        In::store(pre + c, u[0]);
+        In::store(pre + c + next_row, u[1]);
+      }
+      if (act) {
+        activate(u[0], act);
+        activate(u[1], act);
+      }
+      if (residual)
 #pragma unroll
-          for (int x = 0; x < 8; ++x) u[i][x] += residual[i][x];
+        for (int i = 0; i < 2; ++i) {
+          Out::values(r[i], add);
+#pragma unroll
+          for (int x = 0; x < 8; ++x) u[i][x] += add[x];
+        }
       if (c + 16 < COLS) fetch(c + 16);
-      store8(out + c, true, 8, u[0]);
-      store8(out + c + next_row, true, 8, u[1]);
-    } else {
-      const int count = (int)min(p.n - c0 - c - half * 8, (int64_t)8);
+      Out::store(out + c, u[0]);
+      Out::store(out + c + next_row, u[1]);
+    }
+    return;
+  }
+  // the edges, and rows or a bias off the 16-byte boundaries
+#pragma unroll(UNROLL)
+  for (int c = 0; c < COLS; c += 16) {
+    if (c >= columns) continue;
+    const int count = (int)min(p.n - c0 - c - half * 8, (int64_t)8);
+    float u[2][8], add[8];
+    turn(c, c + 16 < columns, u);
+    if (bias || bias_f32) {
+      if (bias) load8(bias + c, p.vectors & kBiasVectors, count, add);
+      else load8(bias_f32 + c, p.vectors & kBiasVectors, count, add);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if (i * 16 + lane / 2 >= rows) continue;
-        if (p.pre) store8(pre + c + i * next_row, p.vectors & kVectors, count, u[i]);
-        activate(u[i], p.act);
-        if (p.residual)
+      for (int x = 0; x < 8; ++x) u[0][x] += add[x], u[1][x] += add[x];
+    }
 #pragma unroll
-          for (int x = 0; x < 8; ++x) u[i][x] += residual[i][x];
-        store8(out + c + i * next_row, p.vectors & kVectors, count, u[i]);
+    for (int i = 0; i < 2; ++i) {
+      if (i * 16 + lane / 2 >= rows) continue;
+      if (pre) store8(pre + c + i * next_row, p.vectors & kVectors, count, u[i]);
+      activate(u[i], act);
+      if (residual) {
+        load8(residual + c + i * residual_row, p.vectors & kResidualVectors, count, add);
+#pragma unroll
+        for (int x = 0; x < 8; ++x) u[i][x] += add[x];
       }
-      if (c + 16 < columns) fetch(c + 16);
+      store8(out + c + i * next_row, p.vectors & kVectors, count, u[i]);
     }
   }
 }
 
-// A along the result's rows, B along its columns.
 // What follows a product keeps 16 epilogue warps busy (a plain one's 8 wait for its stores;
 // the sums of passes of an fp32 result leave no registers for 16).
 template <typename O, typename B, int PAIR_, int NT_, bool AMN_, bool BMN_, bool PLAIN> struct LinearJob : NoLookAhead {
@@ -428,7 +478,8 @@ extern "C" int oz_linear(const oz_linear_args *args, void *stream) {
                  0, a.bias_dtype == OZ_F32, a.act, tile::instruction(a.dtype)};
   if ((uintptr_t)a.y % 16 == 0 && a.n * es % 16 == 0 && (!a.pre || ((uintptr_t)a.pre % 16 == 0 && a.n % 8 == 0)))
     p.vectors |= kVectors;
-  if ((uintptr_t)a.residual % 16 == 0 && (a.rows == 1 || a.residual_sr * es % 16 == 0)) p.vectors |= kResidualVectors;
+  if (!a.residual || ((uintptr_t)a.residual % 16 == 0 && (a.rows == 1 || a.residual_sr * es % 16 == 0)))
+    p.vectors |= kResidualVectors;
   if ((uintptr_t)a.bias % 16 == 0) p.vectors |= kBiasVectors;
   if (a.k == 0) {
     const dim3 grid((unsigned)std::min<int64_t>((a.rows * a.n + 255) / 256, stream::sm_count() * 8));
