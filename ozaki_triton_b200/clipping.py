@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import ctypes
+from array import array
 from typing import Iterable, Optional, Sequence
 
 import torch
@@ -13,6 +14,7 @@ from .experts import _CURRENT_DEVICE, _LEVEL, _OnDevice, _check_places, _check_t
 
 CLIP_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 _CODES = {t: _OZ_DTYPE[t] for t in CLIP_DTYPES}
+_ALLOWED = frozenset(CLIP_DTYPES)
 
 
 def _dense(t: torch.Tensor) -> bool:
@@ -50,33 +52,34 @@ def clip_gradients(grads: Iterable[torch.Tensor], max_norm: float, *, eps: float
     assert len(outs) == len(grads), f"{len(grads)} gradients, but {len(outs)} results"
     if _LEVEL._current_level >= 0:
         _check_tangents(*grads, *outs)
-    n = len(grads)
-    device = grads[0].get_device()
-    for t in grads if out is None else grads + outs:
-        if t.dtype not in _CODES:
-            raise AssertionError(f"unsupported dtype: {t.dtype}")
-        if t.get_device() != device or device < 0:
-            _check_places(grads[0], t)
-        if not t.is_contiguous() and not _dense(t):
-            raise AssertionError(f"a gradient of shape {tuple(t.shape)} and strides {t.stride()} is not dense")
-    if out is not None:
+    n, first = len(grads), grads[0]
+    device = first.get_device()
+    given = grads if out is None else grads + outs
+    types = [t.dtype for t in given]
+    if not _ALLOWED.issuperset(types):
+        raise AssertionError(f"unsupported dtype: {next(t for t in types if t not in _ALLOWED)}")
+    if device < 0 or any([t.get_device() != device for t in given]):
+        _check_places(*given)
+    if not all([t.is_contiguous() for t in given]):
+        for t in given:
+            assert _dense(t), f"a gradient of shape {tuple(t.shape)} and strides {t.stride()} is not dense"
         for g, o in zip(grads, outs):
-            if g.shape != o.shape or (g.stride() != o.stride() and not (g.is_contiguous() and o.is_contiguous())):
-                raise AssertionError(f"a result must be laid out like its gradient: {tuple(o.shape)}, strides "
-                                     f"{o.stride()} for {tuple(g.shape)}, strides {g.stride()}")
+            assert g.stride() == o.stride() or (g.is_contiguous() and o.is_contiguous()), \
+                f"a result must be laid out like its gradient: strides {o.stride()} for {g.stride()}"
+    if out is not None and not all([g.is_same_size(o) for g, o in zip(grads, outs)]):
+        raise AssertionError("a result must have its gradient's shape")
     lib = _lib.load()
-    norm = grads[0].new_empty((), dtype=torch.float32)
+    norm = first.new_empty((), dtype=torch.float32)
     size = lib.oz_clip_workspace_bytes(n)
-    workspace = grads[0].new_empty((size,), dtype=torch.uint8)
-    pointers = ctypes.c_void_p * n
-    from_ = pointers(*[t.data_ptr() for t in grads])
-    to = from_ if out is None else pointers(*[t.data_ptr() for t in outs])
-    sizes = (ctypes.c_int64 * n)(*[t.numel() for t in grads])
-    types = (ctypes.c_int32 * n)(*[_CODES[t.dtype] for t in grads])
-    out_types = types if out is None else (ctypes.c_int32 * n)(*[_CODES[t.dtype] for t in outs])
-    address = ctypes.addressof
-    args = _lib.ClipArgs(address(from_), address(to), address(sizes), address(types), address(out_types),
-                         norm.data_ptr(), workspace.data_ptr(), size, float(max_norm), float(eps), n, 0)
+    workspace = first.new_empty((size,), dtype=torch.uint8)
+    # addresses, sizes and types as the library takes them
+    pointers = array("Q", [t.data_ptr() for t in given])
+    sizes = array("q", [t.numel() for t in grads])
+    codes = array("i", [_CODES[t] for t in types])
+    at, at_codes = pointers.buffer_info()[0], codes.buffer_info()[0]
+    second = 0 if out is None else n
+    args = _lib.ClipArgs(at, at + 8 * second, sizes.buffer_info()[0], at_codes, at_codes + 4 * second, norm.data_ptr(),
+                         workspace.data_ptr(), size, float(max_norm), float(eps), n, 0)
     if _CURRENT_DEVICE() == device:
         status = lib.oz_clip(ctypes.byref(args), _stream_of(device))
     else:

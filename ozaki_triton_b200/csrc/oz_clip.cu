@@ -3,8 +3,8 @@
 //
 //   norm = sqrt(sum of all squares),  out = g min(1, max_norm / (norm + eps))
 //
-// Two launches read the gradients: the first sums squares (fp32 in a thread's
-// piece, fp64 across pieces, in an order that does not depend on timing), the
+// Two launches read the gradients: the first sums squares (fp32 within 16
+// bytes, fp64 beyond, in an order that does not depend on timing), the
 // second has every block add up the first's sums and scales.  Bound by memory:
 // the gradients are read twice and the results written once.
 
@@ -19,8 +19,9 @@ namespace {
 using namespace stream;
 
 constexpr int kThreads = 256;
-constexpr int kPiece = 8192;          // elements of a block's turn
-constexpr int kAtOnce = 4;            // 16-byte loads of a thread on their way
+constexpr int kBlocksPerSm = 4, kScaleBlocksPerSm = 3;      // resident together
+constexpr int kSmallPiece = 8192, kLargePiece = 16384;     // elements of a block's turn
+constexpr int kAtOnce = 4;            // 16-byte loads of a thread: these are worked on while as many are on their way
 
 struct Tensor {
   const void *g;
@@ -31,7 +32,7 @@ struct Tensor {
 };
 template <int N> struct Table {
   Tensor t[N];
-  int tensors, pieces;
+  int tensors, pieces, piece;          // piece: its elements
 };
 struct Sums {
   double *partial;                    // one of each block of each summing launch
@@ -40,12 +41,6 @@ struct Sums {
   float max_norm, eps;
 };
 
-// The pieces of this block, one after the other in memory, and the tensor of the first.
-struct Share { int first, end; };
-template <int N> __device__ __forceinline__ Share share_of(const Table<N> &table) {
-  return {(int)((int64_t)table.pieces * blockIdx.x / gridDim.x),
-          (int)((int64_t)table.pieces * (blockIdx.x + 1) / gridDim.x)};
-}
 template <int N> __device__ __forceinline__ int tensor_of(const Table<N> &table, int piece) {
   int low = 0, high = table.tensors - 1;      // the last tensor whose first piece is not after it
   while (low < high) {
@@ -76,45 +71,50 @@ __device__ __forceinline__ void set_element(void *out, int64_t i, int type, floa
   else static_cast<__nv_bfloat16 *>(out)[i] = from_f32<__nv_bfloat16>(v);
 }
 
-// Loads 16-byte runs j of [0, runs) of a piece kAtOnce at a time, calls f(run, bits).
-template <typename F> __device__ __forceinline__ void each_run(const uint4 *g, int runs, F f) {
+// Calls f(run, bits) for this thread's runs (16 bytes, or 8) of a piece.
+template <typename U, typename F> __device__ __forceinline__ void each_run(const U *g, int runs, F f) {
+  constexpr int kAtOnce = oz::kAtOnce * 16 / sizeof(U);
+  U u[kAtOnce], next[kAtOnce];
+  auto load = [&](int i, U (&to)[kAtOnce]) {
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j)
+      if (i + j * kThreads < runs) to[j] = g[i + j * kThreads];
+  };
+  load(threadIdx.x, u);
 #pragma unroll 1
-  for (int i0 = threadIdx.x; i0 < runs; i0 += kThreads * kAtOnce) {
-    uint4 u[kAtOnce];
+  for (int i = threadIdx.x; i < runs; i += kThreads * kAtOnce) {
+    load(i + kThreads * kAtOnce, next);
 #pragma unroll
     for (int j = 0; j < kAtOnce; ++j)
-      if (i0 + j * kThreads < runs) u[j] = g[i0 + j * kThreads];
+      if (i + j * kThreads < runs) f(i + j * kThreads, u[j]);
 #pragma unroll
-    for (int j = 0; j < kAtOnce; ++j)
-      if (i0 + j * kThreads < runs) f(i0 + j * kThreads, u[j]);
+    for (int j = 0; j < kAtOnce; ++j) u[j] = next[j];
   }
 }
 
 template <int N>
-__global__ void __launch_bounds__(kThreads, 6) norm_kernel(const __grid_constant__ Table<N> table, double *partial) {
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm) norm_kernel(const __grid_constant__ Table<N> table, double *partial) {
   start_after_earlier_kernels();
   double all = 0;
-  const Share share = share_of(table);
-  int at = tensor_of(table, share.first);
-  for (int piece = share.first; piece < share.end; ++piece) {
+  // neighbouring blocks take neighbouring pieces: what is read at a time lies together
+  int at = tensor_of(table, min((int)blockIdx.x, table.pieces - 1));
+  for (int piece = blockIdx.x; piece < table.pieces; piece += gridDim.x) {
     while (at + 1 < table.tensors && table.t[at + 1].first <= piece) ++at;
     const Tensor &t = table.t[at];
-    const int64_t from = (int64_t)(piece - t.first) * kPiece;
-    const int n = (int)min(t.n - from, (int64_t)kPiece), type = t.types & 15, es = type == OZ_F32 ? 4 : 2;
+    const int64_t from = (int64_t)(piece - t.first) * table.piece;
+    const int n = (int)min(t.n - from, (int64_t)table.piece), type = t.types & 15, es = type == OZ_F32 ? 4 : 2;
     const char *g = static_cast<const char *>(t.g) + from * es;
     const int runs = t.types >> 8 & 1 ? n * es / 16 : 0;
-    float s = 0.f;
     each_run(reinterpret_cast<const uint4 *>(g), runs, [&](int, const uint4 &u) {
-      if (type == OZ_F32) s += squares<float>(u);
-      else if (type == OZ_F16) s += squares<__half>(u);
-      else s += squares<__nv_bfloat16>(u);
+      if (type == OZ_F32) all += squares<float>(u);
+      else if (type == OZ_F16) all += squares<__half>(u);
+      else all += squares<__nv_bfloat16>(u);
     });
 #pragma unroll 1
     for (int i = runs * (16 / es) + threadIdx.x; i < n; i += kThreads) {
       const float v = element(g, i, type);
-      s = fmaf(v, v, s);
+      all += v * v;
     }
-    all += s;
   }
   __shared__ double warp_sum[kThreads / 32];
 #pragma unroll
@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(kThreads, 6) norm_kernel(const __grid_constant
   }
 }
 
-// A run of T, scaled, to run r of out (its size is V elements of O, 8 to 32 bytes).
+// A run of T, scaled, to run r of out.
 template <typename T, typename O> __device__ __forceinline__ void scaled(const uint4 &u, O *out, int r, float scale) {
   constexpr int V = 16 / sizeof(T);
   float v[V];
@@ -136,20 +136,25 @@ template <typename T, typename O> __device__ __forceinline__ void scaled(const u
   for (int x = 0; x < V; ++x) v[x] *= scale;
   out += (int64_t)r * V;
   if constexpr (sizeof(O) == sizeof(T)) {
-    __stcs(reinterpret_cast<uint4 *>(out), pack<O>(v));
-  } else if constexpr (sizeof(O) == 4) {
-    __stcs(reinterpret_cast<float4 *>(out), make_float4(v[0], v[1], v[2], v[3]));
-    __stcs(reinterpret_cast<float4 *>(out) + 1, make_float4(v[4], v[5], v[6], v[7]));
-  } else {
+    *reinterpret_cast<uint4 *>(out) = pack<O>(v);
+  } else {                                    // fp32 to 16 bits
     O w[V];
 #pragma unroll
     for (int x = 0; x < V; ++x) w[x] = from_f32<O>(v[x]);
-    __stcs(reinterpret_cast<uint2 *>(out), *reinterpret_cast<const uint2 *>(w));
+    *reinterpret_cast<uint2 *>(out) = *reinterpret_cast<const uint2 *>(w);
   }
 }
+// 16 bits to fp32: 8 bytes, so that a warp's results are next to each other (from 16 bytes a lane
+// wrote two halves of 32: 631 us for 400 million gradients, this 543).
+template <typename T> __device__ __forceinline__ void widened(const uint2 &u, float *out, int r, float scale) {
+  const T *e = reinterpret_cast<const T *>(&u);
+  reinterpret_cast<float4 *>(out)[r] =
+      make_float4(to_f32(e[0]) * scale, to_f32(e[1]) * scale, to_f32(e[2]) * scale, to_f32(e[3]) * scale);
+}
 
-template <int N>
-__global__ void __launch_bounds__(kThreads, 4) scale_kernel(const __grid_constant__ Table<N> table, const Sums sums) {
+// PAIR: the types of all gradients and results (type | to << 4), or 0 where they differ.
+template <int N, int PAIR>
+__global__ void __launch_bounds__(kThreads, kScaleBlocksPerSm) scale_kernel(const __grid_constant__ Table<N> table, const Sums sums) {
   __shared__ float shared_scale;
   __shared__ double warp_sum[kThreads / 32];
   start_after_earlier_kernels();
@@ -168,30 +173,39 @@ __global__ void __launch_bounds__(kThreads, 4) scale_kernel(const __grid_constan
   }
   __syncthreads();
   const float scale = shared_scale;
-  const Share share = share_of(table);
-  if (share.first >= share.end) return;
+  if ((int)blockIdx.x >= table.pieces) return;
   // the pieces read last are the first here: some of them are still in L2
-  int at = tensor_of(table, share.end - 1);
-  for (int piece = share.end - 1; piece >= share.first; --piece) {
+  int at = tensor_of(table, table.pieces - 1 - (int)blockIdx.x);
+  for (int piece = table.pieces - 1 - (int)blockIdx.x; piece >= 0; piece -= gridDim.x) {
     while (table.t[at].first > piece) --at;
     const Tensor &t = table.t[at];
-    const int64_t from = (int64_t)(piece - t.first) * kPiece;
-    const int n = (int)min(t.n - from, (int64_t)kPiece), type = t.types & 15, to = t.types >> 4 & 15;
+    const int64_t from = (int64_t)(piece - t.first) * table.piece;
+    const int types = PAIR ? PAIR : t.types, type = types & 15, to = types >> 4 & 15;
+    const int n = (int)min(t.n - from, (int64_t)table.piece);
     const int es = type == OZ_F32 ? 4 : 2, os = to == OZ_F32 ? 4 : 2;
     const char *g = static_cast<const char *>(t.g) + from * es;
     char *out = static_cast<char *>(t.out) + from * os;
     const int runs = t.types >> 8 & 1 ? n * es / 16 : 0;
-    each_run(reinterpret_cast<const uint4 *>(g), runs, [&](int r, const uint4 &u) {
-      auto run = [&](auto g0) {
-        using T = decltype(g0);
-        if (to == OZ_F32) scaled<T>(u, reinterpret_cast<float *>(out), r, scale);
-        else if (to == OZ_F16) scaled<T>(u, reinterpret_cast<__half *>(out), r, scale);
-        else scaled<T>(u, reinterpret_cast<__nv_bfloat16 *>(out), r, scale);
-      };
-      if (type == OZ_F32) run(float{});
-      else if (type == OZ_F16) run(__half{});
-      else run(__nv_bfloat16{});
-    });
+    if (es == 2 && os == 4) {
+      each_run(reinterpret_cast<const uint2 *>(g), 2 * runs, [&](int r, const uint2 &u) {
+        if (type == OZ_F16) widened<__half>(u, reinterpret_cast<float *>(out), r, scale);
+        else widened<__nv_bfloat16>(u, reinterpret_cast<float *>(out), r, scale);
+      });
+    } else {
+      each_run(reinterpret_cast<const uint4 *>(g), runs, [&](int r, const uint4 &u) {
+        if (type == OZ_F32) {
+          if (to == OZ_F32) scaled<float>(u, reinterpret_cast<float *>(out), r, scale);
+          else if (to == OZ_F16) scaled<float>(u, reinterpret_cast<__half *>(out), r, scale);
+          else scaled<float>(u, reinterpret_cast<__nv_bfloat16 *>(out), r, scale);
+        } else if (type == OZ_F16) {
+          if (to == OZ_F16) scaled<__half>(u, reinterpret_cast<__half *>(out), r, scale);
+          else scaled<__half>(u, reinterpret_cast<__nv_bfloat16 *>(out), r, scale);
+        } else {
+          if (to == OZ_F16) scaled<__nv_bfloat16>(u, reinterpret_cast<__half *>(out), r, scale);
+          else scaled<__nv_bfloat16>(u, reinterpret_cast<__nv_bfloat16 *>(out), r, scale);
+        }
+      });
+    }
 #pragma unroll 1
     for (int i = runs * (16 / es) + threadIdx.x; i < n; i += kThreads)
       set_element(out, i, to, element(g, i, type) * scale);
@@ -200,12 +214,12 @@ __global__ void __launch_bounds__(kThreads, 4) scale_kernel(const __grid_constan
 
 // A launch takes the addresses of at most this many tensors as arguments.
 constexpr int kFew = 64, kMany = 640;
-constexpr int kBlocksPerSm = 6, kScaleBlocksPerSm = 4;      // resident together
 
 int blocks_of(int64_t pieces, int per_sm) { return (int)std::min<int64_t>(pieces, (int64_t)sm_count() * per_sm); }
 
-template <int N> Table<N> table_of(const oz_clip_args &a, int first, int count) {
+template <int N> Table<N> table_of(const oz_clip_args &a, int first, int count, int piece) {
   Table<N> table;
+  table.piece = piece;
   int64_t pieces = 0;
   table.tensors = 0;
   for (int i = first; i < first + count; ++i) {
@@ -215,21 +229,23 @@ template <int N> Table<N> table_of(const oz_clip_args &a, int first, int count) 
     const bool runs = (uintptr_t)a.grads[i] % 16 == 0 && (uintptr_t)a.outs[i] % (es == 4 && os == 2 ? 8 : 16) == 0;
     table.t[table.tensors++] = Tensor{a.grads[i], a.outs[i], n, (int)pieces,
                                       a.dtypes[i] | a.out_dtypes[i] << 4 | (runs ? 1 << 8 : 0)};
-    pieces += (n + kPiece - 1) / kPiece;
+    pieces += (n + piece - 1) / piece;
   }
   table.pieces = (int)pieces;
   return table;
 }
-int64_t pieces_of(const oz_clip_args &a, int first, int count) {
+int64_t pieces_of(const oz_clip_args &a, int piece) {
   int64_t pieces = 0;
-  for (int i = first; i < first + count; ++i) pieces += (a.sizes[i] + kPiece - 1) / kPiece;
+  for (int i = 0; i < a.tensors; ++i) pieces += (a.sizes[i] + piece - 1) / piece;
   return pieces;
 }
 
 template <int N> int run(const oz_clip_args &a, Sums sums, cudaStream_t st) {
   sums.blocks = 0;
+  // large pieces where every block has several of them
+  const int piece = pieces_of(a, kLargePiece) >= (int64_t)sm_count() * kBlocksPerSm * 4 ? kLargePiece : kSmallPiece;
   for (int i = 0; i < a.tensors; i += N) {
-    const auto table = table_of<N>(a, i, std::min(N, a.tensors - i));
+    const auto table = table_of<N>(a, i, std::min(N, a.tensors - i), piece);
     if (!table.pieces) continue;
     const int blocks = blocks_of(table.pieces, kBlocksPerSm);
     if (int rc = launch(norm_kernel<N>, dim3(blocks), kThreads, 0, st, "norm_kernel launch", table,
@@ -240,11 +256,24 @@ template <int N> int run(const oz_clip_args &a, Sums sums, cudaStream_t st) {
   // the last tensors first, like the pieces in a launch
   const int last = a.tensors ? (a.tensors - 1) / N * N : 0;
   for (int i = last; i >= 0; i -= N) {
-    const auto table = table_of<N>(a, i, std::min(N, a.tensors - i));
+    const auto table = table_of<N>(a, i, std::min(N, a.tensors - i), piece);
     if (!table.pieces && i != last) continue;                   // one launch at least writes the norm
-    if (int rc = launch(scale_kernel<N>, dim3(std::max(1, blocks_of(table.pieces, kScaleBlocksPerSm))), kThreads, 0, st,
-                        "scale_kernel launch", table, sums))
-      return rc;
+    int types = table.tensors ? table.t[0].types & 255 : 0;
+    for (int j = 1; j < table.tensors; ++j)
+      if ((table.t[j].types & 255) != types) types = 0;
+    auto scale = [&](auto pair) {
+      return launch(scale_kernel<N, decltype(pair)::value>, dim3(std::max(1, blocks_of(table.pieces, kScaleBlocksPerSm))),
+                    kThreads, 0, st, "scale_kernel launch", table, sums);
+    };
+    constexpr int F = OZ_F32, H = OZ_F16, B = OZ_BF16;
+    int rc;
+    if (types == (F | F << 4)) rc = scale(std::integral_constant<int, F | F << 4>{});
+    else if (types == (H | H << 4)) rc = scale(std::integral_constant<int, H | H << 4>{});
+    else if (types == (B | B << 4)) rc = scale(std::integral_constant<int, B | B << 4>{});
+    else if (types == (H | F << 4)) rc = scale(std::integral_constant<int, H | F << 4>{});
+    else if (types == (B | F << 4)) rc = scale(std::integral_constant<int, B | F << 4>{});
+    else rc = scale(std::integral_constant<int, 0>{});
+    if (rc) return rc;
   }
   return OZ_OK;
 }
@@ -290,7 +319,7 @@ extern "C" int oz_clip(const oz_clip_args *args, void *stream) {
   } catch (...) {
     return set_error(OZ_ERR_INVALID, "out of host memory");
   }
-  if (pieces_of(a, 0, a.tensors) > INT32_MAX / 2) return set_error(OZ_ERR_INVALID, "size out of range");
+  if (pieces_of(a, kSmallPiece) > INT32_MAX / 2) return set_error(OZ_ERR_INVALID, "size out of range");
   // results that share memory would be scaled twice, or in parts
   std::sort(ranges.begin(), ranges.end(), [](const Range &x, const Range &y) { return x.from < y.from; });
   for (size_t i = 1; i < ranges.size(); ++i)

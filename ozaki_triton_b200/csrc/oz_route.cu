@@ -749,9 +749,10 @@ template <typename T, int V> __global__ void __launch_bounds__(256, 6) dispatch_
   }
 }
 
+constexpr int combine_blocks(int k) { return k >= 8 ? 3 : k >= 4 ? 4 : 5; }       // of an SM
 // y[t] = sum_j w rows[slot], in the order of j, K loads on their way at a time; the next
 // token's slots are loaded before this one's rows arrive.
-template <typename T, int V, int K> __global__ void __launch_bounds__(256, K >= 8 ? 3 : K >= 4 ? 4 : 5) combine_kernel(
+template <typename T, int V, int K> __global__ void __launch_bounds__(256, combine_blocks(K)) combine_kernel(
     const RowsParams p, const Spread at) {
   start_after_earlier_kernels();
   const int group = (int)threadIdx.x / at.threads, in = (int)threadIdx.x - group * at.threads;
@@ -786,6 +787,104 @@ template <typename T, int V, int K> __global__ void __launch_bounds__(256, K >= 
       Run<T, V>::store(static_cast<T *>(p.x_out) + t * p.d + c, y);
     }
     picks = next;
+  }
+}
+
+// Rows of 16-bit elements off the 16-byte boundaries: a warp moves 512 elements of a row at a
+// time by aligned words, whatever the rows' parities.  Words holds 8 words a lane of a
+// source from its element c0 on (they start in the middle of one where the source's
+// address does: the halves that belong to neither stay unused, but share their word with
+// an element, so they can be read).  pair(i) with parity h is elements h + 2 m, h + 2 m + 1, m
+// = 32 i + lane, counted from c0.
+constexpr int kWordSpan = 512;
+struct Words {
+  uint32_t direct[8], shifted[8];
+  int off;
+  __device__ __forceinline__ void load(const unsigned short *from, int count) {
+    const int lane = threadIdx.x % 32;
+    off = (int)((uintptr_t)from >> 1 & 1);
+    const uint32_t *words = reinterpret_cast<const uint32_t *>(from - off);
+    uint32_t w[9];
+#pragma unroll
+    for (int i = 0; i < 9; ++i) {
+      const int j = i * 32 + lane;
+      w[i] = 2 * j - off < count && (i < 8 || lane == 0) ? __ldg(words + j) : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t down = __shfl_down_sync(0xffffffffu, w[i], 1), over = __shfl_sync(0xffffffffu, w[i + 1], 0);
+      const uint32_t next = lane == 31 ? over : down;
+      direct[i] = off ? next : w[i];
+      shifted[i] = __funnelshift_r(w[i], next, 16);
+    }
+  }
+  __device__ __forceinline__ uint32_t pair(int i, int h) const { return off == h ? direct[i] : shifted[i]; }
+};
+
+__global__ void __launch_bounds__(256, 4) dispatch_words_kernel(const RowsParams p, int blocks) {
+  using E = unsigned short;
+  start_after_earlier_kernels();
+  if ((int)blockIdx.x >= blocks) return clear_rest<__half, 1>(p, blocks);
+  const int lane = threadIdx.x % 32, parts = (p.d + kWordSpan - 1) / kWordSpan;
+  const int64_t all = p.tokens * parts;
+  for (int64_t v = (int64_t)blockIdx.x * 8 + threadIdx.x / 32; v < all; v += (int64_t)blocks * 8) {
+    const int64_t t = v / parts;
+    const int c0 = (int)(v - t * parts) * kWordSpan, count = min(p.d - c0, kWordSpan);
+    const E *from = static_cast<const E *>(p.x) + t * p.x_row + c0;
+    Words words;
+    words.load(from, count);
+    for (int j = 0; j < p.k; ++j) {
+      const int64_t s = slot_of(p, t * p.k + j);
+      if (s < 0) continue;
+      E *to = static_cast<E *>(p.rows_out) + s * p.d + c0;
+      const int h = (int)((uintptr_t)to >> 1 & 1);
+      uint32_t *pairs = reinterpret_cast<uint32_t *>(to + h);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (h + 2 * (i * 32 + lane) + 1 < count) pairs[i * 32 + lane] = words.pair(i, h);
+      if (lane == 0 && h) to[0] = from[0];
+      if (lane == 1 && (count - h) % 2) to[count - 1] = from[count - 1];
+    }
+  }
+}
+
+template <typename T> __global__ void __launch_bounds__(256, 3) combine_words_kernel(const RowsParams p) {
+  using E = unsigned short;
+  start_after_earlier_kernels();
+  const int lane = threadIdx.x % 32, parts = (p.d + kWordSpan - 1) / kWordSpan;
+  const int64_t all = p.tokens * parts;
+  auto low = [](uint32_t u) { const E e = (E)u; return to_f32(*reinterpret_cast<const T *>(&e)); };
+  for (int64_t v = (int64_t)blockIdx.x * 8 + threadIdx.x / 32; v < all; v += (int64_t)gridDim.x * 8) {
+    const int64_t t = v / parts;
+    const int c0 = (int)(v - t * parts) * kWordSpan, count = min(p.d - c0, kWordSpan);
+    T *to = static_cast<T *>(p.x_out) + t * p.d + c0;
+    const int h = (int)((uintptr_t)to >> 1 & 1);
+    float y[8][2] = {}, edge = 0.f;               // edge: lane 0's first element, lane 1's last
+    const int at = lane == 0 ? 0 : count - 1;
+    const bool single = lane == 0 ? h != 0 : lane == 1 && (count - h) % 2;
+#pragma unroll 2
+    for (int j = 0; j < p.k; ++j) {
+      const int64_t s = slot_of(p, t * p.k + j);
+      if (s < 0) continue;
+      const float w = p.weights ? __ldg(p.weights + t * p.k + j) : 1.f;
+      const E *from = static_cast<const E *>(p.rows) + s * p.rows_row + c0;
+      Words words;
+      words.load(from, count);
+      if (single) edge = fmaf(w, low(__ldg(from + at)), edge);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t u = words.pair(i, h);
+        y[i][0] = fmaf(w, low(u), y[i][0]);
+        y[i][1] = fmaf(w, low(u >> 16), y[i][1]);
+      }
+    }
+    uint32_t *pairs = reinterpret_cast<uint32_t *>(to + h);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      T e[2] = {from_f32<T>(y[i][0]), from_f32<T>(y[i][1])};
+      if (h + 2 * (i * 32 + lane) + 1 < count) pairs[i * 32 + lane] = *reinterpret_cast<const uint32_t *>(e);
+    }
+    if (single) to[at] = from_f32<T>(edge);
   }
 }
 
@@ -877,6 +976,12 @@ Spread spread_over(int64_t runs, int64_t tokens, bool warps, int resident, int64
   s.tokens = 256 / s.threads;
   blocks = std::min<int64_t>((tokens + s.tokens - 1) / s.tokens, (int64_t)sm_count() * resident);
   return s;
+}
+
+// Blocks of 8 warps, a warp 512 elements of a row at a time.
+int64_t word_blocks(int64_t tokens, int64_t d, int resident) {
+  const int64_t warps = tokens * ((d + kWordSpan - 1) / kWordSpan);
+  return std::min<int64_t>((warps + 7) / 8, (int64_t)sm_count() * resident);
 }
 
 bool vectors_ok(const void *base, int64_t pitch, int64_t rows, int es) {
@@ -980,6 +1085,11 @@ extern "C" int oz_dispatch(const oz_rows_args *args, void *stream) {
     const bool wide = vectors_ok(a.x, a.x_row, a.tokens, ES) && vectors_ok(a.rows_out, a.d, a.tokens * a.picks, ES) &&
                       a.d * ES % 16 == 0;
     int64_t blocks;
+    if (!wide && ES == 2 && a.d >= 64) {
+      blocks = word_blocks(a.tokens, a.d, 4);
+      return launch(dispatch_words_kernel, dim3((unsigned)(blocks + kClearBlocks)), 256, 0, st,
+                    "dispatch_words_kernel launch", p, (int)blocks);
+    }
     const Spread at = spread_over(a.d / (wide ? 16 / ES : 1), a.tokens, false, 6, blocks);
     const dim3 grid((unsigned)(blocks + kClearBlocks));
     return wide ? launch(dispatch_kernel<T, 16 / ES>, grid, 256, 0, st, "dispatch_kernel launch", p, at, (int)blocks)
@@ -1003,7 +1113,12 @@ extern "C" int oz_combine(const oz_rows_args *args, void *stream) {
     const bool wide = vectors_ok(a.rows, a.rows_row, a.tokens * a.picks, ES) && vectors_ok(a.x_out, a.d, a.tokens, ES) &&
                       a.d * ES % 16 == 0;
     int64_t blocks;
-    const Spread at = spread_over(a.d / (wide ? 16 / ES : 1), a.tokens, false, a.picks > 4 ? 3 : a.picks > 2 ? 4 : 5, blocks);
+    if constexpr (ES == 2)
+      if (!wide && a.d >= 64) {
+        blocks = word_blocks(a.tokens, a.d, 3);
+        return launch(combine_words_kernel<T>, dim3((unsigned)blocks), 256, 0, st, "combine_words_kernel launch", p);
+      }
+    const Spread at = spread_over(a.d / (wide ? 16 / ES : 1), a.tokens, false, combine_blocks(a.picks <= 6 ? a.picks : 8), blocks);
     auto with = [&](auto k) {
       constexpr int K = decltype(k)::value;
       const dim3 grid((unsigned)blocks);
@@ -1012,6 +1127,7 @@ extern "C" int oz_combine(const oz_rows_args *args, void *stream) {
     };
     if (a.picks <= 2) return with(std::integral_constant<int, 2>{});
     if (a.picks <= 4) return with(std::integral_constant<int, 4>{});
+    if (a.picks <= 6) return with(std::integral_constant<int, 6>{});
     return with(std::integral_constant<int, 8>{});
   });
 }
