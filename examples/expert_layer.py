@@ -3,9 +3,10 @@
     python examples/expert_layer.py
 
 Every token goes to one of the experts (two products with a SiLU between
-them).  Training runs the ragged products forward and backward and updates
-each stack of expert weights with an orthogonalised momentum; serving
-quantises the weights to 4 bits and runs a few tokens at a time.
+them).  Training routes the tokens, runs the ragged products forward and
+backward, clips the gradients by their common norm and updates each stack of
+expert weights with an orthogonalised momentum; serving quantises the weights to
+4 bits and runs a few tokens at a time.
 """
 
 import os
@@ -18,29 +19,17 @@ sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 import ozaki_triton_b200 as oz  # noqa: E402
 
 
-def route(x, router):
-    """Tokens in the order of their experts: (order, row offsets of the groups, gate)."""
-    gate, expert = torch.softmax(x.float() @ router, -1).max(-1)
-    order = torch.argsort(expert, stable=True)
-    counts = torch.bincount(expert, minlength=router.shape[1])
-    offsets = torch.zeros(router.shape[1] + 1, dtype=torch.int64, device=x.device)
-    offsets[1:] = torch.cumsum(counts, 0)
-    return order, offsets, gate
-
-
 def layer(x, router, up, down):
-    order, offsets, gate = route(x, router)
-    hidden = F.silu(oz.grouped_matmul(x[order], up, offsets))
-    rows = oz.grouped_matmul(hidden, down, offsets)
-    return torch.empty_like(rows).index_copy(0, order, rows) * gate[:, None].to(x.dtype)
+    routing = oz.route(x.float() @ router, 1)
+    hidden = F.silu(oz.grouped_matmul(oz.dispatch(x, routing), up, routing.offsets))
+    return oz.combine(oz.grouped_matmul(hidden, down, routing.offsets), routing)
 
 
 def layer_4bit(x, router, up4, down4):
     """The same with weights from quantize_w4."""
-    order, offsets, gate = route(x, router)
-    hidden = F.silu(oz.matmul_w4(x[order], *up4, offsets=offsets))
-    rows = oz.matmul_w4(hidden, *down4, offsets=offsets)
-    return torch.empty_like(rows).index_copy(0, order, rows) * gate[:, None].to(x.dtype)
+    routing = oz.route(x.float() @ router, 1)
+    hidden = F.silu(oz.matmul_w4(oz.dispatch(x, routing), *up4, offsets=routing.offsets))
+    return oz.combine(oz.matmul_w4(hidden, *down4, offsets=routing.offsets), routing)
 
 
 def main(tokens=2048, width=256, hidden=512, experts=8, steps=60, seed=0, dtype=torch.bfloat16, log=print):
@@ -54,6 +43,7 @@ def main(tokens=2048, width=256, hidden=512, experts=8, steps=60, seed=0, dtype=
     target = [normal(experts, width, hidden).to(dtype), normal(experts, hidden, width).to(dtype)]
     weights = [normal(experts, width, hidden), normal(experts, hidden, width)]          # fp32 masters
     momentum = [torch.zeros_like(w) for w in weights]
+    clipped = [torch.empty_like(w) for w in weights]
     losses = []
     for step in range(steps):
         x = torch.randn(tokens, width, generator=g, device="cuda").to(dtype)
@@ -62,9 +52,10 @@ def main(tokens=2048, width=256, hidden=512, experts=8, steps=60, seed=0, dtype=
         used = [w.to(dtype).requires_grad_() for w in weights]
         loss = F.mse_loss(layer(x, router, *used).float(), want.float())
         loss.backward()
+        oz.clip_gradients([u.grad for u in used], 1.0, out=clipped)
         rate = 0.02 * (1 - step / steps)
-        for w, m, u in zip(weights, momentum, used):
-            m.mul_(0.9).add_(u.grad)
+        for w, m, c in zip(weights, momentum, clipped):
+            m.mul_(0.9).add_(c)
             w.sub_(rate * oz.orthogonalize(m))
         losses.append(loss.detach())
         if step % 20 == 0:
