@@ -10,6 +10,7 @@
 // it is multiplied, its sum is not.
 
 #include <algorithm>
+#include <type_traits>
 
 #include "oz_linear.cuh"
 
@@ -21,35 +22,6 @@ using namespace tile;
 using namespace linear;
 
 struct OutTile { int row, column; };
-
-// V values of 8 consecutive columns, as vectors or, up to `count`, one by one.
-template <typename E> __device__ __forceinline__ void load8(const E *from, bool vectors, int count, float (&v)[8]) {
-  if (vectors && count >= 8) {
-    if constexpr (sizeof(E) == 4) {
-      const float4 a = __ldg(reinterpret_cast<const float4 *>(from)), b = __ldg(reinterpret_cast<const float4 *>(from) + 1);
-      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-    } else {
-      stream::unpack<E>(__ldg(reinterpret_cast<const uint4 *>(from)), v);
-    }
-  } else {
-#pragma unroll
-    for (int x = 0; x < 8; ++x) v[x] = x < count ? to_f32(__ldg(from + x)) : 0.f;
-  }
-}
-template <typename E> __device__ __forceinline__ void store8(E *to, bool vectors, int count, const float (&v)[8]) {
-  if (vectors && count >= 8) {
-    if constexpr (sizeof(E) == 4) {
-      reinterpret_cast<float4 *>(to)[0] = make_float4(v[0], v[1], v[2], v[3]);
-      reinterpret_cast<float4 *>(to)[1] = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-      *reinterpret_cast<uint4 *>(to) = stream::pack<E>(v);
-    }
-  } else {
-#pragma unroll
-    for (int x = 0; x < 8; ++x)
-      if (x < count) to[x] = from_f32<E>(v[x]);
-  }
-}
 
 // 8 aligned values of E as they lie in memory.
 template <typename E> struct Run8 {
@@ -65,7 +37,16 @@ template <typename E> struct Run8 {
 #pragma unroll
     for (int x = 0; x < 8; ++x) v[x] = to_f32(e[x]);
   }
-  static __device__ __forceinline__ void store(E *p, const float (&v)[8]) { store8(p, true, 8, v); }
+  static __device__ __forceinline__ void store(E *p, const float (&v)[8]) {
+    constexpr int V = 16 / sizeof(E);
+#pragma unroll
+    for (int h = 0; h < 8 / V; ++h) {
+      float w[V];
+#pragma unroll
+      for (int x = 0; x < V; ++x) w[x] = v[h * V + x];
+      reinterpret_cast<uint4 *>(p)[h] = stream::pack<E>(w);
+    }
+  }
 };
 
 // The columns of a source 16 at a time, the next ones on their way (accumulators in tensor
@@ -93,31 +74,48 @@ template <int N> struct Ahead16<Registers<N>> {
 // 16 bytes each, next to the neighbouring lane's.  Accumulators, bias and residual of the next
 // columns are on their way meanwhile.  (A lane's own row instead, with the bias and the
 // residual read element by element, took 8192 x 8192 results of 4096 terms from 338 us to
-// 365 and 549.)
+// 365 and 549.)  For rows of a multiple of 8 columns on 16-byte boundaries.
 template <typename O, typename B, int COLS, int UNROLL, class Source>
-__device__ __forceinline__ void finish_rows(const Params &p, const Source &source, unsigned char *mine, int64_t r0,
-                                            int64_t c0) {
+__device__ __forceinline__ void finish_vectors(const Params &p, const Source &source, unsigned char *mine, int64_t r0,
+                                               int64_t c0) {
+  using Out = Run8<O>;
+  using In = Run8<B>;
   const int lane = threadIdx.x % 32, half = lane % 2;
   const int rows = (int)min(p.rows - r0, (int64_t)32), columns = (int)min(p.n - c0, (int64_t)COLS);
   if (rows <= 0 || columns <= 0) return;
   const int64_t at = (r0 + lane / 2) * p.ld + c0 + half * 8, next_row = 16 * p.ld;
-  const int64_t residual_row = 16 * p.residual_ld;
   O *out = static_cast<O *>(p.out) + at;
   B *pre = p.pre ? static_cast<B *>(p.pre) + at : nullptr;
   const O *residual = p.residual ? static_cast<const O *>(p.residual) + (r0 + lane / 2) * p.residual_ld + c0 + half * 8
                                  : nullptr;
+  const int64_t residual_row = 16 * p.residual_ld;
   const B *bias = p.bias && !p.bias_f32 ? static_cast<const B *>(p.bias) + c0 + half * 8 : nullptr;
   const float *bias_f32 = p.bias && p.bias_f32 ? static_cast<const float *>(p.bias) + c0 + half * 8 : nullptr;
-  const int act = p.act;
+  const int act = p.act, mine_end = columns - half * 8;            // this lane's columns: c < mine_end
+  const bool one = lane / 2 < rows, two = 16 + lane / 2 < rows;
+  typename In::Raw b{};
+  typename Run8<float>::Raw b32{};
+  typename Out::Raw r[2]{};
+  auto fetch = [&](int c) {
+    if (c >= mine_end) return;
+    if (bias) b = In::load(bias + c);
+    if (bias_f32) b32 = Run8<float>::load(bias_f32 + c);
+    if (residual) {
+      if (one) r[0] = Out::load(residual + c);
+      if (two) r[1] = Out::load(residual + c + residual_row);
+    }
+  };
   Ahead16<Source> ahead{source};
   ahead.start(0);
-  // this lane's part of 16 columns' accumulators, through the staging
-  auto turn = [&](int c, bool more, float (&u)[2][8]) {
-    float v[16];
+  fetch(0);
+#pragma unroll(UNROLL)
+  for (int c = 0; c < COLS; c += 16) {
+    if (c >= columns) continue;
+    float v[16], u[2][8], add[8];
     ahead.finish(v);
 #pragma unroll
     for (int x = 0; x < 4; ++x) *staged(mine, lane, x) = *reinterpret_cast<uint4 *>(&v[x * 4]);
-    if (more) ahead.start(c + 16);
+    if (c + 16 < columns) ahead.start(c + 16);
     __syncwarp();
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -129,90 +127,84 @@ __device__ __forceinline__ void finish_rows(const Params &p, const Source &sourc
         for (int x = 0; x < 4; ++x) u[i][h * 4 + x] = f[x];
       }
     __syncwarp();
-  };
-  constexpr int kAll = kVectors | kResidualVectors | kBiasVectors;
-  if (rows == 32 && columns == COLS && (p.vectors & kAll) == kAll) {
-    using Out = Run8<O>;
-    using In = Run8<B>;
-    typename In::Raw b{};
-    typename Out::Raw r[2]{};
-    float4 b32[2]{};
-    auto fetch = [&](int c) {
-      if (bias) b = In::load(bias + c);
-      if (bias_f32) {
-        b32[0] = __ldg(reinterpret_cast<const float4 *>(bias_f32 + c));
-        b32[1] = __ldg(reinterpret_cast<const float4 *>(bias_f32 + c) + 1);
-      }
-      if (residual) {
-        r[0] = Out::load(residual + c);
-        r[1] = Out::load(residual + c + residual_row);
-      }
-    };
-    fetch(0);
-#pragma unroll(UNROLL)
-    for (int c = 0; c < COLS; c += 16) {
-      float u[2][8], add[8];
-      turn(c, c + 16 < COLS, u);
-      if (bias || bias_f32) {
-        if (bias) In::values(b, add);
-        else add[0] = b32[0].x, add[1] = b32[0].y, add[2] = b32[0].z, add[3] = b32[0].w, add[4] = b32[1].x,
-             add[5] = b32[1].y, add[6] = b32[1].z, add[7] = b32[1].w;
-#pragma unroll
-        for (int x = 0; x < 8; ++x) u[0][x] += add[x], u[1][x] += add[x];
-      }
-      if (pre) {
-        In::store(pre + c, u[0]);
-        In::store(pre + c + next_row, u[1]);
-      }
-      if (act) {
-        activate(u[0], act);
-        activate(u[1], act);
-      }
-      if (residual)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          Out::values(r[i], add);
-#pragma unroll
-          for (int x = 0; x < 8; ++x) u[i][x] += add[x];
-        }
-      if (c + 16 < COLS) fetch(c + 16);
-      Out::store(out + c, u[0]);
-      Out::store(out + c + next_row, u[1]);
-    }
-    return;
-  }
-  // the edges, and rows or a bias off the 16-byte boundaries
-#pragma unroll(UNROLL)
-  for (int c = 0; c < COLS; c += 16) {
-    if (c >= columns) continue;
-    const int count = (int)min(p.n - c0 - c - half * 8, (int64_t)8);
-    float u[2][8], add[8];
-    turn(c, c + 16 < columns, u);
     if (bias || bias_f32) {
-      if (bias) load8(bias + c, p.vectors & kBiasVectors, count, add);
-      else load8(bias_f32 + c, p.vectors & kBiasVectors, count, add);
+      if (bias) In::values(b, add);
+      else Run8<float>::values(b32, add);
 #pragma unroll
       for (int x = 0; x < 8; ++x) u[0][x] += add[x], u[1][x] += add[x];
     }
+    const bool there = c < mine_end;
+    if (pre) {
+      if (there && one) In::store(pre + c, u[0]);
+      if (there && two) In::store(pre + c + next_row, u[1]);
+    }
+    if (act) {
+      activate(u[0], act);
+      activate(u[1], act);
+    }
+    if (residual)
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      if (i * 16 + lane / 2 >= rows) continue;
-      if (pre) store8(pre + c + i * next_row, p.vectors & kVectors, count, u[i]);
-      activate(u[i], act);
-      if (residual) {
-        load8(residual + c + i * residual_row, p.vectors & kResidualVectors, count, add);
+      for (int i = 0; i < 2; ++i) {
+        Out::values(r[i], add);
 #pragma unroll
         for (int x = 0; x < 8; ++x) u[i][x] += add[x];
       }
-      store8(out + c + i * next_row, p.vectors & kVectors, count, u[i]);
-    }
+    fetch(c + 16);
+    if (there && one) Out::store(out + c, u[0]);
+    if (there && two) Out::store(out + c + next_row, u[1]);
   }
 }
 
+// The same for any rows, element by element: a lane has one column of every other row, so an
+// instruction touches 2 rows of 16 columns.
+template <typename O, typename B, int COLS, int UNROLL, class Source>
+__device__ __forceinline__ void finish_elements(const Params &p, const Source &source, unsigned char *mine, int64_t r0,
+                                                int64_t c0) {
+  const int lane = threadIdx.x % 32, side = lane / 16, in = lane % 16;
+  const int rows = (int)min(p.rows - r0, (int64_t)32), columns = (int)min(p.n - c0, (int64_t)COLS);
+  if (rows <= 0 || columns <= 0) return;
+  const int64_t at = (r0 + side) * p.ld + c0 + in, residual_at = (r0 + side) * p.residual_ld + c0 + in;
+  Ahead16<Source> ahead{source};
+  ahead.start(0);
+#pragma unroll(UNROLL)
+  for (int c = 0; c < COLS; c += 16) {
+    if (c >= columns) continue;
+    const bool there = c + in < columns;
+    O r[16];
+    if (p.residual)
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (there && 2 * i + side < rows)
+          r[i] = static_cast<const O *>(p.residual)[residual_at + c + 2 * i * p.residual_ld];
+    const float bias = p.bias && there ? bias_at<B>(p, c0 + c + in) : 0.f;
+    float v[16], u[16];
+    ahead.finish(v);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) *staged(mine, lane, x) = *reinterpret_cast<uint4 *>(&v[x * 4]);
+    if (c + 16 < columns) ahead.start(c + 16);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      u[i] = reinterpret_cast<const float *>(staged(mine, 2 * i + side, in / 4))[in % 4] + bias;
+    __syncwarp();
+    if (p.pre)
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (there && 2 * i + side < rows) static_cast<B *>(p.pre)[at + c + 2 * i * p.ld] = from_f32<B>(u[i]);
+    activate(u, p.act);
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (there && 2 * i + side < rows)
+        static_cast<O *>(p.out)[at + c + 2 * i * p.ld] = from_f32<O>(p.residual ? u[i] + to_f32(r[i]) : u[i]);
+  }
+}
+
+// What follows a product: nothing, or bias, activation and residual by vectors or by elements.
+enum Form { kPlain, kByVectors, kByElements };
 // What follows a product keeps 16 epilogue warps busy (a plain one's 8 wait for its stores;
 // the sums of passes of an fp32 result leave no registers for 16).
-template <typename O, typename B, int PAIR_, int NT_, bool AMN_, bool BMN_, bool PLAIN> struct LinearJob : NoLookAhead {
-  static constexpr int EPILOGUE_WARPS = PLAIN || NT_ < 256 || sizeof(O) == 4 ? 8 : 16;
+template <typename O, typename B, int PAIR_, int NT_, bool AMN_, bool BMN_, int FORM> struct LinearJob : NoLookAhead {
+  static constexpr int EPILOGUE_WARPS = FORM == kPlain || NT_ < 256 || sizeof(O) == 4 ? 8 : 16;
   static constexpr int PAIR = PAIR_, NT = NT_, PLANES = 1, PASS = sizeof(O) == 4 ? 8 : 0;
   static constexpr bool AMN = AMN_, BMN = BMN_, RAGGED = false;
   using Params = linear::Params;
@@ -240,10 +232,12 @@ template <typename O, typename B, int PAIR_, int NT_, bool AMN_, bool BMN_, bool
     const int64_t r0 = t.extra.row + row, c0 = t.extra.column + column;
     const int rows = (int)(p.rows - r0);
     O *out = static_cast<O *>(p.out) + r0 * p.ld + c0;
-    if constexpr (PLAIN) {
+    if constexpr (FORM == kPlain) {
       write_rows<O, NT / 2>(source, mine, out, p.ld, rows, p.n - c0, p.vectors & kVectors);
     } else {
-      finish_rows<O, B, NT * 4 / EPILOGUE_WARPS, PASS ? NT / 2 : 1>(p, source, mine, r0, c0);
+      constexpr int COLS = NT * 4 / EPILOGUE_WARPS, UNROLL = PASS ? COLS : 1;
+      if constexpr (FORM == kByVectors) finish_vectors<O, B, COLS, UNROLL>(p, source, mine, r0, c0);
+      else finish_elements<O, B, COLS, UNROLL>(p, source, mine, r0, c0);
     }
   }
   static __device__ void finish(const Params &, int, int) {}
@@ -264,19 +258,19 @@ int run_job(const Side &a, const Side &b, Params p, cudaStream_t st, const char 
   return launch<J>(ta, tb, p, rows * columns, st, what);
 }
 
-template <typename O, typename B, bool PLAIN>
+template <typename O, typename B, int FORM>
 int product(bool pair, const Side &a, const Side &b, const Params &p, cudaStream_t st, const char *what) {
   if (a.mn) {
-    if constexpr (PLAIN)
-      return pair ? run_job<LinearJob<O, B, 2, 256, true, true, true>>(a, b, p, st, what)
-                  : run_job<LinearJob<O, B, 1, 128, true, true, true>>(a, b, p, st, what);
+    if constexpr (FORM == kPlain)
+      return pair ? run_job<LinearJob<O, B, 2, 256, true, true, kPlain>>(a, b, p, st, what)
+                  : run_job<LinearJob<O, B, 1, 128, true, true, kPlain>>(a, b, p, st, what);
     return set_error(OZ_ERR_UNSUPPORTED, "operand layout");
   }
   if (b.mn)
-    return pair ? run_job<LinearJob<O, B, 2, 256, false, true, PLAIN>>(a, b, p, st, what)
-                : run_job<LinearJob<O, B, 1, 128, false, true, PLAIN>>(a, b, p, st, what);
-  return pair ? run_job<LinearJob<O, B, 2, 256, false, false, PLAIN>>(a, b, p, st, what)
-              : run_job<LinearJob<O, B, 1, 128, false, false, PLAIN>>(a, b, p, st, what);
+    return pair ? run_job<LinearJob<O, B, 2, 256, false, true, FORM>>(a, b, p, st, what)
+                : run_job<LinearJob<O, B, 1, 128, false, true, FORM>>(a, b, p, st, what);
+  return pair ? run_job<LinearJob<O, B, 2, 256, false, false, FORM>>(a, b, p, st, what)
+              : run_job<LinearJob<O, B, 1, 128, false, false, FORM>>(a, b, p, st, what);
 }
 
 // How a product is divided, by the least estimated time (us, one B200, fitted to 690
@@ -314,16 +308,26 @@ Plan plan_product(int64_t rows, int64_t k, int64_t n, bool rows_mn) {
   return plan;
 }
 
-template <bool PLAIN>
+template <int FORM>
+int product_in(bool pair, int dtype, int out_dtype, const Side &a, const Side &b, const Params &p, cudaStream_t st,
+               const char *what) {
+  if (dtype == OZ_F16)
+    return out_dtype == OZ_F32 ? product<float, __half, FORM>(pair, a, b, p, st, what)
+                               : product<__half, __half, FORM>(pair, a, b, p, st, what);
+  return out_dtype == OZ_F32 ? product<float, __nv_bfloat16, FORM>(pair, a, b, p, st, what)
+                             : product<__nv_bfloat16, __nv_bfloat16, FORM>(pair, a, b, p, st, what);
+}
+
 int product_of(int dtype, int out_dtype, const Side &a, const Side &b, const Params &p, cudaStream_t st,
                const char *what) {
   const Plan plan = plan_product(p.rows, p.k, p.n, a.mn);
   if (plan.split.tile_rows) return split_product(plan.split, dtype, out_dtype, a, b, p, st, what);
-  if (dtype == OZ_F16)
-    return out_dtype == OZ_F32 ? product<float, __half, PLAIN>(plan.pair, a, b, p, st, what)
-                               : product<__half, __half, PLAIN>(plan.pair, a, b, p, st, what);
-  return out_dtype == OZ_F32 ? product<float, __nv_bfloat16, PLAIN>(plan.pair, a, b, p, st, what)
-                             : product<__nv_bfloat16, __nv_bfloat16, PLAIN>(plan.pair, a, b, p, st, what);
+  if (!p.bias && !p.act && !p.residual && !p.pre)
+    return product_in<kPlain>(plan.pair, dtype, out_dtype, a, b, p, st, what);
+  constexpr int kAll = kVectors | kResidualVectors | kBiasVectors;
+  if ((p.vectors & kAll) == kAll && p.n % 8 == 0)
+    return product_in<kByVectors>(plan.pair, dtype, out_dtype, a, b, p, st, what);
+  return product_in<kByElements>(plan.pair, dtype, out_dtype, a, b, p, st, what);
 }
 
 // ---------------------------------------------------------------------------
@@ -377,7 +381,14 @@ template <typename T, int V> __global__ void __launch_bounds__(256, 5) slope_ker
         R::values(a[q], v);
         if (p.pre) {
           R::values(b[q], u);
-          times_slope(v, u, p.act);
+          if constexpr (V == 1) {
+            float v2[2] = {v[0], v[0]};
+            const float u2[2] = {u[0], u[0]};
+            times_slope(v2, u2, p.act);
+            v[0] = v2[0];
+          } else {
+            times_slope(v, u, p.act);
+          }
           stream::Run<T, V>::store(du + at * p.du_sr, v);
         }
 #pragma unroll
@@ -452,7 +463,7 @@ template <typename O, typename B> __global__ void __launch_bounds__(256) empty_k
     const int64_t r = i / p.n, c = i - r * p.n;
     const float u = p.bias ? bias_at<B>(p, c) : 0.f;
     if (p.pre) static_cast<B *>(p.pre)[r * p.ld + c] = from_f32<B>(u);
-    float v[1] = {u};
+    float v[2] = {u, u};
     activate(v, p.act);
     float y = v[0];
     if (p.residual) y += to_f32(static_cast<const O *>(p.residual)[r * p.residual_ld + c]);
@@ -496,10 +507,7 @@ extern "C" int oz_linear(const oz_linear_args *args, void *stream) {
   Operand ops[2] = {{a.x, a.rows, a.x_sr, 1, 0, (int)a.k},
                     {a.w, across ? a.k : a.n, across ? a.w_sk : a.w_sn, 1, 0, (int)(across ? a.n : a.k)}};
   if (int rc = lay_out(ops, 2, a.workspace, a.workspace_bytes, st)) return rc;
-  if (!a.bias && !a.act && !a.residual && !a.pre)
-    return product_of<true>(a.dtype, a.out_dtype, Side{ops[0].p, ops[0].row, false}, Side{ops[1].p, ops[1].row, across},
-                            p, st, "product launch");
-  return product_of<false>(a.dtype, a.out_dtype, Side{ops[0].p, ops[0].row, false}, Side{ops[1].p, ops[1].row, across}, p,
+  return product_of(a.dtype, a.out_dtype, Side{ops[0].p, ops[0].row, false}, Side{ops[1].p, ops[1].row, across}, p,
                            st, "product launch");
 }
 
@@ -583,14 +591,14 @@ extern "C" int oz_linear_backward(const oz_linear_backward_args *args, void *str
     // dx (rows, k) = du (rows, n) w^T: w's rows along n where it is stored across
     Params p{a.dx, nullptr, nullptr, nullptr, a.k, 0, (int)a.rows, (int)a.n, (int)a.k, 0, 0,
                    (uintptr_t)a.dx % 16 == 0 && a.k % 8 == 0, 0, OZ_ACT_NONE, tile::instruction(a.dtype)};
-    if (int rc = product_of<true>(a.dtype, a.dtype, Side{ops[0].p, ops[0].row, false},
+    if (int rc = product_of(a.dtype, a.dtype, Side{ops[0].p, ops[0].row, false},
                                   Side{ops[at_w].p, ops[at_w].row, !across}, p, st, "dx launch"))
       return rc;
   }
   if (want_w) {
     Params p{a.dw, nullptr, nullptr, nullptr, a.n, 0, (int)a.k, (int)a.rows, (int)a.n, 0, 0,
                    (uintptr_t)a.dw % 16 == 0 && a.n * dw_size % 16 == 0, 0, OZ_ACT_NONE, tile::instruction(a.dtype)};
-    return product_of<true>(a.dtype, a.dw_dtype, Side{ops[at_x].p, ops[at_x].row, true},
+    return product_of(a.dtype, a.dw_dtype, Side{ops[at_x].p, ops[at_x].row, true},
                             Side{ops[0].p, ops[0].row, true}, p, st, "dw launch");
   }
   return OZ_OK;

@@ -243,6 +243,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
       }
     }
   }
+  __syncwarp();                                // lane 0 of the first two warps comes from its loop
   if (splits > 1) cluster_sync();
   else __syncthreads();
   if (warp >= 2) {

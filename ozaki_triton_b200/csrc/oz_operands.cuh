@@ -2,6 +2,7 @@
 // read them: where their rows do not start on 16-byte boundaries they are copied first.
 #pragma once
 
+#include "oz_stream.cuh"
 #include "oz_tile.cuh"
 
 namespace oz {
@@ -38,6 +39,7 @@ constexpr int kPart = 2048;
 
 __global__ void __launch_bounds__(256, 6) repitch_kernel(const __grid_constant__ RepitchAll all_jobs) {
   const Repitch &p = all_jobs.job[blockIdx.y];
+  stream::start_after_earlier_kernels();
   const int lane = threadIdx.x % 32;
   const uint64_t all = (uint64_t)p.lines * p.parts;
   for (uint64_t v = (uint64_t)blockIdx.x * 8 + threadIdx.x / 32; v < all; v += (uint64_t)gridDim.x * 8) {
@@ -108,9 +110,8 @@ inline int lay_out(Operand *ops, int count, void *workspace, int64_t workspace_b
     most = max(most, (o.rows * o.mats * parts + 7) / 8);
   }
   if (!n) return OZ_OK;
-  count_launch();
-  repitch_kernel<<<dim3((unsigned)min(most, (int64_t)sm_count() * 16), n), 256, 0, st>>>(all);
-  return check_cuda(cudaGetLastError(), "repitch_kernel launch");
+  return stream::launch(repitch_kernel, dim3((unsigned)min(most, (int64_t)tile::sm_count() * 16), n), 256, 0, st,
+                        "repitch_kernel launch", all);
 }
 
 }  // namespace

@@ -186,7 +186,8 @@ def fused_matmul(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] 
 
     Differentiable in x, w, bias and residual (once; second derivatives and
     forward-mode derivatives are refused).  With an activation the forward pass
-    then keeps u = x @ w + bias, rounded to the operands' dtype.  With
+    then keeps u = x @ w + bias, rounded to the operands' dtype; the gradient of an
+    fp32 result is rounded to that dtype before anything else.  With
     ``return_pre`` the result is (y, u), u None without an activation, for
     ``fused_matmul_backward``; no gradient is recorded.
     """

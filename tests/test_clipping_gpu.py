@@ -76,6 +76,7 @@ def test_special_values():
     zero = [torch.zeros(100, device=DEV), torch.zeros(3, device=DEV).bfloat16()]
     assert check(zero, 1.0).item() == 0
     assert oz.clip_gradients(zero, 1.0, eps=0.0).item() == 0 and not zero[0].any()
+    assert oz.clip_gradients([torch.empty(0, device=DEV)], 1.0).item() == 0
     for value in (float("inf"), float("nan")):
         grads = [torch.ones(1000, device=DEV), torch.ones(10, device=DEV)]
         grads[0][77] = value
