@@ -346,7 +346,7 @@ constexpr int kSlopeRows = 8;  // rows of a block's pass, a warp each
 
 // 32 lanes take 32 V columns of a row; a warp's next two rows are on their way while it
 // works on the two before.
-template <typename T, int V> __global__ void __launch_bounds__(256, 5) slope_kernel(const SlopeParams p) {
+template <typename T, int V> __global__ void __launch_bounds__(256, 4) slope_kernel(const SlopeParams p) {
   constexpr int AT_ONCE = 2;
   using R = stream::Raw<T, V>;
   __shared__ float part[kSlopeRows][32 * V];
@@ -436,7 +436,7 @@ int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
 // Rows of a block of slope_kernel: as many blocks as the GPU holds at once.
 int slope_rows(int64_t rows, int n) {
   const int64_t columns = (n + 255) / 256;
-  const int64_t want = std::max<int64_t>(1, stream::sm_count() * 5 / columns);
+  const int64_t want = std::max<int64_t>(1, stream::sm_count() * 4 / columns);
   const int64_t per = std::max<int64_t>(64, (rows + want - 1) / want);
   return (int)((per + 15) / 16 * 16);
 }
