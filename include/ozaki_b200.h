@@ -351,7 +351,9 @@ int oz_orthogonalize(const void *g, int dtype, int64_t batch, int64_t m, int64_t
  *   residual : (rows, n) of y's type, unit stride along n, row pitch residual_sr, or NULL
  *   y        : contiguous (rows, n) of x's type or fp32 (out_dtype)
  *   pre      : contiguous (rows, n) of x's type for u, or NULL
- *   workspace: as in oz_grouped_matmul, for copies of operands off the 16-byte boundaries
+ *   workspace: oz_linear_workspace_bytes() bytes for these arguments (copies of operands off the
+ *              16-byte boundaries that cannot be read as they are), 256-byte aligned; may be 0
+ *              bytes and NULL
  */
 enum oz_activation { OZ_ACT_NONE = 0, OZ_ACT_RELU = 1, OZ_ACT_GELU = 2, OZ_ACT_SILU = 3 };
 typedef struct {
@@ -360,6 +362,7 @@ typedef struct {
   int64_t rows, k, n, x_sr, w_sk, w_sn, residual_sr, workspace_bytes;
   int32_t dtype, out_dtype, bias_dtype, act;
 } oz_linear_args;
+int64_t oz_linear_workspace_bytes(const oz_linear_args *args);
 int oz_linear(const oz_linear_args *args, void *stream);
 
 /*

@@ -88,6 +88,7 @@ SIGNATURES = {
     "oz_orthogonalize_workspace_bytes": (_i64, [_int, _i64, _i64, _i64, _i32, _i32]),
     "oz_orthogonalize": (_int, [_vp, _int, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _vp,
                                 ctypes.c_double, _i32, _vp, _vp, _i64, _vp]),
+    "oz_linear_workspace_bytes": (_i64, [ctypes.POINTER(LinearArgs)]),
     "oz_linear": (_int, [ctypes.POINTER(LinearArgs), _vp]),
     "oz_linear_backward_workspace_bytes": (_i64, [_i64, _i64, _i32, _i32]),
     "oz_linear_backward": (_int, [ctypes.POINTER(LinearBackwardArgs), _vp]),

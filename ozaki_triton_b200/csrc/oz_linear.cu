@@ -287,11 +287,12 @@ int product(bool pair, const Side &a, const Side &b, const Params &p, cudaStream
 struct Plan {
   bool pair;                   // the engine's tiles: 256 x 256 by pairs of CTAs, or 128 x 128
   SplitPlan split;             // of 0 rows: the engine
+  bool loose;                  // operands off the 16-byte boundaries are read as they are
 };
 Plan plan_product(int64_t rows, int64_t k, int64_t n, bool rows_mn) {
   const int64_t sms = tile::sm_count(), blocks = (k + kBlock - 1) / kBlock;
   auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
-  Plan plan{false, {0, 1}};
+  Plan plan{false, {0, 1}, false};
   double best = 3.3 + up(up(rows, 128) * up(n, 128), sms) * (0.32 * blocks + 0.9);
   const double pairs = 3.6 + up(up(rows, 256) * up(n, 256) * 2, sms) * (0.347 * blocks + 1.9);
   if (pairs < best) plan.pair = true, best = pairs;
@@ -318,9 +319,8 @@ int product_in(bool pair, int dtype, int out_dtype, const Side &a, const Side &b
                              : product<__nv_bfloat16, __nv_bfloat16, FORM>(pair, a, b, p, st, what);
 }
 
-int product_of(int dtype, int out_dtype, const Side &a, const Side &b, const Params &p, cudaStream_t st,
+int product_of(const Plan &plan, int dtype, int out_dtype, const Side &a, const Side &b, const Params &p, cudaStream_t st,
                const char *what) {
-  const Plan plan = plan_product(p.rows, p.k, p.n, a.mn);
   if (plan.split.tile_rows) return split_product(plan.split, dtype, out_dtype, a, b, p, st, what);
   if (!p.bias && !p.act && !p.residual && !p.pre)
     return product_in<kPlain>(plan.pair, dtype, out_dtype, a, b, p, st, what);
@@ -455,6 +455,37 @@ int check_linear(int dtype, int out_dtype, int act, int64_t rows, int64_t k, int
 // A weight (k, n) as an operand: stored across its rows' dimension or along it.
 bool stored_across(int64_t n, int64_t w_sk, int64_t w_sn) { return w_sn == 1 || (n == 1 && w_sk != 1); }
 
+// The operands x and w of a product and how it is divided.  Small products read operands off
+// the 16-byte boundaries as they are where a CTA has few pieces of 64 lines of them: 0.75 us
+// each, 1.1 where two CTAs share an SM (67 x 1000 x 1407, 4 pieces: 9.7 us; 300 x 2047 x 515, 12:
+// 20 us).  A copy first takes 11 and 12 us on the device, and 4.4 us more of the host, which
+// is what counts up to 13 us.  Not where fp32 results take their sums in passes: the warps that
+// would load are busy with those.
+Plan linear_operands(const oz_linear_args &a, bool across, Operand (&ops)[2]) {
+  ops[0] = Operand{a.x, a.rows, a.x_sr, 1, 0, (int)a.k};
+  ops[1] = Operand{a.w, across ? a.k : a.n, across ? a.w_sk : a.w_sn, 1, 0, (int)(across ? a.n : a.k)};
+  const Plan whole = plan_product(a.rows, a.k, a.n, false);
+  const bool loose_x = copy_bytes(ops[0]) != 0, loose_w = copy_bytes(ops[1]) != 0;
+  if (!loose_x && !loose_w) return whole;
+  const int64_t sms = tile::sm_count(), blocks = (a.k + kBlock - 1) / kBlock;
+  auto up = [](int64_t v, int64_t by) { return (v + by - 1) / by; };
+  Plan plan{false, {0, 1}, true};
+  double best = 10.5;
+  for (int shape = 0; shape < 3; ++shape) {
+    const int tile_rows = shape == 0 ? 16 : shape == 1 ? 64 : 128;
+    const double end = shape == 0 ? 3.2 : shape == 1 ? 4.5 : 5.8;
+    const int64_t tiles = up(a.rows, tile_rows) * up(a.n, 128);
+    for (int splits = 1; splits <= kMostSplits && splits <= blocks; splits *= 2) {
+      const int64_t pieces = up(blocks, splits) * ((loose_w ? 2 : 0) + (loose_x ? up(tile_rows, 64) : 0));
+      if (a.out_dtype == OZ_F32 && up(blocks, splits) > 8) continue;
+      const double time = up(tiles * splits, 2 * sms) * (end + pieces * (tiles * splits > sms ? 1.1 : 0.75)) +
+                          (splits > 1 ? 0.7 : 0.0);
+      if (time < best) plan.split = SplitPlan{tile_rows, splits}, best = time;
+    }
+  }
+  return plan.split.tile_rows ? plan : whole;
+}
+
 // y of an empty contraction: the epilogue on zeros.
 template <typename O, typename B> __global__ void __launch_bounds__(256) empty_kernel(const Params p) {
   stream::start_after_earlier_kernels();
@@ -473,6 +504,17 @@ template <typename O, typename B> __global__ void __launch_bounds__(256) empty_k
 
 }  // namespace
 }  // namespace oz
+
+extern "C" int64_t oz_linear_workspace_bytes(const oz_linear_args *args) {
+  using namespace oz;
+  if (!args) return OZ_ERR_INVALID;
+  const oz_linear_args &a = *args;
+  if (check_linear(a.dtype, a.out_dtype, a.act, a.rows, a.k, a.n)) return OZ_ERR_INVALID;
+  if (a.rows == 0 || a.n == 0 || a.k == 0) return 0;
+  Operand ops[2];
+  if (linear_operands(a, stored_across(a.n, a.w_sk, a.w_sn), ops).loose) return 0;
+  return copy_bytes(ops[0]) + copy_bytes(ops[1]);
+}
 
 extern "C" int oz_linear(const oz_linear_args *args, void *stream) {
   if (!args) return oz::set_error(OZ_ERR_INVALID, "null arguments");
@@ -504,10 +546,13 @@ extern "C" int oz_linear(const oz_linear_args *args, void *stream) {
   if (!a.x || !a.w) return set_error(OZ_ERR_INVALID, "null pointer");
   const bool across = stored_across(a.n, a.w_sk, a.w_sn);
   if (!across && a.w_sk != 1 && a.k != 1) return set_error(OZ_ERR_INVALID, "w must have a unit stride along k or n");
-  Operand ops[2] = {{a.x, a.rows, a.x_sr, 1, 0, (int)a.k},
-                    {a.w, across ? a.k : a.n, across ? a.w_sk : a.w_sn, 1, 0, (int)(across ? a.n : a.k)}};
-  if (int rc = lay_out(ops, 2, a.workspace, a.workspace_bytes, st)) return rc;
-  return product_of(a.dtype, a.out_dtype, Side{ops[0].p, ops[0].row, false}, Side{ops[1].p, ops[1].row, across}, p,
+  Operand ops[2];
+  const Plan plan = linear_operands(a, across, ops);
+  if ((uintptr_t)a.x % 2 != 0 || (uintptr_t)a.w % 2 != 0)
+    return set_error(OZ_ERR_INVALID, "an operand is not aligned to its elements");
+  if (!plan.loose)
+    if (int rc = lay_out(ops, 2, a.workspace, a.workspace_bytes, st)) return rc;
+  return product_of(plan, a.dtype, a.out_dtype, Side{ops[0].p, ops[0].row, false}, Side{ops[1].p, ops[1].row, across}, p,
                            st, "product launch");
 }
 
@@ -591,14 +636,14 @@ extern "C" int oz_linear_backward(const oz_linear_backward_args *args, void *str
     // dx (rows, k) = du (rows, n) w^T: w's rows along n where it is stored across
     Params p{a.dx, nullptr, nullptr, nullptr, a.k, 0, (int)a.rows, (int)a.n, (int)a.k, 0, 0,
                    (uintptr_t)a.dx % 16 == 0 && a.k % 8 == 0, 0, OZ_ACT_NONE, tile::instruction(a.dtype)};
-    if (int rc = product_of(a.dtype, a.dtype, Side{ops[0].p, ops[0].row, false},
+    if (int rc = product_of(plan_product(a.rows, a.n, a.k, false), a.dtype, a.dtype, Side{ops[0].p, ops[0].row, false},
                                   Side{ops[at_w].p, ops[at_w].row, !across}, p, st, "dx launch"))
       return rc;
   }
   if (want_w) {
     Params p{a.dw, nullptr, nullptr, nullptr, a.n, 0, (int)a.k, (int)a.rows, (int)a.n, 0, 0,
                    (uintptr_t)a.dw % 16 == 0 && a.n * dw_size % 16 == 0, 0, OZ_ACT_NONE, tile::instruction(a.dtype)};
-    return product_of(a.dtype, a.dw_dtype, Side{ops[at_x].p, ops[at_x].row, true},
+    return product_of(plan_product(a.k, a.rows, a.n, true), a.dtype, a.dw_dtype, Side{ops[at_x].p, ops[at_x].row, true},
                             Side{ops[0].p, ops[0].row, true}, p, st, "dw launch");
   }
   return OZ_OK;

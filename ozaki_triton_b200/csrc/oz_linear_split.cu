@@ -13,6 +13,7 @@
 // the other's loads.
 
 #include <algorithm>
+#include <cstring>
 
 #include "oz_linear.cuh"
 
@@ -77,11 +78,56 @@ template <typename E> __device__ __forceinline__ void store4(E *to, bool vectors
   }
 }
 
+// An operand off the 16-byte boundaries: the copy unit cannot read it, so the warps that
+// finish the tile load it meanwhile.  A tile is lines of 64 elements, along the contraction or across it; a thread
+// makes 16 bytes of a line from the one or two aligned 16 bytes that hold them (which share
+// their 16 bytes with an element, so they can be read).
+struct Loose {
+  const void *p;               // none: the copy unit's
+  int64_t pitch;
+  int inner, outer;            // extents along a row and across
+};
+struct LooseTwo { Loose a, b; };
+
+struct Piece {
+  uint4 low, high;
+  int shift, count;            // bytes into `low`; elements
+  // elements [at, at + 8) of row `row`, as far as there are
+  __device__ __forceinline__ void load(const Loose &o, int64_t row, int at) {
+    count = row < o.outer ? min(max(o.inner - at, 0), 8) : 0;
+    low = high = make_uint4(0, 0, 0, 0);
+    shift = 0;
+    if (count == 0) return;
+    const uintptr_t from = (uintptr_t)o.p + 2 * (uintptr_t)(row * o.pitch + at);
+    shift = (int)(from & 15);
+    const uint4 *v = reinterpret_cast<const uint4 *>(from - shift);
+    low = __ldg(v);
+    if (shift + 2 * count > 16) high = __ldg(v + 1);
+  }
+  __device__ __forceinline__ uint4 value() const {
+    uint32_t w[8] = {low.x, low.y, low.z, low.w, high.x, high.y, high.z, high.w};
+    if (shift & 8)
+#pragma unroll
+      for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+    if (shift & 4)
+#pragma unroll
+      for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+    uint32_t out[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      out[i] = shift & 2 ? __funnelshift_r(w[i], w[i + 1], 16) : w[i];
+      const int left = count - 2 * i;
+      if (left < 2) out[i] = left == 1 ? out[i] & 0xFFFFu : 0u;
+    }
+    return make_uint4(out[0], out[1], out[2], out[3]);
+  }
+};
+
 // A: 128 columns of the result, B: NT rows.  O: the result's type, T: the operands'.
 template <typename O, typename T, int NT, bool AMN, bool BMN>
 __global__ void __launch_bounds__(kSplitThreads, 2)
     split_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const Params p,
-                 const int splits) {
+                 const __grid_constant__ LooseTwo loose, const int splits) {
   constexpr int S = split_stages<NT>(), SB = split_stage<NT>(), A_BYTES = kRows * kLine;
   constexpr int PASS = sizeof(O) == 4 ? kPassBlocks : 1 << 28;
   constexpr int kTmemColumns = 2 * NT < 32 ? 32 : 2 * NT;
@@ -108,7 +154,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < S; ++i) {
-      mbar_init(&full[i], 1);
+      mbar_init(&full[i], loose.a.p || loose.b.p ? 1 + kFinishWarps : 1);
       mbar_init(&empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -118,8 +164,8 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
     mbar_init(drain, 1);
     *abort_flag = 0;
     fence_mbar_init();
-    prefetch_tmap(&tm_a);
-    prefetch_tmap(&tm_b);
+    if (!loose.a.p) prefetch_tmap(&tm_a);
+    if (!loose.b.p) prefetch_tmap(&tm_b);
   }
   if (warp == 1) {
     tmem_alloc(tmem_slot, kTmemColumns);
@@ -138,14 +184,16 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
         const int slot = it % S;
         if (!mbar_wait_bounded(&empty[slot], ((it / S) & 1) ^ 1, abort_flag, DEV_TIMEOUT_PRODUCER)) break;
         unsigned char *sa = smem + slot * SB, *sb = sa + A_BYTES;
-        mbar_arrive_expect_tx(&full[slot], SB);
-        if constexpr (AMN) {
+        mbar_arrive_expect_tx(&full[slot], (loose.a.p ? 0 : A_BYTES) + (loose.b.p ? 0 : NT * kLine));
+        if (loose.a.p) {
+        } else if constexpr (AMN) {
           tma_load_3d(sa, &tm_a, &full[slot], column0, kb * kBlock, 0);
           tma_load_3d(sa + kBlock * kLine, &tm_a, &full[slot], column0 + 64, kb * kBlock, 0);
         } else {
           tma_load_3d(sa, &tm_a, &full[slot], kb * kBlock, column0, 0);
         }
-        if constexpr (BMN) {
+        if (loose.b.p) {
+        } else if constexpr (BMN) {
 #pragma unroll
           for (int c = 0; c < NT / 64; ++c)
             tma_load_3d(sb + c * kBlock * kLine, &tm_b, &full[slot], row0 + c * 64, kb * kBlock, 0);
@@ -193,6 +241,57 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
       mbar_settle(drain, 0, abort_flag, DEV_TIMEOUT_MMA);
     }
   } else {
+    if (loose.a.p || loose.b.p) {
+      // 64 lines at a time, two 16 bytes a thread; the next ones are on their way while these
+      // are stored
+      constexpr int A_PARTS = kRows / 64, B_PARTS = (NT + 63) / 64;
+      const int thread = threadIdx.x - 64, line = thread / 8, j = thread % 8;
+      const int a_parts = loose.a.p ? A_PARTS : 0, parts = a_parts + (loose.b.p ? B_PARTS : 0);
+      const int units = (last - first) * parts;
+      auto load = [&](int unit, Piece (&to)[2]) {
+        const int block = (first + unit / parts) * kBlock, part = unit % parts;
+        const bool a = part < a_parts;
+        const int at = (a ? part : part - a_parts) * 64;           // first line, or first element of lines
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int l = line + h * 32;
+          if (a) {
+            if (AMN) to[h].load(loose.a, block + l, column0 + at + j * 8);
+            else to[h].load(loose.a, column0 + at + l, block + j * 8);
+          } else {
+            if (BMN) to[h].load(loose.b, block + l, row0 + at + j * 8);
+            else to[h].load(loose.b, row0 + at + l, block + j * 8);
+          }
+        }
+      };
+      Piece now[2], next[2];
+      load(0, now);
+      bool ok = true;
+#pragma unroll 1
+      for (int unit = 0; unit < units; ++unit) {
+        if (unit + 1 < units) load(unit + 1, next);
+        const int it = unit / parts, part = unit - it * parts, slot = it % S;
+        if (part == 0) {
+          ok = mbar_wait_bounded(&empty[slot], ((it / S) & 1) ^ 1, abort_flag, DEV_TIMEOUT_PRODUCER);
+          if (!__all_sync(0xffffffffu, ok)) break;
+        }
+        const bool a = part < a_parts;
+        unsigned char *to = smem + slot * SB + (a ? part * (64 * kLine) : A_BYTES + (part - a_parts) * (64 * kLine));
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int l = line + h * 32;
+          // (a K-major B of fewer than 64 rows has no more lines than those)
+          if (a || BMN || (part - a_parts) * 64 + l < NT)
+            *reinterpret_cast<uint4 *>(to + l * kLine + ((j ^ (l & 7)) << 4)) = now[h].value();
+          now[h] = next[h];
+        }
+        if (part == parts - 1) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&full[slot]);
+        }
+      }
+    }
     // sums to shared memory (once the last accumulator is there, the products are done with
     // it): two warps a quarter of the lanes, half of the rows each
     constexpr int HALF = NT / 2 < 16 ? 16 : NT / 2;
@@ -317,8 +416,19 @@ int run_split(const Side &a, const Side &b, Params p, int splits, cudaStream_t s
   CUtensorMap tc, tr;
   const int64_t ci = AMN ? p.n : p.k, cr = AMN ? p.k : p.n, ri = BMN ? p.rows : p.k, rr = BMN ? p.k : p.rows;
   const int64_t cp = pitch_bytes(b.pitch, cr, ci), rp = pitch_bytes(a.pitch, rr, ri);
-  if (int rc = make_map(&tc, b.p, ci, cr, 1, cp, cp, AMN ? kBlock : kRows)) return rc;
-  if (int rc = make_map(&tr, a.p, ri, rr, 1, rp, rp, BMN ? kBlock : NT)) return rc;
+  LooseTwo loose{};
+  if (!readable(b.p, cr, b.pitch, 1, 0)) {
+    loose.a = Loose{b.p, b.pitch, (int)ci, (int)cr};
+    memset(&tc, 0, sizeof(tc));                // not used
+  } else if (int rc = make_map(&tc, b.p, ci, cr, 1, cp, cp, AMN ? kBlock : kRows)) {
+    return rc;
+  }
+  if (!readable(a.p, rr, a.pitch, 1, 0)) {
+    loose.b = Loose{a.p, a.pitch, (int)ri, (int)rr};
+    memset(&tr, 0, sizeof(tr));
+  } else if (int rc = make_map(&tr, a.p, ri, rr, 1, rp, rp, BMN ? kBlock : NT)) {
+    return rc;
+  }
   const int64_t rows = (p.rows + NT - 1) / NT, columns = (p.n + kRows - 1) / kRows;
   if (rows * columns * splits > INT32_MAX / 2) return set_error(OZ_ERR_INVALID, "too many tiles");
   p.row_tiles = (int)rows;
@@ -341,7 +451,7 @@ int run_split(const Side &a, const Side &b, Params p, int splits, cudaStream_t s
   cfg.attrs = attr;
   cfg.numAttrs = 2;
   count_launch();
-  return check_cuda(cudaLaunchKernelEx(&cfg, kernel, tc, tr, p, splits), what);
+  return check_cuda(cudaLaunchKernelEx(&cfg, kernel, tc, tr, p, loose, splits), what);
 }
 
 template <typename O, typename T>

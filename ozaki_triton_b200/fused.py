@@ -9,6 +9,7 @@ All calls enqueue their work on the current stream of their tensors' device.
 
 from __future__ import annotations
 
+import ctypes
 from typing import Optional, Tuple, Union
 
 import torch
@@ -55,11 +56,13 @@ def _plan_forward(key, x, w, bias, activation, residual, out_dtype, want_pre) ->
     device = _check_places(x, w, bias, residual)
     copy = (k > 0 and not (_unit(x) and _unit(_along(w)))) or (bias is not None and not _unit(bias)) \
         or (residual is not None and not _unit(residual))
-    workspace = _copy_bytes(x) + _copy_bytes(_along(w)) if k > 0 and rows > 0 and n > 0 and not copy else 0
-    args = _lib.LinearArgs(None, None, None, None, None, None, None, rows, k, n, x.stride(0), *w.stride(),
-                           0 if residual is None else residual.stride(0), workspace, _OZ_DTYPE[x.dtype],
+    args = _lib.LinearArgs(x.data_ptr(), w.data_ptr(), None, None, None, None, None, rows, k, n, x.stride(0), *w.stride(),
+                           0 if residual is None else residual.stride(0), 0, _OZ_DTYPE[x.dtype],
                            _OZ_DTYPE[out_dtype], _OZ_DTYPE[x.dtype if bias is None else bias.dtype],
                            _lib.ACTIVATIONS[activation])
+    # (negative for what oz_linear will refuse)
+    workspace = 0 if copy else max(0, _lib.load().oz_linear_workspace_bytes(ctypes.byref(args)))
+    args.workspace_bytes = workspace
     return _PLANS.keep(key, _make_plan("oz_linear", args, (rows, n), out_dtype, device, rows == 0 or n == 0, copy,
                                        workspace))
 

@@ -248,6 +248,25 @@ def test_layouts(dtype):
     assert oz.device_status() == 0
 
 
+@pytest.mark.parametrize("rows,k,n", [(1, 8191, 129), (3, 777, 2049), (15, 4097, 33), (16, 65, 1001), (40, 1001, 515),
+                                      (64, 2050, 1407), (100, 999, 130), (128, 514, 2001), (250, 1500, 63), (9, 63, 7)])
+def test_operands_off_the_16_byte_boundaries(rows, k, n):
+    # every parity and offset of x's and w's rows; NaN around them
+    g = generator(rows + k)
+    for dx, dw in ((0, 0), (1, 3), (5, 0), (2, 7), (7, 6)):
+        wide = torch.full((rows, k + 9), float("nan"), dtype=torch.bfloat16, device=DEV)
+        x = wide[:, dx:dx + k].copy_(whole(g, rows, k))
+        big = torch.full((k, n + 9), float("nan"), dtype=torch.bfloat16, device=DEV)
+        w = big[:, dw:dw + n].copy_(whole(g, k, n))
+        tall = torch.full((n, k + 9), float("nan"), dtype=torch.bfloat16, device=DEV)
+        wt = tall[:, dw:dw + k].copy_(w.t()).t()
+        u = x.double() @ w.double()
+        for weight in (w, wt):
+            assert torch.equal(oz.fused_matmul(x, weight), u.bfloat16())
+            assert torch.equal(oz.fused_matmul(x, weight, out_dtype=torch.float32).double(), u)
+    assert oz.device_status() == 0
+
+
 def test_empty_sizes():
     z = dict(device=DEV, dtype=torch.bfloat16)
     b, r = torch.randn(6, device=DEV).bfloat16(), torch.randn(4, 6, device=DEV).bfloat16()

@@ -169,7 +169,9 @@ def test_library_entries_validate_without_a_launch():
     assert linear(bias=p, bias_dtype=_lib.OZ_BF16) == unsupported
     assert linear(rows=-1) == bad and linear(k=2 ** 31) == bad and linear(y=None) == bad and linear(x=None) == bad
     assert linear(w_sk=8, w_sn=2) == bad
-    assert linear(k=12, x_sr=12) == bad and "workspace" in lib.oz_last_error().decode()
+    # rows off the 16-byte boundaries, and sums in passes: copied first
+    assert linear(k=12004, x_sr=12004, out_dtype=_lib.OZ_F32) == bad and "workspace" in lib.oz_last_error().decode()
+    assert linear(x=p + 1) == bad and "aligned" in lib.oz_last_error().decode()
     assert linear(rows=0, y=None) == ok and linear(n=0, y=None) == ok
 
     def linear_backward(**kw):
