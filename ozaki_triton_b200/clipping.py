@@ -15,6 +15,7 @@ from .experts import _CURRENT_DEVICE, _LEVEL, _OnDevice, _check_places, _check_t
 CLIP_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 _CODES = {t: _OZ_DTYPE[t] for t in CLIP_DTYPES}
 _ALLOWED = frozenset(CLIP_DTYPES)
+_WORKSPACES = {}             # bytes for so many tensors
 
 
 def _dense(t: torch.Tensor) -> bool:
@@ -69,9 +70,9 @@ def clip_gradients(grads: Iterable[torch.Tensor], max_norm: float, *, eps: float
     if out is not None and not all([g.is_same_size(o) for g, o in zip(grads, outs)]):
         raise AssertionError("a result must have its gradient's shape")
     lib = _lib.load()
-    norm = first.new_empty((), dtype=torch.float32)
-    size = lib.oz_clip_workspace_bytes(n)
-    workspace = first.new_empty((size,), dtype=torch.uint8)
+    norm = first.new_empty_strided((), (), dtype=torch.float32)
+    size = _WORKSPACES.get(n) or _WORKSPACES.setdefault(n, lib.oz_clip_workspace_bytes(n))
+    workspace = first.new_empty_strided((size,), (1,), dtype=torch.uint8)
     # addresses, sizes and types as the library takes them
     pointers = array("Q", [t.data_ptr() for t in given])
     sizes = array("q", [t.numel() for t in grads])
