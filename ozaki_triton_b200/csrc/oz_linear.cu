@@ -273,40 +273,66 @@ int product(bool pair, const Side &a, const Side &b, const Params &p, cudaStream
               : run_job<LinearJob<O, B, 1, 128, false, false, FORM>>(a, b, p, st, what);
 }
 
-// How a product is divided, by the least estimated time (us, one B200, fitted to 690
-// measured times of 90 sizes, 1 to 16000 rows, 8 to 8192 terms and columns: half of them
-// within 10%; the choice is 3% slower than the best one on average).  Engine: its start, and for
-// each wave of tiles a tile's blocks of 64 terms and its end.  Split: for each CTA of the two
-// that an SM holds its start and end, for each CTA of an SM its blocks.  Some pairs (bf16, us):
-//   rows x terms x columns    128 x 128   256 x 256   split (rows of a tile, CTAs)
-//   4 x 3904 x 2600              22.3        25.1      7.2 (16, 8)    9.0 (16, 4)
-//   131 x 7504 x 2688            45          49       16.7 (64, 4)   20.4 (128, 4)
-//   432 x 72 x 2136               4.2         5.9      5.5 (64, 1)    7.4 (128, 1)
-//   720 x 7904 x 3616            76.8        45.2     67.0 (128, 4)
-//   2317 x 3056 x 3360           65.5        41.3     60.2 (128, 1)
+// How a product is divided, by the least estimated time (us, one B200, fitted to 2000 measured
+// times of 180 sizes, 1 to 16000 rows, 8 to 8192 terms and columns, plain and with what may
+// follow: half of them within 10%; the choice is 2% slower than the best one on average, 39% at
+// most).  Engine: its start, and for each wave of tiles a tile's blocks of 64 terms and its
+// end.  Split: for each wave of clusters (two CTAs an SM; clusters of 8 do not fit everywhere) a
+// CTA's start and end and its blocks, which take longer where the SM has two.  Some sizes (bf16, us):
+//   rows x terms x columns          128 x 128   256 x 256   split (rows of a tile, CTAs)
+//   4 x 3904 x 2600                    22.3        25.1      7.2 (16, 8)    9.0 (16, 4)
+//   131 x 7504 x 2688                  45          49       16.7 (64, 4)   20.4 (128, 4)
+//   432 x 72 x 2136                     4.2         5.9      5.5 (64, 1)    7.4 (128, 1)
+//   720 x 7904 x 3616                  76.8        45.2     67.0 (128, 4)
+//   580 x 6504 x 1056, silu, added     36.9        48       24.9 (128, 4)  39.0 (128, 2)
+//   8687 x 160 x 2369, the same        78.5        67.5
 struct Plan {
   bool pair;                   // the engine's tiles: 256 x 256 by pairs of CTAs, or 128 x 128
   SplitPlan split;             // of 0 rows: the engine
   bool loose;                  // operands off the 16-byte boundaries are read as they are
 };
-Plan plan_product(int64_t rows, int64_t k, int64_t n, bool rows_mn) {
-  const int64_t sms = tile::sm_count(), blocks = (k + kBlock - 1) / kBlock;
-  auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
+struct Times {
+  double start, block, end, start_pair, block_pair, end_pair;      // engine
+  double split_end[3], split_block[3], split_shared[3], joined[3]; // for tiles of 16, 64, 128 rows
+};
+constexpr Times kTimes[3] = {
+    {3.3, 0.320, 0.9, 3.6, 0.347, 1.9, {2.9, 4.4, 6.1}, {0.271, 0.290, 0.347}, {0.10, 0.21, 0.32}, {0.85, 0.37, 0}},
+    {2.4, 0.300, 3.9, 0.4, 0.321, 6.7, {4.0, 6.0, 7.6}, {0.292, 0.322, 0.410}, {0.10, 0.15, 0.28}, {0.75, 0, 0}},
+    {3.8, 0.306, 6.1, 2.6, 0.319, 11.2, {4.4, 6.4, 9.1}, {0.292, 0.311, 0.409}, {0.09, 0.21, 0.31}, {0.55, 0, 0}}};
+constexpr int kTileRows[3] = {16, 64, 128};
+int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
+// Clusters that the GPU holds at once, two CTAs an SM.
+int64_t clusters_at_once(int splits) {
+  const int64_t sms = tile::sm_count();
+  return splits == 1 ? 2 * sms : splits == 2 ? sms : splits == 4 ? sms * 70 / 148 : sms * 32 / 148;
+}
+
+Plan plan_product(int64_t rows, int64_t k, int64_t n, bool rows_mn, Form form) {
+  const int64_t sms = tile::sm_count(), blocks = up(k, kBlock);
+  const Times &t = kTimes[form];
   Plan plan{false, {0, 1}, false};
-  double best = 3.3 + up(up(rows, 128) * up(n, 128), sms) * (0.32 * blocks + 0.9);
-  const double pairs = 3.6 + up(up(rows, 256) * up(n, 256) * 2, sms) * (0.347 * blocks + 1.9);
+  double best = t.start + up(up(rows, 128) * up(n, 128), sms) * (t.block * blocks + t.end);
+  const double pairs = t.start_pair + up(up(rows, 256) * up(n, 256) * 2, sms) * (t.block_pair * blocks + t.end_pair);
   if (pairs < best) plan.pair = true, best = pairs;
   for (int shape = rows_mn ? 1 : 0; shape < 3; ++shape) {
-    const int tile_rows = shape == 0 ? 16 : shape == 1 ? 64 : 128;
-    const double end = shape == 0 ? 3.2 : shape == 1 ? 4.5 : 5.8, block = shape == 0 ? 0.224 : shape == 1 ? 0.269 : 0.345;
-    const int64_t tiles = up(rows, tile_rows) * up(n, 128);
+    const int64_t tiles = up(rows, kTileRows[shape]) * up(n, 128);
     for (int splits = 1; splits <= kMostSplits && splits <= blocks; splits *= 2) {
-      const double time = up(tiles * splits, 2 * sms) * end + up(tiles * splits, sms) * up(blocks, splits) * block +
-                          (splits > 1 ? 0.7 : 0.0);
-      if (time < best) plan.split = SplitPlan{tile_rows, splits}, best = time;
+      const int64_t held = clusters_at_once(splits), waves = up(tiles, held), halves = up(2 * tiles, held);
+      const int64_t each = up(blocks, splits);
+      if (waves > 2) break;                    // the engine's CTAs stay; the fit knows no more waves
+      const double time = waves * (t.split_end[shape] + each * t.split_block[shape]) +
+                          (halves - waves) * each * t.split_shared[shape] + (splits > 1 ? t.joined[shape] : 0.0);
+      if (time < best) plan.split = SplitPlan{kTileRows[shape], splits}, best = time;
     }
   }
   return plan;
+}
+
+// What follows the product and how its rows may be moved.
+Form form_of(const Params &p) {
+  if (!p.bias && !p.act && !p.residual && !p.pre) return kPlain;
+  constexpr int kAll = kVectors | kResidualVectors | kBiasVectors;
+  return (p.vectors & kAll) == kAll && p.n % 8 == 0 ? kByVectors : kByElements;
 }
 
 template <int FORM>
@@ -322,12 +348,11 @@ int product_in(bool pair, int dtype, int out_dtype, const Side &a, const Side &b
 int product_of(const Plan &plan, int dtype, int out_dtype, const Side &a, const Side &b, const Params &p, cudaStream_t st,
                const char *what) {
   if (plan.split.tile_rows) return split_product(plan.split, dtype, out_dtype, a, b, p, st, what);
-  if (!p.bias && !p.act && !p.residual && !p.pre)
-    return product_in<kPlain>(plan.pair, dtype, out_dtype, a, b, p, st, what);
-  constexpr int kAll = kVectors | kResidualVectors | kBiasVectors;
-  if ((p.vectors & kAll) == kAll && p.n % 8 == 0)
-    return product_in<kByVectors>(plan.pair, dtype, out_dtype, a, b, p, st, what);
-  return product_in<kByElements>(plan.pair, dtype, out_dtype, a, b, p, st, what);
+  switch (form_of(p)) {
+    case kPlain: return product_in<kPlain>(plan.pair, dtype, out_dtype, a, b, p, st, what);
+    case kByVectors: return product_in<kByVectors>(plan.pair, dtype, out_dtype, a, b, p, st, what);
+    default: return product_in<kByElements>(plan.pair, dtype, out_dtype, a, b, p, st, what);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -461,26 +486,25 @@ bool stored_across(int64_t n, int64_t w_sk, int64_t w_sn) { return w_sn == 1 || 
 // 20 us).  A copy first takes 11 and 12 us on the device, and 4.4 us more of the host, which
 // is what counts up to 13 us.  Not where fp32 results take their sums in passes: the warps that
 // would load are busy with those.
-Plan linear_operands(const oz_linear_args &a, bool across, Operand (&ops)[2]) {
+// (Whether they are read so does not depend on the form.)
+Plan linear_operands(const oz_linear_args &a, bool across, Form form, Operand (&ops)[2]) {
   ops[0] = Operand{a.x, a.rows, a.x_sr, 1, 0, (int)a.k};
   ops[1] = Operand{a.w, across ? a.k : a.n, across ? a.w_sk : a.w_sn, 1, 0, (int)(across ? a.n : a.k)};
-  const Plan whole = plan_product(a.rows, a.k, a.n, false);
+  const Plan whole = plan_product(a.rows, a.k, a.n, false, form);
   const bool loose_x = copy_bytes(ops[0]) != 0, loose_w = copy_bytes(ops[1]) != 0;
   if (!loose_x && !loose_w) return whole;
-  const int64_t sms = tile::sm_count(), blocks = (a.k + kBlock - 1) / kBlock;
-  auto up = [](int64_t v, int64_t by) { return (v + by - 1) / by; };
+  const int64_t sms = tile::sm_count(), blocks = up(a.k, kBlock);
   Plan plan{false, {0, 1}, true};
   double best = 10.5;
   for (int shape = 0; shape < 3; ++shape) {
-    const int tile_rows = shape == 0 ? 16 : shape == 1 ? 64 : 128;
-    const double end = shape == 0 ? 3.2 : shape == 1 ? 4.5 : 5.8;
-    const int64_t tiles = up(a.rows, tile_rows) * up(a.n, 128);
+    const int64_t tiles = up(a.rows, kTileRows[shape]) * up(a.n, 128);
     for (int splits = 1; splits <= kMostSplits && splits <= blocks; splits *= 2) {
-      const int64_t pieces = up(blocks, splits) * ((loose_w ? 2 : 0) + (loose_x ? up(tile_rows, 64) : 0));
+      const int64_t pieces = up(blocks, splits) * ((loose_w ? 2 : 0) + (loose_x ? up(kTileRows[shape], 64) : 0));
       if (a.out_dtype == OZ_F32 && up(blocks, splits) > 8) continue;
-      const double time = up(tiles * splits, 2 * sms) * (end + pieces * (tiles * splits > sms ? 1.1 : 0.75)) +
-                          (splits > 1 ? 0.7 : 0.0);
-      if (time < best) plan.split = SplitPlan{tile_rows, splits}, best = time;
+      const double time = up(tiles, clusters_at_once(splits)) *
+                              (kTimes[kPlain].split_end[shape] + pieces * (tiles * splits > sms ? 1.1 : 0.75)) +
+                          kTimes[kPlain].joined[shape];
+      if (time < best) plan.split = SplitPlan{kTileRows[shape], splits}, best = time;
     }
   }
   return plan.split.tile_rows ? plan : whole;
@@ -512,7 +536,7 @@ extern "C" int64_t oz_linear_workspace_bytes(const oz_linear_args *args) {
   if (check_linear(a.dtype, a.out_dtype, a.act, a.rows, a.k, a.n)) return OZ_ERR_INVALID;
   if (a.rows == 0 || a.n == 0 || a.k == 0) return 0;
   Operand ops[2];
-  if (linear_operands(a, stored_across(a.n, a.w_sk, a.w_sn), ops).loose) return 0;
+  if (linear_operands(a, stored_across(a.n, a.w_sk, a.w_sn), kPlain, ops).loose) return 0;
   return copy_bytes(ops[0]) + copy_bytes(ops[1]);
 }
 
@@ -547,7 +571,7 @@ extern "C" int oz_linear(const oz_linear_args *args, void *stream) {
   const bool across = stored_across(a.n, a.w_sk, a.w_sn);
   if (!across && a.w_sk != 1 && a.k != 1) return set_error(OZ_ERR_INVALID, "w must have a unit stride along k or n");
   Operand ops[2];
-  const Plan plan = linear_operands(a, across, ops);
+  const Plan plan = linear_operands(a, across, form_of(p), ops);
   if ((uintptr_t)a.x % 2 != 0 || (uintptr_t)a.w % 2 != 0)
     return set_error(OZ_ERR_INVALID, "an operand is not aligned to its elements");
   if (!plan.loose)
@@ -636,14 +660,14 @@ extern "C" int oz_linear_backward(const oz_linear_backward_args *args, void *str
     // dx (rows, k) = du (rows, n) w^T: w's rows along n where it is stored across
     Params p{a.dx, nullptr, nullptr, nullptr, a.k, 0, (int)a.rows, (int)a.n, (int)a.k, 0, 0,
                    (uintptr_t)a.dx % 16 == 0 && a.k % 8 == 0, 0, OZ_ACT_NONE, tile::instruction(a.dtype)};
-    if (int rc = product_of(plan_product(a.rows, a.n, a.k, false), a.dtype, a.dtype, Side{ops[0].p, ops[0].row, false},
+    if (int rc = product_of(plan_product(a.rows, a.n, a.k, false, kPlain), a.dtype, a.dtype, Side{ops[0].p, ops[0].row, false},
                                   Side{ops[at_w].p, ops[at_w].row, !across}, p, st, "dx launch"))
       return rc;
   }
   if (want_w) {
     Params p{a.dw, nullptr, nullptr, nullptr, a.n, 0, (int)a.k, (int)a.rows, (int)a.n, 0, 0,
                    (uintptr_t)a.dw % 16 == 0 && a.n * dw_size % 16 == 0, 0, OZ_ACT_NONE, tile::instruction(a.dtype)};
-    return product_of(plan_product(a.k, a.rows, a.n, true), a.dtype, a.dw_dtype, Side{ops[at_x].p, ops[at_x].row, true},
+    return product_of(plan_product(a.k, a.rows, a.n, true, kPlain), a.dtype, a.dw_dtype, Side{ops[at_x].p, ops[at_x].row, true},
                             Side{ops[0].p, ops[0].row, true}, p, st, "dw launch");
   }
   return OZ_OK;
