@@ -370,7 +370,8 @@ struct SlopeParams {
 constexpr int kSlopeRows = 8;  // rows of a block's pass, a warp each
 
 // 32 lanes take 32 V columns of a row; a warp's next two rows are on their way while it
-// works on the two before.
+// works on the two before.  8192 x 8192 (403 MB, 62 us at the memory's rate): silu 74 us with the
+// sums, gelu 92 (instructions); 5 blocks an SM spilled and took 88 and 108.
 template <typename T, int V> __global__ void __launch_bounds__(256, 4) slope_kernel(const SlopeParams p) {
   constexpr int AT_ONCE = 2;
   using R = stream::Raw<T, V>;

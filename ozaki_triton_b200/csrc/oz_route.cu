@@ -243,7 +243,8 @@ int route_smem(int e, int k, int chunk) {
 // for 4 tokens of 64 experts and 8 picks).  Ranks among the tokens of a round come from
 // one bit a token and expert in shared memory (set in any order, counted by popc), so there
 // is no sort.  With one block of one round the rows are final, else they count from the
-// block's first pick of the expert, and route_scan and route_place add the rest.
+// block's first pick of the expert, and route_scan and route_place add the rest.  32768 tokens,
+// 64 experts, 8 picks, bf16: 15 us (58 % of the issue slots), with the other two 25.
 template <int LPT, int VPL, int K, bool PACKED>
 __global__ void __launch_bounds__(kPickThreads, VPL == 16 && K <= 8 ? 4 : 1) route_pick(const RouteParams p) {
   extern __shared__ unsigned char smem[];
@@ -572,7 +573,9 @@ struct RouteBackward {
 };
 
 // dlogits, LPT lanes a token: the softmax again from the logits; a token's row then goes
-// through shared memory, where one lane for each pick adds its part.
+// through shared memory, where one lane for each pick adds its part.  16384 tokens, 256 experts, 8
+// picks, fp32 (35 MB, 5.4 us at the memory's rate): 13 us, bound by the latency of its sums over lanes
+// (picks added by the lanes that hold them: 23 us).
 template <int LPT, int VPL> __global__ void __launch_bounds__(256) route_backward(const RouteBackward p) {
   extern __shared__ unsigned char smem[];
   constexpr int GROUPS = 32 / LPT, WIDE = LPT * VPL;
@@ -714,6 +717,8 @@ template <typename T, int V> __device__ __forceinline__ void clear_rest(const Ro
 // How the threads of a block lie over tokens and columns: `tokens` tokens side by side,
 // `threads` threads each, which take the columns in steps of threads * V.
 struct Spread { int tokens, threads; };
+// Runs of a thread at a time: 4 where they are single elements.
+__host__ __device__ constexpr int at_once(int v) { return v == 1 ? 4 : 1; }
 
 // The slots of a token's picks, -1 where there is no row, loaded ahead of the rows they name.
 template <int K> struct Picks {
@@ -735,15 +740,23 @@ template <typename T, int V> __global__ void __launch_bounds__(256, 6) dispatch_
   start_after_earlier_kernels();
   if ((int)blockIdx.x >= blocks) return clear_rest<T, V>(p, blocks);
   const int group = (int)threadIdx.x / at.threads, in = (int)threadIdx.x - group * at.threads;
+  constexpr int U = at_once(V);
+  const int step = at.threads * V;
   if (group >= at.tokens) return;
   for (int64_t t = (int64_t)blockIdx.x * at.tokens + group; t < p.tokens; t += (int64_t)blocks * at.tokens) {
-    for (int c = in * V; c < p.d; c += at.threads * V) {
-      const auto v = Raw<T, V>::load(static_cast<const T *>(p.x) + t * p.x_row + c);
+    for (int c = in * V; c < p.d; c += U * step) {
+      typename Raw<T, V>::Type v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (c + u * step < p.d) v[u] = Raw<T, V>::load(static_cast<const T *>(p.x) + t * p.x_row + c + u * step);
       T *to = static_cast<T *>(p.rows_out) + c;
 #pragma unroll 4
       for (int j = 0; j < p.k; ++j) {
         const int64_t s = slot_of(p, t * p.k + j);
-        if (s >= 0) Raw<T, V>::store(to + s * p.d, v);
+        if (s < 0) continue;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (c + u * step < p.d) Raw<T, V>::store(to + s * p.d + u * step, v[u]);
       }
     }
   }
@@ -751,12 +764,16 @@ template <typename T, int V> __global__ void __launch_bounds__(256, 6) dispatch_
 
 constexpr int combine_blocks(int k) { return k >= 8 ? 3 : k >= 4 ? 4 : 5; }       // of an SM
 // y[t] = sum_j w rows[slot], in the order of j, K loads on their way at a time; the next
-// token's slots are loaded before this one's rows arrive.
+// token's slots are loaded before this one's rows arrive.  32768 x 2048, 6 picks, bf16: 151 us
+// (941 MB, 146 at the memory's rate); with loads converted as they came in 284, with registers for
+// 8 loads 176.
 template <typename T, int V, int K> __global__ void __launch_bounds__(256, combine_blocks(K)) combine_kernel(
     const RowsParams p, const Spread at) {
   start_after_earlier_kernels();
   const int group = (int)threadIdx.x / at.threads, in = (int)threadIdx.x - group * at.threads;
   if (group >= at.tokens) return;
+  constexpr int U = at_once(V);
+  const int width = at.threads * V;
   const int64_t step = (int64_t)gridDim.x * at.tokens;
   int64_t t = (int64_t)blockIdx.x * at.tokens + group;
   Picks<K> picks, next;
@@ -764,27 +781,37 @@ template <typename T, int V, int K> __global__ void __launch_bounds__(256, combi
   for (; t < p.tokens; t += step) {
     next.load(p, t + step, 0);
 #pragma unroll 1
-    for (int c = in * V; c < p.d; c += at.threads * V) {
+    for (int c = in * V; c < p.d; c += U * width) {
       const T *from = static_cast<const T *>(p.rows) + c;
-      float y[V] = {};
+      float y[U][V] = {};
 #pragma unroll 1
       for (int j0 = 0; j0 < p.k; j0 += K) {
         if (p.k > K) picks.load(p, t, j0);
-        typename Raw<T, V>::Type v[K];
+        typename Raw<T, V>::Type v[K][U];
 #pragma unroll
         for (int j = 0; j < K; ++j)
-          if (picks.slot[j] >= 0) v[j] = Raw<T, V>::load(from + (int64_t)picks.slot[j] * p.rows_row);
+          if (picks.slot[j] >= 0)
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+              if (U == 1 || c + u * width < p.d)
+                v[j][u] = Raw<T, V>::load(from + (int64_t)picks.slot[j] * p.rows_row + u * width);
 #pragma unroll
         for (int j = 0; j < K; ++j)
           if (picks.slot[j] >= 0) {
             const float w = p.weights ? __ldg(p.weights + t * p.k + j0 + j) : 1.f;
-            float u[V];
-            Raw<T, V>::values(v[j], u);
 #pragma unroll
-            for (int i = 0; i < V; ++i) y[i] = fmaf(w, u[i], y[i]);
+            for (int u = 0; u < U; ++u) {
+              float e[V];
+              Raw<T, V>::values(v[j][u], e);
+#pragma unroll
+              for (int i = 0; i < V; ++i) y[u][i] = fmaf(w, e[i], y[u][i]);
+            }
           }
       }
-      Run<T, V>::store(static_cast<T *>(p.x_out) + t * p.d + c, y);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (U == 1 || c + u * width < p.d)
+          Run<T, V>::store(static_cast<T *>(p.x_out) + t * p.d + c + u * width, y[u]);
     }
     picks = next;
   }
@@ -795,7 +822,7 @@ template <typename T, int V, int K> __global__ void __launch_bounds__(256, combi
 // source from its element c0 on (they start in the middle of one where the source's
 // address does: the halves that belong to neither stay unused, but share their word with
 // an element, so they can be read).  pair(i) with parity h is elements h + 2 m, h + 2 m + 1, m
-// = 32 i + lane, counted from c0.
+// = 32 i + lane, counted from c0.  dispatch, 5003 x 1001, 2 picks: 8.6 us, by elements 18.5.
 constexpr int kWordSpan = 512;
 struct Words {
   uint32_t direct[8], shifted[8];
@@ -889,7 +916,9 @@ template <typename T> __global__ void __launch_bounds__(256, 3) combine_words_ke
 }
 
 // drows[slot] = w dy[t], dw[t, j] = dy[t] . rows[slot]: `at.threads` threads (whole warps) a
-// token, K picks at a time.
+// token, K picks at a time.  8192 x 2816, 4 picks, bf16: 74 us (416 MB, 64 at the memory's rate).
+// Single elements (rows off the 16-byte boundaries) go 4 at a time: 20000 x 1001, 4 picks, bf16 137
+// us, one at a time 206.
 template <typename T, int V, int K>
 __global__ void __launch_bounds__(256, 3) combine_backward_kernel(const RowsParams p, const Spread at, int blocks) {
   __shared__ float sums[8][K];
@@ -897,6 +926,8 @@ __global__ void __launch_bounds__(256, 3) combine_backward_kernel(const RowsPara
   if ((int)blockIdx.x >= blocks) return clear_rest<T, V>(p, blocks);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, parts = at.threads / 32;
   const int group = warp / parts, in = (int)threadIdx.x - group * at.threads;
+  constexpr int U = at_once(V);
+  const int width = at.threads * V;
   const int64_t step = (int64_t)blocks * at.tokens;
   int64_t t = (int64_t)blockIdx.x * at.tokens + group;
   Picks<K> picks, next;
@@ -913,26 +944,37 @@ __global__ void __launch_bounds__(256, 3) combine_backward_kernel(const RowsPara
         weight[j] = picks.slot[j] >= 0 ? __ldg(p.weights + t * p.k + j0 + j) : 0.f;
       }
       if (t < p.tokens) {
-        for (int c = in * V; c < p.d; c += at.threads * V) {
-          typename Raw<T, V>::Type v[K];
-          const auto raw = Raw<T, V>::load(static_cast<const T *>(p.x) + t * p.x_row + c);
+        for (int c = in * V; c < p.d; c += U * width) {
+          typename Raw<T, V>::Type v[K][U], raw[U];
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            if (U == 1 || c + u * width < p.d)
+              raw[u] = Raw<T, V>::load(static_cast<const T *>(p.x) + t * p.x_row + c + u * width);
 #pragma unroll
           for (int j = 0; j < K; ++j)
             if (picks.slot[j] >= 0)
-              v[j] = Raw<T, V>::load(static_cast<const T *>(p.rows) + (int64_t)picks.slot[j] * p.rows_row + c);
-          float dy[V];
-          Raw<T, V>::values(raw, dy);
 #pragma unroll
-          for (int j = 0; j < K; ++j) {
-            if (picks.slot[j] < 0) continue;
-            float u[V];
-            Raw<T, V>::values(v[j], u);
+              for (int u = 0; u < U; ++u)
+                if (U == 1 || c + u * width < p.d)
+                  v[j][u] = Raw<T, V>::load(static_cast<const T *>(p.rows) + (int64_t)picks.slot[j] * p.rows_row + c +
+                                            u * width);
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-              dot[j] = fmaf(dy[i], u[i], dot[j]);
-              u[i] = weight[j] * dy[i];
+          for (int u = 0; u < U; ++u) {
+            if (U > 1 && c + u * width >= p.d) continue;
+            float dy[V];
+            Raw<T, V>::values(raw[u], dy);
+#pragma unroll
+            for (int j = 0; j < K; ++j) {
+              if (picks.slot[j] < 0) continue;
+              float e[V];
+              Raw<T, V>::values(v[j][u], e);
+#pragma unroll
+              for (int i = 0; i < V; ++i) {
+                dot[j] = fmaf(dy[i], e[i], dot[j]);
+                e[i] = weight[j] * dy[i];
+              }
+              Run<T, V>::store(static_cast<T *>(p.rows_out) + (int64_t)picks.slot[j] * p.d + c + u * width, e);
             }
-            Run<T, V>::store(static_cast<T *>(p.rows_out) + (int64_t)picks.slot[j] * p.d + c, u);
           }
         }
       }
@@ -1090,7 +1132,7 @@ extern "C" int oz_dispatch(const oz_rows_args *args, void *stream) {
       return launch(dispatch_words_kernel, dim3((unsigned)(blocks + kClearBlocks)), 256, 0, st,
                     "dispatch_words_kernel launch", p, (int)blocks);
     }
-    const Spread at = spread_over(a.d / (wide ? 16 / ES : 1), a.tokens, false, 6, blocks);
+    const Spread at = spread_over(wide ? a.d / (16 / ES) : (a.d + 3) / 4, a.tokens, false, 6, blocks);
     const dim3 grid((unsigned)(blocks + kClearBlocks));
     return wide ? launch(dispatch_kernel<T, 16 / ES>, grid, 256, 0, st, "dispatch_kernel launch", p, at, (int)blocks)
                 : launch(dispatch_kernel<T, 1>, grid, 256, 0, st, "dispatch_kernel launch", p, at, (int)blocks);
@@ -1118,7 +1160,7 @@ extern "C" int oz_combine(const oz_rows_args *args, void *stream) {
         blocks = word_blocks(a.tokens, a.d, 3);
         return launch(combine_words_kernel<T>, dim3((unsigned)blocks), 256, 0, st, "combine_words_kernel launch", p);
       }
-    const Spread at = spread_over(a.d / (wide ? 16 / ES : 1), a.tokens, false, combine_blocks(a.picks <= 6 ? a.picks : 8), blocks);
+    const Spread at = spread_over(wide ? a.d / (16 / ES) : (a.d + 3) / 4, a.tokens, false, combine_blocks(a.picks <= 6 ? a.picks : 8), blocks);
     auto with = [&](auto k) {
       constexpr int K = decltype(k)::value;
       const dim3 grid((unsigned)blocks);
@@ -1150,7 +1192,7 @@ extern "C" int oz_combine_backward(const oz_rows_args *args, void *stream) {
     const bool wide = vectors_ok(a.x, a.x_row, a.tokens, ES) && vectors_ok(a.rows, a.rows_row, n, ES) &&
                       vectors_ok(a.rows_out, a.d, n, ES) && a.d * ES % 16 == 0;
     int64_t blocks;
-    const Spread at = spread_over(a.d / (wide ? 16 / ES : 1), a.tokens, true, 3, blocks);
+    const Spread at = spread_over(wide ? a.d / (16 / ES) : (a.d + 3) / 4, a.tokens, true, 3, blocks);
     const dim3 grid((unsigned)(blocks + kClearBlocks));
     const char *what = "combine_backward_kernel launch";
     return wide ? launch(combine_backward_kernel<T, 16 / ES, 4>, grid, 256, 0, st, what, p, at, (int)blocks)

@@ -297,6 +297,15 @@ def test_rows_of_other_layouts():
     assert torch.equal(oz.combine(rows, turned), oz.combine(rows, r))
 
 
+def test_rows_without_columns():
+    r = oz.route(torch.randn(20, 8, device=DEV), 2)
+    x, rows = torch.empty(20, 0, device=DEV), torch.empty(40, 0, device=DEV)
+    assert oz.dispatch(x, r).shape == (40, 0) and oz.combine(rows, r).shape == (20, 0)
+    assert oz.dispatch_backward(rows, r).shape == (20, 0)
+    drows, dweights = oz.combine_backward(x, rows, r)
+    assert drows.shape == (40, 0) and dweights.shape == (20, 2) and not dweights.any()
+
+
 def test_a_routing_made_by_hand_stays_in_bounds():
     g = generator(6)
     x = torch.randn(40, 64, generator=g, device=DEV)
