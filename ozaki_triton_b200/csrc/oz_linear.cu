@@ -304,7 +304,8 @@ int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // Clusters that the GPU holds at once, two CTAs an SM.
 int64_t clusters_at_once(int splits) {
   const int64_t sms = tile::sm_count();
-  return splits == 1 ? 2 * sms : splits == 2 ? sms : splits == 4 ? sms * 70 / 148 : sms * 32 / 148;
+  return splits == 1 ? 2 * sms : splits == 2 ? sms : splits == 4 ? sms * 70 / 148 : splits == 8 ? sms * 32 / 148
+                                                                                               : sms * 14 / 148;
 }
 
 Plan plan_product(int64_t rows, int64_t k, int64_t n, bool rows_mn, Form form) {
@@ -365,20 +366,23 @@ struct SlopeParams {
   int64_t dy_sr, pre_sr, du_sr;
   int64_t rows;
   int n, act, per;             // rows of a block
+  int lanes;                   // of a row: a power of 2
 };
 
-constexpr int kSlopeRows = 8;  // rows of a block's pass, a warp each
+constexpr int kSlopeRows = 8;  // warps of a block
 
-// 32 lanes take 32 V columns of a row; a warp's next two rows are on their way while it
-// works on the two before.  8192 x 8192 (403 MB, 62 us at the memory's rate): silu 74 us with the
-// sums, gelu 92 (instructions); 5 blocks an SM spilled and took 88 and 108.
+// p.lanes lanes take a row's columns (or 32 V of them), so a warp has 32 / p.lanes rows; its
+// next two sets of rows are on their way while it works on the two before.  8192 x 8192 (403
+// MB, 62 us at the memory's rate): silu 74 us with the sums, gelu 92 (instructions); 5 blocks an
+// SM spilled and took 88 and 108.
 template <typename T, int V> __global__ void __launch_bounds__(256, 4) slope_kernel(const SlopeParams p) {
   constexpr int AT_ONCE = 2;
   using R = stream::Raw<T, V>;
   __shared__ float part[kSlopeRows][32 * V];
   stream::start_after_earlier_kernels();
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int c = (blockIdx.x * 32 + lane) * V;
+  const int c = (blockIdx.x * 32 + lane % p.lanes) * V;
+  const int first = warp * (32 / p.lanes) + lane / p.lanes, apart = kSlopeRows * (32 / p.lanes);
   const int64_t r0 = (int64_t)blockIdx.y * p.per;
   const int rows = (int)min((int64_t)p.per, p.rows - r0);
   float sum[V] = {};
@@ -389,19 +393,19 @@ template <typename T, int V> __global__ void __launch_bounds__(256, 4) slope_ker
     auto load = [&](int r, auto &to_a, auto &to_b) {
 #pragma unroll
       for (int q = 0; q < AT_ONCE; ++q) {
-        const int at = r + q * kSlopeRows;
+        const int at = r + q * apart;
         if (at >= rows) continue;
         to_a[q] = R::load(dy + at * p.dy_sr);
         if (p.pre) to_b[q] = R::load(pre + at * p.pre_sr);
       }
     };
-    load(warp, a, b);
+    load(first, a, b);
 #pragma unroll 1
-    for (int r = warp; r < rows; r += AT_ONCE * kSlopeRows) {
-      load(r + AT_ONCE * kSlopeRows, next_a, next_b);
+    for (int r = first; r < rows; r += AT_ONCE * apart) {
+      load(r + AT_ONCE * apart, next_a, next_b);
 #pragma unroll
       for (int q = 0; q < AT_ONCE; ++q) {
-        const int at = r + q * kSlopeRows;
+        const int at = r + q * apart;
         if (at >= rows) continue;
         float v[V], u[V];
         R::values(a[q], v);
@@ -428,10 +432,14 @@ template <typename T, int V> __global__ void __launch_bounds__(256, 4) slope_ker
     }
   }
   if (!p.sums) return;
+  for (int o = p.lanes; o < 32; o *= 2)
 #pragma unroll
-  for (int x = 0; x < V; ++x) part[warp][lane * V + x] = sum[x];
+    for (int x = 0; x < V; ++x) sum[x] += __shfl_xor_sync(0xffffffffu, sum[x], o);
+  if (lane < p.lanes)
+#pragma unroll
+    for (int x = 0; x < V; ++x) part[warp][lane * V + x] = sum[x];
   __syncthreads();
-  for (int i = threadIdx.x; i < 32 * V; i += 256) {
+  for (int i = threadIdx.x; i < p.lanes * V; i += 256) {
     const int column = blockIdx.x * 32 * V + i;
     if (column >= p.n) continue;
     float s = 0.f;
@@ -621,10 +629,11 @@ extern "C" int oz_linear_backward(const oz_linear_backward_args *args, void *str
     void *out = a.act ? space : nullptr;
     float *sums = !a.db ? nullptr : blocks == 1 ? a.db
                   : reinterpret_cast<float *>(space + (a.act ? align256(a.rows * pitch * 2) : 0));
-    const SlopeParams s{a.dy, a.act ? a.pre : nullptr, out, sums, a.dy_sr, a.pre_sr, pitch, a.rows, (int)a.n, a.act, per};
+    SlopeParams s{a.dy, a.act ? a.pre : nullptr, out, sums, a.dy_sr, a.pre_sr, pitch, a.rows, (int)a.n, a.act, per, 32};
     auto fits = [&](const void *base, int64_t sr) { return !base || ((uintptr_t)base % 16 == 0 && (a.rows == 1 || sr % 8 == 0)); };
     const bool wide = fits(s.dy, s.dy_sr) && fits(s.pre, s.pre_sr) && a.n % 8 == 0;
     const int v = wide ? 8 : 1;
+    while (s.lanes > 1 && s.lanes / 2 * v >= a.n) s.lanes /= 2;
     if (blocks > 65535) return set_error(OZ_ERR_INVALID, "size out of range");
     const dim3 grid((unsigned)((a.n + 32 * v - 1) / (32 * v)), (unsigned)blocks);
     const char *what = "slope_kernel launch";

@@ -143,7 +143,7 @@ struct Side {
 // oz_linear_split.cu: results of few tiles of 128 columns by `tile_rows` (16, 64 or 128; 16
 // only where the rows are not stored across the contraction), the contraction over `splits`
 // CTAs of a cluster.
-constexpr int kMostSplits = 8;
+constexpr int kMostSplits = 16;
 struct SplitPlan { int tile_rows, splits; };
 int split_product(const SplitPlan &plan, int dtype, int out_dtype, const Side &a, const Side &b, const Params &p,
                   cudaStream_t st, const char *what);

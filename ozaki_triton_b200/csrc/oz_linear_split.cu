@@ -4,7 +4,7 @@
 //   y = act(x w + bias) + residual     (or a plain product)
 //
 // What bounds them is the way of the operands' bytes to the SMs, so the contraction is
-// divided over the CTAs of a cluster (up to 8), each with 128 columns of the result
+// divided over the CTAs of a cluster (up to 16), each with 128 columns of the result
 // by up to 128 of its rows: tcgen05 products with the columns as A (their weights are
 // read once, however few rows there are), fp32 sums in tensor memory.  The CTAs
 // then put their sums into shared memory and each adds up, over the cluster, the
@@ -368,13 +368,14 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
             if (r0 + i * step < rows)
               load4(static_cast<const O *>(p.residual) + (int64_t)(row0 + r0 + i * step) * p.residual_ld + column,
                     p.vectors & kResidualVectors, count, residual[i]);
-        float4 v[AT_ONCE][kMostSplits];
+        // 8 CTAs' sums on their way at a time, added in the order of the CTAs
+        float4 v[AT_ONCE][8];
 #pragma unroll
         for (int i = 0; i < AT_ONCE; ++i) {
           const int r = min(r0 + i * step, rows - 1);
           if (splits > 1) {
 #pragma unroll
-            for (int s = 0; s < kMostSplits; ++s)
+            for (int s = 0; s < 8; ++s)
               if (s < splits) v[i][s] = load_cluster(map_to_cta(mine + (uint32_t)(r * kRows * 4), s));
           } else {
             v[i][0] = *reinterpret_cast<const float4 *>(partial + r * kRows + lane * 4);
@@ -384,11 +385,25 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
         for (int i = 0; i < AT_ONCE; ++i) {
           u[i][0] = v[i][0].x, u[i][1] = v[i][0].y, u[i][2] = v[i][0].z, u[i][3] = v[i][0].w;
 #pragma unroll
-          for (int s = 1; s < kMostSplits; ++s)
+          for (int s = 1; s < 8; ++s)
             if (s < splits) u[i][0] += v[i][s].x, u[i][1] += v[i][s].y, u[i][2] += v[i][s].z, u[i][3] += v[i][s].w;
+        }
+        if (splits > 8)
+#pragma unroll 1
+          for (int i = 0; i < AT_ONCE; ++i) {
+            const int r = min(r0 + i * step, rows - 1);
+#pragma unroll
+            for (int s = 0; s < 8; ++s) v[0][s] = load_cluster(map_to_cta(mine + (uint32_t)(r * kRows * 4), 8 + s));
+#pragma unroll
+            for (int s = 0; s < 8; ++s)
+#pragma unroll
+              for (int j = 0; j < AT_ONCE; ++j)
+                if (i == j) u[j][0] += v[0][s].x, u[j][1] += v[0][s].y, u[j][2] += v[0][s].z, u[j][3] += v[0][s].w;
+          }
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i)
 #pragma unroll
           for (int x = 0; x < 4; ++x) u[i][x] += bias[x];
-        }
 #pragma unroll
         for (int i = 0; i < AT_ONCE; ++i) {
           if (r0 + i * step >= rows) continue;
@@ -410,6 +425,25 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
     tc_fence_after();
     tmem_dealloc(tmem, kTmemColumns);
   }
+}
+
+// Clusters of 16 are past what every GPU of the kind must hold: a kernel has to ask, once a device.
+int allow_large_clusters(const void *kernel, const char *what) {
+  constexpr int kDevs = 64;
+  static std::mutex mu;
+  static std::unordered_map<const void *, bool> asked[kDevs];
+  int dev = -1;
+  const bool known = cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < kDevs;
+  if (known) {
+    std::lock_guard<std::mutex> lk(mu);
+    if (asked[dev].count(kernel)) return OZ_OK;
+  }
+  const int rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), what);
+  if (rc == OZ_OK && known) {
+    std::lock_guard<std::mutex> lk(mu);
+    asked[dev][kernel] = true;
+  }
+  return rc;
 }
 
 template <typename O, typename T, int NT, bool AMN, bool BMN>
@@ -438,6 +472,8 @@ int run_split(const Side &a, const Side &b, Params p, int splits, cudaStream_t s
   auto kernel = split_kernel<O, T, NT, AMN, BMN>;
   constexpr int smem = split_smem<NT>();
   if (int rc = set_smem_once((const void *)kernel, smem, what)) return rc;
+  if (splits > 8)
+    if (int rc = allow_large_clusters((const void *)kernel, what)) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(rows * columns * splits));
   cfg.blockDim = dim3(kSplitThreads);

@@ -267,6 +267,28 @@ def test_operands_off_the_16_byte_boundaries(rows, k, n):
     assert oz.device_status() == 0
 
 
+@pytest.mark.parametrize("rows,k,n", [(1, 8192, 64), (5, 16384, 200), (40, 12000, 72), (100, 20001, 136), (200, 9000, 260)])
+def test_long_contractions(rows, k, n):
+    # few tiles: the contraction over as many as 16 CTAs.  Sums of up to 20001 terms of magnitude
+    # 4 at most are exact in fp32
+    g = generator(k)
+    x, w, dy = (whole(g, *s, most=2).bfloat16() for s in ((rows, k), (k, n), (k, n)))
+    bias, residual = whole(g, n).bfloat16(), whole(g, rows, n).bfloat16()
+    u = x.double() @ w.double()
+    assert torch.equal(oz.fused_matmul(x, w), u.bfloat16())
+    assert torch.equal(oz.fused_matmul(x, w, out_dtype=torch.float32).double(), u)
+    y, pre = oz.fused_matmul(x, w, bias, activation="relu", residual=residual, return_pre=True)
+    assert torch.equal(pre, (u + bias.double()).bfloat16())
+    assert torch.equal(y, ((u + bias.double()).clamp(min=0) + residual.double()).bfloat16())
+    # k rows now: dw (rows, n) sums over them
+    tall = x.t().contiguous()
+    dx, dw, db = oz.fused_matmul_backward(dy, tall, torch.ones(rows, n, device=DEV).bfloat16(), bias=True,
+                                          dw_dtype=torch.float32)
+    assert torch.equal(dw.double(), x.double() @ dy.double()) and torch.equal(db.double(), dy.double().sum(0))
+    assert torch.equal(dx, dy.double().sum(1, keepdim=True).expand(k, rows).bfloat16())
+    assert oz.device_status() == 0
+
+
 def test_empty_sizes():
     z = dict(device=DEV, dtype=torch.bfloat16)
     b, r = torch.randn(6, device=DEV).bfloat16(), torch.randn(4, 6, device=DEV).bfloat16()
