@@ -286,6 +286,8 @@ int product(bool pair, const Side &a, const Side &b, const Params &p, cudaStream
 //   720 x 7904 x 3616                  76.8        45.2     67.0 (128, 4)
 //   580 x 6504 x 1056, silu, added     36.9        48       24.9 (128, 4)  39.0 (128, 2)
 //   8687 x 160 x 2369, the same        78.5        67.5
+// and by pairs that share a contraction, silu: 299 x 4632 x 3880 28.1 (2 pairs) where the others take
+// 34.0, 580 x 6504 x 1056 18.4 (4 pairs; 24.6), 536 x 7504 x 2688 32.9 (2; 42.3).
 struct Plan {
   bool pair;                   // the engine's tiles: 256 x 256 by pairs of CTAs, or 128 x 128
   SplitPlan split;             // of 0 rows: the engine
@@ -308,7 +310,7 @@ int64_t clusters_at_once(int splits) {
                                                                                                : sms * 14 / 148;
 }
 
-Plan plan_product(int64_t rows, int64_t k, int64_t n, bool rows_mn, Form form) {
+Plan plan_product(int64_t rows, int64_t k, int64_t n, bool rows_mn, Form form, bool fp32) {
   const int64_t sms = tile::sm_count(), blocks = up(k, kBlock);
   const Times &t = kTimes[form];
   Plan plan{false, {0, 1}, false};
@@ -322,9 +324,16 @@ Plan plan_product(int64_t rows, int64_t k, int64_t n, bool rows_mn, Form form) {
       const int64_t each = up(blocks, splits);
       if (waves > 2) break;                    // the engine's CTAs stay; the fit knows no more waves
       const double time = waves * (t.split_end[shape] + each * t.split_block[shape]) +
-                          (halves - waves) * each * t.split_shared[shape] + (splits > 1 ? t.joined[shape] : 0.0);
+                          (halves - waves) * each * t.split_shared[shape] + (splits > 1 ? t.joined[shape] : 0.0) + (splits > 8 ? 1.0 : 0.0);
       if (time < best) plan.split = SplitPlan{kTileRows[shape], splits}, best = time;
     }
+  }
+  // tiles of 256 x 256 whose contraction 2 or 4 pairs of CTAs share, in one wave (as many as 34
+  // and 14 clusters are held at once)
+  for (int splits = 2; !fp32 && splits <= 4 && splits <= blocks; splits *= 2) {
+    const double time = (splits == 2 ? 12.0 : 8.8) + up(blocks, splits) * 0.35;
+    if (up(rows, 256) * up(n, 256) <= (splits == 2 ? sms * 34 / 148 : sms * 14 / 148) && time < best)
+      plan.split = SplitPlan{kPairTile, splits}, best = time;
   }
   return plan;
 }
@@ -499,7 +508,7 @@ bool stored_across(int64_t n, int64_t w_sk, int64_t w_sn) { return w_sn == 1 || 
 Plan linear_operands(const oz_linear_args &a, bool across, Form form, Operand (&ops)[2]) {
   ops[0] = Operand{a.x, a.rows, a.x_sr, 1, 0, (int)a.k};
   ops[1] = Operand{a.w, across ? a.k : a.n, across ? a.w_sk : a.w_sn, 1, 0, (int)(across ? a.n : a.k)};
-  const Plan whole = plan_product(a.rows, a.k, a.n, false, form);
+  const Plan whole = plan_product(a.rows, a.k, a.n, false, form, a.out_dtype == OZ_F32);
   const bool loose_x = copy_bytes(ops[0]) != 0, loose_w = copy_bytes(ops[1]) != 0;
   if (!loose_x && !loose_w) return whole;
   const int64_t sms = tile::sm_count(), blocks = up(a.k, kBlock);
@@ -507,7 +516,7 @@ Plan linear_operands(const oz_linear_args &a, bool across, Form form, Operand (&
   double best = 10.5;
   for (int shape = 0; shape < 3; ++shape) {
     const int64_t tiles = up(a.rows, kTileRows[shape]) * up(a.n, 128);
-    for (int splits = 1; splits <= kMostSplits && splits <= blocks; splits *= 2) {
+    for (int splits = 1; splits <= 8 && splits <= blocks; splits *= 2) {      // (16: 15 us where 8 take 12)
       const int64_t pieces = up(blocks, splits) * ((loose_w ? 2 : 0) + (loose_x ? up(kTileRows[shape], 64) : 0));
       if (a.out_dtype == OZ_F32 && up(blocks, splits) > 8) continue;
       const double time = up(tiles, clusters_at_once(splits)) *
@@ -670,14 +679,15 @@ extern "C" int oz_linear_backward(const oz_linear_backward_args *args, void *str
     // dx (rows, k) = du (rows, n) w^T: w's rows along n where it is stored across
     Params p{a.dx, nullptr, nullptr, nullptr, a.k, 0, (int)a.rows, (int)a.n, (int)a.k, 0, 0,
                    (uintptr_t)a.dx % 16 == 0 && a.k % 8 == 0, 0, OZ_ACT_NONE, tile::instruction(a.dtype)};
-    if (int rc = product_of(plan_product(a.rows, a.n, a.k, false, kPlain), a.dtype, a.dtype, Side{ops[0].p, ops[0].row, false},
+    if (int rc = product_of(plan_product(a.rows, a.n, a.k, false, kPlain, false), a.dtype, a.dtype, Side{ops[0].p, ops[0].row, false},
                                   Side{ops[at_w].p, ops[at_w].row, !across}, p, st, "dx launch"))
       return rc;
   }
   if (want_w) {
     Params p{a.dw, nullptr, nullptr, nullptr, a.n, 0, (int)a.k, (int)a.rows, (int)a.n, 0, 0,
                    (uintptr_t)a.dw % 16 == 0 && a.n * dw_size % 16 == 0, 0, OZ_ACT_NONE, tile::instruction(a.dtype)};
-    return product_of(plan_product(a.k, a.rows, a.n, true, kPlain), a.dtype, a.dw_dtype, Side{ops[at_x].p, ops[at_x].row, true},
+    return product_of(plan_product(a.k, a.rows, a.n, true, kPlain, a.dw_dtype == OZ_F32),
+                      a.dtype, a.dw_dtype, Side{ops[at_x].p, ops[at_x].row, true},
                             Side{ops[0].p, ops[0].row, true}, p, st, "dw launch");
   }
   return OZ_OK;

@@ -144,6 +144,8 @@ struct Side {
 // only where the rows are not stored across the contraction), the contraction over `splits`
 // CTAs of a cluster.
 constexpr int kMostSplits = 16;
+// Or, for 16-bit results, of tiles of 256 x 256 by pairs of CTAs, 2 or 4 pairs a cluster.
+constexpr int kPairTile = 256;
 struct SplitPlan { int tile_rows, splits; };
 int split_product(const SplitPlan &plan, int dtype, int out_dtype, const Side &a, const Side &b, const Params &p,
                   cudaStream_t st, const char *what);

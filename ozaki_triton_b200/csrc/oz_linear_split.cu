@@ -125,6 +125,83 @@ struct Piece {
   }
 };
 
+// Adds up rows part, part + splits, ... of the cluster's sums (128 columns from column0 on; CTA
+// first + apart s holds the s-th part of the contraction) and finishes them: the 8 last warps, a
+// warp a row, 4 columns a lane.
+template <typename O, typename T>
+__device__ __forceinline__ void join_rows(const Params &p, const float *partial, int part, int splits, int first, int apart,
+                                          int row0, int rows, int column0) {
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int column = column0 + lane * 4, count = min(p.n - column, 4);
+  const uint32_t mine = smem_u32(partial) + (uint32_t)lane * 16;
+  float bias[4] = {};
+  if (p.bias && count > 0) {
+    if (p.bias_f32) load4(static_cast<const float *>(p.bias) + column, p.vectors & kBiasVectors, count, bias);
+    else load4(static_cast<const T *>(p.bias) + column, p.vectors & kBiasVectors, count, bias);
+  }
+  if (count > 0) {
+    // two rows side by side: one's way through the instructions hides the other's
+    constexpr int AT_ONCE = 2;
+    const int step = kFinishWarps * splits;
+    for (int r0 = part + (warp - 2) * splits; r0 < rows; r0 += AT_ONCE * step) {
+      float u[AT_ONCE][4], residual[AT_ONCE][4];
+      if (p.residual)
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i)
+          if (r0 + i * step < rows)
+            load4(static_cast<const O *>(p.residual) + (int64_t)(row0 + r0 + i * step) * p.residual_ld + column,
+                  p.vectors & kResidualVectors, count, residual[i]);
+      // 8 CTAs' sums on their way at a time, added in the order of the CTAs
+      float4 v[AT_ONCE][8];
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i) {
+        const int r = min(r0 + i * step, rows - 1);
+        if (splits > 1) {
+#pragma unroll
+          for (int s = 0; s < 8; ++s)
+            if (s < splits) v[i][s] = load_cluster(map_to_cta(mine + (uint32_t)(r * kRows * 4), first + apart * s));
+        } else {
+          v[i][0] = *reinterpret_cast<const float4 *>(partial + r * kRows + lane * 4);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i) {
+        u[i][0] = v[i][0].x, u[i][1] = v[i][0].y, u[i][2] = v[i][0].z, u[i][3] = v[i][0].w;
+#pragma unroll
+        for (int s = 1; s < 8; ++s)
+          if (s < splits) u[i][0] += v[i][s].x, u[i][1] += v[i][s].y, u[i][2] += v[i][s].z, u[i][3] += v[i][s].w;
+      }
+      if (splits > 8)
+#pragma unroll 1
+        for (int i = 0; i < AT_ONCE; ++i) {
+          const int r = min(r0 + i * step, rows - 1);
+#pragma unroll
+          for (int s = 0; s < 8; ++s) v[0][s] = load_cluster(map_to_cta(mine + (uint32_t)(r * kRows * 4), first + apart * (8 + s)));
+#pragma unroll
+          for (int s = 0; s < 8; ++s)
+#pragma unroll
+            for (int j = 0; j < AT_ONCE; ++j)
+              if (i == j) u[j][0] += v[0][s].x, u[j][1] += v[0][s].y, u[j][2] += v[0][s].z, u[j][3] += v[0][s].w;
+        }
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) u[i][x] += bias[x];
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i) {
+        if (r0 + i * step >= rows) continue;
+        const int64_t at = (int64_t)(row0 + r0 + i * step) * p.ld + column;
+        if (p.pre) store4(static_cast<T *>(p.pre) + at, p.vectors & kVectors, count, u[i]);
+        activate(u[i], p.act);
+        if (p.residual)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) u[i][x] += residual[i][x];
+        store4(static_cast<O *>(p.out) + at, p.vectors & kVectors, count, u[i]);
+      }
+    }
+  }
+}
+
 // A: 128 columns of the result, B: NT rows.  O: the result's type, T: the operands'.
 template <typename O, typename T, int NT, bool AMN, bool BMN>
 __global__ void __launch_bounds__(kSplitThreads, 2)
@@ -348,75 +425,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
   if (splits > 1) cluster_sync();
   else __syncthreads();
   if (warp >= 2) {
-    // a warp a row, 4 columns a lane
-    const int rows = min(p.rows - row0, NT), column = column0 + lane * 4, count = min(p.n - column, 4);
-    const uint32_t mine = smem_u32(partial) + (uint32_t)lane * 16;
-    float bias[4] = {};
-    if (p.bias && count > 0) {
-      if (p.bias_f32) load4(static_cast<const float *>(p.bias) + column, p.vectors & kBiasVectors, count, bias);
-      else load4(static_cast<const T *>(p.bias) + column, p.vectors & kBiasVectors, count, bias);
-    }
-    if (count > 0) {
-      // two rows side by side: one's way through the instructions hides the other's
-      constexpr int AT_ONCE = 2;
-      const int step = kFinishWarps * splits;
-      for (int r0 = rank + (warp - 2) * splits; r0 < rows; r0 += AT_ONCE * step) {
-        float u[AT_ONCE][4], residual[AT_ONCE][4];
-        if (p.residual)
-#pragma unroll
-          for (int i = 0; i < AT_ONCE; ++i)
-            if (r0 + i * step < rows)
-              load4(static_cast<const O *>(p.residual) + (int64_t)(row0 + r0 + i * step) * p.residual_ld + column,
-                    p.vectors & kResidualVectors, count, residual[i]);
-        // 8 CTAs' sums on their way at a time, added in the order of the CTAs
-        float4 v[AT_ONCE][8];
-#pragma unroll
-        for (int i = 0; i < AT_ONCE; ++i) {
-          const int r = min(r0 + i * step, rows - 1);
-          if (splits > 1) {
-#pragma unroll
-            for (int s = 0; s < 8; ++s)
-              if (s < splits) v[i][s] = load_cluster(map_to_cta(mine + (uint32_t)(r * kRows * 4), s));
-          } else {
-            v[i][0] = *reinterpret_cast<const float4 *>(partial + r * kRows + lane * 4);
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < AT_ONCE; ++i) {
-          u[i][0] = v[i][0].x, u[i][1] = v[i][0].y, u[i][2] = v[i][0].z, u[i][3] = v[i][0].w;
-#pragma unroll
-          for (int s = 1; s < 8; ++s)
-            if (s < splits) u[i][0] += v[i][s].x, u[i][1] += v[i][s].y, u[i][2] += v[i][s].z, u[i][3] += v[i][s].w;
-        }
-        if (splits > 8)
-#pragma unroll 1
-          for (int i = 0; i < AT_ONCE; ++i) {
-            const int r = min(r0 + i * step, rows - 1);
-#pragma unroll
-            for (int s = 0; s < 8; ++s) v[0][s] = load_cluster(map_to_cta(mine + (uint32_t)(r * kRows * 4), 8 + s));
-#pragma unroll
-            for (int s = 0; s < 8; ++s)
-#pragma unroll
-              for (int j = 0; j < AT_ONCE; ++j)
-                if (i == j) u[j][0] += v[0][s].x, u[j][1] += v[0][s].y, u[j][2] += v[0][s].z, u[j][3] += v[0][s].w;
-          }
-#pragma unroll
-        for (int i = 0; i < AT_ONCE; ++i)
-#pragma unroll
-          for (int x = 0; x < 4; ++x) u[i][x] += bias[x];
-#pragma unroll
-        for (int i = 0; i < AT_ONCE; ++i) {
-          if (r0 + i * step >= rows) continue;
-          const int64_t at = (int64_t)(row0 + r0 + i * step) * p.ld + column;
-          if (p.pre) store4(static_cast<T *>(p.pre) + at, p.vectors & kVectors, count, u[i]);
-          activate(u[i], p.act);
-          if (p.residual)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) u[i][x] += residual[i][x];
-          store4(static_cast<O *>(p.out) + at, p.vectors & kVectors, count, u[i]);
-        }
-      }
-    }
+    join_rows<O, T>(p, partial, rank, splits, 0, 1, row0, min(p.rows - row0, NT), column0);
   }
   tc_fence_before();
   if (splits > 1) cluster_sync();              // nobody's sums go away while they are read
@@ -424,6 +433,156 @@ __global__ void __launch_bounds__(kSplitThreads, 2)
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, kTmemColumns);
+  }
+}
+
+// The same for results of a few tiles of 256 x 256, whose operands' way from L2 to the SMs
+// bounds them: pairs of CTAs hold half of a tile's columns and rows each (as in the tile engine)
+// and multiply them by one instruction, and the 2 or 4 pairs of a cluster share the contraction.
+// 16-bit results only: their sums are of one pass.
+constexpr int kPairRows = 256, kPairStage = 2 * kRows * kLine, kPairStages = 6;
+constexpr int kPairSmem = 1024 + kPairStages * kPairStage + 256;
+
+// Arrive on the barrier at this offset of both CTAs of pair q once the products so far are done.
+__device__ __forceinline__ void commit_to_pair(uint32_t bar, int q) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+      "h"((uint16_t)(3 << (2 * q)))
+      : "memory");
+}
+
+template <typename T, bool AMN, bool BMN>
+__global__ void __launch_bounds__(kSplitThreads, 1)
+    pair_split_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const Params p,
+                      const int splits) {
+  constexpr int S = kPairStages, SB = kPairStage, A_BYTES = kRows * kLine, NT = kPairRows;
+  static_assert(NT * kRows * 4 <= S * SB && kPairSmem <= kSmemLimit, "shared memory");
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  float *partial = reinterpret_cast<float *>(smem);            // [NT][128], after the products
+  uint64_t *full = reinterpret_cast<uint64_t *>(smem + S * SB);
+  uint64_t *empty = full + S;
+  uint64_t *acc_full = empty + S;
+  uint64_t *drain = acc_full + 1;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int rank = (int)cluster_ctarank(), q = rank / 2, half = rank % 2;
+  const bool leader = half == 0;
+  const int tile = blockIdx.x / (2 * splits);
+  const int column0 = tile / p.row_tiles * (2 * kRows) + half * kRows, row0 = tile % p.row_tiles * NT;
+  const int blocks = (p.k + kBlock - 1) / kBlock;
+  const int first = (int)((int64_t)blocks * q / splits), last = (int)((int64_t)blocks * (q + 1) / splits);
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    mbar_init(acc_full, 1);
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    prefetch_tmap(&tm_a);
+    prefetch_tmap(&tm_b);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, NT);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  stream::start_after_earlier_kernels();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int it = 0;
+      const int br = row0 + half * kRows;
+      for (int kb = first; kb < last; ++kb, ++it) {
+        const int slot = it % S;
+        if (!mbar_wait_bounded(&empty[slot], ((it / S) & 1) ^ 1, abort_flag, DEV_TIMEOUT_PRODUCER)) break;
+        unsigned char *sa = smem + slot * SB, *sb = sa + A_BYTES;
+        if (leader) mbar_arrive_expect_tx(&full[slot], 2 * SB);
+        const uint32_t bar = map_to_cta(smem_u32(&full[slot]), 2 * q);
+        if constexpr (AMN) {
+          tma_load_3d_pair(sa, &tm_a, bar, column0, kb * kBlock, 0);
+          tma_load_3d_pair(sa + kBlock * kLine, &tm_a, bar, column0 + 64, kb * kBlock, 0);
+        } else {
+          tma_load_3d_pair(sa, &tm_a, bar, kb * kBlock, column0, 0);
+        }
+        if constexpr (BMN) {
+          tma_load_3d_pair(sb, &tm_b, bar, br, kb * kBlock, 0);
+          tma_load_3d_pair(sb + kBlock * kLine, &tm_b, bar, br + 64, kb * kBlock, 0);
+        } else {
+          tma_load_3d_pair(sb, &tm_b, bar, kb * kBlock, br, 0);
+        }
+      }
+      // every load has landed, and every stage is reported as read, before shared memory is used for
+      // something else or goes away
+      if (leader)
+        for (int k = max(it - S, 0); k < it; ++k)
+          if (!mbar_settle(&full[k % S], (k / S) & 1, abort_flag, DEV_TIMEOUT_PRODUCER)) break;
+      for (int k = max(it - S, 0); k < it; ++k)
+        if (!mbar_settle(&empty[k % S], (k / S) & 1, abort_flag, DEV_TIMEOUT_PRODUCER)) break;
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && leader) {
+      const uint32_t base = smem_u32(smem);
+      const uint64_t a_desc = operand_desc<AMN>(base), b_desc = operand_desc<BMN>(base + A_BYTES);
+      constexpr uint64_t a_step = AMN ? (16 * kLine) >> 4 : 2, b_step = BMN ? (16 * kLine) >> 4 : 2;
+      const uint32_t idesc = p.idesc | (uint32_t)(NT >> 3) << 17 | (uint32_t)((2 * kRows) >> 4) << 24 |
+                             (AMN ? 1u << 15 : 0u) | (BMN ? 1u << 16 : 0u);
+      int slot = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int kb = first; kb < last; ++kb) {
+        if (!(ok = wait_cluster(&full[slot], phase, abort_flag, DEV_TIMEOUT_MMA))) break;
+        tc_fence_after();
+        const uint64_t ad = a_desc + slot * (SB >> 4), bd = b_desc + slot * (SB >> 4);
+#pragma unroll
+        for (int kk = 0; kk < kBlock / 16; ++kk)
+          tc_mma_pair<1>(tmem, ad + kk * a_step, bd + kk * b_step, idesc, kk || kb > first ? 1u : 0u);
+        commit_to_pair(smem_u32(&empty[slot]), q);
+        if (++slot == S) {
+          slot = 0;
+          phase ^= 1;
+        }
+      }
+      if (ok) commit_to_pair(smem_u32(acc_full), q);
+      tc_commit_pair(smem_u32(drain));
+      mbar_settle(drain, 0, abort_flag, DEV_TIMEOUT_MMA);
+    }
+  } else {
+    // sums to shared memory (once they are there, the products are done with it): two warps a
+    // quarter of the lanes, half of the rows each
+    const int sub = warp & 3, from = (warp - 2) / 4 * (NT / 2), rows = min(p.rows - row0 - from, NT / 2);
+    const uint32_t columns = tmem + ((uint32_t)(sub * 32) << 16) + (uint32_t)from;
+    float *to = partial + from * kRows + sub * 32 + lane;
+    const bool ok = mbar_wait_bounded(acc_full, 0, abort_flag, DEV_TIMEOUT_EPILOGUE);
+    if (__all_sync(0xffffffffu, ok)) {
+      tc_fence_after();
+#pragma unroll 1
+      for (int r0 = 0; r0 < rows; r0 += 16) {
+        uint32_t v[16];
+        tmem_ld16_at(columns + (uint32_t)r0, v);
+        tmem_ld_wait16(v);
+#pragma unroll
+        for (int x = 0; x < 16; ++x)
+          if (r0 + x < rows) to[(r0 + x) * kRows] = __uint_as_float(v[x]);
+      }
+    }
+  }
+  __syncwarp();
+  cluster_sync();
+  if (warp >= 2) join_rows<T, T>(p, partial, q, splits, half, 2, row0, min(p.rows - row0, NT), column0);
+  tc_fence_before();
+  cluster_sync();                              // nobody's sums go away while they are read
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, NT);
   }
 }
 
@@ -492,6 +651,45 @@ int run_split(const Side &a, const Side &b, Params p, int splits, cudaStream_t s
   return check_cuda(cudaLaunchKernelEx(&cfg, kernel, tc, tr, p, loose, splits), what);
 }
 
+template <typename T, bool AMN, bool BMN>
+int run_pairs(const Side &a, const Side &b, Params p, int splits, cudaStream_t st, const char *what) {
+  CUtensorMap tc, tr;
+  const int64_t ci = AMN ? p.n : p.k, cr = AMN ? p.k : p.n, ri = BMN ? p.rows : p.k, rr = BMN ? p.k : p.rows;
+  const int64_t cp = pitch_bytes(b.pitch, cr, ci), rp = pitch_bytes(a.pitch, rr, ri);
+  if (int rc = make_map(&tc, b.p, ci, cr, 1, cp, cp, AMN ? kBlock : kRows)) return rc;
+  if (int rc = make_map(&tr, a.p, ri, rr, 1, rp, rp, BMN ? kBlock : kRows)) return rc;
+  const int64_t rows = (p.rows + kPairRows - 1) / kPairRows, columns = (p.n + 2 * kRows - 1) / (2 * kRows);
+  if (rows * columns * splits > INT32_MAX / 4) return set_error(OZ_ERR_INVALID, "too many tiles");
+  p.row_tiles = (int)rows;
+  p.column_tiles = (int)columns;
+  auto kernel = pair_split_kernel<T, AMN, BMN>;
+  if (int rc = set_smem_once((const void *)kernel, kPairSmem, what)) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(rows * columns * splits * 2));
+  cfg.blockDim = dim3(kSplitThreads);
+  cfg.dynamicSmemBytes = kPairSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2 * splits;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  count_launch();
+  return check_cuda(cudaLaunchKernelEx(&cfg, kernel, tc, tr, p, splits), what);
+}
+
+template <typename T>
+int pairs_of(int splits, const Side &a, const Side &b, const Params &p, cudaStream_t st, const char *what) {
+  if (a.mn) return b.mn ? run_pairs<T, true, true>(a, b, p, splits, st, what)
+                        : set_error(OZ_ERR_UNSUPPORTED, "operand layout");
+  return b.mn ? run_pairs<T, true, false>(a, b, p, splits, st, what)
+              : run_pairs<T, false, false>(a, b, p, splits, st, what);
+}
+
 template <typename O, typename T>
 int split_of(const SplitPlan &plan, const Side &a, const Side &b, const Params &p, cudaStream_t st, const char *what) {
   const int s = plan.splits;
@@ -515,6 +713,11 @@ namespace linear {
 
 int split_product(const SplitPlan &plan, int dtype, int out_dtype, const Side &a, const Side &b, const Params &p,
                   cudaStream_t st, const char *what) {
+  if (plan.tile_rows == kPairTile) {
+    if (out_dtype != dtype) return set_error(OZ_ERR_UNSUPPORTED, "output dtype %d", out_dtype);
+    return dtype == OZ_F16 ? pairs_of<__half>(plan.splits, a, b, p, st, what)
+                           : pairs_of<__nv_bfloat16>(plan.splits, a, b, p, st, what);
+  }
   if (dtype == OZ_F16)
     return out_dtype == OZ_F32 ? split_of<float, __half>(plan, a, b, p, st, what)
                                : split_of<__half, __half>(plan, a, b, p, st, what);

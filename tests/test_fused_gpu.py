@@ -289,6 +289,27 @@ def test_long_contractions(rows, k, n):
     assert oz.device_status() == 0
 
 
+@pytest.mark.parametrize("rows,k,n", [(580, 6504, 1056), (299, 4632, 3880), (536, 7504, 2688), (3384, 4608, 384),
+                                      (257, 8192, 519)])
+def test_middle_sizes(rows, k, n):
+    # a few tiles of 256 x 256, whose contraction pairs of CTAs share
+    g = generator(n)
+    x, w = whole(g, rows, k, most=2).bfloat16(), whole(g, k, n, most=2).bfloat16()
+    bias, residual = whole(g, n).bfloat16(), whole(g, rows, n).bfloat16()
+    u = x.double() @ w.double()
+    for weight in (w, w.t().contiguous().t()):
+        y, pre = oz.fused_matmul(x, weight, bias, activation="relu", residual=residual, return_pre=True)
+        assert torch.equal(pre, (u + bias.double()).bfloat16())
+        assert torch.equal(y, ((u + bias.double()).clamp(min=0) + residual.double()).bfloat16())
+        assert torch.equal(oz.fused_matmul(x, weight), u.bfloat16())
+    tall = x.t().contiguous()                         # dw (rows, n) sums over k rows
+    dy = w
+    dx, dw, _ = oz.fused_matmul_backward(dy, tall, torch.ones(rows, n, device=DEV).bfloat16())
+    assert torch.equal(dw, u.bfloat16())
+    assert torch.equal(dx, dy.double().sum(1, keepdim=True).expand(k, rows).bfloat16())
+    assert oz.device_status() == 0
+
+
 def test_empty_sizes():
     z = dict(device=DEV, dtype=torch.bfloat16)
     b, r = torch.randn(6, device=DEV).bfloat16(), torch.randn(4, 6, device=DEV).bfloat16()
