@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(kThreads, kScaleBlocksPerSm) scale_kernel(cons
   __shared__ double warp_sum[kThreads / 32];
   start_after_earlier_kernels();
   double all = 0;
-  for (int i = threadIdx.x; i < sums.blocks; i += kThreads) all += __ldg(sums.partial + i);
+  for (int i = threadIdx.x; i < sums.blocks; i += kThreads) all += *(sums.partial + i);
 #pragma unroll
   for (int o = 16; o > 0; o /= 2) all += __shfl_xor_sync(0xffffffffu, all, o);
   if (threadIdx.x % 32 == 0) warp_sum[threadIdx.x / 32] = all;

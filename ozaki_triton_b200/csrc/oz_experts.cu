@@ -22,8 +22,8 @@ namespace {
 using namespace tile;
 
 __device__ __forceinline__ int64_t load_offset(const void *offsets, int wide, int64_t i) {
-  return wide ? __ldg(static_cast<const long long *>(offsets) + i)
-              : (int64_t)__ldg(static_cast<const int *>(offsets) + i);
+  return wide ? *(static_cast<const long long *>(offsets) + i)
+              : (int64_t)*(static_cast<const int *>(offsets) + i);
 }
 
 // Row range of group e, clamped so that a bad offset never leaves the tensor.

@@ -29,7 +29,7 @@ template <typename E> struct Run8 {
   static __device__ __forceinline__ Raw load(const E *p) {
     Raw r;
 #pragma unroll
-    for (int h = 0; h < (int)sizeof(E) / 2; ++h) r.u[h] = __ldg(reinterpret_cast<const uint4 *>(p) + h);
+    for (int h = 0; h < (int)sizeof(E) / 2; ++h) r.u[h] = *(reinterpret_cast<const uint4 *>(p) + h);
     return r;
   }
   static __device__ __forceinline__ void values(const Raw &r, float (&v)[8]) {
@@ -386,7 +386,7 @@ constexpr int kSlopeRows = 8;  // warps of a block
 // SM spilled and took 88 and 108.
 template <typename T, int V> __global__ void __launch_bounds__(256, 4) slope_kernel(const SlopeParams p) {
   constexpr int AT_ONCE = 2;
-  using R = stream::Raw<T, V>;
+  using R = stream::Raw<T, V, true>;
   __shared__ float part[kSlopeRows][32 * V];
   stream::start_after_earlier_kernels();
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -466,7 +466,7 @@ __global__ void __launch_bounds__(256) sums_kernel(const float *sums, float *out
   double s = 0;
   if (c < n)
 #pragma unroll 8
-    for (int r = warp; r < rows; r += 8) s += __ldg(sums + (int64_t)r * n + c);
+    for (int r = warp; r < rows; r += 8) s += *(sums + (int64_t)r * n + c);
   part[warp][lane] = s;
   __syncthreads();
   if (warp || c >= n) return;

@@ -128,8 +128,8 @@ constexpr int kVectors = 1, kResidualVectors = 2, kBiasVectors = 4;    // rows o
 
 // The bias has the operands' type B or fp32.
 template <typename B> __device__ __forceinline__ float bias_at(const Params &p, int64_t c) {
-  if (p.bias_f32) return __ldg(static_cast<const float *>(p.bias) + c);
-  return to_f32(__ldg(static_cast<const B *>(p.bias) + c));
+  if (p.bias_f32) return *(static_cast<const float *>(p.bias) + c);
+  return to_f32(*(static_cast<const B *>(p.bias) + c));
 }
 
 // Two operands of a result (rows, n): one along its rows, one along its columns, each

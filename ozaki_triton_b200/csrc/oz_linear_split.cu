@@ -49,17 +49,17 @@ __device__ __forceinline__ float4 load_cluster(uint32_t addr) {
 template <typename E> __device__ __forceinline__ void load4(const E *from, bool vectors, int count, float (&v)[4]) {
   if (vectors && count >= 4) {
     if constexpr (sizeof(E) == 4) {
-      const float4 a = __ldg(reinterpret_cast<const float4 *>(from));
+      const float4 a = *(reinterpret_cast<const float4 *>(from));
       v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
     } else {
-      const uint2 a = __ldg(reinterpret_cast<const uint2 *>(from));
+      const uint2 a = *(reinterpret_cast<const uint2 *>(from));
       const E *e = reinterpret_cast<const E *>(&a);
 #pragma unroll
       for (int x = 0; x < 4; ++x) v[x] = to_f32(e[x]);
     }
   } else {
 #pragma unroll
-    for (int x = 0; x < 4; ++x) v[x] = x < count ? to_f32(__ldg(from + x)) : 0.f;
+    for (int x = 0; x < 4; ++x) v[x] = x < count ? to_f32(*(from + x)) : 0.f;
   }
 }
 template <typename E> __device__ __forceinline__ void store4(E *to, bool vectors, int count, const float (&v)[4]) {
@@ -103,8 +103,8 @@ struct Piece {
     const uintptr_t from = (uintptr_t)o.p + 2 * (uintptr_t)(row * o.pitch + at);
     shift = (int)(from & 15);
     const uint4 *v = reinterpret_cast<const uint4 *>(from - shift);
-    low = __ldg(v);
-    if (shift + 2 * count > 16) high = __ldg(v + 1);
+    low = *(v);
+    if (shift + 2 * count > 16) high = *(v + 1);
   }
   __device__ __forceinline__ uint4 value() const {
     uint32_t w[8] = {low.x, low.y, low.z, low.w, high.x, high.y, high.z, high.w};

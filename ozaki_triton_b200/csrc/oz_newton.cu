@@ -84,7 +84,7 @@ template <int DTYPE> struct Eight {
     const uint4 *q = reinterpret_cast<const uint4 *>(static_cast<const char *>(p) + i * (kWords / 2));
 #pragma unroll
     for (int x = 0; x < kWords / 4; ++x) {
-      const uint4 a = __ldg(q + x);
+      const uint4 a = *(q + x);
       w[4 * x] = a.x, w[4 * x + 1] = a.y, w[4 * x + 2] = a.z, w[4 * x + 3] = a.w;
     }
   }
@@ -95,8 +95,8 @@ template <int DTYPE> struct Eight {
 #pragma unroll
     for (int x = 0; x < 8; ++x)
       if (x < left) {
-        if (DTYPE == OZ_F32) w[x % kWords] = __ldg(static_cast<const uint32_t *>(p) + i + x * step);
-        else w[x / 2 % kWords] |= (uint32_t)__ldg(static_cast<const unsigned short *>(p) + i + x * step) << x % 2 * 16;
+        if (DTYPE == OZ_F32) w[x % kWords] = *(static_cast<const uint32_t *>(p) + i + x * step);
+        else w[x / 2 % kWords] |= (uint32_t)*(static_cast<const unsigned short *>(p) + i + x * step) << x % 2 * 16;
       }
   }
   __device__ __forceinline__ void floats(float (&v)[8]) const {

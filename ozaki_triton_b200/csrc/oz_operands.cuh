@@ -61,7 +61,7 @@ __global__ void __launch_bounds__(256, 6) repitch_kernel(const __grid_constant__
 #pragma unroll
       for (int i = 0; i < 9; ++i) {
         const int j = j0 + i * 32 + lane;
-        w[i] = 2 * j - off < count && (i < 8 || lane == 0) ? __ldg(words + j) : 0;
+        w[i] = 2 * j - off < count && (i < 8 || lane == 0) ? *(words + j) : 0;
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {

@@ -58,10 +58,10 @@ __device__ __forceinline__ void load_row(const Logits &g, int64_t t, bool there,
     if (g.vectors) {                          // whole groups of 4
       if (there && e < g.e) {
         if constexpr (sizeof(T) == 4) {
-          const float4 u = __ldg(reinterpret_cast<const float4 *>(from + e));
+          const float4 u = *(reinterpret_cast<const float4 *>(from + e));
           v[i] = u.x, v[i + 1] = u.y, v[i + 2] = u.z, v[i + 3] = u.w;
         } else {
-          const uint2 u = __ldg(reinterpret_cast<const uint2 *>(from + e));
+          const uint2 u = *(reinterpret_cast<const uint2 *>(from + e));
           const T *w = reinterpret_cast<const T *>(&u);
 #pragma unroll
           for (int x = 0; x < 4; ++x) v[i + x] = to_f32(w[x]);
@@ -85,9 +85,9 @@ __device__ __forceinline__ void load_row(const Logits &g, int64_t t, bool there,
 
 __device__ __forceinline__ float logit(const Logits &g, int64_t t, int e) {
   const int64_t at = t * g.row + e * g.col;
-  if (g.dtype == OZ_F32) return __ldg(static_cast<const float *>(g.p) + at);
-  if (g.dtype == OZ_F16) return to_f32(__ldg(static_cast<const __half *>(g.p) + at));
-  return to_f32(__ldg(static_cast<const __nv_bfloat16 *>(g.p) + at));
+  if (g.dtype == OZ_F32) return *(static_cast<const float *>(g.p) + at);
+  if (g.dtype == OZ_F16) return to_f32(*(static_cast<const __half *>(g.p) + at));
+  return to_f32(*(static_cast<const __nv_bfloat16 *>(g.p) + at));
 }
 
 struct RouteParams {
@@ -700,14 +700,14 @@ struct RowsParams {
 
 // A slot that is a row, else -1.
 __device__ __forceinline__ int64_t slot_of(const RowsParams &p, int64_t pick) {
-  const int s = __ldg(p.slots + pick);
+  const int s = *(p.slots + pick);
   return s >= 0 && s < p.row_count ? s : -1;
 }
 
 // Zeros in the rows after the last pick's, by the blocks from `first` on.
 template <typename T, int V> __device__ __forceinline__ void clear_rest(const RowsParams &p, int first) {
   const int64_t n = p.d / V, end = p.row_count * n;
-  const int64_t from = min(max((int64_t)__ldg(p.offsets + p.experts), (int64_t)0), p.row_count) * n;
+  const int64_t from = min(max((int64_t)*(p.offsets + p.experts), (int64_t)0), p.row_count) * n;
   float zero[V] = {};
   for (int64_t i = from + (int64_t)(blockIdx.x - first) * blockDim.x + threadIdx.x; i < end;
        i += (int64_t)(gridDim.x - first) * blockDim.x)
@@ -728,7 +728,7 @@ template <int K> struct Picks {
     for (int j = 0; j < K; ++j) {
       slot[j] = -1;
       if (t < p.tokens && j0 + j < p.k) {
-        const int s = __ldg(p.slots + t * p.k + j0 + j);
+        const int s = *(p.slots + t * p.k + j0 + j);
         slot[j] = s >= 0 && s < p.row_count ? s : -1;
       }
     }
@@ -798,7 +798,7 @@ template <typename T, int V, int K> __global__ void __launch_bounds__(256, combi
 #pragma unroll
         for (int j = 0; j < K; ++j)
           if (picks.slot[j] >= 0) {
-            const float w = p.weights ? __ldg(p.weights + t * p.k + j0 + j) : 1.f;
+            const float w = p.weights ? *(p.weights + t * p.k + j0 + j) : 1.f;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
               float e[V];
@@ -835,7 +835,7 @@ struct Words {
 #pragma unroll
     for (int i = 0; i < 9; ++i) {
       const int j = i * 32 + lane;
-      w[i] = 2 * j - off < count && (i < 8 || lane == 0) ? __ldg(words + j) : 0;
+      w[i] = 2 * j - off < count && (i < 8 || lane == 0) ? *(words + j) : 0;
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -893,11 +893,11 @@ template <typename T> __global__ void __launch_bounds__(256, 3) combine_words_ke
     for (int j = 0; j < p.k; ++j) {
       const int64_t s = slot_of(p, t * p.k + j);
       if (s < 0) continue;
-      const float w = p.weights ? __ldg(p.weights + t * p.k + j) : 1.f;
+      const float w = p.weights ? *(p.weights + t * p.k + j) : 1.f;
       const E *from = static_cast<const E *>(p.rows) + s * p.rows_row + c0;
       Words words;
       words.load(from, count);
-      if (single) edge = fmaf(w, low(__ldg(from + at)), edge);
+      if (single) edge = fmaf(w, low(*(from + at)), edge);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const uint32_t u = words.pair(i, h);
@@ -941,7 +941,7 @@ __global__ void __launch_bounds__(256, 3) combine_backward_kernel(const RowsPara
 #pragma unroll
       for (int j = 0; j < K; ++j) {
         dot[j] = 0.f;
-        weight[j] = picks.slot[j] >= 0 ? __ldg(p.weights + t * p.k + j0 + j) : 0.f;
+        weight[j] = picks.slot[j] >= 0 ? *(p.weights + t * p.k + j0 + j) : 0.f;
       }
       if (t < p.tokens) {
         for (int c = in * V; c < p.d; c += U * width) {

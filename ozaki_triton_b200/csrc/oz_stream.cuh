@@ -34,13 +34,24 @@ template <typename T> __device__ __forceinline__ uint4 pack(const float (&v)[16 
   return u;
 }
 
+// 16 bytes that are read once: they take no place in L1.  Not held in order against stores: for
+// memory that the kernel does not write.  (du of 8192 x 8192 and its products 538 us a call, by plain
+// loads 553; rows to tokens and back are 1 to 2 us faster by plain ones, of 75 and 168.)
+__device__ __forceinline__ uint4 read_once(const void *p) {
+  uint4 u;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
+               : "l"(p));
+  return u;
+}
+
 // V consecutive elements of T: 16 bytes, or one element where rows do not start
-// on 16-byte boundaries.  Read once (no use of them is left for L1).
+// on 16-byte boundaries.
 template <typename T, int V> struct Run {
   static_assert(V == 1 || V * sizeof(T) == 16, "one element or 16 bytes");
   static __device__ __forceinline__ void load(const T *p, float (&v)[V]) {
     if constexpr (V == 1) v[0] = to_f32(*p);
-    else unpack<T>(__ldg(reinterpret_cast<const uint4 *>(p)), v);
+    else unpack<T>(*reinterpret_cast<const uint4 *>(p), v);
   }
   static __device__ __forceinline__ void store(T *p, const float (&v)[V]) {
     if constexpr (V == 1) *p = from_f32<T>(v[0]);
@@ -49,11 +60,12 @@ template <typename T, int V> struct Run {
 };
 
 // The same as it lies in memory: few registers for loads on their way.
-template <typename T, int V> struct Raw {
+template <typename T, int V, bool ONCE = false> struct Raw {
   using Type = typename std::conditional<V == 1, T, uint4>::type;
   static __device__ __forceinline__ Type load(const T *p) {
     if constexpr (V == 1) return *p;
-    else return __ldg(reinterpret_cast<const uint4 *>(p));
+    else if constexpr (ONCE) return read_once(p);
+    else return *reinterpret_cast<const uint4 *>(p);
   }
   static __device__ __forceinline__ void store(T *p, const Type &v) { *reinterpret_cast<Type *>(p) = v; }
   static __device__ __forceinline__ void values(const Type &r, float (&v)[V]) {
@@ -62,6 +74,9 @@ template <typename T, int V> struct Raw {
   }
 };
 
+// What follows reads by plain loads alone: a read-only one (ld.global.nc, __ldg) may be moved before
+// the wait, and may find in L1 what stood there before an earlier kernel wrote it, as that kernel
+// runs during this one's life.
 __device__ __forceinline__ void start_after_earlier_kernels() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");

@@ -58,8 +58,8 @@ __device__ __forceinline__ void expert_rows(const W4Params &p, int e, int &begin
     return;
   }
   auto at = [&](int i) {
-    return p.wide ? (int64_t)__ldg(static_cast<const long long *>(p.offsets) + i)
-                  : (int64_t)__ldg(static_cast<const int *>(p.offsets) + i);
+    return p.wide ? (int64_t)*(static_cast<const long long *>(p.offsets) + i)
+                  : (int64_t)*(static_cast<const int *>(p.offsets) + i);
   };
   begin = (int)min(max(at(e), (int64_t)0), (int64_t)p.rows);
   end = (int)min(max(at(e + 1), (int64_t)begin), (int64_t)p.rows);

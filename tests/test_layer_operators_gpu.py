@@ -307,3 +307,30 @@ def test_gradients_past_32_bit_offsets():
     assert abs(norm.item() - want) <= 1e-6 * want
     one = torch.tensor(1 / want).bfloat16().item()
     assert bool((big[:1000] == one).all()) and bool((big[-1000:] == one).all()) and big.float().amax() == one
+
+
+def test_calls_that_reuse_memory_follow_one_another():
+    # a kernel may start while those before it run: the routing, the sums and the rows of each turn
+    # stand where those of the turn before stood, and no other kernel comes between
+    torch.manual_seed(3)
+    scores = [torch.randn(96, 16, device="cuda") for _ in range(8)]
+    x = torch.randn(96, 64, device="cuda", dtype=torch.bfloat16)
+    w = torch.randn(64, 64, device="cuda", dtype=torch.bfloat16)
+    grads = [torch.randn(5000, device="cuda") * (i + 1) for i in range(8)]
+    spare = torch.empty(5000, device="cuda")
+
+    def turn(i):
+        r = oz.route(scores[i], 2)
+        rows = oz.dispatch(x, r)
+        y = oz.combine(rows, r)
+        u = oz.fused_matmul(y, w, residual=y)
+        return y, u, oz.clip_gradients([grads[i]], 1.0, out=[spare])
+
+    want = []
+    for i in range(8):
+        want.append(turn(i))
+        torch.cuda.synchronize()
+    for _ in range(20):
+        found = [turn(i) for i in range(8)]
+        for a, b in zip(found, want):
+            assert all(torch.equal(s, t) for s, t in zip(a, b))
