@@ -574,7 +574,7 @@ struct RouteBackward {
 
 // dlogits, LPT lanes a token: the softmax again from the logits; a token's row then goes
 // through shared memory, where one lane for each pick adds its part.  16384 tokens, 256 experts, 8
-// picks, fp32 (35 MB, 5.4 us at the memory's rate): 13 us, bound by the latency of its sums over lanes
+// picks, fp32 (35 MB, 5.4 us at the memory's rate): 15 us, bound by the latency of its sums over lanes
 // (picks added by the lanes that hold them: 23 us).
 template <int LPT, int VPL> __global__ void __launch_bounds__(256) route_backward(const RouteBackward p) {
   extern __shared__ unsigned char smem[];
@@ -764,7 +764,7 @@ template <typename T, int V> __global__ void __launch_bounds__(256, 6) dispatch_
 
 constexpr int combine_blocks(int k) { return k >= 8 ? 3 : k >= 4 ? 4 : 5; }       // of an SM
 // y[t] = sum_j w rows[slot], in the order of j, K loads on their way at a time; the next
-// token's slots are loaded before this one's rows arrive.  32768 x 2048, 6 picks, bf16: 151 us
+// token's slots are loaded before this one's rows arrive.  32768 x 2048, 6 picks, bf16: 154 us
 // (941 MB, 146 at the memory's rate); with loads converted as they came in 284, with registers for
 // 8 loads 176.
 template <typename T, int V, int K> __global__ void __launch_bounds__(256, combine_blocks(K)) combine_kernel(
