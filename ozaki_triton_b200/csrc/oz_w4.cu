@@ -220,6 +220,7 @@ __global__ void __launch_bounds__(kWarps * 32, (W4Shape<RT, NB, PER>::kCtas))
     prefetch_tmap(&tm_x);
   }
   __syncthreads();
+  // what follows reads by plain loads alone: read-only ones may find what stood there before
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
@@ -286,9 +287,9 @@ __global__ void __launch_bounds__(kWarps * 32, (W4Shape<RT, NB, PER>::kCtas))
         const uint32_t group = p.group == kChunk ? k32 / 4 : p.group == 32 ? k32 : __umulhi(k32, p.per_group);
         if (entry_at[i] != kNowhere && (int)group < p.groups) {
           const int64_t at = entry_at[i] + group;
-          scale_bits[i] = scale_bytes == 4 ? __ldg(static_cast<const uint32_t *>(p.scales) + at)
-                                           : __ldg(static_cast<const unsigned short *>(p.scales) + at);
-          if (p.zeros) zero_bits[i] = __ldg(p.zeros + at);
+          scale_bits[i] = scale_bytes == 4 ? *(static_cast<const uint32_t *>(p.scales) + at)
+                                           : *(static_cast<const unsigned short *>(p.scales) + at);
+          if (p.zeros) zero_bits[i] = *(p.zeros + at);
         } else {
           scale_bits[i] = 0;                              // nothing there: adds nothing
         }
