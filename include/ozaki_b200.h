@@ -454,6 +454,7 @@ int oz_combine_backward(const oz_rows_args *args, void *stream);
  * Gradients scaled to a common norm (no counterpart in the reference):
  *   *norm = sqrt(sum of the squares of all tensors),
  *   outs[i] = grads[i] * min(1, max_norm / (*norm + eps))
+ * The norm and the factor are fp32; squares may leave its range as long as the norm does not.
  * Host arrays of `tensors` addresses, sizes (contiguous elements) and types (fp32, fp16 or
  * bf16).  outs[i] may be grads[i] where the types agree; results that share memory otherwise are
  * refused.  norm: fp32 on the device.  workspace: oz_clip_workspace_bytes() bytes, 16-byte

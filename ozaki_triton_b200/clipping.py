@@ -44,9 +44,10 @@ def clip_gradients(grads: Iterable[torch.Tensor], max_norm: float, *, eps: float
     as many tensors of the same shapes and strides, of any of these dtypes (the fp32
     gradients of bf16 weights, say); they must not share memory with each other or
     with gradients other than their own.  Returns the norm as a 0-dimensional fp32
-    tensor; nothing waits for it.  A norm that is not finite scales by 0 (an infinite
-    one) or makes every result NaN.  Forward-mode derivatives are refused, and no
-    gradient is recorded.
+    tensor; nothing waits for it.  Squares may leave fp32's range as long as the norm does
+    not (a factor below 1.2e-38 has fewer bits).  A norm that is not finite in fp32 scales
+    by 0 (an infinite one) or makes every result NaN.  Forward-mode derivatives are refused,
+    and no gradient is recorded.
     """
     grads = list(grads)
     assert grads, "at least one gradient is needed"
