@@ -231,7 +231,8 @@ def _plan_rows(key, call, x, rows, slots, offsets, weights) -> _Plan:
     device = _check_places(given, x, slots, offsets, weights)
     d = given.shape[1]
     shape = (tokens, d) if call == "oz_combine" else (tokens * picks, d)
-    copy = not all(t is None or t.stride(1) == 1 or t.shape[1] == 1 for t in (x, rows)) \
+    # (a tensor without elements has no copy of other strides, and needs none)
+    copy = not all(t is None or t.stride(1) == 1 or t.shape[1] == 1 or t.numel() == 0 for t in (x, rows)) \
         or (weights is not None and not weights.is_contiguous())
     args = _lib.RowsArgs(None, None, None, None, None, None, None, None, tokens, d, 0 if x is None else x.stride(0),
                          0 if rows is None else rows.stride(0), offsets.shape[0] - 1, picks,
