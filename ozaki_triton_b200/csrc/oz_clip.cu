@@ -318,6 +318,7 @@ extern "C" int oz_clip(const oz_clip_args *args, void *stream) {
         if (dt != OZ_F32 && dt != OZ_F16 && dt != OZ_BF16)
           return set_error(OZ_ERR_UNSUPPORTED, "unsupported dtype %d of tensor %d (fp32, fp16 or bf16)", dt, i);
       if (a.sizes[i] < 0) return set_error(OZ_ERR_INVALID, "negative size of tensor %d", i);
+      if (a.sizes[i] > (int64_t)1 << 42) return set_error(OZ_ERR_INVALID, "size out of range");
       if (a.sizes[i] == 0) continue;
       if (!a.grads[i] || !a.outs[i]) return set_error(OZ_ERR_INVALID, "null pointer of tensor %d", i);
       const int es = dtype_size(a.dtypes[i]), os = dtype_size(a.out_dtypes[i]);

@@ -601,7 +601,8 @@ extern "C" int oz_linear(const oz_linear_args *args, void *stream) {
 // Workspace of the backward pass beside the operands' copies: du and partial sums.
 extern "C" int64_t oz_linear_backward_workspace_bytes(int64_t rows, int64_t n, int32_t act, int32_t sums) {
   using namespace oz;
-  if (rows < 0 || n < 0) return OZ_ERR_INVALID;
+  if (rows < 0 || n < 0) return set_error(OZ_ERR_INVALID, "negative size");
+  if (rows > (1 << 30) || n > (1 << 30)) return set_error(OZ_ERR_INVALID, "size out of range");
   if (rows == 0 || n == 0) return 0;
   const int64_t blocks = (rows + slope_rows(rows, (int)n) - 1) / slope_rows(rows, (int)n);
   return (act ? align256(rows * ((n + 7) / 8 * 8) * 2) : 0) + (sums && blocks > 1 ? align256(blocks * n * 4) : 0);

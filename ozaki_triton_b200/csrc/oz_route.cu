@@ -1036,7 +1036,7 @@ int check_rows(const oz_rows_args &a) {
                      (long long)a.d, a.experts, a.picks);
   if (a.dtype != OZ_F32 && a.dtype != OZ_F16 && a.dtype != OZ_BF16)
     return set_error(OZ_ERR_UNSUPPORTED, "unsupported dtype %d (fp32, fp16 or bf16)", a.dtype);
-  if (a.tokens * a.picks > INT32_MAX / 2 || a.d > (1 << 24) || a.picks > kMaxPicks)
+  if (a.tokens > INT32_MAX / 2 / a.picks || a.d > (1 << 24) || a.picks > kMaxPicks)
     return set_error(OZ_ERR_INVALID, "size out of range");
   return OZ_OK;
 }
@@ -1048,7 +1048,9 @@ constexpr int kClearBlocks = 64;     // zero the rows that no pick has
 
 extern "C" int64_t oz_route_workspace_bytes(int64_t rows, int32_t experts) {
   using namespace oz;
-  if (rows < 0 || experts < 1 || experts > kMaxExperts) return OZ_ERR_INVALID;
+  if (rows < 0 || experts < 1 || experts > kMaxExperts)
+    return set_error(OZ_ERR_INVALID, "bad size (rows=%lld experts=%d)", (long long)rows, experts);
+  if (rows > INT32_MAX / 2) return set_error(OZ_ERR_INVALID, "size out of range");
   const RoutePlan r = route_plan(rows, experts);
   // sums of p, then what the blocks counted
   return r.blocks <= 1 ? 0 : (int64_t)experts * 8 + (int64_t)r.blocks * (experts * 8 + 4) + experts * 4;
@@ -1063,7 +1065,7 @@ extern "C" int oz_route(const oz_route_args *args, void *stream) {
     return set_error(OZ_ERR_INVALID, "experts must be in [1, %d], got %d", kMaxExperts, a.experts);
   if (a.picks < 1 || a.picks > kMaxPicks || a.picks > a.experts)
     return set_error(OZ_ERR_INVALID, "picks must be in [1, %d] and at most the experts, got %d", kMaxPicks, a.picks);
-  if (a.rows * a.picks > INT32_MAX / 2) return set_error(OZ_ERR_INVALID, "size out of range");
+  if (a.rows > INT32_MAX / 2 / a.picks) return set_error(OZ_ERR_INVALID, "size out of range");
   if (!a.offsets || !a.counts || !a.tokens || !a.loss || (a.rows > 0 && (!a.logits || !a.weights || !a.chosen || !a.slots)))
     return set_error(OZ_ERR_INVALID, "null pointer");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
@@ -1098,7 +1100,7 @@ extern "C" int oz_route_backward(const oz_route_backward_args *args, void *strea
   if (a.rows < 0) return set_error(OZ_ERR_INVALID, "negative size");
   if (a.experts < 1 || a.experts > kMaxExperts || a.picks < 1 || a.picks > kMaxPicks || a.picks > a.experts)
     return set_error(OZ_ERR_INVALID, "bad size (experts=%d picks=%d)", a.experts, a.picks);
-  if (a.rows * a.picks > INT32_MAX / 2) return set_error(OZ_ERR_INVALID, "size out of range");
+  if (a.rows > INT32_MAX / 2 / a.picks) return set_error(OZ_ERR_INVALID, "size out of range");
   if (a.rows == 0) return OZ_OK;
   if (!a.logits || !a.weights || !a.chosen || !a.counts || !a.tokens || !a.dlogits)
     return set_error(OZ_ERR_INVALID, "null pointer");

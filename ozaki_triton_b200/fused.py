@@ -109,9 +109,11 @@ def _plan_backward(key, dy, x, w, pre, activation, dw_dtype, needs) -> _Plan:
     copy = not (_unit(dy) and _unit(x) and _unit(_along(w)) and (pre is None or _unit(pre)))
     act, workspace = _lib.ACTIVATIONS[activation], 0
     empty = (rows == 0 or n == 0) and k == 0
-    if rows > 0 and n > 0 and not copy:
+    if rows > 0 and n > 0:
         workspace = _lib.load().oz_linear_backward_workspace_bytes(rows, n, act, needs[2])
-        if k > 0:
+        if workspace < 0:
+            _lib.check(workspace)
+        if k > 0 and not copy:
             workspace += (0 if act else _copy_bytes(dy)) + (_copy_bytes(_along(w)) if needs[0] else 0) \
                 + (_copy_bytes(x) if needs[1] else 0)
     args = _lib.LinearBackwardArgs(None, None, None, None, None, None, None, None, rows, k, n, dy.stride(0), x.stride(0),

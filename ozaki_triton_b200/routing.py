@@ -70,6 +70,8 @@ def _plan_route(key, logits, picks, normalize) -> _Plan:
     device = _check_places(logits)
     rows, experts = logits.shape
     size = _lib.load().oz_route_workspace_bytes(rows, experts)
+    if size < 0:
+        _lib.check(size)
     args = _lib.RouteArgs(None, None, None, None, None, None, None, None, None, rows, *logits.stride(), size, experts,
                           picks, bool(normalize), _OZ_DTYPE[logits.dtype])
     return _PLANS.keep(key, _make_plan("oz_route", args, (rows, picks), logits.dtype, device, False, False, size))
