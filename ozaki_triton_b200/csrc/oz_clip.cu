@@ -303,6 +303,7 @@ extern "C" int oz_clip(const oz_clip_args *args, void *stream) {
   if (a.tensors < 0) return set_error(OZ_ERR_INVALID, "negative size");
   if (!a.norm || (a.tensors > 0 && (!a.grads || !a.outs || !a.sizes || !a.dtypes || !a.out_dtypes)))
     return set_error(OZ_ERR_INVALID, "null pointer");
+  if (!aligned(4, {a.norm})) return not_aligned();
   if (!(a.max_norm >= 0) || !(a.eps >= 0)) return set_error(OZ_ERR_INVALID, "max_norm and eps must not be negative");
   const int64_t bytes = oz_clip_workspace_bytes(a.tensors);
   if (!a.workspace || (uintptr_t)a.workspace % 16 != 0 || a.workspace_bytes < bytes)

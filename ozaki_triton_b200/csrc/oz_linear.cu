@@ -569,6 +569,9 @@ extern "C" int oz_linear(const oz_linear_args *args, void *stream) {
   if (!a.y) return set_error(OZ_ERR_INVALID, "null pointer");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int es = dtype_size(a.out_dtype);
+  if (!stream::aligned(es, {a.y, a.residual}) || !stream::aligned(2, {a.pre}) ||
+      !stream::aligned(dtype_size(a.bias_dtype), {a.bias}))
+    return stream::not_aligned();
   Params p{a.y, a.pre, a.bias, a.residual, a.n, a.residual_sr, (int)a.rows, (int)a.k, (int)a.n, 0, 0,
                  0, a.bias_dtype == OZ_F32, a.act, tile::instruction(a.dtype)};
   if ((uintptr_t)a.y % 16 == 0 && a.n * es % 16 == 0 && (!a.pre || ((uintptr_t)a.pre % 16 == 0 && a.n % 8 == 0)))
@@ -615,6 +618,8 @@ extern "C" int oz_linear_backward(const oz_linear_backward_args *args, void *str
   if (int rc = check_linear(a.dtype, a.dw_dtype, a.act, a.rows, a.k, a.n)) return rc;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int dw_size = dtype_size(a.dw_dtype);
+  if (!stream::aligned(2, {a.dy, a.x, a.w, a.pre, a.dx}) || !stream::aligned(dw_size, {a.dw}) || !stream::aligned(4, {a.db}))
+    return stream::not_aligned();
   if (a.rows == 0 || a.n == 0) {
     if (a.dx && a.rows * a.k)
       if (int rc = check_cuda(cudaMemsetAsync(a.dx, 0, (size_t)(a.rows * a.k * 2), st), "cudaMemsetAsync")) return rc;

@@ -1038,6 +1038,9 @@ int check_rows(const oz_rows_args &a) {
     return set_error(OZ_ERR_UNSUPPORTED, "unsupported dtype %d (fp32, fp16 or bf16)", a.dtype);
   if (a.tokens > INT32_MAX / 2 / a.picks || a.d > (1 << 24) || a.picks > kMaxPicks)
     return set_error(OZ_ERR_INVALID, "size out of range");
+  if (!aligned(dtype_size(a.dtype), {a.x, a.rows, a.x_out, a.rows_out}) ||
+      !aligned(4, {a.slots, a.offsets, a.weights, a.dweights}))
+    return not_aligned();
   return OZ_OK;
 }
 
@@ -1076,6 +1079,9 @@ extern "C" int oz_route(const oz_route_args *args, void *stream) {
                      (long long)bytes, (long long)a.workspace_bytes, a.workspace);
   if (a.dtype != OZ_F32 && a.dtype != OZ_F16 && a.dtype != OZ_BF16)
     return set_error(OZ_ERR_UNSUPPORTED, "unsupported dtype %d (fp32, fp16 or bf16)", a.dtype);
+  if (!aligned(dtype_size(a.dtype), {a.logits}) ||
+      !aligned(4, {a.weights, a.loss, a.chosen, a.slots, a.offsets, a.counts, a.tokens}))
+    return not_aligned();
   RouteParams p{logits_of(a.logits, a.rows, a.row, a.col, a.experts, a.dtype), a.weights, a.loss, a.chosen, a.slots,
                 a.offsets, a.counts, a.tokens, nullptr, nullptr, nullptr, nullptr, nullptr, a.rows, a.experts, a.picks,
                 a.normalize, r.chunk, r.per, r.blocks};
@@ -1107,6 +1113,9 @@ extern "C" int oz_route_backward(const oz_route_backward_args *args, void *strea
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (a.dtype != OZ_F32 && a.dtype != OZ_F16 && a.dtype != OZ_BF16)
     return set_error(OZ_ERR_UNSUPPORTED, "unsupported dtype %d (fp32, fp16 or bf16)", a.dtype);
+  if (!aligned(dtype_size(a.dtype), {a.logits}) ||
+      !aligned(4, {a.dweights, a.dloss, a.weights, a.chosen, a.counts, a.tokens}))
+    return not_aligned();
   if ((uintptr_t)a.dlogits % 16 != 0) return set_error(OZ_ERR_INVALID, "dlogits must start on a 16-byte boundary");
   const RouteBackward p{logits_of(a.logits, a.rows, a.row, a.col, a.experts, a.dtype), a.dweights, a.dloss, a.weights,
                         a.chosen, a.counts, a.tokens, a.dlogits, a.rows, a.experts, a.picks, a.normalize};

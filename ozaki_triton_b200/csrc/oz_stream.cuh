@@ -3,6 +3,7 @@
 // with the end of the kernel before.
 #pragma once
 
+#include <initializer_list>
 #include <type_traits>
 
 #include "oz_common.cuh"
@@ -111,6 +112,14 @@ inline int sm_count() {
   }();
   return n;
 }
+
+// Whether all addresses are multiples of an element's size (NULL is).
+inline bool aligned(int size, std::initializer_list<const void *> addresses) {
+  for (const void *p : addresses)
+    if ((uintptr_t)p % size != 0) return false;
+  return true;
+}
+inline int not_aligned() { return set_error(OZ_ERR_INVALID, "a tensor is not aligned to its elements"); }
 
 // Calls f with a value of the element type that `dtype` names.
 template <typename F> int with_type(int dtype, F f) {
