@@ -599,16 +599,15 @@ __device__ __forceinline__ uint4 *staged(unsigned char *mine, int r, int u) {
 
 // Rounds the warp's 32 x COLS accumulators to O and writes the first `rows`
 // rows and `cols` columns of them to out (row pitch ld): every lane rounds
-// its row into the staging, then 4 lanes write 64 consecutive bytes of a row.  A source
-// that computes much for each element takes its columns in a loop (UNROLL = 1).
-template <typename O, int COLS, int UNROLL = COLS, class Source>
+// its row into the staging, then 4 lanes write 64 consecutive bytes of a row.
+template <typename O, int COLS, class Source>
 __device__ __forceinline__ void write_rows(const Source &source, unsigned char *mine, O *out, int64_t ld,
                                            int rows, int64_t cols, bool vectors) {
   constexpr int ES = (int)sizeof(O), CH = 64 / ES;        // columns staged at a time
   const int lane = threadIdx.x % 32;
   O *to = out + (lane / 4) * ld + (lane % 4) * (16 / ES);
   const bool whole = vectors && rows >= 32;
-#pragma unroll(UNROLL)
+#pragma unroll
   for (int c0 = 0; c0 < COLS; c0 += CH) {
     if (c0 >= cols || rows <= 0) continue;
 #pragma unroll
