@@ -202,7 +202,13 @@ __device__ __forceinline__ void finish_elements(const Params &p, const Source &s
 // What follows a product: nothing, or bias, activation and residual by vectors or by elements.
 enum Form { kPlain, kByVectors, kByElements };
 // What follows a product keeps 16 epilogue warps busy (a plain one's 8 wait for its stores;
-// the sums of passes of an fp32 result leave no registers for 16).
+// the sums of passes of an fp32 result leave no registers for 16, and where something follows
+// them they lie in local memory: 4096^3 108 us plain, 175 to 190 with bias, gelu and residual).
+// A 16-bit result's whole contraction is added in one accumulator, whose additions cut off below
+// fp32's last bit: all-positive terms come out 2e-5 too small with 4096 of them, 1e-4 with 16384 and
+// 4e-4 with 65536, as in cuBLAS, beside the half unit of 5e-4 (fp16) or 4e-3 (bf16) of the
+// rounding.  Passes of 8 blocks added in registers, as for fp32 results, keep 2.5e-6 at any
+// length, and cost registers and time that a 16-bit result seldom shows.
 template <typename O, typename B, int PAIR_, int NT_, bool AMN_, bool BMN_, int FORM> struct LinearJob : NoLookAhead {
   static constexpr int EPILOGUE_WARPS = FORM == kPlain || NT_ < 256 || sizeof(O) == 4 ? 8 : 16;
   static constexpr int PAIR = PAIR_, NT = NT_, PLANES = 1, PASS = sizeof(O) == 4 ? 8 : 0;
@@ -286,8 +292,9 @@ int product(bool pair, const Side &a, const Side &b, const Params &p, cudaStream
 //   720 x 7904 x 3616                  76.8        45.2     67.0 (128, 4)
 //   580 x 6504 x 1056, silu, added     36.9        48       24.9 (128, 4)  39.0 (128, 2)
 //   8687 x 160 x 2369, the same        78.5        67.5
-// and by pairs that share a contraction, silu: 299 x 4632 x 3880 28.1 (2 pairs) where the others take
-// 34.0, 580 x 6504 x 1056 18.4 (4 pairs; 24.6), 536 x 7504 x 2688 32.9 (2; 42.3).
+// and by pairs that share a contraction, silu: 299 x 4632 x 3880 27.9 (2 pairs) where the others take
+// 34.0, 536 x 7504 x 2688 31.7 (2; 42.3), 580 x 6504 x 1024 18.3 (4).  4 pairs take 14 tiles at most:
+// 580 x 6504 x 1056 has 15 and takes 24.3 (128 rows, 4 CTAs).
 struct Plan {
   bool pair;                   // the engine's tiles: 256 x 256 by pairs of CTAs, or 128 x 128
   SplitPlan split;             // of 0 rows: the engine

