@@ -351,10 +351,12 @@ int oz_orthogonalize(const void *g, int dtype, int64_t batch, int64_t m, int64_t
  *   residual : (rows, n) of y's type, unit stride along n, row pitch residual_sr, or NULL
  *   y        : contiguous (rows, n) of x's type or fp32 (out_dtype)
  *   pre      : contiguous (rows, n) of x's type for u, or NULL
- * All addresses here and below are multiples of their elements' size (others: OZ_ERR_INVALID).
  *   workspace: oz_linear_workspace_bytes() bytes for these arguments (copies of operands off the
  *              16-byte boundaries that cannot be read as they are), 256-byte aligned; may be 0
  *              bytes and NULL
+ *
+ * Here and in the entries down to oz_clip every address is a multiple of its elements' size
+ * (others: OZ_ERR_INVALID).
  */
 enum oz_activation { OZ_ACT_NONE = 0, OZ_ACT_RELU = 1, OZ_ACT_GELU = 2, OZ_ACT_SILU = 3 };
 typedef struct {
